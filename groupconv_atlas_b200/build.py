@@ -1,8 +1,9 @@
 """Build recipe for the in-tree drop-in library ``libgroupconv.so``.
 
-One nvcc invocation compiles the C ABI (``csrc/common.cpp``) and the sm_100a
-CUDA engine (``csrc/conv_cuda.cu``) into a shared library that sits next to
-this file.  The CUDA runtime is linked as a shared library so that, inside a
+nvcc compiles the C ABI (``csrc/common.cpp``), the shared host helpers and the
+sm_100a CUDA engines (``csrc/conv_cuda.cu``, ``csrc/norm_cuda.cu``), each source
+to an object of its own (only those older than what they include, in parallel),
+and links them into a shared library that sits next to this file.  The CUDA runtime is linked as a shared library so that, inside a
 process that already loaded PyTorch's CUDA runtime, both use one runtime
 instance (one current device per thread, one primary context).
 
@@ -12,7 +13,9 @@ instance (one current device per thread, one primary context).
 from __future__ import annotations
 
 import argparse
+import concurrent.futures
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -23,6 +26,7 @@ ROOT = PACKAGE.parent
 CSRC = PACKAGE / 'csrc'
 INCLUDE = ROOT / 'include'
 LIBRARY = PACKAGE / 'libgroupconv.so'
+OBJECTS = PACKAGE / '_build'
 ARCH = ['-gencode', 'arch=compute_100a,code=sm_100a']
 
 
@@ -48,30 +52,63 @@ def stale(target: Path = LIBRARY) -> bool:
     return any(p.stat().st_mtime > built for p in dependencies())
 
 
-def command(output: Path = LIBRARY, extra: list[str] | None = None) -> list[str]:
+def includes(source: Path) -> list[Path]:
+    """The source and every file of this library that it includes."""
+    found, todo = [], [source]
+    while todo:
+        path = todo.pop()
+        found.append(path)
+        for name in re.findall(r'^#include "([^"]+)"', path.read_text(), flags=re.M):
+            todo += [d / name for d in (CSRC, INCLUDE) if (d / name).exists() and d / name not in found]
+    return found
+
+
+def compile_command(source: Path, output: Path, extra: list[str] | None = None) -> list[str]:
+    return [nvcc(), *ARCH, '-O3', '-lineinfo', '-std=c++17', '-Xcompiler', '-fPIC,-Wall', '-Xptxas', '-warn-spills',
+            f'-I{INCLUDE}', f'-I{CSRC}', *(extra or []), '-c', str(source), '-o', str(output)]
+
+
+def link_command(objects: list[Path], output: Path) -> list[str]:
     cuda_lib = Path(nvcc()).resolve().parent.parent / 'lib64'
-    return [nvcc(), *ARCH, '-O3', '-lineinfo', '-std=c++17', '-shared',
-            '-Xcompiler', '-fPIC,-Wall', '-Xptxas', '-warn-spills',
-            '-cudart', 'shared', f'-I{INCLUDE}', f'-I{CSRC}',
-            f'-Xlinker', f'-rpath,{cuda_lib}',
-            *(extra or []), '-o', str(output), *map(str, sources())]
+    return [nvcc(), *ARCH, '-shared', '-cudart', 'shared', '-Xlinker', f'-rpath,{cuda_lib}', '-o', str(output),
+            *map(str, objects)]
+
+
+def run_tool(cmd: list[str], verbose: bool) -> None:
+    if verbose:
+        print(' '.join(cmd), flush=True)
+    result = subprocess.run(cmd, capture_output=True, text=True)
+    if result.returncode != 0:
+        sys.stderr.write(result.stdout + result.stderr)
+        raise RuntimeError(f'{Path(cmd[0]).name} failed with exit code {result.returncode}')
+    if verbose and (result.stdout or result.stderr):
+        sys.stderr.write(result.stdout + result.stderr)
 
 
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> Path:
     """Compile the library when a source is newer than it (or when forced)."""
     if not force and not stale():
         return LIBRARY
-    tmp = LIBRARY.with_suffix('.so.part')
-    cmd = command(tmp, extra)
-    if verbose:
-        print(' '.join(cmd), flush=True)
-    result = subprocess.run(cmd, capture_output=True, text=True)
-    if result.returncode != 0:
-        sys.stderr.write(result.stdout + result.stderr)
-        raise RuntimeError(f'nvcc failed with exit code {result.returncode}')
-    if verbose and (result.stdout or result.stderr):
-        sys.stderr.write(result.stdout + result.stderr)
-    tmp.replace(LIBRARY)
+    OBJECTS.mkdir(exist_ok=True)
+    todo, objects = [], []
+    for source in sources():
+        target = OBJECTS / (source.name + '.o')
+        objects.append(target)
+        deps = [*includes(source), Path(__file__)]
+        if force or not target.exists() or any(d.stat().st_mtime > target.stat().st_mtime for d in deps):
+            todo.append((source, target))
+
+    def compile_one(item):
+        source, target = item
+        part = target.with_suffix('.part')
+        run_tool(compile_command(source, part, extra), verbose)
+        part.replace(target)
+
+    with concurrent.futures.ThreadPoolExecutor() as pool:
+        list(pool.map(compile_one, todo))
+    part = LIBRARY.with_suffix('.so.part')
+    run_tool(link_command(objects, part), verbose)
+    part.replace(LIBRARY)
     return LIBRARY
 
 
@@ -103,13 +140,8 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
            *[f'-I{d}' for d in cpp_extension.include_paths()], f'-I{sysconfig.get_paths()["include"]}',
            f'-I{cuda_include}', f'-I{INCLUDE}', str(TORCH_EXT_SOURCE),
            f'-L{PACKAGE}', '-lgroupconv', f'-L{torch_lib}', '-lc10', '-lc10_cuda', '-ltorch', '-ltorch_cpu',
-           '-ltorch_python', f'-Wl,-rpath,$ORIGIN', f'-Wl,-rpath,{torch_lib}', '-o', str(target) + '.part']
-    if verbose:
-        print(' '.join(cmd), flush=True)
-    result = subprocess.run(cmd, capture_output=True, text=True)
-    if result.returncode != 0:
-        sys.stderr.write(result.stdout + result.stderr)
-        raise RuntimeError(f'g++ failed with exit code {result.returncode}')
+           '-ltorch_cuda', '-ltorch_python', f'-Wl,-rpath,$ORIGIN', f'-Wl,-rpath,{torch_lib}', '-o', str(target) + '.part']
+    run_tool(cmd, verbose)
     Path(str(target) + '.part').replace(target)
     return target
 

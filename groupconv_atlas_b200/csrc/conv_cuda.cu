@@ -24,6 +24,7 @@
 #include <vector>
 
 #include "device_util.cuh"
+#include "host_util.h"
 #include "kernel_direct.cuh"
 #include "kernel_general.cuh"
 #include "kernel_dw.cuh"
@@ -37,164 +38,18 @@ namespace {
 
 using gcb::DirectParams;
 using gcb::GeneralParams;
+using gcb::PlanRecord;
+using gcb::record_plan;
+using gcb::round_up;
+using gcb::ceil_div;
+using gcb::aligned16;
+using gcb::DeviceFacts;
+using gcb::device_facts;
+using gcb::kernel_occupancy;
+using gcb::launch_pdl;
+using gcb::check_pointer;
 
 constexpr int kStages = 3;
-
-// The last launch's plan on this thread, kept as numbers and formatted only
-// when gc_b200_last_plan asks for it (formatting costs about a third of a
-// microsecond, a tenth of the host time of a call).
-struct PlanRecord {
-    enum Kind { kNone, kDirect, kWide, kTf32, kSmall, kGeneral, kDw, kDwS2, kNhwc } kind = kNone;
-    const char *name = "";  // variant name, static storage
-    bool tma = false;
-    long long v[14] = {};
-};
-thread_local PlanRecord g_last;
-thread_local std::string g_plan;
-
-std::string format_plan(const PlanRecord &r) {
-    char buf[400];
-    const long long *v = r.v;
-    switch (r.kind) {
-    case PlanRecord::kDirect:
-        std::snprintf(buf, sizeof(buf),
-                      "kernel=direct_%s engine=group variant=%s grid=%lld block=%lld smem=%lld ctas_per_sm=%lld "
-                      "cb=%lld bh=%lld items=%lld cells=%lld stages=%lld pitch=%lld rows=%lld bulk_w=%lld "
-                      "vec_store=%lld",
-                      r.tma ? "tma" : "ldg", r.name, v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9],
-                      v[10], v[11], v[12]);
-        break;
-    case PlanRecord::kWide:
-        std::snprintf(buf, sizeof(buf),
-                      "kernel=direct_%s engine=wide variant=%s grid=%lld block=%lld smem=%lld ctas_per_sm=%lld "
-                      "kc=%lld chunks=%lld co_item=%lld bh=%lld items=%lld cells=%lld pitch=%lld rows=%lld "
-                      "vec_store=%lld",
-                      r.tma ? "tma" : "ldg", r.name, v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9],
-                      v[10], v[11], v[12]);
-        break;
-    case PlanRecord::kTf32:
-        std::snprintf(buf, sizeof(buf),
-                      "kernel=tf32x3 engine=tcgen05 n_cta=%lld block=320 smem=%lld M=%lld N=%lld nb=%lld sp=%lld "
-                      "strips=%lld items=%lld chunks=%lld rows_b=%lld ks=%lld layout=%s",
-                      v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9], v[10], r.name);
-        break;
-    case PlanRecord::kSmall:
-        std::snprintf(buf, sizeof(buf),
-                      "kernel=small grid=%lld block=%lld smem=%lld ctas_per_sm=%lld cob=%lld cb=%lld items=%lld "
-                      "vec=%lld stages=%lld",
-                      v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8]);
-        break;
-    case PlanRecord::kDw:
-        std::snprintf(buf, sizeof(buf),
-                      "kernel=general engine=depthwise k=%lld grid=%lld block=%lld smem=%lld bh=%lld bands=%lld "
-                      "pitch=%lld items=%lld",
-                      v[0], v[1], v[7], v[2], v[3], v[4], v[5], v[6]);
-        break;
-    case PlanRecord::kDwS2:
-        std::snprintf(buf, sizeof(buf),
-                      "kernel=general engine=depthwise_cells k=%lld stride=%lld grid=%lld block=256 cells=%lld "
-                      "vec_in=%lld vec_out=%lld",
-                      v[0], v[5], v[1], v[2], v[3], v[4]);
-        break;
-    case PlanRecord::kNhwc:
-        std::snprintf(buf, sizeof(buf), "kernel=nhwc engine=%s grid=%lld block=%lld cpg=%lld bias=%lld rows=%lld",
-                      r.name, v[0], v[1], v[2], v[3], v[4]);
-        break;
-    case PlanRecord::kGeneral:
-        std::snprintf(buf, sizeof(buf), "kernel=general grid=%lld block=%lld run=%lld cob=%lld index=%s runs=%lld",
-                      v[0], v[1], v[2], v[3], v[4] ? "32" : "64", v[5]);
-        break;
-    default:
-        buf[0] = '\0';
-    }
-    return buf;
-}
-
-template <class... T>
-void record_plan(PlanRecord::Kind kind, const char *name, bool tma, T... values) {
-    g_last.kind = kind;
-    g_last.name = name;
-    g_last.tma = tma;
-    const long long vals[] = {static_cast<long long>(values)...};
-    for (size_t i = 0; i < sizeof...(T); ++i) g_last.v[i] = vals[i];
-}
-
-long long round_up(long long v, long long m) { return (v + m - 1) / m * m; }
-long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
-
-// ---- device facts, cached per device -----------------------------------------
-struct DeviceFacts {
-    int sms = 0;
-    int smem_optin = 0;   // max dynamic shared memory per block (opt-in)
-    int smem_per_sm = 0;  // shared memory per multiprocessor
-};
-
-std::mutex g_mutex;
-std::map<int, DeviceFacts> g_facts;
-std::map<std::pair<int, const void *>, bool> g_attr_done;
-std::map<std::tuple<int, const void *, int, size_t>, int> g_occupancy;
-
-int device_facts(int dev, DeviceFacts &out) {
-    std::lock_guard<std::mutex> lock(g_mutex);
-    auto it = g_facts.find(dev);
-    if (it != g_facts.end()) {
-        out = it->second;
-        return GC_OK;
-    }
-    DeviceFacts f;
-    cudaError_t e = cudaDeviceGetAttribute(&f.sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e == cudaSuccess)
-        e = cudaDeviceGetAttribute(&f.smem_optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
-    if (e == cudaSuccess)
-        e = cudaDeviceGetAttribute(&f.smem_per_sm, cudaDevAttrMaxSharedMemoryPerMultiprocessor, dev);
-    if (e != cudaSuccess) return gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
-    g_facts[dev] = f;
-    out = f;
-    return GC_OK;
-}
-
-// Opt a kernel into the device's full dynamic shared memory once, then ask
-// the occupancy calculator (cached) how many CTAs fit per SM.
-int kernel_occupancy(int dev, const void *fn, int threads, size_t smem, int smem_optin,
-                     int &ctas) {
-    std::lock_guard<std::mutex> lock(g_mutex);
-    auto key = std::make_tuple(dev, fn, threads, smem);
-    auto it = g_occupancy.find(key);
-    if (it != g_occupancy.end()) {
-        ctas = it->second;
-        return GC_OK;
-    }
-    auto akey = std::make_pair(dev, fn);
-    if (!g_attr_done[akey]) {
-        cudaError_t e =
-            cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_optin);
-        if (e != cudaSuccess) return gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
-        g_attr_done[akey] = true;
-    }
-    int n = 0;
-    cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, threads, smem);
-    if (e != cudaSuccess) return gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
-    g_occupancy[key] = n;
-    ctas = n;
-    return GC_OK;
-}
-
-// Launch on the caller's stream with programmatic stream serialization: the
-// kernel may start its prologue while the previous kernel in the stream
-// drains, and waits (griddepcontrol.wait) before touching global memory.
-cudaError_t launch_pdl(const void *fn, dim3 grid, dim3 block, void **args, size_t smem, cudaStream_t stream) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelExC(&cfg, fn, args);
-}
 
 // ---- TMA descriptor encoding ---------------------------------------------------
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
@@ -347,7 +202,6 @@ const Variant &wide_variant(long long cpg) {
     return w1;
 }
 
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Whether the TMA staging can serve this shape and this input pointer.
 bool tma_eligible(const gc_shape *p, const void *x) {
@@ -690,6 +544,7 @@ int plan_wide(const gc_shape *p, bool tma, bool y_aligned, int dev, const Device
 }
 
 using PlanKey = std::tuple<int, long long, long long, long long, long long, long long, int>;
+std::mutex g_mutex;
 std::map<PlanKey, EnginePlan> g_plans;
 
 // Plan for the direct engines, cached per (device, shape, staging, alignment).
@@ -1529,22 +1384,6 @@ bool b_geometry(const gc_shape *p) {
            p->pw == 1 && p->dh == 1 && p->dw == 1;
 }
 
-// Device memory on the descriptor's device, which must be the current device
-// (reference groupconv.cu:130-139).  Managed and mapped host memory are
-// outside the contract.
-int check_pointer(const gc_tensor *t, int current) {
-    cudaPointerAttributes attr;
-    std::memset(&attr, 0, sizeof(attr));
-    cudaError_t e = cudaPointerGetAttributes(&attr, t->data);
-    if (e != cudaSuccess) {
-        cudaGetLastError();  // the failed query must not poison the next launch check
-        return gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
-    }
-    if (attr.type != cudaMemoryTypeDevice || attr.device != t->device_index || attr.device != current)
-        return gc_error(GC_INVALID, "CUDA pointer must be device memory on descriptor/current device");
-    return GC_OK;
-}
-
 int device_and_stream_checks(const gc_tensor *x, const gc_tensor *w, const gc_tensor *y,
                              void *stream, int &current) {
     cudaError_t e = cudaGetDevice(&current);
@@ -1775,8 +1614,9 @@ int gc_b200_autotune(const gc_shape *p, const gc_tensor *x, const gc_tensor *w, 
 }
 
 const char *gc_b200_last_plan(void) {
-    g_plan = format_plan(g_last);
-    return g_plan.c_str();
+    thread_local std::string text;
+    text = gcb::format_plan(gcb::last_plan());
+    return text.c_str();
 }
 
 int gc_b200_device_status(uint32_t *status, int clear) {
