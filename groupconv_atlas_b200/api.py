@@ -40,6 +40,14 @@ LAYOUTS = {'nchw': NCHW, 'nhwc': NHWC}
 # Activations of gc_b200_conv_ex.
 ACT_NONE, ACT_RELU, ACT_RELU6 = 0, 1, 2
 ACTIVATIONS = {'none': ACT_NONE, 'relu': ACT_RELU, 'relu6': ACT_RELU6}
+# Activations of gc_b200_group_norm.
+ACT_SILU = 3
+NORM_ACTIVATIONS = {**ACTIVATIONS, 'silu': ACT_SILU}
+# 16-bit element types of gc_b200_group_norm and gc_b200_dropout.
+B200_F16, B200_BF16 = 16, 17
+# What one decision of gc_b200_dropout covers.
+DROP_ELEMENT, DROP_CHANNEL = 0, 1
+DROP_SCOPES = {'element': DROP_ELEMENT, 'channel': DROP_CHANNEL}
 STATUS_TMA_TIMEOUT = 0x1
 STATUS_MMA_TIMEOUT = 0x2
 
@@ -146,6 +154,32 @@ def tensor(array):
     return Tensor(ptr, size, dtype, device, index, len(shape), dims, strd)
 
 
+def view(array):
+    """Descriptor for the entry points that also take float16 and bfloat16
+    torch tensors and strided views: ``bytes`` covers the view from its first
+    to its last element (rank at most 4)."""
+    desc = tensor(array)
+    desc.dtype = {'torch.float16': B200_F16, 'torch.bfloat16': B200_BF16}.get(str(array.dtype), desc.dtype)
+    if 0 not in tuple(array.shape):
+        span = 1 + sum((n - 1) * desc.strides[i] for i, n in enumerate(array.shape))
+        desc.bytes = span * array.element_size() if hasattr(array, 'element_size') else span * array.itemsize
+    return desc
+
+
+class DropoutArgs(ct.Structure):
+    """gc_b200_dropout_args; the three addresses are device words or None."""
+    _fields_ = [('p', ct.c_double), ('seed', ct.c_uint64), ('offset', ct.c_uint64), ('seed_ptr', ct.c_void_p),
+                ('offset_ptr', ct.c_void_p), ('used', ct.c_void_p), ('scope', ct.c_int32)]
+
+
+def dropout_args(p, seed=0, offset=0, scope='element', seed_ptr=None, offset_ptr=None, used=None):
+    scope = DROP_SCOPES.get(scope, scope) if isinstance(scope, str) else scope
+    for value in (seed, offset):
+        if not 0 <= operator.index(value) < 1 << 64:
+            raise ValueError('seed and offset are unsigned 64-bit integers')
+    return DropoutArgs(p, seed, offset, seed_ptr, offset_ptr, used, native_int(scope))
+
+
 class NativeError(RuntimeError):
     def __init__(self, status, message):
         self.status = status
@@ -192,6 +226,14 @@ class Native:
         lib.gc_b200_selftest_wait_timeout.argtypes = [ct.c_uint32, ct.c_void_p]
         lib.gc_b200_conv_ex.argtypes = [ct.POINTER(CShape)] + [ct.POINTER(Tensor)] * 4 + [ct.c_int, ct.c_int,
                                                                                               ct.c_void_p]
+        ptr = ct.POINTER(Tensor)
+        lib.gc_b200_group_norm_workspace.argtypes = [ptr] * 2 + [ct.c_int64, ct.POINTER(ct.c_uint64)]
+        lib.gc_b200_group_norm.argtypes = ([ptr] * 5 + [ct.c_int64, ct.c_double, ct.c_int, ct.POINTER(DropoutArgs),
+                                                        ct.c_void_p, ct.c_uint64, ct.c_void_p])
+        lib.gc_b200_group_norm_backward_workspace.argtypes = [ptr] * 3 + [ct.c_int64, ct.POINTER(ct.c_uint64)]
+        lib.gc_b200_group_norm_backward.argtypes = ([ptr] * 8 + [ct.c_int64, ct.c_int, ct.POINTER(DropoutArgs),
+                                                                 ct.c_void_p, ct.c_uint64, ct.c_void_p])
+        lib.gc_b200_dropout.argtypes = [ptr] * 3 + [ct.POINTER(DropoutArgs), ct.c_void_p]
         lib.gc_b200_autotune.argtypes = [ct.POINTER(CShape)] + [ct.POINTER(Tensor)] * 3 + [ct.c_int, ct.c_void_p]
         lib.gc_b200_probe_ffma.argtypes = [ct.c_void_p, ct.c_int, ct.c_int, ct.c_void_p]
         lib.gc_b200_probe_ffma_flops.argtypes = [ct.c_int, ct.c_int]
@@ -254,6 +296,61 @@ class Native:
         p, xd, wd, yd = cshape(shape), tensor(x), tensor(w), tensor(y)
         self.check(self.lib.gc_b200_autotune(ct.byref(p), ct.byref(xd), ct.byref(wd), ct.byref(yd),
                                              native_int(candidates), self._stream(stream)))
+        return y
+
+    @staticmethod
+    def _views(*arrays):
+        """Descriptors of the arrays that are given, and pointers (or None) to pass."""
+        descs = [view(a) if a is not None else None for a in arrays]
+        return descs, [ct.byref(d) if d is not None else None for d in descs]
+
+    @staticmethod
+    def _space(workspace):
+        return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+
+    def group_norm_workspace(self, x, y, groups):
+        """Bytes of device memory that group_norm needs for these tensors."""
+        size = ct.c_uint64(0)
+        _, ptrs = self._views(x, y)
+        self.check(self.lib.gc_b200_group_norm_workspace(*ptrs, native_int(groups, 64), ct.byref(size)))
+        return size.value
+
+    def group_norm(self, x, y, groups, gamma=None, beta=None, eps=1e-5, activation='none', dropout=None, stats=None,
+                   workspace=None, stream=0):
+        """gc_b200_group_norm on borrowed channels-last device tensors:
+        activation 'none', 'relu', 'relu6' or 'silu'; dropout from
+        dropout_args(); stats an FP32 (N, groups, 2) tensor for the gradient;
+        workspace a device tensor of group_norm_workspace() bytes."""
+        act = NORM_ACTIVATIONS.get(activation, activation) if isinstance(activation, str) else activation
+        _, (xp, gp, bp, yp, sp) = self._views(x, gamma, beta, y, stats)
+        self.check(self.lib.gc_b200_group_norm(xp, gp, bp, yp, sp, native_int(groups, 64), eps, native_int(act),
+                                               ct.byref(dropout) if dropout is not None else None,
+                                               *self._space(workspace), self._stream(stream)))
+        return y
+
+    def group_norm_backward_workspace(self, dy, x, dx, groups):
+        """Bytes of device memory that group_norm_backward needs for these tensors."""
+        size = ct.c_uint64(0)
+        _, ptrs = self._views(dy, x, dx)
+        self.check(self.lib.gc_b200_group_norm_backward_workspace(*ptrs, native_int(groups, 64), ct.byref(size)))
+        return size.value
+
+    def group_norm_backward(self, dy, x, stats, dx, groups, gamma=None, beta=None, dgamma=None, dbeta=None,
+                            activation='none', dropout=None, workspace=None, stream=0):
+        """gc_b200_group_norm_backward: gradients of group_norm from its x,
+        gamma, beta, activation, dropout and stored stats."""
+        act = NORM_ACTIVATIONS.get(activation, activation) if isinstance(activation, str) else activation
+        _, ptrs = self._views(dy, x, gamma, beta, stats, dx, dgamma, dbeta)
+        self.check(self.lib.gc_b200_group_norm_backward(*ptrs, native_int(groups, 64), native_int(act),
+                                                        ct.byref(dropout) if dropout is not None else None,
+                                                        *self._space(workspace), self._stream(stream)))
+        return dx
+
+    def dropout(self, x, y, dropout, residual=None, stream=0):
+        """gc_b200_dropout: y = [residual +] dropout(x) with dropout_args()."""
+        _, (xp, rp, yp) = self._views(x, residual, y)
+        self.check(self.lib.gc_b200_dropout(xp, rp, yp, ct.byref(dropout) if dropout is not None else None,
+                                            self._stream(stream)))
         return y
 
     def last_plan(self):

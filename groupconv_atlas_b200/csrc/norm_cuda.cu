@@ -1,0 +1,629 @@
+// gc_b200_group_norm, its gradient, and gc_b200_dropout: descriptor checks,
+// plans and launches.  As in the convolution backend nothing here allocates,
+// synchronizes or keeps state between calls; a call can be captured into a
+// CUDA graph.
+#include "groupconv.h"
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <initializer_list>
+
+#include "host_util.h"
+#include "kernel_dropout.cuh"
+#include "kernel_norm.cuh"
+
+namespace {
+
+using gcb::ceil_div;
+using gcb::DropParams;
+using gcb::DropoutParams;
+using gcb::NormParams;
+using gcb::PlanRecord;
+
+typedef __int128 wide;  // products of descriptor fields, before they are known to fit
+
+// ---- descriptors ------------------------------------------------------------------------
+int elem_type(int dtype) {
+    return dtype == GC_F32 ? gcb::kElemF32 : dtype == GC_B200_F16 ? gcb::kElemF16
+         : dtype == GC_B200_BF16 ? gcb::kElemBF16 : -1;
+}
+int elem_size(int type) { return type == gcb::kElemF32 ? 4 : 2; }
+
+// What every descriptor of these entry points has to satisfy (GC_INVALID
+// conditions, then FP64 as a valid type outside this set).
+int check_fields(const gc_tensor *t, int rank_low, int rank_high, int64_t &count) {
+    if (t == nullptr) return gc_error(GC_INVALID, "null tensor descriptor");
+    if (t->rank < rank_low || t->rank > rank_high) return gc_error(GC_INVALID, "tensor rank out of range");
+    if (t->device != GC_CUDA || t->device_index < 0) return gc_error(GC_INVALID, "tensor must be CUDA memory");
+    if (t->dtype != GC_F64 && elem_type(t->dtype) < 0) return gc_error(GC_INVALID, "unknown tensor dtype");
+    wide n = 1;
+    for (int i = 0; i < t->rank; ++i) {
+        if (t->dims[i] < 0) return gc_error(GC_INVALID, "tensor dimensions must not be negative");
+        n *= t->dims[i];
+        if (n > PTRDIFF_MAX / 8) return gc_error(GC_INVALID, "tensor element count overflow");
+    }
+    count = static_cast<int64_t>(n);
+    if (count == 0) return GC_OK;
+    if (t->data == nullptr) return gc_error(GC_INVALID, "null tensor buffer");
+    const uintptr_t base = reinterpret_cast<uintptr_t>(t->data);
+    const unsigned item = t->dtype == GC_F64 ? 8 : elem_size(elem_type(t->dtype));
+    if (base % item != 0) return gc_error(GC_INVALID, "tensor data is not element aligned");
+    if (t->bytes > UINTPTR_MAX - base) return gc_error(GC_INVALID, "tensor pointer range overflow");
+    if (t->bytes / item < static_cast<uint64_t>(count)) return gc_error(GC_INVALID, "tensor buffer is too small");
+    return GC_OK;
+}
+
+bool same_dims(const gc_tensor *a, const gc_tensor *b) {
+    if (a->rank != b->rank) return false;
+    for (int i = 0; i < a->rank; ++i)
+        if (a->dims[i] != b->dims[i]) return false;
+    return true;
+}
+
+// A channels-last tensor as images of evenly spaced pixels.
+struct View {
+    char *data = nullptr;
+    long long n = 0, c = 0, px = 0;
+    long long ldn = 0, ldp = 0;  // element strides of an image and of a pixel
+    int type = 0;
+    uint64_t span = 0;  // bytes from the first to the end of the last element
+};
+
+int view_of(const gc_tensor *t, View &v) {
+    const int64_t *d = t->dims, *s = t->strides;
+    if (t->dtype == GC_F64) return gc_error(GC_UNSUPPORTED, "FP64 tensors are not supported here");
+    v.data = static_cast<char *>(t->data);
+    v.type = elem_type(t->dtype);
+    v.n = d[0];
+    v.c = d[1];
+    v.px = 1;
+    v.ldp = v.c;
+    bool even = true;
+    for (int i = t->rank - 1; i >= 2; --i) {  // axes of one image, innermost first
+        if (d[i] > 1) {
+            if (v.px == 1) v.ldp = s[i];
+            else even = even && s[i] >= 0 && static_cast<wide>(v.ldp) * v.px == s[i];
+        }
+        v.px *= d[i];
+    }
+    if (v.n == 0 || v.px == 0) return GC_OK;
+    if (v.ldp < v.c || (v.c > 1 && s[1] != 1) || !even)
+        return gc_error(GC_UNSUPPORTED, "tensor is not channels last with evenly spaced pixels");
+    const wide image = static_cast<wide>(v.px - 1) * v.ldp + v.c;
+    wide total = image;
+    v.ldn = 0;
+    if (v.n > 1) {
+        if (s[0] < image) return gc_error(GC_UNSUPPORTED, "tensor's images overlap or interleave");
+        v.ldn = s[0];
+        total += static_cast<wide>(v.n - 1) * v.ldn;
+    }
+    total *= elem_size(v.type);
+    if (total > static_cast<wide>(t->bytes)) return gc_error(GC_INVALID, "tensor buffer is too small");
+    v.span = static_cast<uint64_t>(total);
+    return GC_OK;
+}
+
+bool ranges_meet(const void *a, uint64_t an, const void *b, uint64_t bn) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return an != 0 && bn != 0 && x < y + bn && y < x + an;
+}
+struct Range {
+    const void *p;
+    uint64_t bytes;
+};
+// Outputs against inputs and against one another.
+bool outputs_meet(std::initializer_list<Range> outs, std::initializer_list<Range> ins) {
+    for (const Range *o = outs.begin(); o != outs.end(); ++o) {
+        for (const Range &i : ins)
+            if (ranges_meet(o->p, o->bytes, i.p, i.bytes)) return true;
+        for (const Range *q = outs.begin(); q != o; ++q)
+            if (ranges_meet(o->p, o->bytes, q->p, q->bytes)) return true;
+    }
+    return false;
+}
+
+// A nullable vector of one parameter per channel.
+int check_channel_vector(const gc_tensor *t, const gc_tensor *x) {
+    if (t == nullptr) return GC_OK;
+    int64_t count = 0;
+    int st = check_fields(t, 1, 1, count);
+    if (st != GC_OK) return st;
+    if (count != x->dims[1]) return gc_error(GC_INVALID, "channel parameters must have C elements");
+    if (t->dtype != GC_F32 && t->dtype != x->dtype)
+        return gc_error(GC_INVALID, "channel parameters must be F32 or of the data's type");
+    if (t->device_index != x->device_index) return gc_error(GC_INVALID, "tensor device indices differ");
+    return GC_OK;
+}
+int check_channel_layout(const gc_tensor *t) {
+    if (t != nullptr && t->dims[0] > 1 && t->strides[0] != 1)
+        return gc_error(GC_UNSUPPORTED, "channel parameters must be dense");
+    return GC_OK;
+}
+Range range_of(const gc_tensor *t) {
+    if (t == nullptr) return {nullptr, 0};
+    uint64_t n = t->dtype == GC_F64 ? 8 : elem_size(elem_type(t->dtype));
+    for (int i = 0; i < t->rank; ++i) n *= static_cast<uint64_t>(t->dims[i]);
+    return {t->data, n};
+}
+
+int check_stats(const gc_tensor *t, const gc_tensor *x, int64_t groups) {
+    int64_t count = 0;
+    int st = check_fields(t, 3, 3, count);
+    if (st != GC_OK) return st;
+    if (t->dtype != GC_F32 || t->dims[0] != x->dims[0] || t->dims[1] != groups || t->dims[2] != 2)
+        return gc_error(GC_INVALID, "stats must be an F32 tensor of dims (N, groups, 2)");
+    if (t->device_index != x->device_index) return gc_error(GC_INVALID, "tensor device indices differ");
+    if (reinterpret_cast<uintptr_t>(t->data) % 8 != 0) return gc_error(GC_INVALID, "stats must be 8-byte aligned");
+    return GC_OK;
+}
+bool dense_stats(const gc_tensor *t) {
+    return t->strides[2] == 1 && (t->dims[1] == 1 || t->strides[1] == 2) &&
+           (t->dims[0] <= 1 || t->strides[0] == 2 * t->dims[1]);
+}
+
+int check_dropout(const gc_b200_dropout_args *d, DropParams &out) {
+    out = DropParams{};
+    if (d == nullptr) return GC_OK;
+    if (!(d->p >= 0.0 && d->p <= 1.0)) return gc_error(GC_INVALID, "dropout probability must be in 0..1");
+    if (d->scope != GC_B200_DROP_ELEMENT && d->scope != GC_B200_DROP_CHANNEL)
+        return gc_error(GC_INVALID, "unknown dropout scope");
+    for (const void *p : {static_cast<const void *>(d->seed_ptr), static_cast<const void *>(d->offset_ptr),
+                          static_cast<const void *>(d->used)})
+        if (reinterpret_cast<uintptr_t>(p) % 8 != 0) return gc_error(GC_INVALID, "dropout words are not 8-byte aligned");
+    if (d->used != nullptr)
+        for (const uint64_t *p : {d->seed_ptr, d->offset_ptr})
+            if (p != nullptr && ranges_meet(d->used, 16, p, 8))
+                return gc_error(GC_INVALID, "the words in use must not overwrite the given ones");
+    out.threshold = static_cast<uint32_t>(std::nearbyint(65536.0 * d->p));
+    out.scale = out.threshold < 65536 ? static_cast<float>(65536.0 / (65536.0 - out.threshold)) : 0.0f;
+    out.channel = d->scope == GC_B200_DROP_CHANNEL;
+    out.seed = d->seed;
+    out.offset = d->offset;
+    out.seed_ptr = d->seed_ptr;
+    out.offset_ptr = d->offset_ptr;
+    out.used = d->used;
+    return GC_OK;
+}
+
+// The current device, the pointers' device and the stream (reference
+// groupconv.cu:130-139, :185-191).
+int check_call(std::initializer_list<const gc_tensor *> tensors, std::initializer_list<const void *> words,
+               int device_index, void *stream, int &dev) {
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
+    for (const gc_tensor *t : tensors)
+        if (t != nullptr && range_of(t).bytes != 0) {
+            const int st = gcb::check_pointer(t, dev);
+            if (st != GC_OK) return st;
+        }
+    for (const void *p : words)
+        if (p != nullptr) {
+            const int st = gcb::check_device_memory(p, device_index, dev);
+            if (st != GC_OK) return st;
+        }
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    e = cudaStreamIsCapturing(reinterpret_cast<cudaStream_t>(stream), &cs);
+    return e == cudaSuccess ? GC_OK : gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
+}
+
+int launched(cudaError_t e) {
+    if (e == cudaSuccess) e = cudaGetLastError();
+    else cudaGetLastError();
+    return e == cudaSuccess ? gc_error(GC_OK, "") : gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
+}
+
+// ---- group norm: plan ---------------------------------------------------------------------
+int vector_of(const View &v) { return v.type == gcb::kElemF32 ? 4 : 8; }
+
+// Every pixel of every given view starts on a 16-byte boundary.
+bool vector_access(std::initializer_list<const View *> views) {
+    for (const View *v : views) {
+        const int e = vector_of(*v);
+        if (v->c % e || v->ldp % e || v->ldn % e || !gcb::aligned16(v->data)) return false;
+    }
+    return true;
+}
+
+// The split path's work split: blocks of up to 256 vector columns, chunks of
+// pixels such that there are about 16 blocks for each SM, but at least eight
+// pixels for each thread.
+void plan_split(NormParams &P, int v, int sms) {
+    P.vcols = P.c / v;
+    P.cblocks = static_cast<int>(ceil_div(P.vcols, gcb::kNormThreads));
+    P.vb = static_cast<int>(ceil_div(P.vcols, P.cblocks));
+    P.lanes = gcb::kNormThreads / P.vb;
+    const long long wanted = std::max<long long>(1, ceil_div(16LL * sms, P.n * P.cblocks));
+    P.chunk_rows = std::min(P.px, std::max<long long>(ceil_div(P.px, wanted), 8LL * P.lanes));
+    P.chunks = static_cast<int>(ceil_div(P.px, P.chunk_rows));
+    P.items = P.n * P.chunks * P.cblocks;
+}
+
+uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
+
+struct NormSpace {  // the workspace's parts, in this order
+    uint64_t stats = 0, part = 0, chan = 0, gsum = 0;
+    uint64_t total() const { return stats + part + chan + gsum; }
+};
+
+// Bytes of the workspace for a plan that is already in P.
+NormSpace space_of(const NormParams &P, bool backward) {
+    NormSpace s;
+    const uint64_t n = P.n;
+    s.part = up16(n * P.chunks * P.c * sizeof(float2));
+    if (backward) {
+        s.chan = up16(n * P.c * sizeof(float2));
+        s.gsum = up16(n * P.groups * sizeof(float2));
+    } else {
+        s.stats = up16(n * P.groups * sizeof(float2));
+    }
+    return s;
+}
+
+struct NormPlan {
+    bool vec = false;
+    int type = 0;
+};
+
+// Checks shared by the workspace queries and the calls: data tensors that
+// have the same dims and type, then their layout.  views[0] is x's.
+int check_data(std::initializer_list<const gc_tensor *> tensors, int64_t groups, View *views, NormParams &P,
+               NormPlan &plan) {
+    const gc_tensor *first = *tensors.begin();
+    int64_t count = 0;
+    for (const gc_tensor *t : tensors) {
+        const int st = check_fields(t, 2, 4, count);
+        if (st != GC_OK) return st;
+        if (!same_dims(t, first)) return gc_error(GC_INVALID, "tensor dimensions differ");
+        if (t->dtype != first->dtype) return gc_error(GC_INVALID, "tensor dtypes differ");
+        if (t->device_index != first->device_index) return gc_error(GC_INVALID, "tensor device indices differ");
+    }
+    if (first->dims[1] < 1 || first->dims[1] > INT32_MAX) return gc_error(GC_INVALID, "channel count out of range");
+    if (groups < 1 || first->dims[1] % groups != 0) return gc_error(GC_INVALID, "channels must be divisible by groups");
+    P = NormParams{};
+    int i = 0;
+    plan.vec = true;
+    for (const gc_tensor *t : tensors) {
+        const int st = view_of(t, views[i]);
+        if (st != GC_OK) return st;
+        plan.vec = plan.vec && vector_access({&views[i]});
+        ++i;
+    }
+    P.n = views[0].n;
+    P.px = views[0].px;
+    P.c = static_cast<int>(views[0].c);
+    P.groups = static_cast<int>(groups);
+    P.cpg = P.c / P.groups;
+    plan.type = views[0].type;
+    return GC_OK;
+}
+
+bool empty(const NormParams &P) { return P.n == 0 || P.px == 0; }
+
+int plan_norm(NormParams &P, NormPlan &plan) {
+    int dev = -1;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
+    gcb::DeviceFacts facts;
+    const int st = gcb::device_facts(dev, facts);
+    if (st != GC_OK) return st;
+    plan_split(P, plan.vec ? (plan.type == gcb::kElemF32 ? 4 : 8) : 1, facts.sms);
+    return GC_OK;
+}
+
+void set_param(const gc_tensor *t, const void *&p, int &type) {
+    p = t != nullptr ? t->data : nullptr;
+    type = t != nullptr ? elem_type(t->dtype) : 0;
+}
+
+// ---- kernel tables --------------------------------------------------------------------------
+// The vector kernels are compiled for each activation; the scalar ones, for
+// tensors whose pixels are not 16-byte aligned, choose it at run time.
+enum NormKernel { kMoments, kApply, kGradSums, kGradApply };
+
+template <class T, int V, int ACT>
+const void *norm_instance(NormKernel k) {
+    switch (k) {
+    case kApply: return reinterpret_cast<const void *>(&gcb::norm_apply_kernel<T, V, ACT>);
+    case kGradSums: return reinterpret_cast<const void *>(&gcb::norm_grad_sums_kernel<T, V, ACT>);
+    case kGradApply: return reinterpret_cast<const void *>(&gcb::norm_grad_apply_kernel<T, V, ACT>);
+    default: return reinterpret_cast<const void *>(&gcb::norm_moments_kernel<T, V>);
+    }
+}
+template <class T>
+const void *norm_typed(NormKernel k, bool vec, int act) {
+    constexpr int V = gcb::kVec<T>;
+    if (!vec) return norm_instance<T, 1, -1>(k);
+    if (act == gcb::kActRelu) return norm_instance<T, V, gcb::kActRelu>(k);
+    if (act == gcb::kActRelu6) return norm_instance<T, V, gcb::kActRelu6>(k);
+    if (act == gcb::kActSilu) return norm_instance<T, V, gcb::kActSilu>(k);
+    return norm_instance<T, V, gcb::kActNone>(k);
+}
+const void *norm_kernel(NormKernel k, const NormPlan &plan, int act) {
+    if (plan.type == gcb::kElemF16) return norm_typed<__half>(k, plan.vec, act);
+    if (plan.type == gcb::kElemBF16) return norm_typed<__nv_bfloat16>(k, plan.vec, act);
+    return norm_typed<float>(k, plan.vec, act);
+}
+
+unsigned grid_of(long long items) { return static_cast<unsigned>(std::min<long long>(items, INT32_MAX)); }
+
+cudaError_t launch(const void *fn, long long blocks, NormParams &P, cudaStream_t s) {
+    void *args[] = {&P};
+    return gcb::launch_pdl(fn, dim3(grid_of(blocks)), dim3(gcb::kNormThreads), args, 0, s);
+}
+
+int check_workspace(const void *p, uint64_t bytes, uint64_t need) {
+    if (need == 0) return GC_OK;
+    if (p == nullptr || bytes < need) return gc_error(GC_INVALID, "workspace is missing or too small");
+    if (!gcb::aligned16(p)) return gc_error(GC_INVALID, "workspace must be 16-byte aligned");
+    return GC_OK;
+}
+
+bool known_activation(int a) {
+    return a == GC_B200_ACT_NONE || a == GC_B200_ACT_RELU || a == GC_B200_ACT_RELU6 || a == GC_B200_ACT_SILU;
+}
+
+// ---- dropout ----------------------------------------------------------------------------------
+// Whether the axes, taken in some order, fill memory without gaps or overlap.
+bool dense_any_order(const gc_tensor *t) {
+    bool used[4] = {false, false, false, false};
+    wide expect = 1;
+    for (int step = 0; step < t->rank; ++step) {
+        int pick = -1;
+        for (int i = 0; i < t->rank; ++i)
+            if (!used[i] && (t->dims[i] == 1 || t->strides[i] == expect) && (pick < 0 || t->dims[i] == 1)) pick = i;
+        if (pick < 0) return false;
+        used[pick] = true;
+        expect *= t->dims[pick];
+    }
+    return true;
+}
+
+// (N, C, ..) in plain order, the innermost axis last?
+bool plain_order(const gc_tensor *t) {
+    wide expect = 1;
+    for (int i = t->rank - 1; i >= 0; --i) {
+        if (t->dims[i] > 1 && t->strides[i] != expect) return false;
+        expect *= t->dims[i];
+    }
+    return true;
+}
+bool channels_last_order(const gc_tensor *t) {
+    if (t->dims[1] > 1 && t->strides[1] != 1) return false;
+    wide expect = t->dims[1];
+    for (int i = t->rank - 1; i >= 2; --i) {
+        if (t->dims[i] > 1 && t->strides[i] != expect) return false;
+        expect *= t->dims[i];
+    }
+    return t->dims[0] <= 1 || t->strides[0] == expect;
+}
+
+template <class T>
+const void *dropout_typed(bool vec, bool channel) {
+    if (channel)
+        return vec ? reinterpret_cast<const void *>(&gcb::dropout_kernel<T, true, true>)
+                   : reinterpret_cast<const void *>(&gcb::dropout_kernel<T, false, true>);
+    return vec ? reinterpret_cast<const void *>(&gcb::dropout_kernel<T, true, false>)
+               : reinterpret_cast<const void *>(&gcb::dropout_kernel<T, false, false>);
+}
+
+}  // namespace
+
+extern "C" {
+
+int gc_b200_group_norm_workspace(const gc_tensor *x, const gc_tensor *y, int64_t groups, uint64_t *bytes) {
+    if (bytes == nullptr) return gc_error(GC_INVALID, "null size pointer");
+    View v[2];
+    NormParams P;
+    NormPlan plan;
+    int st = check_data({x, y}, groups, v, P, plan);
+    if (st != GC_OK) return st;
+    *bytes = 0;
+    if (empty(P)) return gc_error(GC_OK, "");
+    st = plan_norm(P, plan);
+    if (st != GC_OK) return st;
+    *bytes = space_of(P, false).total();
+    return gc_error(GC_OK, "");
+}
+
+int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tensor *beta, gc_tensor *y,
+                       gc_tensor *stats, int64_t groups, double eps, int activation,
+                       const gc_b200_dropout_args *dropout, void *workspace, uint64_t workspace_bytes, void *stream) {
+    View v[2];
+    NormParams P;
+    NormPlan plan;
+    int st = check_data({x, y}, groups, v, P, plan);
+    if (st != GC_OK) return st;
+    if (!(eps >= 0.0) || !std::isfinite(eps)) return gc_error(GC_INVALID, "eps must be finite and not negative");
+    for (const gc_tensor *t : {gamma, beta})
+        if ((st = check_channel_vector(t, x)) != GC_OK) return st;
+    if (stats != nullptr && (st = check_stats(stats, x, groups)) != GC_OK) return st;
+    DropParams drop;
+    if ((st = check_dropout(dropout, drop)) != GC_OK) return st;
+    if (outputs_meet({{y->data, v[1].span}, range_of(stats)}, {{x->data, v[0].span}, range_of(gamma), range_of(beta)}))
+        return gc_error(GC_INVALID, "outputs must not overlap inputs");
+    if (!known_activation(activation)) return gc_error(GC_UNSUPPORTED, "unknown activation");
+    for (const gc_tensor *t : {gamma, beta})
+        if ((st = check_channel_layout(t)) != GC_OK) return st;
+    if (stats != nullptr && !dense_stats(stats)) return gc_error(GC_UNSUPPORTED, "stats must be dense");
+    if (empty(P)) return gc_error(GC_OK, "");
+    int dev = -1;
+    st = check_call({x, y, gamma, beta, stats}, {drop.seed_ptr, drop.offset_ptr, drop.used}, x->device_index, stream,
+                    dev);
+    if (st != GC_OK) return st;
+    if ((st = plan_norm(P, plan)) != GC_OK) return st;
+    const NormSpace space = space_of(P, false);
+    if ((st = check_workspace(workspace, workspace_bytes, space.total())) != GC_OK) return st;
+    if (space.total() != 0 && (st = gcb::check_device_memory(workspace, x->device_index, dev)) != GC_OK) return st;
+    P.x = v[0].data;
+    P.x_ldn = v[0].ldn;
+    P.x_ldp = v[0].ldp;
+    P.y = v[1].data;
+    P.y_ldn = v[1].ldn;
+    P.y_ldp = v[1].ldp;
+    set_param(gamma, P.gamma, P.gamma_type);
+    set_param(beta, P.beta, P.beta_type);
+    P.eps = static_cast<float>(eps);
+    P.act = activation;
+    P.drop = drop;
+    char *w = static_cast<char *>(workspace);
+    P.stats = reinterpret_cast<float2 *>(stats != nullptr ? static_cast<char *>(stats->data) : w);
+    P.part = reinterpret_cast<float2 *>(w + space.stats);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    cudaError_t e = launch(norm_kernel(kMoments, plan, activation), P.items, P, s);
+    if (e == cudaSuccess)
+        e = launch(reinterpret_cast<const void *>(&gcb::norm_finalize_kernel), P.n * P.groups, P, s);
+    if (e == cudaSuccess) e = launch(norm_kernel(kApply, plan, activation), P.items, P, s);
+    gcb::record_plan(PlanRecord::kNorm, "split", false, P.items, gcb::kNormThreads, 0, 1, P.vb, P.chunk_rows,
+                     plan.vec ? 1 : 0, 3);
+    return launched(e);
+}
+
+int gc_b200_group_norm_backward_workspace(const gc_tensor *dy, const gc_tensor *x, const gc_tensor *dx,
+                                          int64_t groups, uint64_t *bytes) {
+    if (bytes == nullptr) return gc_error(GC_INVALID, "null size pointer");
+    View v[3];
+    NormParams P;
+    NormPlan plan;
+    int st = check_data({x, dy, dx}, groups, v, P, plan);
+    if (st != GC_OK) return st;
+    *bytes = 0;
+    if (empty(P)) return gc_error(GC_OK, "");
+    st = plan_norm(P, plan);
+    if (st != GC_OK) return st;
+    *bytes = space_of(P, true).total();
+    return gc_error(GC_OK, "");
+}
+
+int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const gc_tensor *gamma,
+                                const gc_tensor *beta, const gc_tensor *stats, gc_tensor *dx, gc_tensor *dgamma,
+                                gc_tensor *dbeta, int64_t groups, int activation,
+                                const gc_b200_dropout_args *dropout, void *workspace, uint64_t workspace_bytes,
+                                void *stream) {
+    View v[3];
+    NormParams P;
+    NormPlan plan;
+    int st = check_data({x, dy, dx}, groups, v, P, plan);
+    if (st != GC_OK) return st;
+    for (const gc_tensor *t : {gamma, beta, static_cast<const gc_tensor *>(dgamma),
+                               static_cast<const gc_tensor *>(dbeta)})
+        if ((st = check_channel_vector(t, x)) != GC_OK) return st;
+    if ((st = check_stats(stats, x, groups)) != GC_OK) return st;
+    DropParams drop;
+    if ((st = check_dropout(dropout, drop)) != GC_OK) return st;
+    if (outputs_meet({{dx->data, v[2].span}, range_of(dgamma), range_of(dbeta)},
+                     {{x->data, v[0].span}, {dy->data, v[1].span}, range_of(gamma), range_of(beta), range_of(stats)}))
+        return gc_error(GC_INVALID, "outputs must not overlap inputs");
+    if (!known_activation(activation)) return gc_error(GC_UNSUPPORTED, "unknown activation");
+    for (const gc_tensor *t : {gamma, beta, static_cast<const gc_tensor *>(dgamma),
+                               static_cast<const gc_tensor *>(dbeta)})
+        if ((st = check_channel_layout(t)) != GC_OK) return st;
+    if (!dense_stats(stats)) return gc_error(GC_UNSUPPORTED, "stats must be dense");
+    int dev = -1;
+    st = check_call({x, dy, dx, gamma, beta, stats, dgamma, dbeta}, {drop.seed_ptr, drop.offset_ptr, drop.used},
+                    x->device_index, stream, dev);
+    if (st != GC_OK) return st;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (empty(P)) {  // sums over nothing
+        cudaError_t e = cudaSuccess;
+        for (const gc_tensor *t : {dgamma, dbeta})
+            if (t != nullptr && e == cudaSuccess) e = cudaMemsetAsync(t->data, 0, range_of(t).bytes, s);
+        return launched(e);
+    }
+    if ((st = plan_norm(P, plan)) != GC_OK) return st;
+    const NormSpace space = space_of(P, true);
+    if ((st = check_workspace(workspace, workspace_bytes, space.total())) != GC_OK) return st;
+    if (space.total() != 0 && (st = gcb::check_device_memory(workspace, x->device_index, dev)) != GC_OK) return st;
+    P.x = v[0].data;
+    P.x_ldn = v[0].ldn;
+    P.x_ldp = v[0].ldp;
+    P.dy = v[1].data;
+    P.dy_ldn = v[1].ldn;
+    P.dy_ldp = v[1].ldp;
+    P.y = v[2].data;
+    P.y_ldn = v[2].ldn;
+    P.y_ldp = v[2].ldp;
+    set_param(gamma, P.gamma, P.gamma_type);
+    set_param(beta, P.beta, P.beta_type);
+    const void *q = nullptr;
+    set_param(dgamma, q, P.dgamma_type);
+    P.dgamma = const_cast<void *>(q);
+    set_param(dbeta, q, P.dbeta_type);
+    P.dbeta = const_cast<void *>(q);
+    P.act = activation;
+    P.drop = drop;
+    P.stats = static_cast<float2 *>(stats->data);
+    char *w = static_cast<char *>(workspace);
+    P.part = reinterpret_cast<float2 *>(w);
+    P.chan = reinterpret_cast<float2 *>(w + space.part);
+    P.gsum = reinterpret_cast<float2 *>(w + space.part + space.chan);
+    cudaError_t e = launch(norm_kernel(kGradSums, plan, activation), P.items, P, s);
+    if (e == cudaSuccess)
+        e = launch(reinterpret_cast<const void *>(&gcb::norm_grad_finalize_kernel), P.n * P.groups, P, s);
+    if (e == cudaSuccess) e = launch(norm_kernel(kGradApply, plan, activation), P.items, P, s);
+    const bool params = P.dgamma != nullptr || P.dbeta != nullptr;
+    if (e == cudaSuccess && params)
+        e = launch(reinterpret_cast<const void *>(&gcb::norm_grad_params_kernel), ceil_div(P.c, 32), P, s);
+    gcb::record_plan(PlanRecord::kNorm, "split_backward", false, P.items, gcb::kNormThreads, 0, 1, P.vb, P.chunk_rows,
+                     plan.vec ? 1 : 0, params ? 4 : 3);
+    return launched(e);
+}
+
+int gc_b200_dropout(const gc_tensor *x, const gc_tensor *residual, gc_tensor *y,
+                    const gc_b200_dropout_args *dropout, void *stream) {
+    int64_t count = 0;
+    for (const gc_tensor *t : {x, static_cast<const gc_tensor *>(y), residual}) {
+        if (t == nullptr && t == residual && x != nullptr && y != nullptr) continue;
+        const int st = check_fields(t, 1, 4, count);
+        if (st != GC_OK) return st;
+        if (!same_dims(t, x)) return gc_error(GC_INVALID, "tensor dimensions differ");
+        if (t->dtype != x->dtype) return gc_error(GC_INVALID, "tensor dtypes differ");
+        if (t->device_index != x->device_index) return gc_error(GC_INVALID, "tensor device indices differ");
+    }
+    if (dropout == nullptr) return gc_error(GC_INVALID, "null dropout arguments");
+    DropParams drop;
+    int st = check_dropout(dropout, drop);
+    if (st != GC_OK) return st;
+    if (outputs_meet({range_of(y)}, {range_of(x), range_of(residual)}))
+        return gc_error(GC_INVALID, "outputs must not overlap inputs");
+    if (drop.channel && x->rank < 2) return gc_error(GC_INVALID, "channel dropout needs a channel axis");
+    if (x->dtype == GC_F64) return gc_error(GC_UNSUPPORTED, "FP64 tensors are not supported here");
+    if (count == 0) return gc_error(GC_OK, "");
+    for (const gc_tensor *t : {static_cast<const gc_tensor *>(y), residual})
+        if (t != nullptr)
+            for (int i = 0; i < x->rank; ++i)
+                if (x->dims[i] > 1 && t->strides[i] != x->strides[i])
+                    return gc_error(GC_UNSUPPORTED, "tensors must have the same strides");
+    if (!dense_any_order(x)) return gc_error(GC_UNSUPPORTED, "tensors must be dense");
+    DropoutParams P{};
+    if (drop.channel) {
+        const bool plain = plain_order(x);
+        if (!plain && !channels_last_order(x))
+            return gc_error(GC_UNSUPPORTED, "channel dropout needs plain or channels-last order");
+        P.channels = static_cast<uint64_t>(x->dims[1]);
+        P.image = static_cast<uint64_t>(count / x->dims[0]);
+        P.inner = plain ? P.image / P.channels : 1;
+    }
+    int dev = -1;
+    st = check_call({x, y, residual}, {drop.seed_ptr, drop.offset_ptr, drop.used}, x->device_index, stream, dev);
+    if (st != GC_OK) return st;
+    P.x = x->data;
+    P.residual = residual != nullptr ? residual->data : nullptr;
+    P.y = y->data;
+    P.count = static_cast<uint64_t>(count);
+    P.groups = (P.count + 7) / 8;
+    P.drop = drop;
+    const bool vec = gcb::aligned16(P.x) && gcb::aligned16(P.y) && gcb::aligned16(P.residual);
+    const int type = elem_type(x->dtype);
+    const void *fn = type == gcb::kElemF16    ? dropout_typed<__half>(vec, drop.channel)
+                     : type == gcb::kElemBF16 ? dropout_typed<__nv_bfloat16>(vec, drop.channel)
+                                              : dropout_typed<float>(vec, drop.channel);
+    const unsigned grid = grid_of(ceil_div(static_cast<long long>(P.groups), 256));
+    void *args[] = {&P};
+    const cudaError_t e = gcb::launch_pdl(fn, dim3(grid), dim3(256), args, 0, reinterpret_cast<cudaStream_t>(stream));
+    gcb::record_plan(PlanRecord::kDropout, drop.channel ? "channel" : "element", false, grid, 256, vec ? 1 : 0);
+    return launched(e);
+}
+
+}  // extern "C"

@@ -6,13 +6,20 @@
 // element strides, the tensor's device and device index, float32 or float64.
 // Errors come back as gc_status values with the library's thread-local
 // message; nothing here computes a convolution.  conv_ex does the same for
-// gc_b200_conv_ex (bias, activation, channels-last output).
+// gc_b200_conv_ex (bias, activation, channels-last output); group_norm and
+// dropout do it for gc_b200_group_norm and gc_b200_dropout and record their
+// gradients with autograd.
 #include <torch/extension.h>
+#include <ATen/cuda/CUDAGeneratorImpl.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
+#include <mutex>
 #include <stdexcept>
 #include <string>
+#include <tuple>
+#include <vector>
 
 #include "groupconv.h"
 
@@ -83,10 +90,317 @@ at::Tensor conv_ex(const at::Tensor &x, const at::Tensor &w, const c10::optional
     return y;
 }
 
+
+// ---- group norm and dropout -----------------------------------------------------
+
+[[noreturn]] void fail(int status) {
+    throw std::runtime_error("gc_status " + std::to_string(status) + ": " + gc_last_error());
+}
+
+// As describe(), for the entry points that also take 16-bit types and strided
+// views: bytes covers the view from its first to its last element.
+gc_tensor describe_view(const at::Tensor &t) {
+    gc_tensor d = describe(t);
+    if (t.scalar_type() == at::kHalf) d.dtype = GC_B200_F16;
+    if (t.scalar_type() == at::kBFloat16) d.dtype = GC_B200_BF16;
+    if (t.numel() > 0) {
+        int64_t last = 1;
+        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+        d.bytes = static_cast<uint64_t>(last) * t.element_size();
+    }
+    return d;
+}
+
+void *stream_of(const at::Tensor &t) {
+    return t.is_cuda() ? static_cast<void *>(c10::cuda::getCurrentCUDAStream(t.get_device()).stream()) : nullptr;
+}
+
+at::Tensor workspace_of(uint64_t bytes, const at::Tensor &like) {
+    return bytes == 0 ? at::Tensor()
+                      : at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte).memory_format(
+                                                                     at::MemoryFormat::Contiguous));
+}
+
+// Dense (N, C, ..) with the channels innermost, which is what channels_last
+// means for rank 4 and what this library computes for ranks 2 and 3 too.
+at::Tensor empty_channels_last(const at::Tensor &x) {
+    std::vector<int64_t> strides(x.dim());
+    int64_t expect = x.size(1);
+    strides[1] = 1;
+    for (int64_t i = x.dim() - 1; i >= 2; --i) {
+        strides[i] = expect;
+        expect *= std::max<int64_t>(x.size(i), 1);
+    }
+    strides[0] = expect;
+    return at::empty_strided(x.sizes(), strides, x.options());
+}
+
+// Whether gc_b200_group_norm reads t as it lies: channel stride 1, evenly
+// spaced pixels, images that do not interleave.
+bool pixels_in_order(const at::Tensor &t) {
+    if (t.size(1) > 1 && t.stride(1) != 1) return false;
+    int64_t px = 1, ldp = t.size(1);
+    for (int64_t i = t.dim() - 1; i >= 2; --i) {
+        if (t.size(i) > 1) {
+            if (px == 1) ldp = t.stride(i);
+            else if (t.stride(i) != ldp * px) return false;
+        }
+        px *= t.size(i);
+    }
+    return ldp >= t.size(1) && (t.size(0) <= 1 || t.stride(0) >= (px - 1) * ldp + t.size(1));
+}
+at::Tensor in_order(const at::Tensor &t) {
+    if (t.numel() == 0 || pixels_in_order(t)) return t;
+    at::Tensor copy = empty_channels_last(t);
+    copy.copy_(t);
+    return copy;
+}
+
+// The dropout of one forward call and of its gradient.
+struct Drop {
+    gc_b200_dropout_args args{};
+    at::Tensor used;  // the device words in effect, when the generator's are known only to a captured graph
+    bool on = false;
+};
+
+// seed given: that seed and offset.  Otherwise torch's CUDA generator, which
+// also works inside a graph capture (a replay draws anew); the top bit of the
+// offset keeps these draws apart from torch's own, which count from 0.
+Drop make_drop(const at::Tensor &x, double p, int64_t scope, const c10::optional<uint64_t> &seed, uint64_t offset,
+               bool grad) {
+    Drop d;
+    d.on = p != 0.0;
+    d.args.p = p;
+    d.args.scope = static_cast<int32_t>(scope);
+    if (!d.on) return d;
+    if (seed.has_value()) {
+        d.args.seed = *seed;
+        d.args.offset = offset;
+        return d;
+    }
+    if (!x.is_cuda()) return d;  // refused by the call
+    auto *gen = at::get_generator_or_default<at::CUDAGeneratorImpl>(
+        c10::nullopt, at::cuda::detail::getDefaultCUDAGenerator(x.get_device()));
+    at::PhiloxCudaState state;
+    {
+        std::lock_guard<std::mutex> lock(gen->mutex_);
+        state = gen->philox_cuda_state(4);
+    }
+    constexpr uint64_t kOwn = 1ull << 63;
+    if (state.captured_) {
+        d.args.seed_ptr = reinterpret_cast<const uint64_t *>(state.seed_.ptr);
+        d.args.offset_ptr = reinterpret_cast<const uint64_t *>(state.offset_.ptr);
+        d.args.offset = kOwn + state.offset_intragraph_;
+        if (grad) {
+            d.used = at::empty({2}, x.options().dtype(at::kLong).memory_format(at::MemoryFormat::Contiguous));
+            d.args.used = reinterpret_cast<uint64_t *>(d.used.data_ptr<int64_t>());
+        }
+    } else {
+        d.args.seed = state.seed_.val;
+        d.args.offset = kOwn + state.offset_.val;
+    }
+    return d;
+}
+
+// What a gradient has to keep of a forward call's dropout, and that again.
+void save_drop(c10::IValue &out, const Drop &d) {
+    out = c10::IValue(std::tuple<bool, double, int64_t, int64_t, int64_t>(
+        d.on, d.args.p, d.args.scope, static_cast<int64_t>(d.args.seed), static_cast<int64_t>(d.args.offset)));
+}
+Drop load_drop(const c10::IValue &v, const at::Tensor &used) {
+    const auto &e = v.toTupleRef().elements();
+    Drop d;
+    d.on = e[0].toBool();
+    d.args.p = e[1].toDouble();
+    d.args.scope = static_cast<int32_t>(e[2].toInt());
+    if (used.defined()) {
+        const uint64_t *w = reinterpret_cast<const uint64_t *>(used.data_ptr<int64_t>());
+        d.args.seed_ptr = w;
+        d.args.offset_ptr = w + 1;
+    } else {
+        d.args.seed = static_cast<uint64_t>(e[3].toInt());
+        d.args.offset = static_cast<uint64_t>(e[4].toInt());
+    }
+    return d;
+}
+
+void no_double_backward() {
+    if (at::GradMode::is_enabled())
+        throw std::runtime_error("the gradient of this operation is not differentiable (create_graph)");
+}
+
+struct NormArgs {
+    int64_t groups = 1, activation = 0;
+    double eps = 0.0;
+};
+
+// One gc_b200_group_norm call; stats undefined for none.
+at::Tensor norm_forward(const at::Tensor &x, const at::Tensor &gamma, const at::Tensor &beta, const NormArgs &a,
+                        const Drop &drop, at::Tensor stats) {
+    at::Tensor y = empty_channels_last(x);
+    const gc_tensor xd = describe_view(x);
+    gc_tensor yd = describe_view(y), gd{}, bd{}, sd{};
+    if (gamma.defined()) gd = describe_view(gamma);
+    if (beta.defined()) bd = describe_view(beta);
+    if (stats.defined()) sd = describe_view(stats);
+    uint64_t bytes = 0;
+    int st = gc_b200_group_norm_workspace(&xd, &yd, a.groups, &bytes);
+    if (st != GC_OK) fail(st);
+    const at::Tensor space = workspace_of(bytes, x);
+    st = gc_b200_group_norm(&xd, gamma.defined() ? &gd : nullptr, beta.defined() ? &bd : nullptr, &yd,
+                            stats.defined() ? &sd : nullptr, a.groups, a.eps, static_cast<int>(a.activation),
+                            drop.on ? &drop.args : nullptr, space.defined() ? space.data_ptr() : nullptr, bytes,
+                            stream_of(x));
+    if (st != GC_OK) fail(st);
+    return y;
+}
+
+struct GroupNorm : torch::autograd::Function<GroupNorm> {
+    static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x,
+                              const c10::optional<at::Tensor> &gamma, const c10::optional<at::Tensor> &beta,
+                              NormArgs a, Drop drop) {
+        const at::Tensor g = gamma.value_or(at::Tensor()), b = beta.value_or(at::Tensor());
+        at::Tensor stats = at::empty({x.size(0), a.groups, 2}, x.options().dtype(at::kFloat).memory_format(
+                                                                  at::MemoryFormat::Contiguous));
+        at::Tensor y = norm_forward(x, g, b, a, drop, stats);
+        ctx->save_for_backward({x, g, b, stats, drop.used});
+        ctx->saved_data["groups"] = a.groups;
+        ctx->saved_data["activation"] = a.activation;
+        save_drop(ctx->saved_data["drop"], drop);
+        return y;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                   torch::autograd::variable_list grads) {
+        no_double_backward();
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &gamma = saved[1], &beta = saved[2], &stats = saved[3];
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        const Drop drop = load_drop(ctx->saved_data["drop"], saved[4]);
+        const int64_t groups = ctx->saved_data["groups"].toInt();
+        c10::OptionalDeviceGuard guard(x.device());
+        const at::Tensor dy = in_order(grads[0]);
+        at::Tensor dx = empty_channels_last(x), dgamma, dbeta;
+        // needs_input_grad counts the tensors that were given
+        if (gamma.defined() && ctx->needs_input_grad(1)) dgamma = at::empty_like(gamma);
+        if (beta.defined() && ctx->needs_input_grad(gamma.defined() ? 2 : 1)) dbeta = at::empty_like(beta);
+        const gc_tensor xd = describe_view(x), dyd = describe_view(dy);
+        gc_tensor dxd = describe_view(dx), sd = describe_view(stats), gd{}, bd{}, dgd{}, dbd{};
+        if (gamma.defined()) gd = describe_view(gamma);
+        if (beta.defined()) bd = describe_view(beta);
+        if (dgamma.defined()) dgd = describe_view(dgamma);
+        if (dbeta.defined()) dbd = describe_view(dbeta);
+        uint64_t bytes = 0;
+        int st = gc_b200_group_norm_backward_workspace(&dyd, &xd, &dxd, groups, &bytes);
+        if (st != GC_OK) fail(st);
+        const at::Tensor space = workspace_of(bytes, x);
+        st = gc_b200_group_norm_backward(
+            &dyd, &xd, gamma.defined() ? &gd : nullptr, beta.defined() ? &bd : nullptr, &sd, &dxd,
+            dgamma.defined() ? &dgd : nullptr, dbeta.defined() ? &dbd : nullptr, groups,
+            static_cast<int>(ctx->saved_data["activation"].toInt()), drop.on ? &drop.args : nullptr,
+            space.defined() ? space.data_ptr() : nullptr, bytes, stream_of(x));
+        if (st != GC_OK) fail(st);
+        return {dx, dgamma, dbeta, at::Tensor(), at::Tensor()};
+    }
+};
+
+bool wants_grad(const at::Tensor &t) { return t.defined() && t.requires_grad(); }
+
+at::Tensor group_norm(const at::Tensor &x, const c10::optional<at::Tensor> &gamma,
+                      const c10::optional<at::Tensor> &beta, int64_t groups, double eps, int64_t activation, double p,
+                      int64_t scope, const c10::optional<uint64_t> &seed, uint64_t offset) {
+    if (x.dim() < 2 || x.dim() > 4) throw std::invalid_argument("input must have 2 to 4 axes (N, C, ..)");
+    c10::OptionalDeviceGuard guard;
+    if (x.is_cuda()) guard.reset_device(x.device());
+    const at::Tensor g = gamma.value_or(at::Tensor()), b = beta.value_or(at::Tensor());
+    const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(g) || wants_grad(b));
+    const at::Tensor xi = in_order(x);
+    const Drop drop = make_drop(x, p, scope, seed, offset, grad);
+    const NormArgs a{groups, activation, eps};
+    return grad ? GroupNorm::apply(xi, gamma, beta, a, drop) : norm_forward(xi, g, b, a, drop, at::Tensor());
+}
+
+// One gc_b200_dropout call on tensors that lie alike.
+at::Tensor dropout_forward(const at::Tensor &x, const at::Tensor &residual, const Drop &drop) {
+    at::Tensor y = at::empty_like(x);
+    const gc_tensor xd = describe_view(x);
+    gc_tensor yd = describe_view(y), rd{};
+    if (residual.defined()) rd = describe_view(residual);
+    const int st = gc_b200_dropout(&xd, residual.defined() ? &rd : nullptr, &yd, &drop.args, stream_of(x));
+    if (st != GC_OK) fail(st);
+    return y;
+}
+
+// `t` laid out like `like`, which is dense.
+at::Tensor laid_out_like(const at::Tensor &t, const at::Tensor &like) {
+    if (t.sizes() != like.sizes() || t.numel() == 0) return t;  // refused by the call, or nothing to lay out
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.size(i) > 1 && t.stride(i) != like.stride(i)) {
+            at::Tensor copy = at::empty_strided(like.sizes(), like.strides(), t.options());
+            copy.copy_(t);
+            return copy;
+        }
+    return t;
+}
+
+struct Dropout : torch::autograd::Function<Dropout> {
+    static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x,
+                              const c10::optional<at::Tensor> &residual, Drop drop) {
+        // the gradient needs x's layout only, so nothing of its data is kept
+        ctx->saved_data["sizes"] = x.sizes().vec();
+        ctx->saved_data["strides"] = x.strides().vec();
+        ctx->saved_data["residual"] = residual.has_value() && residual->defined();
+        ctx->save_for_backward({drop.used});
+        save_drop(ctx->saved_data["drop"], drop);
+        return dropout_forward(x, residual.value_or(at::Tensor()), drop);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                   torch::autograd::variable_list grads) {
+        no_double_backward();
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
+        const auto saved = ctx->get_saved_variables();
+        const Drop drop = load_drop(ctx->saved_data["drop"], saved[0]);
+        c10::OptionalDeviceGuard guard(grads[0].device());
+        at::Tensor dx;
+        if (ctx->needs_input_grad(0)) {
+            // the mask goes by place in memory: dy has to lie as x did
+            const auto sizes = ctx->saved_data["sizes"].toIntVector(), strides = ctx->saved_data["strides"].toIntVector();
+            at::Tensor dy = grads[0];
+            bool same = true;
+            for (size_t i = 0; i < sizes.size(); ++i) same = same && (sizes[i] <= 1 || dy.stride(i) == strides[i]);
+            if (!same) {
+                dy = at::empty_strided(sizes, strides, grads[0].options());
+                dy.copy_(grads[0]);
+            }
+            dx = dropout_forward(dy, at::Tensor(), drop);
+        }
+        return {dx, ctx->saved_data["residual"].toBool() ? grads[0] : at::Tensor(), at::Tensor()};
+    }
+};
+
+at::Tensor dropout(const at::Tensor &x, const c10::optional<at::Tensor> &residual, double p, int64_t scope,
+                   const c10::optional<uint64_t> &seed, uint64_t offset) {
+    if (x.dim() < 1 || x.dim() > 4) throw std::invalid_argument("input must have 1 to 4 axes");
+    c10::OptionalDeviceGuard guard;
+    if (x.is_cuda()) guard.reset_device(x.device());
+    // dense in the order of its axes, else copied; channel decisions know two orders
+    at::Tensor xi = x;
+    const bool plain = x.is_contiguous();
+    const bool last = x.dim() == 4 && x.is_contiguous(at::MemoryFormat::ChannelsLast);
+    if (!plain && !last && (scope == GC_B200_DROP_CHANNEL || !x.is_non_overlapping_and_dense())) xi = x.contiguous();
+    const at::Tensor r0 = residual.value_or(at::Tensor());
+    c10::optional<at::Tensor> r;
+    if (r0.defined()) r = laid_out_like(r0, xi);
+    const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(r0));
+    Drop drop = make_drop(x, p, scope, seed, offset, grad);
+    return grad ? Dropout::apply(xi, r, drop) : dropout_forward(xi, r.value_or(at::Tensor()), drop);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_gcb_torch, m) {
     m.doc() = "gc_cuda_conv for torch tensors: output allocation and the C ABI call in C++";
     m.def("conv", &conv, "y = gc_cuda_conv(x, w) on the current CUDA stream");
     m.def("conv_ex", &conv_ex, "y = act(conv(x, w) + bias) through gc_b200_conv_ex on the current CUDA stream");
+    m.def("group_norm", &group_norm, "gc_b200_group_norm on the current CUDA stream, with its gradient");
+    m.def("dropout", &dropout, "gc_b200_dropout on the current CUDA stream, with its gradient");
 }

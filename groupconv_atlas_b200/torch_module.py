@@ -12,6 +12,10 @@ just in device time.  Without that front end the module falls back to ctypes
 descriptors built once per input geometry (only their data pointers change per
 call).  Both paths run the same CUDA kernels; outputs are computed on the GPU
 only, and a missing library or an unsupported geometry raises NativeError.
+
+Between convolutions: group_norm_act and B200GroupNormAct (GroupNorm ->
+activation -> dropout as one gc_b200_group_norm call) and dropout and
+B200Dropout (gc_b200_dropout), all with gradients through the C++ front end.
 """
 from __future__ import annotations
 
@@ -206,6 +210,145 @@ def fuse_conv_bn_act(module: torch.nn.Module, predicate, native: api.Native | No
             except ValueError:
                 continue
             child._modules[attr] = fused
+            replaced.append(f'{name}.{attr}' if name else attr)
+    return replaced
+
+
+def _front_end(name: str):
+    """An entry point of the C++ front end, which these operators need: their
+    gradients are recorded with autograd there."""
+    try:
+        from . import _gcb_torch
+    except ImportError as e:
+        raise FileNotFoundError('the PyTorch front end is not built: '
+                                'groupconv_atlas_b200.build.build_torch_ext()') from e
+    return getattr(_gcb_torch, name)
+
+
+def _native_call(op, *args):
+    try:
+        return op(*args)
+    except RuntimeError as e:
+        text = str(e)
+        if text.startswith('gc_status '):
+            status, _, message = text[len('gc_status '):].partition(': ')
+            raise api.NativeError(int(status), message) from None
+        raise
+
+
+def _scope_code(scope: str) -> int:
+    if scope not in api.DROP_SCOPES:
+        raise ValueError(f"dropout scope must be one of {', '.join(api.DROP_SCOPES)}")
+    return api.DROP_SCOPES[scope]
+
+
+def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
+                   bias: torch.Tensor | None = None, eps: float = 1e-5, activation: str = 'none',
+                   dropout: float = 0.0, scope: str = 'element', seed: int | None = None,
+                   offset: int = 0) -> torch.Tensor:
+    """dropout(activation(group_norm(x))) as one gc_b200_group_norm call.
+
+    x is (N, C), (N, C, L) or (N, C, H, W), float32, float16 or bfloat16, and is
+    computed channels last: a channels_last tensor, or a channel slice of one,
+    is read as it lies, anything else is copied first.  The result is dense and
+    channels last.  weight and bias have C elements, float32 or x's type.
+    activation is 'none', 'relu', 'relu6' or 'silu'.
+
+    dropout is the probability of dropping, per 'element' or per 'channel' of
+    an image (scope).  With a seed, the decisions are those of (seed, offset),
+    see include/groupconv.h; without one they come from torch's CUDA generator,
+    also inside a graph capture.  Differentiable once; the gradient draws the
+    mask again, so none is stored."""
+    if activation not in api.NORM_ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(api.NORM_ACTIVATIONS)}")
+    return _native_call(_front_end('group_norm'), x, weight, bias, groups, eps, api.NORM_ACTIVATIONS[activation],
+                        dropout, _scope_code(scope), seed, offset)
+
+
+def dropout(x: torch.Tensor, p: float, residual: torch.Tensor | None = None, scope: str = 'element',
+            seed: int | None = None, offset: int = 0) -> torch.Tensor:
+    """[residual +] dropout(x) as one gc_b200_dropout call; x has one to four
+    axes.  A decision goes by its element's place in memory (scope 'element')
+    or by image and channel (scope 'channel'); a residual of other strides than
+    x is copied first.  seed and offset as in group_norm_act."""
+    return _native_call(_front_end('dropout'), x, residual, p, _scope_code(scope), seed, offset)
+
+
+def _norm_activation_name(act: torch.nn.Module | None) -> str:
+    return 'silu' if isinstance(act, torch.nn.SiLU) else _activation_name(act)
+
+
+class B200GroupNormAct(torch.nn.Module):
+    """GroupNorm -> activation -> dropout as one call, in training and
+    inference.  Keeps the norm's own parameters (and their names); dropout
+    (torch.nn.Dropout, or Dropout2d for whole channels) acts in training only."""
+
+    def __init__(self, norm: torch.nn.GroupNorm, act: torch.nn.Module | None = None,
+                 drop: torch.nn.Module | None = None):
+        super().__init__()
+        self.groups, self.eps = norm.num_groups, norm.eps
+        self.weight, self.bias = norm.weight, norm.bias
+        self.activation = _norm_activation_name(act)
+        if drop is not None and not isinstance(drop, (torch.nn.Dropout, torch.nn.Dropout2d)):
+            raise ValueError(f'{type(drop).__name__} has no epilogue in gc_b200_group_norm')
+        self.p = drop.p if drop is not None else 0.0
+        self.scope = 'channel' if isinstance(drop, torch.nn.Dropout2d) else 'element'
+        self.train(norm.training)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return group_norm_act(x, self.groups, self.weight, self.bias, self.eps, self.activation,
+                              self.p if self.training else 0.0, self.scope)
+
+    def extra_repr(self) -> str:
+        return f'groups={self.groups}, eps={self.eps}, activation={self.activation}, p={self.p}, scope={self.scope}'
+
+
+class B200Dropout(torch.nn.Module):
+    """Dropout without a stored mask; forward(x, residual) also adds the
+    residual, in evaluation too.  scope 'channel' drops whole channels."""
+
+    def __init__(self, p: float = 0.5, scope: str = 'element'):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError('dropout probability must be between 0 and 1')
+        _scope_code(scope)
+        self.p, self.scope = p, scope
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        if not self.training or self.p == 0.0:
+            return x if residual is None else residual + x
+        return dropout(x, self.p, residual, self.scope)
+
+    def extra_repr(self) -> str:
+        return f'p={self.p}, scope={self.scope}'
+
+
+def fuse_norm_act(module: torch.nn.Module) -> list[str]:
+    """In every Sequential, replace each GroupNorm with the activation (none,
+    ReLU, ReLU6, SiLU) and the dropout (Dropout, Dropout2d) that follow it by
+    one B200GroupNormAct; the members it takes over become Identity, so every
+    other member keeps its name.  Returns the dotted names replaced."""
+    replaced = []
+    for name, child in list(module.named_modules()):
+        if not isinstance(child, torch.nn.Sequential):
+            continue
+        members = list(child._modules.items())
+        for at, (attr, norm) in enumerate(members):
+            if not isinstance(norm, torch.nn.GroupNorm):
+                continue
+            act = drop = None
+            taken = []
+            for follower, sub in members[at + 1:]:
+                if drop is None and isinstance(sub, (torch.nn.Dropout, torch.nn.Dropout2d)):
+                    drop = sub
+                elif drop is None and act is None and isinstance(sub, (torch.nn.ReLU, torch.nn.ReLU6, torch.nn.SiLU)):
+                    act = sub
+                else:
+                    break
+                taken.append(follower)
+            child._modules[attr] = B200GroupNormAct(norm, act, drop)
+            for follower in taken:
+                child._modules[follower] = torch.nn.Identity()
             replaced.append(f'{name}.{attr}' if name else attr)
     return replaced
 

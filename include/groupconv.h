@@ -161,6 +161,98 @@ int gc_b200_conv_ex(const gc_shape *p, const gc_tensor *x, const gc_tensor *w,
                     const gc_tensor *bias, gc_tensor *y, int layout,
                     int activation, void *stream);
 
+/* ---- normalisation and dropout between convolutions -----------------------
+ * What a network with group normalisation runs between two convolutions.  (A
+ * batch normalisation folds into the convolution's weights; a group
+ * normalisation cannot, its statistics are the input's own.)
+ *
+ * Element types.  These entry points take F32 tensors like the convolutions
+ * and two 16-bit types as well; every sum, statistic and intermediate is held
+ * in 32 bits, and only the stored result is rounded to the tensor's type. */
+#define GC_B200_F16 16
+#define GC_B200_BF16 17
+
+/* Activation of gc_b200_group_norm only: v / (1 + exp(-v)). */
+#define GC_B200_ACT_SILU 3
+
+/* What one keep-or-drop decision covers. */
+#define GC_B200_DROP_ELEMENT 0 /* one element                      */
+#define GC_B200_DROP_CHANNEL 1 /* a whole channel of one image     */
+
+/* Dropout from a counter-based generator; the mask is never stored.
+ *   keep(j) = draw(j) >= t,  t = round(65536 p),  q = t / 65536
+ *   kept values are divided by 1 - q (the probability that is applied, at
+ *   most 2^-17 from p); dropped ones become 0 whatever they hold.
+ * draw(j) is 16 bits of Philox4x32-10 (Salmon, Moraes, Dror and Shaw, 2011):
+ * key = seed, counter = (j / 8 in 64 bits, offset in 64 bits), half j % 2 (low
+ * one first) of word (j % 8) / 2.  j is the element's place in the dense
+ * memory order of the tensor, or n * C + c with GC_B200_DROP_CHANNEL.  A
+ * gradient repeats the mask by passing the same seed and offset; two calls
+ * with different offsets have independent masks.
+ *   seed_ptr, offset_ptr   nullable device words, added to seed and offset
+ *                          when the kernel runs (so a captured graph can draw
+ *                          anew at each replay);
+ *   used                   nullable device pair that receives the seed and
+ *                          offset in effect, for a later gradient.  Must not
+ *                          be one of the two words above. */
+typedef struct {
+    double p; /* 0 <= p <= 1 */
+    uint64_t seed, offset;
+    const uint64_t *seed_ptr, *offset_ptr;
+    uint64_t *used;
+    int32_t scope;
+} gc_b200_dropout_args;
+
+/* Group normalisation, activation and dropout of a channels-last tensor, as
+ * one call:
+ *   y = dropout(act((x - mean) / sqrt(var + eps) * gamma[c] + beta[c]))
+ * with mean and (biased) variance over the pixels and the C / groups channels
+ * of one group of one image.
+ *   x, y        same dims and type, rank 2 (N, C), 3 (N, C, L) or 4
+ *               (N, C, H, W); the channel stride is 1 and the pixels of an
+ *               image are evenly spaced (strides (.., 1, W * P, P) with
+ *               P >= C): channels_last tensors and channel slices of them.
+ *               Other strides -> GC_UNSUPPORTED.  N, H, W of 0 are valid and
+ *               launch nothing.
+ *   gamma, beta NULL, or rank-1 dense tensors of C elements, F32 or x's type.
+ *   stats       NULL, or a dense F32 tensor of dims (N, groups, 2) that
+ *               receives mean and 1 / sqrt(var + eps) for the gradient.
+ *   activation  GC_B200_ACT_NONE, _RELU, _RELU6 or _SILU (a NaN stays NaN).
+ *   dropout     NULL for none.
+ *   workspace   16-byte aligned device memory of at least the bytes that
+ *               gc_b200_group_norm_workspace gives for these tensors (NULL
+ *               when that is 0); its contents need not be set and are
+ *               undefined afterwards.
+ * Outputs overlap no input.  Validation, device, stream, allocation and
+ * capture rules are those of gc_cuda_conv.  Results are bitwise reproducible. */
+int gc_b200_group_norm_workspace(const gc_tensor *x, const gc_tensor *y, int64_t groups, uint64_t *bytes);
+int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tensor *beta, gc_tensor *y,
+                       gc_tensor *stats, int64_t groups, double eps, int activation,
+                       const gc_b200_dropout_args *dropout, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* Its gradient.  x, gamma, beta, groups, activation and dropout are the
+ * forward call's, stats is what it stored, dy the gradient of y.
+ *   dx             like x;
+ *   dgamma, dbeta  NULL, or rank-1 dense tensors of C elements, F32 or x's
+ *                  type (with N, H or W of 0 they are set to 0).
+ * The derivative of ReLU at 0 and of ReLU6 at 0 and 6 is 0. */
+int gc_b200_group_norm_backward_workspace(const gc_tensor *dy, const gc_tensor *x, const gc_tensor *dx,
+                                          int64_t groups, uint64_t *bytes);
+int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const gc_tensor *gamma,
+                                const gc_tensor *beta, const gc_tensor *stats, gc_tensor *dx, gc_tensor *dgamma,
+                                gc_tensor *dbeta, int64_t groups, int activation,
+                                const gc_b200_dropout_args *dropout, void *workspace, uint64_t workspace_bytes,
+                                void *stream);
+
+/* y = [residual +] dropout(x), the sum in 32 bits.  x, residual (nullable)
+ * and y have the same dims, type and strides: rank 1 to 4, dense in any
+ * order of the axes; GC_B200_DROP_CHANNEL needs rank 2 to 4 in plain
+ * (N, C, ..) or channels-last order.  The gradient of x is the same call on
+ * dy without a residual; that of the residual is dy.  An empty tensor is
+ * valid.  y overlaps no input.  Same rules as above otherwise. */
+int gc_b200_dropout(const gc_tensor *x, const gc_tensor *residual, gc_tensor *y,
+                    const gc_b200_dropout_args *dropout, void *stream);
+
 /* Benchmark mode (the counterpart of a framework's "benchmark" convolution
  * search): for a shape that implementation 3 serves with a direct engine,
  * time the planner's `candidates` best-scored tilings (1..64) on these
