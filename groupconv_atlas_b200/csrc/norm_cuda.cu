@@ -9,6 +9,10 @@
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
+#include <map>
+#include <mutex>
+#include <numeric>
+#include <tuple>
 
 #include "host_util.h"
 #include "kernel_dropout.cuh"
@@ -242,15 +246,27 @@ void plan_split(NormParams &P, int v, int sms) {
 
 uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
 
+struct NormPlan {
+    bool vec = false;
+    int type = 0;
+    bool resident = false;
+    int threads = gcb::kNormThreads;
+    size_t smem = 0;
+};
+
 struct NormSpace {  // the workspace's parts, in this order
     uint64_t stats = 0, part = 0, chan = 0, gsum = 0;
     uint64_t total() const { return stats + part + chan + gsum; }
 };
 
 // Bytes of the workspace for a plan that is already in P.
-NormSpace space_of(const NormParams &P, bool backward) {
+NormSpace space_of(const NormParams &P, const NormPlan &plan, bool backward) {
     NormSpace s;
     const uint64_t n = P.n;
+    if (plan.resident) {
+        if (backward) s.part = up16(static_cast<uint64_t>(P.stride * P.cluster) * P.c * sizeof(float2));
+        return s;
+    }
     s.part = up16(n * P.chunks * P.c * sizeof(float2));
     if (backward) {
         s.chan = up16(n * P.c * sizeof(float2));
@@ -260,11 +276,6 @@ NormSpace space_of(const NormParams &P, bool backward) {
     }
     return s;
 }
-
-struct NormPlan {
-    bool vec = false;
-    int type = 0;
-};
 
 // Checks shared by the workspace queries and the calls: data tensors that
 // have the same dims and type, then their layout.  views[0] is x's.
@@ -301,14 +312,138 @@ int check_data(std::initializer_list<const gc_tensor *> tensors, int64_t groups,
 
 bool empty(const NormParams &P) { return P.n == 0 || P.px == 0; }
 
-int plan_norm(NormParams &P, NormPlan &plan) {
+// ---- resident path: plan --------------------------------------------------------------------
+// What a plan depends on.
+struct ResidentKey {
+    int dev, type, backward, drop;
+    long long n, px;
+    int c, groups;
+    bool operator<(const ResidentKey &o) const {
+        return std::tie(dev, type, backward, drop, n, px, c, groups) <
+               std::tie(o.dev, o.type, o.backward, o.drop, o.n, o.px, o.c, o.groups);
+    }
+};
+struct ResidentPlan {
+    bool ok = false;
+    int cb = 0, threads = 0, cluster = 0;
+    size_t smem = 0;
+};
+
+// Fills the resident fields of P for a choice; false when it does not apply.
+bool set_resident(NormParams &P, int v, int cb, int cluster, int threads, bool backward, bool bits, size_t limit,
+                  size_t &smem) {
+    P.cb = cb;
+    P.vr = cb / v;
+    if (P.vr > threads) return false;
+    P.lanes = threads / P.vr;
+    P.sub = v % P.cpg == 0 ? v / P.cpg : P.cpg % v == 0 ? 1 : v;
+    P.gcols = static_cast<int>(static_cast<long long>(P.cpg) * P.sub / v);
+    P.gb = cb / P.cpg;
+    P.bundles = P.c / cb;
+    P.cluster = cluster;
+    const long long rows = ceil_div(P.px, cluster);
+    if (rows > (1 << 20)) return false;
+    P.rows = static_cast<int>(rows);
+    P.iters = static_cast<int>(ceil_div(rows, P.lanes));
+    smem = static_cast<size_t>(P.iters) * threads * (backward ? 32 : 16) +
+           gcb::resident_extra(P, threads, backward) +
+           (bits ? static_cast<size_t>(P.iters) * threads : 0);
+    return smem <= limit;
+}
+
+// Clusters per bundle: as many as the device holds at once, evenly loaded.
+long long resident_stride(const NormParams &P, int threads, size_t smem, const gcb::DeviceFacts &f, int &occ) {
+    // 128 registers a thread allow 512 threads per SM
+    occ = static_cast<int>(std::min<size_t>(gcb::kResidentThreads / threads, f.smem_per_sm / (smem + 1024)));
+    occ = std::max(1, occ);
+    const long long most = std::max(1LL, static_cast<long long>(occ) * f.sms / (static_cast<long long>(P.bundles) * P.cluster));
+    return ceil_div(P.n, ceil_div(P.n, most));
+}
+
+// Estimated time in microseconds of a choice that is set in P.
+double resident_cost(const NormParams &P, int v, int threads, size_t smem, bool backward, const gcb::DeviceFacts &f) {
+    int occ = 1;
+    const long long stride = resident_stride(P, threads, smem, f, occ);
+    const double rounds = static_cast<double>(ceil_div(P.n, stride));
+    const double ctas = static_cast<double>(stride) * P.bundles * P.cluster;
+    const double esize = v == 4 ? 4 : 2;
+    const double bytes = (backward ? 3.0 : 2.0) * esize * P.n * P.px * P.c;
+    const double lanes = static_cast<double>(P.vr * P.lanes) / threads;
+    const double ragged = static_cast<double>(P.px) / (static_cast<double>(P.lanes) * P.iters * P.cluster);
+    const double run = P.cb * esize;
+    const double run_eff = run >= 128 ? 1.0 : run >= 64 ? 0.97 : run >= 32 ? 0.9 : 0.6;
+    const double gap = (backward ? 2.5 : 2.0) + (P.cluster > 1 ? 0.7 : 0.0) + (P.cluster > 8 ? 0.4 : 0.0);
+    const double rate = 6.0e6 * run_eff * std::min(1.0, ctas / f.sms) * (0.5 + 0.5 * lanes * ragged);  // bytes per us
+    return bytes / rate + gap * (1.0 + (rounds - 1.0) / occ);
+}
+
+std::mutex g_mutex;
+std::map<ResidentKey, ResidentPlan> g_resident;
+
+ResidentPlan choose_resident(const NormParams &base, int v, bool backward, bool bits, const gcb::DeviceFacts &f) {
+    ResidentPlan best;
+    double best_cost = 0.0;
+    const int unit = std::lcm(base.cpg, v);  // channels: whole groups and whole vectors
+    const int units = base.c / unit;
+    for (int m = 1; m <= units && static_cast<long long>(m) * unit / v <= gcb::kNormThreads; ++m) {
+        if (units % m) continue;
+        for (int cluster = 1; cluster <= 16; cluster *= 2)
+            for (int threads = 64; threads <= gcb::kResidentThreads; threads *= 2) {
+                NormParams P = base;
+                size_t smem = 0;
+                if (!set_resident(P, v, m * unit, cluster, threads, backward, bits, f.smem_optin, smem)) continue;
+                if (P.n * P.bundles * cluster > INT32_MAX) continue;
+                const double cost = resident_cost(P, v, threads, smem, backward, f);
+                if (!best.ok || cost < best_cost) {
+                    best_cost = cost;
+                    best.ok = true;
+                    best.cb = m * unit;
+                    best.threads = threads;
+                    best.cluster = cluster;
+                    best.smem = smem;
+                }
+            }
+    }
+    return best;
+}
+
+int plan_norm(NormParams &P, NormPlan &plan, bool backward) {
     int dev = -1;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
     gcb::DeviceFacts facts;
     const int st = gcb::device_facts(dev, facts);
     if (st != GC_OK) return st;
-    plan_split(P, plan.vec ? (plan.type == gcb::kElemF32 ? 4 : 8) : 1, facts.sms);
+    const int v = plan.vec ? (plan.type == gcb::kElemF32 ? 4 : 8) : 1;
+    if (plan.vec) {
+        // room for the decision bytes is planned for whether they are needed
+        // or not, so that a tensor's workspace does not depend on the dropout
+        const ResidentKey key{dev, plan.type, backward, 0, P.n, P.px, P.c, P.groups};
+        ResidentPlan r;
+        bool known = false;
+        {
+            std::lock_guard<std::mutex> lock(g_mutex);
+            const auto it = g_resident.find(key);
+            if (it != g_resident.end()) {
+                r = it->second;
+                known = true;
+            }
+        }
+        if (!known) {
+            r = choose_resident(P, v, backward, backward, facts);
+            std::lock_guard<std::mutex> lock(g_mutex);
+            g_resident[key] = r;
+        }
+        if (r.ok) {
+            set_resident(P, v, r.cb, r.cluster, r.threads, backward, backward, facts.smem_optin, plan.smem);
+            plan.resident = true;
+            plan.threads = r.threads;
+            int occ = 1;
+            P.stride = resident_stride(P, r.threads, plan.smem, facts, occ);
+            return GC_OK;
+        }
+    }
+    plan_split(P, v, facts.sms);
     return GC_OK;
 }
 
@@ -344,6 +479,54 @@ const void *norm_kernel(NormKernel k, const NormPlan &plan, int act) {
     if (plan.type == gcb::kElemF16) return norm_typed<__half>(k, plan.vec, act);
     if (plan.type == gcb::kElemBF16) return norm_typed<__nv_bfloat16>(k, plan.vec, act);
     return norm_typed<float>(k, plan.vec, act);
+}
+
+// The resident kernels with dropout choose the activation at run time.
+template <class T>
+const void *resident_typed(bool backward, int act, bool drop) {
+#define GCB_RESIDENT(ACT, DROP)                                                            \
+    (backward ? reinterpret_cast<const void *>(&gcb::norm_resident_grad_kernel<T, ACT, DROP>) \
+              : reinterpret_cast<const void *>(&gcb::norm_resident_kernel<T, ACT, DROP>))
+    if (drop) return GCB_RESIDENT(-1, true);
+    if (act == gcb::kActRelu) return GCB_RESIDENT(gcb::kActRelu, false);
+    if (act == gcb::kActRelu6) return GCB_RESIDENT(gcb::kActRelu6, false);
+    if (act == gcb::kActSilu) return GCB_RESIDENT(gcb::kActSilu, false);
+    return GCB_RESIDENT(gcb::kActNone, false);
+#undef GCB_RESIDENT
+}
+const void *resident_kernel(const NormPlan &plan, bool backward, int act, bool drop) {
+    if (plan.type == gcb::kElemF16) return resident_typed<__half>(backward, act, drop);
+    if (plan.type == gcb::kElemBF16) return resident_typed<__nv_bfloat16>(backward, act, drop);
+    return resident_typed<float>(backward, act, drop);
+}
+
+// Opts a kernel into the shared memory and the cluster sizes it may be
+// launched with, once per device.
+int prepare_resident(const void *fn, int dev, int smem_optin) {
+    static std::map<std::pair<int, const void *>, bool> done;
+    std::lock_guard<std::mutex> lock(g_mutex);
+    bool &flag = done[{dev, fn}];
+    if (flag) return GC_OK;
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_optin);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
+    }
+    flag = true;
+    return GC_OK;
+}
+
+int launch_resident(NormParams &P, const NormPlan &plan, bool backward, int dev, cudaStream_t s, cudaError_t &e) {
+    gcb::DeviceFacts facts;
+    int st = gcb::device_facts(dev, facts);
+    if (st != GC_OK) return st;
+    const void *fn = resident_kernel(plan, backward, P.act, P.drop.threshold != 0);
+    if ((st = prepare_resident(fn, dev, facts.smem_optin)) != GC_OK) return st;
+    void *args[] = {&P};
+    const unsigned grid = static_cast<unsigned>(static_cast<long long>(P.stride) * P.bundles * P.cluster);
+    e = gcb::launch_pdl(fn, dim3(grid), dim3(plan.threads), args, plan.smem, s, P.cluster);
+    return GC_OK;
 }
 
 unsigned grid_of(long long items) { return static_cast<unsigned>(std::min<long long>(items, INT32_MAX)); }
@@ -421,9 +604,9 @@ int gc_b200_group_norm_workspace(const gc_tensor *x, const gc_tensor *y, int64_t
     if (st != GC_OK) return st;
     *bytes = 0;
     if (empty(P)) return gc_error(GC_OK, "");
-    st = plan_norm(P, plan);
+    st = plan_norm(P, plan, false);
     if (st != GC_OK) return st;
-    *bytes = space_of(P, false).total();
+    *bytes = space_of(P, plan, false).total();
     return gc_error(GC_OK, "");
 }
 
@@ -452,8 +635,8 @@ int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
     st = check_call({x, y, gamma, beta, stats}, {drop.seed_ptr, drop.offset_ptr, drop.used}, x->device_index, stream,
                     dev);
     if (st != GC_OK) return st;
-    if ((st = plan_norm(P, plan)) != GC_OK) return st;
-    const NormSpace space = space_of(P, false);
+    if ((st = plan_norm(P, plan, false)) != GC_OK) return st;
+    const NormSpace space = space_of(P, plan, false);
     if ((st = check_workspace(workspace, workspace_bytes, space.total())) != GC_OK) return st;
     if (space.total() != 0 && (st = gcb::check_device_memory(workspace, x->device_index, dev)) != GC_OK) return st;
     P.x = v[0].data;
@@ -471,7 +654,15 @@ int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
     P.stats = reinterpret_cast<float2 *>(stats != nullptr ? static_cast<char *>(stats->data) : w);
     P.part = reinterpret_cast<float2 *>(w + space.stats);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    cudaError_t e = launch(norm_kernel(kMoments, plan, activation), P.items, P, s);
+    cudaError_t e = cudaSuccess;
+    if (plan.resident) {
+        if (stats == nullptr) P.stats = nullptr;
+        if ((st = launch_resident(P, plan, false, dev, s, e)) != GC_OK) return st;
+        gcb::record_plan(PlanRecord::kNorm, "resident", false, static_cast<long long>(P.stride) * P.bundles * P.cluster,
+                         plan.threads, plan.smem, P.cluster, P.cb, P.rows, 1, 1);
+        return launched(e);
+    }
+    e = launch(norm_kernel(kMoments, plan, activation), P.items, P, s);
     if (e == cudaSuccess)
         e = launch(reinterpret_cast<const void *>(&gcb::norm_finalize_kernel), P.n * P.groups, P, s);
     if (e == cudaSuccess) e = launch(norm_kernel(kApply, plan, activation), P.items, P, s);
@@ -490,9 +681,9 @@ int gc_b200_group_norm_backward_workspace(const gc_tensor *dy, const gc_tensor *
     if (st != GC_OK) return st;
     *bytes = 0;
     if (empty(P)) return gc_error(GC_OK, "");
-    st = plan_norm(P, plan);
+    st = plan_norm(P, plan, true);
     if (st != GC_OK) return st;
-    *bytes = space_of(P, true).total();
+    *bytes = space_of(P, plan, true).total();
     return gc_error(GC_OK, "");
 }
 
@@ -531,8 +722,8 @@ int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
             if (t != nullptr && e == cudaSuccess) e = cudaMemsetAsync(t->data, 0, range_of(t).bytes, s);
         return launched(e);
     }
-    if ((st = plan_norm(P, plan)) != GC_OK) return st;
-    const NormSpace space = space_of(P, true);
+    if ((st = plan_norm(P, plan, true)) != GC_OK) return st;
+    const NormSpace space = space_of(P, plan, true);
     if ((st = check_workspace(workspace, workspace_bytes, space.total())) != GC_OK) return st;
     if (space.total() != 0 && (st = gcb::check_device_memory(workspace, x->device_index, dev)) != GC_OK) return st;
     P.x = v[0].data;
@@ -558,13 +749,26 @@ int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
     P.part = reinterpret_cast<float2 *>(w);
     P.chan = reinterpret_cast<float2 *>(w + space.part);
     P.gsum = reinterpret_cast<float2 *>(w + space.part + space.chan);
-    cudaError_t e = launch(norm_kernel(kGradSums, plan, activation), P.items, P, s);
+    cudaError_t e = cudaSuccess;
+    const bool params = P.dgamma != nullptr || P.dbeta != nullptr;
+    const void *sums = reinterpret_cast<const void *>(&gcb::norm_grad_params_kernel);
+    if (plan.resident) {
+        if (!params) P.part = nullptr;
+        if ((st = launch_resident(P, plan, true, dev, s, e)) != GC_OK) return st;
+        P.chan = P.part;
+        P.sum_rows = static_cast<long long>(P.stride) * P.cluster;
+        if (e == cudaSuccess && params) e = launch(sums, ceil_div(P.c, 32), P, s);
+        gcb::record_plan(PlanRecord::kNorm, "resident_backward", false,
+                         static_cast<long long>(P.stride) * P.bundles * P.cluster, plan.threads, plan.smem, P.cluster,
+                         P.cb, P.rows, 1, params ? 2 : 1);
+        return launched(e);
+    }
+    P.sum_rows = P.n;
+    e = launch(norm_kernel(kGradSums, plan, activation), P.items, P, s);
     if (e == cudaSuccess)
         e = launch(reinterpret_cast<const void *>(&gcb::norm_grad_finalize_kernel), P.n * P.groups, P, s);
     if (e == cudaSuccess) e = launch(norm_kernel(kGradApply, plan, activation), P.items, P, s);
-    const bool params = P.dgamma != nullptr || P.dbeta != nullptr;
-    if (e == cudaSuccess && params)
-        e = launch(reinterpret_cast<const void *>(&gcb::norm_grad_params_kernel), ceil_div(P.c, 32), P, s);
+    if (e == cudaSuccess && params) e = launch(sums, ceil_div(P.c, 32), P, s);
     gcb::record_plan(PlanRecord::kNorm, "split_backward", false, P.items, gcb::kNormThreads, 0, 1, P.vb, P.chunk_rows,
                      plan.vec ? 1 : 0, params ? 4 : 3);
     return launched(e);

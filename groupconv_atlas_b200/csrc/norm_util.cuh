@@ -108,28 +108,142 @@ __device__ __forceinline__ void store_param(void *p, int type, long long i, floa
     else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// ---- activations --------------------------------------------------------------------
-// Comparisons are written so that a NaN passes through.
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// ---- pairs of floats ------------------------------------------------------------------
+// sm_100 adds and multiplies two floats in one instruction; the kernels are
+// bound by issue slots at 16-bit types, so their arithmetic runs on pairs.
+struct f2 {
+    uint64_t v;
+};
+__device__ __forceinline__ f2 pair(float a, float b) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ f2 pair(float a) { return pair(a, a); }
+__device__ __forceinline__ void split(f2 p, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v));
+}
+__device__ __forceinline__ f2 operator+(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ f2 operator*(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
 
+// A thread's V values as pairs; V = 1 leaves the second half unused (0).
+template <int V>
+struct Lanes {
+    static constexpr int kPairs = (V + 1) / 2;
+    f2 p[kPairs];
+};
+template <int V>
+__device__ __forceinline__ Lanes<V> lanes_of(const float (&v)[V]) {
+    Lanes<V> r;
+    if constexpr (V == 1) {
+        r.p[0] = pair(v[0], 0.0f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) r.p[i] = pair(v[2 * i], v[2 * i + 1]);
+    }
+    return r;
+}
+template <int V>
+__device__ __forceinline__ void values_of(const Lanes<V> &l, float (&v)[V]) {
+    if constexpr (V == 1) {
+        float unused;
+        split(l.p[0], v[0], unused);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) split(l.p[i], v[2 * i], v[2 * i + 1]);
+    }
+}
+template <class T, int V>
+__device__ __forceinline__ Lanes<V> load_lanes(const T *p) {
+    float v[V];
+    load_elems<T, V>(p, v);
+    return lanes_of<V>(v);
+}
+template <class T, int V>
+__device__ __forceinline__ Lanes<V> unpack_lanes(const uint4 &u, const T *tag) {
+    float v[V];
+    unpack(u, v, tag);
+    return lanes_of<V>(v);
+}
+template <class T, int V>
+__device__ __forceinline__ void store_lanes(T *p, const Lanes<V> &l) {
+    float v[V];
+    values_of<V>(l, v);
+    store_elems<T, V>(p, v);
+}
+// Kept values scaled, the others 0 whatever they hold.
+template <int V>
+__device__ __forceinline__ Lanes<V> keep_lanes(const Lanes<V> &l, uint32_t bits, float scale) {
+    float v[V];
+    values_of<V>(l, v);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = bits >> j & 1u ? v[j] * scale : 0.0f;
+    return lanes_of<V>(v);
+}
+
+// ---- activations --------------------------------------------------------------------
+// 1 / (1 + 2^(-z log2 e)) of two values with three of the special-function
+// unit's instructions instead of four (that unit, a sixteenth of an SM's issue
+// width, bounds the 16-bit kernels): one reciprocal serves both,
+// 1 / p = q / (p q).  The power is held at 2^62 so that p q stays finite; z
+// below -43 then gives 2^-62 where the exact value is smaller still.  The
+// approximate instructions are good to about 2^-22 relative each, and the
+// rounding of z log2 e moves the power by at most |z| 2^-24.
+__device__ __forceinline__ f2 sigmoid2(f2 z) {
+    float a, b, p, q, r;
+    split(z * pair(-1.4426950408889634f), a, b);
+    a = fminf(a, 62.0f);
+    b = fminf(b, 62.0f);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+    split(pair(a, b) + pair(1.0f), p, q);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(p * q));
+    return pair(q, p) * pair(r);
+}
+
+// Comparisons are written so that a NaN passes through.
+__device__ __forceinline__ float relu(float z) { return z < 0.0f ? 0.0f : z; }
+__device__ __forceinline__ float relu6(float z) { return z < 0.0f ? 0.0f : z > 6.0f ? 6.0f : z; }
+
+// ACT -1: the activation is `act`, known at run time.
 template <int ACT>
-__device__ __forceinline__ float activate(float z) {
-    if (ACT == kActRelu) return z < 0.0f ? 0.0f : z;
-    if (ACT == kActRelu6) return z < 0.0f ? 0.0f : z > 6.0f ? 6.0f : z;
-    if (ACT == kActSilu) return z * sigmoid(z);
-    return z;
+__device__ __forceinline__ f2 activate(int act, f2 z) {
+    if constexpr (ACT >= 0) act = ACT;
+    if (act == kActSilu) return z * sigmoid2(z);
+    if (act == kActNone) return z;
+    float a, b;
+    split(z, a, b);
+    return act == kActRelu ? pair(relu(a), relu(b)) : pair(relu6(a), relu6(b));
 }
 
 // g * act'(z)
 template <int ACT>
-__device__ __forceinline__ float activate_grad(float z, float g) {
-    if (ACT == kActRelu) return z <= 0.0f ? 0.0f : g;
-    if (ACT == kActRelu6) return z <= 0.0f || z >= 6.0f ? 0.0f : g;
-    if (ACT == kActSilu) {
-        const float s = sigmoid(z);
-        return g * (s * fmaf(z, 1.0f - s, 1.0f));
+__device__ __forceinline__ f2 activate_grad(int act, f2 z, f2 g) {
+    if constexpr (ACT >= 0) act = ACT;
+    if (act == kActSilu) {
+        const f2 s = sigmoid2(z);
+        return g * (s * fma2(z, fma2(s, pair(-1.0f), pair(1.0f)), pair(1.0f)));
     }
-    return g;
+    if (act == kActNone) return g;
+    float a, b, ga, gb;
+    split(z, a, b);
+    split(g, ga, gb);
+    const float top = act == kActRelu6 ? 6.0f : __int_as_float(0x7f800000);
+    const bool open = act == kActRelu6;
+    return pair(a <= 0.0f || (open && a >= top) ? 0.0f : ga, b <= 0.0f || (open && b >= top) ? 0.0f : gb);
 }
 
 // ---- dropout ------------------------------------------------------------------------
