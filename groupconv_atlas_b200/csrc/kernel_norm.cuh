@@ -31,7 +31,6 @@ namespace gcb {
 
 constexpr int kNormThreads = 256;      // split path
 constexpr int kResidentThreads = 512;  // resident path, at most
-constexpr int kNormRun = 64;  // pixels of a thread that share a pivot (below)
 
 struct NormParams {
     const void *x, *dy;
@@ -72,32 +71,6 @@ struct NormParams {
     DropParams drop;
 };
 
-struct NormItem {
-    long long n, p0, p1;  // image, first and one-past-last pixel
-    int chunk, vcol;
-};
-
-__device__ __forceinline__ NormItem norm_item(const NormParams &P, long long item, int col) {
-    NormItem it;
-    const int cb = static_cast<int>(item % P.cblocks);
-    const long long t = item / P.cblocks;
-    it.chunk = static_cast<int>(t % P.chunks);
-    it.n = t / P.chunks;
-    it.vcol = cb * P.vb + col;
-    it.p0 = it.chunk * P.chunk_rows;
-    it.p1 = min(P.px, it.p0 + P.chunk_rows);
-    return it;
-}
-
-// (count, mean, sum of squares about the mean) of two disjoint sets joined.
-__device__ __forceinline__ void join_moments(float &n, float &mean, float &m2, float nb, float mb, float m2b) {
-    if (nb == 0.0f) return;
-    const float total = n + nb, f = nb / total, d = mb - mean;
-    mean = fmaf(d, f, mean);
-    m2 += m2b + d * d * (n * f);
-    n = total;
-}
-
 // The per-channel values of a thread, as pairs.
 template <int V>
 struct Coefs {
@@ -124,118 +97,372 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
     return v;
 }
 
-// ---- split path, forward ---------------------------------------------------------------
-// Moments of one chunk per channel.  A thread sums x - pivot and its square
-// over runs of at most 64 of its pixels, the pivot being the run's first
-// value: it is one of the values, so the squares about it exceed the squares
-// about the mean at most by the run's length, and the cancellation in
-// sum d^2 - (sum d)^2 / n costs at most 64 rounding errors whatever the data's
-// mean.  Runs, pixel lanes and chunks are joined as (count, mean, squares).
-template <class T, int V>
-__global__ void __launch_bounds__(kNormThreads) norm_moments_kernel(const __grid_constant__ NormParams P) {
-    __shared__ float2 sm[kNormThreads * V];
-    __shared__ float cnt[kNormThreads];
-    griddep_wait();
-    griddep_launch_dependents();
-    const int tid = threadIdx.x, lane = tid / P.vb, col = tid - lane * P.vb;
-    int half = 1;
-    while (half * 2 < P.lanes) half *= 2;
-    for (long long item = blockIdx.x; item < P.items; item += gridDim.x) {
-        const NormItem it = norm_item(P, item, col);
-        const bool active = lane < P.lanes && it.vcol < P.vcols;
-        float mean[V], m2[V], n = 0.0f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) mean[j] = m2[j] = 0.0f;
-        if (active) {
-            const T *x = static_cast<const T *>(P.x) + it.n * P.x_ldn + static_cast<long long>(it.vcol) * V;
-            const long long step = static_cast<long long>(P.lanes) * kNormRun;
-            for (long long base = it.p0 + lane; base < it.p1; base += step) {
-                const long long end = min(it.p1, base + step);
-                float piv[V], s[V], q[V];
-                load_elems<T, V>(x + base * P.x_ldp, piv);
-#pragma unroll
-                for (int j = 0; j < V; ++j) s[j] = q[j] = 0.0f;
-                float k = 1.0f;
-#pragma unroll 4
-                for (long long p = base + P.lanes; p < end; p += P.lanes) {
-                    float v[V];
-                    load_elems<T, V>(x + p * P.x_ldp, v);
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        const float d = v[j] - piv[j];
-                        s[j] += d;
-                        q[j] = fmaf(d, d, q[j]);
-                    }
-                    k += 1.0f;
-                }
-                const float inv = 1.0f / k;
-                const float before = n;
+// ---- sums of a block ---------------------------------------------------------------------
+// Where a thread (lane, col) holds a value pair for each of its V channels:
+// rows of channel pairs that meet in shared memory, one a warp where a warp
+// holds whole pixel lanes (they are added by shuffles first), else one a lane.
+__host__ __device__ inline int sum_rows_of(int threads, int vr, int lanes) { return 32 % vr == 0 ? threads / 32 : lanes; }
+// Entries of shared memory that channel_sums needs for a block of cb channels.
+__host__ __device__ inline size_t channel_sums_space(int threads, int vr, int lanes, int cb) {
+    return static_cast<size_t>(sum_rows_of(threads, vr, lanes)) * cb + threads;
+}
+
+// Adds s and t over the block's pixel lanes and calls f(c, sums) once for each
+// channel c of the block, from some thread.  `scratch` may be reused after the
+// next barrier.
+template <int V, class F>
+__device__ __forceinline__ void channel_sums(int vr, int lanes, int cb, int at, int local, float (&s)[V], float (&t)[V],
+                                             float2 *scratch, F f) {
+    const int threads = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const bool warp_rows = 32 % vr == 0;
+    const int rows = sum_rows_of(threads, vr, lanes), segs = threads / cb;
+    float2 *segsum = scratch, *red = scratch + threads;
+    if (at < lanes) {
+        if (warp_rows)  // every lane of the block takes part: 32 is a multiple of vr
+            for (int o = vr; o < 32; o <<= 1) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    float nj = before;
-                    join_moments(nj, mean[j], m2[j], k, fmaf(s[j], inv, piv[j]), fmaxf(0.0f, fmaf(-s[j] * inv, s[j], q[j])));
-                    if (j == V - 1) n = nj;
+                    s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
+                    t[j] += __shfl_xor_sync(0xffffffffu, t[j], o);
                 }
             }
-        }
-        __syncthreads();  // the previous item's values are no longer read
-        if (lane < P.lanes) {
-            if (col == 0) cnt[lane] = n;
+        if (!warp_rows || lane < vr) {
+            float2 *out = red + (warp_rows ? warp : at) * cb + local;
 #pragma unroll
-            for (int j = 0; j < V; ++j) sm[tid * V + j] = make_float2(mean[j], m2[j]);
+            for (int j = 0; j < V; ++j) out[j] = make_float2(s[j], t[j]);
         }
-        for (int h = half; h > 0; h >>= 1) {
-            __syncthreads();
-            float nb = 0.0f;
-            if (lane < h && lane + h < P.lanes) {
-                n = cnt[lane];
-                nb = cnt[lane + h];
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float2 b = sm[(tid + h * P.vb) * V + j];
-                    float nj = n;
-                    join_moments(nj, mean[j], m2[j], nb, b.x, b.y);
-                    sm[tid * V + j] = make_float2(mean[j], m2[j]);
-                }
+    }
+    __syncthreads();
+    if (segs > 1) {
+        const int seg = tid / cb, c = tid - seg * cb;
+        float2 sum = make_float2(0.0f, 0.0f);
+        if (seg < segs) {
+            for (int l = seg; l < rows; l += segs) {
+                const float2 v = red[l * cb + c];
+                sum.x += v.x;
+                sum.y += v.y;
             }
-            __syncthreads();
-            if (lane < h && lane + h < P.lanes && col == 0) cnt[lane] = n + nb;
+            segsum[tid] = sum;
         }
-        if (lane == 0 && it.vcol < P.vcols) {
-            float2 *out = P.part + (it.n * P.chunks + it.chunk) * P.c + static_cast<long long>(it.vcol) * V;
-#pragma unroll
-            for (int j = 0; j < V; ++j) out[j] = make_float2(mean[j], m2[j]);
+        __syncthreads();
+    }
+    const float2 *parts = segs > 1 ? segsum : red;
+    const int count = segs > 1 ? min(segs, rows) : rows;
+    for (int c = tid; c < cb; c += threads) {
+        float2 sum = make_float2(0.0f, 0.0f);
+        for (int i = 0; i < count; ++i) {
+            const float2 v = parts[i * cb + c];
+            sum.x += v.x;
+            sum.y += v.y;
         }
+        f(c, sum);
     }
 }
 
-// Joins a group's chunks and channels: one block per (image, group).
+// ---- split path ----------------------------------------------------------------------------
+// A block streams a chunk of pixels of up to 256 vector columns.  16-byte
+// vectors go through a ring in shared memory that is private to each thread
+// (kRing copies in flight, no barrier); single elements are loaded kAhead at a
+// time.
+constexpr int kRing = 16, kAhead = 8;
+__device__ __forceinline__ void copy_vector(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// Raw elements as loaded: 16 bytes, or one element.
+template <class T, int V>
+struct Raw {
+    uint4 u;
+};
+template <class T>
+struct Raw<T, 1> {
+    T u;
+};
+template <class T, int V>
+__device__ __forceinline__ Raw<T, V> load_raw(const T *p) {
+    Raw<T, V> r;
+    if constexpr (V == 1) r.u = *p;
+    else r.u = __ldg(reinterpret_cast<const uint4 *>(p));
+    return r;
+}
+template <class T, int V>
+__device__ __forceinline__ Lanes<V> lanes_of_raw(const Raw<T, V> &r) {
+    float v[V];
+    if constexpr (V == 1) v[0] = to_float(r.u);
+    else unpack(r.u, v, static_cast<const T *>(nullptr));
+    return lanes_of<V>(v);
+}
+
+struct SplitPlace {
+    long long n, p0;  // image, first pixel of the thread
+    int chunk, lane, col, count;  // count: vectors of this thread
+    int c0;                       // first channel of the thread, 0 where it has none
+    int width;                    // channels of this block
+    int first;                    // first channel of this block
+};
+__device__ __forceinline__ SplitPlace split_place(const NormParams &P, int v) {
+    SplitPlace s;
+    const unsigned item = blockIdx.x;
+    const unsigned cb = item % P.cblocks, t = item / P.cblocks;
+    s.chunk = t % P.chunks;
+    s.n = t / P.chunks;
+    s.lane = threadIdx.x / P.vb;
+    s.col = threadIdx.x - s.lane * P.vb;
+    const int columns = min(P.vb, P.vcols - static_cast<int>(cb) * P.vb);
+    s.first = static_cast<int>(cb) * P.vb * v;
+    s.width = columns * v;
+    const bool active = s.lane < P.lanes && s.col < columns;
+    const long long p0 = s.chunk * P.chunk_rows, p1 = min(P.px, p0 + P.chunk_rows);
+    s.p0 = p0 + s.lane;
+    s.count = active && s.p0 < p1 ? static_cast<int>((p1 - s.p0 + P.lanes - 1) / P.lanes) : 0;
+    s.c0 = active ? s.first + s.col * v : 0;
+    return s;
+}
+
+// Calls f(k, vector) for a thread's vectors.  ring: kRing * kNormThreads
+// vectors of shared memory (V > 1).
+template <class T, int V, class F>
+__device__ __forceinline__ void for_vectors(uint4 *ring, const T *p, long long step, int count, F f) {
+    if constexpr (V == 1) {
+        for (int k = 0; k < count; k += kAhead) {
+            Raw<T, V> raw[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u, p += step)
+                if (k + u < count) raw[u] = load_raw<T, V>(p);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (k + u < count) f(k + u, lanes_of_raw<T, V>(raw[u]));
+        }
+    } else {
+        const uint4 *mine = ring + threadIdx.x;
+        const uint32_t addr = smem_addr(mine);
+        constexpr uint32_t kPitch = kNormThreads * sizeof(uint4);
+#pragma unroll
+        for (int u = 0; u < kRing; ++u, p += step) {
+            if (u < count) copy_vector(addr + u * kPitch, p);
+            cp_async_commit();
+        }
+#pragma unroll 4
+        for (int k = 0; k < count; ++k, p += step) {
+            const int slot = k % kRing;
+            cp_async_wait<kRing - 1>();
+            const Lanes<V> v = unpack_lanes<T, V>(mine[slot * kNormThreads], p);
+            if (k + kRing < count) copy_vector(addr + slot * kPitch, p);
+            cp_async_commit();
+            f(k, v);
+        }
+    }
+}
+// The same for two tensors: f(k, vector of p, vector of q).
+template <class T, int V, class F>
+__device__ __forceinline__ void for_vector_pairs(uint4 *ring, const T *p, long long pstep, const T *q, long long qstep,
+                                                 int count, F f) {
+    if constexpr (V == 1) {
+        constexpr int kPair = kAhead / 2;
+        for (int k = 0; k < count; k += kPair) {
+            Raw<T, V> a[kPair], b[kPair];
+#pragma unroll
+            for (int u = 0; u < kPair; ++u, p += pstep, q += qstep)
+                if (k + u < count) {
+                    a[u] = load_raw<T, V>(p);
+                    b[u] = load_raw<T, V>(q);
+                }
+#pragma unroll
+            for (int u = 0; u < kPair; ++u)
+                if (k + u < count) f(k + u, lanes_of_raw<T, V>(a[u]), lanes_of_raw<T, V>(b[u]));
+        }
+    } else {
+        constexpr int kHalf = kRing / 2;
+        const uint4 *mine = ring + threadIdx.x;
+        const uint32_t addr = smem_addr(mine);
+        constexpr uint32_t kPitch = kNormThreads * sizeof(uint4);
+#pragma unroll
+        for (int u = 0; u < kHalf; ++u, p += pstep, q += qstep) {
+            if (u < count) {
+                copy_vector(addr + 2 * u * kPitch, p);
+                copy_vector(addr + (2 * u + 1) * kPitch, q);
+            }
+            cp_async_commit();
+        }
+#pragma unroll 2
+        for (int k = 0; k < count; ++k, p += pstep, q += qstep) {
+            const int slot = 2 * (k % kHalf);
+            cp_async_wait<kHalf - 1>();
+            const Lanes<V> v = unpack_lanes<T, V>(mine[slot * kNormThreads], p);
+            const Lanes<V> g = unpack_lanes<T, V>(mine[(slot + 1) * kNormThreads], p);
+            if (k + kHalf < count) {
+                copy_vector(addr + slot * kPitch, p);
+                copy_vector(addr + (slot + 1) * kPitch, q);
+            }
+            cp_async_commit();
+            f(k, v, g);
+        }
+    }
+}
+// Bytes of the ring.
+__host__ __device__ inline size_t ring_space(int v) { return v == 1 ? 0 : kRing * kNormThreads * sizeof(uint4); }
+
+// Moments of a thread's values of one channel each: sums about a pivot, which
+// is the first of at most 64 values.  As one of the values it lies so near the
+// mean that the squares about it exceed those about the mean at most by the
+// factor 64; cancellation in q - s^2 / n costs no more than that many roundings
+// whatever the data's mean.  Runs of 64 are joined as (mean, squares).
+constexpr int kNormRun = 64;
+template <int V>
+struct Moments {
+    Lanes<V> minus, s, q;
+    float mean[V], m2[V], n = 0.0f;
+    __device__ __forceinline__ void start(const Lanes<V> &v) {
+#pragma unroll
+        for (int i = 0; i < Lanes<V>::kPairs; ++i) {
+            minus.p[i] = v.p[i] * pair(-1.0f);
+            s.p[i] = q.p[i] = pair(0.0f);
+        }
+    }
+    __device__ __forceinline__ void add(const Lanes<V> &v) {
+#pragma unroll
+        for (int i = 0; i < Lanes<V>::kPairs; ++i) {
+            const f2 d = v.p[i] + minus.p[i];
+            s.p[i] = s.p[i] + d;
+            q.p[i] = fma2(d, d, q.p[i]);
+        }
+    }
+    // The run's count values become part of (n, mean, m2).
+    __device__ __forceinline__ void finish(int count) {
+        float first[V], sv[V], qv[V];
+        values_of<V>(minus, first);
+        values_of<V>(s, sv);
+        values_of<V>(q, qv);
+        const float k = static_cast<float>(count), inv = 1.0f / k, total = n + k, f = k / total;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float run = fmaf(sv[j], inv, -first[j]);
+            float squares = fmaf(-sv[j] * inv, sv[j], qv[j]);
+            squares = squares < 0.0f ? 0.0f : squares;  // a NaN stays
+            if (n == 0.0f) {
+                mean[j] = run;
+                m2[j] = squares;
+            } else {
+                const float d = run - mean[j];
+                mean[j] = fmaf(d, f, mean[j]);
+                m2[j] += squares + d * d * (n * f);
+            }
+        }
+        n = total;
+    }
+};
+
+// Per chunk and channel: mean and squares about it.  The threads' moments are
+// moved to one pivot per channel, the mean of pixel lane 0, and then add up.
+template <class T, int V>
+__global__ void __launch_bounds__(kNormThreads, 3) norm_moments_kernel(const __grid_constant__ NormParams P) {
+    extern __shared__ __align__(16) unsigned char nsm[];
+    uint4 *ring = reinterpret_cast<uint4 *>(nsm);
+    float *pivot = reinterpret_cast<float *>(nsm + ring_space(V));  // [width]
+    float2 *scratch = reinterpret_cast<float2 *>(pivot + (P.vb * V + 1) / 2 * 2);
+    griddep_wait();
+    griddep_launch_dependents();
+    const SplitPlace at = split_place(P, V);
+    Moments<V> m;
+#pragma unroll
+    for (int j = 0; j < V; ++j) m.mean[j] = m.m2[j] = 0.0f;
+    const T *x = static_cast<const T *>(P.x) + at.n * P.x_ldn + at.p0 * P.x_ldp + at.c0;
+    const long long step = static_cast<long long>(P.lanes) * P.x_ldp;
+    for_vectors<T, V>(ring, x, step, at.count, [&](int i, const Lanes<V> &v) {
+        if (i % kNormRun == 0) {
+            if (i > 0) m.finish(kNormRun);
+            m.start(v);
+        }
+        m.add(v);
+    });
+    if (at.count > 0) m.finish((at.count - 1) % kNormRun + 1);
+    const int local = at.c0 - at.first;
+    if (at.lane == 0 && at.count > 0) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) pivot[local + j] = m.mean[j];
+    }
+    __syncthreads();
+    const bool any = at.count > 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float e = any ? m.mean[j] - pivot[local + j] : 0.0f, ne = m.n * e;
+        m.mean[j] = ne;
+        m.m2[j] = any ? fmaf(ne, e, m.m2[j]) : 0.0f;
+    }
+    float2 *out = P.part + (at.n * P.chunks + at.chunk) * P.c + at.first;
+    const float rows = static_cast<float>(min(P.chunk_rows, P.px - at.chunk * P.chunk_rows));
+    channel_sums<V>(P.vb, P.lanes, P.vb * V, at.lane, at.lane < P.lanes ? at.col * V : 0, m.mean, m.m2, scratch, [&](int c, float2 sum) {
+        const float d = sum.x / rows;
+        if (c < at.width) out[c] = make_float2(pivot[c] + d, fmaf(-d, sum.x, sum.y));
+    });
+}
+
+// Joins a group's chunks and channels: a team of TEAM threads (a warp, or the
+// block) per (image, group).
+template <int TEAM>
+__device__ __forceinline__ float team_sum(float v, float *red) {
+    if constexpr (TEAM == 32) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    } else {
+        return block_sum(v, red);
+    }
+}
+
+template <int TEAM>
 __global__ void __launch_bounds__(kNormThreads) norm_finalize_kernel(const __grid_constant__ NormParams P) {
+    constexpr int kHeld = 8;  // entries a thread holds on to for the second pass
     __shared__ float red[32];
     griddep_wait();
     griddep_launch_dependents();
     const float total = static_cast<float>(P.px) * static_cast<float>(P.cpg);
-    const long long entries = static_cast<long long>(P.chunks) * P.cpg;
-    for (long long ng = blockIdx.x; ng < P.n * P.groups; ng += gridDim.x) {
+    const unsigned entries = static_cast<unsigned>(P.chunks) * P.cpg;
+    const int me = threadIdx.x % TEAM;
+    const long long teams = static_cast<long long>(gridDim.x) * (kNormThreads / TEAM);
+    for (long long ng = (static_cast<long long>(blockIdx.x) * kNormThreads + threadIdx.x) / TEAM; ng < P.n * P.groups;
+         ng += teams) {
         const long long n = ng / P.groups;
         const float2 *part = P.part + n * P.chunks * P.c + (ng - n * P.groups) * P.cpg;
-        float s = 0.0f;
-        for (long long i = threadIdx.x; i < entries; i += kNormThreads) {
-            const long long k = i / P.cpg;
-            const float rows = static_cast<float>(min(P.chunk_rows, P.px - k * P.chunk_rows));
-            s = fmaf(rows, part[k * P.c + (i - k * P.cpg)].x, s);
+        auto entry = [&](unsigned i, float &rows) {
+            const unsigned chunk = i / P.cpg;
+            rows = static_cast<float>(min(P.chunk_rows, P.px - chunk * P.chunk_rows));
+            return part[static_cast<long long>(chunk) * P.c + (i - chunk * P.cpg)];
+        };
+        float2 held[kHeld];
+        float held_rows[kHeld], s = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) {
+            const unsigned i = me + u * TEAM;
+            held[u] = make_float2(0.0f, 0.0f);
+            held_rows[u] = 0.0f;
+            if (i < entries) held[u] = entry(i, held_rows[u]);
         }
-        const float mean = block_sum(s, red) / total;
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) s = fmaf(held_rows[u], held[u].x, s);
+        const unsigned rest = me + kHeld * TEAM;
+#pragma unroll 4
+        for (unsigned i = rest; i < entries; i += TEAM) {
+            float rows;
+            const float2 v = entry(i, rows);
+            s = fmaf(rows, v.x, s);
+        }
+        const float mean = team_sum<TEAM>(s, red) / total;
         float q = 0.0f;
-        for (long long i = threadIdx.x; i < entries; i += kNormThreads) {
-            const long long k = i / P.cpg;
-            const float rows = static_cast<float>(min(P.chunk_rows, P.px - k * P.chunk_rows));
-            const float2 v = part[k * P.c + (i - k * P.cpg)];
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) {
+            const float d = held[u].x - mean;
+            if (held_rows[u] > 0.0f) q += fmaf(held_rows[u] * d, d, held[u].y);
+        }
+#pragma unroll 4
+        for (unsigned i = rest; i < entries; i += TEAM) {
+            float rows;
+            const float2 v = entry(i, rows);
             const float d = v.x - mean;
             q += fmaf(rows * d, d, v.y);
         }
-        const float var = block_sum(q, red) / total;
-        if (threadIdx.x == 0) P.stats[ng] = make_float2(mean, 1.0f / sqrtf(var + P.eps));
+        const float var = team_sum<TEAM>(q, red) / total;
+        if (me == 0) P.stats[ng] = make_float2(mean, 1.0f / sqrtf(var + P.eps));
     }
 }
 
@@ -252,39 +479,50 @@ __device__ __forceinline__ Coefs<V> split_coefs(const NormParams &P, long long n
     return {lanes_of<V>(mean), lanes_of<V>(a), lanes_of<V>(b)};
 }
 
+// Dropout decisions of a thread's vectors, pixel by pixel.
+template <int V, bool DROP>
+struct Keeper {
+    DropState ds;
+    uint32_t keep = ~0u;
+    uint64_t at, step;
+    __device__ __forceinline__ Keeper(const NormParams &P, bool writer, long long n, long long p0, int c0, int lanes) {
+        if (!DROP) return;
+        ds = drop_state(P.drop, writer);
+        at = (static_cast<uint64_t>(n) * P.px + p0) * P.c + c0;
+        step = static_cast<uint64_t>(lanes) * P.c;
+        if (P.drop.channel) keep = keep_bits<V>(P.drop, ds, static_cast<uint64_t>(n) * P.c + c0);
+    }
+    __device__ __forceinline__ Lanes<V> apply(const NormParams &P, const Lanes<V> &v) {
+        if (!DROP) return v;
+        if (!P.drop.channel) keep = keep_bits<V>(P.drop, ds, at);
+        at += step;
+        return keep_lanes<V>(v, keep, P.drop.scale);
+    }
+};
+
 // Normalises, activates and drops out: the second pass over x.
-template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(const __grid_constant__ NormParams P) {
+template <class T, int V, int ACT, bool DROP>
+__global__ void __launch_bounds__(kNormThreads, 3) norm_apply_kernel(const __grid_constant__ NormParams P) {
+    extern __shared__ __align__(16) unsigned char nsm[];
+    uint4 *ring = reinterpret_cast<uint4 *>(nsm);
     griddep_wait();
     griddep_launch_dependents();
-    const int tid = threadIdx.x, lane = tid / P.vb, col = tid - lane * P.vb;
-    DropState ds{};
-    if (P.drop.threshold) ds = drop_state(P.drop, blockIdx.x == 0 && tid == 0);
-    for (long long item = blockIdx.x; item < P.items; item += gridDim.x) {
-        const NormItem it = norm_item(P, item, col);
-        if (lane >= P.lanes || it.vcol >= P.vcols) continue;
-        const int c0 = it.vcol * V;
-        const Coefs<V> coefs = split_coefs<V>(P, it.n, c0);
-        uint32_t keep = ~0u;
-        if (P.drop.threshold && P.drop.channel) keep = keep_bits<V>(P.drop, ds, static_cast<uint64_t>(it.n) * P.c + c0);
-        const T *x = static_cast<const T *>(P.x) + it.n * P.x_ldn + c0;
-        T *y = static_cast<T *>(P.y) + it.n * P.y_ldn + c0;
-#pragma unroll 2
-        for (long long p = it.p0 + lane; p < it.p1; p += P.lanes) {
-            Lanes<V> v = load_lanes<T, V>(x + p * P.x_ldp);
+    const SplitPlace at = split_place(P, V);
+    Keeper<V, DROP> drop(P, blockIdx.x == 0 && threadIdx.x == 0, at.n, at.p0, at.c0, P.lanes);
+    if (at.count == 0) return;
+    const Coefs<V> coefs = split_coefs<V>(P, at.n, at.c0);
+    const T *x = static_cast<const T *>(P.x) + at.n * P.x_ldn + at.p0 * P.x_ldp + at.c0;
+    T *y = static_cast<T *>(P.y) + at.n * P.y_ldn + at.p0 * P.y_ldp + at.c0;
+    const long long ystep = static_cast<long long>(P.lanes) * P.y_ldp;
+    for_vectors<T, V>(ring, x, static_cast<long long>(P.lanes) * P.x_ldp, at.count, [&](int, Lanes<V> v) {
 #pragma unroll
-            for (int i = 0; i < Lanes<V>::kPairs; ++i) {
-                f2 d;
-                v.p[i] = activate<ACT>(P.act, normalise<V>(coefs, i, v.p[i], d));
-            }
-            if (P.drop.threshold) {
-                if (!P.drop.channel)
-                    keep = keep_bits<V>(P.drop, ds, (static_cast<uint64_t>(it.n) * P.px + p) * P.c + c0);
-                v = keep_lanes<V>(v, keep, P.drop.scale);
-            }
-            store_lanes<T, V>(y + p * P.y_ldp, v);
+        for (int i = 0; i < Lanes<V>::kPairs; ++i) {
+            f2 d;
+            v.p[i] = activate<ACT>(P.act, normalise<V>(coefs, i, v.p[i], d));
         }
-    }
+        store_lanes<T, V>(y, drop.apply(P, v));
+        y += ystep;
+    });
 }
 
 // ---- split path, gradient ----------------------------------------------------------------
@@ -316,147 +554,117 @@ __device__ __forceinline__ Lanes<V> grad_result(int act, const Coefs<V> &k, cons
 }
 
 // Per chunk and channel: sum dz, sum dz (x - mean).
-template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_grad_sums_kernel(const __grid_constant__ NormParams P) {
-    __shared__ float2 sm[kNormThreads * V];
+template <class T, int V, int ACT, bool DROP>
+__global__ void __launch_bounds__(kNormThreads, 2) norm_grad_sums_kernel(const __grid_constant__ NormParams P) {
+    extern __shared__ __align__(16) unsigned char nsm[];
     griddep_wait();
     griddep_launch_dependents();
-    const int tid = threadIdx.x, lane = tid / P.vb, col = tid - lane * P.vb;
-    DropState ds{};
-    if (P.drop.threshold) ds = drop_state(P.drop, false);
-    int half = 1;
-    while (half * 2 < P.lanes) half *= 2;
-    for (long long item = blockIdx.x; item < P.items; item += gridDim.x) {
-        const NormItem it = norm_item(P, item, col);
-        float s[V], t[V];
+    const SplitPlace at = split_place(P, V);
+    uint4 *ring = reinterpret_cast<uint4 *>(nsm);
+    Keeper<V, DROP> drop(P, false, at.n, at.p0, at.c0, P.lanes);
+    const Coefs<V> coefs = split_coefs<V>(P, at.n, at.c0);
+    Lanes<V> s2, t2;
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = t[j] = 0.0f;
-        if (lane < P.lanes && it.vcol < P.vcols) {
-            const int c0 = it.vcol * V;
-            const Coefs<V> coefs = split_coefs<V>(P, it.n, c0);
-            Lanes<V> s2, t2;
-#pragma unroll
-            for (int i = 0; i < Lanes<V>::kPairs; ++i) s2.p[i] = t2.p[i] = pair(0.0f);
-            uint32_t keep = ~0u;
-            if (P.drop.threshold && P.drop.channel)
-                keep = keep_bits<V>(P.drop, ds, static_cast<uint64_t>(it.n) * P.c + c0);
-            const T *x = static_cast<const T *>(P.x) + it.n * P.x_ldn + c0;
-            const T *dy = static_cast<const T *>(P.dy) + it.n * P.dy_ldn + c0;
-#pragma unroll 2
-            for (long long p = it.p0 + lane; p < it.p1; p += P.lanes) {
-                const Lanes<V> v = load_lanes<T, V>(x + p * P.x_ldp);
-                Lanes<V> g = load_lanes<T, V>(dy + p * P.dy_ldp);
-                if (P.drop.threshold) {
-                    if (!P.drop.channel)
-                        keep = keep_bits<V>(P.drop, ds, (static_cast<uint64_t>(it.n) * P.px + p) * P.c + c0);
-                    g = keep_lanes<V>(g, keep, P.drop.scale);
-                }
-                grad_sums<V, ACT>(P.act, coefs, v, g, s2, t2);
-            }
-            values_of<V>(s2, s);
-            values_of<V>(t2, t);
-        }
-        __syncthreads();
-        if (lane < P.lanes) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) sm[tid * V + j] = make_float2(s[j], t[j]);
-        }
-        for (int h = half; h > 0; h >>= 1) {
-            __syncthreads();
-            if (lane < h && lane + h < P.lanes) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float2 o = sm[(tid + h * P.vb) * V + j];
-                    s[j] += o.x;
-                    t[j] += o.y;
-                    sm[tid * V + j] = make_float2(s[j], t[j]);
-                }
-            }
-        }
-        if (lane == 0 && it.vcol < P.vcols) {
-            float2 *out = P.part + (it.n * P.chunks + it.chunk) * P.c + static_cast<long long>(it.vcol) * V;
-#pragma unroll
-            for (int j = 0; j < V; ++j) out[j] = make_float2(s[j], t[j]);
-        }
-    }
+    for (int i = 0; i < Lanes<V>::kPairs; ++i) s2.p[i] = t2.p[i] = pair(0.0f);
+    const T *x = static_cast<const T *>(P.x) + at.n * P.x_ldn + at.p0 * P.x_ldp + at.c0;
+    const T *dy = static_cast<const T *>(P.dy) + at.n * P.dy_ldn + at.p0 * P.dy_ldp + at.c0;
+    for_vector_pairs<T, V>(ring, x, static_cast<long long>(P.lanes) * P.x_ldp, dy, static_cast<long long>(P.lanes) * P.dy_ldp,
+                           at.count, [&](int, const Lanes<V> &v, const Lanes<V> &g) {
+                               grad_sums<V, ACT>(P.act, coefs, v, drop.apply(P, g), s2, t2);
+                           });
+    float s[V], t[V];
+    values_of<V>(s2, s);
+    values_of<V>(t2, t);
+    float2 *out = P.part + (at.n * P.chunks + at.chunk) * P.c + at.first;
+    channel_sums<V>(P.vb, P.lanes, P.vb * V, at.lane, at.lane < P.lanes ? at.col * V : 0, s, t,
+                    reinterpret_cast<float2 *>(nsm + ring_space(V)), [&](int c, float2 sum) {
+                        if (c < at.width) out[c] = sum;
+                    });
 }
 
-// Per (image, group): the channels' sums over all chunks, and the group's k1, k2.
+// Per (image, channel): the sums over all chunks; then per group k1 and k2.  A
+// team per group: channel by channel, its lanes over the chunks.
+template <int TEAM>
 __global__ void __launch_bounds__(kNormThreads) norm_grad_finalize_kernel(const __grid_constant__ NormParams P) {
     __shared__ float red[32];
     griddep_wait();
     griddep_launch_dependents();
     const float total = static_cast<float>(P.px) * static_cast<float>(P.cpg);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    for (long long ng = blockIdx.x; ng < P.n * P.groups; ng += gridDim.x) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x % TEAM / 32;
+    const long long teams = static_cast<long long>(gridDim.x) * (kNormThreads / TEAM);
+    for (long long ng = (static_cast<long long>(blockIdx.x) * kNormThreads + threadIdx.x) / TEAM; ng < P.n * P.groups;
+         ng += teams) {
         const long long n = ng / P.groups;
         const int c0 = static_cast<int>(ng - n * P.groups) * P.cpg;
         const float2 st = P.stats[ng];
         float s1 = 0.0f, s2 = 0.0f;
-        for (int k = warp; k < P.cpg; k += warps) {
+        // four channels at a time, so that their loads are in flight together
+        for (int k = 4 * warp; k < P.cpg; k += 4 * (TEAM / 32)) {
             const float2 *part = P.part + n * P.chunks * P.c + c0 + k;
-            float s = 0.0f, t = 0.0f;
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
             for (int i = lane; i < P.chunks; i += 32) {
-                const float2 v = part[static_cast<long long>(i) * P.c];
-                s += v.x;
-                t += v.y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (k + j < P.cpg) {
+                        const float2 v = part[static_cast<long long>(i) * P.c + j];
+                        s[j] += v.x;
+                        t[j] += v.y;
+                    }
             }
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                s += __shfl_xor_sync(0xffffffffu, s, o);
-                t += __shfl_xor_sync(0xffffffffu, t, o);
-            }
-            t *= st.y;
-            if (lane == 0) {
-                const float gm = P.gamma ? load_param(P.gamma, P.gamma_type, c0 + k) : 1.0f;
-                P.chan[n * P.c + c0 + k] = make_float2(s, t);
-                s1 = fmaf(gm, s, s1);
-                s2 = fmaf(gm, t, s2);
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
+                    t[j] += __shfl_xor_sync(0xffffffffu, t[j], o);
+                }
+                if (lane == j && k + j < P.cpg) {
+                    const float w = t[j] * st.y;
+                    const float gm = P.gamma ? load_param(P.gamma, P.gamma_type, c0 + k + j) : 1.0f;
+                    P.chan[n * P.c + c0 + k + j] = make_float2(s[j], w);
+                    s1 = fmaf(gm, s[j], s1);
+                    s2 = fmaf(gm, w, s2);
+                }
             }
         }
-        s1 = block_sum(s1, red);
-        s2 = block_sum(s2, red);
-        if (threadIdx.x == 0) P.gsum[ng] = make_float2(st.y * s1 / total, st.y * st.y * s2 / total);
+        s1 = team_sum<TEAM>(s1, red);
+        s2 = team_sum<TEAM>(s2, red);
+        if (threadIdx.x % TEAM == 0) P.gsum[ng] = make_float2(st.y * s1 / total, st.y * st.y * s2 / total);
     }
 }
 
-template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_grad_apply_kernel(const __grid_constant__ NormParams P) {
+template <class T, int V, int ACT, bool DROP>
+__global__ void __launch_bounds__(kNormThreads, 2) norm_grad_apply_kernel(const __grid_constant__ NormParams P) {
+    extern __shared__ __align__(16) unsigned char nsm[];
+    uint4 *ring = reinterpret_cast<uint4 *>(nsm);
     griddep_wait();
     griddep_launch_dependents();
-    const int tid = threadIdx.x, lane = tid / P.vb, col = tid - lane * P.vb;
-    DropState ds{};
-    if (P.drop.threshold) ds = drop_state(P.drop, blockIdx.x == 0 && tid == 0);
-    for (long long item = blockIdx.x; item < P.items; item += gridDim.x) {
-        const NormItem it = norm_item(P, item, col);
-        if (lane >= P.lanes || it.vcol >= P.vcols) continue;
-        const int c0 = it.vcol * V;
-        const Coefs<V> coefs = split_coefs<V>(P, it.n, c0);
+    const SplitPlace at = split_place(P, V);
+    Keeper<V, DROP> drop(P, blockIdx.x == 0 && threadIdx.x == 0, at.n, at.p0, at.c0, P.lanes);
+    if (at.count == 0) return;
+    const Coefs<V> coefs = split_coefs<V>(P, at.n, at.c0);
+    Lanes<V> mk1, mk2;
+    {
         float k1[V], k2[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float2 k = P.gsum[it.n * P.groups + (c0 + j) / P.cpg];
+            const float2 k = P.gsum[at.n * P.groups + (at.c0 + j) / P.cpg];
             k1[j] = -k.x;
             k2[j] = -k.y;
         }
-        const Lanes<V> mk1 = lanes_of<V>(k1), mk2 = lanes_of<V>(k2);
-        uint32_t keep = ~0u;
-        if (P.drop.threshold && P.drop.channel) keep = keep_bits<V>(P.drop, ds, static_cast<uint64_t>(it.n) * P.c + c0);
-        const T *x = static_cast<const T *>(P.x) + it.n * P.x_ldn + c0;
-        const T *dy = static_cast<const T *>(P.dy) + it.n * P.dy_ldn + c0;
-        T *dx = static_cast<T *>(P.y) + it.n * P.y_ldn + c0;
-#pragma unroll 2
-        for (long long p = it.p0 + lane; p < it.p1; p += P.lanes) {
-            const Lanes<V> v = load_lanes<T, V>(x + p * P.x_ldp);
-            Lanes<V> g = load_lanes<T, V>(dy + p * P.dy_ldp);
-            if (P.drop.threshold) {
-                if (!P.drop.channel)
-                    keep = keep_bits<V>(P.drop, ds, (static_cast<uint64_t>(it.n) * P.px + p) * P.c + c0);
-                g = keep_lanes<V>(g, keep, P.drop.scale);
-            }
-            store_lanes<T, V>(dx + p * P.y_ldp, grad_result<V, ACT>(P.act, coefs, mk1, mk2, v, g));
-        }
+        mk1 = lanes_of<V>(k1);
+        mk2 = lanes_of<V>(k2);
     }
+    const T *x = static_cast<const T *>(P.x) + at.n * P.x_ldn + at.p0 * P.x_ldp + at.c0;
+    const T *dy = static_cast<const T *>(P.dy) + at.n * P.dy_ldn + at.p0 * P.dy_ldp + at.c0;
+    T *dx = static_cast<T *>(P.y) + at.n * P.y_ldn + at.p0 * P.y_ldp + at.c0;
+    const long long ystep = static_cast<long long>(P.lanes) * P.y_ldp;
+    for_vector_pairs<T, V>(ring, x, static_cast<long long>(P.lanes) * P.x_ldp, dy, static_cast<long long>(P.lanes) * P.dy_ldp,
+                           at.count, [&](int, const Lanes<V> &v, const Lanes<V> &g) {
+                               store_lanes<T, V>(dx, grad_result<V, ACT>(P.act, coefs, mk1, mk2, v, drop.apply(P, g)));
+                               dx += ystep;
+                           });
 }
 
 // dgamma, dbeta: the channels' sums over all rows (images, or CTAs of the
@@ -468,12 +676,14 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_params_kernel(const __
     const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
     float s = 0.0f, t = 0.0f;
-    if (c < P.c)
+    if (c < P.c) {
+#pragma unroll 8
         for (long long n = row; n < P.sum_rows; n += kNormThreads / 32) {
             const float2 v = P.chan[n * P.c + c];
             s += v.x;
             t += v.y;
         }
+    }
     sm[threadIdx.x] = make_float2(s, t);
     __syncthreads();
     if (row == 0 && c < P.c) {
@@ -533,9 +743,6 @@ __device__ __forceinline__ void wait_part(int part) {
     else if (part == 2) cp_async_wait<kParts - 3>();
     else cp_async_wait<0>();
 }
-__device__ __forceinline__ void copy_vector(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 
 // Calls f(j, group) for a thread's V channels, the group counted within the unit.
 template <int V, class F>
@@ -548,15 +755,10 @@ __device__ __forceinline__ void for_channels(const NormParams &P, const Resident
     }
 }
 
-// Rows of the gradient's channel sums that meet in shared memory: one a warp
-// where a warp holds whole pixel lanes (they are added by shuffles first),
-// else one a lane.
-__host__ __device__ inline int grad_rows(int threads, int vr, int lanes) { return 32 % vr == 0 ? threads / 32 : lanes; }
-
 // Shared memory of the resident kernels behind the tiles.
 __host__ __device__ inline size_t resident_extra(const NormParams &P, int threads, bool grad) {
     const size_t gb = P.gb, cb = P.cb;
-    const size_t entries = grad ? grad_rows(threads, P.vr, P.lanes) * cb + threads + 2 * cb
+    const size_t entries = grad ? channel_sums_space(threads, P.vr, P.lanes, P.cb) + 2 * cb
                                 : static_cast<size_t>(P.lanes) * P.vr * P.sub;
     return (entries + 4 * gb) * sizeof(float2);
 }
@@ -799,17 +1001,12 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
     float2 *gst = fin + P.gb;           // mean, rstd of the unit's groups
     float2 *weighted = gst + P.gb;      // [cb]: gamma * the channel's sums
     float2 *acc = weighted + P.cb;      // [cb]: the channel's sums over this CTA's images
-    float2 *segsum = acc + P.cb;        // [segs][cb]
-    float2 *red = segsum + threads;     // [rows][cb]
-    const int rows = grad_rows(threads, P.vr, P.lanes);
-    const bool warp_rows = 32 % P.vr == 0;
-    uint8_t *bits = reinterpret_cast<uint8_t *>(red + rows * P.cb);
+    float2 *scratch = acc + P.cb;       // channel_sums
+    uint8_t *bits = reinterpret_cast<uint8_t *>(scratch + channel_sums_space(threads, P.vr, P.lanes, P.cb));
     const int rank = blockIdx.x % P.cluster;
     const unsigned unit = blockIdx.x / P.cluster;
     const int bundle = unit % P.bundles;
     const Resident r = resident_place(P, rank, bundle, V);
-    // threads that share a channel's summing (none where a unit has more channels than threads)
-    const int segs = threads / P.cb;
     const uint4 *x_at = tx + tid, *g_at = x_at + tiles;
     const uint32_t x_addr = smem_addr(x_at), g_addr = smem_addr(g_at), pitch = 16 * threads;
     griddep_wait();
@@ -885,52 +1082,17 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
                 grad_sums<V, ACT>(P.act, coefs, v, g, s2, t2);
             }
         }
-        // channel sums over the CTA's pixels: by shuffles, then in two steps
-        if (r.lane < P.lanes) {
+        // channel sums over the CTA's pixels
+        {
             float s[V], t[V];
             values_of<V>(s2, s);
             values_of<V>(t2, t);
-            if (warp_rows)  // every lane of the block takes part: 32 is a multiple of vr
-                for (int o = P.vr; o < 32; o <<= 1) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
-                        t[j] += __shfl_xor_sync(0xffffffffu, t[j], o);
-                    }
-                }
-            if (!warp_rows || lane < P.vr) {
-                float2 *out = red + (warp_rows ? warp : r.lane) * P.cb + r.local;
-#pragma unroll
-                for (int j = 0; j < V; ++j) out[j] = make_float2(s[j], t[j]);
-            }
-        }
-        __syncthreads();
-        if (segs > 1) {
-            const int seg = tid / P.cb, c = tid - seg * P.cb;
-            float2 sum = make_float2(0.0f, 0.0f);
-            if (seg < segs) {
-                for (int l = seg; l < rows; l += segs) {
-                    const float2 v = red[l * P.cb + c];
-                    sum.x += v.x;
-                    sum.y += v.y;
-                }
-                segsum[tid] = sum;
-            }
-            __syncthreads();
-        }
-        const float2 *parts = segs > 1 ? segsum : red;
-        const int count = segs > 1 ? segs : rows;
-        for (int c = tid; c < P.cb; c += threads) {
-            float2 sum = make_float2(0.0f, 0.0f);
-            for (int i = 0; i < count; ++i) {
-                const float2 v = parts[i * P.cb + c];
-                sum.x += v.x;
-                sum.y += v.y;
-            }
-            sum.y *= gst[c / P.cpg].y;
-            const float w = P.gamma ? load_param(P.gamma, P.gamma_type, bundle * P.cb + c) : 1.0f;
-            weighted[c] = make_float2(w * sum.x, w * sum.y);
-            acc[c] = make_float2(acc[c].x + sum.x, acc[c].y + sum.y);
+            channel_sums<V>(P.vr, P.lanes, P.cb, r.lane, r.local, s, t, scratch, [&](int c, float2 sum) {
+                sum.y *= gst[c / P.cpg].y;
+                const float w = P.gamma ? load_param(P.gamma, P.gamma_type, bundle * P.cb + c) : 1.0f;
+                weighted[c] = make_float2(w * sum.x, w * sum.y);
+                acc[c] = make_float2(acc[c].x + sum.x, acc[c].y + sum.y);
+            });
         }
         __syncthreads();
         float2 *mine = exch + turn * P.gb;

@@ -230,18 +230,25 @@ bool vector_access(std::initializer_list<const View *> views) {
     return true;
 }
 
-// The split path's work split: blocks of up to 256 vector columns, chunks of
-// pixels such that there are about 16 blocks for each SM, but at least eight
-// pixels for each thread.
-void plan_split(NormParams &P, int v, int sms) {
+// The split path's work split: blocks of up to 256 vector columns and chunks
+// of pixels such that one wave of blocks (three per SM, two in the gradient)
+// streams everything, but at least eight pixels for each thread.
+void plan_split(NormParams &P, int v, bool backward, int sms) {
     P.vcols = P.c / v;
     P.cblocks = static_cast<int>(ceil_div(P.vcols, gcb::kNormThreads));
     P.vb = static_cast<int>(ceil_div(P.vcols, P.cblocks));
     P.lanes = gcb::kNormThreads / P.vb;
-    const long long wanted = std::max<long long>(1, ceil_div(16LL * sms, P.n * P.cblocks));
+    const long long wanted = std::max<long long>(1, (backward ? 2LL : 3LL) * sms / (P.n * P.cblocks));
     P.chunk_rows = std::min(P.px, std::max<long long>(ceil_div(P.px, wanted), 8LL * P.lanes));
     P.chunks = static_cast<int>(ceil_div(P.px, P.chunk_rows));
     P.items = P.n * P.chunks * P.cblocks;
+}
+// Shared memory of the split path's kernels: the ring, and what the sums need.
+size_t split_smem(const NormParams &P, int v, bool sums, bool backward) {
+    size_t bytes = gcb::ring_space(v);
+    if (sums) bytes += gcb::channel_sums_space(gcb::kNormThreads, P.vb, P.lanes, P.vb * v) * sizeof(float2);
+    if (sums && !backward) bytes += ceil_div(P.vb * v, 2) * 2 * sizeof(float);
+    return bytes;
 }
 
 uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
@@ -252,6 +259,7 @@ struct NormPlan {
     bool resident = false;
     int threads = gcb::kNormThreads;
     size_t smem = 0;
+    int width() const { return !vec ? 1 : type == gcb::kElemF32 ? 4 : 8; }  // elements of a vector
 };
 
 struct NormSpace {  // the workspace's parts, in this order
@@ -414,7 +422,7 @@ int plan_norm(NormParams &P, NormPlan &plan, bool backward) {
     gcb::DeviceFacts facts;
     const int st = gcb::device_facts(dev, facts);
     if (st != GC_OK) return st;
-    const int v = plan.vec ? (plan.type == gcb::kElemF32 ? 4 : 8) : 1;
+    const int v = plan.width();
     if (plan.vec) {
         // room for the decision bytes is planned for whether they are needed
         // or not, so that a tensor's workspace does not depend on the dropout
@@ -443,7 +451,8 @@ int plan_norm(NormParams &P, NormPlan &plan, bool backward) {
             return GC_OK;
         }
     }
-    plan_split(P, v, facts.sms);
+    plan_split(P, v, backward, facts.sms);
+    if (P.items > INT32_MAX) return gc_error(GC_UNSUPPORTED, "more images than a grid has blocks");
     return GC_OK;
 }
 
@@ -453,32 +462,34 @@ void set_param(const gc_tensor *t, const void *&p, int &type) {
 }
 
 // ---- kernel tables --------------------------------------------------------------------------
-// The vector kernels are compiled for each activation; the scalar ones, for
-// tensors whose pixels are not 16-byte aligned, choose it at run time.
+// The vector kernels without dropout are compiled for each activation; the
+// others choose it at run time.
 enum NormKernel { kMoments, kApply, kGradSums, kGradApply };
 
-template <class T, int V, int ACT>
+template <class T, int V, int ACT, bool DROP>
 const void *norm_instance(NormKernel k) {
     switch (k) {
-    case kApply: return reinterpret_cast<const void *>(&gcb::norm_apply_kernel<T, V, ACT>);
-    case kGradSums: return reinterpret_cast<const void *>(&gcb::norm_grad_sums_kernel<T, V, ACT>);
-    case kGradApply: return reinterpret_cast<const void *>(&gcb::norm_grad_apply_kernel<T, V, ACT>);
+    case kApply: return reinterpret_cast<const void *>(&gcb::norm_apply_kernel<T, V, ACT, DROP>);
+    case kGradSums: return reinterpret_cast<const void *>(&gcb::norm_grad_sums_kernel<T, V, ACT, DROP>);
+    case kGradApply: return reinterpret_cast<const void *>(&gcb::norm_grad_apply_kernel<T, V, ACT, DROP>);
     default: return reinterpret_cast<const void *>(&gcb::norm_moments_kernel<T, V>);
     }
 }
 template <class T>
-const void *norm_typed(NormKernel k, bool vec, int act) {
+const void *norm_typed(NormKernel k, bool vec, int act, bool drop) {
     constexpr int V = gcb::kVec<T>;
-    if (!vec) return norm_instance<T, 1, -1>(k);
-    if (act == gcb::kActRelu) return norm_instance<T, V, gcb::kActRelu>(k);
-    if (act == gcb::kActRelu6) return norm_instance<T, V, gcb::kActRelu6>(k);
-    if (act == gcb::kActSilu) return norm_instance<T, V, gcb::kActSilu>(k);
-    return norm_instance<T, V, gcb::kActNone>(k);
+    if (!vec) return drop ? norm_instance<T, 1, -1, true>(k) : norm_instance<T, 1, -1, false>(k);
+    if (drop) return norm_instance<T, V, -1, true>(k);
+    if (act == gcb::kActRelu) return norm_instance<T, V, gcb::kActRelu, false>(k);
+    if (act == gcb::kActRelu6) return norm_instance<T, V, gcb::kActRelu6, false>(k);
+    if (act == gcb::kActSilu) return norm_instance<T, V, gcb::kActSilu, false>(k);
+    return norm_instance<T, V, gcb::kActNone, false>(k);
 }
-const void *norm_kernel(NormKernel k, const NormPlan &plan, int act) {
-    if (plan.type == gcb::kElemF16) return norm_typed<__half>(k, plan.vec, act);
-    if (plan.type == gcb::kElemBF16) return norm_typed<__nv_bfloat16>(k, plan.vec, act);
-    return norm_typed<float>(k, plan.vec, act);
+const void *norm_kernel(NormKernel k, const NormPlan &plan, const NormParams &P) {
+    const bool drop = P.drop.threshold != 0;
+    if (plan.type == gcb::kElemF16) return norm_typed<__half>(k, plan.vec, P.act, drop);
+    if (plan.type == gcb::kElemBF16) return norm_typed<__nv_bfloat16>(k, plan.vec, P.act, drop);
+    return norm_typed<float>(k, plan.vec, P.act, drop);
 }
 
 // The resident kernels with dropout choose the activation at run time.
@@ -502,7 +513,7 @@ const void *resident_kernel(const NormPlan &plan, bool backward, int act, bool d
 
 // Opts a kernel into the shared memory and the cluster sizes it may be
 // launched with, once per device.
-int prepare_resident(const void *fn, int dev, int smem_optin) {
+int prepare_kernel(const void *fn, int dev, int smem_optin) {
     static std::map<std::pair<int, const void *>, bool> done;
     std::lock_guard<std::mutex> lock(g_mutex);
     bool &flag = done[{dev, fn}];
@@ -522,7 +533,7 @@ int launch_resident(NormParams &P, const NormPlan &plan, bool backward, int dev,
     int st = gcb::device_facts(dev, facts);
     if (st != GC_OK) return st;
     const void *fn = resident_kernel(plan, backward, P.act, P.drop.threshold != 0);
-    if ((st = prepare_resident(fn, dev, facts.smem_optin)) != GC_OK) return st;
+    if ((st = prepare_kernel(fn, dev, facts.smem_optin)) != GC_OK) return st;
     void *args[] = {&P};
     const unsigned grid = static_cast<unsigned>(static_cast<long long>(P.stride) * P.bundles * P.cluster);
     e = gcb::launch_pdl(fn, dim3(grid), dim3(plan.threads), args, plan.smem, s, P.cluster);
@@ -531,9 +542,31 @@ int launch_resident(NormParams &P, const NormPlan &plan, bool backward, int dev,
 
 unsigned grid_of(long long items) { return static_cast<unsigned>(std::min<long long>(items, INT32_MAX)); }
 
-cudaError_t launch(const void *fn, long long blocks, NormParams &P, cudaStream_t s) {
+cudaError_t launch(const void *fn, long long blocks, NormParams &P, cudaStream_t s, size_t smem = 0) {
     void *args[] = {&P};
-    return gcb::launch_pdl(fn, dim3(grid_of(blocks)), dim3(gcb::kNormThreads), args, 0, s);
+    return gcb::launch_pdl(fn, dim3(grid_of(blocks)), dim3(gcb::kNormThreads), args, smem, s);
+}
+
+// A kernel of the split path that streams data.
+int launch_split(NormKernel k, NormParams &P, const NormPlan &plan, int dev, cudaStream_t s, cudaError_t &e) {
+    gcb::DeviceFacts facts;
+    int st = gcb::device_facts(dev, facts);
+    if (st != GC_OK) return st;
+    const void *fn = norm_kernel(k, plan, P);
+    if ((st = prepare_kernel(fn, dev, facts.smem_optin)) != GC_OK) return st;
+    e = launch(fn, P.items, P, s, split_smem(P, plan.width(), k == kMoments || k == kGradSums, k == kGradSums));
+    return GC_OK;
+}
+
+// The kernels that join partial results per group: a warp per group, or a
+// block where a group has more than 256 entries.
+cudaError_t launch_finalize(bool backward, NormParams &P, cudaStream_t s) {
+    const bool block = static_cast<long long>(P.chunks) * P.cpg > 256;
+    const void *fn = backward ? (block ? reinterpret_cast<const void *>(&gcb::norm_grad_finalize_kernel<gcb::kNormThreads>)
+                                       : reinterpret_cast<const void *>(&gcb::norm_grad_finalize_kernel<32>))
+                              : (block ? reinterpret_cast<const void *>(&gcb::norm_finalize_kernel<gcb::kNormThreads>)
+                                       : reinterpret_cast<const void *>(&gcb::norm_finalize_kernel<32>));
+    return launch(fn, block ? P.n * P.groups : ceil_div(P.n * P.groups, gcb::kNormThreads / 32), P, s);
 }
 
 int check_workspace(const void *p, uint64_t bytes, uint64_t need) {
@@ -662,10 +695,9 @@ int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
                          plan.threads, plan.smem, P.cluster, P.cb, P.rows, 1, 1);
         return launched(e);
     }
-    e = launch(norm_kernel(kMoments, plan, activation), P.items, P, s);
-    if (e == cudaSuccess)
-        e = launch(reinterpret_cast<const void *>(&gcb::norm_finalize_kernel), P.n * P.groups, P, s);
-    if (e == cudaSuccess) e = launch(norm_kernel(kApply, plan, activation), P.items, P, s);
+    if ((st = launch_split(kMoments, P, plan, dev, s, e)) != GC_OK) return st;
+    if (e == cudaSuccess) e = launch_finalize(false, P, s);
+    if (e == cudaSuccess && (st = launch_split(kApply, P, plan, dev, s, e)) != GC_OK) return st;
     gcb::record_plan(PlanRecord::kNorm, "split", false, P.items, gcb::kNormThreads, 0, 1, P.vb, P.chunk_rows,
                      plan.vec ? 1 : 0, 3);
     return launched(e);
@@ -764,10 +796,9 @@ int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
         return launched(e);
     }
     P.sum_rows = P.n;
-    e = launch(norm_kernel(kGradSums, plan, activation), P.items, P, s);
-    if (e == cudaSuccess)
-        e = launch(reinterpret_cast<const void *>(&gcb::norm_grad_finalize_kernel), P.n * P.groups, P, s);
-    if (e == cudaSuccess) e = launch(norm_kernel(kGradApply, plan, activation), P.items, P, s);
+    if ((st = launch_split(kGradSums, P, plan, dev, s, e)) != GC_OK) return st;
+    if (e == cudaSuccess) e = launch_finalize(true, P, s);
+    if (e == cudaSuccess && (st = launch_split(kGradApply, P, plan, dev, s, e)) != GC_OK) return st;
     if (e == cudaSuccess && params) e = launch(sums, ceil_div(P.c, 32), P, s);
     gcb::record_plan(PlanRecord::kNorm, "split_backward", false, P.items, gcb::kNormThreads, 0, 1, P.vb, P.chunk_rows,
                      plan.vec ? 1 : 0, params ? 4 : 3);
