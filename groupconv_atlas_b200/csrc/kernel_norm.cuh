@@ -220,7 +220,19 @@ __device__ __forceinline__ SplitPlace split_place(const NormParams &P, int v) {
 }
 
 // Calls f(k, vector) for a thread's vectors.  ring: kRing * kNormThreads
-// vectors of shared memory (V > 1).
+// vectors of shared memory (V > 1).  start_vectors issues the first copies and
+// may run before the wait for an earlier launch that does not write the data.
+template <int V, class T>
+__device__ __forceinline__ void start_vectors(uint4 *ring, const T *p, long long step, int count) {
+    if constexpr (V > 1) {
+        const uint32_t addr = smem_addr(ring + threadIdx.x);
+#pragma unroll
+        for (int u = 0; u < kRing; ++u, p += step) {
+            if (u < count) copy_vector(addr + u * kNormThreads * sizeof(uint4), p);
+            cp_async_commit();
+        }
+    }
+}
 template <class T, int V, class F>
 __device__ __forceinline__ void for_vectors(uint4 *ring, const T *p, long long step, int count, F f) {
     if constexpr (V == 1) {
@@ -237,11 +249,7 @@ __device__ __forceinline__ void for_vectors(uint4 *ring, const T *p, long long s
         const uint4 *mine = ring + threadIdx.x;
         const uint32_t addr = smem_addr(mine);
         constexpr uint32_t kPitch = kNormThreads * sizeof(uint4);
-#pragma unroll
-        for (int u = 0; u < kRing; ++u, p += step) {
-            if (u < count) copy_vector(addr + u * kPitch, p);
-            cp_async_commit();
-        }
+        p += kRing * step;
 #pragma unroll 4
         for (int k = 0; k < count; ++k, p += step) {
             const int slot = k % kRing;
@@ -254,6 +262,22 @@ __device__ __forceinline__ void for_vectors(uint4 *ring, const T *p, long long s
     }
 }
 // The same for two tensors: f(k, vector of p, vector of q).
+template <int V, class T>
+__device__ __forceinline__ void start_vector_pairs(uint4 *ring, const T *p, long long pstep, const T *q, long long qstep,
+                                                   int count) {
+    if constexpr (V > 1) {
+        const uint32_t addr = smem_addr(ring + threadIdx.x);
+        constexpr uint32_t kPitch = kNormThreads * sizeof(uint4);
+#pragma unroll
+        for (int u = 0; u < kRing / 2; ++u, p += pstep, q += qstep) {
+            if (u < count) {
+                copy_vector(addr + 2 * u * kPitch, p);
+                copy_vector(addr + (2 * u + 1) * kPitch, q);
+            }
+            cp_async_commit();
+        }
+    }
+}
 template <class T, int V, class F>
 __device__ __forceinline__ void for_vector_pairs(uint4 *ring, const T *p, long long pstep, const T *q, long long qstep,
                                                  int count, F f) {
@@ -276,14 +300,8 @@ __device__ __forceinline__ void for_vector_pairs(uint4 *ring, const T *p, long l
         const uint4 *mine = ring + threadIdx.x;
         const uint32_t addr = smem_addr(mine);
         constexpr uint32_t kPitch = kNormThreads * sizeof(uint4);
-#pragma unroll
-        for (int u = 0; u < kHalf; ++u, p += pstep, q += qstep) {
-            if (u < count) {
-                copy_vector(addr + 2 * u * kPitch, p);
-                copy_vector(addr + (2 * u + 1) * kPitch, q);
-            }
-            cp_async_commit();
-        }
+        p += kHalf * pstep;
+        q += kHalf * qstep;
 #pragma unroll 2
         for (int k = 0; k < count; ++k, p += pstep, q += qstep) {
             const int slot = 2 * (k % kHalf);
@@ -368,6 +386,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_moments_kernel(const __g
     for (int j = 0; j < V; ++j) m.mean[j] = m.m2[j] = 0.0f;
     const T *x = static_cast<const T *>(P.x) + at.n * P.x_ldn + at.p0 * P.x_ldp + at.c0;
     const long long step = static_cast<long long>(P.lanes) * P.x_ldp;
+    start_vectors<V>(ring, x, step, at.count);
     for_vectors<T, V>(ring, x, step, at.count, [&](int i, const Lanes<V> &v) {
         if (i % kNormRun == 0) {
             if (i > 0) m.finish(kNormRun);
@@ -489,7 +508,7 @@ struct Keeper {
         if (!DROP) return;
         ds = drop_state(P.drop, writer);
         at = (static_cast<uint64_t>(n) * P.px + p0) * P.c + c0;
-        step = static_cast<uint64_t>(lanes) * P.c;
+        step = static_cast<uint64_t>(static_cast<long long>(lanes) * P.c);  // modulo 2^64 where it goes down
         if (P.drop.channel) keep = keep_bits<V>(P.drop, ds, static_cast<uint64_t>(n) * P.c + c0);
     }
     __device__ __forceinline__ Lanes<V> apply(const NormParams &P, const Lanes<V> &v) {
@@ -500,21 +519,26 @@ struct Keeper {
     }
 };
 
-// Normalises, activates and drops out: the second pass over x.
+// Normalises, activates and drops out: the second pass over x, from a chunk's
+// end to its start, because the first pass left the ends in the L2 cache.  x
+// is not written by the launches that this one follows, so its first copies
+// are issued before the wait for their results.
 template <class T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(kNormThreads, 3) norm_apply_kernel(const __grid_constant__ NormParams P) {
     extern __shared__ __align__(16) unsigned char nsm[];
     uint4 *ring = reinterpret_cast<uint4 *>(nsm);
+    const SplitPlace at = split_place(P, V);
+    const long long last = at.p0 + static_cast<long long>(max(0, at.count - 1)) * P.lanes;
+    const T *x = static_cast<const T *>(P.x) + at.n * P.x_ldn + last * P.x_ldp + at.c0;
+    const long long xstep = -static_cast<long long>(P.lanes) * P.x_ldp, ystep = -static_cast<long long>(P.lanes) * P.y_ldp;
+    start_vectors<V>(ring, x, xstep, at.count);
     griddep_wait();
     griddep_launch_dependents();
-    const SplitPlace at = split_place(P, V);
-    Keeper<V, DROP> drop(P, blockIdx.x == 0 && threadIdx.x == 0, at.n, at.p0, at.c0, P.lanes);
+    Keeper<V, DROP> drop(P, blockIdx.x == 0 && threadIdx.x == 0, at.n, last, at.c0, -P.lanes);
     if (at.count == 0) return;
     const Coefs<V> coefs = split_coefs<V>(P, at.n, at.c0);
-    const T *x = static_cast<const T *>(P.x) + at.n * P.x_ldn + at.p0 * P.x_ldp + at.c0;
-    T *y = static_cast<T *>(P.y) + at.n * P.y_ldn + at.p0 * P.y_ldp + at.c0;
-    const long long ystep = static_cast<long long>(P.lanes) * P.y_ldp;
-    for_vectors<T, V>(ring, x, static_cast<long long>(P.lanes) * P.x_ldp, at.count, [&](int, Lanes<V> v) {
+    T *y = static_cast<T *>(P.y) + at.n * P.y_ldn + last * P.y_ldp + at.c0;
+    for_vectors<T, V>(ring, x, xstep, at.count, [&](int, Lanes<V> v) {
 #pragma unroll
         for (int i = 0; i < Lanes<V>::kPairs; ++i) {
             f2 d;
@@ -561,17 +585,18 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_grad_sums_kernel(const _
     griddep_launch_dependents();
     const SplitPlace at = split_place(P, V);
     uint4 *ring = reinterpret_cast<uint4 *>(nsm);
+    const T *x = static_cast<const T *>(P.x) + at.n * P.x_ldn + at.p0 * P.x_ldp + at.c0;
+    const T *dy = static_cast<const T *>(P.dy) + at.n * P.dy_ldn + at.p0 * P.dy_ldp + at.c0;
+    const long long xstep = static_cast<long long>(P.lanes) * P.x_ldp, gstep = static_cast<long long>(P.lanes) * P.dy_ldp;
+    start_vector_pairs<V>(ring, x, xstep, dy, gstep, at.count);
     Keeper<V, DROP> drop(P, false, at.n, at.p0, at.c0, P.lanes);
     const Coefs<V> coefs = split_coefs<V>(P, at.n, at.c0);
     Lanes<V> s2, t2;
 #pragma unroll
     for (int i = 0; i < Lanes<V>::kPairs; ++i) s2.p[i] = t2.p[i] = pair(0.0f);
-    const T *x = static_cast<const T *>(P.x) + at.n * P.x_ldn + at.p0 * P.x_ldp + at.c0;
-    const T *dy = static_cast<const T *>(P.dy) + at.n * P.dy_ldn + at.p0 * P.dy_ldp + at.c0;
-    for_vector_pairs<T, V>(ring, x, static_cast<long long>(P.lanes) * P.x_ldp, dy, static_cast<long long>(P.lanes) * P.dy_ldp,
-                           at.count, [&](int, const Lanes<V> &v, const Lanes<V> &g) {
-                               grad_sums<V, ACT>(P.act, coefs, v, drop.apply(P, g), s2, t2);
-                           });
+    for_vector_pairs<T, V>(ring, x, xstep, dy, gstep, at.count, [&](int, const Lanes<V> &v, const Lanes<V> &g) {
+        grad_sums<V, ACT>(P.act, coefs, v, drop.apply(P, g), s2, t2);
+    });
     float s[V], t[V];
     values_of<V>(s2, s);
     values_of<V>(t2, t);
@@ -634,14 +659,20 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_finalize_kernel(const 
     }
 }
 
+// The second pass over x and dy, like norm_apply_kernel.
 template <class T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(kNormThreads, 2) norm_grad_apply_kernel(const __grid_constant__ NormParams P) {
     extern __shared__ __align__(16) unsigned char nsm[];
     uint4 *ring = reinterpret_cast<uint4 *>(nsm);
+    const SplitPlace at = split_place(P, V);
+    const long long last = at.p0 + static_cast<long long>(max(0, at.count - 1)) * P.lanes;
+    const T *x = static_cast<const T *>(P.x) + at.n * P.x_ldn + last * P.x_ldp + at.c0;
+    const T *dy = static_cast<const T *>(P.dy) + at.n * P.dy_ldn + last * P.dy_ldp + at.c0;
+    const long long down = -static_cast<long long>(P.lanes), xstep = down * P.x_ldp, gstep = down * P.dy_ldp;
+    start_vector_pairs<V>(ring, x, xstep, dy, gstep, at.count);
     griddep_wait();
     griddep_launch_dependents();
-    const SplitPlace at = split_place(P, V);
-    Keeper<V, DROP> drop(P, blockIdx.x == 0 && threadIdx.x == 0, at.n, at.p0, at.c0, P.lanes);
+    Keeper<V, DROP> drop(P, blockIdx.x == 0 && threadIdx.x == 0, at.n, last, at.c0, -P.lanes);
     if (at.count == 0) return;
     const Coefs<V> coefs = split_coefs<V>(P, at.n, at.c0);
     Lanes<V> mk1, mk2;
@@ -656,15 +687,12 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_grad_apply_kernel(const 
         mk1 = lanes_of<V>(k1);
         mk2 = lanes_of<V>(k2);
     }
-    const T *x = static_cast<const T *>(P.x) + at.n * P.x_ldn + at.p0 * P.x_ldp + at.c0;
-    const T *dy = static_cast<const T *>(P.dy) + at.n * P.dy_ldn + at.p0 * P.dy_ldp + at.c0;
-    T *dx = static_cast<T *>(P.y) + at.n * P.y_ldn + at.p0 * P.y_ldp + at.c0;
-    const long long ystep = static_cast<long long>(P.lanes) * P.y_ldp;
-    for_vector_pairs<T, V>(ring, x, static_cast<long long>(P.lanes) * P.x_ldp, dy, static_cast<long long>(P.lanes) * P.dy_ldp,
-                           at.count, [&](int, const Lanes<V> &v, const Lanes<V> &g) {
-                               store_lanes<T, V>(dx, grad_result<V, ACT>(P.act, coefs, mk1, mk2, v, drop.apply(P, g)));
-                               dx += ystep;
-                           });
+    T *dx = static_cast<T *>(P.y) + at.n * P.y_ldn + last * P.y_ldp + at.c0;
+    const long long ystep = down * P.y_ldp;
+    for_vector_pairs<T, V>(ring, x, xstep, dy, gstep, at.count, [&](int, const Lanes<V> &v, const Lanes<V> &g) {
+        store_lanes<T, V>(dx, grad_result<V, ACT>(P.act, coefs, mk1, mk2, v, drop.apply(P, g)));
+        dx += ystep;
+    });
 }
 
 // dgamma, dbeta: the channels' sums over all rows (images, or CTAs of the

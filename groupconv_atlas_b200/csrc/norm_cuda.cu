@@ -232,7 +232,10 @@ bool vector_access(std::initializer_list<const View *> views) {
 
 // The split path's work split: blocks of up to 256 vector columns and chunks
 // of pixels such that one wave of blocks (three per SM, two in the gradient)
-// streams everything, but at least eight pixels for each thread.
+// streams everything, but at least eight pixels for each thread.  (Launching
+// sets of images small enough for the second pass to find them in the L2 cache
+// was slower: a set's three launches cost about 10 us beside its data, N8 C128
+// 256x256 bf16 forward 78 us in one set, 108 us in four.)
 void plan_split(NormParams &P, int v, bool backward, int sms) {
     P.vcols = P.c / v;
     P.cblocks = static_cast<int>(ceil_div(P.vcols, gcb::kNormThreads));
@@ -243,6 +246,7 @@ void plan_split(NormParams &P, int v, bool backward, int sms) {
     P.chunks = static_cast<int>(ceil_div(P.px, P.chunk_rows));
     P.items = P.n * P.chunks * P.cblocks;
 }
+
 // Shared memory of the split path's kernels: the ring, and what the sums need.
 size_t split_smem(const NormParams &P, int v, bool sums, bool backward) {
     size_t bytes = gcb::ring_space(v);
@@ -368,21 +372,32 @@ long long resident_stride(const NormParams &P, int threads, size_t smem, const g
     return ceil_div(P.n, ceil_div(P.n, most));
 }
 
-// Estimated time in microseconds of a choice that is set in P.
+// Estimated time in microseconds of a resident choice that is set in P: its
+// phases (load; per image of a cluster the first pass, the sums, the second
+// pass) with constants fitted to 1500 measured choices of 24 shapes on a B200;
+// the choice it makes is on average 4 % slower than the best of them.
 double resident_cost(const NormParams &P, int v, int threads, size_t smem, bool backward, const gcb::DeviceFacts &f) {
     int occ = 1;
     const long long stride = resident_stride(P, threads, smem, f, occ);
     const double rounds = static_cast<double>(ceil_div(P.n, stride));
-    const double ctas = static_cast<double>(stride) * P.bundles * P.cluster;
-    const double esize = v == 4 ? 4 : 2;
-    const double bytes = (backward ? 3.0 : 2.0) * esize * P.n * P.px * P.c;
-    const double lanes = static_cast<double>(P.vr * P.lanes) / threads;
-    const double ragged = static_cast<double>(P.px) / (static_cast<double>(P.lanes) * P.iters * P.cluster);
-    const double run = P.cb * esize;
-    const double run_eff = run >= 128 ? 1.0 : run >= 64 ? 0.97 : run >= 32 ? 0.9 : 0.6;
-    const double gap = (backward ? 2.5 : 2.0) + (P.cluster > 1 ? 0.7 : 0.0) + (P.cluster > 8 ? 0.4 : 0.0);
-    const double rate = 6.0e6 * run_eff * std::min(1.0, ctas / f.sms) * (0.5 + 0.5 * lanes * ragged);  // bytes per us
-    return bytes / rate + gap * (1.0 + (rounds - 1.0) / occ);
+    const double per_sm = std::ceil(static_cast<double>(stride) * P.bundles * P.cluster / f.sms);  // CTAs of the fullest SM
+    const double run = P.cb * (v == 4 ? 4.0 : 2.0);
+    const double kb = per_sm * P.iters * P.lanes * P.vr * 16.0 * (backward ? 2 : 1) / 1024.0 /
+                      (run >= 64 ? 1.0 : run >= 32 ? 0.78 : 0.43);  // narrow runs waste sectors
+    double sums = 1.4 + (P.cluster > 1 ? 1.4 : 0.0) + (P.cluster > 8 ? 0.4 : 0.0) + 0.12 * per_sm * threads / 512;
+    if (backward) sums += 32 % P.vr != 0 ? 2.0 : 0.0;
+    else sums += 0.22 * P.vr * P.lanes * P.sub / 512;
+    // per vector of a thread: latency with few warps, issue slots with many
+    const double crowd = P.iters * std::max(1.0, per_sm * threads / 32 / 6.2);
+    const double first = std::max(kb / 1300.0, crowd * (v == 4 ? 0.0 : 0.031) * (backward ? 1.5 : 1.0));
+    const double second = std::max(kb / (backward ? 36.0 : 34.0), crowd * (v == 4 ? 0.09 : 0.14) * (backward ? 2.5 : 1.0));
+    return 2.3 + kb / 88.0 + rounds * (first + sums + second) + (backward ? 1.65 : 0.0);
+}
+// The same for the split path: its launches' fixed times and the data at the
+// rates they reach.
+double split_cost(const NormParams &P, int v, bool backward) {
+    const double mb = static_cast<double>(P.n) * P.px * P.c * (v == 4 ? 4.0 : 2.0) * 1e-6;
+    return backward ? 12.9 + 2 * mb / 6.0 + 3 * mb / 6.6 : 8.6 + mb / 5.5 + 2 * mb / 6.6;
 }
 
 std::mutex g_mutex;
@@ -390,7 +405,7 @@ std::map<ResidentKey, ResidentPlan> g_resident;
 
 ResidentPlan choose_resident(const NormParams &base, int v, bool backward, bool bits, const gcb::DeviceFacts &f) {
     ResidentPlan best;
-    double best_cost = 0.0;
+    double best_cost = split_cost(base, v, backward);
     const int unit = std::lcm(base.cpg, v);  // channels: whole groups and whole vectors
     const int units = base.c / unit;
     for (int m = 1; m <= units && static_cast<long long>(m) * unit / v <= gcb::kNormThreads; ++m) {
@@ -402,7 +417,7 @@ ResidentPlan choose_resident(const NormParams &base, int v, bool backward, bool 
                 if (!set_resident(P, v, m * unit, cluster, threads, backward, bits, f.smem_optin, smem)) continue;
                 if (P.n * P.bundles * cluster > INT32_MAX) continue;
                 const double cost = resident_cost(P, v, threads, smem, backward, f);
-                if (!best.ok || cost < best_cost) {
+                if (cost < best_cost) {
                     best_cost = cost;
                     best.ok = true;
                     best.cb = m * unit;
