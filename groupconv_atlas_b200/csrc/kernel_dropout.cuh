@@ -1,6 +1,11 @@
-// Dropout of a dense tensor from the counter-based generator, with an optional
-// residual sum.  A thread takes eight elements at consecutive places, which is
-// one generator block: 16 bytes of a 16-bit tensor or 32 of FP32.
+// Dropout from the counter-based generator, with an optional residual sum.
+//
+// dropout_kernel          one decision per element
+// channel_dropout_kernel  one decision per channel of an image, channels last
+// plane_dropout_kernel    the same in plain order
+// A decision per channel is drawn once for all the pixels that a thread takes.
+// All three stream 16-byte vectors through the per-thread rings, or single
+// elements where a tensor is not aligned.
 #pragma once
 #include "norm_util.cuh"
 
@@ -9,68 +14,124 @@ namespace gcb {
 struct DropoutParams {
     const void *x, *residual;  // residual nullable
     void *y;
-    uint64_t count;
-    uint64_t groups;       // ceil(count / 8)
-    uint64_t image, inner; // channel scope: elements of an image, and of a channel (1: channels last)
-    uint64_t channels;
+    uint64_t count;            // elements
+    // one decision per channel
+    uint64_t decisions;        // images * channels
+    uint64_t row;              // pixels of an image
+    uint64_t chunk, chunks;    // pixels per block (channels last) or warp (plain), chunks of an image or plane
+    int channels, vcols, vb, cblocks, lanes;  // channels last: columns as in the norm's split path
     DropParams drop;
 };
 
-// Decision index of the element at place i with one decision per channel.
-__device__ __forceinline__ uint64_t channel_index(const DropoutParams &P, uint64_t i) {
-    if (P.inner != 1) return i / P.inner;  // (n, c, pixels): n * C + c
-    return i / P.image * P.channels + i % P.channels;
+// y = drop(x) [+ residual] for the vectors at k * step from x, y, residual;
+// drop(k, vector).
+template <class T, int V, class F>
+__device__ __forceinline__ void drop_vectors(uint4 *ring, const T *x, const T *residual, T *y, long long step, int count,
+                                             F drop) {
+    if (residual != nullptr) {
+        start_vector_pairs<V>(ring, x, step, residual, step, count);
+        for_vector_pairs<T, V>(ring, x, step, residual, step, count, [&](int k, const Lanes<V> &v, const Lanes<V> &r) {
+            Lanes<V> s = drop(k, v);
+#pragma unroll
+            for (int i = 0; i < Lanes<V>::kPairs; ++i) s.p[i] = s.p[i] + r.p[i];
+            store_lanes<T, V>(y, s);
+            y += step;
+        });
+    } else {
+        start_vectors<V>(ring, x, step, count);
+        for_vectors<T, V>(ring, x, step, count, [&](int k, const Lanes<V> &v) {
+            store_lanes<T, V>(y, drop(k, v));
+            y += step;
+        });
+    }
 }
 
-template <class T, bool VEC, bool CHANNEL>
-__global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutParams P) {
-    constexpr int V = kVec<T>;
+// Two neighbouring threads of an FP32 tensor compute the same generator block,
+// which costs less than accesses of half a sector.  16-bit tensors are bound
+// by the generator's products (19 of 32 x 32 -> 64 bits for eight elements).
+template <class T, int V>
+__global__ void __launch_bounds__(kStreamThreads, 3) dropout_kernel(const __grid_constant__ DropoutParams P) {
+    extern __shared__ __align__(16) unsigned char nsm[];
     griddep_wait();
     griddep_launch_dependents();
-    const DropState ds = drop_state(P.drop, blockIdx.x == 0 && threadIdx.x == 0);
+    const Philox gen(P.drop, blockIdx.x == 0 && threadIdx.x == 0);
     const T *x = static_cast<const T *>(P.x), *res = static_cast<const T *>(P.residual);
     T *y = static_cast<T *>(P.y);
-    for (uint64_t g = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; g < P.groups;
-         g += static_cast<uint64_t>(gridDim.x) * blockDim.x) {
-        const uint64_t i0 = 8 * g;
-        const int here = static_cast<int>(min(static_cast<uint64_t>(8), P.count - i0));
-        uint32_t keep = 0;
-        if (!CHANNEL) {
-            keep = keep_bits<8>(P.drop, ds, i0);
-        } else {
-            uint64_t block = ~static_cast<uint64_t>(0);
-            uint32_t bits = 0;
-            for (int k = 0; k < here; ++k) {
-                const uint64_t j = channel_index(P, i0 + k);
-                if (j >> 3 != block) {
-                    block = j >> 3;
-                    bits = keep_bits<8>(P.drop, ds, block << 3);
-                }
-                keep |= (bits >> (j & 7) & 1u) << k;
-            }
-        }
-        if (VEC && here == 8) {
-#pragma unroll
-            for (int h = 0; h < 8 / V; ++h) {
-                float v[V];
-                load_elems<T, V>(x + i0 + h * V, v);
-#pragma unroll
-                for (int k = 0; k < V; ++k) v[k] = keep >> (h * V + k) & 1u ? v[k] * P.drop.scale : 0.0f;
-                if (res != nullptr) {
-                    float r[V];
-                    load_elems<T, V>(res + i0 + h * V, r);
-#pragma unroll
-                    for (int k = 0; k < V; ++k) v[k] += r[k];
-                }
-                store_elems<T, V>(y + i0 + h * V, v);
-            }
-        } else {
-            for (int k = 0; k < here; ++k) {
-                float v = keep >> k & 1u ? to_float(x[i0 + k]) * P.drop.scale : 0.0f;
-                if (res != nullptr) v += to_float(res[i0 + k]);
-                y[i0 + k] = from_float<T>(v);
-            }
-        }
+    const uint64_t step = static_cast<uint64_t>(gridDim.x) * kStreamThreads;
+    const uint64_t first = static_cast<uint64_t>(blockIdx.x) * kStreamThreads + threadIdx.x, whole = P.count / V;
+    // every 2^31 - 1 vectors of a thread anew: the loops count in 32 bits
+    constexpr uint64_t kMost = 0x7fffffff;
+    for (uint64_t g = first; g < whole; g += kMost * step) {
+        const int count = static_cast<int>(min(kMost, (whole - g + step - 1) / step));
+        drop_vectors<T, V>(reinterpret_cast<uint4 *>(nsm), x + V * g, res == nullptr ? res : res + V * g, y + V * g,
+                           static_cast<long long>(V * step), count, [&](int k, const Lanes<V> &v) {
+                               if (P.drop.threshold == 0) return v;
+                               return drop_lanes<V>(v, Draws<V>(gen, V * (g + k * step)), P.drop);
+                           });
+    }
+    const uint64_t i = whole * V + first;  // fewer than V elements are left
+    if (i < P.count) {
+        const bool keep = P.drop.threshold == 0 || Draws<1>(gen, i).keep(0, P.drop.limit);
+        float v = keep ? to_float(x[i]) * P.drop.scale : 0.0f;
+        if (res != nullptr) v += to_float(res[i]);
+        y[i] = from_float<T>(v);
+    }
+}
+
+// A thread keeps one vector of channels (V = 1: one channel) for the pixels of
+// its block's chunk.
+template <class T, int V>
+__global__ void __launch_bounds__(kStreamThreads, 3) channel_dropout_kernel(const __grid_constant__ DropoutParams P) {
+    extern __shared__ __align__(16) unsigned char nsm[];
+    griddep_wait();
+    griddep_launch_dependents();
+    const Philox gen(P.drop, blockIdx.x == 0 && threadIdx.x == 0);
+    const unsigned cb = blockIdx.x % P.cblocks, t = blockIdx.x / P.cblocks;
+    const uint64_t n = t / P.chunks, first = (t - n * P.chunks) * P.chunk;
+    const int lane = threadIdx.x / P.vb, col = static_cast<int>(cb) * P.vb + threadIdx.x % P.vb;
+    const uint64_t p0 = first + lane, last = min(P.row, first + P.chunk);
+    if (lane >= P.lanes || col >= P.vcols || p0 >= last) return;
+    const uint64_t c0 = static_cast<uint64_t>(col) * V;
+    uint32_t keep = ~0u;
+    if (P.drop.threshold) keep = Draws<V>(gen, n * P.channels + c0).bits(P.drop.limit);
+    const uint64_t at = (n * P.row + p0) * P.channels + c0;
+    const T *res = static_cast<const T *>(P.residual);
+    drop_vectors<T, V>(reinterpret_cast<uint4 *>(nsm), static_cast<const T *>(P.x) + at, res == nullptr ? res : res + at,
+                       static_cast<T *>(P.y) + at, static_cast<long long>(P.lanes) * P.channels,
+                       static_cast<int>((last - p0 + P.lanes - 1) / P.lanes),
+                       [&](int, const Lanes<V> &v) { return drop_lanes<V>(v, keep, P.drop); });
+}
+
+// A warp takes a chunk of one channel's pixels, with single elements up to the
+// first 16-byte boundary and behind the last (V > 1: the bases of the three
+// tensors are aligned).
+template <class T, int V>
+__global__ void __launch_bounds__(kStreamThreads, 3) plane_dropout_kernel(const __grid_constant__ DropoutParams P) {
+    extern __shared__ __align__(16) unsigned char nsm[];
+    griddep_wait();
+    griddep_launch_dependents();
+    const Philox gen(P.drop, blockIdx.x == 0 && threadIdx.x == 0);
+    const T *x = static_cast<const T *>(P.x), *res = static_cast<const T *>(P.residual);
+    T *y = static_cast<T *>(P.y);
+    const int lane = threadIdx.x & 31;
+    const uint64_t warps = static_cast<uint64_t>(gridDim.x) * (kStreamThreads / 32);
+    for (uint64_t item = static_cast<uint64_t>(blockIdx.x) * (kStreamThreads / 32) + threadIdx.x / 32;
+         item < P.decisions * P.chunks; item += warps) {
+        const uint64_t j = item / P.chunks, p0 = (item - j * P.chunks) * P.chunk;
+        const uint64_t begin = j * P.row + p0, end = j * P.row + min(P.row, p0 + P.chunk);
+        const uint32_t keep = P.drop.threshold == 0 || Draws<1>(gen, j).keep(0, P.drop.limit) ? ~0u : 0u;
+        const uint64_t low = min(end, (begin + V - 1) / V * V), high = max(low, end / V * V), i0 = low + lane * V;
+        auto single = [&](uint64_t i) {  // fewer than a warp's lanes on either side
+            float v = keep ? to_float(x[i]) * P.drop.scale : 0.0f;
+            if (res != nullptr) v += to_float(res[i]);
+            y[i] = from_float<T>(v);
+        };
+        if (begin + lane < low) single(begin + lane);
+        if (high + lane < end) single(high + lane);
+        const int count = i0 < high ? static_cast<int>((high - i0 + 32 * V - 1) / (32 * V)) : 0;
+        drop_vectors<T, V>(reinterpret_cast<uint4 *>(nsm), x + i0, res == nullptr ? res : res + i0, y + i0, 32 * V, count,
+                           [&](int, const Lanes<V> &v) { return drop_lanes<V>(v, keep, P.drop); });
+        cp_async_wait<0>();  // the ring is used again
     }
 }
 

@@ -29,8 +29,8 @@
 
 namespace gcb {
 
-constexpr int kNormThreads = 256;      // split path
-constexpr int kResidentThreads = 512;  // resident path, at most
+constexpr int kNormThreads = kStreamThreads;  // split path
+constexpr int kResidentThreads = 512;         // resident path, at most
 
 struct NormParams {
     const void *x, *dy;
@@ -160,38 +160,10 @@ __device__ __forceinline__ void channel_sums(int vr, int lanes, int cb, int at, 
 }
 
 // ---- split path ----------------------------------------------------------------------------
-// A block streams a chunk of pixels of up to 256 vector columns.  16-byte
-// vectors go through a ring in shared memory that is private to each thread
-// (kRing copies in flight, no barrier); single elements are loaded kAhead at a
-// time.
-constexpr int kRing = 16, kAhead = 8;
-__device__ __forceinline__ void copy_vector(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-
-// Raw elements as loaded: 16 bytes, or one element.
-template <class T, int V>
-struct Raw {
-    uint4 u;
-};
-template <class T>
-struct Raw<T, 1> {
-    T u;
-};
-template <class T, int V>
-__device__ __forceinline__ Raw<T, V> load_raw(const T *p) {
-    Raw<T, V> r;
-    if constexpr (V == 1) r.u = *p;
-    else r.u = __ldg(reinterpret_cast<const uint4 *>(p));
-    return r;
-}
-template <class T, int V>
-__device__ __forceinline__ Lanes<V> lanes_of_raw(const Raw<T, V> &r) {
-    float v[V];
-    if constexpr (V == 1) v[0] = to_float(r.u);
-    else unpack(r.u, v, static_cast<const T *>(nullptr));
-    return lanes_of<V>(v);
-}
+// A block streams a chunk of pixels of up to 256 vector columns.  Blocks per
+// SM: what the rings of shared memory and the registers of the vector kernels
+// allow; single elements need more threads to keep as many bytes in flight.
+__host__ __device__ constexpr int split_blocks(int v, bool backward) { return v == 1 ? 4 : backward ? 2 : 3; }
 
 struct SplitPlace {
     long long n, p0;  // image, first pixel of the thread
@@ -218,107 +190,6 @@ __device__ __forceinline__ SplitPlace split_place(const NormParams &P, int v) {
     s.c0 = active ? s.first + s.col * v : 0;
     return s;
 }
-
-// Calls f(k, vector) for a thread's vectors.  ring: kRing * kNormThreads
-// vectors of shared memory (V > 1).  start_vectors issues the first copies and
-// may run before the wait for an earlier launch that does not write the data.
-template <int V, class T>
-__device__ __forceinline__ void start_vectors(uint4 *ring, const T *p, long long step, int count) {
-    if constexpr (V > 1) {
-        const uint32_t addr = smem_addr(ring + threadIdx.x);
-#pragma unroll
-        for (int u = 0; u < kRing; ++u, p += step) {
-            if (u < count) copy_vector(addr + u * kNormThreads * sizeof(uint4), p);
-            cp_async_commit();
-        }
-    }
-}
-template <class T, int V, class F>
-__device__ __forceinline__ void for_vectors(uint4 *ring, const T *p, long long step, int count, F f) {
-    if constexpr (V == 1) {
-        for (int k = 0; k < count; k += kAhead) {
-            Raw<T, V> raw[kAhead];
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u, p += step)
-                if (k + u < count) raw[u] = load_raw<T, V>(p);
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u)
-                if (k + u < count) f(k + u, lanes_of_raw<T, V>(raw[u]));
-        }
-    } else {
-        const uint4 *mine = ring + threadIdx.x;
-        const uint32_t addr = smem_addr(mine);
-        constexpr uint32_t kPitch = kNormThreads * sizeof(uint4);
-        p += kRing * step;
-#pragma unroll 4
-        for (int k = 0; k < count; ++k, p += step) {
-            const int slot = k % kRing;
-            cp_async_wait<kRing - 1>();
-            const Lanes<V> v = unpack_lanes<T, V>(mine[slot * kNormThreads], p);
-            if (k + kRing < count) copy_vector(addr + slot * kPitch, p);
-            cp_async_commit();
-            f(k, v);
-        }
-    }
-}
-// The same for two tensors: f(k, vector of p, vector of q).
-template <int V, class T>
-__device__ __forceinline__ void start_vector_pairs(uint4 *ring, const T *p, long long pstep, const T *q, long long qstep,
-                                                   int count) {
-    if constexpr (V > 1) {
-        const uint32_t addr = smem_addr(ring + threadIdx.x);
-        constexpr uint32_t kPitch = kNormThreads * sizeof(uint4);
-#pragma unroll
-        for (int u = 0; u < kRing / 2; ++u, p += pstep, q += qstep) {
-            if (u < count) {
-                copy_vector(addr + 2 * u * kPitch, p);
-                copy_vector(addr + (2 * u + 1) * kPitch, q);
-            }
-            cp_async_commit();
-        }
-    }
-}
-template <class T, int V, class F>
-__device__ __forceinline__ void for_vector_pairs(uint4 *ring, const T *p, long long pstep, const T *q, long long qstep,
-                                                 int count, F f) {
-    if constexpr (V == 1) {
-        constexpr int kPair = kAhead / 2;
-        for (int k = 0; k < count; k += kPair) {
-            Raw<T, V> a[kPair], b[kPair];
-#pragma unroll
-            for (int u = 0; u < kPair; ++u, p += pstep, q += qstep)
-                if (k + u < count) {
-                    a[u] = load_raw<T, V>(p);
-                    b[u] = load_raw<T, V>(q);
-                }
-#pragma unroll
-            for (int u = 0; u < kPair; ++u)
-                if (k + u < count) f(k + u, lanes_of_raw<T, V>(a[u]), lanes_of_raw<T, V>(b[u]));
-        }
-    } else {
-        constexpr int kHalf = kRing / 2;
-        const uint4 *mine = ring + threadIdx.x;
-        const uint32_t addr = smem_addr(mine);
-        constexpr uint32_t kPitch = kNormThreads * sizeof(uint4);
-        p += kHalf * pstep;
-        q += kHalf * qstep;
-#pragma unroll 2
-        for (int k = 0; k < count; ++k, p += pstep, q += qstep) {
-            const int slot = 2 * (k % kHalf);
-            cp_async_wait<kHalf - 1>();
-            const Lanes<V> v = unpack_lanes<T, V>(mine[slot * kNormThreads], p);
-            const Lanes<V> g = unpack_lanes<T, V>(mine[(slot + 1) * kNormThreads], p);
-            if (k + kHalf < count) {
-                copy_vector(addr + slot * kPitch, p);
-                copy_vector(addr + (slot + 1) * kPitch, q);
-            }
-            cp_async_commit();
-            f(k, v, g);
-        }
-    }
-}
-// Bytes of the ring.
-__host__ __device__ inline size_t ring_space(int v) { return v == 1 ? 0 : kRing * kNormThreads * sizeof(uint4); }
 
 // Moments of a thread's values of one channel each: sums about a pivot, which
 // is the first of at most 64 values.  As one of the values it lies so near the
@@ -373,7 +244,7 @@ struct Moments {
 // Per chunk and channel: mean and squares about it.  The threads' moments are
 // moved to one pivot per channel, the mean of pixel lane 0, and then add up.
 template <class T, int V>
-__global__ void __launch_bounds__(kNormThreads, 3) norm_moments_kernel(const __grid_constant__ NormParams P) {
+__global__ void __launch_bounds__(kNormThreads, split_blocks(V, false)) norm_moments_kernel(const __grid_constant__ NormParams P) {
     extern __shared__ __align__(16) unsigned char nsm[];
     uint4 *ring = reinterpret_cast<uint4 *>(nsm);
     float *pivot = reinterpret_cast<float *>(nsm + ring_space(V));  // [width]
@@ -498,24 +369,24 @@ __device__ __forceinline__ Coefs<V> split_coefs(const NormParams &P, long long n
     return {lanes_of<V>(mean), lanes_of<V>(a), lanes_of<V>(b)};
 }
 
-// Dropout decisions of a thread's vectors, pixel by pixel.
+// Dropout of a thread's vectors, pixel by pixel.
 template <int V, bool DROP>
 struct Keeper {
-    DropState ds;
-    uint32_t keep = ~0u;
+    Philox gen;
+    Draws<V> draws;
     uint64_t at, step;
     __device__ __forceinline__ Keeper(const NormParams &P, bool writer, long long n, long long p0, int c0, int lanes) {
         if (!DROP) return;
-        ds = drop_state(P.drop, writer);
+        gen = Philox(P.drop, writer);
         at = (static_cast<uint64_t>(n) * P.px + p0) * P.c + c0;
         step = static_cast<uint64_t>(static_cast<long long>(lanes) * P.c);  // modulo 2^64 where it goes down
-        if (P.drop.channel) keep = keep_bits<V>(P.drop, ds, static_cast<uint64_t>(n) * P.c + c0);
+        if (P.drop.channel) draws = Draws<V>(gen, static_cast<uint64_t>(n) * P.c + c0);
     }
     __device__ __forceinline__ Lanes<V> apply(const NormParams &P, const Lanes<V> &v) {
         if (!DROP) return v;
-        if (!P.drop.channel) keep = keep_bits<V>(P.drop, ds, at);
+        if (!P.drop.channel) draws = Draws<V>(gen, at);
         at += step;
-        return keep_lanes<V>(v, keep, P.drop.scale);
+        return drop_lanes<V>(v, draws, P.drop);
     }
 };
 
@@ -524,7 +395,7 @@ struct Keeper {
 // is not written by the launches that this one follows, so its first copies
 // are issued before the wait for their results.
 template <class T, int V, int ACT, bool DROP>
-__global__ void __launch_bounds__(kNormThreads, 3) norm_apply_kernel(const __grid_constant__ NormParams P) {
+__global__ void __launch_bounds__(kNormThreads, DROP ? 2 : split_blocks(V, false)) norm_apply_kernel(const __grid_constant__ NormParams P) {
     extern __shared__ __align__(16) unsigned char nsm[];
     uint4 *ring = reinterpret_cast<uint4 *>(nsm);
     const SplitPlace at = split_place(P, V);
@@ -579,7 +450,7 @@ __device__ __forceinline__ Lanes<V> grad_result(int act, const Coefs<V> &k, cons
 
 // Per chunk and channel: sum dz, sum dz (x - mean).
 template <class T, int V, int ACT, bool DROP>
-__global__ void __launch_bounds__(kNormThreads, 2) norm_grad_sums_kernel(const __grid_constant__ NormParams P) {
+__global__ void __launch_bounds__(kNormThreads, DROP ? 2 : split_blocks(V, true)) norm_grad_sums_kernel(const __grid_constant__ NormParams P) {
     extern __shared__ __align__(16) unsigned char nsm[];
     griddep_wait();
     griddep_launch_dependents();
@@ -661,7 +532,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_finalize_kernel(const 
 
 // The second pass over x and dy, like norm_apply_kernel.
 template <class T, int V, int ACT, bool DROP>
-__global__ void __launch_bounds__(kNormThreads, 2) norm_grad_apply_kernel(const __grid_constant__ NormParams P) {
+__global__ void __launch_bounds__(kNormThreads, DROP ? 2 : split_blocks(V, true)) norm_grad_apply_kernel(const __grid_constant__ NormParams P) {
     extern __shared__ __align__(16) unsigned char nsm[];
     uint4 *ring = reinterpret_cast<uint4 *>(nsm);
     const SplitPlace at = split_place(P, V);
@@ -809,8 +680,8 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_kernel(cons
     const uint32_t tile_addr = smem_addr(tile_at), pitch = 16 * threads;
     griddep_wait();
     griddep_launch_dependents();
-    DropState ds{};
-    if (DROP) ds = drop_state(P.drop, blockIdx.x == 0 && tid == 0);
+    Philox gen;
+    if (DROP) gen = Philox(P.drop, blockIdx.x == 0 && tid == 0);
     const long long xstep = static_cast<long long>(P.lanes) * P.x_ldp, ystep = static_cast<long long>(P.lanes) * P.y_ldp;
     const T *x = static_cast<const T *>(P.x) + (unit / P.bundles) * P.x_ldn + r.p0 * P.x_ldp + r.c0;
     {
@@ -978,8 +849,8 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_kernel(cons
             coefs.a = lanes_of<V>(a);
         }
         T *y = static_cast<T *>(P.y) + n * P.y_ldn + r.p0 * P.y_ldp + r.c0;
-        uint32_t keep = ~0u;
-        if (DROP && P.drop.channel) keep = keep_bits<V>(P.drop, ds, static_cast<uint64_t>(n) * P.c + r.c0);
+        Draws<V> draws;
+        if (DROP && P.drop.channel) draws = Draws<V>(gen, static_cast<uint64_t>(n) * P.c + r.c0);
         uint64_t at = (static_cast<uint64_t>(n) * P.px + r.p0) * P.c + r.c0;
         const bool more = n + P.stride < P.n;
         x += P.stride * P.x_ldn;
@@ -1001,9 +872,9 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_kernel(cons
                     v.p[i] = activate<ACT>(P.act, normalise<V>(coefs, i, v.p[i], d));
                 }
                 if (DROP) {
-                    if (!P.drop.channel) keep = keep_bits<V>(P.drop, ds, at);
+                    if (!P.drop.channel) draws = Draws<V>(gen, at);
                     at += static_cast<uint64_t>(P.lanes) * P.c;
-                    v = keep_lanes<V>(v, keep, P.drop.scale);
+                    v = drop_lanes<V>(v, draws, P.drop);
                 }
                 store_lanes<T, V>(y, v);
             }
@@ -1039,8 +910,8 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
     const uint32_t x_addr = smem_addr(x_at), g_addr = smem_addr(g_at), pitch = 16 * threads;
     griddep_wait();
     griddep_launch_dependents();
-    DropState ds{};
-    if (DROP) ds = drop_state(P.drop, blockIdx.x == 0 && tid == 0);
+    Philox gen;
+    if (DROP) gen = Philox(P.drop, blockIdx.x == 0 && tid == 0);
     const long long xstep = static_cast<long long>(P.lanes) * P.x_ldp;
     const long long gstep = static_cast<long long>(P.lanes) * P.dy_ldp;
     const long long ystep = static_cast<long long>(P.lanes) * P.y_ldp;
@@ -1088,7 +959,7 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
 #pragma unroll
         for (int i = 0; i < Lanes<V>::kPairs; ++i) s2.p[i] = t2.p[i] = pair(0.0f);
         uint32_t keep = ~0u;
-        if (DROP && P.drop.channel) keep = keep_bits<V>(P.drop, ds, static_cast<uint64_t>(n) * P.c + r.c0);
+        if (DROP && P.drop.channel) keep = Draws<V>(gen, static_cast<uint64_t>(n) * P.c + r.c0).bits(P.drop.limit);
         uint64_t at = (static_cast<uint64_t>(n) * P.px + r.p0) * P.c + r.c0;
         int k = 0;
 #pragma unroll
@@ -1101,11 +972,11 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
                 Lanes<V> g = unpack_lanes<T, V>(g_at[k * threads], x);
                 if (DROP) {
                     if (!P.drop.channel) {
-                        keep = keep_bits<V>(P.drop, ds, at);
+                        keep = Draws<V>(gen, at).bits(P.drop.limit);
                         bits[k * threads + tid] = static_cast<uint8_t>(keep);
                     }
                     at += static_cast<uint64_t>(P.lanes) * P.c;
-                    g = keep_lanes<V>(g, keep, P.drop.scale);
+                    g = drop_lanes<V>(g, keep, P.drop);
                 }
                 grad_sums<V, ACT>(P.act, coefs, v, g, s2, t2);
             }
@@ -1189,7 +1060,7 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
                 }
                 if (DROP) {
                     if (!P.drop.channel) keep = bits[k * threads + tid];
-                    g = keep_lanes<V>(g, keep, P.drop.scale);
+                    g = drop_lanes<V>(g, keep, P.drop);
                 }
                 store_lanes<T, V>(dx, grad_result<V, ACT>(P.act, coefs, mk1, mk2, v, g));
             }

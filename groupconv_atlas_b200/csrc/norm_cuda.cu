@@ -181,6 +181,7 @@ int check_dropout(const gc_b200_dropout_args *d, DropParams &out) {
             if (p != nullptr && ranges_meet(d->used, 16, p, 8))
                 return gc_error(GC_INVALID, "the words in use must not overwrite the given ones");
     out.threshold = static_cast<uint32_t>(std::nearbyint(65536.0 * d->p));
+    out.limit = out.threshold != 0 ? (out.threshold << 16) - 1u : 0u;  // 65536 wraps to all ones: nothing is above
     out.scale = out.threshold < 65536 ? static_cast<float>(65536.0 / (65536.0 - out.threshold)) : 0.0f;
     out.channel = d->scope == GC_B200_DROP_CHANNEL;
     out.seed = d->seed;
@@ -231,8 +232,7 @@ bool vector_access(std::initializer_list<const View *> views) {
 }
 
 // The split path's work split: blocks of up to 256 vector columns and chunks
-// of pixels such that one wave of blocks (three per SM, two in the gradient)
-// streams everything, but at least eight pixels for each thread.  (Launching
+// of pixels such that one wave of blocks streams everything, but at least eight pixels for each thread.  (Launching
 // sets of images small enough for the second pass to find them in the L2 cache
 // was slower: a set's three launches cost about 10 us beside its data, N8 C128
 // 256x256 bf16 forward 78 us in one set, 108 us in four.)
@@ -241,7 +241,7 @@ void plan_split(NormParams &P, int v, bool backward, int sms) {
     P.cblocks = static_cast<int>(ceil_div(P.vcols, gcb::kNormThreads));
     P.vb = static_cast<int>(ceil_div(P.vcols, P.cblocks));
     P.lanes = gcb::kNormThreads / P.vb;
-    const long long wanted = std::max<long long>(1, (backward ? 2LL : 3LL) * sms / (P.n * P.cblocks));
+    const long long wanted = std::max<long long>(1, static_cast<long long>(gcb::split_blocks(v, backward)) * sms / (P.n * P.cblocks));
     P.chunk_rows = std::min(P.px, std::max<long long>(ceil_div(P.px, wanted), 8LL * P.lanes));
     P.chunks = static_cast<int>(ceil_div(P.px, P.chunk_rows));
     P.items = P.n * P.chunks * P.cblocks;
@@ -630,13 +630,16 @@ bool channels_last_order(const gc_tensor *t) {
     return t->dims[0] <= 1 || t->strides[0] == expect;
 }
 
+enum DropoutKernel { kElements, kChannels, kPlanes };
+template <class T, int V>
+const void *dropout_instance(DropoutKernel k) {
+    return k == kElements   ? reinterpret_cast<const void *>(&gcb::dropout_kernel<T, V>)
+           : k == kChannels ? reinterpret_cast<const void *>(&gcb::channel_dropout_kernel<T, V>)
+                            : reinterpret_cast<const void *>(&gcb::plane_dropout_kernel<T, V>);
+}
 template <class T>
-const void *dropout_typed(bool vec, bool channel) {
-    if (channel)
-        return vec ? reinterpret_cast<const void *>(&gcb::dropout_kernel<T, true, true>)
-                   : reinterpret_cast<const void *>(&gcb::dropout_kernel<T, false, true>);
-    return vec ? reinterpret_cast<const void *>(&gcb::dropout_kernel<T, true, false>)
-               : reinterpret_cast<const void *>(&gcb::dropout_kernel<T, false, false>);
+const void *dropout_typed(DropoutKernel k, bool vec) {
+    return vec ? dropout_instance<T, gcb::kVec<T>>(k) : dropout_instance<T, 1>(k);
 }
 
 }  // namespace
@@ -846,33 +849,63 @@ int gc_b200_dropout(const gc_tensor *x, const gc_tensor *residual, gc_tensor *y,
                 if (x->dims[i] > 1 && t->strides[i] != x->strides[i])
                     return gc_error(GC_UNSUPPORTED, "tensors must have the same strides");
     if (!dense_any_order(x)) return gc_error(GC_UNSUPPORTED, "tensors must be dense");
-    DropoutParams P{};
-    if (drop.channel) {
-        const bool plain = plain_order(x);
-        if (!plain && !channels_last_order(x))
-            return gc_error(GC_UNSUPPORTED, "channel dropout needs plain or channels-last order");
-        P.channels = static_cast<uint64_t>(x->dims[1]);
-        P.image = static_cast<uint64_t>(count / x->dims[0]);
-        P.inner = plain ? P.image / P.channels : 1;
-    }
+    const bool plain = plain_order(x);
+    if (drop.channel && !plain && !channels_last_order(x))
+        return gc_error(GC_UNSUPPORTED, "channel dropout needs plain or channels-last order");
     int dev = -1;
     st = check_call({x, y, residual}, {drop.seed_ptr, drop.offset_ptr, drop.used}, x->device_index, stream, dev);
     if (st != GC_OK) return st;
+    gcb::DeviceFacts facts;
+    if ((st = gcb::device_facts(dev, facts)) != GC_OK) return st;
+    DropoutParams P{};
     P.x = x->data;
     P.residual = residual != nullptr ? residual->data : nullptr;
     P.y = y->data;
     P.count = static_cast<uint64_t>(count);
-    P.groups = (P.count + 7) / 8;
     P.drop = drop;
-    const bool vec = gcb::aligned16(P.x) && gcb::aligned16(P.y) && gcb::aligned16(P.residual);
-    const int type = elem_type(x->dtype);
-    const void *fn = type == gcb::kElemF16    ? dropout_typed<__half>(vec, drop.channel)
-                     : type == gcb::kElemBF16 ? dropout_typed<__nv_bfloat16>(vec, drop.channel)
-                                              : dropout_typed<float>(vec, drop.channel);
-    const unsigned grid = grid_of(ceil_div(static_cast<long long>(P.groups), 256));
+    bool vec = gcb::aligned16(P.x) && gcb::aligned16(P.y) && gcb::aligned16(P.residual);
+    const int type = elem_type(x->dtype), per_vector = type == gcb::kElemF32 ? 4 : 8;
+    DropoutKernel kind = kElements;
+    const long long wave = 3LL * facts.sms, threads = gcb::kStreamThreads;  // one wave of blocks
+    long long grid = std::min<long long>(ceil_div(count, threads * (vec ? per_vector : 1)), wave);
+    if (drop.channel) {
+        const long long images = x->dims[0], channels = x->dims[1], px = count / images / channels;
+        if (channels > INT32_MAX) return gc_error(GC_UNSUPPORTED, "channel count out of range");
+        P.decisions = static_cast<uint64_t>(images * channels);
+        P.channels = static_cast<int>(channels);
+        P.row = static_cast<uint64_t>(px);
+        if (plain && px > 1) {
+            kind = kPlanes;
+            const long long warps = threads / 32, least = 32LL * (vec ? 4 * per_vector : gcb::kAhead);
+            const long long wanted = std::max<long long>(1, wave * warps / (images * channels));
+            P.chunk = static_cast<uint64_t>(gcb::round_up(ceil_div(px, wanted), least));
+            P.chunks = (P.row + P.chunk - 1) / P.chunk;
+            grid = static_cast<long long>(
+                std::min<uint64_t>((P.decisions * P.chunks + warps - 1) / warps, static_cast<uint64_t>(wave)));
+        } else {
+            kind = kChannels;
+            vec = vec && channels % per_vector == 0;
+            P.vcols = static_cast<int>(vec ? channels / per_vector : channels);
+            P.cblocks = static_cast<int>(ceil_div(P.vcols, threads));
+            P.vb = static_cast<int>(ceil_div(P.vcols, P.cblocks));
+            P.lanes = static_cast<int>(threads / P.vb);
+            const long long wanted = std::max<long long>(1, wave / (images * P.cblocks));
+            P.chunk = static_cast<uint64_t>(std::max<long long>(ceil_div(px, wanted), 4LL * P.lanes));
+            P.chunks = (P.row + P.chunk - 1) / P.chunk;
+            const wide blocks = static_cast<wide>(images) * static_cast<wide>(P.chunks) * P.cblocks;
+            if (blocks > INT32_MAX) return gc_error(GC_UNSUPPORTED, "more images than a grid has blocks");
+            grid = static_cast<long long>(blocks);
+        }
+    }
+    const void *fn = type == gcb::kElemF16    ? dropout_typed<__half>(kind, vec)
+                     : type == gcb::kElemBF16 ? dropout_typed<__nv_bfloat16>(kind, vec)
+                                              : dropout_typed<float>(kind, vec);
+    if ((st = prepare_kernel(fn, dev, facts.smem_optin)) != GC_OK) return st;
     void *args[] = {&P};
-    const cudaError_t e = gcb::launch_pdl(fn, dim3(grid), dim3(256), args, 0, reinterpret_cast<cudaStream_t>(stream));
-    gcb::record_plan(PlanRecord::kDropout, drop.channel ? "channel" : "element", false, grid, 256, vec ? 1 : 0);
+    const cudaError_t e = gcb::launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(gcb::kStreamThreads), args,
+                                          gcb::ring_space(vec ? per_vector : 1), reinterpret_cast<cudaStream_t>(stream));
+    static const char *const names[] = {"element", "channels_last", "planes"};
+    gcb::record_plan(PlanRecord::kDropout, names[kind], false, grid, gcb::kStreamThreads, vec ? 1 : 0);
     return launched(e);
 }
 

@@ -184,15 +184,141 @@ __device__ __forceinline__ void store_lanes(T *p, const Lanes<V> &l) {
     values_of<V>(l, v);
     store_elems<T, V>(p, v);
 }
-// Kept values scaled, the others 0 whatever they hold.
-template <int V>
-__device__ __forceinline__ Lanes<V> keep_lanes(const Lanes<V> &l, uint32_t bits, float scale) {
+// ---- streaming ------------------------------------------------------------------------
+// A thread of a 256-thread block walks over vectors that lie a fixed step
+// apart.  16-byte vectors go through a ring in shared memory that is private
+// to the thread (kRing copies in flight, no barrier: a read-only stream at
+// 6.4 TB/s, where batches of eight register loads reached 5.5); single
+// elements are loaded kAhead at a time.
+constexpr int kStreamThreads = 256, kRing = 16, kAhead = 16;
+__device__ __forceinline__ void copy_vector(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// Raw elements as loaded: 16 bytes, or one element.
+template <class T, int V>
+struct Raw {
+    uint4 u;
+};
+template <class T>
+struct Raw<T, 1> {
+    T u;
+};
+template <class T, int V>
+__device__ __forceinline__ Raw<T, V> load_raw(const T *p) {
+    Raw<T, V> r;
+    if constexpr (V == 1) r.u = *p;
+    else r.u = __ldg(reinterpret_cast<const uint4 *>(p));
+    return r;
+}
+template <class T, int V>
+__device__ __forceinline__ Lanes<V> lanes_of_raw(const Raw<T, V> &r) {
     float v[V];
-    values_of<V>(l, v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = bits >> j & 1u ? v[j] * scale : 0.0f;
+    if constexpr (V == 1) v[0] = to_float(r.u);
+    else unpack(r.u, v, static_cast<const T *>(nullptr));
     return lanes_of<V>(v);
 }
+
+// Calls f(k, vector) for a thread's vectors.  ring: kRing * kStreamThreads
+// vectors of shared memory (V > 1).  start_vectors issues the first copies and
+// may run before the wait for an earlier launch that does not write the data.
+template <int V, class T>
+__device__ __forceinline__ void start_vectors(uint4 *ring, const T *p, long long step, int count) {
+    if constexpr (V > 1) {
+        const uint32_t addr = smem_addr(ring + threadIdx.x);
+#pragma unroll
+        for (int u = 0; u < kRing; ++u, p += step) {
+            if (u < count) copy_vector(addr + u * kStreamThreads * sizeof(uint4), p);
+            cp_async_commit();
+        }
+    }
+}
+template <class T, int V, class F>
+__device__ __forceinline__ void for_vectors(uint4 *ring, const T *p, long long step, int count, F f) {
+    if constexpr (V == 1) {
+        for (int k = 0; k < count; k += kAhead) {
+            Raw<T, V> raw[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u, p += step)
+                if (k + u < count) raw[u] = load_raw<T, V>(p);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (k + u < count) f(k + u, lanes_of_raw<T, V>(raw[u]));
+        }
+    } else {
+        const uint4 *mine = ring + threadIdx.x;
+        const uint32_t addr = smem_addr(mine);
+        constexpr uint32_t kPitch = kStreamThreads * sizeof(uint4);
+        p += kRing * step;
+#pragma unroll 4
+        for (int k = 0; k < count; ++k, p += step) {
+            const int slot = k % kRing;
+            cp_async_wait<kRing - 1>();
+            const Lanes<V> v = unpack_lanes<T, V>(mine[slot * kStreamThreads], p);
+            if (k + kRing < count) copy_vector(addr + slot * kPitch, p);
+            cp_async_commit();
+            f(k, v);
+        }
+    }
+}
+// The same for two tensors: f(k, vector of p, vector of q).
+template <int V, class T>
+__device__ __forceinline__ void start_vector_pairs(uint4 *ring, const T *p, long long pstep, const T *q, long long qstep,
+                                                   int count) {
+    if constexpr (V > 1) {
+        const uint32_t addr = smem_addr(ring + threadIdx.x);
+        constexpr uint32_t kPitch = kStreamThreads * sizeof(uint4);
+#pragma unroll
+        for (int u = 0; u < kRing / 2; ++u, p += pstep, q += qstep) {
+            if (u < count) {
+                copy_vector(addr + 2 * u * kPitch, p);
+                copy_vector(addr + (2 * u + 1) * kPitch, q);
+            }
+            cp_async_commit();
+        }
+    }
+}
+template <class T, int V, class F>
+__device__ __forceinline__ void for_vector_pairs(uint4 *ring, const T *p, long long pstep, const T *q, long long qstep,
+                                                 int count, F f) {
+    if constexpr (V == 1) {
+        constexpr int kPair = kAhead / 2;
+        for (int k = 0; k < count; k += kPair) {
+            Raw<T, V> a[kPair], b[kPair];
+#pragma unroll
+            for (int u = 0; u < kPair; ++u, p += pstep, q += qstep)
+                if (k + u < count) {
+                    a[u] = load_raw<T, V>(p);
+                    b[u] = load_raw<T, V>(q);
+                }
+#pragma unroll
+            for (int u = 0; u < kPair; ++u)
+                if (k + u < count) f(k + u, lanes_of_raw<T, V>(a[u]), lanes_of_raw<T, V>(b[u]));
+        }
+    } else {
+        constexpr int kHalf = kRing / 2;
+        const uint4 *mine = ring + threadIdx.x;
+        const uint32_t addr = smem_addr(mine);
+        constexpr uint32_t kPitch = kStreamThreads * sizeof(uint4);
+        p += kHalf * pstep;
+        q += kHalf * qstep;
+#pragma unroll 2
+        for (int k = 0; k < count; ++k, p += pstep, q += qstep) {
+            const int slot = 2 * (k % kHalf);
+            cp_async_wait<kHalf - 1>();
+            const Lanes<V> v = unpack_lanes<T, V>(mine[slot * kStreamThreads], p);
+            const Lanes<V> g = unpack_lanes<T, V>(mine[(slot + 1) * kStreamThreads], p);
+            if (k + kHalf < count) {
+                copy_vector(addr + slot * kPitch, p);
+                copy_vector(addr + (slot + 1) * kPitch, q);
+            }
+            cp_async_commit();
+            f(k, v, g);
+        }
+    }
+}
+// Bytes of the ring.
+__host__ __device__ inline size_t ring_space(int v) { return v == 1 ? 0 : kRing * kStreamThreads * sizeof(uint4); }
 
 // ---- activations --------------------------------------------------------------------
 // 1 / (1 + 2^(-z log2 e)) of two values with three of the special-function
@@ -247,81 +373,113 @@ __device__ __forceinline__ f2 activate_grad(int act, f2 z, f2 g) {
 }
 
 // ---- dropout ------------------------------------------------------------------------
-// Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy
-// as 1, 2, 3", 2011): ten rounds of two 32 x 32 -> 64 bit products.  Sixteen
-// bits a decision make one call serve eight elements: the ten rounds are about
-// 50 instructions, and with 32 bits a decision the generator, not the memory,
-// would bound 16-bit tensors.
-__device__ __forceinline__ uint4 philox(uint64_t block, uint64_t offset, uint64_t seed) {
-    uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32);
-    uint32_t c2 = static_cast<uint32_t>(offset), c3 = static_cast<uint32_t>(offset >> 32);
-    uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
-#pragma unroll
-    for (int r = 0; r < 10; ++r) {
-        const uint64_t a = static_cast<uint64_t>(c0) * 0xD2511F53u;
-        const uint64_t b = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
-        c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k0;
-        c1 = static_cast<uint32_t>(b);
-        c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k1;
-        c3 = static_cast<uint32_t>(a);
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
-    }
-    return make_uint4(c0, c1, c2, c3);
-}
-
 struct DropParams {
-    uint32_t threshold;  // keep when the 16-bit draw is at least this; 0 = keep all, 65536 = drop all
-    float scale;         // 1 / (1 - threshold / 65536), 0 when everything is dropped
+    uint32_t threshold;  // t: keep when the 16-bit draw is at least this; 0 = no dropout, 65536 = drop all
+    uint32_t limit;      // 65536 t - 1: the draw in a word's upper half is kept when the word is above it
+    float scale;         // 1 / (1 - t / 65536), 0 when everything is dropped
     int channel;         // one decision per channel of an image
     uint64_t seed, offset;
     const uint64_t *seed_ptr, *offset_ptr;  // nullable, added to seed and offset
     uint64_t *used;                         // nullable, receives what is in effect
 };
 
-struct DropState {
-    uint64_t seed, offset;
+// Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy
+// as 1, 2, 3", 2011): ten rounds of two 32 x 32 -> 64 bit products.  Sixteen
+// bits a decision make one block of four words serve eight elements: with 32
+// bits the generator, not the memory, would bound 16-bit tensors.  The first
+// product of the offset and the round keys are the same for every block of a
+// launch and are computed once; the keys are kept from being recomputed (an
+// integer addition takes as many issue slots as two of FP32).
+struct Philox {
+    uint32_t key[20], first, c3;  // first: high word of the first round's second product, keyed
+    uint32_t low;                 // its low word
+    __device__ __forceinline__ Philox() {}
+    // To be called after the wait for earlier launches (the words may be theirs).
+    __device__ __forceinline__ Philox(const DropParams &p, bool writer) {
+        uint64_t seed = p.seed, offset = p.offset;
+        if (p.seed_ptr != nullptr) seed += *p.seed_ptr;
+        if (p.offset_ptr != nullptr) offset += *p.offset_ptr;
+        if (writer && p.used != nullptr) {
+            p.used[0] = seed;
+            p.used[1] = offset;
+        }
+        uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
+#pragma unroll
+        for (int r = 0; r < 10; ++r) {
+            key[2 * r] = k0;
+            key[2 * r + 1] = k1;
+            asm("" : "+r"(key[2 * r]), "+r"(key[2 * r + 1]));
+            k0 += 0x9E3779B9u;
+            k1 += 0xBB67AE85u;
+        }
+        const uint64_t b = static_cast<uint64_t>(static_cast<uint32_t>(offset)) * 0xCD9E8D57u;
+        first = static_cast<uint32_t>(b >> 32) ^ key[0];
+        low = static_cast<uint32_t>(b);
+        c3 = static_cast<uint32_t>(offset >> 32) ^ key[1];
+    }
+    __device__ __forceinline__ uint4 operator()(uint64_t block) const {
+        const uint64_t a = static_cast<uint64_t>(static_cast<uint32_t>(block)) * 0xD2511F53u;
+        uint32_t x0 = first ^ static_cast<uint32_t>(block >> 32), x1 = low;
+        uint32_t x2 = static_cast<uint32_t>(a >> 32) ^ c3, x3 = static_cast<uint32_t>(a);
+#pragma unroll
+        for (int r = 1; r < 10; ++r) {
+            const uint64_t u = static_cast<uint64_t>(x0) * 0xD2511F53u;
+            const uint64_t v = static_cast<uint64_t>(x2) * 0xCD9E8D57u;
+            x0 = static_cast<uint32_t>(v >> 32) ^ x1 ^ key[2 * r];
+            x1 = static_cast<uint32_t>(v);
+            x2 = static_cast<uint32_t>(u >> 32) ^ x3 ^ key[2 * r + 1];
+            x3 = static_cast<uint32_t>(u);
+        }
+        return make_uint4(x0, x1, x2, x3);
+    }
 };
 
-// To be called after the wait for earlier launches (the words may be theirs).
-__device__ __forceinline__ DropState drop_state(const DropParams &p, bool writer) {
-    DropState s{p.seed, p.offset};
-    if (p.seed_ptr != nullptr) s.seed += *p.seed_ptr;
-    if (p.offset_ptr != nullptr) s.offset += *p.offset_ptr;
-    if (writer && p.used != nullptr) {
-        p.used[0] = s.seed;
-        p.used[1] = s.offset;
-    }
-    return s;
-}
-
-// Keep bits (bit k: draw j0 + k) of V consecutive decisions; j0 is a multiple
-// of V and V divides 8, so that one block holds them all.
+// The draws of V consecutive decisions, two a word (V = 1: in the upper half).
 template <int V>
-__device__ __forceinline__ uint32_t keep_bits(const DropParams &p, const DropState &s, uint64_t j0) {
-    const uint4 w = philox(j0 >> 3, s.offset, s.seed);
-    const int first = static_cast<int>(j0 & 7);
-    uint32_t bits = 0;
-    if constexpr (V == 8) {
-        const uint32_t d[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            bits |= ((d[k] & 0xffffu) >= p.threshold ? 1u : 0u) << (2 * k);
-            bits |= ((d[k] >> 16) >= p.threshold ? 2u : 0u) << (2 * k);
+struct Draws {
+    uint32_t w[(V + 1) / 2];
+    // j0 is a multiple of V and V divides 8, so that one block holds them all.
+    __device__ __forceinline__ Draws(const Philox &gen, uint64_t j0) {
+        const uint4 b = gen(j0 >> 3);
+        const int at = static_cast<int>(j0 & 7);
+        if constexpr (V == 8) {
+            w[0] = b.x, w[1] = b.y, w[2] = b.z, w[3] = b.w;
+        } else if constexpr (V == 4) {
+            w[0] = at ? b.z : b.x, w[1] = at ? b.w : b.y;
+        } else {
+            static_assert(V == 1, "vectors of 8, 4 or 1");
+            const uint32_t d = at < 4 ? (at < 2 ? b.x : b.y) : (at < 6 ? b.z : b.w);
+            w[0] = at & 1 ? d : d << 16;
         }
-    } else if constexpr (V == 4) {
-        const uint32_t d[2] = {first ? w.z : w.x, first ? w.w : w.y};
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            bits |= ((d[k] & 0xffffu) >= p.threshold ? 1u : 0u) << (2 * k);
-            bits |= ((d[k] >> 16) >= p.threshold ? 2u : 0u) << (2 * k);
-        }
-    } else {
-        static_assert(V == 1, "vectors of 8, 4 or 1");
-        const uint32_t d = first < 4 ? (first < 2 ? w.x : w.y) : (first < 6 ? w.z : w.w);
-        bits = ((first & 1 ? d >> 16 : d & 0xffffu) >= p.threshold) ? 1u : 0u;
     }
-    return bits;
+    __device__ __forceinline__ Draws() {}
+    __device__ __forceinline__ bool keep(int j, uint32_t limit) const {
+        return (V == 1 || (j & 1) ? w[j / 2] : w[j / 2] << 16) > limit;
+    }
+    __device__ __forceinline__ uint32_t bits(uint32_t limit) const {
+        uint32_t r = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) r |= keep(j, limit) ? 1u << j : 0u;
+        return r;
+    }
+};
+
+// Kept values scaled, the others 0 whatever they hold.
+template <int V>
+__device__ __forceinline__ Lanes<V> drop_lanes(const Lanes<V> &l, const Draws<V> &d, const DropParams &p) {
+    float v[V];
+    values_of<V>(l, v);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = d.keep(j, p.limit) ? v[j] * p.scale : 0.0f;
+    return lanes_of<V>(v);
+}
+template <int V>
+__device__ __forceinline__ Lanes<V> drop_lanes(const Lanes<V> &l, uint32_t bits, const DropParams &p) {
+    float v[V];
+    values_of<V>(l, v);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = bits >> j & 1u ? v[j] * p.scale : 0.0f;
+    return lanes_of<V>(v);
 }
 
 }  // namespace gcb
