@@ -11,14 +11,17 @@
 // gradients with autograd.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAGeneratorImpl.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
+#include <memory>
 #include <mutex>
 #include <stdexcept>
 #include <string>
-#include <tuple>
 #include <vector>
 
 #include "groupconv.h"
@@ -202,24 +205,14 @@ Drop make_drop(const at::Tensor &x, double p, int64_t scope, const c10::optional
     return d;
 }
 
-// What a gradient has to keep of a forward call's dropout, and that again.
-void save_drop(c10::IValue &out, const Drop &d) {
-    out = c10::IValue(std::tuple<bool, double, int64_t, int64_t, int64_t>(
-        d.on, d.args.p, d.args.scope, static_cast<int64_t>(d.args.seed), static_cast<int64_t>(d.args.offset)));
-}
-Drop load_drop(const c10::IValue &v, const at::Tensor &used) {
-    const auto &e = v.toTupleRef().elements();
-    Drop d;
-    d.on = e[0].toBool();
-    d.args.p = e[1].toDouble();
-    d.args.scope = static_cast<int32_t>(e[2].toInt());
-    if (used.defined()) {
-        const uint64_t *w = reinterpret_cast<const uint64_t *>(used.data_ptr<int64_t>());
+// The dropout again in the gradient: the words that were in effect.
+Drop again(Drop d) {
+    d.args.used = nullptr;
+    if (d.used.defined()) {
+        const uint64_t *w = reinterpret_cast<const uint64_t *>(d.used.data_ptr<int64_t>());
+        d.args.seed = d.args.offset = 0;
         d.args.seed_ptr = w;
         d.args.offset_ptr = w + 1;
-    } else {
-        d.args.seed = static_cast<uint64_t>(e[3].toInt());
-        d.args.offset = static_cast<uint64_t>(e[4].toInt());
     }
     return d;
 }
@@ -255,51 +248,56 @@ at::Tensor norm_forward(const at::Tensor &x, const at::Tensor &gamma, const at::
     return y;
 }
 
-struct GroupNorm : torch::autograd::Function<GroupNorm> {
-    static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x,
-                              const c10::optional<at::Tensor> &gamma, const c10::optional<at::Tensor> &beta,
-                              NormArgs a, Drop drop) {
-        const at::Tensor g = gamma.value_or(at::Tensor()), b = beta.value_or(at::Tensor());
-        at::Tensor stats = at::empty({x.size(0), a.groups, 2}, x.options().dtype(at::kFloat).memory_format(
-                                                                  at::MemoryFormat::Contiguous));
-        at::Tensor y = norm_forward(x, g, b, a, drop, stats);
-        ctx->save_for_backward({x, g, b, stats, drop.used});
-        ctx->saved_data["groups"] = a.groups;
-        ctx->saved_data["activation"] = a.activation;
-        save_drop(ctx->saved_data["drop"], drop);
-        return y;
+void no_forward_mode(const at::Tensor &t) {
+    if (t.defined() && t._fw_grad(/*level=*/0).defined())
+        throw std::runtime_error("this operation has no forward-mode derivative");
+}
+
+// The gradients are plain autograd nodes: a training step's host time counts,
+// and a torch::autograd::Function's context costs several microseconds of it.
+struct GroupNormGrad : torch::autograd::Node {
+    torch::autograd::SavedVariable x_, gamma_, beta_;
+    bool has_gamma_ = false, has_beta_ = false;
+    at::Tensor stats_;
+    NormArgs a_;
+    Drop drop_;
+
+    std::string name() const override { return "GroupNormGrad"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        x_.reset_data();
+        gamma_.reset_data();
+        beta_.reset_data();
     }
-    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
-                                                   torch::autograd::variable_list grads) {
+    torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
         no_double_backward();
-        const auto saved = ctx->get_saved_variables();
-        const at::Tensor &x = saved[0], &gamma = saved[1], &beta = saved[2], &stats = saved[3];
-        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
-        const Drop drop = load_drop(ctx->saved_data["drop"], saved[4]);
-        const int64_t groups = ctx->saved_data["groups"].toInt();
+        const at::Tensor x = x_.unpack(), gamma = has_gamma_ ? gamma_.unpack() : at::Tensor(),
+                         beta = has_beta_ ? beta_.unpack() : at::Tensor();
+        const Drop drop = again(drop_);
         c10::OptionalDeviceGuard guard(x.device());
         const at::Tensor dy = in_order(grads[0]);
         at::Tensor dx = empty_channels_last(x), dgamma, dbeta;
-        // needs_input_grad counts the tensors that were given
-        if (gamma.defined() && ctx->needs_input_grad(1)) dgamma = at::empty_like(gamma);
-        if (beta.defined() && ctx->needs_input_grad(gamma.defined() ? 2 : 1)) dbeta = at::empty_like(beta);
-        const gc_tensor xd = describe_view(x), dyd = describe_view(dy);
-        gc_tensor dxd = describe_view(dx), sd = describe_view(stats), gd{}, bd{}, dgd{}, dbd{};
-        if (gamma.defined()) gd = describe_view(gamma);
-        if (beta.defined()) bd = describe_view(beta);
+        if (has_gamma_ && task_should_compute_output(1)) dgamma = at::empty_like(gamma);
+        if (has_beta_ && task_should_compute_output(2)) dbeta = at::empty_like(beta);
+        const gc_tensor xd = describe_view(x), dyd = describe_view(dy), sd = describe_view(stats_);
+        gc_tensor dxd = describe_view(dx), gd{}, bd{}, dgd{}, dbd{};
+        if (has_gamma_) gd = describe_view(gamma);
+        if (has_beta_) bd = describe_view(beta);
         if (dgamma.defined()) dgd = describe_view(dgamma);
         if (dbeta.defined()) dbd = describe_view(dbeta);
         uint64_t bytes = 0;
-        int st = gc_b200_group_norm_backward_workspace(&dyd, &xd, &dxd, groups, &bytes);
+        int st = gc_b200_group_norm_backward_workspace(&dyd, &xd, &dxd, a_.groups, &bytes);
         if (st != GC_OK) fail(st);
         const at::Tensor space = workspace_of(bytes, x);
         st = gc_b200_group_norm_backward(
-            &dyd, &xd, gamma.defined() ? &gd : nullptr, beta.defined() ? &bd : nullptr, &sd, &dxd,
-            dgamma.defined() ? &dgd : nullptr, dbeta.defined() ? &dbd : nullptr, groups,
-            static_cast<int>(ctx->saved_data["activation"].toInt()), drop.on ? &drop.args : nullptr,
-            space.defined() ? space.data_ptr() : nullptr, bytes, stream_of(x));
+            &dyd, &xd, has_gamma_ ? &gd : nullptr, has_beta_ ? &bd : nullptr, &sd, &dxd,
+            dgamma.defined() ? &dgd : nullptr, dbeta.defined() ? &dbd : nullptr, a_.groups,
+            static_cast<int>(a_.activation), drop.on ? &drop.args : nullptr, space.defined() ? space.data_ptr() : nullptr,
+            bytes, stream_of(x));
         if (st != GC_OK) fail(st);
-        return {dx, dgamma, dbeta, at::Tensor(), at::Tensor()};
+        return {dx, dgamma, dbeta};
     }
 };
 
@@ -316,7 +314,23 @@ at::Tensor group_norm(const at::Tensor &x, const c10::optional<at::Tensor> &gamm
     const at::Tensor xi = in_order(x);
     const Drop drop = make_drop(x, p, scope, seed, offset, grad);
     const NormArgs a{groups, activation, eps};
-    return grad ? GroupNorm::apply(xi, gamma, beta, a, drop) : norm_forward(xi, g, b, a, drop, at::Tensor());
+    if (!grad) return norm_forward(xi, g, b, a, drop, at::Tensor());
+    for (const at::Tensor &t : {x, g, b}) no_forward_mode(t);
+    const at::Tensor stats =
+        at::empty({x.size(0), groups, 2}, x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
+    at::Tensor y = norm_forward(xi, g, b, a, drop, stats);
+    auto node = std::shared_ptr<GroupNormGrad>(new GroupNormGrad(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(xi, g, b));
+    node->x_ = torch::autograd::SavedVariable(xi, false);
+    node->has_gamma_ = g.defined();
+    node->has_beta_ = b.defined();
+    if (g.defined()) node->gamma_ = torch::autograd::SavedVariable(g, false);
+    if (b.defined()) node->beta_ = torch::autograd::SavedVariable(b, false);
+    node->stats_ = stats;
+    node->a_ = a;
+    node->drop_ = drop;
+    torch::autograd::set_history(y, node);
+    return y;
 }
 
 // One gc_b200_dropout call on tensors that lie alike.
@@ -342,38 +356,29 @@ at::Tensor laid_out_like(const at::Tensor &t, const at::Tensor &like) {
     return t;
 }
 
-struct Dropout : torch::autograd::Function<Dropout> {
-    static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x,
-                              const c10::optional<at::Tensor> &residual, Drop drop) {
-        // the gradient needs x's layout only, so nothing of its data is kept
-        ctx->saved_data["sizes"] = x.sizes().vec();
-        ctx->saved_data["strides"] = x.strides().vec();
-        ctx->saved_data["residual"] = residual.has_value() && residual->defined();
-        ctx->save_for_backward({drop.used});
-        save_drop(ctx->saved_data["drop"], drop);
-        return dropout_forward(x, residual.value_or(at::Tensor()), drop);
-    }
-    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
-                                                   torch::autograd::variable_list grads) {
+// Nothing of the data is kept: the gradient needs x's layout and the draws.
+struct DropoutGrad : torch::autograd::Node {
+    std::vector<int64_t> sizes_, strides_;
+    Drop drop_;
+
+    std::string name() const override { return "DropoutGrad"; }
+    torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor()};
         no_double_backward();
-        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
-        const auto saved = ctx->get_saved_variables();
-        const Drop drop = load_drop(ctx->saved_data["drop"], saved[0]);
         c10::OptionalDeviceGuard guard(grads[0].device());
         at::Tensor dx;
-        if (ctx->needs_input_grad(0)) {
+        if (task_should_compute_output(0)) {
             // the mask goes by place in memory: dy has to lie as x did
-            const auto sizes = ctx->saved_data["sizes"].toIntVector(), strides = ctx->saved_data["strides"].toIntVector();
             at::Tensor dy = grads[0];
             bool same = true;
-            for (size_t i = 0; i < sizes.size(); ++i) same = same && (sizes[i] <= 1 || dy.stride(i) == strides[i]);
+            for (size_t i = 0; i < sizes_.size(); ++i) same = same && (sizes_[i] <= 1 || dy.stride(i) == strides_[i]);
             if (!same) {
-                dy = at::empty_strided(sizes, strides, grads[0].options());
+                dy = at::empty_strided(sizes_, strides_, grads[0].options());
                 dy.copy_(grads[0]);
             }
-            dx = dropout_forward(dy, at::Tensor(), drop);
+            dx = dropout_forward(dy, at::Tensor(), again(drop_));
         }
-        return {dx, ctx->saved_data["residual"].toBool() ? grads[0] : at::Tensor(), at::Tensor()};
+        return {dx, grads[0]};
     }
 };
 
@@ -392,7 +397,18 @@ at::Tensor dropout(const at::Tensor &x, const c10::optional<at::Tensor> &residua
     if (r0.defined()) r = laid_out_like(r0, xi);
     const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(r0));
     Drop drop = make_drop(x, p, scope, seed, offset, grad);
-    return grad ? Dropout::apply(xi, r, drop) : dropout_forward(xi, r.value_or(at::Tensor()), drop);
+    const at::Tensor ri = r.value_or(at::Tensor());
+    at::Tensor y = dropout_forward(xi, ri, drop);
+    if (!grad) return y;
+    no_forward_mode(x);
+    no_forward_mode(r0);
+    auto node = std::shared_ptr<DropoutGrad>(new DropoutGrad(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(xi, ri));
+    node->sizes_ = xi.sizes().vec();
+    node->strides_ = xi.strides().vec();
+    node->drop_ = drop;
+    torch::autograd::set_history(y, node);
+    return y;
 }
 
 }  // namespace
