@@ -247,7 +247,8 @@ template <class T, int V>
 __global__ void __launch_bounds__(kNormThreads, split_blocks(V, false)) norm_moments_kernel(const __grid_constant__ NormParams P) {
     extern __shared__ __align__(16) unsigned char nsm[];
     uint4 *ring = reinterpret_cast<uint4 *>(nsm);
-    float *pivot = reinterpret_cast<float *>(nsm + ring_space(V));  // [width]
+    // the sums' space is the ring's, which is read no more by then
+    float *pivot = reinterpret_cast<float *>(nsm);  // [width]
     float2 *scratch = reinterpret_cast<float2 *>(pivot + (P.vb * V + 1) / 2 * 2);
     griddep_wait();
     griddep_launch_dependents();
@@ -267,6 +268,7 @@ __global__ void __launch_bounds__(kNormThreads, split_blocks(V, false)) norm_mom
     });
     if (at.count > 0) m.finish((at.count - 1) % kNormRun + 1);
     const int local = at.c0 - at.first;
+    __syncthreads();
     if (at.lane == 0 && at.count > 0) {
 #pragma unroll
         for (int j = 0; j < V; ++j) pivot[local + j] = m.mean[j];
@@ -356,17 +358,28 @@ __global__ void __launch_bounds__(kNormThreads) norm_finalize_kernel(const __gri
     }
 }
 
+// gamma and beta of a thread's channels.
 template <int V>
-__device__ __forceinline__ Coefs<V> split_coefs(const NormParams &P, long long n, int c0) {
-    float mean[V], a[V], b[V];
+struct Affine {
+    float gamma[V], beta[V];
+    __device__ __forceinline__ Affine(const NormParams &P, int c0) {
+        load_params<V>(P.gamma, P.gamma_type, c0, 1.0f, gamma);
+        load_params<V>(P.beta, P.beta_type, c0, 0.0f, beta);
+    }
+};
+template <int V>
+__device__ __forceinline__ Coefs<V> split_coefs(const NormParams &P, const Affine<V> &affine, long long n, int c0) {
+    float mean[V], a[V];
+    const float2 *stats = P.stats + n * P.groups;
+    int g = c0 / P.cpg, at = c0 - g * P.cpg;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float2 st = P.stats[n * P.groups + (c0 + j) / P.cpg];
+        const float2 st = stats[g];
         mean[j] = -st.x;
-        a[j] = st.y * (P.gamma ? load_param(P.gamma, P.gamma_type, c0 + j) : 1.0f);
-        b[j] = P.beta ? load_param(P.beta, P.beta_type, c0 + j) : 0.0f;
+        a[j] = st.y * affine.gamma[j];
+        if (++at == P.cpg) at = 0, g = min(g + 1, P.groups - 1);
     }
-    return {lanes_of<V>(mean), lanes_of<V>(a), lanes_of<V>(b)};
+    return {lanes_of<V>(mean), lanes_of<V>(a), lanes_of<V>(affine.beta)};
 }
 
 // Dropout of a thread's vectors, pixel by pixel.
@@ -403,11 +416,12 @@ __global__ void __launch_bounds__(kNormThreads, DROP ? 2 : split_blocks(V, false
     const T *x = static_cast<const T *>(P.x) + at.n * P.x_ldn + last * P.x_ldp + at.c0;
     const long long xstep = -static_cast<long long>(P.lanes) * P.x_ldp, ystep = -static_cast<long long>(P.lanes) * P.y_ldp;
     start_vectors<V>(ring, x, xstep, at.count);
+    const Affine<V> affine(P, at.c0);
     griddep_wait();
     griddep_launch_dependents();
     Keeper<V, DROP> drop(P, blockIdx.x == 0 && threadIdx.x == 0, at.n, last, at.c0, -P.lanes);
     if (at.count == 0) return;
-    const Coefs<V> coefs = split_coefs<V>(P, at.n, at.c0);
+    const Coefs<V> coefs = split_coefs<V>(P, affine, at.n, at.c0);
     T *y = static_cast<T *>(P.y) + at.n * P.y_ldn + last * P.y_ldp + at.c0;
     for_vectors<T, V>(ring, x, xstep, at.count, [&](int, Lanes<V> v) {
 #pragma unroll
@@ -460,8 +474,9 @@ __global__ void __launch_bounds__(kNormThreads, DROP ? 2 : split_blocks(V, true)
     const T *dy = static_cast<const T *>(P.dy) + at.n * P.dy_ldn + at.p0 * P.dy_ldp + at.c0;
     const long long xstep = static_cast<long long>(P.lanes) * P.x_ldp, gstep = static_cast<long long>(P.lanes) * P.dy_ldp;
     start_vector_pairs<V>(ring, x, xstep, dy, gstep, at.count);
+    const Affine<V> affine(P, at.c0);
     Keeper<V, DROP> drop(P, false, at.n, at.p0, at.c0, P.lanes);
-    const Coefs<V> coefs = split_coefs<V>(P, at.n, at.c0);
+    const Coefs<V> coefs = split_coefs<V>(P, affine, at.n, at.c0);
     Lanes<V> s2, t2;
 #pragma unroll
     for (int i = 0; i < Lanes<V>::kPairs; ++i) s2.p[i] = t2.p[i] = pair(0.0f);
@@ -472,8 +487,9 @@ __global__ void __launch_bounds__(kNormThreads, DROP ? 2 : split_blocks(V, true)
     values_of<V>(s2, s);
     values_of<V>(t2, t);
     float2 *out = P.part + (at.n * P.chunks + at.chunk) * P.c + at.first;
+    __syncthreads();  // the sums' space is the ring's
     channel_sums<V>(P.vb, P.lanes, P.vb * V, at.lane, at.lane < P.lanes ? at.col * V : 0, s, t,
-                    reinterpret_cast<float2 *>(nsm + ring_space(V)), [&](int c, float2 sum) {
+                    reinterpret_cast<float2 *>(nsm), [&](int c, float2 sum) {
                         if (c < at.width) out[c] = sum;
                     });
 }
@@ -541,19 +557,23 @@ __global__ void __launch_bounds__(kNormThreads, DROP ? 2 : split_blocks(V, true)
     const T *dy = static_cast<const T *>(P.dy) + at.n * P.dy_ldn + last * P.dy_ldp + at.c0;
     const long long down = -static_cast<long long>(P.lanes), xstep = down * P.x_ldp, gstep = down * P.dy_ldp;
     start_vector_pairs<V>(ring, x, xstep, dy, gstep, at.count);
+    const Affine<V> affine(P, at.c0);
     griddep_wait();
     griddep_launch_dependents();
     Keeper<V, DROP> drop(P, blockIdx.x == 0 && threadIdx.x == 0, at.n, last, at.c0, -P.lanes);
     if (at.count == 0) return;
-    const Coefs<V> coefs = split_coefs<V>(P, at.n, at.c0);
+    const Coefs<V> coefs = split_coefs<V>(P, affine, at.n, at.c0);
     Lanes<V> mk1, mk2;
     {
         float k1[V], k2[V];
+        const float2 *sums = P.gsum + at.n * P.groups;
+        int g = at.c0 / P.cpg, in = at.c0 - g * P.cpg;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float2 k = P.gsum[at.n * P.groups + (at.c0 + j) / P.cpg];
+            const float2 k = sums[g];
             k1[j] = -k.x;
             k2[j] = -k.y;
+            if (++in == P.cpg) in = 0, g = min(g + 1, P.groups - 1);
         }
         mk1 = lanes_of<V>(k1);
         mk2 = lanes_of<V>(k2);
@@ -695,14 +715,9 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_kernel(cons
             cp_async_commit();
         }
     }
-    float gm[V], bt[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        gm[j] = P.gamma ? load_param(P.gamma, P.gamma_type, r.c0 + j) : 1.0f;
-        bt[j] = P.beta ? load_param(P.beta, P.beta_type, r.c0 + j) : 0.0f;
-    }
+    const Affine<V> affine(P, r.c0);
     Coefs<V> coefs;
-    coefs.b = lanes_of<V>(bt);
+    coefs.b = lanes_of<V>(affine.beta);
     const float total = static_cast<float>(P.px) * static_cast<float>(P.cpg);
     const float members = static_cast<float>(r.rows) * static_cast<float>(P.cpg);
     int turn = 0;
@@ -843,7 +858,7 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_kernel(cons
             for_channels<V>(P, r, [&](int j, int g) {
                 const float2 st = fin[g];
                 mean[j] = -st.x;
-                a[j] = st.y * gm[j];
+                a[j] = st.y * affine.gamma[j];
             });
             coefs.minus_mean = lanes_of<V>(mean);
             coefs.a = lanes_of<V>(a);
@@ -933,14 +948,9 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
     }
     for (int c = tid; c < P.cb; c += threads) acc[c] = make_float2(0.0f, 0.0f);
     for (int g = tid; g < P.gb; g += threads) gst[g] = P.stats[(unit / P.bundles) * P.groups + bundle * P.gb + g];
-    float gm[V], bt[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        gm[j] = P.gamma ? load_param(P.gamma, P.gamma_type, r.c0 + j) : 1.0f;
-        bt[j] = P.beta ? load_param(P.beta, P.beta_type, r.c0 + j) : 0.0f;
-    }
+    const Affine<V> affine(P, r.c0);
     Coefs<V> coefs;
-    coefs.b = lanes_of<V>(bt);
+    coefs.b = lanes_of<V>(affine.beta);
     const float total = static_cast<float>(P.px) * static_cast<float>(P.cpg);
     int turn = 0;
     for (long long n = unit / P.bundles; n < P.n; n += P.stride, turn ^= 1) {
@@ -950,7 +960,7 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
             for_channels<V>(P, r, [&](int j, int g) {
                 const float2 st = gst[g];
                 mean[j] = -st.x;
-                a[j] = st.y * gm[j];
+                a[j] = st.y * affine.gamma[j];
             });
             coefs.minus_mean = lanes_of<V>(mean);
             coefs.a = lanes_of<V>(a);

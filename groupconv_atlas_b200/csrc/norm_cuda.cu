@@ -247,12 +247,13 @@ void plan_split(NormParams &P, int v, bool backward, int sms) {
     P.items = P.n * P.chunks * P.cblocks;
 }
 
-// Shared memory of the split path's kernels: the ring, and what the sums need.
+// Shared memory of the split path's kernels: the ring, and in its place after
+// the data what the sums need.
 size_t split_smem(const NormParams &P, int v, bool sums, bool backward) {
-    size_t bytes = gcb::ring_space(v);
-    if (sums) bytes += gcb::channel_sums_space(gcb::kNormThreads, P.vb, P.lanes, P.vb * v) * sizeof(float2);
-    if (sums && !backward) bytes += ceil_div(P.vb * v, 2) * 2 * sizeof(float);
-    return bytes;
+    size_t after = 0;
+    if (sums) after += gcb::channel_sums_space(gcb::kNormThreads, P.vb, P.lanes, P.vb * v) * sizeof(float2);
+    if (sums && !backward) after += ceil_div(P.vb * v, 2) * 2 * sizeof(float);
+    return std::max(gcb::ring_space(v), after);
 }
 
 uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }

@@ -96,7 +96,28 @@ __device__ __forceinline__ void store_elems(T *p, const float (&v)[V]) {
     }
 }
 
-// Element i of a parameter vector whose type is known at run time.
+// Elements [i, i + V) of a parameter vector whose type is known at run time, or
+// `none` where there is no vector.  One branch for all of them, so that their
+// loads are in flight together.
+template <int V>
+__device__ __forceinline__ void load_params(const void *p, int type, long long i, float none, float (&v)[V]) {
+    if (p == nullptr) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = none;
+    } else if (type == kElemF32) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = __ldg(static_cast<const float *>(p) + i + j);
+    } else {
+        uint16_t u[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) u[j] = __ldg(static_cast<const unsigned short *>(p) + i + j);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            v[j] = type == kElemBF16 ? __uint_as_float(static_cast<uint32_t>(u[j]) << 16)
+                                     : __half2float(__ushort_as_half(u[j]));
+    }
+}
+// Element i of such a vector.
 __device__ __forceinline__ float load_param(const void *p, int type, long long i) {
     if (type == kElemF32) return __ldg(static_cast<const float *>(p) + i);
     if (type == kElemF16) return __half2float(static_cast<const __half *>(p)[i]);
