@@ -25,6 +25,8 @@
 #pragma once
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "norm_util.cuh"
 
 namespace gcb {
@@ -674,6 +676,10 @@ __device__ __forceinline__ void for_channels(const NormParams &P, const Resident
     }
 }
 
+// Bytes of iters slots per thread, rounded up for what follows.
+__host__ __device__ inline size_t tile_bytes(int iters, int threads, int slot) {
+    return (static_cast<size_t>(iters) * threads * slot + 15) / 16 * 16;
+}
 // Shared memory of the resident kernels behind the tiles.
 __host__ __device__ inline size_t resident_extra(const NormParams &P, int threads, bool grad) {
     const size_t gb = P.gb, cb = P.cb;
@@ -682,13 +688,34 @@ __host__ __device__ inline size_t resident_extra(const NormParams &P, int thread
     return (entries + 4 * gb) * sizeof(float2);
 }
 
-template <class T, int ACT, bool DROP>
+// A thread's place in a tile: a 16-byte vector, or one element (V = 1, for
+// tensors whose pixels are not multiples of 16 bytes; 16-bit elements have no
+// asynchronous copy and pass through a register).
+template <class T, int V>
+using Slot = typename std::conditional<V == 1, T, uint4>::type;
+template <class T, int V>
+__device__ __forceinline__ void copy_slot(Slot<T, V> *dst, uint32_t addr, const T *src) {
+    if constexpr (V > 1) copy_vector(addr, src);
+    else if constexpr (sizeof(T) == 4) cp_async_4(dst, src, true);
+    else *dst = *src;
+}
+template <class T, int V>
+__device__ __forceinline__ Lanes<V> read_slot(const Slot<T, V> &s) {
+    if constexpr (V > 1) {
+        return unpack_lanes<T, V>(s, static_cast<const T *>(nullptr));
+    } else {
+        const float v[1] = {to_float(s)};
+        return lanes_of<1>(v);
+    }
+}
+
+template <class T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_kernel(const __grid_constant__ NormParams P) {
-    constexpr int V = kVec<T>, kPairs = Lanes<V>::kPairs;
+    constexpr int kPairs = Lanes<V>::kPairs;
     extern __shared__ __align__(16) unsigned char nsm[];
     const int threads = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
-    uint4 *tile = reinterpret_cast<uint4 *>(nsm);
-    float2 *exch = reinterpret_cast<float2 *>(tile + static_cast<size_t>(P.iters) * threads);  // [2][gb]
+    Slot<T, V> *tile = reinterpret_cast<Slot<T, V> *>(nsm);
+    float2 *exch = reinterpret_cast<float2 *>(nsm + tile_bytes(P.iters, threads, sizeof(Slot<T, V>)));  // [2][gb]
     float2 *fin = exch + 2 * P.gb;
     float *pivot = reinterpret_cast<float *>(fin + P.gb);
     float2 *red = fin + 2 * P.gb;  // [lanes][vr][sub]
@@ -696,8 +723,8 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_kernel(cons
     const unsigned unit = blockIdx.x / P.cluster;
     const int bundle = unit % P.bundles;
     const Resident r = resident_place(P, rank, bundle, V);
-    const uint4 *tile_at = tile + tid;
-    const uint32_t tile_addr = smem_addr(tile_at), pitch = 16 * threads;
+    Slot<T, V> *tile_at = tile + tid;
+    const uint32_t tile_addr = smem_addr(tile_at), pitch = sizeof(Slot<T, V>) * threads;
     griddep_wait();
     griddep_launch_dependents();
     Philox gen;
@@ -711,7 +738,7 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_kernel(cons
         for (int part = 0; part < kParts; ++part) {
             const int to = part_end(P.iters, r.count, part);
 #pragma unroll 4
-            for (; k < to; ++k, src += xstep) copy_vector(tile_addr + k * pitch, src);
+            for (; k < to; ++k, src += xstep) copy_slot<T, V>(tile_at + k * threads, tile_addr + k * pitch, src);
             cp_async_commit();
         }
     }
@@ -733,14 +760,14 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_kernel(cons
         for (int part = 0; part < kParts; ++part) {
             wait_part(part);
             if (part == 0 && r.count > 0) {
-                const Lanes<V> v = unpack_lanes<T, V>(tile_at[0], x);
+                const Lanes<V> v = read_slot<T, V>(tile_at[0]);
 #pragma unroll
                 for (int i = 0; i < kPairs; ++i) minus.p[i] = v.p[i] * pair(-1.0f);
             }
             const int to = part_end(P.iters, r.count, part);
 #pragma unroll 4
             for (; k < to; ++k) {
-                const Lanes<V> v = unpack_lanes<T, V>(tile_at[k * threads], x);
+                const Lanes<V> v = read_slot<T, V>(tile_at[k * threads]);
 #pragma unroll
                 for (int i = 0; i < kPairs; ++i) {
                     const f2 d = v.p[i] + minus.p[i];
@@ -876,9 +903,9 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_kernel(cons
             const int to = part_end(P.iters, r.count, part);
 #pragma unroll 2
             for (; k < to; ++k, y += ystep) {
-                Lanes<V> v = unpack_lanes<T, V>(tile_at[k * threads], x);
+                Lanes<V> v = read_slot<T, V>(tile_at[k * threads]);
                 if (more) {
-                    copy_vector(tile_addr + k * pitch, src);
+                    copy_slot<T, V>(tile_at + k * threads, tile_addr + k * pitch, src);
                     src += xstep;
                 }
 #pragma unroll
@@ -903,14 +930,13 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_kernel(cons
 // The gradient: x and dy resident.  First pass: sum dz and sum dz (x - mean)
 // per channel; second pass: dx.  Element decisions of the dropout are drawn in
 // the first pass and kept as one byte a vector in shared memory.
-template <class T, int ACT, bool DROP>
+template <class T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel(const __grid_constant__ NormParams P) {
-    constexpr int V = kVec<T>;
     extern __shared__ __align__(16) unsigned char nsm[];
     const int threads = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
     const size_t tiles = static_cast<size_t>(P.iters) * threads;
-    uint4 *tx = reinterpret_cast<uint4 *>(nsm);
-    float2 *exch = reinterpret_cast<float2 *>(tx + 2 * tiles);  // [2][gb]
+    Slot<T, V> *tx = reinterpret_cast<Slot<T, V> *>(nsm);
+    float2 *exch = reinterpret_cast<float2 *>(nsm + tile_bytes(2 * P.iters, threads, sizeof(Slot<T, V>)));  // [2][gb]
     float2 *fin = exch + 2 * P.gb;
     float2 *gst = fin + P.gb;           // mean, rstd of the unit's groups
     float2 *weighted = gst + P.gb;      // [cb]: gamma * the channel's sums
@@ -921,8 +947,8 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
     const unsigned unit = blockIdx.x / P.cluster;
     const int bundle = unit % P.bundles;
     const Resident r = resident_place(P, rank, bundle, V);
-    const uint4 *x_at = tx + tid, *g_at = x_at + tiles;
-    const uint32_t x_addr = smem_addr(x_at), g_addr = smem_addr(g_at), pitch = 16 * threads;
+    Slot<T, V> *x_at = tx + tid, *g_at = x_at + tiles;
+    const uint32_t x_addr = smem_addr(x_at), g_addr = smem_addr(g_at), pitch = sizeof(Slot<T, V>) * threads;
     griddep_wait();
     griddep_launch_dependents();
     Philox gen;
@@ -940,8 +966,8 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
             const int to = part_end(P.iters, r.count, part);
 #pragma unroll 2
             for (; k < to; ++k, sx += xstep, sg += gstep) {
-                copy_vector(x_addr + k * pitch, sx);
-                copy_vector(g_addr + k * pitch, sg);
+                copy_slot<T, V>(x_at + k * threads, x_addr + k * pitch, sx);
+                copy_slot<T, V>(g_at + k * threads, g_addr + k * pitch, sg);
             }
             cp_async_commit();
         }
@@ -978,8 +1004,8 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
             const int to = part_end(P.iters, r.count, part);
 #pragma unroll 2
             for (; k < to; ++k) {
-                const Lanes<V> v = unpack_lanes<T, V>(x_at[k * threads], x);
-                Lanes<V> g = unpack_lanes<T, V>(g_at[k * threads], x);
+                const Lanes<V> v = read_slot<T, V>(x_at[k * threads]);
+                Lanes<V> g = read_slot<T, V>(g_at[k * threads]);
                 if (DROP) {
                     if (!P.drop.channel) {
                         keep = Draws<V>(gen, at).bits(P.drop.limit);
@@ -1060,11 +1086,11 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
             const int to = part_end(P.iters, r.count, part);
 #pragma unroll 2
             for (; k < to; ++k, dx += ystep) {
-                const Lanes<V> v = unpack_lanes<T, V>(x_at[k * threads], x);
-                Lanes<V> g = unpack_lanes<T, V>(g_at[k * threads], x);
+                const Lanes<V> v = read_slot<T, V>(x_at[k * threads]);
+                Lanes<V> g = read_slot<T, V>(g_at[k * threads]);
                 if (more) {
-                    copy_vector(x_addr + k * pitch, sx);
-                    copy_vector(g_addr + k * pitch, sg);
+                    copy_slot<T, V>(x_at + k * threads, x_addr + k * pitch, sx);
+                    copy_slot<T, V>(g_at + k * threads, g_addr + k * pitch, sg);
                     sx += xstep;
                     sg += gstep;
                 }

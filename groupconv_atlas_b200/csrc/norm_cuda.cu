@@ -265,6 +265,7 @@ struct NormPlan {
     int threads = gcb::kNormThreads;
     size_t smem = 0;
     int width() const { return !vec ? 1 : type == gcb::kElemF32 ? 4 : 8; }  // elements of a vector
+    int slot() const { return vec ? 16 : elem_size(type); }                 // its bytes
 };
 
 struct NormSpace {  // the workspace's parts, in this order
@@ -328,12 +329,12 @@ bool empty(const NormParams &P) { return P.n == 0 || P.px == 0; }
 // ---- resident path: plan --------------------------------------------------------------------
 // What a plan depends on.
 struct ResidentKey {
-    int dev, type, backward, drop;
+    int dev, type, backward, vec;
     long long n, px;
     int c, groups;
     bool operator<(const ResidentKey &o) const {
-        return std::tie(dev, type, backward, drop, n, px, c, groups) <
-               std::tie(o.dev, o.type, o.backward, o.drop, o.n, o.px, o.c, o.groups);
+        return std::tie(dev, type, backward, vec, n, px, c, groups) <
+               std::tie(o.dev, o.type, o.backward, o.vec, o.n, o.px, o.c, o.groups);
     }
 };
 struct ResidentPlan {
@@ -343,8 +344,8 @@ struct ResidentPlan {
 };
 
 // Fills the resident fields of P for a choice; false when it does not apply.
-bool set_resident(NormParams &P, int v, int cb, int cluster, int threads, bool backward, bool bits, size_t limit,
-                  size_t &smem) {
+bool set_resident(NormParams &P, int v, int slot, int cb, int cluster, int threads, bool backward, bool bits,
+                  size_t limit, size_t &smem) {
     P.cb = cb;
     P.vr = cb / v;
     if (P.vr > threads) return false;
@@ -358,8 +359,7 @@ bool set_resident(NormParams &P, int v, int cb, int cluster, int threads, bool b
     if (rows > (1 << 20)) return false;
     P.rows = static_cast<int>(rows);
     P.iters = static_cast<int>(ceil_div(rows, P.lanes));
-    smem = static_cast<size_t>(P.iters) * threads * (backward ? 32 : 16) +
-           gcb::resident_extra(P, threads, backward) +
+    smem = gcb::tile_bytes((backward ? 2 : 1) * P.iters, threads, slot) + gcb::resident_extra(P, threads, backward) +
            (bits ? static_cast<size_t>(P.iters) * threads : 0);
     return smem <= limit;
 }
@@ -377,36 +377,40 @@ long long resident_stride(const NormParams &P, int threads, size_t smem, const g
 // phases (load; per image of a cluster the first pass, the sums, the second
 // pass) with constants fitted to 1500 measured choices of 24 shapes on a B200;
 // the choice it makes is on average 4 % slower than the best of them.
-double resident_cost(const NormParams &P, int v, int threads, size_t smem, bool backward, const gcb::DeviceFacts &f) {
+double resident_cost(const NormParams &P, int v, int slot, int threads, size_t smem, bool backward,
+                     const gcb::DeviceFacts &f) {
     int occ = 1;
     const long long stride = resident_stride(P, threads, smem, f, occ);
     const double rounds = static_cast<double>(ceil_div(P.n, stride));
     const double per_sm = std::ceil(static_cast<double>(stride) * P.bundles * P.cluster / f.sms);  // CTAs of the fullest SM
-    const double run = P.cb * (v == 4 ? 4.0 : 2.0);
-    const double kb = per_sm * P.iters * P.lanes * P.vr * 16.0 * (backward ? 2 : 1) / 1024.0 /
+    const double run = P.cb * static_cast<double>(slot) / v;
+    const double kb = per_sm * P.iters * P.lanes * P.vr * static_cast<double>(slot) * (backward ? 2 : 1) / 1024.0 /
                       (run >= 64 ? 1.0 : run >= 32 ? 0.78 : 0.43);  // narrow runs waste sectors
     double sums = 1.4 + (P.cluster > 1 ? 1.4 : 0.0) + (P.cluster > 8 ? 0.4 : 0.0) + 0.12 * per_sm * threads / 512;
     if (backward) sums += 32 % P.vr != 0 ? 2.0 : 0.0;
     else sums += 0.22 * P.vr * P.lanes * P.sub / 512;
     // per vector of a thread: latency with few warps, issue slots with many
     const double crowd = P.iters * std::max(1.0, per_sm * threads / 32 / 6.2);
-    const double first = std::max(kb / 1300.0, crowd * (v == 4 ? 0.0 : 0.031) * (backward ? 1.5 : 1.0));
-    const double second = std::max(kb / (backward ? 36.0 : 34.0), crowd * (v == 4 ? 0.09 : 0.14) * (backward ? 2.5 : 1.0));
+    const double first = std::max(kb / 1300.0, crowd * (v == 1 ? 0.02 : v == 4 ? 0.0 : 0.031) * (backward ? 1.5 : 1.0));
+    const double second = std::max(kb / (backward ? 36.0 : 34.0),
+                                   crowd * (v == 1 ? 0.05 : v == 4 ? 0.09 : 0.14) * (backward ? 2.5 : 1.0));
     return 2.3 + kb / 88.0 + rounds * (first + sums + second) + (backward ? 1.65 : 0.0);
 }
 // The same for the split path: its launches' fixed times and the data at the
 // rates they reach.
-double split_cost(const NormParams &P, int v, bool backward) {
-    const double mb = static_cast<double>(P.n) * P.px * P.c * (v == 4 ? 4.0 : 2.0) * 1e-6;
+double split_cost(const NormParams &P, int v, int slot, bool backward) {
+    const double elements = static_cast<double>(P.n) * P.px * P.c, mb = elements * slot / v * 1e-6;
+    if (v == 1) return backward ? 12.9 + elements * 4.1e-6 : 8.6 + elements * (slot == 4 ? 2.8e-6 : 2.3e-6);
     return backward ? 12.9 + 2 * mb / 6.0 + 3 * mb / 6.6 : 8.6 + mb / 5.5 + 2 * mb / 6.6;
 }
 
 std::mutex g_mutex;
 std::map<ResidentKey, ResidentPlan> g_resident;
 
-ResidentPlan choose_resident(const NormParams &base, int v, bool backward, bool bits, const gcb::DeviceFacts &f) {
+ResidentPlan choose_resident(const NormParams &base, int v, int slot, bool backward, bool bits,
+                             const gcb::DeviceFacts &f) {
     ResidentPlan best;
-    double best_cost = split_cost(base, v, backward);
+    double best_cost = split_cost(base, v, slot, backward);
     const int unit = std::lcm(base.cpg, v);  // channels: whole groups and whole vectors
     const int units = base.c / unit;
     for (int m = 1; m <= units && static_cast<long long>(m) * unit / v <= gcb::kNormThreads; ++m) {
@@ -415,9 +419,9 @@ ResidentPlan choose_resident(const NormParams &base, int v, bool backward, bool 
             for (int threads = 64; threads <= gcb::kResidentThreads; threads *= 2) {
                 NormParams P = base;
                 size_t smem = 0;
-                if (!set_resident(P, v, m * unit, cluster, threads, backward, bits, f.smem_optin, smem)) continue;
+                if (!set_resident(P, v, slot, m * unit, cluster, threads, backward, bits, f.smem_optin, smem)) continue;
                 if (P.n * P.bundles * cluster > INT32_MAX) continue;
-                const double cost = resident_cost(P, v, threads, smem, backward, f);
+                const double cost = resident_cost(P, v, slot, threads, smem, backward, f);
                 if (cost < best_cost) {
                     best_cost = cost;
                     best.ok = true;
@@ -439,10 +443,10 @@ int plan_norm(NormParams &P, NormPlan &plan, bool backward) {
     const int st = gcb::device_facts(dev, facts);
     if (st != GC_OK) return st;
     const int v = plan.width();
-    if (plan.vec) {
+    {
         // room for the decision bytes is planned for whether they are needed
         // or not, so that a tensor's workspace does not depend on the dropout
-        const ResidentKey key{dev, plan.type, backward, 0, P.n, P.px, P.c, P.groups};
+        const ResidentKey key{dev, plan.type, backward, plan.vec, P.n, P.px, P.c, P.groups};
         ResidentPlan r;
         bool known = false;
         {
@@ -454,12 +458,12 @@ int plan_norm(NormParams &P, NormPlan &plan, bool backward) {
             }
         }
         if (!known) {
-            r = choose_resident(P, v, backward, backward, facts);
+            r = choose_resident(P, v, plan.slot(), backward, backward, facts);
             std::lock_guard<std::mutex> lock(g_mutex);
             g_resident[key] = r;
         }
         if (r.ok) {
-            set_resident(P, v, r.cb, r.cluster, r.threads, backward, backward, facts.smem_optin, plan.smem);
+            set_resident(P, v, plan.slot(), r.cb, r.cluster, r.threads, backward, backward, facts.smem_optin, plan.smem);
             plan.resident = true;
             plan.threads = r.threads;
             int occ = 1;
@@ -508,23 +512,25 @@ const void *norm_kernel(NormKernel k, const NormPlan &plan, const NormParams &P)
     return norm_typed<float>(k, plan.vec, P.act, drop);
 }
 
-// The resident kernels with dropout choose the activation at run time.
+template <class T, int V, int ACT, bool DROP>
+const void *resident_instance(bool backward) {
+    return backward ? reinterpret_cast<const void *>(&gcb::norm_resident_grad_kernel<T, V, ACT, DROP>)
+                    : reinterpret_cast<const void *>(&gcb::norm_resident_kernel<T, V, ACT, DROP>);
+}
 template <class T>
-const void *resident_typed(bool backward, int act, bool drop) {
-#define GCB_RESIDENT(ACT, DROP)                                                            \
-    (backward ? reinterpret_cast<const void *>(&gcb::norm_resident_grad_kernel<T, ACT, DROP>) \
-              : reinterpret_cast<const void *>(&gcb::norm_resident_kernel<T, ACT, DROP>))
-    if (drop) return GCB_RESIDENT(-1, true);
-    if (act == gcb::kActRelu) return GCB_RESIDENT(gcb::kActRelu, false);
-    if (act == gcb::kActRelu6) return GCB_RESIDENT(gcb::kActRelu6, false);
-    if (act == gcb::kActSilu) return GCB_RESIDENT(gcb::kActSilu, false);
-    return GCB_RESIDENT(gcb::kActNone, false);
-#undef GCB_RESIDENT
+const void *resident_typed(bool backward, bool vec, int act, bool drop) {
+    constexpr int V = gcb::kVec<T>;
+    if (!vec) return drop ? resident_instance<T, 1, -1, true>(backward) : resident_instance<T, 1, -1, false>(backward);
+    if (drop) return resident_instance<T, V, -1, true>(backward);
+    if (act == gcb::kActRelu) return resident_instance<T, V, gcb::kActRelu, false>(backward);
+    if (act == gcb::kActRelu6) return resident_instance<T, V, gcb::kActRelu6, false>(backward);
+    if (act == gcb::kActSilu) return resident_instance<T, V, gcb::kActSilu, false>(backward);
+    return resident_instance<T, V, gcb::kActNone, false>(backward);
 }
 const void *resident_kernel(const NormPlan &plan, bool backward, int act, bool drop) {
-    if (plan.type == gcb::kElemF16) return resident_typed<__half>(backward, act, drop);
-    if (plan.type == gcb::kElemBF16) return resident_typed<__nv_bfloat16>(backward, act, drop);
-    return resident_typed<float>(backward, act, drop);
+    if (plan.type == gcb::kElemF16) return resident_typed<__half>(backward, plan.vec, act, drop);
+    if (plan.type == gcb::kElemBF16) return resident_typed<__nv_bfloat16>(backward, plan.vec, act, drop);
+    return resident_typed<float>(backward, plan.vec, act, drop);
 }
 
 // Opts a kernel into the shared memory and the cluster sizes it may be
@@ -711,7 +717,7 @@ int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
         if (stats == nullptr) P.stats = nullptr;
         if ((st = launch_resident(P, plan, false, dev, s, e)) != GC_OK) return st;
         gcb::record_plan(PlanRecord::kNorm, "resident", false, static_cast<long long>(P.stride) * P.bundles * P.cluster,
-                         plan.threads, plan.smem, P.cluster, P.cb, P.rows, 1, 1);
+                         plan.threads, plan.smem, P.cluster, P.cb, P.rows, plan.vec ? 1 : 0, 1);
         return launched(e);
     }
     if ((st = launch_split(kMoments, P, plan, dev, s, e)) != GC_OK) return st;
@@ -811,7 +817,7 @@ int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
         if (e == cudaSuccess && params) e = launch(sums, ceil_div(P.c, 32), P, s);
         gcb::record_plan(PlanRecord::kNorm, "resident_backward", false,
                          static_cast<long long>(P.stride) * P.bundles * P.cluster, plan.threads, plan.smem, P.cluster,
-                         P.cb, P.rows, 1, params ? 2 : 1);
+                         P.cb, P.rows, plan.vec ? 1 : 0, params ? 2 : 1);
         return launched(e);
     }
     P.sum_rows = P.n;
