@@ -373,35 +373,37 @@ long long resident_stride(const NormParams &P, int threads, size_t smem, const g
     return ceil_div(P.n, ceil_div(P.n, most));
 }
 
-// Estimated time in microseconds of a resident choice that is set in P: its
-// phases (load; per image of a cluster the first pass, the sums, the second
-// pass) with constants fitted to 1500 measured choices of 24 shapes on a B200;
-// the choice it makes is on average 4 % slower than the best of them.
+// Estimated cost of a resident choice that is set in P: its phases (load; for
+// each image of a cluster the first pass, the sums, the second pass).  The
+// constants are fitted, to 6300 choices of 112 shapes timed on a B200, so that
+// the cheapest choice is the fastest one; they follow the times in
+// microseconds only roughly.  On those shapes the choice is 5 % slower than the
+// best on average, and at most 1.25 times where a call takes more than 6 us
+// (once 1.39, with 255 channels of FP32).
 double resident_cost(const NormParams &P, int v, int slot, int threads, size_t smem, bool backward,
                      const gcb::DeviceFacts &f) {
     int occ = 1;
     const long long stride = resident_stride(P, threads, smem, f, occ);
     const double rounds = static_cast<double>(ceil_div(P.n, stride));
     const double per_sm = std::ceil(static_cast<double>(stride) * P.bundles * P.cluster / f.sms);  // CTAs of the fullest SM
-    const double run = P.cb * static_cast<double>(slot) / v;
+    const double run = P.cb * static_cast<double>(slot) / v;  // bytes of a pixel that lie together
     const double kb = per_sm * P.iters * P.lanes * P.vr * static_cast<double>(slot) * (backward ? 2 : 1) / 1024.0 /
-                      (run >= 64 ? 1.0 : run >= 32 ? 0.78 : 0.43);  // narrow runs waste sectors
-    double sums = 1.4 + (P.cluster > 1 ? 1.4 : 0.0) + (P.cluster > 8 ? 0.4 : 0.0) + 0.12 * per_sm * threads / 512;
-    if (backward) sums += 32 % P.vr != 0 ? 2.0 : 0.0;
-    else sums += 0.22 * P.vr * P.lanes * P.sub / 512;
+                      (run >= 64 ? 1.0 : run >= 32 ? 0.51 : 0.26);
+    double sums = 1.13 + (P.cluster > 1 ? 2.61 : 0.0) + (P.cluster > 8 ? 1.73 : 0.0) + 1.48 * per_sm * threads / 512;
+    if (backward) sums += 0.35 + (32 % P.vr != 0 ? 0.14 : 0.0);
+    else sums += 0.05 * P.vr * P.lanes * P.sub / 512;
     // per vector of a thread: latency with few warps, issue slots with many
-    const double crowd = P.iters * std::max(1.0, per_sm * threads / 32 / 6.2);
-    const double first = std::max(kb / 1300.0, crowd * (v == 1 ? 0.02 : v == 4 ? 0.0 : 0.031) * (backward ? 1.5 : 1.0));
-    const double second = std::max(kb / (backward ? 36.0 : 34.0),
-                                   crowd * (v == 1 ? 0.05 : v == 4 ? 0.09 : 0.14) * (backward ? 2.5 : 1.0));
-    return 2.3 + kb / 88.0 + rounds * (first + sums + second) + (backward ? 1.65 : 0.0);
+    const double crowd = P.iters * std::max(1.0, per_sm * threads / 32 / 11.1);
+    const double first = std::max(kb / 103.0, crowd * (v == 1 ? 0.047 : v == 4 ? 0.027 : 0.0125) * (backward ? 10.7 : 1.0));
+    const double second = std::max(kb / (backward ? 237.0 : 38.0),
+                                   crowd * (v == 1 ? 0.147 : v == 4 ? 0.112 : 0.225) * (backward ? 1.33 : 1.0));
+    return 0.4 + kb / 190.0 + rounds * (first + sums + second) + (backward ? 1.0 : 0.0);
 }
-// The same for the split path: its launches' fixed times and the data at the
-// rates they reach.
+// The same for the split path.
 double split_cost(const NormParams &P, int v, int slot, bool backward) {
     const double elements = static_cast<double>(P.n) * P.px * P.c, mb = elements * slot / v * 1e-6;
-    if (v == 1) return backward ? 12.9 + elements * 4.1e-6 : 8.6 + elements * (slot == 4 ? 2.8e-6 : 2.3e-6);
-    return backward ? 12.9 + 2 * mb / 6.0 + 3 * mb / 6.6 : 8.6 + mb / 5.5 + 2 * mb / 6.6;
+    if (v == 1) return backward ? 10.0 + elements * 4.76e-6 : 15.3 + elements * (slot == 4 ? 6.4e-6 : 2.1e-6);
+    return backward ? 10.0 + 2 * mb / 6.0 + 3 * mb / 6.6 : 15.3 + mb / 5.5 + 2 * mb / 6.6;
 }
 
 std::mutex g_mutex;
