@@ -192,6 +192,8 @@ int check_dropout(const gc_b200_dropout_args *d, DropParams &out) {
     return GC_OK;
 }
 
+Range used_words(const DropParams &d) { return {d.used, d.used != nullptr ? 16u : 0u}; }
+
 // The current device, the pointers' device and the stream (reference
 // groupconv.cu:130-139, :185-191).
 int check_call(std::initializer_list<const gc_tensor *> tensors, std::initializer_list<const void *> words,
@@ -684,8 +686,9 @@ int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
     if (stats != nullptr && (st = check_stats(stats, x, groups)) != GC_OK) return st;
     DropParams drop;
     if ((st = check_dropout(dropout, drop)) != GC_OK) return st;
-    if (outputs_meet({{y->data, v[1].span}, range_of(stats)}, {{x->data, v[0].span}, range_of(gamma), range_of(beta)}))
-        return gc_error(GC_INVALID, "outputs must not overlap inputs");
+    if (outputs_meet({{y->data, v[1].span}, range_of(stats), used_words(drop), {workspace, workspace_bytes}},
+                     {{x->data, v[0].span}, range_of(gamma), range_of(beta)}))
+        return gc_error(GC_INVALID, "outputs and workspace must not overlap inputs or one another");
     if (!known_activation(activation)) return gc_error(GC_UNSUPPORTED, "unknown activation");
     for (const gc_tensor *t : {gamma, beta})
         if ((st = check_channel_layout(t)) != GC_OK) return st;
@@ -762,9 +765,10 @@ int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
     if ((st = check_stats(stats, x, groups)) != GC_OK) return st;
     DropParams drop;
     if ((st = check_dropout(dropout, drop)) != GC_OK) return st;
-    if (outputs_meet({{dx->data, v[2].span}, range_of(dgamma), range_of(dbeta)},
+    if (outputs_meet({{dx->data, v[2].span}, range_of(dgamma), range_of(dbeta), used_words(drop),
+                      {workspace, workspace_bytes}},
                      {{x->data, v[0].span}, {dy->data, v[1].span}, range_of(gamma), range_of(beta), range_of(stats)}))
-        return gc_error(GC_INVALID, "outputs must not overlap inputs");
+        return gc_error(GC_INVALID, "outputs and workspace must not overlap inputs or one another");
     if (!known_activation(activation)) return gc_error(GC_UNSUPPORTED, "unknown activation");
     for (const gc_tensor *t : {gamma, beta, static_cast<const gc_tensor *>(dgamma),
                                static_cast<const gc_tensor *>(dbeta)})
@@ -847,7 +851,7 @@ int gc_b200_dropout(const gc_tensor *x, const gc_tensor *residual, gc_tensor *y,
     DropParams drop;
     int st = check_dropout(dropout, drop);
     if (st != GC_OK) return st;
-    if (outputs_meet({range_of(y)}, {range_of(x), range_of(residual)}))
+    if (outputs_meet({range_of(y), used_words(drop)}, {range_of(x), range_of(residual)}))
         return gc_error(GC_INVALID, "outputs must not overlap inputs");
     if (drop.channel && x->rank < 2) return gc_error(GC_INVALID, "channel dropout needs a channel axis");
     if (x->dtype == GC_F64) return gc_error(GC_UNSUPPORTED, "FP64 tensors are not supported here");

@@ -309,7 +309,9 @@ at::Tensor group_norm(const at::Tensor &x, const c10::optional<at::Tensor> &gamm
     if (x.dim() < 2 || x.dim() > 4) throw std::invalid_argument("input must have 2 to 4 axes (N, C, ..)");
     c10::OptionalDeviceGuard guard;
     if (x.is_cuda()) guard.reset_device(x.device());
-    const at::Tensor g = gamma.value_or(at::Tensor()), b = beta.value_or(at::Tensor());
+    at::Tensor g = gamma.value_or(at::Tensor()), b = beta.value_or(at::Tensor());
+    if (g.defined()) g = g.contiguous();
+    if (b.defined()) b = b.contiguous();
     const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(g) || wants_grad(b));
     const at::Tensor xi = in_order(x);
     const Drop drop = make_drop(x, p, scope, seed, offset, grad);

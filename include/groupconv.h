@@ -193,8 +193,9 @@ int gc_b200_conv_ex(const gc_shape *p, const gc_tensor *x, const gc_tensor *w,
  *                          when the kernel runs (so a captured graph can draw
  *                          anew at each replay);
  *   used                   nullable device pair that receives the seed and
- *                          offset in effect, for a later gradient.  Must not
- *                          be one of the two words above. */
+ *                          offset in effect, for a later gradient (unless t is
+ *                          0: nothing is drawn then).  Must not overlap the
+ *                          two words above. */
 typedef struct {
     double p; /* 0 <= p <= 1 */
     uint64_t seed, offset;
@@ -223,7 +224,7 @@ typedef struct {
  *               gc_b200_group_norm_workspace gives for these tensors (NULL
  *               when that is 0); its contents need not be set and are
  *               undefined afterwards.
- * Outputs overlap no input.  Validation, device, stream, allocation and
+ * Outputs and workspace overlap neither inputs nor one another.  Validation, device, stream, allocation and
  * capture rules are those of gc_cuda_conv.  Results are bitwise reproducible. */
 int gc_b200_group_norm_workspace(const gc_tensor *x, const gc_tensor *y, int64_t groups, uint64_t *bytes);
 int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tensor *beta, gc_tensor *y,

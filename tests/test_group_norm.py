@@ -18,7 +18,12 @@ TYPES = {'f32': torch.float32, 'f16': torch.float16, 'bf16': torch.bfloat16}
 SHAPES = [((1, 32, 7, 7), 8), ((2, 45, 5, 9), 9), ((3, 40, 11, 13), 4), ((2, 96, 1, 1), 1), ((1, 8, 1, 1), 8),
           ((5, 256, 9, 9), 32), ((2, 2056, 3, 3), 257), ((1, 1, 33, 17), 1), ((2, 64, 90, 70), 16), ((3, 24, 1, 50), 3),
           ((4, 48, 1000), 6), ((70, 64), 8), ((2, 16, 300, 2), 16), ((2, 30, 64, 65), 2), ((1, 512, 40, 3), 1),
-          ((3, 7, 1), 7), ((1, 1040, 5, 6), 2), ((2, 128, 64, 64), 32)]
+          ((3, 7, 1), 7), ((1, 1040, 5, 6), 2), ((2, 128, 64, 64), 32),
+          # more images than the GPU holds at once: a cluster takes several in turn
+          ((600, 64, 4, 4), 4), ((900, 15, 5, 3), 5), ((1300, 24, 2, 2), 1)]
+
+# Groups too large for shared memory, by vectors and by single elements.
+SPLIT_SHAPES = [((1, 64, 300, 260), 1), ((2, 255, 100, 90), 1)]
 
 
 def make(dims, dtype, seed=0, shift=0.5):
@@ -94,6 +99,25 @@ def check_step(native, x, gamma, beta, dy, groups, act, p=0.0, scope='element', 
 def test_forward_and_gradient(native, torch_cuda, dims, groups, dtype):
     x, gamma, beta, dy = make(dims, TYPES[dtype])
     check_step(native, x, gamma, beta, dy, groups, 'silu')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dims,groups', SPLIT_SHAPES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('p,scope,act', [(0.0, 'element', 'silu'), (0.25, 'element', 'none'), (0.25, 'channel', 'relu')])
+def test_groups_that_are_read_twice(native, torch_cuda, dims, groups, dtype, p, scope, act):
+    x, gamma, beta, dy = make(dims, TYPES[dtype], 20)
+    check_step(native, x, gamma, beta, dy, groups, act, p, scope)
+    assert 'split_backward' in native.last_plan()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dims,groups', [((600, 64, 4, 4), 4), ((900, 15, 5, 3), 5)])
+@pytest.mark.parametrize('scope', ['element', 'channel'])
+def test_dropout_of_many_images(native, torch_cuda, dims, groups, scope):
+    x, gamma, beta, dy = make(dims, torch.bfloat16, 21)
+    check_step(native, x, gamma, beta, dy, groups, 'silu', 0.5, scope)
+    assert 'resident_backward' in native.last_plan()
 
 
 @pytest.mark.gpu
@@ -362,6 +386,104 @@ def test_generator_draws(native, torch_cuda):
 
 
 @pytest.mark.gpu
+def test_probability_that_rounds_to_nothing(native, torch_cuda):
+    x = make((2, 32, 6, 6), torch.float32, 16)[0].cuda()
+    leaf = x.clone(memory_format=torch.preserve_format).requires_grad_()
+    y = torch_module.group_norm_act(leaf, 4, dropout=1e-6)
+    assert torch.equal(y, torch_module.group_norm_act(x, 4))
+    assert torch.autograd.grad(y.sum(), leaf)[0].shape == x.shape
+
+
+@pytest.mark.gpu
+def test_expanded_gradients_and_strided_parameters(native, torch_cuda):
+    x, gamma, beta, _ = (t.cuda() for t in make((2, 32, 6, 7), torch.float32, 17))
+    leaf = x.requires_grad_()
+    wide = torch.stack([gamma, gamma], 1)[:, 0].detach().requires_grad_()  # stride 2
+    y = torch_module.group_norm_act(leaf, 4, wide, beta, activation='silu')
+    dx, dw = torch.autograd.grad(y.sum(), [leaf, wide])
+    z = torch_module.group_norm_act(leaf, 4, gamma.detach().requires_grad_(), beta, activation='silu')
+    assert torch.equal(y, z)
+    assert torch.equal(dx, torch.autograd.grad(z, leaf, torch.ones_like(z))[0]) and dw.shape == wide.shape
+
+
+@pytest.mark.gpu
+def test_changed_inputs_and_released_graphs_are_refused(native, torch_cuda):
+    x = torch.randn((2, 8, 3, 3), device='cuda')
+    leaf = x.clone().requires_grad_()
+    mid = leaf * 1
+    y = torch_module.group_norm_act(mid.to(memory_format=torch.channels_last).contiguous(memory_format=torch.channels_last), 2)
+    torch.autograd.grad(y.sum(), leaf)
+    with pytest.raises(RuntimeError, match='second time'):
+        torch.autograd.grad(y.sum(), leaf)
+    w = torch.ones(8, device='cuda', requires_grad=True)
+    v = w * 1
+    y = torch_module.group_norm_act(x, 2, v)
+    v.add_(1)
+    with pytest.raises(RuntimeError, match='inplace operation'):
+        torch.autograd.grad(y.sum(), w)
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused(native, torch_cuda):
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn((2, 8, 3, 3), device='cuda', requires_grad=True)
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            torch_module.group_norm_act(fwd.make_dual(x, torch.ones_like(x)), 2)
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            torch_module.dropout(fwd.make_dual(x, torch.ones_like(x)), 0.5)
+
+
+FIRST_USE = """
+import torch
+from groupconv_atlas_b200 import torch_module
+x = torch.randn(4, 64, 40, 40, device='cuda').to(memory_format=torch.channels_last)
+w = torch.randn(4, 45, 30, 30, device='cuda').to(memory_format=torch.channels_last)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    a = [t.requires_grad_() for t in (x, w)]
+    y = [torch_module.group_norm_act(a[0], 8, activation='silu', dropout=0.1),
+         torch_module.group_norm_act(a[1], 9, activation='relu6'), torch_module.dropout(a[0], 0.2, scope='channel')]
+    g = torch.autograd.grad(y, a, [torch.ones_like(t) for t in y])
+graph.replay()
+torch.cuda.synchronize()
+assert all(bool(torch.isfinite(t).all()) for t in (*y, *g)) and bool(y[1].any())
+"""
+
+
+@pytest.mark.gpu
+def test_first_use_inside_a_capture(native, torch_cuda):
+    """Nothing that a first call sets up disturbs a capture."""
+    import subprocess
+    import sys
+    done = subprocess.run([sys.executable, '-c', FIRST_USE], cwd=api.ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_two_threads_and_streams(native, torch_cuda):
+    """Calls of two host threads on streams of their own do not meet."""
+    import threading
+    inputs = [make((3, 64, 30, 30), torch.bfloat16, seed)[0].cuda() for seed in (18, 19)]
+    want = [torch_module.group_norm_act(x, 8, activation='silu') for x in inputs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(50):
+                got = torch_module.group_norm_act(inputs[i], 8, activation='silu')
+                stream.synchronize()
+                if not torch.equal(got, want[i]):
+                    bad.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
+
+
+@pytest.mark.gpu
 def test_no_double_backward(native, torch_cuda):
     x = torch.randn((1, 8, 3, 3), device='cuda', requires_grad=True)
     y = torch_module.group_norm_act(x, 2)
@@ -583,17 +705,16 @@ def test_front_end_refusals(native):
 
 @pytest.mark.gpu
 def test_device_refusals(native, torch_cuda):
-    x = torch.randn((2, 8, 30, 30), device='cuda').to(memory_format=torch.channels_last)
+    x = torch.randn((1, 8, 1000, 600), device='cuda').to(memory_format=torch.channels_last)
     y = torch.full_like(x, 7.0)
     need = native.group_norm_workspace(x, y, 2)
-    if need:
+    assert need > 0
+    for workspace in (None, space(need - 16), space(need + 16)[8:], torch.empty(need, dtype=torch.uint8).pin_memory()):
         with pytest.raises(api.NativeError) as err:
-            native.group_norm(x, y, 2)
+            native.group_norm(x, y, 2, workspace=workspace)
         assert err.value.status == api.GC_INVALID
-        with pytest.raises(api.NativeError):
-            native.group_norm(x, y, 2, workspace=space(need + 16)[8:])
-        with pytest.raises(api.NativeError):
-            native.group_norm(x, y, 2, workspace=torch.empty(need, dtype=torch.uint8).pin_memory())
+    with pytest.raises(api.NativeError):
+        native.group_norm(x, y, 2, workspace=x)
     with pytest.raises(api.NativeError):
         torch_module.group_norm_act(x, 2, torch.ones(8))  # parameters in host memory
     with pytest.raises(api.NativeError):
