@@ -410,7 +410,7 @@ struct Keeper {
 // is not written by the launches that this one follows, so its first copies
 // are issued before the wait for their results.
 template <class T, int V, int ACT, bool DROP>
-__global__ void __launch_bounds__(kNormThreads, DROP ? 2 : split_blocks(V, false)) norm_apply_kernel(const __grid_constant__ NormParams P) {
+__global__ void __launch_bounds__(kNormThreads, split_blocks(V, false)) norm_apply_kernel(const __grid_constant__ NormParams P) {
     extern __shared__ __align__(16) unsigned char nsm[];
     uint4 *ring = reinterpret_cast<uint4 *>(nsm);
     const SplitPlace at = split_place(P, V);

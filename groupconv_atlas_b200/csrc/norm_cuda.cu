@@ -486,8 +486,9 @@ void set_param(const gc_tensor *t, const void *&p, int &type) {
 }
 
 // ---- kernel tables --------------------------------------------------------------------------
-// The vector kernels without dropout are compiled for each activation; the
-// others choose it at run time.
+// The vector kernels without dropout are compiled for each activation, those
+// with dropout for SiLU (the gradient of N8 C128 256x256 bf16 takes 150 us
+// instead of 166); the others choose it at run time.
 enum NormKernel { kMoments, kApply, kGradSums, kGradApply };
 
 template <class T, int V, int ACT, bool DROP>
@@ -503,6 +504,7 @@ template <class T>
 const void *norm_typed(NormKernel k, bool vec, int act, bool drop) {
     constexpr int V = gcb::kVec<T>;
     if (!vec) return drop ? norm_instance<T, 1, -1, true>(k) : norm_instance<T, 1, -1, false>(k);
+    if (drop && act == gcb::kActSilu) return norm_instance<T, V, gcb::kActSilu, true>(k);
     if (drop) return norm_instance<T, V, -1, true>(k);
     if (act == gcb::kActRelu) return norm_instance<T, V, gcb::kActRelu, false>(k);
     if (act == gcb::kActRelu6) return norm_instance<T, V, gcb::kActRelu6, false>(k);
@@ -525,6 +527,7 @@ template <class T>
 const void *resident_typed(bool backward, bool vec, int act, bool drop) {
     constexpr int V = gcb::kVec<T>;
     if (!vec) return drop ? resident_instance<T, 1, -1, true>(backward) : resident_instance<T, 1, -1, false>(backward);
+    if (drop && act == gcb::kActSilu) return resident_instance<T, V, gcb::kActSilu, true>(backward);
     if (drop) return resident_instance<T, V, -1, true>(backward);
     if (act == gcb::kActRelu) return resident_instance<T, V, gcb::kActRelu, false>(backward);
     if (act == gcb::kActRelu6) return resident_instance<T, V, gcb::kActRelu6, false>(backward);

@@ -236,14 +236,20 @@ at::Tensor norm_forward(const at::Tensor &x, const at::Tensor &gamma, const at::
     if (gamma.defined()) gd = describe_view(gamma);
     if (beta.defined()) bd = describe_view(beta);
     if (stats.defined()) sd = describe_view(stats);
-    uint64_t bytes = 0;
-    int st = gc_b200_group_norm_workspace(&xd, &yd, a.groups, &bytes);
-    if (st != GC_OK) fail(st);
-    const at::Tensor space = workspace_of(bytes, x);
-    st = gc_b200_group_norm(&xd, gamma.defined() ? &gd : nullptr, beta.defined() ? &bd : nullptr, &yd,
-                            stats.defined() ? &sd : nullptr, a.groups, a.eps, static_cast<int>(a.activation),
-                            drop.on ? &drop.args : nullptr, space.defined() ? space.data_ptr() : nullptr, bytes,
-                            stream_of(x));
+    // The resident path needs no workspace, so the call is tried without one
+    // first; the query costs small calls a tenth of their host time.
+    auto call = [&](void *space, uint64_t bytes) {
+        return gc_b200_group_norm(&xd, gamma.defined() ? &gd : nullptr, beta.defined() ? &bd : nullptr, &yd,
+                                  stats.defined() ? &sd : nullptr, a.groups, a.eps, static_cast<int>(a.activation),
+                                  drop.on ? &drop.args : nullptr, space, bytes, stream_of(x));
+    };
+    int st = call(nullptr, 0);
+    if (st == GC_INVALID) {
+        uint64_t bytes = 0;
+        if ((st = gc_b200_group_norm_workspace(&xd, &yd, a.groups, &bytes)) != GC_OK) fail(st);
+        const at::Tensor space = workspace_of(bytes, x);
+        st = call(space.defined() ? space.data_ptr() : nullptr, bytes);
+    }
     if (st != GC_OK) fail(st);
     return y;
 }

@@ -214,15 +214,21 @@ def fuse_conv_bn_act(module: torch.nn.Module, predicate, native: api.Native | No
     return replaced
 
 
-def _front_end(name: str):
-    """An entry point of the C++ front end, which these operators need: their
-    gradients are recorded with autograd there."""
-    try:
-        from . import _gcb_torch
-    except ImportError as e:
-        raise FileNotFoundError('the PyTorch front end is not built: '
-                                'groupconv_atlas_b200.build.build_torch_ext()') from e
-    return getattr(_gcb_torch, name)
+_ops = None
+
+
+def _front_end():
+    """The C++ front end, which these operators need: their gradients are
+    recorded with autograd there."""
+    global _ops
+    if _ops is None:
+        try:
+            from . import _gcb_torch
+        except ImportError as e:
+            raise FileNotFoundError('the PyTorch front end is not built: '
+                                    'groupconv_atlas_b200.build.build_torch_ext()') from e
+        _ops = _gcb_torch
+    return _ops
 
 
 def _native_call(op, *args):
@@ -237,9 +243,10 @@ def _native_call(op, *args):
 
 
 def _scope_code(scope: str) -> int:
-    if scope not in api.DROP_SCOPES:
+    code = api.DROP_SCOPES.get(scope)
+    if code is None:
         raise ValueError(f"dropout scope must be one of {', '.join(api.DROP_SCOPES)}")
-    return api.DROP_SCOPES[scope]
+    return code
 
 
 def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
@@ -259,10 +266,11 @@ def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = N
     see include/groupconv.h; without one they come from torch's CUDA generator,
     also inside a graph capture.  Differentiable once; the gradient draws the
     mask again, so none is stored."""
-    if activation not in api.NORM_ACTIVATIONS:
+    act = api.NORM_ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {', '.join(api.NORM_ACTIVATIONS)}")
-    return _native_call(_front_end('group_norm'), x, weight, bias, groups, eps, api.NORM_ACTIVATIONS[activation],
-                        dropout, _scope_code(scope), seed, offset)
+    return _native_call((_ops or _front_end()).group_norm, x, weight, bias, groups, eps, act, dropout,
+                        _scope_code(scope), seed, offset)
 
 
 def dropout(x: torch.Tensor, p: float, residual: torch.Tensor | None = None, scope: str = 'element',
@@ -271,7 +279,7 @@ def dropout(x: torch.Tensor, p: float, residual: torch.Tensor | None = None, sco
     axes.  A decision goes by its element's place in memory (scope 'element')
     or by image and channel (scope 'channel'); a residual of other strides than
     x is copied first.  seed and offset as in group_norm_act."""
-    return _native_call(_front_end('dropout'), x, residual, p, _scope_code(scope), seed, offset)
+    return _native_call((_ops or _front_end()).dropout, x, residual, p, _scope_code(scope), seed, offset)
 
 
 def _norm_activation_name(act: torch.nn.Module | None) -> str:
