@@ -12,16 +12,16 @@
 // z and x - mean come from the same two operations in both directions, so the
 // gradient sees the activation's argument that the forward pass saw.
 //
-// Two paths.  The resident path (end of this file) reads x, and dy, once: a
-// cluster of CTAs holds all pixels of some whole groups of an image in shared
-// memory.  It takes every tensor whose pixels are multiples of 16 bytes and
-// whose groups fit.
+// Two paths, of which the host takes the one that it estimates to be faster.
+// The resident path (end of this file) reads x, and dy, once: a cluster of CTAs
+// holds all pixels of some whole groups of an image in shared memory.  One
+// launch forward, two for the gradient.
 //
-// The split path runs for every supported tensor: partial results of chunks of
-// pixels per channel, one reduction per group, and a second pass over the
-// data.  A vector of V channels per thread (16 bytes, or one element where a
-// pixel is not a multiple of 16 bytes); a block covers up to 256 vector columns
-// and walks down its chunk of pixels.
+// The split path takes what does not fit: partial results of chunks of pixels
+// per channel, one reduction per group, and a second pass over the data.
+//
+// In both a thread works on vectors of V channels: 16 bytes, or one element
+// where a pixel is not a multiple of 16 bytes.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -245,6 +245,9 @@ struct Moments {
 
 // Per chunk and channel: mean and squares about it.  The threads' moments are
 // moved to one pivot per channel, the mean of pixel lane 0, and then add up.
+// Bound by the memory once a launch's fixed 7 us are behind (first copies,
+// sums across the block, SMs that finish late): N8 C128 256x256 bf16, 134 MB,
+// 29 us.
 template <class T, int V>
 __global__ void __launch_bounds__(kNormThreads, split_blocks(V, false)) norm_moments_kernel(const __grid_constant__ NormParams P) {
     extern __shared__ __align__(16) unsigned char nsm[];
@@ -408,7 +411,8 @@ struct Keeper {
 // Normalises, activates and drops out: the second pass over x, from a chunk's
 // end to its start, because the first pass left the ends in the L2 cache.  x
 // is not written by the launches that this one follows, so its first copies
-// are issued before the wait for their results.
+// are issued before the wait for their results.  N8 C128 256x256 bf16 with
+// SiLU: 268 MB read and written in 42 us (6.4 TB/s).
 template <class T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(kNormThreads, split_blocks(V, false)) norm_apply_kernel(const __grid_constant__ NormParams P) {
     extern __shared__ __align__(16) unsigned char nsm[];
@@ -464,7 +468,8 @@ __device__ __forceinline__ Lanes<V> grad_result(int act, const Coefs<V> &k, cons
     return r;
 }
 
-// Per chunk and channel: sum dz, sum dz (x - mean).
+// Per chunk and channel: sum dz, sum dz (x - mean).  N8 C128 256x256 bf16 with
+// SiLU: 268 MB in 47 us (5.7 TB/s).
 template <class T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(kNormThreads, DROP ? 2 : split_blocks(V, true)) norm_grad_sums_kernel(const __grid_constant__ NormParams P) {
     extern __shared__ __align__(16) unsigned char nsm[];
@@ -548,7 +553,8 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_finalize_kernel(const 
     }
 }
 
-// The second pass over x and dy, like norm_apply_kernel.
+// The second pass over x and dy, like norm_apply_kernel.  The same shape: 403 MB
+// in 63 us (6.4 TB/s); with dropout the generator's products bound both.
 template <class T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(kNormThreads, DROP ? 2 : split_blocks(V, true)) norm_grad_apply_kernel(const __grid_constant__ NormParams P) {
     extern __shared__ __align__(16) unsigned char nsm[];
@@ -629,6 +635,15 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_params_kernel(const __
 // arithmetic and stores with the next unit's loads.  Only the sums cross
 // threads (shared memory) and CTAs (distributed shared memory), in a fixed
 // order.
+//
+// Measured (forward, SiLU): N32 C256 56x56 bf16 27 us, of which 4.4 us are the
+// first load at the memory's rate, 2 x 4 us first pass and sums, 7 us a second
+// pass that stores and loads (memory) and 6.6 us one that only stores (issue
+// slots and special functions); the tensor is 1.7 times what the SMs hold.
+// N16 C256 14x14 FP32 4.8 us, N1 C32 56x56 FP32 4.5 us (latencies: a load, two
+// block barriers, one cluster barrier, a store).  Gradient of N32 C256 28x28
+// bf16 19 us: load 4.7, first pass 3.4, sums 2.2, second pass 4.1, the launch
+// that adds up the parameters' gradients 3.
 
 namespace cg = cooperative_groups;
 

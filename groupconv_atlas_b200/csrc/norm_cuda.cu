@@ -234,16 +234,22 @@ bool vector_access(std::initializer_list<const View *> views) {
 }
 
 // The split path's work split: blocks of up to 256 vector columns and chunks
-// of pixels such that one wave of blocks streams everything, but at least eight pixels for each thread.  (Launching
-// sets of images small enough for the second pass to find them in the L2 cache
-// was slower: a set's three launches cost about 10 us beside its data, N8 C128
-// 256x256 bf16 forward 78 us in one set, 108 us in four.)
+// of pixels such that one wave of blocks streams everything, but at least eight
+// pixels for each thread.  Two waves where a thread has 64 vectors even then,
+// because the SMs are not served alike (N64 C128 112x112 FP32 forward: 211 us
+// in one wave, 200 in two; N8 C128 256x256 bf16: 71 and 77).  Launching sets of
+// images small enough for the second pass to find them in the L2 cache was
+// slower: a set's three launches cost about 10 us beside its data (the latter
+// shape: 78 us in one set, 108 in four).
 void plan_split(NormParams &P, int v, bool backward, int sms) {
     P.vcols = P.c / v;
     P.cblocks = static_cast<int>(ceil_div(P.vcols, gcb::kNormThreads));
     P.vb = static_cast<int>(ceil_div(P.vcols, P.cblocks));
     P.lanes = gcb::kNormThreads / P.vb;
-    const long long wanted = std::max<long long>(1, static_cast<long long>(gcb::split_blocks(v, backward)) * sms / (P.n * P.cblocks));
+    const long long wave = static_cast<long long>(gcb::split_blocks(v, backward)) * sms;
+    // vectors of a thread if one wave of blocks takes everything
+    const long long each = ceil_div(P.n * P.px, wave * P.lanes) * P.cblocks;
+    const long long wanted = std::max<long long>(1, (each >= 128 ? 2 : 1) * wave / (P.n * P.cblocks));
     P.chunk_rows = std::min(P.px, std::max<long long>(ceil_div(P.px, wanted), 8LL * P.lanes));
     P.chunks = static_cast<int>(ceil_div(P.px, P.chunk_rows));
     P.items = P.n * P.chunks * P.cblocks;
@@ -882,8 +888,12 @@ int gc_b200_dropout(const gc_tensor *x, const gc_tensor *residual, gc_tensor *y,
     bool vec = gcb::aligned16(P.x) && gcb::aligned16(P.y) && gcb::aligned16(P.residual);
     const int type = elem_type(x->dtype), per_vector = type == gcb::kElemF32 ? 4 : 8;
     DropoutKernel kind = kElements;
-    const long long wave = 3LL * facts.sms, threads = gcb::kStreamThreads;  // one wave of blocks
-    long long grid = std::min<long long>(ceil_div(count, threads * (vec ? per_vector : 1)), wave);
+    // Blocks: up to four waves of them, so that the SMs that are served faster
+    // take more, but for more than one wave at least eight vectors a thread
+    // (N32 C256 56x56 FP32 40 us in one wave, 35 in four).
+    const long long wave = 3LL * facts.sms, threads = gcb::kStreamThreads;
+    const long long vectors = ceil_div(count, vec ? per_vector : 1);
+    long long grid = std::max(std::min(ceil_div(vectors, threads), wave), std::min(ceil_div(vectors, 8 * threads), 4 * wave));
     if (drop.channel) {
         const long long images = x->dims[0], channels = x->dims[1], px = count / images / channels;
         if (channels > INT32_MAX) return gc_error(GC_UNSUPPORTED, "channel count out of range");
@@ -893,11 +903,11 @@ int gc_b200_dropout(const gc_tensor *x, const gc_tensor *residual, gc_tensor *y,
         if (plain && px > 1) {
             kind = kPlanes;
             const long long warps = threads / 32, least = 32LL * (vec ? 4 * per_vector : gcb::kAhead);
-            const long long wanted = std::max<long long>(1, wave * warps / (images * channels));
+            const long long wanted = std::max<long long>(1, 4 * wave * warps / (images * channels));
             P.chunk = static_cast<uint64_t>(gcb::round_up(ceil_div(px, wanted), least));
             P.chunks = (P.row + P.chunk - 1) / P.chunk;
             grid = static_cast<long long>(
-                std::min<uint64_t>((P.decisions * P.chunks + warps - 1) / warps, static_cast<uint64_t>(wave)));
+                std::min<uint64_t>((P.decisions * P.chunks + warps - 1) / warps, static_cast<uint64_t>(4 * wave)));
         } else {
             kind = kChannels;
             vec = vec && channels % per_vector == 0;
@@ -905,8 +915,8 @@ int gc_b200_dropout(const gc_tensor *x, const gc_tensor *residual, gc_tensor *y,
             P.cblocks = static_cast<int>(ceil_div(P.vcols, threads));
             P.vb = static_cast<int>(ceil_div(P.vcols, P.cblocks));
             P.lanes = static_cast<int>(threads / P.vb);
-            const long long wanted = std::max<long long>(1, wave / (images * P.cblocks));
-            P.chunk = static_cast<uint64_t>(std::max<long long>(ceil_div(px, wanted), 4LL * P.lanes));
+            const long long wanted = std::max<long long>(1, (vec ? 4 : 1) * wave / (images * P.cblocks));
+            P.chunk = static_cast<uint64_t>(std::max<long long>(ceil_div(px, wanted), (vec ? 8LL : 4LL) * P.lanes));
             P.chunks = (P.row + P.chunk - 1) / P.chunk;
             const wide blocks = static_cast<wide>(images) * static_cast<wide>(P.chunks) * P.cblocks;
             if (blocks > INT32_MAX) return gc_error(GC_UNSUPPORTED, "more images than a grid has blocks");
