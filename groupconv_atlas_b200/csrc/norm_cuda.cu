@@ -269,7 +269,7 @@ uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
 struct NormPlan {
     bool vec = false;
     int type = 0;
-    bool resident = false;
+    bool resident = false, small = false;
     int threads = gcb::kNormThreads;
     size_t smem = 0;
     int width() const { return !vec ? 1 : type == gcb::kElemF32 ? 4 : 8; }  // elements of a vector
@@ -285,6 +285,10 @@ struct NormSpace {  // the workspace's parts, in this order
 NormSpace space_of(const NormParams &P, const NormPlan &plan, bool backward) {
     NormSpace s;
     const uint64_t n = P.n;
+    if (plan.small) {
+        if (backward) s.part = up16(static_cast<uint64_t>(P.nblocks) * P.c * sizeof(float2));
+        return s;
+    }
     if (plan.resident) {
         if (backward) s.part = up16(static_cast<uint64_t>(P.stride * P.cluster) * P.c * sizeof(float2));
         return s;
@@ -346,7 +350,8 @@ struct ResidentKey {
     }
 };
 struct ResidentPlan {
-    bool ok = false;
+    bool ok = false, small = false;
+    double cost = 0.0;  // of the resident or split path
     int cb = 0, threads = 0, cluster = 0;
     size_t smem = 0;
 };
@@ -407,11 +412,14 @@ double resident_cost(const NormParams &P, int v, int slot, int threads, size_t s
                                    crowd * (v == 1 ? 0.147 : v == 4 ? 0.112 : 0.225) * (backward ? 1.33 : 1.0));
     return 0.4 + kb / 190.0 + rounds * (first + sums + second) + (backward ? 1.0 : 0.0);
 }
-// The same for the split path.
-double split_cost(const NormParams &P, int v, int slot, bool backward) {
+// The same for the split path.  Images that are more than a wave of blocks
+// cost a block's fixed time for each further wave, in both data passes.
+double split_cost(const NormParams &P, int v, int slot, bool backward, const gcb::DeviceFacts &f) {
+    const double blocks = static_cast<double>(P.n) * ceil_div(P.c / v, gcb::kNormThreads);
+    const double extra = 5.0 * std::max(0.0, blocks / (gcb::split_blocks(v, backward) * f.sms) - 1.0);
     const double elements = static_cast<double>(P.n) * P.px * P.c, mb = elements * slot / v * 1e-6;
-    if (v == 1) return backward ? 10.0 + elements * 4.76e-6 : 15.3 + elements * (slot == 4 ? 6.4e-6 : 2.1e-6);
-    return backward ? 10.0 + 2 * mb / 6.0 + 3 * mb / 6.6 : 15.3 + mb / 5.5 + 2 * mb / 6.6;
+    if (v == 1) return extra + (backward ? 10.0 + elements * 4.76e-6 : 15.3 + elements * (slot == 4 ? 6.4e-6 : 2.1e-6));
+    return extra + (backward ? 10.0 + 2 * mb / 6.0 + 3 * mb / 6.6 : 15.3 + mb / 5.5 + 2 * mb / 6.6);
 }
 
 std::mutex g_mutex;
@@ -420,7 +428,7 @@ std::map<ResidentKey, ResidentPlan> g_resident;
 ResidentPlan choose_resident(const NormParams &base, int v, int slot, bool backward, bool bits,
                              const gcb::DeviceFacts &f) {
     ResidentPlan best;
-    double best_cost = split_cost(base, v, slot, backward);
+    double best_cost = split_cost(base, v, slot, backward, f);
     const int unit = std::lcm(base.cpg, v);  // channels: whole groups and whole vectors
     const int units = base.c / unit;
     for (int m = 1; m <= units && static_cast<long long>(m) * unit / v <= gcb::kNormThreads; ++m) {
@@ -442,7 +450,27 @@ ResidentPlan choose_resident(const NormParams &base, int v, int slot, bool backw
                 }
             }
     }
+    best.cost = best_cost;
     return best;
+}
+
+// The small path: threads per group so that each holds about four elements.
+// False where a group is too large for a warp.
+bool set_small(NormParams &P, int sms) {
+    if (static_cast<wide>(P.px) * P.cpg > 32 * 16) return false;
+    const int elements = static_cast<int>(P.px) * P.cpg;
+    P.team = 1;
+    while (P.team < 32 && 4 * P.team < elements) P.team *= 2;
+    P.gb = std::min(P.groups, gcb::kNormThreads / P.team);
+    P.gblocks = static_cast<int>(ceil_div(P.groups, P.gb));
+    const long long images = gcb::kNormThreads / P.team / P.gb;
+    P.nblocks = std::min(ceil_div(P.n, images), std::max<long long>(1, ceil_div(8LL * sms, P.gblocks)));
+    return P.nblocks * P.gblocks <= INT32_MAX;
+}
+// Its time in the same units: element accesses reach about 2 TB/s.
+double small_cost(const NormParams &P, int v, int slot, bool backward) {
+    const double mb = static_cast<double>(P.n) * P.px * P.c * slot / v * 1e-6;
+    return (backward ? 5.0 : 3.0) + (backward ? 3.0 : 2.0) * mb / 2.0;
 }
 
 int plan_norm(NormParams &P, NormPlan &plan, bool backward) {
@@ -469,8 +497,14 @@ int plan_norm(NormParams &P, NormPlan &plan, bool backward) {
         }
         if (!known) {
             r = choose_resident(P, v, plan.slot(), backward, backward, facts);
+            NormParams Q = P;
+            r.small = set_small(Q, facts.sms) && small_cost(P, v, plan.slot(), backward) < r.cost;
             std::lock_guard<std::mutex> lock(g_mutex);
             g_resident[key] = r;
+        }
+        if (r.small) {
+            plan.small = set_small(P, facts.sms);
+            return GC_OK;
         }
         if (r.ok) {
             set_resident(P, v, plan.slot(), r.cb, r.cluster, r.threads, backward, backward, facts.smem_optin, plan.smem);
@@ -544,6 +578,20 @@ const void *resident_kernel(const NormPlan &plan, bool backward, int act, bool d
     if (plan.type == gcb::kElemF16) return resident_typed<__half>(backward, plan.vec, act, drop);
     if (plan.type == gcb::kElemBF16) return resident_typed<__nv_bfloat16>(backward, plan.vec, act, drop);
     return resident_typed<float>(backward, plan.vec, act, drop);
+}
+
+template <class T>
+const void *small_typed(bool backward, bool four) {
+    return backward ? (four ? reinterpret_cast<const void *>(&gcb::norm_small_kernel<T, 4, true>)
+                            : reinterpret_cast<const void *>(&gcb::norm_small_kernel<T, 16, true>))
+                    : (four ? reinterpret_cast<const void *>(&gcb::norm_small_kernel<T, 4, false>)
+                            : reinterpret_cast<const void *>(&gcb::norm_small_kernel<T, 16, false>));
+}
+const void *small_kernel(const NormParams &P, const NormPlan &plan, bool backward) {
+    const bool four = P.px * P.cpg <= 4LL * P.team;
+    if (plan.type == gcb::kElemF16) return small_typed<__half>(backward, four);
+    if (plan.type == gcb::kElemBF16) return small_typed<__nv_bfloat16>(backward, four);
+    return small_typed<float>(backward, four);
 }
 
 // Opts a kernel into the shared memory and the cluster sizes it may be
@@ -727,6 +775,13 @@ int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
     P.part = reinterpret_cast<float2 *>(w + space.stats);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
+    if (plan.small) {
+        if (stats == nullptr) P.stats = nullptr;
+        e = launch(small_kernel(P, plan, false), P.nblocks * P.gblocks, P, s);
+        gcb::record_plan(PlanRecord::kNorm, "small", false, P.nblocks * P.gblocks, gcb::kNormThreads, 0, 1,
+                         P.gb * P.cpg, P.px, 0, 1);
+        return launched(e);
+    }
     if (plan.resident) {
         if (stats == nullptr) P.stats = nullptr;
         if ((st = launch_resident(P, plan, false, dev, s, e)) != GC_OK) return st;
@@ -824,6 +879,16 @@ int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
     cudaError_t e = cudaSuccess;
     const bool params = P.dgamma != nullptr || P.dbeta != nullptr;
     const void *sums = reinterpret_cast<const void *>(&gcb::norm_grad_params_kernel);
+    if (plan.small) {
+        if (!params) P.part = nullptr;
+        e = launch(small_kernel(P, plan, true), P.nblocks * P.gblocks, P, s);
+        P.chan = P.part;
+        P.sum_rows = P.nblocks;
+        if (e == cudaSuccess && params) e = launch(sums, ceil_div(P.c, 32), P, s);
+        gcb::record_plan(PlanRecord::kNorm, "small_backward", false, P.nblocks * P.gblocks, gcb::kNormThreads, 0, 1,
+                         P.gb * P.cpg, P.px, 0, params ? 2 : 1);
+        return launched(e);
+    }
     if (plan.resident) {
         if (!params) P.part = nullptr;
         if ((st = launch_resident(P, plan, true, dev, s, e)) != GC_OK) return st;

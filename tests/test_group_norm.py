@@ -20,7 +20,7 @@ SHAPES = [((1, 32, 7, 7), 8), ((2, 45, 5, 9), 9), ((3, 40, 11, 13), 4), ((2, 96,
           ((4, 48, 1000), 6), ((70, 64), 8), ((2, 16, 300, 2), 16), ((2, 30, 64, 65), 2), ((1, 512, 40, 3), 1),
           ((3, 7, 1), 7), ((1, 1040, 5, 6), 2), ((2, 128, 64, 64), 32),
           # more images than the GPU holds at once: a cluster takes several in turn
-          ((600, 64, 4, 4), 4), ((900, 15, 5, 3), 5), ((1300, 24, 2, 2), 1)]
+          ((600, 64, 4, 4), 4), ((900, 15, 5, 3), 5), ((1300, 24, 2, 2), 1), ((600, 64, 8, 8), 4), ((600, 63, 6, 6), 3)]
 
 # Groups too large for shared memory, by vectors and by single elements.
 SPLIT_SHAPES = [((1, 64, 300, 260), 1), ((2, 255, 100, 90), 1)]
@@ -111,13 +111,30 @@ def test_groups_that_are_read_twice(native, torch_cuda, dims, groups, dtype, p, 
     assert 'split_backward' in native.last_plan()
 
 
+# Many images of few pixels: one element a group, a vector's worth, none of
+# these, as many as a warp holds, more groups than a block's threads.
+SMALL_SHAPES = [((5000, 24, 2, 2), 3), ((3001, 40), 5), ((2003, 45, 3, 3), 5), ((30000, 8, 4, 5), 1), ((6000, 7), 7),
+                ((1500, 600, 1), 300)]
+
+
 @pytest.mark.gpu
-@pytest.mark.parametrize('dims,groups', [((600, 64, 4, 4), 4), ((900, 15, 5, 3), 5)])
+@pytest.mark.parametrize('dims,groups', SMALL_SHAPES, ids=[f'{"x".join(map(str, d))}g{g}' for d, g in SMALL_SHAPES])
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('p,scope,act', [(0.0, 'element', 'silu'), (0.25, 'element', 'none'), (0.25, 'channel', 'relu6')])
+def test_many_images_of_few_pixels(native, torch_cuda, dims, groups, dtype, p, scope, act):
+    x, gamma, beta, dy = make(dims, TYPES[dtype], 22)
+    check_step(native, x, gamma, beta, dy, groups, act, p, scope)
+    assert 'small_backward' in native.last_plan()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dims,groups,path', [((600, 64, 8, 8), 4, 'resident'), ((900, 15, 5, 3), 5, ''),
+                                              ((600, 63, 6, 6), 3, ''), ((600, 64, 4, 4), 4, '')])
 @pytest.mark.parametrize('scope', ['element', 'channel'])
-def test_dropout_of_many_images(native, torch_cuda, dims, groups, scope):
+def test_dropout_of_many_images(native, torch_cuda, dims, groups, path, scope):
     x, gamma, beta, dy = make(dims, torch.bfloat16, 21)
     check_step(native, x, gamma, beta, dy, groups, 'silu', 0.5, scope)
-    assert 'resident_backward' in native.last_plan()
+    assert path in native.last_plan()
 
 
 @pytest.mark.gpu
