@@ -16,8 +16,10 @@ constexpr unsigned kStatusMmaTimeout = 0x2u;
 // gives up: two seconds of GPU global time.  Normal waits take microseconds.
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 
-// Status word of this library on each device (one translation unit holds
-// all device code, so the definition lives here).
+// Status word of this library on each device.  Every kernel that waits with a
+// limit is in one translation unit, conv_cuda.cu, whose copy
+// gc_b200_device_status reads; the others include this header for its copies
+// and barriers only.
 __device__ unsigned int g_status = 0;
 
 __device__ __forceinline__ void raise_status(unsigned bits) { atomicOr(&g_status, bits); }

@@ -710,11 +710,14 @@ const void *dropout_typed(DropoutKernel k, bool vec) {
     return vec ? dropout_instance<T, gcb::kVec<T>>(k) : dropout_instance<T, 1>(k);
 }
 
+// Host memory that ran out must not leave a C entry point as an exception.
+int internal_error() { return gc_error(GC_DEVICE_ERROR, "host resources exhausted"); }
+
 }  // namespace
 
 extern "C" {
 
-int gc_b200_group_norm_workspace(const gc_tensor *x, const gc_tensor *y, int64_t groups, uint64_t *bytes) {
+int gc_b200_group_norm_workspace(const gc_tensor *x, const gc_tensor *y, int64_t groups, uint64_t *bytes) try {
     if (bytes == nullptr) return gc_error(GC_INVALID, "null size pointer");
     View v[2];
     NormParams P;
@@ -727,11 +730,13 @@ int gc_b200_group_norm_workspace(const gc_tensor *x, const gc_tensor *y, int64_t
     if (st != GC_OK) return st;
     *bytes = space_of(P, plan, false).total();
     return gc_error(GC_OK, "");
+} catch (...) {
+    return internal_error();
 }
 
 int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tensor *beta, gc_tensor *y,
                        gc_tensor *stats, int64_t groups, double eps, int activation,
-                       const gc_b200_dropout_args *dropout, void *workspace, uint64_t workspace_bytes, void *stream) {
+                       const gc_b200_dropout_args *dropout, void *workspace, uint64_t workspace_bytes, void *stream) try {
     View v[2];
     NormParams P;
     NormPlan plan;
@@ -795,10 +800,12 @@ int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
     gcb::record_plan(PlanRecord::kNorm, "split", false, P.items, gcb::kNormThreads, 0, 1, P.vb, P.chunk_rows,
                      plan.vec ? 1 : 0, 3);
     return launched(e);
+} catch (...) {
+    return internal_error();
 }
 
 int gc_b200_group_norm_backward_workspace(const gc_tensor *dy, const gc_tensor *x, const gc_tensor *dx,
-                                          int64_t groups, uint64_t *bytes) {
+                                          int64_t groups, uint64_t *bytes) try {
     if (bytes == nullptr) return gc_error(GC_INVALID, "null size pointer");
     View v[3];
     NormParams P;
@@ -811,13 +818,15 @@ int gc_b200_group_norm_backward_workspace(const gc_tensor *dy, const gc_tensor *
     if (st != GC_OK) return st;
     *bytes = space_of(P, plan, true).total();
     return gc_error(GC_OK, "");
+} catch (...) {
+    return internal_error();
 }
 
 int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const gc_tensor *gamma,
                                 const gc_tensor *beta, const gc_tensor *stats, gc_tensor *dx, gc_tensor *dgamma,
                                 gc_tensor *dbeta, int64_t groups, int activation,
                                 const gc_b200_dropout_args *dropout, void *workspace, uint64_t workspace_bytes,
-                                void *stream) {
+                                void *stream) try {
     View v[3];
     NormParams P;
     NormPlan plan;
@@ -908,10 +917,12 @@ int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
     gcb::record_plan(PlanRecord::kNorm, "split_backward", false, P.items, gcb::kNormThreads, 0, 1, P.vb, P.chunk_rows,
                      plan.vec ? 1 : 0, params ? 4 : 3);
     return launched(e);
+} catch (...) {
+    return internal_error();
 }
 
 int gc_b200_dropout(const gc_tensor *x, const gc_tensor *residual, gc_tensor *y,
-                    const gc_b200_dropout_args *dropout, void *stream) {
+                    const gc_b200_dropout_args *dropout, void *stream) try {
     int64_t count = 0;
     for (const gc_tensor *t : {x, static_cast<const gc_tensor *>(y), residual}) {
         if (t == nullptr && t == residual && x != nullptr && y != nullptr) continue;
@@ -998,6 +1009,8 @@ int gc_b200_dropout(const gc_tensor *x, const gc_tensor *residual, gc_tensor *y,
     static const char *const names[] = {"element", "channels_last", "planes"};
     gcb::record_plan(PlanRecord::kDropout, names[kind], false, grid, gcb::kStreamThreads, vec ? 1 : 0);
     return launched(e);
+} catch (...) {
+    return internal_error();
 }
 
 }  // extern "C"

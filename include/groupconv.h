@@ -267,9 +267,10 @@ int gc_b200_dropout(const gc_tensor *x, const gc_tensor *residual, gc_tensor *y,
 int gc_b200_autotune(const gc_shape *p, const gc_tensor *x, const gc_tensor *w,
                      gc_tensor *y, int candidates, void *stream);
 
-/* Launch plan chosen by the last successful gc_cuda_conv / gc_b200_conv call
- * on the calling thread: kernel family name, grid, block, shared memory and
- * work split, as one line of text.  Empty before the first launch. */
+/* Launch plan chosen by the last successful gc_cuda_conv, gc_b200_conv,
+ * gc_b200_group_norm, its gradient or gc_b200_dropout call on the calling
+ * thread: kernel family name, grid, block, shared memory and work split, as
+ * one line of text.  Empty before the first launch. */
 const char *gc_b200_last_plan(void);
 
 /* Device-side status word shared by every kernel of this library on the
