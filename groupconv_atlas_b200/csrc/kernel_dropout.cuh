@@ -1,6 +1,7 @@
 // Dropout from the counter-based generator, with an optional residual sum.
 //
-// dropout_kernel          one decision per element
+// dropout_kernel          one decision per element, or (MAP) per channel of
+//                         many small images in either order
 // channel_dropout_kernel  one decision per channel of an image, channels last
 // plane_dropout_kernel    the same in plain order
 // A decision per channel is drawn once for all the pixels that a thread takes.
@@ -19,6 +20,7 @@ struct DropoutParams {
     uint64_t decisions;        // images * channels
     uint64_t row;              // pixels of an image
     uint64_t chunk, chunks;    // pixels per block (channels last) or warp (plain), chunks of an image or plane
+    uint64_t image;            // MAP: elements of an image, channels last; 0 in plain order
     int channels, vcols, vb, cblocks, lanes;  // channels last: columns as in the norm's split path
     DropParams drop;
 };
@@ -46,10 +48,36 @@ __device__ __forceinline__ void drop_vectors(uint4 *ring, const T *x, const T *r
     }
 }
 
+// The channel of an image that element i belongs to.
+__device__ __forceinline__ uint64_t decision_of(const DropoutParams &P, uint64_t i) {
+    if (P.count <= 0xffffffffu) {  // for the shorter division
+        const uint32_t k = static_cast<uint32_t>(i), c = static_cast<uint32_t>(P.channels);
+        if (P.image == 0) return k / static_cast<uint32_t>(P.row);
+        return k / static_cast<uint32_t>(P.image) * c + k % c;
+    }
+    return P.image == 0 ? i / P.row : i / P.image * P.channels + i % P.channels;
+}
+
+// The decisions on the V elements from i, a multiple of V; channels last, V
+// divides the channels.
+template <int V>
+__device__ __forceinline__ uint32_t mapped_bits(const DropoutParams &P, const Philox &gen, uint64_t i) {
+    uint64_t j = decision_of(P, i);
+    if (P.image != 0) return Draws<V>(gen, j).bits(P.drop.limit);
+    uint64_t left = (j + 1) * P.row - i;  // of the plane that i lies in
+    uint32_t bits = 0;
+    for (int k = 0; k < V; left = P.row, ++j) {
+        const int take = static_cast<int>(min(left, static_cast<uint64_t>(V - k)));
+        if (Draws<1>(gen, j).keep(0, P.drop.limit)) bits |= ((1u << take) - 1u) << k;
+        k += take;
+    }
+    return bits;
+}
+
 // Two neighbouring threads of an FP32 tensor compute the same generator block,
 // which costs less than accesses of half a sector.  16-bit tensors are bound
 // by the generator's products (19 of 32 x 32 -> 64 bits for eight elements).
-template <class T, int V>
+template <class T, int V, bool MAP>
 __global__ void __launch_bounds__(kStreamThreads, 3) dropout_kernel(const __grid_constant__ DropoutParams P) {
     extern __shared__ __align__(16) unsigned char nsm[];
     griddep_wait();
@@ -66,12 +94,14 @@ __global__ void __launch_bounds__(kStreamThreads, 3) dropout_kernel(const __grid
         drop_vectors<T, V>(reinterpret_cast<uint4 *>(nsm), x + V * g, res == nullptr ? res : res + V * g, y + V * g,
                            static_cast<long long>(V * step), count, [&](int k, const Lanes<V> &v) {
                                if (P.drop.threshold == 0) return v;
-                               return drop_lanes<V>(v, Draws<V>(gen, V * (g + k * step)), P.drop);
+                               const uint64_t i = V * (g + k * step);
+                               if constexpr (MAP) return drop_lanes<V>(v, mapped_bits<V>(P, gen, i), P.drop);
+                               else return drop_lanes<V>(v, Draws<V>(gen, i), P.drop);
                            });
     }
     const uint64_t i = whole * V + first;  // fewer than V elements are left
     if (i < P.count) {
-        const bool keep = P.drop.threshold == 0 || Draws<1>(gen, i).keep(0, P.drop.limit);
+        const bool keep = P.drop.threshold == 0 || Draws<1>(gen, MAP ? decision_of(P, i) : i).keep(0, P.drop.limit);
         float v = keep ? to_float(x[i]) * P.drop.scale : 0.0f;
         if (res != nullptr) v += to_float(res[i]);
         y[i] = from_float<T>(v);

@@ -146,6 +146,74 @@ def test_places_past_32_bits(native, torch_cuda):
     assert abs(float((y[: 1 << 20] != 0).double().mean()) - 0.5) < 0.01
 
 
+# Planes from a few elements to several vectors of a warp, images from one to
+# thousands: each kernel of the channel decisions, with and without whole
+# vectors, and places where a vector spans several planes.
+CHANNEL_SHAPES = [(700, 24, 2, 2), (300, 20, 3, 5), (129, 64, 4, 4), (2000, 9, 1, 2), (513, 16), (37, 48, 11, 11),
+                  (5, 48, 17, 31), (3, 45, 19, 29), (2, 1, 3, 7), (64, 3, 1, 3)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('shape', CHANNEL_SHAPES, ids=lambda s: 'x'.join(map(str, s)))
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('layout', ['nchw', 'nhwc'])
+@pytest.mark.parametrize('shift', [0, 1])
+def test_channel_decisions(native, torch_cuda, shape, dtype, layout, shift):
+    g = torch.Generator().manual_seed(6)
+    n = int(np.prod(shape))
+
+    def place(t):  # behind `shift` elements of a guarded buffer
+        b = torch.full((n + 16,), 7.0, dtype=TYPES[dtype], device='cuda')
+        t = b[shift:shift + n].as_strided(t.shape, t.stride(), shift).copy_(t)
+        return t, b
+
+    x, r = (torch.randn(shape, generator=g).to(TYPES[dtype]) for _ in range(2))
+    if layout == 'nhwc':
+        x, r = channels_last(x), channels_last(r)
+    for residual in (None, r):
+        want, tol, keep = expected(x, 0.4, 3, 2 ** 40, 'channel', layout, residual)
+        out, guard = place(torch.zeros_like(x))
+        run(native, place(x)[0], 0.4, 3, 2 ** 40, 'channel', None if residual is None else place(residual)[0], out)
+        assert_close(out, want, tol, native.last_plan())
+        assert (guard[:shift] == 7).all() and (guard[shift + n:] == 7).all()
+    pixels, size = n // shape[0] // shape[1], x.element_size()
+    small = pixels * size < 512 if layout == 'nchw' else pixels * size * shape[1] <= 8192
+    if shape[1] > 1:  # with one channel the two orders are one
+        engine = 'element' if pixels == 1 else 'small_images' if small else 'planes' if layout == 'nchw' else 'channels_last'
+        assert f'engine={engine} ' in native.last_plan()
+
+
+def blocks_of_draws(first, count, seed, offset):
+    """The draws of `count` generator blocks from block `first` on; seed and
+    offset below 2^32."""
+    u, low = np.uint64, np.uint64(0xFFFFFFFF)
+    at = np.arange(first, first + count, dtype=u)
+    c = [at & low, at >> u(32), np.full(count, offset, u), np.zeros(count, u)]
+    for i in range(10):
+        k0, k1 = u((seed + i * 0x9E3779B9) & 0xFFFFFFFF), u((i * 0xBB67AE85) & 0xFFFFFFFF)
+        a, b = c[0] * u(0xD2511F53), c[2] * u(0xCD9E8D57)
+        c = [(b >> u(32)) ^ c[1] ^ k0, b & low, (a >> u(32)) ^ c[3] ^ k1, a & low]
+    return torch.from_numpy(np.stack(c, 1).astype('<u4').reshape(-1).view('<u2').astype(np.int64))
+
+
+def test_blocks_of_draws():
+    assert torch.equal(blocks_of_draws(3, 4, 8, 9), torch.from_numpy(philox(56, 8, 9)[24:].astype(np.int64)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('layout', ['nchw', 'nhwc'])
+def test_small_images_past_32_bits(native, torch_cuda, layout):
+    """Places above 2^32 of 2^28 + 2 images of 8 channels and 2 pixels."""
+    n = (1 << 28) + 2
+    if torch.cuda.mem_get_info()[0] < 5 * 16 * n:
+        pytest.skip('needs 20 GB of device memory')
+    x = torch.ones(16 * n, dtype=torch.bfloat16, device='cuda')
+    x = x.view(n, 8, 1, 2) if layout == 'nchw' else x.view(n, 1, 2, 8).permute(0, 3, 1, 2)
+    y = run(native, x, 0.5, 8, 9, 'channel')
+    keep = (blocks_of_draws(n - 4, 4, 8, 9) >= 32768).view(4, 8, 1, 1).expand(4, 8, 1, 2)
+    assert torch.equal(y[-4:].cpu() != 0, keep) and 'engine=small_images ' in native.last_plan()
+
+
 # ---- the torch front end ----------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', TYPES)
