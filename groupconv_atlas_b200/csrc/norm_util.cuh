@@ -342,23 +342,28 @@ __device__ __forceinline__ void for_vector_pairs(uint4 *ring, const T *p, long l
 __host__ __device__ inline size_t ring_space(int v) { return v == 1 ? 0 : kRing * kStreamThreads * sizeof(uint4); }
 
 // ---- activations --------------------------------------------------------------------
-// 1 / (1 + 2^(-z log2 e)) of two values with three of the special-function
-// unit's instructions instead of four (that unit, a sixteenth of an SM's issue
-// width, bounds the 16-bit kernels): one reciprocal serves both,
-// 1 / p = q / (p q).  The power is held at 2^62 so that p q stays finite; z
-// below -43 then gives 2^-62 where the exact value is smaller still.  The
-// approximate instructions are good to about 2^-22 relative each, and the
-// rounding of z log2 e moves the power by at most |z| 2^-24.
-__device__ __forceinline__ f2 sigmoid2(f2 z) {
+// s = 1 / p, p = 1 + e, e = 2^(-z log2 e), and rest = 1 - s = e s of two values,
+// with three of the special-function unit's instructions instead of four (that
+// unit, a sixteenth of an SM's issue width, bounds the 16-bit kernels): one
+// reciprocal serves both, r = 1 / (p q 2^-126), 1 / p = (q 2^-126) r.  The scale
+// lets e go up to 2^127 in both: p q 2^-126 then is infinite and r 0.  e is held
+// there, and s, below the normal numbers, becomes 0: z s is 0 for every finite z
+// below -88, and NaN at -inf like v / (1 + exp(-v)).  (Branches for what leaves
+// the range kept the pairs from overlapping and cost up to 16 %.)  1 - s is e s
+// and not a difference because the slope multiplies it by z: the reciprocal's
+// error would grow with z.  The approximate instructions are good to about 2^-22
+// relative each, and the rounding of z log2 e moves the power by at most |z| 2^-24.
+__device__ __forceinline__ void sigmoid2(f2 z, f2 &s, f2 &rest) {
     float a, b, p, q, r;
     split(z * pair(-1.4426950408889634f), a, b);
-    a = fminf(a, 62.0f);
-    b = fminf(b, 62.0f);
+    a = fminf(a, 127.0f);
+    b = fminf(b, 127.0f);
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
-    split(pair(a, b) + pair(1.0f), p, q);
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(p * q));
-    return pair(q, p) * pair(r);
+    split(fma2(pair(a, b), pair(0x1p-126f), pair(0x1p-126f)), p, q);  // p 2^-126, q 2^-126
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(p, b, p)));
+    asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(s.v) : "l"(pair(q, p).v), "l"(pair(r).v));
+    rest = pair(a, b) * s;
 }
 
 // Comparisons are written so that a NaN passes through.
@@ -369,7 +374,11 @@ __device__ __forceinline__ float relu6(float z) { return z < 0.0f ? 0.0f : z > 6
 template <int ACT>
 __device__ __forceinline__ f2 activate(int act, f2 z) {
     if constexpr (ACT >= 0) act = ACT;
-    if (act == kActSilu) return z * sigmoid2(z);
+    if (act == kActSilu) {
+        f2 s, rest;
+        sigmoid2(z, s, rest);
+        return z * s;
+    }
     if (act == kActNone) return z;
     float a, b;
     split(z, a, b);
@@ -381,8 +390,9 @@ template <int ACT>
 __device__ __forceinline__ f2 activate_grad(int act, f2 z, f2 g) {
     if constexpr (ACT >= 0) act = ACT;
     if (act == kActSilu) {
-        const f2 s = sigmoid2(z);
-        return g * (s * fma2(z, fma2(s, pair(-1.0f), pair(1.0f)), pair(1.0f)));
+        f2 s, rest;
+        sigmoid2(z, s, rest);
+        return g * (s * fma2(z, rest, pair(1.0f)));
     }
     if (act == kActNone) return g;
     float a, b, ga, gb;

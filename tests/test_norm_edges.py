@@ -1,0 +1,95 @@
+"""Group norm and dropout at the edges of their ranges: arguments far from zero,
+several images a cluster, long sums, and calls that the front end refuses."""
+import numpy as np
+import pytest
+import torch
+
+from tests.norm_helpers import HALF, K, TINY, U, NormReference, assert_close
+from tests.test_group_norm import TYPES, make, run_backward, run_forward
+
+# ---- arguments of SiLU far from zero --------------------------------------------------------------
+# The resident path by vectors and by single elements, the small path, the split path.
+FAR_SHAPES = [((2, 32, 6, 7), 4, 'resident'), ((2, 45, 5, 9), 9, 'resident'), ((5000, 24, 2, 2), 3, 'small'),
+              ((1, 64, 300, 260), 1, 'split'), ((1, 255, 100, 90), 1, 'split')]
+FAR = {0: -1e12, 3: -1e20, 5: -3e38, 6: 3e38, 9: 1e12, 10: -1e4, 12: 1e4}  # channel: beta
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dims,groups,path', FAR_SHAPES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('params', ['f32', 'bf16'])
+def test_silu_of_arguments_far_from_zero(native, torch_cuda, dims, groups, path, dtype, params):
+    """Below -1e3 silu and its slope are 0 in every type, above 1e3 they are z
+    and 1.  dx, dgamma and dbeta are therefore those of a beta of 40 in the high
+    channels (where the slope differs from 1 by 2e-16) and of dy = 0 in the low
+    ones."""
+    if params == 'bf16' and dtype != 'bf16':
+        pytest.skip('parameters are FP32 or of the data type')
+    x, gamma, beta, dy = make(dims, TYPES[dtype], 30)
+    gamma, beta = gamma.to(TYPES[params]), beta.to(TYPES[params])
+    far = beta.clone()
+    low, high = torch.zeros(dims[1], dtype=torch.bool), torch.zeros(dims[1], dtype=torch.bool)
+    for c, value in FAR.items():
+        far[c], beta[c] = value, 40.0 if value > 0 else 0.0
+        (high if value > 0 else low)[c] = True
+    dy[:, low] = 0
+    ref = NormReference(x, groups, gamma, beta, 1e-5, 'silu').backward(dy)
+    given = dy.clone(memory_format=torch.preserve_format)
+    given[:, low] = 3.0  # what the slope has to hide
+    y, stats = run_forward(native, x.cuda(), groups, gamma.cuda(), far.cuda(), act='silu')
+    assert f'engine={path} ' in native.last_plan()
+    dx, dgamma, dbeta = run_backward(native, given.cuda(), x.cuda(), stats, groups, gamma.cuda(), far.cuda(), 'silu')
+    y, rest = y.cpu(), ~(low | high)
+    assert (y[:, low] == 0).all()
+    assert_close(y[:, rest], ref.y[:, rest], ref.tol_y[:, rest], 'y')
+    for c in torch.nonzero(high).flatten().tolist():
+        want = ref.xhat[:, c] * ref.gamma[:, c] + far[c].double()
+        if x.dtype == torch.float16 and far[c] > 1e5:
+            assert (y[:, c] == float('inf')).all()  # past the type's range
+        else:
+            tol = (HALF[x.dtype] + 16 * U) * want.abs() + ref.err[:, c] * ref.gamma[:, c].abs() * (ref.xhat[:, c].abs() + 1)
+            assert_close(y[:, c], want, tol, f'y at {float(far[c])}')
+    assert_close(dx, ref.dx, ref.tol_dx, f'dx [{native.last_plan()}]')
+    for name, got in (('dgamma', dgamma), ('dbeta', dbeta)):
+        want = getattr(ref, name)
+        assert_close(got, want, getattr(ref, 'tol_' + name) + HALF[got.dtype] * want.abs() + 2.0 ** -25, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dims,groups,path', FAR_SHAPES)
+@pytest.mark.parametrize('dtype', TYPES)
+def test_silu_and_its_slope_over_the_whole_range(native, torch_cuda, dims, groups, path, dtype):
+    """With gamma = 0, z is beta and dbeta the slope times the sum of dy (1 here).
+    The exponential is off by 2 |z| u (the product with log2 e and that
+    constant) and 4 u, the sum, product, reciprocal and products behind it by
+    another 8 u: (2 |z| + 12) u of s and of 1 - s.  The sigmoid below 2^-126 is 0."""
+    c, count = dims[1], int(np.prod(dims)) // dims[1]
+    x = make(dims, TYPES[dtype], 31)[0].cuda()
+    beta = torch.linspace(-110, 110, c)
+    gamma = torch.zeros(c)
+    y, stats = run_forward(native, x, groups, gamma.cuda(), beta.cuda(), act='silu')
+    _, _, dbeta = run_backward(native, torch.ones_like(x), x, stats, groups, gamma.cuda(), beta.cuda(), 'silu')
+    z = beta.double()
+    s, t = torch.sigmoid(z), torch.sigmoid(-z)
+    e = (2 * z.abs() + 12) * U
+    tiny = 128 * 2.0 ** -126
+    shape = (1, c) + (1,) * (len(dims) - 2)
+    want = z * s
+    tol = (e + HALF[x.dtype]) * want.abs() + tiny + TINY[x.dtype]
+    assert_close(y, want.reshape(shape), tol.reshape(shape), 'y')
+    slope = s * (1 + z * t)
+    tol = s * (1 + 2 * z.abs() * t) * e + K * U * slope.abs() + tiny
+    assert_close(dbeta / count, slope, tol + U * slope.abs(), 'dbeta')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dims,groups', [((2, 32, 6, 7), 4), ((2, 45, 5, 9), 9), ((5000, 24, 2, 2), 3)])
+def test_silu_of_infinities(native, torch_cuda, dims, groups):
+    """v / (1 + exp(-v)) is NaN at -inf and inf at inf; other channels are untouched."""
+    x, gamma, beta, _ = make(dims, torch.float32, 32)
+    ref = NormReference(x, groups, gamma, beta, act='silu')
+    beta[1], beta[4] = float('-inf'), float('inf')
+    y = run_forward(native, x.cuda(), groups, gamma.cuda(), beta.cuda(), act='silu')[0].cpu()
+    assert torch.isnan(y[:, 1]).all() and (y[:, 4] == float('inf')).all()
+    rest = [c for c in range(dims[1]) if c not in (1, 4)]
+    assert_close(y[:, rest], ref.y[:, rest], ref.tol_y[:, rest], 'y')
