@@ -254,6 +254,8 @@ at::Tensor norm_forward(const at::Tensor &x, const at::Tensor &gamma, const at::
     return y;
 }
 
+// Asked of every operand whether it requires a gradient or not: the primal of a
+// dual tensor usually does not, and its tangent would be lost.
 void no_forward_mode(const at::Tensor &t) {
     if (t.defined() && t._fw_grad(/*level=*/0).defined())
         throw std::runtime_error("this operation has no forward-mode derivative");
@@ -316,6 +318,7 @@ at::Tensor group_norm(const at::Tensor &x, const c10::optional<at::Tensor> &gamm
     c10::OptionalDeviceGuard guard;
     if (x.is_cuda()) guard.reset_device(x.device());
     at::Tensor g = gamma.value_or(at::Tensor()), b = beta.value_or(at::Tensor());
+    for (const at::Tensor &t : {x, g, b}) no_forward_mode(t);
     if (g.defined()) g = g.contiguous();
     if (b.defined()) b = b.contiguous();
     const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(g) || wants_grad(b));
@@ -323,7 +326,6 @@ at::Tensor group_norm(const at::Tensor &x, const c10::optional<at::Tensor> &gamm
     const Drop drop = make_drop(x, p, scope, seed, offset, grad);
     const NormArgs a{groups, activation, eps};
     if (!grad) return norm_forward(xi, g, b, a, drop, at::Tensor());
-    for (const at::Tensor &t : {x, g, b}) no_forward_mode(t);
     const at::Tensor stats =
         at::empty({x.size(0), groups, 2}, x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
     at::Tensor y = norm_forward(xi, g, b, a, drop, stats);
@@ -395,12 +397,14 @@ at::Tensor dropout(const at::Tensor &x, const c10::optional<at::Tensor> &residua
     if (x.dim() < 1 || x.dim() > 4) throw std::invalid_argument("input must have 1 to 4 axes");
     c10::OptionalDeviceGuard guard;
     if (x.is_cuda()) guard.reset_device(x.device());
+    const at::Tensor r0 = residual.value_or(at::Tensor());
+    no_forward_mode(x);
+    no_forward_mode(r0);
     // dense in the order of its axes, else copied; channel decisions know two orders
     at::Tensor xi = x;
     const bool plain = x.is_contiguous();
     const bool last = x.dim() == 4 && x.is_contiguous(at::MemoryFormat::ChannelsLast);
     if (!plain && !last && (scope == GC_B200_DROP_CHANNEL || !x.is_non_overlapping_and_dense())) xi = x.contiguous();
-    const at::Tensor r0 = residual.value_or(at::Tensor());
     c10::optional<at::Tensor> r;
     if (r0.defined()) r = laid_out_like(r0, xi);
     const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(r0));
@@ -408,8 +412,6 @@ at::Tensor dropout(const at::Tensor &x, const c10::optional<at::Tensor> &residua
     const at::Tensor ri = r.value_or(at::Tensor());
     at::Tensor y = dropout_forward(xi, ri, drop);
     if (!grad) return y;
-    no_forward_mode(x);
-    no_forward_mode(r0);
     auto node = std::shared_ptr<DropoutGrad>(new DropoutGrad(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(xi, ri));
     node->sizes_ = xi.sizes().vec();

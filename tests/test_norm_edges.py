@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+from groupconv_atlas_b200 import torch_module
 from tests.norm_helpers import HALF, K, TINY, U, NormReference, assert_close
 from tests.test_group_norm import TYPES, make, run_backward, run_forward
 
@@ -93,3 +94,20 @@ def test_silu_of_infinities(native, torch_cuda, dims, groups):
     assert torch.isnan(y[:, 1]).all() and (y[:, 4] == float('inf')).all()
     rest = [c for c in range(dims[1]) if c not in (1, 4)]
     assert_close(y[:, rest], ref.y[:, rest], ref.tol_y[:, rest], 'y')
+
+
+# ---- what the front end refuses -------------------------------------------------------------------
+@pytest.mark.parametrize('grad', [True, False])
+@pytest.mark.parametrize('operand', ['x', 'weight', 'bias', 'dropout x', 'residual'])
+def test_forward_mode_of_any_operand_is_refused(operand, grad):
+    """Duals whose primal requires no gradient too: their tangent would be lost.
+    Refused before anything else, on the host's tensors as on the device's."""
+    import torch.autograd.forward_ad as fwd
+    x, w, b = torch.randn(2, 8, 3, 3), torch.ones(8), torch.zeros(8)
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        dual = lambda name, t: fwd.make_dual(t, torch.ones_like(t)) if name == operand else t
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            if operand in ('dropout x', 'residual'):
+                torch_module.dropout(dual('dropout x', x), 0.5, dual('residual', x.clone()))
+            else:
+                torch_module.group_norm_act(dual('x', x), 2, dual('weight', w), dual('bias', b))
