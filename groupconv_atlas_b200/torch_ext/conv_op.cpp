@@ -14,6 +14,8 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -98,6 +100,15 @@ at::Tensor conv_ex(const at::Tensor &x, const at::Tensor &w, const c10::optional
 
 [[noreturn]] void fail(int status) {
     throw std::runtime_error("gc_status " + std::to_string(status) + ": " + gc_last_error());
+}
+
+// A tracer records what passes through the dispatcher: of these calls only the
+// output's allocation, so that the recorded graph would return memory that
+// nothing writes.
+void no_tracing() {
+    if (torch::jit::tracer::isTracing() ||
+        c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value())
+        throw std::runtime_error("this operation cannot be traced");
 }
 
 // As describe(), for the entry points that also take 16-bit types and strided
@@ -314,6 +325,7 @@ bool wants_grad(const at::Tensor &t) { return t.defined() && t.requires_grad(); 
 at::Tensor group_norm(const at::Tensor &x, const c10::optional<at::Tensor> &gamma,
                       const c10::optional<at::Tensor> &beta, int64_t groups, double eps, int64_t activation, double p,
                       int64_t scope, const c10::optional<uint64_t> &seed, uint64_t offset) {
+    no_tracing();
     if (x.dim() < 2 || x.dim() > 4) throw std::invalid_argument("input must have 2 to 4 axes (N, C, ..)");
     c10::OptionalDeviceGuard guard;
     if (x.is_cuda()) guard.reset_device(x.device());
@@ -394,6 +406,7 @@ struct DropoutGrad : torch::autograd::Node {
 
 at::Tensor dropout(const at::Tensor &x, const c10::optional<at::Tensor> &residual, double p, int64_t scope,
                    const c10::optional<uint64_t> &seed, uint64_t offset) {
+    no_tracing();
     if (x.dim() < 1 || x.dim() > 4) throw std::invalid_argument("input must have 1 to 4 axes");
     c10::OptionalDeviceGuard guard;
     if (x.is_cuda()) guard.reset_device(x.device());

@@ -111,3 +111,15 @@ def test_forward_mode_of_any_operand_is_refused(operand, grad):
                 torch_module.dropout(dual('dropout x', x), 0.5, dual('residual', x.clone()))
             else:
                 torch_module.group_norm_act(dual('x', x), 2, dual('weight', w), dual('bias', b))
+
+
+@pytest.mark.parametrize('call', [lambda x: torch_module.group_norm_act(x, 2), lambda x: torch_module.dropout(x, 0.5)],
+                         ids=['group_norm', 'dropout'])
+def test_tracing_is_refused(call):
+    """A traced graph would hold the output's allocation alone."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.randn(2, 8, 3, 3)
+    with pytest.raises(RuntimeError, match='cannot be traced'):
+        torch.jit.trace(call, (x,))
+    with pytest.raises(RuntimeError, match='cannot be traced'):
+        make_fx(call)(x)
