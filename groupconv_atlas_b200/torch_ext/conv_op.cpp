@@ -45,10 +45,20 @@ gc_tensor describe(const at::Tensor &t) {
     return d;
 }
 
+// A tracer records what passes through the dispatcher: of these calls only the
+// output's allocation, so that the recorded graph would return memory that
+// nothing writes.
+void no_tracing() {
+    if (torch::jit::tracer::isTracing() ||
+        c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value())
+        throw std::runtime_error("this operation cannot be traced");
+}
+
 // y = conv(x, w) with the layer's geometry; x must be 4-D.  Raises
 // RuntimeError("gc_status <s>: <message>") on any non-OK status.
 at::Tensor conv(const at::Tensor &x, const at::Tensor &w, int64_t cout, int64_t r, int64_t s, int64_t groups,
                 int64_t sh, int64_t sw, int64_t ph, int64_t pw, int64_t dh, int64_t dw, int64_t implementation) {
+    no_tracing();
     if (x.dim() != 4) throw std::invalid_argument("input must be 4-D NCHW");
     const gc_shape p{x.size(0), x.size(1), cout, x.size(2), x.size(3), r, s, groups, sh, sw, ph, pw, dh, dw};
     int64_t ho = 0, wo = 0;
@@ -73,6 +83,7 @@ at::Tensor conv(const at::Tensor &x, const at::Tensor &w, int64_t cout, int64_t 
 at::Tensor conv_ex(const at::Tensor &x, const at::Tensor &w, const c10::optional<at::Tensor> &bias, int64_t cout,
                    int64_t r, int64_t s, int64_t groups, int64_t sh, int64_t sw, int64_t ph, int64_t pw, int64_t dh,
                    int64_t dw, int64_t layout, int64_t activation) {
+    no_tracing();
     if (x.dim() != 4) throw std::invalid_argument("input must be 4-D NCHW");
     const gc_shape p{x.size(0), x.size(1), cout, x.size(2), x.size(3), r, s, groups, sh, sw, ph, pw, dh, dw};
     int64_t ho = 0, wo = 0;
@@ -100,15 +111,6 @@ at::Tensor conv_ex(const at::Tensor &x, const at::Tensor &w, const c10::optional
 
 [[noreturn]] void fail(int status) {
     throw std::runtime_error("gc_status " + std::to_string(status) + ": " + gc_last_error());
-}
-
-// A tracer records what passes through the dispatcher: of these calls only the
-// output's allocation, so that the recorded graph would return memory that
-// nothing writes.
-void no_tracing() {
-    if (torch::jit::tracer::isTracing() ||
-        c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value())
-        throw std::runtime_error("this operation cannot be traced");
 }
 
 // As describe(), for the entry points that also take 16-bit types and strided

@@ -35,6 +35,13 @@ def _cpp_conv():
     return _gcb_torch.conv
 
 
+def _no_tracing():
+    """A tracer would record the output's allocation alone (the C++ front end
+    asks the same)."""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError('this operation cannot be traced')
+
+
 class B200Conv2d(torch.nn.Module):
     """Forward-only replacement of a bias-free ``torch.nn.Conv2d``."""
 
@@ -96,6 +103,7 @@ class B200Conv2d(torch.nn.Module):
                     status, _, message = text[len('gc_status '):].partition(': ')
                     raise api.NativeError(int(status), message) from None
                 raise
+        _no_tracing()
         if x.is_cuda and x.get_device() != torch.cuda.current_device():
             # gc_cuda_conv runs on the current device, which must hold the
             # tensors (nn.Conv2d runs on its input's device)
@@ -179,6 +187,7 @@ class B200ConvBNAct(torch.nn.Module):
                     status, _, message = text[len('gc_status '):].partition(': ')
                     raise api.NativeError(int(status), message) from None
                 raise
+        _no_tracing()
         shape = api.Shape(n=x.shape[0], h=x.shape[2], w=x.shape[3], **self.geometry)
         y = torch.empty(shape.output, device=x.device, dtype=x.dtype,
                         memory_format=torch.channels_last if nhwc else torch.contiguous_format)

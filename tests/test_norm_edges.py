@@ -99,7 +99,7 @@ def test_silu_of_infinities(native, torch_cuda, dims, groups):
 # ---- what the front end refuses -------------------------------------------------------------------
 @pytest.mark.parametrize('grad', [True, False])
 @pytest.mark.parametrize('operand', ['x', 'weight', 'bias', 'dropout x', 'residual'])
-def test_forward_mode_of_any_operand_is_refused(operand, grad):
+def test_forward_mode_of_any_operand_is_refused(native, operand, grad):
     """Duals whose primal requires no gradient too: their tangent would be lost.
     Refused before anything else, on the host's tensors as on the device's."""
     import torch.autograd.forward_ad as fwd
@@ -115,7 +115,7 @@ def test_forward_mode_of_any_operand_is_refused(operand, grad):
 
 @pytest.mark.parametrize('call', [lambda x: torch_module.group_norm_act(x, 2), lambda x: torch_module.dropout(x, 0.5)],
                          ids=['group_norm', 'dropout'])
-def test_tracing_is_refused(call):
+def test_tracing_is_refused(native, call):
     """A traced graph would hold the output's allocation alone."""
     from torch.fx.experimental.proxy_tensor import make_fx
     x = torch.randn(2, 8, 3, 3)
@@ -123,3 +123,14 @@ def test_tracing_is_refused(call):
         torch.jit.trace(call, (x,))
     with pytest.raises(RuntimeError, match='cannot be traced'):
         make_fx(call)(x)
+
+
+@pytest.mark.parametrize('front', [True, False], ids=['C++', 'ctypes'])
+def test_tracing_of_a_convolution_is_refused(native, front):
+    conv = torch_module.B200Conv2d(torch.nn.Conv2d(8, 8, 3, groups=2, bias=False), native, cpp=front)
+    fused = torch_module.B200ConvBNAct(torch.nn.Conv2d(8, 8, 3, groups=2), native=native)
+    if not front:
+        fused._op = None
+    for module in (conv, fused):
+        with pytest.raises(RuntimeError, match='cannot be traced'):
+            torch.jit.trace(module, (torch.randn(2, 8, 5, 5),))
