@@ -72,8 +72,8 @@ std::string format_plan(const PlanRecord &r) {
     case PlanRecord::kNorm:
         std::snprintf(buf, sizeof(buf),
                       "kernel=group_norm engine=%s grid=%lld block=%lld smem=%lld cluster=%lld channels=%lld rows=%lld "
-                      "vec=%lld launches=%lld",
-                      r.name, v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
+                      "vec=%lld launches=%lld rounds=%lld",
+                      r.name, v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8]);
         break;
     case PlanRecord::kDropout:
         std::snprintf(buf, sizeof(buf), "kernel=dropout engine=%s grid=%lld block=%lld vec=%lld", r.name, v[0], v[1],

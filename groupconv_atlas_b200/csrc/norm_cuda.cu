@@ -623,6 +623,13 @@ int launch_resident(NormParams &P, const NormPlan &plan, bool backward, int dev,
     return GC_OK;
 }
 
+// Images that a cluster (resident path) or a team of threads (small path) takes
+// in turn, at most; 1 on the split path.
+long long rounds_of(const NormParams &P, const NormPlan &plan) {
+    if (plan.small) return ceil_div(P.n, P.nblocks * (gcb::kNormThreads / P.team / P.gb));
+    return plan.resident ? ceil_div(P.n, P.stride) : 1;
+}
+
 unsigned grid_of(long long items) { return static_cast<unsigned>(std::min<long long>(items, INT32_MAX)); }
 
 cudaError_t launch(const void *fn, long long blocks, NormParams &P, cudaStream_t s, size_t smem = 0) {
@@ -785,21 +792,21 @@ int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
         if (stats == nullptr) P.stats = nullptr;
         e = launch(small_kernel(P, plan, false), P.nblocks * P.gblocks, P, s);
         gcb::record_plan(PlanRecord::kNorm, "small", false, P.nblocks * P.gblocks, gcb::kNormThreads, 0, 1,
-                         P.gb * P.cpg, P.px, 0, 1);
+                         P.gb * P.cpg, P.px, 0, 1, rounds_of(P, plan));
         return launched(e);
     }
     if (plan.resident) {
         if (stats == nullptr) P.stats = nullptr;
         if ((st = launch_resident(P, plan, false, dev, s, e)) != GC_OK) return st;
         gcb::record_plan(PlanRecord::kNorm, "resident", false, static_cast<long long>(P.stride) * P.bundles * P.cluster,
-                         plan.threads, plan.smem, P.cluster, P.cb, P.rows, plan.vec ? 1 : 0, 1);
+                         plan.threads, plan.smem, P.cluster, P.cb, P.rows, plan.vec ? 1 : 0, 1, rounds_of(P, plan));
         return launched(e);
     }
     if ((st = launch_split(kMoments, P, plan, dev, s, e)) != GC_OK) return st;
     if (e == cudaSuccess) e = launch_finalize(false, P, s);
     if (e == cudaSuccess && (st = launch_split(kApply, P, plan, dev, s, e)) != GC_OK) return st;
     gcb::record_plan(PlanRecord::kNorm, "split", false, P.items, gcb::kNormThreads, 0, 1, P.vb, P.chunk_rows,
-                     plan.vec ? 1 : 0, 3);
+                     plan.vec ? 1 : 0, 3, 1);
     return launched(e);
 } catch (...) {
     return internal_error();
@@ -896,7 +903,7 @@ int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
         P.sum_rows = P.nblocks;
         if (e == cudaSuccess && params) e = launch(sums, ceil_div(P.c, 32), P, s);
         gcb::record_plan(PlanRecord::kNorm, "small_backward", false, P.nblocks * P.gblocks, gcb::kNormThreads, 0, 1,
-                         P.gb * P.cpg, P.px, 0, params ? 2 : 1);
+                         P.gb * P.cpg, P.px, 0, params ? 2 : 1, rounds_of(P, plan));
         return launched(e);
     }
     if (plan.resident) {
@@ -907,7 +914,7 @@ int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
         if (e == cudaSuccess && params) e = launch(sums, ceil_div(P.c, 32), P, s);
         gcb::record_plan(PlanRecord::kNorm, "resident_backward", false,
                          static_cast<long long>(P.stride) * P.bundles * P.cluster, plan.threads, plan.smem, P.cluster,
-                         P.cb, P.rows, plan.vec ? 1 : 0, params ? 2 : 1);
+                         P.cb, P.rows, plan.vec ? 1 : 0, params ? 2 : 1, rounds_of(P, plan));
         return launched(e);
     }
     P.sum_rows = P.n;
@@ -916,7 +923,7 @@ int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
     if (e == cudaSuccess && (st = launch_split(kGradApply, P, plan, dev, s, e)) != GC_OK) return st;
     if (e == cudaSuccess && params) e = launch(sums, ceil_div(P.c, 32), P, s);
     gcb::record_plan(PlanRecord::kNorm, "split_backward", false, P.items, gcb::kNormThreads, 0, 1, P.vb, P.chunk_rows,
-                     plan.vec ? 1 : 0, params ? 4 : 3);
+                     plan.vec ? 1 : 0, params ? 4 : 3, 1);
     return launched(e);
 } catch (...) {
     return internal_error();

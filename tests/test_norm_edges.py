@@ -4,9 +4,9 @@ import numpy as np
 import pytest
 import torch
 
-from groupconv_atlas_b200 import torch_module
+from groupconv_atlas_b200 import api, torch_module
 from tests.norm_helpers import HALF, K, TINY, U, NormReference, assert_close
-from tests.test_group_norm import TYPES, make, run_backward, run_forward
+from tests.test_group_norm import TYPES, check_step, make, run_backward, run_forward
 
 # ---- arguments of SiLU far from zero --------------------------------------------------------------
 # The resident path by vectors and by single elements, the small path, the split path.
@@ -94,6 +94,42 @@ def test_silu_of_infinities(native, torch_cuda, dims, groups):
     assert torch.isnan(y[:, 1]).all() and (y[:, 4] == float('inf')).all()
     rest = [c for c in range(dims[1]) if c not in (1, 4)]
     assert_close(y[:, rest], ref.y[:, rest], ref.tol_y[:, rest], 'y')
+
+
+# ---- clusters that take several images in turn ----------------------------------------------------
+# (dims, groups, type, cluster of the forward pass or None where it takes one
+# image, cluster of the gradient or None): 16-byte vectors and single elements
+# (of 16 bits: copied through registers), clusters of one and of several.
+ROUNDS = [((600, 64, 9, 9), 4, 'f32', None, 1), ((600, 96, 12, 11), 1, 'f32', 1, 2), ((600, 96, 12, 11), 1, 'bf16', None, 1),
+          ((200, 64, 20, 21), 1, 'f32', None, 4), ((40, 96, 40, 40), 1, 'f32', 8, None),
+          ((600, 96, 16, 16), 1, 'bf16', 1, 2), ((150, 64, 40, 40), 4, 'f16', 4, None),
+          ((4000, 15, 5, 7), 1, 'f32', None, 1), ((4000, 15, 5, 7), 1, 'f16', None, 1), ((600, 255, 2, 3), 1, 'f32', 1, None),
+          ((600, 255, 2, 3), 1, 'bf16', 1, None), ((150, 130, 9, 9), 2, 'f16', 1, None), ((600, 15, 28, 28), 1, 'f32', 4, None)]
+
+
+def rounds_of(plan):
+    """(engine, cluster, images that a cluster takes in turn)"""
+    fields = dict(f.split('=') for f in plan.split())
+    return fields['engine'], int(fields['cluster']), int(fields['rounds'])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dims,groups,dtype,forward,backward', ROUNDS)
+@pytest.mark.parametrize('p,scope', [(0.0, 'element'), (0.25, 'element'), (0.25, 'channel')])
+def test_clusters_that_take_several_images(native, torch_cuda, dims, groups, dtype, forward, backward, p, scope):
+    """The tiles filled again during the second pass, exchange buffers in turn,
+    statistics loaded for each image, parameter gradients added over images."""
+    if p and dims[0] * dims[1] * dims[2] * dims[3] > 1 << 23:
+        pytest.skip('the smaller shapes cover dropout')
+    x, gamma, beta, dy = make(dims, TYPES[dtype], 33)
+    run_forward(native, x.cuda(), groups, gamma.cuda(), beta.cuda(), act='silu', drop=api.dropout_args(p) if p else None)
+    engine, cluster, rounds = rounds_of(native.last_plan())
+    if forward is not None:
+        assert engine == 'resident' and cluster == forward and rounds >= 2
+    check_step(native, x, gamma, beta, dy, groups, 'silu', p, scope)
+    engine, cluster, rounds = rounds_of(native.last_plan())
+    if backward is not None:
+        assert engine == 'resident_backward' and cluster == backward and rounds >= 2
 
 
 # ---- what the front end refuses -------------------------------------------------------------------
