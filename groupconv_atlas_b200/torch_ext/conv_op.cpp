@@ -294,10 +294,13 @@ struct GroupNormGrad : torch::autograd::Node {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
         no_double_backward();
-        const at::Tensor x = x_.unpack(), gamma = has_gamma_ ? gamma_.unpack() : at::Tensor(),
-                         beta = has_beta_ ? beta_.unpack() : at::Tensor();
+        // Hooks on saved tensors may give them back with other strides (pinned
+        // copies on the host are plain).
+        const at::Tensor saved = x_.unpack();
+        c10::OptionalDeviceGuard guard(saved.device());
+        const at::Tensor x = in_order(saved), gamma = has_gamma_ ? gamma_.unpack().contiguous() : at::Tensor(),
+                         beta = has_beta_ ? beta_.unpack().contiguous() : at::Tensor();
         const Drop drop = again(drop_);
-        c10::OptionalDeviceGuard guard(x.device());
         const at::Tensor dy = in_order(grads[0]);
         at::Tensor dx = empty_channels_last(x), dgamma, dbeta;
         if (has_gamma_ && task_should_compute_output(1)) dgamma = at::empty_like(gamma);

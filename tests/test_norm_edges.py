@@ -1,5 +1,7 @@
 """Group norm and dropout at the edges of their ranges: arguments far from zero,
 several images a cluster, long sums, and calls that the front end refuses."""
+import contextlib
+
 import numpy as np
 import pytest
 import torch
@@ -130,6 +132,26 @@ def test_clusters_that_take_several_images(native, torch_cuda, dims, groups, dty
     engine, cluster, rounds = rounds_of(native.last_plan())
     if backward is not None:
         assert engine == 'resident_backward' and cluster == backward and rounds >= 2
+
+
+# ---- saved tensors that come back with other strides ----------------------------------------------
+HOOKS = {'host': lambda: torch.autograd.graph.save_on_cpu(),
+         'pinned': lambda: torch.autograd.graph.save_on_cpu(pin_memory=True),
+         'strided': lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: torch.stack([t, t], -1)[..., 0])}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('hooks', HOOKS)
+def test_hooks_on_saved_tensors(native, torch_cuda, hooks):
+    x, gamma, beta, dy = (t.cuda() for t in make((2, 24, 6, 7), torch.float32, 34))
+    grads = []
+    for context in (contextlib.nullcontext, HOOKS[hooks]):
+        leaves = [t.clone(memory_format=torch.preserve_format).requires_grad_() for t in (x, gamma, beta)]
+        with context():
+            y = torch_module.group_norm_act(leaves[0] * 1, 4, leaves[1] * 1, leaves[2] * 1, activation='silu')
+        grads.append(torch.autograd.grad(y, leaves, dy))
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
 
 
 # ---- what the front end refuses -------------------------------------------------------------------
