@@ -342,7 +342,8 @@ at::Tensor group_norm(const at::Tensor &x, const c10::optional<at::Tensor> &gamm
     const at::Tensor xi = in_order(x);
     const Drop drop = make_drop(x, p, scope, seed, offset, grad);
     const NormArgs a{groups, activation, eps};
-    if (!grad) return norm_forward(xi, g, b, a, drop, at::Tensor());
+    const bool whole = groups >= 1 && x.size(1) % groups == 0;  // else refused by the call, before stats of that size
+    if (!grad || !whole) return norm_forward(xi, g, b, a, drop, at::Tensor());
     const at::Tensor stats =
         at::empty({x.size(0), groups, 2}, x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
     at::Tensor y = norm_forward(xi, g, b, a, drop, stats);

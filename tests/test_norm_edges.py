@@ -192,3 +192,12 @@ def test_tracing_of_a_convolution_is_refused(native, front):
     for module in (conv, fused):
         with pytest.raises(RuntimeError, match='cannot be traced'):
             torch.jit.trace(module, (torch.randn(2, 8, 5, 5),))
+
+
+@pytest.mark.parametrize('groups', [0, -2, 3, 16, 1 << 40, 1 << 60])
+@pytest.mark.parametrize('grad', [True, False])
+def test_group_counts_are_refused_by_status(native, groups, grad):
+    """With a gradient wanted too, where statistics would be allocated first."""
+    with pytest.raises(api.NativeError) as err:
+        torch_module.group_norm_act(torch.zeros(2, 8, 3, 3, requires_grad=grad), groups)
+    assert err.value.status == api.GC_INVALID
