@@ -220,6 +220,13 @@ int launched(cudaError_t e) {
     else cudaGetLastError();
     return e == cudaSuccess ? gc_error(GC_OK, "") : gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
 }
+// The same, with the plan of a call that succeeded.
+template <class... T>
+int launched(cudaError_t e, PlanRecord::Kind kind, const char *name, T... values) {
+    const int st = launched(e);
+    if (st == GC_OK) gcb::record_plan(kind, name, false, values...);
+    return st;
+}
 
 // ---- group norm: plan ---------------------------------------------------------------------
 int vector_of(const View &v) { return v.type == gcb::kElemF32 ? 4 : 8; }
@@ -791,23 +798,20 @@ int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
     if (plan.small) {
         if (stats == nullptr) P.stats = nullptr;
         e = launch(small_kernel(P, plan, false), P.nblocks * P.gblocks, P, s);
-        gcb::record_plan(PlanRecord::kNorm, "small", false, P.nblocks * P.gblocks, gcb::kNormThreads, 0, 1,
+        return launched(e, PlanRecord::kNorm, "small", P.nblocks * P.gblocks, gcb::kNormThreads, 0, 1,
                          P.gb * P.cpg, P.px, 0, 1, rounds_of(P, plan));
-        return launched(e);
     }
     if (plan.resident) {
         if (stats == nullptr) P.stats = nullptr;
         if ((st = launch_resident(P, plan, false, dev, s, e)) != GC_OK) return st;
-        gcb::record_plan(PlanRecord::kNorm, "resident", false, static_cast<long long>(P.stride) * P.bundles * P.cluster,
+        return launched(e, PlanRecord::kNorm, "resident", static_cast<long long>(P.stride) * P.bundles * P.cluster,
                          plan.threads, plan.smem, P.cluster, P.cb, P.rows, plan.vec ? 1 : 0, 1, rounds_of(P, plan));
-        return launched(e);
     }
     if ((st = launch_split(kMoments, P, plan, dev, s, e)) != GC_OK) return st;
     if (e == cudaSuccess) e = launch_finalize(false, P, s);
     if (e == cudaSuccess && (st = launch_split(kApply, P, plan, dev, s, e)) != GC_OK) return st;
-    gcb::record_plan(PlanRecord::kNorm, "split", false, P.items, gcb::kNormThreads, 0, 1, P.vb, P.chunk_rows,
+    return launched(e, PlanRecord::kNorm, "split", P.items, gcb::kNormThreads, 0, 1, P.vb, P.chunk_rows,
                      plan.vec ? 1 : 0, 3, 1);
-    return launched(e);
 } catch (...) {
     return internal_error();
 }
@@ -902,9 +906,8 @@ int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
         P.chan = P.part;
         P.sum_rows = P.nblocks;
         if (e == cudaSuccess && params) e = launch(sums, ceil_div(P.c, 32), P, s);
-        gcb::record_plan(PlanRecord::kNorm, "small_backward", false, P.nblocks * P.gblocks, gcb::kNormThreads, 0, 1,
+        return launched(e, PlanRecord::kNorm, "small_backward", P.nblocks * P.gblocks, gcb::kNormThreads, 0, 1,
                          P.gb * P.cpg, P.px, 0, params ? 2 : 1, rounds_of(P, plan));
-        return launched(e);
     }
     if (plan.resident) {
         if (!params) P.part = nullptr;
@@ -912,19 +915,17 @@ int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
         P.chan = P.part;
         P.sum_rows = static_cast<long long>(P.stride) * P.cluster;
         if (e == cudaSuccess && params) e = launch(sums, ceil_div(P.c, 32), P, s);
-        gcb::record_plan(PlanRecord::kNorm, "resident_backward", false,
+        return launched(e, PlanRecord::kNorm, "resident_backward",
                          static_cast<long long>(P.stride) * P.bundles * P.cluster, plan.threads, plan.smem, P.cluster,
                          P.cb, P.rows, plan.vec ? 1 : 0, params ? 2 : 1, rounds_of(P, plan));
-        return launched(e);
     }
     P.sum_rows = P.n;
     if ((st = launch_split(kGradSums, P, plan, dev, s, e)) != GC_OK) return st;
     if (e == cudaSuccess) e = launch_finalize(true, P, s);
     if (e == cudaSuccess && (st = launch_split(kGradApply, P, plan, dev, s, e)) != GC_OK) return st;
     if (e == cudaSuccess && params) e = launch(sums, ceil_div(P.c, 32), P, s);
-    gcb::record_plan(PlanRecord::kNorm, "split_backward", false, P.items, gcb::kNormThreads, 0, 1, P.vb, P.chunk_rows,
+    return launched(e, PlanRecord::kNorm, "split_backward", P.items, gcb::kNormThreads, 0, 1, P.vb, P.chunk_rows,
                      plan.vec ? 1 : 0, params ? 4 : 3, 1);
-    return launched(e);
 } catch (...) {
     return internal_error();
 }
@@ -1031,8 +1032,7 @@ int gc_b200_dropout(const gc_tensor *x, const gc_tensor *residual, gc_tensor *y,
     const cudaError_t e = gcb::launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(gcb::kStreamThreads), args,
                                           gcb::ring_space(vec ? per_vector : 1), reinterpret_cast<cudaStream_t>(stream));
     static const char *const names[] = {"element", "channels_last", "planes", "small_images"};
-    gcb::record_plan(PlanRecord::kDropout, names[kind], false, grid, gcb::kStreamThreads, vec ? 1 : 0);
-    return launched(e);
+    return launched(e, PlanRecord::kDropout, names[kind], grid, gcb::kStreamThreads, vec ? 1 : 0);
 } catch (...) {
     return internal_error();
 }
