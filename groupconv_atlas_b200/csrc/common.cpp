@@ -85,7 +85,11 @@ bool ranges_overlap(const gc_tensor *a, const gc_tensor *b) {
 }  // namespace
 
 int gc_error(int status, const char *message) {
-    g_last_error = message != nullptr ? message : "";
+    try {
+        g_last_error = message != nullptr ? message : "";
+    } catch (...) {  // no memory for the message: the status alone
+        g_last_error.clear();
+    }
     return status;
 }
 

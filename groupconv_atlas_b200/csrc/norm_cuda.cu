@@ -725,7 +725,8 @@ const void *dropout_typed(DropoutKernel k, bool vec) {
     return vec ? dropout_instance<T, gcb::kVec<T>>(k) : dropout_instance<T, 1>(k);
 }
 
-// Host memory that ran out must not leave a C entry point as an exception.
+// No exception leaves a C entry point; those that can arise here come from host
+// memory that ran out.
 int internal_error() { return gc_error(GC_DEVICE_ERROR, "host resources exhausted"); }
 
 }  // namespace

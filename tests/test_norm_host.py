@@ -94,3 +94,29 @@ flag('fake_launch_error').value = 2
 assert CALLS[-1]() == api.GC_DEVICE_ERROR and native.last_plan() == plans[0]
 assert flag('fake_launches').value == before + 1
 """)
+
+
+def test_memory_that_runs_out_is_a_status(run):
+    """No exception and no abort leaves an entry point, also where the message
+    itself finds no memory."""
+    run("""
+import threading
+calls = CALLS + [lambda: lib.gc_b200_group_norm_workspace(ref(tensor(*RESIDENT[:1], PLACE)), ref(tensor(*RESIDENT[:1], 2 * PLACE)),
+                                                          4, ref(ct.c_uint64())),
+                 lambda: lib.gc_b200_group_norm_backward_workspace(
+                     *(ref(tensor(*RESIDENT[:1], (i + 1) * PLACE)) for i in range(3)), 4, ref(ct.c_uint64()))]
+for no_memory in (0, 1):
+    for call in calls:
+        got = []
+
+        def work():  # a thread of its own: its message slot is empty
+            flag('fake_throw').value, flag('fake_no_memory').value = 1, no_memory
+            got.append(call())
+            flag('fake_throw').value = flag('fake_no_memory').value = 0
+            got.append(native.lib.gc_last_error())
+        thread = threading.Thread(target=work)
+        thread.start()
+        thread.join()
+        assert got == [api.GC_DEVICE_ERROR, b'' if no_memory else b'host resources exhausted'], got
+assert CALLS[0]() == 0
+""")
