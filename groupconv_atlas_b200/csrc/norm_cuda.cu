@@ -1,7 +1,8 @@
 // gc_b200_group_norm, its gradient, and gc_b200_dropout: descriptor checks,
-// plans and launches.  As in the convolution backend nothing here allocates,
-// synchronizes or keeps state between calls; a call can be captured into a
-// CUDA graph.
+// plans and launches.  As in the convolution backend nothing here allocates
+// device memory or synchronizes, and a call can be captured into a CUDA graph.
+// What is kept between calls: the plans of shapes, as many as kPlans, and which
+// kernels have been opted into their shared memory.
 #include "groupconv.h"
 
 #include <cuda_runtime.h>
@@ -429,6 +430,8 @@ double split_cost(const NormParams &P, int v, int slot, bool backward, const gcb
     return extra + (backward ? 10.0 + 2 * mb / 6.0 + 3 * mb / 6.6 : 15.3 + mb / 5.5 + 2 * mb / 6.6);
 }
 
+// Plans that are kept; a program whose shapes never repeat starts anew there.
+constexpr size_t kPlans = 4096;
 std::mutex g_mutex;
 std::map<ResidentKey, ResidentPlan> g_resident;
 
@@ -507,6 +510,7 @@ int plan_norm(NormParams &P, NormPlan &plan, bool backward) {
             NormParams Q = P;
             r.small = set_small(Q, facts.sms) && small_cost(P, v, plan.slot(), backward) < r.cost;
             std::lock_guard<std::mutex> lock(g_mutex);
+            if (g_resident.size() >= kPlans) g_resident.clear();
             g_resident[key] = r;
         }
         if (r.small) {

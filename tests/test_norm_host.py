@@ -120,3 +120,17 @@ for no_memory in (0, 1):
         assert got == [api.GC_DEVICE_ERROR, b'' if no_memory else b'host resources exhausted'], got
 assert CALLS[0]() == 0
 """)
+
+
+def test_plans_of_many_shapes_are_bounded(run):
+    """A program whose shapes never repeat keeps a bounded number of plans."""
+    run("""
+def use(first, count):
+    for n in range(first, first + count):
+        assert forward((n, 8, 2, 1), 2) == 0
+    return flag('fake_live').value
+use(1, 100)
+start = use(1, 100)
+assert use(1000, 12000) - start <= 5000, flag('fake_live').value - start
+assert use(20000, 6000) - start <= 5000
+""")
