@@ -194,6 +194,7 @@ int check_dropout(const gc_b200_dropout_args *d, DropParams &out) {
 }
 
 Range used_words(const DropParams &d) { return {d.used, d.used != nullptr ? 16u : 0u}; }
+Range given_word(const uint64_t *p) { return {p, p != nullptr ? 8u : 0u}; }
 
 // The current device, the pointers' device and the stream (reference
 // groupconv.cu:130-139, :185-191).
@@ -769,7 +770,8 @@ int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
     DropParams drop;
     if ((st = check_dropout(dropout, drop)) != GC_OK) return st;
     if (outputs_meet({{y->data, v[1].span}, range_of(stats), used_words(drop), {workspace, workspace_bytes}},
-                     {{x->data, v[0].span}, range_of(gamma), range_of(beta)}))
+                     {{x->data, v[0].span}, range_of(gamma), range_of(beta), given_word(drop.seed_ptr),
+                      given_word(drop.offset_ptr)}))
         return gc_error(GC_INVALID, "outputs and workspace must not overlap inputs or one another");
     if (!known_activation(activation)) return gc_error(GC_UNSUPPORTED, "unknown activation");
     for (const gc_tensor *t : {gamma, beta})
@@ -857,7 +859,8 @@ int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
     if ((st = check_dropout(dropout, drop)) != GC_OK) return st;
     if (outputs_meet({{dx->data, v[2].span}, range_of(dgamma), range_of(dbeta), used_words(drop),
                       {workspace, workspace_bytes}},
-                     {{x->data, v[0].span}, {dy->data, v[1].span}, range_of(gamma), range_of(beta), range_of(stats)}))
+                     {{x->data, v[0].span}, {dy->data, v[1].span}, range_of(gamma), range_of(beta), range_of(stats),
+                      given_word(drop.seed_ptr), given_word(drop.offset_ptr)}))
         return gc_error(GC_INVALID, "outputs and workspace must not overlap inputs or one another");
     if (!known_activation(activation)) return gc_error(GC_UNSUPPORTED, "unknown activation");
     for (const gc_tensor *t : {gamma, beta, static_cast<const gc_tensor *>(dgamma),
@@ -950,7 +953,8 @@ int gc_b200_dropout(const gc_tensor *x, const gc_tensor *residual, gc_tensor *y,
     DropParams drop;
     int st = check_dropout(dropout, drop);
     if (st != GC_OK) return st;
-    if (outputs_meet({range_of(y), used_words(drop)}, {range_of(x), range_of(residual)}))
+    if (outputs_meet({range_of(y), used_words(drop)}, {range_of(x), range_of(residual), given_word(drop.seed_ptr),
+                                                       given_word(drop.offset_ptr)}))
         return gc_error(GC_INVALID, "outputs must not overlap inputs");
     if (drop.channel && x->rank < 2) return gc_error(GC_INVALID, "channel dropout needs a channel axis");
     if (x->dtype == GC_F64) return gc_error(GC_UNSUPPORTED, "FP64 tensors are not supported here");

@@ -191,11 +191,11 @@ int gc_b200_conv_ex(const gc_shape *p, const gc_tensor *x, const gc_tensor *w,
  * with different offsets have independent masks.
  *   seed_ptr, offset_ptr   nullable device words, added to seed and offset
  *                          when the kernel runs (so a captured graph can draw
- *                          anew at each replay);
+ *                          anew at each replay).  Inputs of the call: no output
+ *                          and no workspace overlaps them;
  *   used                   nullable device pair that receives the seed and
  *                          offset in effect, for a later gradient (unless t is
- *                          0: nothing is drawn then).  Must not overlap the
- *                          two words above. */
+ *                          0: nothing is drawn then).  An output of the call. */
 typedef struct {
     double p; /* 0 <= p <= 1 */
     uint64_t seed, offset;
@@ -224,8 +224,9 @@ typedef struct {
  *               gc_b200_group_norm_workspace gives for these tensors (NULL
  *               when that is 0); its contents need not be set and are
  *               undefined afterwards.
- * Outputs and workspace overlap neither inputs nor one another.  Validation, device, stream, allocation and
- * capture rules are those of gc_cuda_conv.  Results are bitwise reproducible. */
+ * Outputs and workspace overlap neither inputs nor one another.  Validation,
+ * device, stream, allocation and capture rules are those of gc_cuda_conv.
+ * Results are bitwise reproducible. */
 int gc_b200_group_norm_workspace(const gc_tensor *x, const gc_tensor *y, int64_t groups, uint64_t *bytes);
 int gc_b200_group_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tensor *beta, gc_tensor *y,
                        gc_tensor *stats, int64_t groups, double eps, int activation,

@@ -134,3 +134,34 @@ start = use(1, 100)
 assert use(1000, 12000) - start <= 5000, flag('fake_live').value - start
 assert use(20000, 6000) - start <= 5000
 """)
+
+
+def test_outputs_over_the_generator_s_words_are_refused(run):
+    """Seed and offset words are inputs: the kernels read them while others of
+    their blocks already write."""
+    run("""
+def norm(drop, workspace=6 * PLACE):
+    x, y = tensor((2, 32, 6, 7), PLACE), tensor((2, 32, 6, 7), 2 * PLACE)
+    return lib.gc_b200_group_norm(ref(x), None, None, ref(y), ref(stats(2, 4, 3 * PLACE)), 4, 1e-5, 3, ref(drop),
+                                  workspace, PLACE, None)
+def grad(drop):
+    x, dy, dx = (tensor((2, 32, 6, 7), (i + 1) * PLACE) for i in range(3))
+    dgamma, dbeta = api.Tensor(), api.Tensor()
+    for t, base in ((dgamma, 4 * PLACE), (dbeta, 4 * PLACE + 4096)):
+        t.data, t.bytes, t.device, t.rank, t.dims[0], t.strides[0] = base, 128, 1, 1, 32, 1
+    return lib.gc_b200_group_norm_backward(ref(dy), ref(x), None, None, ref(stats(2, 4, 5 * PLACE)), ref(dx), ref(dgamma),
+                                           ref(dbeta), 4, 3, ref(drop), 6 * PLACE, PLACE, None)
+def drop(args):
+    x, y = tensor((2, 32, 6, 7), PLACE), tensor((2, 32, 6, 7), 2 * PLACE)
+    return lib.gc_b200_dropout(ref(x), None, ref(y), ref(args), None)
+size = 4 * 2 * 32 * 6 * 7
+places = {norm: [2 * PLACE, 2 * PLACE + size - 8, 3 * PLACE + 8, 6 * PLACE + 800, 7 * PLACE - 8, 8 * PLACE],
+          grad: [3 * PLACE + 8, 4 * PLACE + 120, 4 * PLACE + 4096, 6 * PLACE, 8 * PLACE], drop: [2 * PLACE + size - 8, 8 * PLACE]}
+for call, at in places.items():
+    for word in ('seed_ptr', 'offset_ptr'):
+        for p in at:
+            got = call(api.dropout_args(0.5, used=8 * PLACE, **{word: p}))
+            assert got == api.GC_INVALID, (call.__name__, word, hex(p), got)
+        for p in (9 * PLACE, 8 * PLACE + 16, 8 * PLACE - 8):
+            assert call(api.dropout_args(0.5, used=8 * PLACE, **{word: p})) == 0, native.lib.gc_last_error()
+""")
