@@ -340,32 +340,46 @@ class B200Dropout(torch.nn.Module):
         return f'p={self.p}, scope={self.scope}'
 
 
+def _plain(module: torch.nn.Module, kinds: tuple) -> bool:
+    """One of these classes itself (a subclass may compute something else), and
+    without hooks, which a fused call would not run."""
+    return type(module) in kinds and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                                          or module._backward_pre_hooks)
+
+
 def fuse_norm_act(module: torch.nn.Module) -> list[str]:
     """In every Sequential, replace each GroupNorm with the activation (none,
     ReLU, ReLU6, SiLU) and the dropout (Dropout, Dropout2d) that follow it by
     one B200GroupNormAct; the members it takes over become Identity, so every
-    other member keeps its name.  Returns the dotted names replaced."""
+    other member keeps its name.  Subclasses of these and modules with hooks
+    stay as they are.  Returns the dotted names replaced.
+
+    The replacement differs from torch's modules in three ways: it takes 2 to 4
+    axes (a GroupNorm that sees (N, C, D, H, W) has to stay out of the fused
+    module), its result is dense channels last, and of x's type, under autocast
+    too, where torch's group_norm returns float32."""
+    nn = torch.nn
     replaced = []
     for name, child in list(module.named_modules()):
-        if not isinstance(child, torch.nn.Sequential):
+        if not isinstance(child, nn.Sequential):
             continue
         members = list(child._modules.items())
         for at, (attr, norm) in enumerate(members):
-            if not isinstance(norm, torch.nn.GroupNorm):
+            if not _plain(norm, (nn.GroupNorm,)):
                 continue
             act = drop = None
             taken = []
             for follower, sub in members[at + 1:]:
-                if drop is None and isinstance(sub, (torch.nn.Dropout, torch.nn.Dropout2d)):
+                if drop is None and _plain(sub, (nn.Dropout, nn.Dropout2d)):
                     drop = sub
-                elif drop is None and act is None and isinstance(sub, (torch.nn.ReLU, torch.nn.ReLU6, torch.nn.SiLU)):
+                elif drop is None and act is None and _plain(sub, (nn.ReLU, nn.ReLU6, nn.SiLU)):
                     act = sub
                 else:
                     break
                 taken.append(follower)
             child._modules[attr] = B200GroupNormAct(norm, act, drop)
             for follower in taken:
-                child._modules[follower] = torch.nn.Identity()
+                child._modules[follower] = nn.Identity()
             replaced.append(f'{name}.{attr}' if name else attr)
     return replaced
 

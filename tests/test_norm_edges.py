@@ -201,3 +201,34 @@ def test_group_counts_are_refused_by_status(native, groups, grad):
     with pytest.raises(api.NativeError) as err:
         torch_module.group_norm_act(torch.zeros(2, 8, 3, 3, requires_grad=grad), groups)
     assert err.value.status == api.GC_INVALID
+
+
+# ---- modules --------------------------------------------------------------------------------------
+class OwnNorm(torch.nn.GroupNorm):
+    def forward(self, x):
+        return super().forward(x) + 1
+
+
+class OwnReLU(torch.nn.ReLU):
+    def forward(self, x):
+        return super().forward(x) + 1
+
+
+class OwnDropout(torch.nn.Dropout):
+    def forward(self, x):
+        return x
+
+
+def test_fuse_norm_act_leaves_what_may_do_something_else():
+    """Subclasses have a forward of their own, hooks expect to be called."""
+    nn = torch.nn
+    model = nn.Sequential(OwnNorm(2, 8), nn.ReLU(), nn.GroupNorm(2, 8), OwnReLU(), nn.GroupNorm(2, 8), nn.SiLU(),
+                          OwnDropout(0.5), nn.GroupNorm(2, 8), nn.ReLU(), nn.GroupNorm(2, 8), nn.ReLU())
+    model[8].register_forward_hook(lambda m, i, o: None)
+    model[9].register_forward_pre_hook(lambda m, i: None)
+    before = list(model)
+    assert torch_module.fuse_norm_act(model) == ['2', '4', '7']
+    for i in (0, 1, 3, 6, 8, 9, 10):
+        assert model[i] is before[i]
+    assert [model[i].activation for i in (2, 4, 7)] == ['none', 'silu', 'none']
+    assert isinstance(model[5], nn.Identity)
