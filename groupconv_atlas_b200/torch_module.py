@@ -297,8 +297,9 @@ def _norm_activation_name(act: torch.nn.Module | None) -> str:
 
 class B200GroupNormAct(torch.nn.Module):
     """GroupNorm -> activation -> dropout as one call, in training and
-    inference.  Keeps the norm's own parameters (and their names); dropout
-    (torch.nn.Dropout, or Dropout2d for whole channels) acts in training only."""
+    inference.  Keeps the norm's own parameters (and their names) and the
+    dropout (torch.nn.Dropout, or Dropout2d for whole channels) as its member
+    ``drop``, whose own mode and probability decide."""
 
     def __init__(self, norm: torch.nn.GroupNorm, act: torch.nn.Module | None = None,
                  drop: torch.nn.Module | None = None):
@@ -308,13 +309,24 @@ class B200GroupNormAct(torch.nn.Module):
         self.activation = _norm_activation_name(act)
         if drop is not None and not isinstance(drop, (torch.nn.Dropout, torch.nn.Dropout2d)):
             raise ValueError(f'{type(drop).__name__} has no epilogue in gc_b200_group_norm')
-        self.p = drop.p if drop is not None else 0.0
+        self.drop = drop
         self.scope = 'channel' if isinstance(drop, torch.nn.Dropout2d) else 'element'
-        self.train(norm.training)
+        self.training = norm.training
+
+    @property
+    def p(self) -> float:
+        return 0.0 if self.drop is None else self.drop.p
+
+    @p.setter
+    def p(self, value: float) -> None:
+        if self.drop is None:
+            self.drop = torch.nn.Dropout().train(self.training)
+        self.drop.p = value
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        drop = self.drop
         return group_norm_act(x, self.groups, self.weight, self.bias, self.eps, self.activation,
-                              self.p if self.training else 0.0, self.scope)
+                              drop.p if drop is not None and drop.training else 0.0, self.scope)
 
     def extra_repr(self) -> str:
         return f'groups={self.groups}, eps={self.eps}, activation={self.activation}, p={self.p}, scope={self.scope}'

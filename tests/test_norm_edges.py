@@ -232,3 +232,39 @@ def test_fuse_norm_act_leaves_what_may_do_something_else():
         assert model[i] is before[i]
     assert [model[i].activation for i in (2, 4, 7)] == ['none', 'silu', 'none']
     assert isinstance(model[5], nn.Identity)
+
+
+@pytest.mark.parametrize('norm_mode', [True, False])
+@pytest.mark.parametrize('drop_mode', [True, False])
+def test_a_dropout_keeps_its_own_mode(monkeypatch, norm_mode, drop_mode):
+    """Evaluation with the dropout left in training draws, as before the fusion."""
+    nn = torch.nn
+    seen = []
+    monkeypatch.setattr(torch_module, 'group_norm_act',
+                        lambda x, groups, w, b, eps, act, p, scope: seen.append((p, scope)) or x)
+    drop = nn.Dropout2d(0.3)
+    model = nn.Sequential(nn.GroupNorm(2, 8).train(norm_mode), nn.SiLU(), drop.train(drop_mode))
+    keys = list(model.state_dict())
+    torch_module.fuse_norm_act(model)
+    assert model[0].training == norm_mode and list(model.state_dict()) == keys
+    x = torch.zeros(1, 8, 2, 2)
+    model(x)
+    model.eval()(x)
+    for m in model.modules():
+        if isinstance(m, nn.Dropout2d):
+            m.train()
+    model(x)
+    drop.p = 0.5
+    model(x)
+    model[0].p = 0.25
+    model.train()(x)
+    assert seen == [(0.3 if drop_mode else 0.0, 'channel'), (0.0, 'channel'), (0.3, 'channel'), (0.5, 'channel'),
+                    (0.25, 'channel')]
+    assert model[0].p == 0.25 and 'p=0.25' in model[0].extra_repr()
+
+
+def test_a_norm_without_dropout_can_be_given_one():
+    norm = torch_module.B200GroupNormAct(torch.nn.GroupNorm(2, 8).eval())
+    assert norm.p == 0.0
+    norm.p = 0.1
+    assert norm.p == 0.1 and not norm.drop.training and norm.scope == 'element'
