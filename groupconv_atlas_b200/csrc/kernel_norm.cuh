@@ -25,6 +25,13 @@
 //
 // The small path takes many images of few pixels: a few threads hold a whole
 // group of an image in registers.
+//
+// Sums.  An FP32 sum of n values of one sign, added one after the other, is off
+// by up to n half steps, and by a third of that where the values are alike (a
+// mean's gradient).  Here at most kNormRun values, on the resident path a
+// thread's vectors (some 100), are added in a row before sums are joined: by
+// trees, by as many runs again, or in 64 bits where there may be thousands of
+// them (chunks, images).
 #pragma once
 #include <cooperative_groups.h>
 
@@ -90,6 +97,23 @@ template <int V>
 __device__ __forceinline__ f2 normalise(const Coefs<V> &k, int i, f2 x, f2 &d) {
     d = x + k.minus_mean.p[i];
     return fma2(d, k.a.p[i], k.b.p[i]);
+}
+
+// value(i) for i, i + step, .. below end, added in 32 bits over runs of kNormRun
+// and in 64 bits over the runs.  (64-bit additions of each value cost 14 us where
+// a group has 290 chunks of 255 channels.)
+constexpr int kNormRun = 64;
+template <int UNROLL, class I, class F>
+__device__ __forceinline__ float long_sum(I i, I end, I step, F value) {
+    double total = 0.0;
+    while (i < end) {
+        const I stop = (end - i) / kNormRun < step ? end : i + kNormRun * step;
+        float run = 0.0f;
+#pragma unroll UNROLL
+        for (; i < stop; i += step) run += value(i);
+        total += run;
+    }
+    return static_cast<float>(total);
 }
 
 // Sum of v over the block (every thread gets it).  red: 32 floats of shared memory.
@@ -205,7 +229,6 @@ __device__ __forceinline__ SplitPlace split_place(const NormParams &P, int v) {
 // mean that the squares about it exceed those about the mean at most by the
 // factor 64; cancellation in q - s^2 / n costs no more than that many roundings
 // whatever the data's mean.  Runs of 64 are joined as (mean, squares).
-constexpr int kNormRun = 64;
 template <int V>
 struct Moments {
     Lanes<V> minus, s, q;
@@ -334,7 +357,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_finalize_kernel(const __gri
             return part[static_cast<long long>(chunk) * P.c + (i - chunk * P.cpg)];
         };
         float2 held[kHeld];
-        float held_rows[kHeld], s = 0.0f;
+        float held_rows[kHeld], s = 0.0f, q = 0.0f;
 #pragma unroll
         for (int u = 0; u < kHeld; ++u) {
             const unsigned i = me + u * TEAM;
@@ -345,26 +368,23 @@ __global__ void __launch_bounds__(kNormThreads) norm_finalize_kernel(const __gri
 #pragma unroll
         for (int u = 0; u < kHeld; ++u) s = fmaf(held_rows[u], held[u].x, s);
         const unsigned rest = me + kHeld * TEAM;
-#pragma unroll 4
-        for (unsigned i = rest; i < entries; i += TEAM) {
+        s += long_sum<4, unsigned>(rest, entries, TEAM, [&](unsigned i) {
             float rows;
             const float2 v = entry(i, rows);
-            s = fmaf(rows, v.x, s);
-        }
+            return rows * v.x;
+        });
         const float mean = team_sum<TEAM>(s, red) / total;
-        float q = 0.0f;
 #pragma unroll
         for (int u = 0; u < kHeld; ++u) {
             const float d = held[u].x - mean;
             if (held_rows[u] > 0.0f) q += fmaf(held_rows[u] * d, d, held[u].y);
         }
-#pragma unroll 4
-        for (unsigned i = rest; i < entries; i += TEAM) {
+        q += long_sum<4, unsigned>(rest, entries, TEAM, [&](unsigned i) {
             float rows;
             const float2 v = entry(i, rows);
             const float d = v.x - mean;
-            q += fmaf(rows * d, d, v.y);
-        }
+            return fmaf(rows * d, d, v.y);
+        });
         const float var = team_sum<TEAM>(q, red) / total;
         if (me == 0) P.stats[ng] = make_float2(mean, 1.0f / sqrtf(var + P.eps));
     }
@@ -491,15 +511,24 @@ __global__ void __launch_bounds__(kNormThreads, DROP ? 2 : split_blocks(V, true)
     const Affine<V> affine(P, at.c0);
     Keeper<V, DROP> drop(P, false, at.n, at.p0, at.c0, P.lanes);
     const Coefs<V> coefs = split_coefs<V>(P, affine, at.n, at.c0);
-    Lanes<V> s2, t2;
+    Lanes<V> s2, t2, all_s, all_t;  // of a run, of the runs
 #pragma unroll
-    for (int i = 0; i < Lanes<V>::kPairs; ++i) s2.p[i] = t2.p[i] = pair(0.0f);
-    for_vector_pairs<T, V>(ring, x, xstep, dy, gstep, at.count, [&](int, const Lanes<V> &v, const Lanes<V> &g) {
-        grad_sums<V, ACT>(P.act, coefs, v, drop.apply(P, g), s2, t2);
-    });
+    for (int i = 0; i < Lanes<V>::kPairs; ++i) s2.p[i] = t2.p[i] = all_s.p[i] = all_t.p[i] = pair(0.0f);
+    auto join = [&] {
+#pragma unroll
+        for (int i = 0; i < Lanes<V>::kPairs; ++i) {
+            all_s.p[i] = all_s.p[i] + s2.p[i];
+            all_t.p[i] = all_t.p[i] + t2.p[i];
+            s2.p[i] = t2.p[i] = pair(0.0f);
+        }
+    };
+    for_vector_pairs<T, V, kNormRun>(
+        ring, x, xstep, dy, gstep, at.count,
+        [&](int, const Lanes<V> &v, const Lanes<V> &g) { grad_sums<V, ACT>(P.act, coefs, v, drop.apply(P, g), s2, t2); },
+        join);
     float s[V], t[V];
-    values_of<V>(s2, s);
-    values_of<V>(t2, t);
+    values_of<V>(all_s, s);
+    values_of<V>(all_t, t);
     float2 *out = P.part + (at.n * P.chunks + at.chunk) * P.c + at.first;
     __syncthreads();  // the sums' space is the ring's
     channel_sums<V>(P.vb, P.lanes, P.vb * V, at.lane, at.lane < P.lanes ? at.col * V : 0, s, t,
@@ -523,20 +552,29 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_finalize_kernel(const 
         const long long n = ng / P.groups;
         const int c0 = static_cast<int>(ng - n * P.groups) * P.cpg;
         const float2 st = P.stats[ng];
-        float s1 = 0.0f, s2 = 0.0f;
+        double sum1 = 0.0, sum2 = 0.0;
         // four channels at a time, so that their loads are in flight together
         for (int k = 4 * warp; k < P.cpg; k += 4 * (TEAM / 32)) {
             const float2 *part = P.part + n * P.chunks * P.c + c0 + k;
             float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = lane; i < P.chunks;) {
+                const int stop = min(P.chunks, i + 32 * kNormRun);
+                float rs[4] = {0.0f, 0.0f, 0.0f, 0.0f}, rt[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 2
-            for (int i = lane; i < P.chunks; i += 32) {
+                for (; i < stop; i += 32) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (k + j < P.cpg) {
-                        const float2 v = part[static_cast<long long>(i) * P.c + j];
-                        s[j] += v.x;
-                        t[j] += v.y;
-                    }
+                    for (int j = 0; j < 4; ++j)
+                        if (k + j < P.cpg) {
+                            const float2 v = part[static_cast<long long>(i) * P.c + j];
+                            rs[j] += v.x;
+                            rt[j] += v.y;
+                        }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[j] += rs[j];
+                    t[j] += rt[j];
+                }
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -549,13 +587,13 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_finalize_kernel(const 
                     const float w = t[j] * st.y;
                     const float gm = P.gamma ? load_param(P.gamma, P.gamma_type, c0 + k + j) : 1.0f;
                     P.chan[n * P.c + c0 + k + j] = make_float2(s[j], w);
-                    s1 = fmaf(gm, s[j], s1);
-                    s2 = fmaf(gm, w, s2);
+                    sum1 += gm * s[j];
+                    sum2 += gm * w;
                 }
             }
         }
-        s1 = team_sum<TEAM>(s1, red);
-        s2 = team_sum<TEAM>(s2, red);
+        const float s1 = team_sum<TEAM>(static_cast<float>(sum1), red);
+        const float s2 = team_sum<TEAM>(static_cast<float>(sum2), red);
         if (threadIdx.x % TEAM == 0) P.gsum[ng] = make_float2(st.y * s1 / total, st.y * st.y * s2 / total);
     }
 }
@@ -610,13 +648,24 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_params_kernel(const __
     const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
     float s = 0.0f, t = 0.0f;
-    if (c < P.c) {
+    if (c < P.c && row < P.sum_rows) {
+        double sum_s = 0.0, sum_t = 0.0;
+        const float2 *src = P.chan + static_cast<long long>(row) * P.c + c;
+        const long long step = static_cast<long long>(kNormThreads / 32) * P.c;
+        for (long long left = (P.sum_rows - row + kNormThreads / 32 - 1) / (kNormThreads / 32); left > 0; left -= kNormRun) {
+            const int run = static_cast<int>(min(left, static_cast<long long>(kNormRun)));
+            s = t = 0.0f;
 #pragma unroll 8
-        for (long long n = row; n < P.sum_rows; n += kNormThreads / 32) {
-            const float2 v = P.chan[n * P.c + c];
-            s += v.x;
-            t += v.y;
+            for (int u = 0; u < run; ++u, src += step) {
+                const float2 v = *src;
+                s += v.x;
+                t += v.y;
+            }
+            sum_s += s;
+            sum_t += t;
         }
+        s = static_cast<float>(sum_s);
+        t = static_cast<float>(sum_t);
     }
     sm[threadIdx.x] = make_float2(s, t);
     __syncthreads();
@@ -705,7 +754,7 @@ __host__ __device__ inline size_t tile_bytes(int iters, int threads, int slot) {
 // Shared memory of the resident kernels behind the tiles.
 __host__ __device__ inline size_t resident_extra(const NormParams &P, int threads, bool grad) {
     const size_t gb = P.gb, cb = P.cb;
-    const size_t entries = grad ? channel_sums_space(threads, P.vr, P.lanes, P.cb) + 2 * cb
+    const size_t entries = grad ? channel_sums_space(threads, P.vr, P.lanes, P.cb) + 3 * cb
                                 : static_cast<size_t>(P.lanes) * P.vr * P.sub;
     return (entries + 4 * gb) * sizeof(float2);
 }
@@ -962,8 +1011,8 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
     float2 *fin = exch + 2 * P.gb;
     float2 *gst = fin + P.gb;           // mean, rstd of the unit's groups
     float2 *weighted = gst + P.gb;      // [cb]: gamma * the channel's sums
-    float2 *acc = weighted + P.cb;      // [cb]: the channel's sums over this CTA's images
-    float2 *scratch = acc + P.cb;       // channel_sums
+    double *acc = reinterpret_cast<double *>(weighted + P.cb);  // [2][cb]: the channel's sums over this CTA's images
+    float2 *scratch = weighted + 3 * P.cb;                      // channel_sums
     uint8_t *bits = reinterpret_cast<uint8_t *>(scratch + channel_sums_space(threads, P.vr, P.lanes, P.cb));
     const int rank = blockIdx.x % P.cluster;
     const unsigned unit = blockIdx.x / P.cluster;
@@ -994,7 +1043,7 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
             cp_async_commit();
         }
     }
-    for (int c = tid; c < P.cb; c += threads) acc[c] = make_float2(0.0f, 0.0f);
+    for (int c = tid; c < P.cb; c += threads) acc[c] = acc[P.cb + c] = 0.0;
     for (int g = tid; g < P.gb; g += threads) gst[g] = P.stats[(unit / P.bundles) * P.groups + bundle * P.gb + g];
     const Affine<V> affine(P, r.c0);
     Coefs<V> coefs;
@@ -1048,7 +1097,8 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
                 sum.y *= gst[c / P.cpg].y;
                 const float w = P.gamma ? load_param(P.gamma, P.gamma_type, bundle * P.cb + c) : 1.0f;
                 weighted[c] = make_float2(w * sum.x, w * sum.y);
-                acc[c] = make_float2(acc[c].x + sum.x, acc[c].y + sum.y);
+                acc[c] += sum.x;
+                acc[P.cb + c] += sum.y;
             });
         }
         __syncthreads();
@@ -1127,7 +1177,8 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
     }
     if (P.part != nullptr)
         for (int c = tid; c < P.cb; c += threads)
-            P.part[(static_cast<long long>(unit / P.bundles) * P.cluster + rank) * P.c + bundle * P.cb + c] = acc[c];
+            P.part[(static_cast<long long>(unit / P.bundles) * P.cluster + rank) * P.c + bundle * P.cb + c] =
+                make_float2(static_cast<float>(acc[c]), static_cast<float>(acc[P.cb + c]));
     if (P.cluster > 1) cg::this_cluster().sync();
 }
 
@@ -1244,17 +1295,31 @@ __global__ void __launch_bounds__(kNormThreads) norm_small_kernel(const __grid_c
         for (int k = 0; k < E; ++k)
             if (c[k] >= 0) sm[team * elements + t + k * P.team] = make_float2(sum_s[k], sum_t[k]);
         __syncthreads();
+        // images, then pixels, folded by halves
+        const int block = P.gb * elements;
+        for (int left = images; left > 1;) {
+            const int half = (left + 1) / 2;
+            for (int i = threadIdx.x; i < (left - half) * block; i += kNormThreads) {
+                sm[i].x += sm[i + half * block].x;
+                sm[i].y += sm[i + half * block].y;
+            }
+            left = half;
+            __syncthreads();
+        }
+        for (int left = static_cast<int>(P.px); left > 1;) {
+            const int half = (left + 1) / 2, each = (left - half) * P.cpg;
+            for (int i = threadIdx.x; i < P.gb * each; i += kNormThreads) {
+                const int at = i / each * elements + i % each;
+                sm[at].x += sm[at + half * P.cpg].x;
+                sm[at].y += sm[at + half * P.cpg].y;
+            }
+            left = half;
+            __syncthreads();
+        }
         for (int i = threadIdx.x; i < P.gb * P.cpg; i += kNormThreads) {
             const int gi = i / P.cpg, ci = i - gi * P.cpg, group = static_cast<int>(gblock) * P.gb + gi;
             if (group >= P.groups) break;
-            float2 sum = make_float2(0.0f, 0.0f);
-            for (int m = 0; m < images; ++m)
-                for (int q = 0; q < P.px; ++q) {
-                    const float2 o = sm[(m * P.gb + gi) * elements + q * P.cpg + ci];
-                    sum.x += o.x;
-                    sum.y += o.y;
-                }
-            P.part[static_cast<long long>(nblock) * P.c + group * P.cpg + ci] = sum;
+            P.part[static_cast<long long>(nblock) * P.c + group * P.cpg + ci] = sm[gi * elements + ci];
         }
     }
 }

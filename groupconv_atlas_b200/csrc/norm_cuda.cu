@@ -249,7 +249,8 @@ bool vector_access(std::initializer_list<const View *> views) {
 // in one wave, 200 in two; N8 C128 256x256 bf16: 71 and 77).  Launching sets of
 // images small enough for the second pass to find them in the L2 cache was
 // slower: a set's three launches cost about 10 us beside its data (the latter
-// shape: 78 us in one set, 108 in four).
+// shape: 78 us in one set, 108 in four).  In the gradient a thread takes at most
+// kNormRun runs of kNormRun vectors, for the sake of its sums.
 void plan_split(NormParams &P, int v, bool backward, int sms) {
     P.vcols = P.c / v;
     P.cblocks = static_cast<int>(ceil_div(P.vcols, gcb::kNormThreads));
@@ -260,6 +261,8 @@ void plan_split(NormParams &P, int v, bool backward, int sms) {
     const long long each = ceil_div(P.n * P.px, wave * P.lanes) * P.cblocks;
     const long long wanted = std::max<long long>(1, (each >= 128 ? 2 : 1) * wave / (P.n * P.cblocks));
     P.chunk_rows = std::min(P.px, std::max<long long>(ceil_div(P.px, wanted), 8LL * P.lanes));
+    const long long most = static_cast<long long>(gcb::kNormRun) * gcb::kNormRun * P.lanes;
+    if (backward && P.chunk_rows > most) P.chunk_rows = ceil_div(P.px, ceil_div(P.px, most));
     P.chunks = static_cast<int>(ceil_div(P.px, P.chunk_rows));
     P.items = P.n * P.chunks * P.cblocks;
 }
@@ -465,8 +468,8 @@ ResidentPlan choose_resident(const NormParams &base, int v, int slot, bool backw
     return best;
 }
 
-// The small path: threads per group so that each holds about four elements.
-// False where a group is too large for a warp.
+// The small path: threads per group so that each holds about four elements, and
+// at most kNormRun images in turn.  False where a group is too large for a warp.
 bool set_small(NormParams &P, int sms) {
     if (static_cast<wide>(P.px) * P.cpg > 32 * 16) return false;
     const int elements = static_cast<int>(P.px) * P.cpg;
@@ -476,6 +479,7 @@ bool set_small(NormParams &P, int sms) {
     P.gblocks = static_cast<int>(ceil_div(P.groups, P.gb));
     const long long images = gcb::kNormThreads / P.team / P.gb;
     P.nblocks = std::min(ceil_div(P.n, images), std::max<long long>(1, ceil_div(8LL * sms, P.gblocks)));
+    P.nblocks = std::max(P.nblocks, ceil_div(P.n, images * gcb::kNormRun));
     return P.nblocks * P.gblocks <= INT32_MAX;
 }
 // Its time in the same units: element accesses reach about 2 TB/s.

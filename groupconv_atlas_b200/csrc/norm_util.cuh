@@ -299,22 +299,32 @@ __device__ __forceinline__ void start_vector_pairs(uint4 *ring, const T *p, long
         }
     }
 }
-template <class T, int V, class F>
+// RUN > 0 (a multiple of kRing): end_run() after each RUN vectors and the last.
+struct Nothing {
+    __device__ __forceinline__ void operator()() const {}
+};
+template <class T, int V, int RUN = 0, class F, class E = Nothing>
 __device__ __forceinline__ void for_vector_pairs(uint4 *ring, const T *p, long long pstep, const T *q, long long qstep,
-                                                 int count, F f) {
+                                                 int count, F f, E end_run = {}) {
+    static_assert(RUN % kRing == 0 && RUN % kAhead == 0, "whole turns of the ring");
     if constexpr (V == 1) {
         constexpr int kPair = kAhead / 2;
-        for (int k = 0; k < count; k += kPair) {
-            Raw<T, V> a[kPair], b[kPair];
+        for (int start = 0; start < count;) {
+            const int stop = RUN > 0 ? min(count, start + RUN) : count;
+            for (int k = start; k < stop; k += kPair) {
+                Raw<T, V> a[kPair], b[kPair];
 #pragma unroll
-            for (int u = 0; u < kPair; ++u, p += pstep, q += qstep)
-                if (k + u < count) {
-                    a[u] = load_raw<T, V>(p);
-                    b[u] = load_raw<T, V>(q);
-                }
+                for (int u = 0; u < kPair; ++u, p += pstep, q += qstep)
+                    if (k + u < stop) {
+                        a[u] = load_raw<T, V>(p);
+                        b[u] = load_raw<T, V>(q);
+                    }
 #pragma unroll
-            for (int u = 0; u < kPair; ++u)
-                if (k + u < count) f(k + u, lanes_of_raw<T, V>(a[u]), lanes_of_raw<T, V>(b[u]));
+                for (int u = 0; u < kPair; ++u)
+                    if (k + u < stop) f(k + u, lanes_of_raw<T, V>(a[u]), lanes_of_raw<T, V>(b[u]));
+            }
+            start = stop;
+            end_run();
         }
     } else {
         constexpr int kHalf = kRing / 2;
@@ -323,18 +333,22 @@ __device__ __forceinline__ void for_vector_pairs(uint4 *ring, const T *p, long l
         constexpr uint32_t kPitch = kStreamThreads * sizeof(uint4);
         p += kHalf * pstep;
         q += kHalf * qstep;
+        for (int k = 0; k < count;) {
+            const int stop = RUN > 0 ? min(count, k + RUN) : count;
 #pragma unroll 2
-        for (int k = 0; k < count; ++k, p += pstep, q += qstep) {
-            const int slot = 2 * (k % kHalf);
-            cp_async_wait<kHalf - 1>();
-            const Lanes<V> v = unpack_lanes<T, V>(mine[slot * kStreamThreads], p);
-            const Lanes<V> g = unpack_lanes<T, V>(mine[(slot + 1) * kStreamThreads], p);
-            if (k + kHalf < count) {
-                copy_vector(addr + slot * kPitch, p);
-                copy_vector(addr + (slot + 1) * kPitch, q);
+            for (; k < stop; ++k, p += pstep, q += qstep) {
+                const int slot = 2 * (k % kHalf);
+                cp_async_wait<kHalf - 1>();
+                const Lanes<V> v = unpack_lanes<T, V>(mine[slot * kStreamThreads], p);
+                const Lanes<V> g = unpack_lanes<T, V>(mine[(slot + 1) * kStreamThreads], p);
+                if (k + kHalf < count) {
+                    copy_vector(addr + slot * kPitch, p);
+                    copy_vector(addr + (slot + 1) * kPitch, q);
+                }
+                cp_async_commit();
+                f(k, v, g);
             }
-            cp_async_commit();
-            f(k, v, g);
+            end_run();
         }
     }
 }

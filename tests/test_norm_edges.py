@@ -134,6 +134,57 @@ def test_clusters_that_take_several_images(native, torch_cuda, dims, groups, dty
         assert engine == 'resident_backward' and cluster == backward and rounds >= 2
 
 
+# ---- long sums of one sign ------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize('dims', [(593, 255, 45, 41), (297, 1024, 45, 40)], ids=['elements', 'vectors'])
+def test_gradient_sums_over_long_chunks(native, torch_cuda, dims):
+    """One chunk an image and one pixel lane a block: a thread adds 1800 products
+    for each of its channels.  Added one after the other, these (of the value
+    that a search found worst) are off by 450 half steps."""
+    n, c, h, w = dims
+    if torch.cuda.mem_get_info()[0] < 24 * n * c * h * w:
+        pytest.skip('needs 14 GB of device memory')
+    value = float.fromhex('0x1.171c02p0')
+    g = torch.Generator(device='cuda').manual_seed(35)
+    level = 2 * torch.randn(c, generator=g, device='cuda')
+    x = (torch.randn((n, h, w, c), generator=g, device='cuda') + level).permute(0, 3, 1, 2)
+    dy = torch.full((n, h, w, c), value, device='cuda').permute(0, 3, 1, 2)
+    gamma, beta = torch.ones(c, device='cuda'), torch.zeros(c, device='cuda')
+    _, stats = run_forward(native, x, 1, gamma, beta)
+    dx, dgamma, dbeta = run_backward(native, dy, x, stats, 1, gamma, beta)
+    assert 'engine=split_backward ' in native.last_plan()
+    total = n * h * w
+    assert_close(dbeta, torch.full((c,), total * value, dtype=torch.float64), torch.tensor((K + 1) * U * total * value))
+    want = torch.zeros(c, dtype=torch.float64, device='cuda')
+    tol = torch.zeros_like(want)
+    for i in range(0, n, 27):
+        part = x[i:i + 27].double()
+        sigma, mean = (part.var((1, 2, 3), correction=0, keepdim=True) + 1e-5).sqrt(), part.mean((1, 2, 3), keepdim=True)
+        xhat = (part - mean) / sigma
+        err = K * U * (1 + part.abs().amax((1, 2, 3), keepdim=True) / sigma)  # as in norm_helpers
+        want += value * xhat.sum((0, 2, 3))
+        tol += value * (err * (xhat.abs() + 1) + K * U * xhat.abs()).sum((0, 2, 3))
+    assert_close(dgamma, want.cpu(), (tol + U * want.abs()).cpu())
+
+
+@pytest.mark.gpu
+def test_gradient_sums_over_many_images(native, torch_cuda):
+    """Rows of one channel, 1200 in turn for each thread of a wave of blocks, 256
+    threads a block, 1184 blocks: sums that were added one after the other at
+    each of the three levels."""
+    n = 1200 * 256 * 1184
+    if torch.cuda.mem_get_info()[0] < 24 * n:
+        pytest.skip('needs 9 GB of device memory')
+    value = float.fromhex('0x1.d114p0')
+    x = torch.randn((n, 1), generator=torch.Generator(device='cuda').manual_seed(36), device='cuda')
+    dy = torch.full((n, 1), value, device='cuda')
+    gamma, beta = torch.ones(1, device='cuda'), torch.zeros(1, device='cuda')
+    _, stats = run_forward(native, x, 1, gamma, beta)
+    _, _, dbeta = run_backward(native, dy, x, stats, 1, gamma, beta)
+    assert 'engine=small_backward ' in native.last_plan()
+    assert_close(dbeta, torch.full((1,), n * value, dtype=torch.float64), torch.tensor(72 * U * n * value))
+
+
 # ---- saved tensors that come back with other strides ----------------------------------------------
 HOOKS = {'host': lambda: torch.autograd.graph.save_on_cpu(),
          'pinned': lambda: torch.autograd.graph.save_on_cpu(pin_memory=True),
