@@ -468,30 +468,38 @@ __global__ void __launch_bounds__(kNormThreads, split_blocks(V, false)) norm_app
 }
 
 // ---- split path, gradient ----------------------------------------------------------------
-template <int V, int ACT>
-__device__ __forceinline__ void grad_sums(int act, const Coefs<V> &k, const Lanes<V> &v, const Lanes<V> &g, Lanes<V> &s,
-                                          Lanes<V> &t) {
+// dz = drop(g act'(z)), and x - mean.  The slope comes before the mask, so that
+// a dropped place is 0 whatever it is (NaN where z is infinite).
+template <int V, int ACT, class F>
+__device__ __forceinline__ Lanes<V> grad_inner(int act, const Coefs<V> &k, const Lanes<V> &v, const Lanes<V> &g, Lanes<V> &d,
+                                               F drop) {
+    Lanes<V> dz;
 #pragma unroll
     for (int i = 0; i < Lanes<V>::kPairs; ++i) {
-        f2 d;
-        const f2 z = normalise<V>(k, i, v.p[i], d);
-        const f2 dz = activate_grad<ACT>(act, z, g.p[i]);
-        s.p[i] = s.p[i] + dz;
-        t.p[i] = fma2(dz, d, t.p[i]);
+        const f2 z = normalise<V>(k, i, v.p[i], d.p[i]);
+        dz.p[i] = activate_grad<ACT>(act, z, g.p[i]);
+    }
+    return drop(dz);
+}
+template <int V, int ACT, class F>
+__device__ __forceinline__ void grad_sums(int act, const Coefs<V> &k, const Lanes<V> &v, const Lanes<V> &g, Lanes<V> &s,
+                                          Lanes<V> &t, F drop) {
+    Lanes<V> d;
+    const Lanes<V> dz = grad_inner<V, ACT>(act, k, v, g, d, drop);
+#pragma unroll
+    for (int i = 0; i < Lanes<V>::kPairs; ++i) {
+        s.p[i] = s.p[i] + dz.p[i];
+        t.p[i] = fma2(dz.p[i], d.p[i], t.p[i]);
     }
 }
 // a dz - k1 - k2 (x - mean), with k1 and k2 given negated
-template <int V, int ACT>
+template <int V, int ACT, class F>
 __device__ __forceinline__ Lanes<V> grad_result(int act, const Coefs<V> &k, const Lanes<V> &minus_k1,
-                                                const Lanes<V> &minus_k2, const Lanes<V> &v, const Lanes<V> &g) {
-    Lanes<V> r;
+                                                const Lanes<V> &minus_k2, const Lanes<V> &v, const Lanes<V> &g, F drop) {
+    Lanes<V> d, r = grad_inner<V, ACT>(act, k, v, g, d, drop);
 #pragma unroll
-    for (int i = 0; i < Lanes<V>::kPairs; ++i) {
-        f2 d;
-        const f2 z = normalise<V>(k, i, v.p[i], d);
-        const f2 dz = activate_grad<ACT>(act, z, g.p[i]);
-        r.p[i] = fma2(k.a.p[i], dz, fma2(d, minus_k2.p[i], minus_k1.p[i]));
-    }
+    for (int i = 0; i < Lanes<V>::kPairs; ++i)
+        r.p[i] = fma2(k.a.p[i], r.p[i], fma2(d.p[i], minus_k2.p[i], minus_k1.p[i]));
     return r;
 }
 
@@ -524,7 +532,9 @@ __global__ void __launch_bounds__(kNormThreads, DROP ? 2 : split_blocks(V, true)
     };
     for_vector_pairs<T, V, kNormRun>(
         ring, x, xstep, dy, gstep, at.count,
-        [&](int, const Lanes<V> &v, const Lanes<V> &g) { grad_sums<V, ACT>(P.act, coefs, v, drop.apply(P, g), s2, t2); },
+        [&](int, const Lanes<V> &v, const Lanes<V> &g) {
+            grad_sums<V, ACT>(P.act, coefs, v, g, s2, t2, [&](const Lanes<V> &dz) { return drop.apply(P, dz); });
+        },
         join);
     float s[V], t[V];
     values_of<V>(all_s, s);
@@ -634,7 +644,8 @@ __global__ void __launch_bounds__(kNormThreads, DROP ? 2 : split_blocks(V, true)
     T *dx = static_cast<T *>(P.y) + at.n * P.y_ldn + last * P.y_ldp + at.c0;
     const long long ystep = down * P.y_ldp;
     for_vector_pairs<T, V>(ring, x, xstep, dy, gstep, at.count, [&](int, const Lanes<V> &v, const Lanes<V> &g) {
-        store_lanes<T, V>(dx, grad_result<V, ACT>(P.act, coefs, mk1, mk2, v, drop.apply(P, g)));
+        store_lanes<T, V>(dx, grad_result<V, ACT>(P.act, coefs, mk1, mk2, v, g,
+                                                  [&](const Lanes<V> &dz) { return drop.apply(P, dz); }));
         dx += ystep;
     });
 }
@@ -1066,6 +1077,7 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
 #pragma unroll
         for (int i = 0; i < Lanes<V>::kPairs; ++i) s2.p[i] = t2.p[i] = pair(0.0f);
         uint32_t keep = ~0u;
+        auto drop = [&](const Lanes<V> &dz) { return DROP ? drop_lanes<V>(dz, keep, P.drop) : dz; };
         if (DROP && P.drop.channel) keep = Draws<V>(gen, static_cast<uint64_t>(n) * P.c + r.c0).bits(P.drop.limit);
         uint64_t at = (static_cast<uint64_t>(n) * P.px + r.p0) * P.c + r.c0;
         int k = 0;
@@ -1075,17 +1087,15 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
             const int to = part_end(P.iters, r.count, part);
 #pragma unroll 2
             for (; k < to; ++k) {
-                const Lanes<V> v = read_slot<T, V>(x_at[k * threads]);
-                Lanes<V> g = read_slot<T, V>(g_at[k * threads]);
+                const Lanes<V> v = read_slot<T, V>(x_at[k * threads]), g = read_slot<T, V>(g_at[k * threads]);
                 if (DROP) {
                     if (!P.drop.channel) {
                         keep = Draws<V>(gen, at).bits(P.drop.limit);
                         bits[k * threads + tid] = static_cast<uint8_t>(keep);
                     }
                     at += static_cast<uint64_t>(P.lanes) * P.c;
-                    g = drop_lanes<V>(g, keep, P.drop);
                 }
-                grad_sums<V, ACT>(P.act, coefs, v, g, s2, t2);
+                grad_sums<V, ACT>(P.act, coefs, v, g, s2, t2, drop);
             }
         }
         // channel sums over the CTA's pixels
@@ -1158,19 +1168,15 @@ __global__ void __launch_bounds__(kResidentThreads, 1) norm_resident_grad_kernel
             const int to = part_end(P.iters, r.count, part);
 #pragma unroll 2
             for (; k < to; ++k, dx += ystep) {
-                const Lanes<V> v = read_slot<T, V>(x_at[k * threads]);
-                Lanes<V> g = read_slot<T, V>(g_at[k * threads]);
+                const Lanes<V> v = read_slot<T, V>(x_at[k * threads]), g = read_slot<T, V>(g_at[k * threads]);
                 if (more) {
                     copy_slot<T, V>(x_at + k * threads, x_addr + k * pitch, sx);
                     copy_slot<T, V>(g_at + k * threads, g_addr + k * pitch, sg);
                     sx += xstep;
                     sg += gstep;
                 }
-                if (DROP) {
-                    if (!P.drop.channel) keep = bits[k * threads + tid];
-                    g = drop_lanes<V>(g, keep, P.drop);
-                }
-                store_lanes<T, V>(dx, grad_result<V, ACT>(P.act, coefs, mk1, mk2, v, g));
+                if (DROP && !P.drop.channel) keep = bits[k * threads + tid];
+                store_lanes<T, V>(dx, grad_result<V, ACT>(P.act, coefs, mk1, mk2, v, g, drop));
             }
             cp_async_commit();
         }
@@ -1273,7 +1279,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_small_kernel(const __grid_c
                 if (here && c[k] >= 0) {
                     const float d = v[k] - st.x, up = to_float(dy[p[k] * P.dy_ldp + c[k]]);
                     const float z = fmaf(d, st.y * gm[k], bt[k]);
-                    dz[k] = one(activate_grad<-1>(P.act, pair(z, 0.0f), pair(keep[k] ? up * f[k] : 0.0f, 0.0f)));
+                    dz[k] = keep[k] ? one(activate_grad<-1>(P.act, pair(z, 0.0f), pair(up, 0.0f))) * f[k] : 0.0f;
                     s1 = fmaf(gm[k], dz[k], s1);
                     s2 = fmaf(gm[k] * dz[k], d, s2);
                     sum_s[k] += dz[k];

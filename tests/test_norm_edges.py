@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from groupconv_atlas_b200 import api, torch_module
-from tests.norm_helpers import HALF, K, TINY, U, NormReference, assert_close
+from tests.norm_helpers import HALF, K, TINY, U, NormReference, assert_close, keep_mask
 from tests.test_group_norm import TYPES, check_step, make, run_backward, run_forward
 
 # ---- arguments of SiLU far from zero --------------------------------------------------------------
@@ -96,6 +96,39 @@ def test_silu_of_infinities(native, torch_cuda, dims, groups):
     assert torch.isnan(y[:, 1]).all() and (y[:, 4] == float('inf')).all()
     rest = [c for c in range(dims[1]) if c not in (1, 4)]
     assert_close(y[:, rest], ref.y[:, rest], ref.tol_y[:, rest], 'y')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dims,groups,path', [((4, 32, 6, 7), 4, 'resident'), ((4, 45, 5, 9), 9, 'resident'),
+                                              ((5000, 24, 2, 2), 3, 'small'), ((2, 64, 300, 260), 1, 'split')])
+@pytest.mark.parametrize('act', ['silu', 'none', 'relu'])
+def test_dropped_channels_hide_infinite_arguments(native, torch_cuda, dims, groups, path, act):
+    """dz is 0 where a place is dropped, whatever the slope there is (NaN for SiLU
+    at an infinity): an image whose infinite channels are all dropped has the
+    gradient that it has without them."""
+    x, gamma, beta, dy = make(dims, torch.float32, 37)
+    seed = 0
+    while True:  # an image with both channels dropped
+        keep, scale = keep_mask(x.shape, 0.5, seed, 3, 'channel')
+        kept = keep[:, :, 0, 0]
+        clean = ~kept[:, 2] & ~kept[:, 7]
+        if clean.any():
+            break
+        seed += 1
+    ref = NormReference(x, groups, gamma, beta, act=act, keep=keep, scale=scale)
+    dy = ref.away_from_kinks(dy)
+    ref.backward(dy)
+    beta[2], beta[7] = float('-inf'), float('inf')
+    drop = api.dropout_args(0.5, seed, 3, 'channel')
+    y, stats = run_forward(native, x.cuda(), groups, gamma.cuda(), beta.cuda(), act=act, drop=drop)
+    dx, _, _ = run_backward(native, dy.cuda(), x.cuda(), stats, groups, gamma.cuda(), beta.cuda(), act, drop)
+    assert f'engine={path}_backward ' in native.last_plan()
+    assert_close(y.cpu()[clean], ref.y[clean], ref.tol_y[clean], 'y')
+    assert_close(dx.cpu()[clean], ref.dx[clean], ref.tol_dx[clean], 'dx')
+    drop = api.dropout_args(1.0, seed, 3)
+    y, stats = run_forward(native, x.cuda(), groups, gamma.cuda(), beta.cuda(), act=act, drop=drop)
+    for t in (y, *run_backward(native, dy.cuda(), x.cuda(), stats, groups, gamma.cuda(), beta.cuda(), act, drop)):
+        assert (t == 0).all()
 
 
 # ---- clusters that take several images in turn ----------------------------------------------------
