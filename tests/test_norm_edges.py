@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from groupconv_atlas_b200 import api, torch_module
-from tests.norm_helpers import HALF, K, TINY, U, NormReference, assert_close, keep_mask
+from tests.norm_helpers import HALF, K, TINY, U, NormReference, assert_close, keep_mask, philox
 from tests.test_group_norm import TYPES, check_step, make, run_backward, run_forward
 
 # ---- arguments of SiLU far from zero --------------------------------------------------------------
@@ -352,3 +352,35 @@ def test_a_norm_without_dropout_can_be_given_one():
     assert norm.p == 0.0
     norm.p = 0.1
     assert norm.p == 0.1 and not norm.drop.training and norm.scope == 'element'
+
+
+# ---- the generator --------------------------------------------------------------------------------
+def philox_block(counter, key):
+    """Philox4x32-10 of four counter words and two key words, with Python's integers."""
+    (a, b, c, d), (k, m) = counter, key
+    for _ in range(10):
+        u, v = a * 0xD2511F53, c * 0xCD9E8D57
+        a, b, c, d = (v >> 32) ^ b ^ k, v & 0xFFFFFFFF, (u >> 32) ^ d ^ m, u & 0xFFFFFFFF
+        k, m = (k + 0x9E3779B9) & 0xFFFFFFFF, (m + 0xBB67AE85) & 0xFFFFFFFF
+    return [a, b, c, d]
+
+
+def test_known_answers_of_the_generator():
+    """The vectors published with Random123: zeros, ones, digits of pi."""
+    ones = 0xFFFFFFFF
+    assert philox_block([0] * 4, [0] * 2) == [0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8]
+    assert philox_block([ones] * 4, [ones] * 2) == [0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd]
+    assert philox_block([0x243f6a88, 0x85a308d3, 0x13198a2e, 0x03707344], [0xa4093822, 0x299f31d0]) == [
+        0xd16cfe09, 0x94fdcceb, 0x5001e420, 0x24126ea1]
+
+
+@pytest.mark.parametrize('seed,offset', [(0, 0), (0x299f31d0a4093822, 0x0370734413198a2e), (1 << 32, 0), (1, 0),
+                                         (0, 1 << 32), (0, 1), (2 ** 64 - 1, 2 ** 64 - 1)])
+def test_draws_against_the_generator_s_blocks(seed, offset):
+    """The oracle of the mask tests: key = seed, counter = (block, offset), each
+    the low word first; half j % 2 of word j / 2 of a block is its draw j."""
+    got = philox(8 * 3 + 5, seed, offset)
+    low = 0xFFFFFFFF
+    for j, draw in enumerate(got):
+        words = philox_block([j // 8, 0, offset & low, offset >> 32], [seed & low, seed >> 32])
+        assert draw == words[j % 8 // 2] >> 16 * (j % 2) & 0xFFFF
