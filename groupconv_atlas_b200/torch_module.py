@@ -363,8 +363,9 @@ def fuse_norm_act(module: torch.nn.Module) -> list[str]:
     """In every Sequential, replace each GroupNorm with the activation (none,
     ReLU, ReLU6, SiLU) and the dropout (Dropout, Dropout2d) that follow it by
     one B200GroupNormAct; the members it takes over become Identity, so every
-    other member keeps its name.  Subclasses of these and modules with hooks
-    stay as they are.  Returns the dotted names replaced.
+    other member keeps its name.  Subclasses of these, modules with hooks and
+    Sequentials with a forward of their own, which may call their members in
+    another order, stay as they are.  Returns the dotted names replaced.
 
     The replacement differs from torch's modules in three ways: it takes 2 to 4
     axes (a GroupNorm that sees (N, C, D, H, W) has to stay out of the fused
@@ -373,7 +374,7 @@ def fuse_norm_act(module: torch.nn.Module) -> list[str]:
     nn = torch.nn
     replaced = []
     for name, child in list(module.named_modules()):
-        if not isinstance(child, nn.Sequential):
+        if not isinstance(child, nn.Sequential) or type(child).forward is not nn.Sequential.forward:
             continue
         members = list(child._modules.items())
         for at, (attr, norm) in enumerate(members):

@@ -318,6 +318,23 @@ def test_fuse_norm_act_leaves_what_may_do_something_else():
     assert isinstance(model[5], nn.Identity)
 
 
+class ActivationLast(torch.nn.Sequential):
+    def forward(self, x):
+        return self[1](self[2](self[0](x)))
+
+
+class Named(torch.nn.Sequential):
+    """A subclass that runs as Sequential does."""
+
+
+def test_fuse_norm_act_leaves_sequentials_with_a_forward_of_their_own():
+    nn = torch.nn
+    members = lambda: (nn.GroupNorm(2, 8), nn.ReLU(), nn.Conv2d(8, 8, 1))
+    model = nn.Sequential(ActivationLast(*members()), Named(*members()))
+    assert torch_module.fuse_norm_act(model) == ['1.0']
+    assert isinstance(model[0][1], nn.ReLU) and isinstance(model[1][1], nn.Identity)
+
+
 @pytest.mark.parametrize('norm_mode', [True, False])
 @pytest.mark.parametrize('drop_mode', [True, False])
 def test_a_dropout_keeps_its_own_mode(monkeypatch, norm_mode, drop_mode):
