@@ -8,6 +8,7 @@ import torch
 
 from groupconv_atlas_b200 import api, torch_module
 from tests.norm_helpers import HALF, K, TINY, U, NormReference, assert_close, keep_mask, philox
+from tests.test_dropout import blocks_of_draws
 from tests.test_group_norm import TYPES, check_step, make, run_backward, run_forward
 
 # ---- arguments of SiLU far from zero --------------------------------------------------------------
@@ -216,6 +217,83 @@ def test_gradient_sums_over_many_images(native, torch_cuda):
     _, _, dbeta = run_backward(native, dy, x, stats, 1, gamma, beta)
     assert 'engine=small_backward ' in native.last_plan()
     assert_close(dbeta, torch.full((1,), n * value, dtype=torch.float64), torch.tensor(72 * U * n * value))
+
+
+# ---- more than 2^32 elements ----------------------------------------------------------------------
+def large(dims):
+    """Random bf16 tensors of more than 2^32 elements, channels last: x, dy = 1."""
+    count = int(np.prod(dims))
+    if torch.cuda.mem_get_info()[0] < 12 * count:
+        pytest.skip('needs 52 GB of device memory')
+    shape = (dims[0], *dims[2:], dims[1])
+    x = torch.randn(shape, generator=torch.Generator(device='cuda').manual_seed(38), dtype=torch.bfloat16, device='cuda')
+    return x.movedim(-1, 1), torch.ones(shape, dtype=torch.bfloat16, device='cuda').movedim(-1, 1)
+
+
+def tail_of_the_mask(dims, images, seed, offset):
+    """keep of the last images, shaped like them: draws from their first place on."""
+    place = int(np.prod(dims)) // dims[0]
+    first = (dims[0] - images) * place
+    draws = blocks_of_draws(first // 8, (images * place + 15) // 8, seed, offset)[first % 8:][:images * place]
+    return (draws >= 32768).reshape(images, *dims[2:], dims[1]).movedim(-1, 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dims,groups,path', [((65537, 64, 32, 32), 4, 'resident'), ((268435461, 16), 2, 'small')])
+def test_more_than_2_32_elements(native, torch_cuda, dims, groups, path):
+    """The last images, their mask included; dbeta counts the kept places."""
+    x, dy = large(dims)
+    c = dims[1]
+    gamma, beta = torch.ones(c, device='cuda'), torch.zeros(c, device='cuda')
+    drop = api.dropout_args(0.5, 8, 9)
+    y, stats = run_forward(native, x, groups, gamma, beta, act='silu', drop=drop)
+    assert f'engine={path} ' in native.last_plan()
+    dx, _, dbeta = run_backward(native, dy, x, stats, groups, gamma, beta, 'none', drop)
+    assert f'engine={path}_backward ' in native.last_plan()
+    keep = tail_of_the_mask(dims, 3, 8, 9)
+    last = x[-3:].cpu()
+    for act, got, want in (('silu', y, 'y'), ('none', dx, 'dx')):
+        ref = NormReference(last, groups, act=act, keep=keep, scale=2.0).backward(torch.ones_like(last))
+        assert_close(got[-3:], getattr(ref, want), getattr(ref, 'tol_' + want), want)
+    kept = sum((part != 0).sum([d for d in range(part.dim()) if d != 1]) for part in y.split(1 << 22 if path == 'small' else 1 << 10))
+    # a kept place whose activation is 0 or rounds to it: fewer than one in 2^10
+    assert ((2 * kept <= dbeta * (1 + K * U)) & (dbeta <= 2 * kept * (1 + 2.0 ** -10))).all()
+
+
+@pytest.mark.gpu
+def test_an_image_of_more_than_2_32_elements(native, torch_cuda):
+    """The split path: the last pixels, and both passes' sums over all of them."""
+    dims, groups = (1, 8, 32769, 16384), 2
+    x, dy = large(dims)
+    gamma, beta = torch.ones(8, device='cuda'), torch.zeros(8, device='cuda')
+    drop = api.dropout_args(0.5, 8, 9)
+    y, stats = run_forward(native, x, groups, gamma, beta, drop=drop)
+    assert 'engine=split ' in native.last_plan()
+    dx, _, dbeta = run_backward(native, dy, x, stats, groups, gamma, beta, drop=drop)
+    assert 'engine=split_backward ' in native.last_plan()
+    rows = x[0].movedim(0, -1).reshape(-1, groups, 4)
+    outs = y[0].movedim(0, -1).reshape(-1, groups, 4)
+    parts = range(0, len(rows), 1 << 25)
+    total = 4.0 * len(rows)
+    mean = sum(rows[i:i + (1 << 25)].double().sum((0, 2)) for i in parts) / total
+    var = sum((rows[i:i + (1 << 25)].double() - mean[:, None]).square().sum((0, 2)) for i in parts) / total
+    rstd = (var + 1e-5).rsqrt()
+    err = K * U * (1 + rows[:1 << 25].abs().max() * rstd)  # as in norm_helpers, for |x| up to the sample's largest
+    assert ((stats[0, :, 0] - mean).abs() * rstd <= 2 * err).all() and ((stats[0, :, 1] / rstd - 1).abs() <= 2 * err).all()
+    # s1 and s2 of dz = 2 keep, from the forward pass's own results: y = dz xhat
+    # with a random rounding each
+    s1 = sum(2.0 * (outs[i:i + (1 << 25)] != 0).sum((0, 2)) for i in parts) / total
+    s2 = sum(outs[i:i + (1 << 25)].double().sum((0, 2)) for i in parts) / total
+    count = 1 << 10
+    first = len(rows) - count
+    keep = (blocks_of_draws(first, count, 8, 9) >= 32768).view(count, groups, 4)
+    mean, rstd, s1, s2 = (v.cpu()[:, None] for v in (mean, rstd, s1.double(), s2))
+    xhat = (rows[-count:].cpu().double() - mean) * rstd
+    dz = 2.0 * keep
+    assert_close(outs[-count:], dz * xhat, HALF[x.dtype] * (dz * xhat).abs() + 2e-4)
+    want = rstd * (dz - s1 - xhat * s2)
+    assert_close(dx[0].movedim(0, -1).reshape(-1, groups, 4)[-count:], want, HALF[x.dtype] * want.abs() + 2e-4)
+    assert ((dbeta.view(groups, 4).sum(1).double() / total).cpu() - s1[:, 0]).abs().max() <= 2.0 ** -10
 
 
 # ---- saved tensors that come back with other strides ----------------------------------------------
