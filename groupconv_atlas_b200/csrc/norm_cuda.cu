@@ -400,9 +400,10 @@ long long resident_stride(const NormParams &P, int threads, size_t smem, const g
 
 // Estimated cost of a resident choice that is set in P: its phases (load; for
 // each image of a cluster the first pass, the sums, the second pass).  The
-// constants are fitted, to 6300 choices of 112 shapes timed on a B200, so that
+// constants are fitted, to 5765 choices of 112 shapes timed on a B200, so that
 // the cheapest choice is the fastest one; they follow the times in
-// microseconds only roughly.  On those shapes the choice is 5 % slower than the
+// microseconds only roughly.  Clusters are counted as if any SMs could make one
+// up, though one is placed within a GPC.  On those shapes the choice is 5 % slower than the
 // best on average, and at most 1.25 times where a call takes more than 6 us
 // (once 1.39, with 255 channels of FP32).
 double resident_cost(const NormParams &P, int v, int slot, int threads, size_t smem, bool backward,
@@ -543,8 +544,10 @@ void set_param(const gc_tensor *t, const void *&p, int &type) {
 
 // ---- kernel tables --------------------------------------------------------------------------
 // The vector kernels without dropout are compiled for each activation, those
-// with dropout for SiLU (the gradient of N8 C128 256x256 bf16 takes 150 us
-// instead of 166); the others choose it at run time.
+// with dropout for SiLU: N8 C128 256x256 bf16 92 us and gradient 150 instead of
+// 96 and 167 with the activation chosen at run time, N32 C256 28x28 12.7 and 25
+// instead of 13.4 and 29 (FP32 19 and 30 instead of 21 and 35).  The others
+// choose it at run time (ReLU, gradient of the first: 154 us).
 enum NormKernel { kMoments, kApply, kGradSums, kGradApply };
 
 template <class T, int V, int ACT, bool DROP>
