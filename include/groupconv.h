@@ -168,7 +168,8 @@ int gc_b200_conv_ex(const gc_shape *p, const gc_tensor *x, const gc_tensor *w,
  *
  * Element types.  These entry points take F32 tensors like the convolutions
  * and two 16-bit types as well; every sum, statistic and intermediate is held
- * in 32 bits, and only the stored result is rounded to the tensor's type. */
+ * in 32 bits or more, and only the stored result is rounded to the tensor's
+ * type. */
 #define GC_B200_F16 16
 #define GC_B200_BF16 17
 
@@ -218,7 +219,8 @@ typedef struct {
  *   gamma, beta NULL, or rank-1 dense tensors of C elements, F32 or x's type.
  *   stats       NULL, or a dense F32 tensor of dims (N, groups, 2) that
  *               receives mean and 1 / sqrt(var + eps) for the gradient.
- *   activation  GC_B200_ACT_NONE, _RELU, _RELU6 or _SILU (a NaN stays NaN).
+ *   activation  GC_B200_ACT_NONE, _RELU, _RELU6 or _SILU (a NaN stays NaN; the
+ *               SiLU of -inf is NaN, that of any finite v below -88 is 0).
  *   dropout     NULL for none.
  *   workspace   16-byte aligned device memory of at least the bytes that
  *               gc_b200_group_norm_workspace gives for these tensors (NULL
