@@ -195,8 +195,9 @@ int gc_b200_conv_ex(const gc_shape *p, const gc_tensor *x, const gc_tensor *w,
  *                          anew at each replay).  Inputs of the call: no output
  *                          and no workspace overlaps them;
  *   used                   nullable device pair that receives the seed and
- *                          offset in effect, for a later gradient (unless t is
- *                          0: nothing is drawn then).  An output of the call. */
+ *                          offset in effect, for a later gradient (where t is 0
+ *                          nothing is drawn, and it may stay as it was).  An
+ *                          output of the call. */
 typedef struct {
     double p; /* 0 <= p <= 1 */
     uint64_t seed, offset;
