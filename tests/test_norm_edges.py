@@ -296,6 +296,35 @@ def test_an_image_of_more_than_2_32_elements(native, torch_cuda):
     assert ((dbeta.view(groups, 4).sum(1).double() / total).cpu() - s1[:, 0]).abs().max() <= 2.0 ** -10
 
 
+# ---- repetition -----------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize('dims,groups,path', [((32, 256, 28, 28), 32, 'resident'), ((200, 64, 28, 28), 1, 'resident'),
+                                              ((5000, 24, 2, 2), 3, 'small'), ((2, 64, 300, 260), 1, 'split')])
+@pytest.mark.parametrize('p', [0.0, 0.2])
+def test_steps_repeat_bitwise(native, torch_cuda, dims, groups, path, p):
+    """Whatever else the GPU does and whatever its caches hold: dgamma and dbeta
+    too, in the parameters' 16-bit type."""
+    x, gamma, beta, dy = (t.cuda() for t in make(dims, torch.bfloat16, 39))
+    leaves = [t.requires_grad_() for t in (x, gamma.bfloat16(), beta.bfloat16())]
+    busy, other = torch.empty(1 << 28, dtype=torch.uint8, device='cuda'), torch.cuda.Stream()
+    want = None
+    for i in range(24):
+        if i % 3 == 1:
+            busy.fill_(i)  # larger than the L2 cache
+        if i % 3 == 2:
+            other.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(other):
+                busy.fill_(i)
+        y = torch_module.group_norm_act(leaves[0], groups, *leaves[1:], activation='silu', dropout=p, seed=4, offset=5)
+        if i == 0:
+            assert f'engine={path} ' in native.last_plan()
+        got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+        torch.cuda.synchronize()
+        want = want or got
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 # ---- saved tensors that come back with other strides ----------------------------------------------
 HOOKS = {'host': lambda: torch.autograd.graph.save_on_cpu(),
          'pinned': lambda: torch.autograd.graph.save_on_cpu(pin_memory=True),
