@@ -18,6 +18,7 @@
 #include "host_util.h"
 #include "kernel_dropout.cuh"
 #include "kernel_norm.cuh"
+#include "tensor_checks.cuh"
 
 namespace {
 
@@ -26,47 +27,22 @@ using gcb::DropParams;
 using gcb::DropoutParams;
 using gcb::NormParams;
 using gcb::PlanRecord;
-
-typedef __int128 wide;  // products of descriptor fields, before they are known to fit
+using gcb::Range;
+using gcb::wide;
+using gcb::check_call;
+using gcb::check_fields;
+using gcb::check_workspace;
+using gcb::elem_size;
+using gcb::elem_type;
+using gcb::internal_error;
+using gcb::launched;
+using gcb::outputs_meet;
+using gcb::range_of;
+using gcb::ranges_meet;
+using gcb::same_dims;
+using gcb::up16;
 
 // ---- descriptors ------------------------------------------------------------------------
-int elem_type(int dtype) {
-    return dtype == GC_F32 ? gcb::kElemF32 : dtype == GC_B200_F16 ? gcb::kElemF16
-         : dtype == GC_B200_BF16 ? gcb::kElemBF16 : -1;
-}
-int elem_size(int type) { return type == gcb::kElemF32 ? 4 : 2; }
-
-// What every descriptor of these entry points has to satisfy (GC_INVALID
-// conditions, then FP64 as a valid type outside this set).
-int check_fields(const gc_tensor *t, int rank_low, int rank_high, int64_t &count) {
-    if (t == nullptr) return gc_error(GC_INVALID, "null tensor descriptor");
-    if (t->rank < rank_low || t->rank > rank_high) return gc_error(GC_INVALID, "tensor rank out of range");
-    if (t->device != GC_CUDA || t->device_index < 0) return gc_error(GC_INVALID, "tensor must be CUDA memory");
-    if (t->dtype != GC_F64 && elem_type(t->dtype) < 0) return gc_error(GC_INVALID, "unknown tensor dtype");
-    wide n = 1;
-    for (int i = 0; i < t->rank; ++i) {
-        if (t->dims[i] < 0) return gc_error(GC_INVALID, "tensor dimensions must not be negative");
-        n *= t->dims[i];
-        if (n > PTRDIFF_MAX / 8) return gc_error(GC_INVALID, "tensor element count overflow");
-    }
-    count = static_cast<int64_t>(n);
-    if (count == 0) return GC_OK;
-    if (t->data == nullptr) return gc_error(GC_INVALID, "null tensor buffer");
-    const uintptr_t base = reinterpret_cast<uintptr_t>(t->data);
-    const unsigned item = t->dtype == GC_F64 ? 8 : elem_size(elem_type(t->dtype));
-    if (base % item != 0) return gc_error(GC_INVALID, "tensor data is not element aligned");
-    if (t->bytes > UINTPTR_MAX - base) return gc_error(GC_INVALID, "tensor pointer range overflow");
-    if (t->bytes / item < static_cast<uint64_t>(count)) return gc_error(GC_INVALID, "tensor buffer is too small");
-    return GC_OK;
-}
-
-bool same_dims(const gc_tensor *a, const gc_tensor *b) {
-    if (a->rank != b->rank) return false;
-    for (int i = 0; i < a->rank; ++i)
-        if (a->dims[i] != b->dims[i]) return false;
-    return true;
-}
-
 // A channels-last tensor as images of evenly spaced pixels.
 struct View {
     char *data = nullptr;
@@ -110,25 +86,6 @@ int view_of(const gc_tensor *t, View &v) {
     return GC_OK;
 }
 
-bool ranges_meet(const void *a, uint64_t an, const void *b, uint64_t bn) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return an != 0 && bn != 0 && x < y + bn && y < x + an;
-}
-struct Range {
-    const void *p;
-    uint64_t bytes;
-};
-// Outputs against inputs and against one another.
-bool outputs_meet(std::initializer_list<Range> outs, std::initializer_list<Range> ins) {
-    for (const Range *o = outs.begin(); o != outs.end(); ++o) {
-        for (const Range &i : ins)
-            if (ranges_meet(o->p, o->bytes, i.p, i.bytes)) return true;
-        for (const Range *q = outs.begin(); q != o; ++q)
-            if (ranges_meet(o->p, o->bytes, q->p, q->bytes)) return true;
-    }
-    return false;
-}
-
 // A nullable vector of one parameter per channel.
 int check_channel_vector(const gc_tensor *t, const gc_tensor *x) {
     if (t == nullptr) return GC_OK;
@@ -146,13 +103,6 @@ int check_channel_layout(const gc_tensor *t) {
         return gc_error(GC_UNSUPPORTED, "channel parameters must be dense");
     return GC_OK;
 }
-Range range_of(const gc_tensor *t) {
-    if (t == nullptr) return {nullptr, 0};
-    uint64_t n = t->dtype == GC_F64 ? 8 : elem_size(elem_type(t->dtype));
-    for (int i = 0; i < t->rank; ++i) n *= static_cast<uint64_t>(t->dims[i]);
-    return {t->data, n};
-}
-
 int check_stats(const gc_tensor *t, const gc_tensor *x, int64_t groups) {
     int64_t count = 0;
     int st = check_fields(t, 3, 3, count);
@@ -195,40 +145,6 @@ int check_dropout(const gc_b200_dropout_args *d, DropParams &out) {
 
 Range used_words(const DropParams &d) { return {d.used, d.used != nullptr ? 16u : 0u}; }
 Range given_word(const uint64_t *p) { return {p, p != nullptr ? 8u : 0u}; }
-
-// The current device, the pointers' device and the stream (reference
-// groupconv.cu:130-139, :185-191).
-int check_call(std::initializer_list<const gc_tensor *> tensors, std::initializer_list<const void *> words,
-               int device_index, void *stream, int &dev) {
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
-    for (const gc_tensor *t : tensors)
-        if (t != nullptr && range_of(t).bytes != 0) {
-            const int st = gcb::check_pointer(t, dev);
-            if (st != GC_OK) return st;
-        }
-    for (const void *p : words)
-        if (p != nullptr) {
-            const int st = gcb::check_device_memory(p, device_index, dev);
-            if (st != GC_OK) return st;
-        }
-    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-    e = cudaStreamIsCapturing(reinterpret_cast<cudaStream_t>(stream), &cs);
-    return e == cudaSuccess ? GC_OK : gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
-}
-
-int launched(cudaError_t e) {
-    if (e == cudaSuccess) e = cudaGetLastError();
-    else cudaGetLastError();
-    return e == cudaSuccess ? gc_error(GC_OK, "") : gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
-}
-// The same, with the plan of a call that succeeded.
-template <class... T>
-int launched(cudaError_t e, PlanRecord::Kind kind, const char *name, T... values) {
-    const int st = launched(e);
-    if (st == GC_OK) gcb::record_plan(kind, name, false, values...);
-    return st;
-}
 
 // ---- group norm: plan ---------------------------------------------------------------------
 int vector_of(const View &v) { return v.type == gcb::kElemF32 ? 4 : 8; }
@@ -275,8 +191,6 @@ size_t split_smem(const NormParams &P, int v, bool sums, bool backward) {
     if (sums && !backward) after += ceil_div(P.vb * v, 2) * 2 * sizeof(float);
     return std::max(gcb::ring_space(v), after);
 }
-
-uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
 
 struct NormPlan {
     bool vec = false;
@@ -678,13 +592,6 @@ cudaError_t launch_finalize(bool backward, NormParams &P, cudaStream_t s) {
     return launch(fn, block ? P.n * P.groups : ceil_div(P.n * P.groups, gcb::kNormThreads / 32), P, s);
 }
 
-int check_workspace(const void *p, uint64_t bytes, uint64_t need) {
-    if (need == 0) return GC_OK;
-    if (p == nullptr || bytes < need) return gc_error(GC_INVALID, "workspace is missing or too small");
-    if (!gcb::aligned16(p)) return gc_error(GC_INVALID, "workspace must be 16-byte aligned");
-    return GC_OK;
-}
-
 bool known_activation(int a) {
     return a == GC_B200_ACT_NONE || a == GC_B200_ACT_RELU || a == GC_B200_ACT_RELU6 || a == GC_B200_ACT_SILU;
 }
@@ -736,10 +643,6 @@ template <class T>
 const void *dropout_typed(DropoutKernel k, bool vec) {
     return vec ? dropout_instance<T, gcb::kVec<T>>(k) : dropout_instance<T, 1>(k);
 }
-
-// No exception leaves a C entry point; those that can arise here come from host
-// memory that ran out.
-int internal_error() { return gc_error(GC_DEVICE_ERROR, "host resources exhausted"); }
 
 }  // namespace
 
