@@ -180,6 +180,33 @@ def dropout_args(p, seed=0, offset=0, scope='element', seed_ptr=None, offset_ptr
     return DropoutArgs(p, seed, offset, seed_ptr, offset_ptr, used, native_int(scope))
 
 
+class ScanArgs(ct.Structure):
+    """gc_b200_scan_args."""
+    _fields_ = [(k, ct.POINTER(Tensor)) for k in ('x', 'dt', 'a', 'b', 'c', 'd', 'z', 'dt_bias', 'state')] + [
+        ('lengths', ct.c_void_p), ('softplus', ct.c_int32)]
+
+
+class ScanGrads(ct.Structure):
+    """gc_b200_scan_grads."""
+    _fields_ = [(k, ct.POINTER(Tensor)) for k in ('x', 'dt', 'a', 'b', 'c', 'd', 'z', 'dt_bias', 'state')]
+
+
+def _pointers(struct, arrays):
+    """A structure of descriptor pointers; the descriptors live as long as it does."""
+    struct.descs = {k: view(a) for k, a in arrays.items() if a is not None}
+    for k, d in struct.descs.items():
+        setattr(struct, k, ct.pointer(d))
+    return struct
+
+
+def scan_args(x, dt, a, b, c, d=None, z=None, dt_bias=None, state=None, lengths=None, softplus=True):
+    """Arguments of the selective scan's calls, from borrowed device tensors."""
+    args = _pointers(ScanArgs(), dict(x=x, dt=dt, a=a, b=b, c=c, d=d, z=z, dt_bias=dt_bias, state=state))
+    args.lengths = lengths.data_ptr() if lengths is not None else None
+    args.softplus = 1 if softplus else 0
+    return args
+
+
 class NativeError(RuntimeError):
     def __init__(self, status, message):
         self.status = status
@@ -234,6 +261,20 @@ class Native:
         lib.gc_b200_group_norm_backward.argtypes = ([ptr] * 8 + [ct.c_int64, ct.c_int, ct.POINTER(DropoutArgs),
                                                                  ct.c_void_p, ct.c_uint64, ct.c_void_p])
         lib.gc_b200_dropout.argtypes = [ptr] * 3 + [ct.POINTER(DropoutArgs), ct.c_void_p]
+        lib.gc_b200_layer_norm.argtypes = [ptr] * 5 + [ct.c_double, ct.c_void_p]
+        lib.gc_b200_layer_norm_backward_workspace.argtypes = [ptr] * 3 + [ct.POINTER(ct.c_uint64)]
+        lib.gc_b200_layer_norm_backward.argtypes = [ptr] * 7 + [ct.c_void_p, ct.c_uint64, ct.c_void_p]
+        lib.gc_b200_causal_conv.argtypes = [ptr] * 4 + [ct.c_void_p] + [ptr] * 2 + [ct.c_int, ct.c_void_p]
+        lib.gc_b200_causal_conv_backward_workspace.argtypes = [ptr] * 4 + [ct.POINTER(ct.c_uint64)]
+        lib.gc_b200_causal_conv_backward.argtypes = ([ptr] * 6 + [ct.c_void_p] + [ptr] * 4 + [ct.c_int, ct.c_void_p,
+                                                                                             ct.c_uint64, ct.c_void_p])
+        lib.gc_b200_causal_conv_step.argtypes = [ptr] * 6 + [ct.c_int, ct.c_void_p]
+        scan = ct.POINTER(ScanArgs)
+        lib.gc_b200_selective_scan_sizes.argtypes = [scan] + [ct.POINTER(ct.c_uint64)] * 3
+        lib.gc_b200_selective_scan.argtypes = [scan] + [ptr] * 2 + [ct.c_void_p, ct.c_uint64] * 2 + [ct.c_void_p]
+        lib.gc_b200_selective_scan_backward.argtypes = ([scan] + [ptr] * 2 + [ct.c_void_p, ct.c_uint64, ct.POINTER(ScanGrads),
+                                                                             ct.c_void_p, ct.c_uint64, ct.c_void_p])
+        lib.gc_b200_selective_scan_step.argtypes = [scan] + [ptr] * 2 + [ct.c_void_p]
         lib.gc_b200_autotune.argtypes = [ct.POINTER(CShape)] + [ct.POINTER(Tensor)] * 3 + [ct.c_int, ct.c_void_p]
         lib.gc_b200_probe_ffma.argtypes = [ct.c_void_p, ct.c_int, ct.c_int, ct.c_void_p]
         lib.gc_b200_probe_ffma_flops.argtypes = [ct.c_int, ct.c_int]
@@ -351,6 +392,93 @@ class Native:
         _, (xp, rp, yp) = self._views(x, residual, y)
         self.check(self.lib.gc_b200_dropout(xp, rp, yp, ct.byref(dropout) if dropout is not None else None,
                                             self._stream(stream)))
+        return y
+
+    def layer_norm(self, x, y, gamma=None, beta=None, eps=1e-5, stats=None, stream=0):
+        """gc_b200_layer_norm of the last axis of borrowed device tensors; stats
+        an FP32 (rows, 2) tensor for the gradient."""
+        _, (xp, gp, bp, yp, sp) = self._views(x, gamma, beta, y, stats)
+        self.check(self.lib.gc_b200_layer_norm(xp, gp, bp, yp, sp, eps, self._stream(stream)))
+        return y
+
+    def layer_norm_backward_workspace(self, dy, x, dx):
+        """Bytes of device memory that layer_norm_backward needs for these tensors."""
+        size = ct.c_uint64(0)
+        _, ptrs = self._views(dy, x, dx)
+        self.check(self.lib.gc_b200_layer_norm_backward_workspace(*ptrs, ct.byref(size)))
+        return size.value
+
+    def layer_norm_backward(self, dy, x, stats, dx, gamma=None, dgamma=None, dbeta=None, workspace=None, stream=0):
+        """gc_b200_layer_norm_backward: gradients from layer_norm's x, gamma and stats."""
+        _, ptrs = self._views(dy, x, gamma, stats, dx, dgamma, dbeta)
+        self.check(self.lib.gc_b200_layer_norm_backward(*ptrs, *self._space(workspace), self._stream(stream)))
+        return dx
+
+    @staticmethod
+    def _words(lengths):
+        return None if lengths is None else lengths.data_ptr()
+
+    def causal_conv(self, x, weight, y, bias=None, state=None, lengths=None, state_out=None, activation='none', stream=0):
+        """gc_b200_causal_conv on borrowed device tensors: x, y (N, L, C), weight
+        (C, K), states (N, K - 1, C), lengths N int32 words."""
+        act = NORM_ACTIVATIONS.get(activation, activation) if isinstance(activation, str) else activation
+        _, (xp, wp, bp, sp, yp, op) = self._views(x, weight, bias, state, y, state_out)
+        self.check(self.lib.gc_b200_causal_conv(xp, wp, bp, sp, self._words(lengths), yp, op, native_int(act),
+                                                self._stream(stream)))
+        return y
+
+    def causal_conv_backward_workspace(self, dy, x, weight, dx):
+        """Bytes of device memory that causal_conv_backward needs for these tensors."""
+        size = ct.c_uint64(0)
+        _, ptrs = self._views(dy, x, weight, dx)
+        self.check(self.lib.gc_b200_causal_conv_backward_workspace(*ptrs, ct.byref(size)))
+        return size.value
+
+    def causal_conv_backward(self, dy, x, weight, dx, bias=None, state=None, dstate_out=None, lengths=None, dweight=None,
+                             dbias=None, dstate=None, activation='none', workspace=None, stream=0):
+        """gc_b200_causal_conv_backward: gradients from causal_conv's arguments."""
+        act = NORM_ACTIVATIONS.get(activation, activation) if isinstance(activation, str) else activation
+        _, p = self._views(dy, x, weight, bias, state, dstate_out, dx, dweight, dbias, dstate)
+        self.check(self.lib.gc_b200_causal_conv_backward(*p[:6], self._words(lengths), *p[6:], native_int(act),
+                                                         *self._space(workspace), self._stream(stream)))
+        return dx
+
+    def causal_conv_step(self, x, weight, state, y, bias=None, state_out=None, activation='none', stream=0):
+        """gc_b200_causal_conv_step: x, y (N, C); the state in place without state_out."""
+        act = NORM_ACTIVATIONS.get(activation, activation) if isinstance(activation, str) else activation
+        _, ptrs = self._views(x, weight, bias, state, y, state if state_out is None else state_out)
+        self.check(self.lib.gc_b200_causal_conv_step(*ptrs, native_int(act), self._stream(stream)))
+        return y
+
+    def selective_scan_sizes(self, args):
+        """(workspace, kept, workspace of the gradient) in bytes, for scan_args()."""
+        sizes = [ct.c_uint64(0) for _ in range(3)]
+        self.check(self.lib.gc_b200_selective_scan_sizes(ct.byref(args), *(ct.byref(s) for s in sizes)))
+        return tuple(s.value for s in sizes)
+
+    def selective_scan(self, args, y, state_out=None, kept=None, workspace=None, stream=0):
+        """gc_b200_selective_scan with scan_args(); kept and workspace are device
+        tensors of selective_scan_sizes() bytes."""
+        _, (yp, op) = self._views(y, state_out)
+        self.check(self.lib.gc_b200_selective_scan(ct.byref(args), yp, op, *self._space(kept), *self._space(workspace),
+                                                   self._stream(stream)))
+        return y
+
+    def selective_scan_backward(self, args, dy, kept, grads, dstate_out=None, workspace=None, stream=0):
+        """gc_b200_selective_scan_backward; grads: a dict of tensors by the names
+        of scan_args()."""
+        _, (gp, op) = self._views(dy, dstate_out)
+        out = _pointers(ScanGrads(), grads)
+        self.check(self.lib.gc_b200_selective_scan_backward(ct.byref(args), gp, op, *self._space(kept), ct.byref(out),
+                                                            *self._space(workspace), self._stream(stream)))
+        return grads
+
+    def selective_scan_step(self, args, y, state_out=None, stream=0):
+        """gc_b200_selective_scan_step; the state of scan_args() in place without state_out."""
+        descs, (yp, op) = self._views(y, state_out)
+        if state_out is None:
+            op = args.state
+        self.check(self.lib.gc_b200_selective_scan_step(ct.byref(args), yp, op, self._stream(stream)))
         return y
 
     def last_plan(self):

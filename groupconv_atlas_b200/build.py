@@ -1,11 +1,12 @@
 """Build recipe for the in-tree drop-in library ``libgroupconv.so``.
 
 nvcc compiles the C ABI (``csrc/common.cpp``), the shared host helpers and the
-sm_100a CUDA engines (``csrc/conv_cuda.cu``, ``csrc/norm_cuda.cu``), each source
-to an object of its own (only those older than what they include, in parallel),
-and links them into a shared library that sits next to this file.  The CUDA runtime is linked as a shared library so that, inside a
-process that already loaded PyTorch's CUDA runtime, both use one runtime
-instance (one current device per thread, one primary context).
+sm_100a CUDA engines (``csrc/*.cu``), each source to an object of its own (only
+those older than what they include, in parallel), and links them into a shared
+library that sits next to this file.  The CUDA runtime is linked as a shared
+library so that, inside a process that already loaded PyTorch's CUDA runtime,
+both use one runtime instance (one current device per thread, one primary
+context).
 
     python -m groupconv_atlas_b200.build          # build if stale
     python -m groupconv_atlas_b200.build --force  # always rebuild
@@ -112,7 +113,8 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
     return LIBRARY
 
 
-TORCH_EXT_SOURCE = PACKAGE / 'torch_ext' / 'conv_op.cpp'
+TORCH_EXT = PACKAGE / 'torch_ext'
+TORCH_EXT_SOURCES = [TORCH_EXT / 'conv_op.cpp', TORCH_EXT / 'sequence_op.cpp']
 
 
 def torch_ext_path() -> Path:
@@ -122,26 +124,41 @@ def torch_ext_path() -> Path:
 
 
 def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the PyTorch front end (torch_ext/conv_op.cpp, a thin C++ caller
-    of gc_cuda_conv that allocates the output with PyTorch) against the
-    in-tree library, when it is older than its sources."""
+    """Compile the PyTorch front end (torch_ext/*.cpp, thin C++ callers of the
+    C ABI that allocate outputs with PyTorch) against the in-tree library, when
+    it is older than its sources; each source to an object of its own, in
+    parallel."""
     import sysconfig
     import torch
     from torch.utils import cpp_extension
     target = torch_ext_path()
-    deps = [TORCH_EXT_SOURCE, INCLUDE / 'groupconv.h', LIBRARY, Path(__file__)]
-    if not force and target.exists() and all(d.stat().st_mtime <= target.stat().st_mtime for d in deps):
+    shared = [TORCH_EXT / 'front_end.h', INCLUDE / 'groupconv.h', Path(__file__)]
+    if not force and target.exists() and all(d.stat().st_mtime <= target.stat().st_mtime
+                                             for d in [*TORCH_EXT_SOURCES, *shared, LIBRARY]):
         return target
     cuda_include = Path(nvcc()).resolve().parent.parent / 'include'
     torch_lib = cpp_extension.library_paths()[0]
     abi = int(torch.compiled_with_cxx11_abi())
-    cmd = ['g++', '-O2', '-std=c++17', '-shared', '-fPIC', f'-D_GLIBCXX_USE_CXX11_ABI={abi}',
-           '-DTORCH_EXTENSION_NAME=_gcb_torch', '-DTORCH_API_INCLUDE_EXTENSION_H',
-           *[f'-I{d}' for d in cpp_extension.include_paths()], f'-I{sysconfig.get_paths()["include"]}',
-           f'-I{cuda_include}', f'-I{INCLUDE}', str(TORCH_EXT_SOURCE),
-           f'-L{PACKAGE}', '-lgroupconv', f'-L{torch_lib}', '-lc10', '-lc10_cuda', '-ltorch', '-ltorch_cpu',
-           '-ltorch_cuda', '-ltorch_python', f'-Wl,-rpath,$ORIGIN', f'-Wl,-rpath,{torch_lib}', '-o', str(target) + '.part']
-    run_tool(cmd, verbose)
+    flags = ['-O2', '-std=c++17', '-fPIC', f'-D_GLIBCXX_USE_CXX11_ABI={abi}',
+             '-DTORCH_EXTENSION_NAME=_gcb_torch', '-DTORCH_API_INCLUDE_EXTENSION_H',
+             *[f'-I{d}' for d in cpp_extension.include_paths()], f'-I{sysconfig.get_paths()["include"]}',
+             f'-I{cuda_include}', f'-I{INCLUDE}']
+    OBJECTS.mkdir(exist_ok=True)
+
+    def compile_one(source):
+        out = OBJECTS / (source.name + '.o')
+        if force or not out.exists() or any(d.stat().st_mtime > out.stat().st_mtime for d in [source, *shared]):
+            part = out.with_suffix('.part')
+            run_tool(['g++', *flags, '-c', str(source), '-o', str(part)], verbose)
+            part.replace(out)
+        return out
+
+    with concurrent.futures.ThreadPoolExecutor() as pool:
+        objects = list(pool.map(compile_one, TORCH_EXT_SOURCES))
+    run_tool(['g++', '-shared', *map(str, objects),
+              f'-L{PACKAGE}', '-lgroupconv', f'-L{torch_lib}', '-lc10', '-lc10_cuda', '-ltorch', '-ltorch_cpu',
+              '-ltorch_cuda', '-ltorch_python', f'-Wl,-rpath,$ORIGIN', f'-Wl,-rpath,{torch_lib}', '-o',
+              str(target) + '.part'], verbose)
     Path(str(target) + '.part').replace(target)
     return target
 

@@ -79,6 +79,10 @@ std::string format_plan(const PlanRecord &r) {
         std::snprintf(buf, sizeof(buf), "kernel=dropout engine=%s grid=%lld block=%lld vec=%lld", r.name, v[0], v[1],
                       v[2]);
         break;
+    case PlanRecord::kSequence:
+        std::snprintf(buf, sizeof(buf), "kernel=%s grid=%lld block=%lld vec=%lld lanes=%lld per_lane=%lld parts=%lld "
+                      "launches=%lld", r.name, v[0], v[1], v[2], v[3], v[4], v[5], v[6]);
+        break;
     case PlanRecord::kGeneral:
         std::snprintf(buf, sizeof(buf), "kernel=general grid=%lld block=%lld run=%lld cob=%lld index=%s runs=%lld",
                       v[0], v[1], v[2], v[3], v[4] ? "32" : "64", v[5]);

@@ -15,7 +15,7 @@ namespace gcb {
 // when gc_b200_last_plan asks for it (formatting costs about a third of a
 // microsecond, a tenth of the host time of a call).
 struct PlanRecord {
-    enum Kind { kNone, kDirect, kWide, kTf32, kSmall, kGeneral, kDw, kDwS2, kNhwc, kNorm, kDropout } kind = kNone;
+    enum Kind { kNone, kDirect, kWide, kTf32, kSmall, kGeneral, kDw, kDwS2, kNhwc, kNorm, kDropout, kSequence } kind = kNone;
     const char *name = "";  // variant name, static storage
     bool tma = false;
     long long v[14] = {};

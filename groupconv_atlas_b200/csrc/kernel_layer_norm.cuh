@@ -1,0 +1,320 @@
+// Layer normalisation of rows, and its gradient.
+//
+//   y  = (x - mean) rstd gamma + beta,  rstd = 1 / sqrt(var + eps)
+//   dx = rstd (g - mean(g) - xhat mean(g xhat)),  g = dy gamma, xhat = (x - mean) rstd
+//   dgamma = sum over rows of dy xhat,  dbeta = sum over rows of dy
+//
+// All of it is bound by memory: x (and dy) is read once, held in registers
+// through the sums, and the result written.  A team of threads takes a row: a
+// power of two of at most 32, several to a warp, or a whole block.  The variance
+// is the mean of squares about the mean, from the values in registers.
+#pragma once
+#include "norm_util.cuh"
+
+namespace gcb {
+
+struct LayerNormParams {
+    const void *x, *dy;  // dy: gradient only
+    void *y;             // or dx
+    long long rows, x_ld, dy_ld, y_ld;
+    int c, vcols;        // elements and vectors of a row
+    int team;            // threads that take a row
+    const void *gamma, *beta;
+    int gamma_type, beta_type;
+    float eps;
+    float2 *stats;       // mean and rstd of each row; nullable in the forward pass
+    float *part;         // gradient: dgamma and dbeta of each block, [block][2][c]; NULL where neither is wanted
+};
+
+constexpr int kRowThreads = 256, kRowMost = 512;  // threads of a block of small teams; of a block that is a team
+
+// Sums over a team, the same in every thread.  buf: two turns of [warps][N].
+template <int N>
+__device__ __forceinline__ void team_sums(float (&v)[N], int team, float *buf, int &turn) {
+    for (int o = min(team, 32) / 2; o > 0; o /= 2) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
+    if (team <= 32) return;
+    // A turn's buffer is written again two sums later, behind a barrier that
+    // every thread reaches after reading it.
+    float *mine = buf + turn * (kRowMost / 32) * N;
+    turn ^= 1;
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) mine[warp * N + i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = mine[i];
+    for (int w = 1; w < warps; ++w) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += mine[w * N + i];
+    }
+}
+
+// NV vectors a thread and row, ROWS rows at a time.
+template <class T, int V, int NV, int ROWS>
+__global__ void __launch_bounds__(kRowMost) layer_norm_kernel(const __grid_constant__ LayerNormParams P) {
+    __shared__ float buf[2 * (kRowMost / 32) * ROWS];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int teams = blockDim.x / P.team, team = threadIdx.x / P.team, lane = threadIdx.x - team * P.team;
+    const long long all = static_cast<long long>(gridDim.x) * teams;
+    const float inv = 1.0f / static_cast<float>(P.c);
+    int turn = 0;
+    for (long long first = static_cast<long long>(blockIdx.x) * teams; first < P.rows; first += all * ROWS) {
+        Raw<T, V> raw[ROWS][NV];
+        float s[ROWS], q[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = first + team + r * all;
+            const T *src = static_cast<const T *>(P.x) + row * P.x_ld;
+            s[r] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int v = lane + j * P.team;
+                if (row < P.rows && v < P.vcols) raw[r][j] = load_raw<T, V>(src + static_cast<long long>(v) * V);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = first + team + r * all;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (row < P.rows && lane + j * P.team < P.vcols) {
+                    float e[V];
+                    values_of<V>(lanes_of_raw<T, V>(raw[r][j]), e);
+#pragma unroll
+                    for (int k = 0; k < V; ++k) s[r] += e[k];
+                }
+        }
+        team_sums<ROWS>(s, P.team, buf, turn);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = first + team + r * all;
+            s[r] *= inv;
+            q[r] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (row < P.rows && lane + j * P.team < P.vcols) {
+                    float e[V];
+                    values_of<V>(lanes_of_raw<T, V>(raw[r][j]), e);
+#pragma unroll
+                    for (int k = 0; k < V; ++k) q[r] = fmaf(e[k] - s[r], e[k] - s[r], q[r]);
+                }
+        }
+        team_sums<ROWS>(q, P.team, buf, turn);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) q[r] = 1.0f / sqrtf(fmaf(q[r], inv, P.eps));
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int v = lane + j * P.team;
+            if (v >= P.vcols) continue;
+            float gamma[V], beta[V];
+            load_params<V>(P.gamma, P.gamma_type, static_cast<long long>(v) * V, 1.0f, gamma);
+            load_params<V>(P.beta, P.beta_type, static_cast<long long>(v) * V, 0.0f, beta);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const long long row = first + team + r * all;
+                if (row >= P.rows) continue;
+                float e[V];
+                values_of<V>(lanes_of_raw<T, V>(raw[r][j]), e);
+#pragma unroll
+                for (int k = 0; k < V; ++k) e[k] = fmaf((e[k] - s[r]) * q[r], gamma[k], beta[k]);
+                store_elems<T, V>(static_cast<T *>(P.y) + row * P.y_ld + static_cast<long long>(v) * V, e);
+            }
+        }
+        if (P.stats != nullptr && lane == 0) {
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const long long row = first + team + r * all;
+                if (row < P.rows) P.stats[row] = make_float2(s[r], q[r]);
+            }
+        }
+    }
+}
+
+// The gradient.  A block's teams take rows in turn and add up dgamma and dbeta of
+// their columns in registers, over at most 64 rows (the launch sees to that); at
+// the end the block joins its teams in a fixed order.  Dynamic shared memory:
+// [warps][2][c] values where a row takes at most a warp.
+template <class T, int V, int NV>
+__global__ void __launch_bounds__(kRowMost) layer_norm_grad_kernel(const __grid_constant__ LayerNormParams P) {
+    extern __shared__ float joined[];
+    __shared__ float buf[2 * (kRowMost / 32) * 2];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int teams = blockDim.x / P.team, team = threadIdx.x / P.team, lane = threadIdx.x - team * P.team;
+    const long long all = static_cast<long long>(gridDim.x) * teams;
+    const float inv = 1.0f / static_cast<float>(P.c);
+    float gamma[NV][V], dgamma[NV][V], dbeta[NV][V];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) gamma[j][k] = dgamma[j][k] = dbeta[j][k] = 0.0f;
+        const int v = lane + j * P.team;
+        if (v < P.vcols) load_params<V>(P.gamma, P.gamma_type, static_cast<long long>(v) * V, 1.0f, gamma[j]);
+    }
+    int turn = 0;
+    for (long long first = static_cast<long long>(blockIdx.x) * teams; first < P.rows; first += all) {
+        const long long row = first + team;
+        const bool live = row < P.rows;
+        Raw<T, V> rx[NV], rg[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int v = lane + j * P.team;
+            if (live && v < P.vcols) {
+                rx[j] = load_raw<T, V>(static_cast<const T *>(P.x) + row * P.x_ld + static_cast<long long>(v) * V);
+                rg[j] = load_raw<T, V>(static_cast<const T *>(P.dy) + row * P.dy_ld + static_cast<long long>(v) * V);
+            }
+        }
+        const float2 st = live ? P.stats[row] : make_float2(0.0f, 0.0f);
+        float sums[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (live && lane + j * P.team < P.vcols) {
+                float e[V], d[V];
+                values_of<V>(lanes_of_raw<T, V>(rx[j]), e);
+                values_of<V>(lanes_of_raw<T, V>(rg[j]), d);
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const float xhat = (e[k] - st.x) * st.y, g = d[k] * gamma[j][k];
+                    sums[0] += g;
+                    sums[1] = fmaf(g, xhat, sums[1]);
+                    dgamma[j][k] = fmaf(d[k], xhat, dgamma[j][k]);
+                    dbeta[j][k] += d[k];
+                }
+            }
+        team_sums<2>(sums, P.team, buf, turn);
+        const float m1 = sums[0] * inv, m2 = sums[1] * inv;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int v = lane + j * P.team;
+            if (live && v < P.vcols) {
+                float e[V], d[V];
+                values_of<V>(lanes_of_raw<T, V>(rx[j]), e);
+                values_of<V>(lanes_of_raw<T, V>(rg[j]), d);
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const float xhat = (e[k] - st.x) * st.y;
+                    e[k] = st.y * (fmaf(d[k], gamma[j][k], -m1) - xhat * m2);
+                }
+                store_elems<T, V>(static_cast<T *>(P.y) + row * P.y_ld + static_cast<long long>(v) * V, e);
+            }
+        }
+    }
+    if (P.part == nullptr) return;
+    float *out = P.part + static_cast<long long>(blockIdx.x) * 2 * P.c;
+    if (P.team > 32) {  // one team: the columns are the thread's own
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int v = lane + j * P.team;
+            if (v >= P.vcols) continue;
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                out[v * V + k] = dgamma[j][k];
+                out[P.c + v * V + k] = dbeta[j][k];
+            }
+        }
+        return;
+    }
+    for (int o = P.team; o < 32; o *= 2) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                dgamma[j][k] += __shfl_xor_sync(0xffffffffu, dgamma[j][k], o);
+                dbeta[j][k] += __shfl_xor_sync(0xffffffffu, dbeta[j][k], o);
+            }
+    }
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if ((threadIdx.x & 31) < P.team) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int v = lane + j * P.team;
+            if (v >= P.vcols) continue;
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                joined[(2 * warp) * P.c + v * V + k] = dgamma[j][k];
+                joined[(2 * warp + 1) * P.c + v * V + k] = dbeta[j][k];
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * P.c; i += blockDim.x) {
+        float s = joined[i];
+        for (int w = 1; w < warps; ++w) s += joined[2 * w * P.c + i];
+        out[i] = s;
+    }
+}
+
+// Rows too long for a block's registers: read three times (the second and third
+// time from the caches), one row to a block.
+template <class T>
+__global__ void __launch_bounds__(kRowMost) layer_norm_long_kernel(const __grid_constant__ LayerNormParams P) {
+    __shared__ float buf[2 * (kRowMost / 32)];
+    griddep_wait();
+    griddep_launch_dependents();
+    const float inv = 1.0f / static_cast<float>(P.c);
+    int turn = 0;
+    for (long long row = blockIdx.x; row < P.rows; row += gridDim.x) {
+        const T *src = static_cast<const T *>(P.x) + row * P.x_ld;
+        T *dst = static_cast<T *>(P.y) + row * P.y_ld;
+        float s[1] = {0.0f}, q[1] = {0.0f};
+        for (int i = threadIdx.x; i < P.c; i += kRowMost) s[0] += to_float(src[i]);
+        team_sums<1>(s, kRowMost, buf, turn);
+        const float mean = s[0] * inv;
+        for (int i = threadIdx.x; i < P.c; i += kRowMost) {
+            const float d = to_float(src[i]) - mean;
+            q[0] = fmaf(d, d, q[0]);
+        }
+        team_sums<1>(q, kRowMost, buf, turn);
+        const float rstd = 1.0f / sqrtf(fmaf(q[0], inv, P.eps));
+        for (int i = threadIdx.x; i < P.c; i += kRowMost) {
+            const float gamma = P.gamma != nullptr ? load_param(P.gamma, P.gamma_type, i) : 1.0f;
+            const float beta = P.beta != nullptr ? load_param(P.beta, P.beta_type, i) : 0.0f;
+            dst[i] = from_float<T>(fmaf((to_float(src[i]) - mean) * rstd, gamma, beta));
+        }
+        if (P.stats != nullptr && threadIdx.x == 0) P.stats[row] = make_float2(mean, rstd);
+    }
+}
+
+// A thread's columns of the block's sums are its own, so they add up in the
+// workspace.
+template <class T>
+__global__ void __launch_bounds__(kRowMost) layer_norm_long_grad_kernel(const __grid_constant__ LayerNormParams P) {
+    __shared__ float buf[2 * (kRowMost / 32) * 2];
+    griddep_wait();
+    griddep_launch_dependents();
+    const float inv = 1.0f / static_cast<float>(P.c);
+    float *out = P.part == nullptr ? nullptr : P.part + static_cast<long long>(blockIdx.x) * 2 * P.c;
+    int turn = 0;
+    for (long long row = blockIdx.x; row < P.rows; row += gridDim.x) {
+        const T *x = static_cast<const T *>(P.x) + row * P.x_ld, *dy = static_cast<const T *>(P.dy) + row * P.dy_ld;
+        T *dst = static_cast<T *>(P.y) + row * P.y_ld;
+        const float2 st = P.stats[row];
+        float sums[2] = {0.0f, 0.0f};
+        for (int i = threadIdx.x; i < P.c; i += kRowMost) {
+            const float gamma = P.gamma != nullptr ? load_param(P.gamma, P.gamma_type, i) : 1.0f;
+            const float d = to_float(dy[i]), xhat = (to_float(x[i]) - st.x) * st.y, g = d * gamma;
+            sums[0] += g;
+            sums[1] = fmaf(g, xhat, sums[1]);
+            if (out != nullptr) {
+                const bool fresh = row == blockIdx.x;
+                out[i] = fmaf(d, xhat, fresh ? 0.0f : out[i]);
+                out[P.c + i] = d + (fresh ? 0.0f : out[P.c + i]);
+            }
+        }
+        team_sums<2>(sums, kRowMost, buf, turn);
+        const float m1 = sums[0] * inv, m2 = sums[1] * inv;
+        for (int i = threadIdx.x; i < P.c; i += kRowMost) {
+            const float gamma = P.gamma != nullptr ? load_param(P.gamma, P.gamma_type, i) : 1.0f;
+            const float xhat = (to_float(x[i]) - st.x) * st.y;
+            dst[i] = from_float<T>(st.y * (fmaf(to_float(dy[i]), gamma, -m1) - xhat * m2));
+        }
+    }
+}
+
+}  // namespace gcb

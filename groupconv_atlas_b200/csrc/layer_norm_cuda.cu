@@ -1,0 +1,328 @@
+// gc_b200_layer_norm and its gradient: descriptor checks, plans and launches.
+// Nothing here allocates device memory, synchronizes or keeps anything of a call.
+#include "groupconv.h"
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "host_util.h"
+#include "kernel_layer_norm.cuh"
+#include "sequence_util.cuh"
+
+namespace {
+
+using namespace gcb;
+
+// x as rows of its last axis, evenly spaced.
+struct Rows {
+    Strided t;
+    long long rows = 1, ld = 0;
+};
+int rows_of(const gc_tensor *t, Rows &v) {
+    const int st = strided_of(t, v.t);
+    if (st != GC_OK) return st;
+    const int last = t->rank - 1;
+    v.rows = 1;
+    v.ld = v.t.d[last];
+    bool even = true;
+    for (int i = last - 1; i >= 0; --i) {
+        if (v.t.d[i] > 1) {
+            if (v.rows == 1) v.ld = v.t.s[i];
+            else even = even && static_cast<wide>(v.ld) * v.rows == v.t.s[i];
+        }
+        v.rows *= v.t.d[i];
+    }
+    return even || v.t.empty ? GC_OK : gc_error(GC_UNSUPPORTED, "rows are not evenly spaced");
+}
+
+// Data tensors of the same dims and type; views[0] is x's.
+int check_rows(std::initializer_list<const gc_tensor *> tensors, Rows *views) {
+    const gc_tensor *first = *tensors.begin();
+    int64_t count = 0;
+    for (const gc_tensor *t : tensors) {
+        const int st = check_fields(t, 1, 4, count);
+        if (st != GC_OK) return st;
+        if (!same_dims(t, first)) return gc_error(GC_INVALID, "tensor dimensions differ");
+        if (t->dtype != first->dtype) return gc_error(GC_INVALID, "tensor dtypes differ");
+        if (t->device_index != first->device_index) return gc_error(GC_INVALID, "tensor device indices differ");
+    }
+    const int64_t c = first->dims[first->rank - 1];
+    if (c < 1 || c > INT32_MAX) return gc_error(GC_INVALID, "row length out of range");
+    for (const gc_tensor *t : tensors) {
+        const int st = rows_of(t, *views++);
+        if (st != GC_OK) return st;
+    }
+    return GC_OK;
+}
+
+int check_row_stats(const gc_tensor *t, const gc_tensor *x, long long rows) {
+    int64_t count = 0;
+    const int st = check_fields(t, 2, 2, count);
+    if (st != GC_OK) return st;
+    if (t->dtype != GC_F32 || t->dims[0] != rows || t->dims[1] != 2)
+        return gc_error(GC_INVALID, "stats must be an F32 tensor of dims (rows, 2)");
+    if (t->device_index != x->device_index) return gc_error(GC_INVALID, "tensor device indices differ");
+    if (reinterpret_cast<uintptr_t>(t->data) % 8 != 0) return gc_error(GC_INVALID, "stats must be 8-byte aligned");
+    return GC_OK;
+}
+
+struct RowPlan {
+    bool vec = false, whole = false;  // whole: rows too long for registers
+    int type = 0, v = 1, nv = 1, team = 1, threads = kRowThreads;
+    size_t smem = 0;
+    long long blocks = 0;
+};
+
+const char *const kDenseParams = "parameters must be dense";
+
+// One vector of a row for each thread, two or four where a row would need more
+// than a block; rows of at most a warp share a block.  Single elements are taken
+// four or sixteen a thread.
+void plan_rows(int c, int type, bool vec, bool backward, RowPlan &p) {
+    p.type = type;
+    p.vec = vec;
+    p.v = !vec ? 1 : type == kElemF32 ? 4 : 8;
+    const long long vcols = c / p.v;
+    const int low = vec ? 1 : 4, high = !vec ? 16 : backward && p.v == 8 ? 2 : 4;
+    p.nv = low;
+    if (vec && !backward) {  // short rows stay within a warp, which has no barriers
+        if (vcols > 32 && vcols <= 64) p.nv = 2;
+        else if (vcols > 64 && vcols <= 128) p.nv = 4;
+    } else if (vec && vcols > 32 && vcols <= 64) {
+        p.nv = 2;
+    }
+    while (p.nv < high && ceil_div(vcols, p.nv) > kRowMost) p.nv *= vec ? 2 : 4;
+    const long long lanes = ceil_div(vcols, p.nv);
+    p.whole = lanes > kRowMost;
+    if (p.whole) {
+        p.team = p.threads = kRowMost;
+    } else if (lanes > 32) {
+        p.team = p.threads = static_cast<int>(round_up(lanes, 32));
+    } else {
+        p.threads = kRowThreads;
+        for (p.team = 1; p.team < lanes;) p.team *= 2;
+    }
+    if (backward && !p.whole && p.team <= 32) p.smem = static_cast<size_t>(p.threads / 32) * 2 * c * sizeof(float);
+}
+
+template <class T, int V>
+const void *forward_typed(int nv) {
+    if constexpr (V == 1)
+        return nv == 4 ? reinterpret_cast<const void *>(&layer_norm_kernel<T, 1, 4, 2>)
+                       : reinterpret_cast<const void *>(&layer_norm_kernel<T, 1, 16, 1>);
+    else
+        return nv == 1   ? reinterpret_cast<const void *>(&layer_norm_kernel<T, V, 1, 4>)
+               : nv == 2 ? reinterpret_cast<const void *>(&layer_norm_kernel<T, V, 2, 2>)
+                         : reinterpret_cast<const void *>(&layer_norm_kernel<T, V, 4, 1>);
+}
+template <class T, int V>
+const void *backward_typed(int nv) {
+    if constexpr (V == 1)
+        return nv == 4 ? reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, 1, 4>)
+                       : reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, 1, 16>);
+    else if constexpr (V == 8)
+        return nv == 1 ? reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, V, 1>)
+                       : reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, V, 2>);
+    else
+        return nv == 1   ? reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, V, 1>)
+               : nv == 2 ? reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, V, 2>)
+                         : reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, V, 4>);
+}
+template <class T>
+const void *row_kernel(const RowPlan &p, bool backward) {
+    if (p.whole)
+        return backward ? reinterpret_cast<const void *>(&layer_norm_long_grad_kernel<T>)
+                        : reinterpret_cast<const void *>(&layer_norm_long_kernel<T>);
+    if (p.vec) return backward ? backward_typed<T, kVec<T>>(p.nv) : forward_typed<T, kVec<T>>(p.nv);
+    return backward ? backward_typed<T, 1>(p.nv) : forward_typed<T, 1>(p.nv);
+}
+const void *row_kernel(const RowPlan &p, bool backward) {
+    return p.type == kElemF16    ? row_kernel<__half>(p, backward)
+           : p.type == kElemBF16 ? row_kernel<__nv_bfloat16>(p, backward)
+                                 : row_kernel<float>(p, backward);
+}
+
+// Blocks of the gradient: two a multiprocessor, more where a team would add up
+// more than 64 rows.
+long long grad_blocks(const RowPlan &p, long long rows, int sms) {
+    const int teams = p.threads / p.team;
+    return std::max(std::min(ceil_div(rows, teams), 2LL * sms * (kRowMost / p.threads)),
+                    ceil_div(rows, static_cast<long long>(kSumRun) * teams));
+}
+
+bool vectors(std::initializer_list<const Rows *> views) {
+    for (const Rows *v : views) {
+        const int e = v->t.type == kElemF32 ? 4 : 8;
+        if (!group_aligned(v->t, e) || v->ld % e != 0) return false;
+    }
+    return true;
+}
+
+void set_param(const gc_tensor *t, const void *&p, int &type) {
+    p = t != nullptr ? t->data : nullptr;
+    type = t != nullptr ? elem_type(t->dtype) : kElemF32;
+}
+
+// Dynamic shared memory that a kernel may have beside its own buffer.
+int dynamic_limit(const DeviceFacts &facts) { return facts.smem_optin - 2048; }
+
+int current_facts(DeviceFacts &facts) {
+    int dev = -1;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
+    return device_facts(dev, facts);
+}
+
+}  // namespace
+
+extern "C" {
+
+int gc_b200_layer_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tensor *beta, gc_tensor *y,
+                       gc_tensor *stats, double eps, void *stream) try {
+    Rows v[2];
+    int st = check_rows({x, y}, v);
+    if (st != GC_OK) return st;
+    if (!(eps >= 0.0) || !std::isfinite(eps)) return gc_error(GC_INVALID, "eps must be finite and not negative");
+    const int64_t c = x->dims[x->rank - 1];
+    for (const gc_tensor *t : {gamma, beta})
+        if ((st = check_param(t, x, {c})) != GC_OK) return st;
+    if (stats != nullptr && (st = check_row_stats(stats, x, v[0].rows)) != GC_OK) return st;
+    if (outputs_meet({range_of(v[1].t), range_of(stats)}, {range_of(v[0].t), range_of(gamma), range_of(beta)}))
+        return gc_error(GC_INVALID, "outputs must not overlap inputs or one another");
+    for (const gc_tensor *t : {gamma, beta})
+        if ((st = check_dense(t, kDenseParams)) != GC_OK) return st;
+    if ((st = check_dense(stats, "stats must be dense")) != GC_OK) return st;
+    if (v[0].t.empty) return gc_error(GC_OK, "");
+    int dev = -1;
+    if ((st = check_call({x, y, gamma, beta, stats}, {}, x->device_index, stream, dev)) != GC_OK) return st;
+    DeviceFacts facts;
+    if ((st = device_facts(dev, facts)) != GC_OK) return st;
+    RowPlan plan;
+    plan_rows(static_cast<int>(c), v[0].t.type, vectors({&v[0], &v[1]}), false, plan);
+    LayerNormParams P{};
+    P.x = v[0].t.data;
+    P.x_ld = v[0].ld;
+    P.y = v[1].t.data;
+    P.y_ld = v[1].ld;
+    P.rows = v[0].rows;
+    P.c = static_cast<int>(c);
+    P.vcols = P.c / plan.v;
+    P.team = plan.team;
+    P.eps = static_cast<float>(eps);
+    set_param(gamma, P.gamma, P.gamma_type);
+    set_param(beta, P.beta, P.beta_type);
+    P.stats = stats != nullptr ? static_cast<float2 *>(stats->data) : nullptr;
+    const void *fn = row_kernel(plan, false);
+    int ctas = 1;
+    if ((st = kernel_occupancy(dev, fn, plan.threads, 0, dynamic_limit(facts), ctas)) != GC_OK) return st;
+    const long long grid = std::min(ceil_div(P.rows, plan.threads / plan.team), static_cast<long long>(ctas) * facts.sms);
+    void *args[] = {&P};
+    const cudaError_t e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(plan.threads), args, 0,
+                                     reinterpret_cast<cudaStream_t>(stream));
+    return launched(e, PlanRecord::kSequence, plan.whole ? "layer_norm_long" : "layer_norm", grid, plan.threads,
+                    plan.vec ? 1 : 0, plan.team, plan.nv, 1, 1);
+} catch (...) {
+    return internal_error();
+}
+
+int gc_b200_layer_norm_backward_workspace(const gc_tensor *dy, const gc_tensor *x, const gc_tensor *dx,
+                                          uint64_t *bytes) try {
+    if (bytes == nullptr) return gc_error(GC_INVALID, "null size pointer");
+    Rows v[3];
+    int st = check_rows({x, dy, dx}, v);
+    if (st != GC_OK) return st;
+    *bytes = 0;
+    if (v[0].t.empty) return gc_error(GC_OK, "");
+    DeviceFacts facts;
+    if ((st = current_facts(facts)) != GC_OK) return st;
+    RowPlan plan;
+    const int c = static_cast<int>(x->dims[x->rank - 1]);
+    plan_rows(c, v[0].t.type, vectors({&v[0], &v[1], &v[2]}), true, plan);
+    *bytes = up16(static_cast<uint64_t>(grad_blocks(plan, v[0].rows, facts.sms)) * 2 * c * sizeof(float));
+    return gc_error(GC_OK, "");
+} catch (...) {
+    return internal_error();
+}
+
+int gc_b200_layer_norm_backward(const gc_tensor *dy, const gc_tensor *x, const gc_tensor *gamma,
+                                const gc_tensor *stats, gc_tensor *dx, gc_tensor *dgamma, gc_tensor *dbeta,
+                                void *workspace, uint64_t workspace_bytes, void *stream) try {
+    Rows v[3];
+    int st = check_rows({x, dy, dx}, v);
+    if (st != GC_OK) return st;
+    const int64_t c = x->dims[x->rank - 1];
+    const gc_tensor *const params[] = {gamma, dgamma, dbeta};
+    for (const gc_tensor *t : params)
+        if ((st = check_param(t, x, {c})) != GC_OK) return st;
+    if ((st = check_row_stats(stats, x, v[0].rows)) != GC_OK) return st;
+    if (outputs_meet({range_of(v[2].t), range_of(dgamma), range_of(dbeta), {workspace, workspace_bytes}},
+                     {range_of(v[0].t), range_of(v[1].t), range_of(gamma), range_of(stats)}))
+        return gc_error(GC_INVALID, "outputs and workspace must not overlap inputs or one another");
+    for (const gc_tensor *t : params)
+        if ((st = check_dense(t, kDenseParams)) != GC_OK) return st;
+    if ((st = check_dense(stats, "stats must be dense")) != GC_OK) return st;
+    int dev = -1;
+    if ((st = check_call({x, dy, dx, gamma, stats, dgamma, dbeta}, {}, x->device_index, stream, dev)) != GC_OK) return st;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const bool sums = dgamma != nullptr || dbeta != nullptr;
+    cudaError_t e = cudaSuccess;
+    if (v[0].t.empty) {  // sums over nothing
+        for (const gc_tensor *t : {dgamma, dbeta})
+            if (t != nullptr && e == cudaSuccess) e = cudaMemsetAsync(t->data, 0, range_of(t).bytes, s);
+        return launched(e);
+    }
+    DeviceFacts facts;
+    if ((st = device_facts(dev, facts)) != GC_OK) return st;
+    RowPlan plan;
+    plan_rows(static_cast<int>(c), v[0].t.type, vectors({&v[0], &v[1], &v[2]}), true, plan);
+    const long long grid = grad_blocks(plan, v[0].rows, facts.sms);
+    if (sums) {
+        const uint64_t need = up16(static_cast<uint64_t>(grid) * 2 * c * sizeof(float));
+        if ((st = check_workspace(workspace, workspace_bytes, need)) != GC_OK) return st;
+        if ((st = check_device_memory(workspace, x->device_index, dev)) != GC_OK) return st;
+    }
+    if (grid > INT32_MAX) return gc_error(GC_UNSUPPORTED, "more rows than a grid has blocks");
+    LayerNormParams P{};
+    P.x = v[0].t.data;
+    P.x_ld = v[0].ld;
+    P.dy = v[1].t.data;
+    P.dy_ld = v[1].ld;
+    P.y = v[2].t.data;
+    P.y_ld = v[2].ld;
+    P.rows = v[0].rows;
+    P.c = static_cast<int>(c);
+    P.vcols = P.c / plan.v;
+    P.team = plan.team;
+    set_param(gamma, P.gamma, P.gamma_type);
+    P.stats = static_cast<float2 *>(stats->data);
+    P.part = sums ? static_cast<float *>(workspace) : nullptr;
+    const void *fn = row_kernel(plan, true);
+    int ctas = 1;
+    if ((st = kernel_occupancy(dev, fn, plan.threads, plan.smem, dynamic_limit(facts), ctas)) != GC_OK) return st;
+    void *args[] = {&P};
+    e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(plan.threads), args, plan.smem, s);
+    if (e == cudaSuccess && sums) {
+        SumParams S{};
+        S.part = P.part;
+        S.rows = grid;
+        S.cols = c;
+        S.planes = 2;
+        int i = 0;
+        for (const gc_tensor *t : {dgamma, dbeta}) {
+            S.out[i] = t != nullptr ? t->data : nullptr;
+            S.type[i] = t != nullptr ? elem_type(t->dtype) : kElemF32;
+            S.mul[i++] = 1;
+        }
+        void *sum_args[] = {&S};
+        e = launch_pdl(reinterpret_cast<const void *>(&sum_rows_kernel), dim3(static_cast<unsigned>(2 * ceil_div(c, 32))),
+                       dim3(kSumWarps * 32), sum_args, 0, s);
+    }
+    return launched(e, PlanRecord::kSequence, plan.whole ? "layer_norm_long_backward" : "layer_norm_backward", grid,
+                    plan.threads, plan.vec ? 1 : 0, plan.team, plan.nv, 1, sums ? 2 : 1);
+} catch (...) {
+    return internal_error();
+}
+
+}  // extern "C"

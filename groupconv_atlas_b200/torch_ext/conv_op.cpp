@@ -8,51 +8,12 @@
 // message; nothing here computes a convolution.  conv_ex does the same for
 // gc_b200_conv_ex (bias, activation, channels-last output); group_norm and
 // dropout do it for gc_b200_group_norm and gc_b200_dropout and record their
-// gradients with autograd.
-#include <torch/extension.h>
-#include <ATen/cuda/CUDAGeneratorImpl.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/saved_variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
+// gradients with autograd.  sequence_op.cpp holds the operators on sequences.
+#include "front_end.h"
 
-#include <algorithm>
-#include <memory>
-#include <mutex>
-#include <stdexcept>
-#include <string>
-#include <vector>
-
-#include "groupconv.h"
+using namespace front_end;
 
 namespace {
-
-gc_tensor describe(const at::Tensor &t) {
-    gc_tensor d{};
-    d.data = t.data_ptr();
-    d.bytes = static_cast<uint64_t>(t.numel()) * t.element_size();
-    d.dtype = t.scalar_type() == at::kFloat ? GC_F32 : t.scalar_type() == at::kDouble ? GC_F64 : -1;
-    d.device = t.is_cuda() ? GC_CUDA : t.is_cpu() ? GC_CPU : -1;
-    d.device_index = t.is_cuda() ? t.get_device() : 0;
-    d.rank = static_cast<int32_t>(t.dim());
-    for (int i = 0; i < 4 && i < t.dim(); ++i) {
-        d.dims[i] = t.size(i);
-        d.strides[i] = t.stride(i);
-    }
-    return d;
-}
-
-// A tracer records what passes through the dispatcher: of these calls only the
-// output's allocation, so that the recorded graph would return memory that
-// nothing writes.
-void no_tracing() {
-    if (torch::jit::tracer::isTracing() ||
-        c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value())
-        throw std::runtime_error("this operation cannot be traced");
-}
 
 // y = conv(x, w) with the layer's geometry; x must be 4-D.  Raises
 // RuntimeError("gc_status <s>: <message>") on any non-OK status.
@@ -108,34 +69,6 @@ at::Tensor conv_ex(const at::Tensor &x, const at::Tensor &w, const c10::optional
 
 
 // ---- group norm and dropout -----------------------------------------------------
-
-[[noreturn]] void fail(int status) {
-    throw std::runtime_error("gc_status " + std::to_string(status) + ": " + gc_last_error());
-}
-
-// As describe(), for the entry points that also take 16-bit types and strided
-// views: bytes covers the view from its first to its last element.
-gc_tensor describe_view(const at::Tensor &t) {
-    gc_tensor d = describe(t);
-    if (t.scalar_type() == at::kHalf) d.dtype = GC_B200_F16;
-    if (t.scalar_type() == at::kBFloat16) d.dtype = GC_B200_BF16;
-    if (t.numel() > 0) {
-        int64_t last = 1;
-        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
-        d.bytes = static_cast<uint64_t>(last) * t.element_size();
-    }
-    return d;
-}
-
-void *stream_of(const at::Tensor &t) {
-    return t.is_cuda() ? static_cast<void *>(c10::cuda::getCurrentCUDAStream(t.get_device()).stream()) : nullptr;
-}
-
-at::Tensor workspace_of(uint64_t bytes, const at::Tensor &like) {
-    return bytes == 0 ? at::Tensor()
-                      : at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte).memory_format(
-                                                                     at::MemoryFormat::Contiguous));
-}
 
 // Dense (N, C, ..) with the channels innermost, which is what channels_last
 // means for rank 4 and what this library computes for ranks 2 and 3 too.
@@ -230,11 +163,6 @@ Drop again(Drop d) {
     return d;
 }
 
-void no_double_backward() {
-    if (at::GradMode::is_enabled())
-        throw std::runtime_error("the gradient of this operation is not differentiable (create_graph)");
-}
-
 struct NormArgs {
     int64_t groups = 1, activation = 0;
     double eps = 0.0;
@@ -265,13 +193,6 @@ at::Tensor norm_forward(const at::Tensor &x, const at::Tensor &gamma, const at::
     }
     if (st != GC_OK) fail(st);
     return y;
-}
-
-// Asked of every operand whether it requires a gradient or not: the primal of a
-// dual tensor usually does not, and its tangent would be lost.
-void no_forward_mode(const at::Tensor &t) {
-    if (t.defined() && t._fw_grad(/*level=*/0).defined())
-        throw std::runtime_error("this operation has no forward-mode derivative");
 }
 
 // The gradients are plain autograd nodes: a training step's host time counts,
@@ -324,8 +245,6 @@ struct GroupNormGrad : torch::autograd::Node {
         return {dx, dgamma, dbeta};
     }
 };
-
-bool wants_grad(const at::Tensor &t) { return t.defined() && t.requires_grad(); }
 
 at::Tensor group_norm(const at::Tensor &x, const c10::optional<at::Tensor> &gamma,
                       const c10::optional<at::Tensor> &beta, int64_t groups, double eps, int64_t activation, double p,
@@ -442,10 +361,13 @@ at::Tensor dropout(const at::Tensor &x, const c10::optional<at::Tensor> &residua
 
 }  // namespace
 
+void bind_sequence_ops(pybind11::module_ &m);  // sequence_op.cpp
+
 PYBIND11_MODULE(_gcb_torch, m) {
     m.doc() = "gc_cuda_conv for torch tensors: output allocation and the C ABI call in C++";
     m.def("conv", &conv, "y = gc_cuda_conv(x, w) on the current CUDA stream");
     m.def("conv_ex", &conv_ex, "y = act(conv(x, w) + bias) through gc_b200_conv_ex on the current CUDA stream");
     m.def("group_norm", &group_norm, "gc_b200_group_norm on the current CUDA stream, with its gradient");
     m.def("dropout", &dropout, "gc_b200_dropout on the current CUDA stream, with its gradient");
+    bind_sequence_ops(m);
 }

@@ -16,6 +16,10 @@ only, and a missing library or an unsupported geometry raises NativeError.
 Between convolutions: group_norm_act and B200GroupNormAct (GroupNorm ->
 activation -> dropout as one gc_b200_group_norm call) and dropout and
 B200Dropout (gc_b200_dropout), all with gradients through the C++ front end.
+On rows and sequences (tokens by channels): layer_norm, causal_conv and
+selective_scan with their gradients, causal_conv_step and selective_scan_step for
+one new token of every sequence, and the modules that hold their parameters,
+B200LayerNorm, B200CausalConv1d and B200SelectiveBlock.
 """
 from __future__ import annotations
 
@@ -291,6 +295,85 @@ def dropout(x: torch.Tensor, p: float, residual: torch.Tensor | None = None, sco
     return _native_call((_ops or _front_end()).dropout, x, residual, p, _scope_code(scope), seed, offset)
 
 
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """Layer normalisation of x's last axis as one gc_b200_layer_norm call.
+
+    x is float32, float16 or bfloat16; rows of a wider tensor, and the
+    permuted view (N, H, W, C) of a channels_last tensor, are read as they lie.
+    weight and bias have as many elements as a row, float32 or x's type.  The
+    result is dense.  Differentiable once."""
+    return _native_call((_ops or _front_end()).layer_norm, x, weight, bias, eps)
+
+
+def _sequence_activation(activation: str) -> int:
+    act = api.NORM_ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"activation must be one of {', '.join(api.NORM_ACTIVATIONS)}")
+    return act
+
+
+def _taps(weight: torch.Tensor) -> torch.Tensor:
+    """(C, K); a Conv1d's (C, 1, K) too."""
+    return weight.squeeze(1) if weight.dim() == 3 and weight.shape[1] == 1 else weight
+
+
+def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str = 'none',
+                state: torch.Tensor | None = None, lengths: torch.Tensor | None = None, return_state: bool = False):
+    """Causal depthwise convolution along sequences, one gc_b200_causal_conv call:
+    y[n, t, c] = act(bias[c] + sum_k weight[c, k] u[n, t + k, c]), u being the
+    K - 1 inputs of `state` (zeros without one), then x.
+
+    x is (N, L, C), weight (C, K) or a depthwise Conv1d's (C, 1, K), K <= 8.
+    lengths (N integers on x's device) ends each sequence: what lies behind is
+    not read, and y is 0 there.  With return_state the result is (y, the last
+    K - 1 inputs of each sequence), which continues them in another call or in
+    causal_conv_step.  Differentiable once, the states included."""
+    y, last = _native_call((_ops or _front_end()).causal_conv, x, _taps(weight), bias, _sequence_activation(activation),
+                           state, lengths, return_state)
+    return (y, last) if return_state else y
+
+
+def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor, bias: torch.Tensor | None = None,
+                     activation: str = 'none', state_out: torch.Tensor | None = None) -> torch.Tensor:
+    """causal_conv for one token of every sequence: x and the result are (N, C).
+    state (N, K - 1, C) is updated in place, or the new one written to
+    state_out.  Has no gradient."""
+    return _native_call((_ops or _front_end()).causal_conv_step, x, _taps(weight), state, bias,
+                        _sequence_activation(activation), state_out)
+
+
+def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                   D: torch.Tensor | None = None, z: torch.Tensor | None = None, dt_bias: torch.Tensor | None = None,
+                   softplus: bool = True, state: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                   return_state: bool = False):
+    """Selective state space scan, one gc_b200_selective_scan call:
+    delta = softplus(dt + dt_bias) (or the sum itself),
+    h[t] = exp(delta[t] A) h[t - 1] + delta[t] x[t] B[t],
+    y[t] = (C[t] . h[t] + D x[t]) silu(z[t]).
+
+    x, dt and z are (N, L, channels), B and C (N, L, S) or (N, L, groups, S) of
+    the same type (float32, float16, bfloat16), A (channels, S), S <= 64; A, D
+    and dt_bias float32 or x's type.  state, if given, is float32 (N, channels,
+    S); without one h starts at 0.  lengths as in causal_conv.  With return_state
+    the result is (y, last states).  States and sums are held in 32 bits.
+    Differentiable once, the states included."""
+    y, last = _native_call((_ops or _front_end()).selective_scan, x, dt, A, B, C, D, z, dt_bias, softplus, state, lengths,
+                           return_state)
+    return (y, last) if return_state else y
+
+
+def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                        state: torch.Tensor, D: torch.Tensor | None = None, z: torch.Tensor | None = None,
+                        dt_bias: torch.Tensor | None = None, softplus: bool = True,
+                        state_out: torch.Tensor | None = None) -> torch.Tensor:
+    """selective_scan for one token of every sequence: x, dt, z and the result
+    are (N, channels), B and C (N, S) or (N, groups, S).  state is updated in
+    place, or the new one written to state_out.  Has no gradient."""
+    return _native_call((_ops or _front_end()).selective_scan_step, x, dt, A, B, C, state, D, z, dt_bias, softplus,
+                        state_out)
+
+
 def _norm_activation_name(act: torch.nn.Module | None) -> str:
     return 'silu' if isinstance(act, torch.nn.SiLU) else _activation_name(act)
 
@@ -395,6 +478,134 @@ def fuse_norm_act(module: torch.nn.Module) -> list[str]:
                 child._modules[follower] = nn.Identity()
             replaced.append(f'{name}.{attr}' if name else attr)
     return replaced
+
+
+class B200LayerNorm(torch.nn.Module):
+    """Replacement of a torch.nn.LayerNorm over one axis, the last; keeps its
+    parameters and their names."""
+
+    def __init__(self, norm: torch.nn.LayerNorm):
+        super().__init__()
+        if len(norm.normalized_shape) != 1:
+            raise ValueError('layer norm over more than one axis has no entry point')
+        self.normalized_shape, self.eps = tuple(norm.normalized_shape), norm.eps
+        self.weight, self.bias = norm.weight, norm.bias
+        self.training = norm.training
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1:] != self.normalized_shape:
+            raise ValueError(f'last axis must have {self.normalized_shape[0]} elements')
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+    def extra_repr(self) -> str:
+        return f'{self.normalized_shape}, eps={self.eps}'
+
+
+def substitute_layer_norm(module: torch.nn.Module) -> list[str]:
+    """Replace every LayerNorm over one axis by a B200LayerNorm; returns the
+    dotted names replaced.  Subclasses and modules with hooks stay as they are.
+    The replacement's result is of x's type, under autocast too, where torch's
+    layer_norm returns float32."""
+    replaced = []
+    for name, child in list(module.named_modules()):
+        for attr, sub in list(child._modules.items()):
+            if _plain(sub, (torch.nn.LayerNorm,)) and len(sub.normalized_shape) == 1:
+                child._modules[attr] = B200LayerNorm(sub)
+                replaced.append(f'{name}.{attr}' if name else attr)
+    return replaced
+
+
+class B200CausalConv1d(torch.nn.Module):
+    """A depthwise torch.nn.Conv1d of stride 1 as a causal convolution on (N, L,
+    C), with an activation.  Keeps the convolution's parameters and their names;
+    its padding must be 0 or kernel - 1 (the usual way to make it causal)."""
+
+    def __init__(self, conv: torch.nn.Conv1d, act: torch.nn.Module | None = None):
+        super().__init__()
+        taps = conv.kernel_size[0]
+        if not (conv.groups == conv.in_channels == conv.out_channels and conv.stride == (1,) and conv.dilation == (1,)
+                and conv.padding in ((0,), (taps - 1,)) and conv.padding_mode == 'zeros' and taps <= 8):
+            raise ValueError('a depthwise convolution of stride 1 and at most eight taps is required')
+        self.weight, self.bias = conv.weight, conv.bias
+        self.activation = _norm_activation_name(act)
+        self.training = conv.training
+
+    def forward(self, x: torch.Tensor, state: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                return_state: bool = False):
+        return causal_conv(x, self.weight, self.bias, self.activation, state, lengths, return_state)
+
+    def step(self, x: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
+        return causal_conv_step(x, self.weight, state, self.bias, self.activation)
+
+    def new_state(self, n: int) -> torch.Tensor:
+        return self.weight.new_zeros((n, self.weight.shape[-1] - 1, self.weight.shape[0]))
+
+    def extra_repr(self) -> str:
+        return f'{self.weight.shape[0]}, taps={self.weight.shape[-1]}, activation={self.activation}'
+
+
+class B200SelectiveBlock(torch.nn.Module):
+    """A residual block that mixes along sequences:
+    x + out(scan(conv(in(norm(x))), gate)): layer norm, a projection to a branch
+    and its gate, the causal convolution with SiLU, the projections to the scan's
+    step sizes, B and C, the selective scan with its gate, a projection back.
+
+    forward(x) on (N, L, width) serves training; prefill(x, lengths) runs prompts
+    and returns (result, states); step(x, states) takes one token (N, width) of
+    every sequence and updates the states in place."""
+
+    def __init__(self, width: int, channels: int | None = None, states: int = 16, taps: int = 4, rank: int | None = None,
+                 eps: float = 1e-5, device=None, dtype=None):
+        super().__init__()
+        channels = 2 * width if channels is None else channels
+        rank = -(-width // 16) if rank is None else rank
+        nn, kw = torch.nn, {'device': device, 'dtype': dtype}
+        self.states, self.rank = states, rank
+        self.norm = B200LayerNorm(nn.LayerNorm(width, eps, **kw))
+        self.input = nn.Linear(width, 2 * channels, bias=False, **kw)
+        self.conv = B200CausalConv1d(nn.Conv1d(channels, channels, taps, groups=channels, padding=taps - 1, **kw), nn.SiLU())
+        self.select = nn.Linear(channels, rank + 2 * states, bias=False, **kw)
+        self.dt = nn.Linear(rank, channels, bias=False, **kw)
+        self.output = nn.Linear(channels, width, bias=False, **kw)
+        # the scan's own parameters stay in 32 bits: decays close to 1 do not survive 8 bits of mantissa
+        first = torch.exp(torch.rand(channels, device=device) * 4.6051702 - 6.9077553)  # step sizes of 1e-3 to 1e-1
+        self.dt_bias = nn.Parameter(first + torch.log(-torch.expm1(-first)))
+        self.A_log = nn.Parameter(torch.log(torch.arange(1, states + 1, device=device).float()).repeat(channels, 1))
+        self.D = nn.Parameter(torch.ones(channels, device=device))
+
+    def _scan_inputs(self, u: torch.Tensor):
+        dt, B, C = self.select(u).split((self.rank, self.states, self.states), -1)
+        return self.dt(dt), -torch.exp(self.A_log), B, C
+
+    def _mix(self, x: torch.Tensor, lengths: torch.Tensor | None, states):
+        u, gate = self.input(self.norm(x)).chunk(2, -1)
+        keep = states is not None
+        before, h = states if keep and states else (None, None)
+        u = self.conv(u, before, lengths, keep)
+        u, before = u if keep else (u, None)
+        y = selective_scan(u, *self._scan_inputs(u), D=self.D, z=gate, dt_bias=self.dt_bias, state=h, lengths=lengths,
+                           return_state=keep)
+        y, h = y if keep else (y, None)
+        return x + self.output(y), (before, h)
+
+    def forward(self, x: torch.Tensor, lengths: torch.Tensor | None = None) -> torch.Tensor:
+        return self._mix(x, lengths, None)[0]
+
+    def prefill(self, x: torch.Tensor, lengths: torch.Tensor | None = None, states=()):
+        """(result, states); states of an earlier call continue its sequences."""
+        return self._mix(x, lengths, states)
+
+    def step(self, x: torch.Tensor, states) -> torch.Tensor:
+        before, h = states
+        u, gate = self.input(self.norm(x)).chunk(2, -1)
+        u = self.conv.step(u, before)
+        dt, A, B, C = self._scan_inputs(u)
+        y = selective_scan_step(u, dt, A, B, C, h, D=self.D, z=gate, dt_bias=self.dt_bias)
+        return x + self.output(y)
+
+    def new_states(self, n: int):
+        """States of n sequences that have not begun."""
+        return self.conv.new_state(n), self.D.new_zeros((n, self.D.shape[0], self.states), dtype=torch.float32)
 
 
 def substitute(module: torch.nn.Module, predicate, native: api.Native | None = None) -> list[str]:

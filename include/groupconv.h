@@ -258,6 +258,117 @@ int gc_b200_group_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
 int gc_b200_dropout(const gc_tensor *x, const gc_tensor *residual, gc_tensor *y,
                     const gc_b200_dropout_args *dropout, void *stream);
 
+/* ---- rows and sequences ----------------------------------------------------
+ * What stands between the convolutions of networks that mix along sequences or
+ * normalise each pixel: layer normalisation, a causal depthwise convolution and
+ * the selective state space scan it feeds, each with its gradient, the last two
+ * with a form for one new token of every sequence.
+ *
+ * Element types as above.  Data tensors of one call have one type; parameters
+ * are dense, F32 or of the data's type.  The last axis of a data tensor is dense;
+ * its other strides are free as long as no two elements share memory (for layer
+ * norm the rows are evenly spaced), else GC_UNSUPPORTED.  Axes of 0 are valid.
+ * Sums, statistics and states are held in 32 bits or more; a result is rounded
+ * once.  Outputs and workspaces overlap neither inputs nor one another.
+ * Workspaces are 16-byte aligned device memory whose contents need not be set and
+ * are undefined afterwards; calls that may run at the same time have their own.
+ * Validation, device, stream, allocation and capture rules are those of
+ * gc_cuda_conv.  Results are bitwise reproducible. */
+
+/* Layer normalisation of the last axis of x (rank 1 to 4, C elements a row):
+ *   y = (x - mean) / sqrt(var + eps) * gamma + beta,  var biased
+ *   gamma, beta NULL, or C elements.
+ *   stats       NULL, or a dense F32 tensor of dims (rows, 2) that receives mean
+ *               and 1 / sqrt(var + eps) for the gradient. */
+int gc_b200_layer_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tensor *beta, gc_tensor *y,
+                       gc_tensor *stats, double eps, void *stream);
+
+/* Its gradient, from the stats that it stored.  dgamma, dbeta: NULL, or C
+ * elements (with no rows they are set to 0); without both no workspace is
+ * needed. */
+int gc_b200_layer_norm_backward_workspace(const gc_tensor *dy, const gc_tensor *x, const gc_tensor *dx,
+                                          uint64_t *bytes);
+int gc_b200_layer_norm_backward(const gc_tensor *dy, const gc_tensor *x, const gc_tensor *gamma,
+                                const gc_tensor *stats, gc_tensor *dx, gc_tensor *dgamma, gc_tensor *dbeta,
+                                void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* Causal depthwise convolution along the tokens of sequences, with an activation:
+ *   y[n, t, c] = act(bias[c] + sum_k weight[c, k] u[n, t + k, c])
+ * u being the K - 1 inputs of `state`, then x.
+ *   x, y        (N, L, C), also channel slices of wider tensors.
+ *   weight      (C, K), 1 <= K <= 8;  bias NULL, or C elements.
+ *   state       NULL for zeros, or (N, K - 1, C) of x's type: the inputs before
+ *               these, the oldest first.
+ *   lengths     NULL, or N device words: sequence n ends after lengths[n] tokens
+ *               (values outside 0..L mean the nearer bound).  What lies behind is
+ *               not read, y there is 0.
+ *   state_out   NULL, or like state: the last K - 1 inputs of each sequence, for
+ *               the call that continues it.
+ *   activation  GC_B200_ACT_NONE, _RELU, _RELU6 or _SILU. */
+int gc_b200_causal_conv(const gc_tensor *x, const gc_tensor *weight, const gc_tensor *bias, const gc_tensor *state,
+                        const int32_t *lengths, gc_tensor *y, gc_tensor *state_out, int activation, void *stream);
+
+/* Its gradient.  dstate_out: NULL, or the gradient of state_out; dweight, dbias,
+ * dstate: nullable.  Without dweight and dbias no workspace is needed.  dx is 0
+ * behind a sequence's end. */
+int gc_b200_causal_conv_backward_workspace(const gc_tensor *dy, const gc_tensor *x, const gc_tensor *weight,
+                                           const gc_tensor *dx, uint64_t *bytes);
+int gc_b200_causal_conv_backward(const gc_tensor *dy, const gc_tensor *x, const gc_tensor *weight, const gc_tensor *bias,
+                                 const gc_tensor *state, const gc_tensor *dstate_out, const int32_t *lengths,
+                                 gc_tensor *dx, gc_tensor *dweight, gc_tensor *dbias, gc_tensor *dstate, int activation,
+                                 void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* One token of every sequence: x, y (N, C).  state_out is the state itself
+ * (same memory and strides) or apart from it. */
+int gc_b200_causal_conv_step(const gc_tensor *x, const gc_tensor *weight, const gc_tensor *bias, const gc_tensor *state,
+                             gc_tensor *y, gc_tensor *state_out, int activation, void *stream);
+
+/* Selective state space scan.  Each channel of a sequence has a state h of S
+ * numbers:
+ *   delta = softplus(dt + dt_bias), or dt + dt_bias
+ *   h[t] = exp(delta[t] A) h[t - 1] + delta[t] x[t] B[t]
+ *   y[t] = (C[t] . h[t] + D x[t]) z[t] / (1 + exp(-z[t])), without z the first factor
+ * Channel c reads group c / (channels / G) of B and C.
+ *   x, dt, z    (N, L, C); z nullable.
+ *   b, c        (N, L, G, S), 1 <= S <= 64, G divides C.
+ *   a           (C, S);  d, dt_bias  NULL for none, or C elements.
+ *   state       NULL for zeros, or F32 (N, C, S).
+ *   lengths     as above, nullable. */
+typedef struct {
+    const gc_tensor *x, *dt, *a, *b, *c;
+    const gc_tensor *d, *z, *dt_bias, *state;
+    const int32_t *lengths;
+    int32_t softplus;
+} gc_b200_scan_args;
+
+/* Bytes that the calls below need for these tensors: the workspaces of the scan
+ * and of its gradient, and `kept`, the states that the scan stores on its way for
+ * the gradient. */
+int gc_b200_selective_scan_sizes(const gc_b200_scan_args *args, uint64_t *workspace, uint64_t *kept,
+                                 uint64_t *backward_workspace);
+
+/*   state_out   NULL, or like state: each sequence's last state.
+ *   kept        NULL, or 16-byte aligned device memory for the gradient. */
+int gc_b200_selective_scan(const gc_b200_scan_args *args, gc_tensor *y, gc_tensor *state_out, void *kept,
+                           uint64_t kept_bytes, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* Its gradient, from the same arguments and what the scan kept.  x and dt are
+ * required, z where the scan had one, the others are nullable; each has the
+ * dims of what it is the gradient of, b and c of x's type, a, d and dt_bias F32
+ * or x's type, state F32.  dstate_out: NULL, or the gradient of state_out.
+ * Behind a sequence's end the gradients are 0. */
+typedef struct {
+    gc_tensor *x, *dt, *a, *b, *c;
+    gc_tensor *d, *z, *dt_bias, *state;
+} gc_b200_scan_grads;
+int gc_b200_selective_scan_backward(const gc_b200_scan_args *args, const gc_tensor *dy, const gc_tensor *dstate_out,
+                                    const void *kept, uint64_t kept_bytes, const gc_b200_scan_grads *grads,
+                                    void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* One token of every sequence: x, dt, z, y (N, C), b, c (N, G, S), no lengths.
+ * state_out is the state itself (same memory and strides) or apart from it. */
+int gc_b200_selective_scan_step(const gc_b200_scan_args *args, gc_tensor *y, gc_tensor *state_out, void *stream);
+
 /* Benchmark mode (the counterpart of a framework's "benchmark" convolution
  * search): for a shape that implementation 3 serves with a direct engine,
  * time the planner's `candidates` best-scored tilings (1..64) on these
@@ -272,8 +383,8 @@ int gc_b200_autotune(const gc_shape *p, const gc_tensor *x, const gc_tensor *w,
                      gc_tensor *y, int candidates, void *stream);
 
 /* Launch plan chosen by the last successful gc_cuda_conv, gc_b200_conv,
- * gc_b200_group_norm, its gradient or gc_b200_dropout call on the calling
- * thread: kernel family name, grid, block, shared memory and work split, as
+ * gc_b200_group_norm, its gradient, gc_b200_dropout or a call on rows and
+ * sequences on the calling thread: kernel family name, grid, block, shared memory and work split, as
  * one line of text.  Empty before the first launch. */
 const char *gc_b200_last_plan(void);
 
