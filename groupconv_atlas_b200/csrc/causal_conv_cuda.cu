@@ -146,7 +146,7 @@ struct GradPlan {
 GradPlan plan_grad(const ConvCall &call, bool vec, int sms) {
     GradPlan p;
     p.vec = vec;
-    const long long vcols = call.c / (vec ? 4 : 1);
+    const long long vcols = ceil_div(call.c, vec ? 4 : 1);
     p.tiles = ceil_div(vcols, 32);
     p.cols = static_cast<int>(ceil_div(vcols, p.tiles));
     p.workers = kConvThreads / p.cols;

@@ -136,6 +136,19 @@ int kernel_occupancy(int dev, const void *fn, int threads, size_t smem, int smem
     return GC_OK;
 }
 
+int opt_in_smem(int dev, const void *fn, int bytes) {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    bool &done = g_attr_done[std::make_pair(dev, fn)];
+    if (done) return GC_OK;
+    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return gc_error(GC_DEVICE_ERROR, cudaGetErrorString(e));
+    }
+    done = true;
+    return GC_OK;
+}
+
 cudaError_t launch_pdl(const void *fn, dim3 grid, dim3 block, void **args, size_t smem, cudaStream_t stream,
                        int cluster) {
     cudaLaunchConfig_t cfg = {};

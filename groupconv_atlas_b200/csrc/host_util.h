@@ -48,6 +48,10 @@ int device_facts(int dev, DeviceFacts &out);  // cached per device
 // the occupancy calculator (cached) how many CTAs fit per SM.
 int kernel_occupancy(int dev, const void *fn, int threads, size_t smem, int smem_optin, int &ctas);
 
+// Opt a kernel into `bytes` of dynamic shared memory, once per device (a kernel
+// always asks for the same).
+int opt_in_smem(int dev, const void *fn, int bytes);
+
 // Launch on the caller's stream with programmatic stream serialization: the
 // kernel may start its prologue while the previous kernel in the stream
 // drains, and waits (griddepcontrol.wait) before touching global memory.

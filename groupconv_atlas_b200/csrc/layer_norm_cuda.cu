@@ -215,9 +215,8 @@ int gc_b200_layer_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
     set_param(beta, P.beta, P.beta_type);
     P.stats = stats != nullptr ? static_cast<float2 *>(stats->data) : nullptr;
     const void *fn = row_kernel(plan, false);
-    int ctas = 1;
-    if ((st = kernel_occupancy(dev, fn, plan.threads, 0, dynamic_limit(facts), ctas)) != GC_OK) return st;
-    const long long grid = std::min(ceil_div(P.rows, plan.threads / plan.team), static_cast<long long>(ctas) * facts.sms);
+    // as many blocks as a multiprocessor has threads for; each takes rows in turn
+    const long long grid = std::min(ceil_div(P.rows, plan.threads / plan.team), 2048LL / plan.threads * facts.sms);
     void *args[] = {&P};
     const cudaError_t e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(plan.threads), args, 0,
                                      reinterpret_cast<cudaStream_t>(stream));
@@ -299,8 +298,7 @@ int gc_b200_layer_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
     P.stats = static_cast<float2 *>(stats->data);
     P.part = sums ? static_cast<float *>(workspace) : nullptr;
     const void *fn = row_kernel(plan, true);
-    int ctas = 1;
-    if ((st = kernel_occupancy(dev, fn, plan.threads, plan.smem, dynamic_limit(facts), ctas)) != GC_OK) return st;
+    if (plan.smem > 48 * 1024 && (st = opt_in_smem(dev, fn, dynamic_limit(facts))) != GC_OK) return st;
     void *args[] = {&P};
     e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(plan.threads), args, plan.smem, s);
     if (e == cudaSuccess && sums) {
