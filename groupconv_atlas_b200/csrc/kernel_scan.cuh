@@ -12,14 +12,18 @@
 //
 // What bounds these kernels is the exponential of every (token, channel, state):
 // the special-function unit does 16 a clock and multiprocessor.  A channel's
-// states are spread over P lanes of R each; a block takes THREADS / P channels
-// and walks along the tokens in tiles that are staged in shared memory, where
-// softplus, gate and products of a token and channel are formed once for its P
-// lanes.  Where sequences and channels alone are too few to fill the GPU, each
+// states are spread over P lanes of R = 4 each, held as pairs of floats; a block
+// takes THREADS / P channels and walks along the tokens in tiles of 16.  A tile's
+// inputs are copied to shared memory while the tile before is worked on; softplus,
+// gate and products of a token and channel are then formed once for its P lanes.
+// Where sequences and channels alone are too few to fill the GPU, each
 // sequence is cut into segments: a first launch gives each segment's effect on
 // the state (what it adds, and the sum of its deltas, whose product with A is its
 // decay's logarithm), from which every block forms the state that it starts with.
 #pragma once
+#include <cstring>
+#include <type_traits>
+
 #include "norm_util.cuh"
 
 namespace gcb {
@@ -44,7 +48,7 @@ struct ScanParams {
     const int *lengths;                // nullable
     long long n, l;
     int channels, states, groups, cpg; // cpg: channels of a group
-    int type, vec, softplus;           // vec: four channels in one access
+    int vec, bvec, softplus;           // vec, bvec: four channels, four states of B and C in one access
     int tiles;                         // blocks that share a group's channels
     long long seg_len;
     int segs;
@@ -54,128 +58,150 @@ struct ScanParams {
     float *part_a, *part_d;            // [n * segs][channels][states], [n * segs][2][channels] (D, dt_bias)
 };
 
-// ---- four channels of a token -----------------------------------------------------------
+// ---- four elements ---------------------------------------------------------------------------
+template <class T>
 struct Four {
-    uint4 u;
+    typename std::conditional<sizeof(T) == 4, uint4, uint2>::type u;
 };
-__device__ __forceinline__ Four load_four(const void *p, int type, bool vec, long long at, int valid) {
-    Four r;
-    r.u = make_uint4(0u, 0u, 0u, 0u);
-    if (valid <= 0) return r;
-    if (type == kElemF32) {
-        const float *q = static_cast<const float *>(p) + at;
-        if (vec) {
-            r.u = __ldg(reinterpret_cast<const uint4 *>(q));
-        } else {
-            r.u.x = __float_as_uint(q[0]);
-            if (valid > 1) r.u.y = __float_as_uint(q[1]);
-            if (valid > 2) r.u.z = __float_as_uint(q[2]);
-            if (valid > 3) r.u.w = __float_as_uint(q[3]);
-        }
+// `valid` elements from p; in one access where `vec` (valid is then 4 or none).
+template <class T>
+__device__ __forceinline__ Four<T> load_four(const T *p, bool vec, int valid) {
+    Four<T> r;
+    if (vec && valid > 0) {
+        r.u = *reinterpret_cast<const decltype(r.u) *>(p);
     } else {
-        const unsigned short *q = static_cast<const unsigned short *>(p) + at;
-        if (vec) {
-            const uint2 t = __ldg(reinterpret_cast<const uint2 *>(q));
-            r.u.x = t.x;
-            r.u.y = t.y;
-        } else {
-            r.u.x = q[0];
-            if (valid > 1) r.u.x |= static_cast<uint32_t>(q[1]) << 16;
-            if (valid > 2) r.u.y = q[2];
-            if (valid > 3) r.u.y |= static_cast<uint32_t>(q[3]) << 16;
-        }
+        T e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = i < valid ? p[i] : from_float<T>(0.0f);
+        memcpy(&r.u, e, sizeof(r.u));
     }
     return r;
 }
-__device__ __forceinline__ void floats_of(const Four &r, int type, float (&v)[4]) {
-    if (type == kElemF32) {
-        unpack(r.u, v, static_cast<const float *>(nullptr));
+template <class T>
+__device__ __forceinline__ void floats_of(const Four<T> &r, f2 (&v)[2]) {
+    if constexpr (sizeof(T) == 4) {
+        v[0] = pair(__uint_as_float(r.u.x), __uint_as_float(r.u.y));
+        v[1] = pair(__uint_as_float(r.u.z), __uint_as_float(r.u.w));
     } else {
         float w[8];
-        if (type == kElemBF16) unpack(r.u, w, static_cast<const __nv_bfloat16 *>(nullptr));
-        else unpack(r.u, w, static_cast<const __half *>(nullptr));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = w[i];
+        unpack(make_uint4(r.u.x, r.u.y, 0u, 0u), w, static_cast<const T *>(nullptr));
+        v[0] = pair(w[0], w[1]);
+        v[1] = pair(w[2], w[3]);
     }
 }
-__device__ __forceinline__ void store_four(const void *p, int type, bool vec, long long at, int valid, const float (&v)[4]) {
-    if (valid <= 0) return;
-    void *out = const_cast<void *>(p);
-    if (!vec) {
+template <class T>
+__device__ __forceinline__ void store_zeros(T *p, bool vec, int valid) {
+    if (vec && valid > 0) {
+        Four<T> r;
+        memset(&r.u, 0, sizeof(r.u));
+        *reinterpret_cast<decltype(r.u) *>(p) = r.u;
+    } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (i < valid) store_param(out, type, at + i, v[i]);
-    } else if (type == kElemF32) {
-        float *q = static_cast<float *>(out) + at;
-        __stcs(reinterpret_cast<uint4 *>(q), pack(v, q));
-    } else {
-        const float w[8] = {v[0], v[1], v[2], v[3], 0.0f, 0.0f, 0.0f, 0.0f};
-        const uint4 u = type == kElemBF16 ? pack(w, static_cast<const __nv_bfloat16 *>(nullptr))
-                                          : pack(w, static_cast<const __half *>(nullptr));
-        __stcs(reinterpret_cast<uint2 *>(static_cast<unsigned short *>(out) + at), make_uint2(u.x, u.y));
+            if (i < valid) p[i] = from_float<T>(0.0f);
     }
 }
+// Four elements to a thread's own place in shared memory.
+template <class T>
+__device__ __forceinline__ void copy_four(const void *dst, const T *p) {
+    if constexpr (sizeof(T) == 4)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(p) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_addr(dst)), "l"(p) : "memory");
+}
 
-// ---- scalars ------------------------------------------------------------------------------
+// ---- functions of a token and channel -----------------------------------------------------
 __device__ __forceinline__ float exp2_fast(float v) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
+}
+__device__ __forceinline__ f2 exp2_fast(f2 v) {
+    float a, b;
+    split(v, a, b);
+    return pair(exp2_fast(a), exp2_fast(b));
 }
 __device__ __forceinline__ float rcp_fast(float v) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
+__device__ __forceinline__ float sum_of(f2 v) {
+    float a, b;
+    split(v, a, b);
+    return a + b;
+}
 constexpr float kLog2E = 1.4426950408889634f;
 
-// softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|), and its slope, the sigmoid.
-// log(1 + e) = 2 artanh(e / (2 + e)) by the series of the inverse hyperbolic
-// tangent, whose argument is at most 1/3: the first term left out is below 2e-8
-// of the sum.  Step sizes far below 1 come from small e, where a logarithm of the
-// rounded 1 + e would lose what matters.
-__device__ __forceinline__ void softplus(float v, float &value, float &slope) {
-    const float e = exp2_fast(-fabsf(v) * kLog2E);
-    const float u = e * rcp_fast(2.0f + e), w = u * u;
-    float s = fmaf(w, 1.0f / 13.0f, 1.0f / 11.0f);
-    s = fmaf(w, s, 1.0f / 9.0f);
-    s = fmaf(w, s, 1.0f / 7.0f);
-    s = fmaf(w, s, 1.0f / 5.0f);
-    s = fmaf(w, s, 1.0f / 3.0f);
-    s = fmaf(w, s, 1.0f);
-    value = fmaxf(v, 0.0f) + 2.0f * u * s;
-    const float r = rcp_fast(1.0f + e);
-    slope = v >= 0.0f ? r : e * r;
-}
-__device__ __forceinline__ float scan_delta(const ScanParams &P, float raw, float &slope) {
-    if (!P.softplus) {
-        slope = 1.0f;
-        return raw;
+// softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|), and (SLOPE) its slope, the
+// sigmoid.  log(1 + e) = 2 artanh(e / (2 + e)) by the series of the inverse
+// hyperbolic tangent, whose argument is at most 1/3: the first term left out is
+// below 2e-8 of the sum.  Step sizes far below 1 come from small e, where a
+// logarithm of the rounded 1 + e would lose what matters.  Two denominators share
+// a reciprocal; they are between 1 and 3.
+template <bool SLOPE>
+__device__ __forceinline__ void softplus2(f2 v, f2 &value, f2 &slope) {
+    float v0, v1, p0, p1;
+    split(v, v0, v1);
+    const f2 e = exp2_fast(pair(fabsf(v0), fabsf(v1)) * pair(-kLog2E));
+    split(e + pair(2.0f), p0, p1);
+    const f2 u = e * (pair(p1, p0) * pair(rcp_fast(p0 * p1))), w = u * u;
+    f2 s = fma2(w, pair(1.0f / 13.0f), pair(1.0f / 11.0f));
+    s = fma2(w, s, pair(1.0f / 9.0f));
+    s = fma2(w, s, pair(1.0f / 7.0f));
+    s = fma2(w, s, pair(1.0f / 5.0f));
+    s = fma2(w, s, pair(1.0f / 3.0f));
+    s = fma2(w, s, pair(1.0f));
+    value = fma2(u + u, s, pair(fmaxf(v0, 0.0f), fmaxf(v1, 0.0f)));
+    if constexpr (SLOPE) {
+        float e0, e1;
+        split(e, e0, e1);
+        split(e + pair(1.0f), p0, p1);
+        const f2 r = pair(p1, p0) * pair(rcp_fast(p0 * p1));  // 1 / (1 + e)
+        slope = pair(v0 >= 0.0f ? 1.0f : e0, v1 >= 0.0f ? 1.0f : e1) * r;
     }
-    float v;
-    softplus(raw, v, slope);
-    return v;
 }
-// z / (1 + exp(-z)) and its slope for four values.
-__device__ __forceinline__ void gates(const float (&z)[4], float (&gate)[4], float (&slope)[4]) {
+// delta of four channels, and its slope against dt.
+template <bool SLOPE>
+__device__ __forceinline__ void scan_deltas(bool softplus, const f2 (&raw)[2], const f2 (&bias)[2], f2 (&delta)[2],
+                                            f2 (&slope)[2]) {
 #pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-        f2 s, rest;
-        const f2 zz = pair(z[i], z[i + 1]);
-        sigmoid2(zz, s, rest);
-        split(zz * s, gate[i], gate[i + 1]);
-        split(s * fma2(zz, rest, pair(1.0f)), slope[i], slope[i + 1]);
+    for (int i = 0; i < 2; ++i) {
+        const f2 v = raw[i] + bias[i];
+        if (softplus) {
+            softplus2<SLOPE>(v, delta[i], slope[i]);
+        } else {
+            delta[i] = v;
+            slope[i] = pair(1.0f);
+        }
     }
+}
+// z / (1 + exp(-z)) and (SLOPE) its slope, of two values.
+template <bool SLOPE>
+__device__ __forceinline__ void gate2(f2 z, f2 &gate, f2 &slope) {
+    f2 s, rest;
+    sigmoid2(z, s, rest);
+    gate = z * s;
+    if constexpr (SLOPE) slope = s * fma2(z, rest, pair(1.0f));
 }
 
-// ---- a thread's place ---------------------------------------------------------------------
+// ---- shapes and places ---------------------------------------------------------------------
+template <int SP_, int THREADS_>
+struct ScanShape {
+    static constexpr int SP = SP_, THREADS = THREADS_, T = kScanChunk;
+    static constexpr int R = SP >= 4 ? 4 : 1, NP = (R + 1) / 2;  // states of a lane, as pairs
+    static constexpr int P = SP / R, CB = THREADS / P;           // lanes of a channel, channels of a block
+    static constexpr int GROUPS = CB / 4, NG = T * GROUPS > THREADS ? T * GROUPS / THREADS : 1;
+    static constexpr int QUADS = SP >= 4 ? SP / 4 : 1;           // of a token's B or C
+};
+
 // A warp's lanes: channel * P + part; a part has the states part * R ...
-template <int SP, int R, int THREADS>
+template <class S>
 struct ScanPlace {
-    static constexpr int P = SP / R, CB = THREADS / P;
-    long long n, len;
+    long long n, len, begin, stop, end;  // the segment's tokens; end: of those in the sequence
     int seg, group, tile, first, count;  // first channel of the block, its channels
-    int chan, part;                      // the thread's, from `first`
+    int chan, part, channel;             // the thread's
+    bool live;
     __device__ __forceinline__ explicit ScanPlace(const ScanParams &Q) {
         const int per = Q.groups * Q.tiles;
         long long b = blockIdx.x;
@@ -185,60 +211,173 @@ struct ScanPlace {
         n = b / Q.segs;
         group = gt / Q.tiles;
         tile = gt - group * Q.tiles;
-        first = group * Q.cpg + tile * CB;
-        count = min(CB, Q.cpg - tile * CB);
-        chan = threadIdx.x / P;
-        part = threadIdx.x % P;
+        first = group * Q.cpg + tile * S::CB;
+        count = min(S::CB, Q.cpg - tile * S::CB);
+        chan = threadIdx.x / S::P;
+        part = threadIdx.x % S::P;
+        channel = first + chan;
+        live = chan < count;
         len = Q.l;
         if (Q.lengths != nullptr) {
             const int v = Q.lengths[n];
             len = v < 0 ? 0 : min(static_cast<long long>(v), Q.l);
         }
+        begin = seg * Q.seg_len;
+        stop = min(Q.l, begin + Q.seg_len);
+        end = min(len, stop);
     }
-    __device__ __forceinline__ bool live() const { return chan < count; }
-    __device__ __forceinline__ int channel() const { return first + chan; }
 };
 
-// R states of a [..][states] tensor at `p`, zeros where there are none.
-template <int R>
-__device__ __forceinline__ void load_states(const float *p, int part, int states, bool live, float (&v)[R]) {
+// A lane's states of a [..][states] tensor, as pairs; zeros where there are none.
+// `swap` reorders them: place r holds state r ^ swap.
+template <class S>
+__device__ __forceinline__ void load_states(const float *p, int part, int states, bool live, int swap, f2 (&v)[S::NP]) {
+    float f[4] = {};
 #pragma unroll
-    for (int r = 0; r < R; ++r) v[r] = live && part * R + r < states ? p[part * R + r] : 0.0f;
-}
-template <int R>
-__device__ __forceinline__ void store_states(float *p, int part, int states, bool live, const float (&v)[R]) {
+    for (int r = 0; r < S::R; ++r) {
+        const int s = part * S::R + (r ^ swap);
+        f[r] = live && s < states ? p[s] : 0.0f;
+    }
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-        if (live && part * R + r < states) p[part * R + r] = v[r];
+    for (int i = 0; i < S::NP; ++i) v[i] = pair(f[2 * i], f[2 * i + 1]);
 }
-// A log2(e): the exponentials are powers of 2.
-template <int R>
-__device__ __forceinline__ void load_decay(const ScanParams &Q, long long channel, int part, bool live, float (&v)[R]) {
+template <class S>
+__device__ __forceinline__ void store_states(float *p, int part, int states, bool live, int swap, const f2 (&v)[S::NP]) {
+    float f[4];
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-        v[r] = live && part * R + r < Q.states ? load_param(Q.a, Q.a_type, channel * Q.states + part * R + r) * kLog2E : 0.0f;
+    for (int i = 0; i < S::NP; ++i) split(v[i], f[2 * i], f[2 * i + 1]);
+    if (S::R == 4 && swap == 0 && states % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        if (live && part * 4 < states)
+            *reinterpret_cast<float4 *>(p + part * 4) = make_float4(f[0], f[1], f[2], f[3]);
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < S::R; ++r) {
+        const int s = part * S::R + (r ^ swap);
+        if (live && s < states) p[s] = f[r];
+    }
 }
-
-// B or C of `count` tokens from t0 into sm[token][SP], zeros beyond.
-template <int SP>
-__device__ __forceinline__ void stage_states(const ScanParams &Q, const TokenView &v, long long n, long long t0, int group,
-                                             int count, int tokens, float *sm) {
-    for (int i = threadIdx.x; i < tokens * SP; i += blockDim.x) {
-        const int t = i / SP, s = i - t * SP;
-        sm[i] = t < count && s < Q.states ? load_param(v.p, Q.type, n * v.ldn + (t0 + t) * v.ldt + group * v.ldg + s) : 0.0f;
+// A log2(e): the exponentials are powers of 2.  Infinities become the largest
+// numbers, whose exponentials are the same, so that a step size of 0 leaves a
+// state as it is; tiles are filled up with such steps.
+template <class S>
+__device__ __forceinline__ void load_decay(const ScanParams &Q, const ScanPlace<S> &at, int swap, f2 (&v)[S::NP]) {
+    float f[4] = {};
+#pragma unroll
+    for (int r = 0; r < S::R; ++r) {
+        const int s = at.part * S::R + (r ^ swap);
+        if (at.live && s < Q.states) f[r] = load_param(Q.a, Q.a_type, static_cast<long long>(at.channel) * Q.states + s) * kLog2E;
+        if (f[r] > 3e38f) f[r] = 3e38f;
+        if (f[r] < -3e38f) f[r] = -3e38f;
+    }
+#pragma unroll
+    for (int i = 0; i < S::NP; ++i) v[i] = pair(f[2 * i], f[2 * i + 1]);
+}
+// A lane's states of a token from shared memory.
+template <class S>
+__device__ __forceinline__ void tile_states(const float *p, f2 (&v)[S::NP]) {
+    if constexpr (S::R == 4) {
+        const float4 f = *reinterpret_cast<const float4 *>(p);
+        v[0] = pair(f.x, f.y);
+        v[1] = pair(f.z, f.w);
+    } else {
+        v[0] = pair(*p, 0.0f);
     }
 }
 
+// The copies of a tile: fours of channels of NT tensors, and quads of the states
+// of B (PB) and C (PC).  A thread reads only what it copied itself, so that no
+// barrier is needed, and the copies take no registers while they are under way;
+// tensors that cannot be copied in groups are read directly.
+template <class T, class S, int NT, int NP>
+struct ScanRaw {
+    static constexpr int NQ = (NP * S::T * S::QUADS + S::THREADS - 1) / S::THREADS;
+    Four<T> four[NT][S::NG][S::THREADS];
+    Four<T> quad[NQ][S::THREADS];
+};
+template <class T, class S, int NT, bool PB, bool PC>
+struct ScanFetch {
+    static constexpr int NP = PB + PC, ROWS = S::THREADS / S::GROUPS;  // ROWS: tokens that the threads take at once
+    using Raw = ScanRaw<T, S, NT, NP>;
+    TokenView in[NT], b, c;
+    const ScanPlace<S> &at;
+    int gc, valid, row;   // the thread's first channel in the block, how many of its four there are, its first token
+    int states;
+    bool vec, bvec;
+    __device__ __forceinline__ ScanFetch(const ScanParams &Q, const ScanPlace<S> &place) : b(Q.b), c(Q.c), at(place) {
+        gc = (threadIdx.x % S::GROUPS) * 4;
+        valid = at.count - gc;
+        row = threadIdx.x / S::GROUPS;
+        states = Q.states;
+        vec = Q.vec;
+        bvec = Q.bvec;
+    }
+    __device__ __forceinline__ const T *four_at(int k, int g, long long t0) const {
+        return static_cast<const T *>(in[k].p) + at.n * in[k].ldn + (t0 + row + g * ROWS) * in[k].ldt + at.first + gc;
+    }
+    __device__ __forceinline__ static bool is_b(int id) { return PB && (!PC || id < S::T * S::QUADS); }
+    __device__ __forceinline__ const T *quad_at(int id, long long t0, int t, int s) const {
+        return is_b(id) ? static_cast<const T *>(b.p) + at.n * b.ldn + (t0 + t) * b.ldt + at.group * b.ldg + s
+                        : static_cast<const T *>(c.p) + at.n * c.ldn + (t0 + t) * c.ldt + at.group * c.ldg + s;
+    }
+    __device__ __forceinline__ void start(Raw &raw, long long t0, int tokens) const {
+        if (vec && valid > 0) {
+#pragma unroll
+            for (int g = 0; g < S::NG; ++g)
+                if (row + g * ROWS < tokens) {
+#pragma unroll
+                    for (int k = 0; k < NT; ++k)
+                        if (in[k].p != nullptr) copy_four<T>(&raw.four[k][g][threadIdx.x], four_at(k, g, t0));
+                }
+        }
+        if (bvec) {
+#pragma unroll
+            for (int i = 0; i < Raw::NQ; ++i) {
+                const int id = threadIdx.x + i * S::THREADS, t = id / S::QUADS % S::T, s = id % S::QUADS * 4;
+                if (id < NP * S::T * S::QUADS && t < tokens && s < states)
+                    copy_four<T>(&raw.quad[i][threadIdx.x], quad_at(id, t0, t, s));
+            }
+        }
+        cp_async_commit();
+    }
+    // four channels of tensor k at the thread's g-th token, which is one of the tile's
+    __device__ __forceinline__ void four(const Raw &raw, int k, int g, long long t0, f2 (&v)[2]) const {
+        Four<T> f;
+        if (vec && valid > 0) f = raw.four[k][g][threadIdx.x];
+        else f = load_four<T>(four_at(k, g, t0), false, valid);
+        floats_of<T>(f, v);
+    }
+    // put(is B, token, first state, four states) for every quad of the tile; zeros where there are none
+    template <class F>
+    __device__ __forceinline__ void quads(const Raw &raw, long long t0, int tokens, F put) const {
+#pragma unroll
+        for (int i = 0; i < Raw::NQ; ++i) {
+            const int id = threadIdx.x + i * S::THREADS, t = id / S::QUADS % S::T, s = id % S::QUADS * 4;
+            if (id >= NP * S::T * S::QUADS) continue;
+            f2 v[2] = {pair(0.0f), pair(0.0f)};
+            if (t < tokens && s < states) {
+                Four<T> f;
+                if (bvec) f = raw.quad[i][threadIdx.x];
+                else f = load_four<T>(quad_at(id, t0, t, s), false, states - s);
+                floats_of<T>(f, v);
+            }
+            float4 w;
+            split(v[0], w.x, w.y);
+            split(v[1], w.z, w.w);
+            put(is_b(id), t, s, w);
+        }
+    }
+};
+
 // Sums of four values over the P lanes of a channel.  The lanes share the work:
-// afterwards lane p of a channel has the sums first .. first + N - 1 in v.
+// afterwards lane p < 4 of a channel has the sums first .. first + N - 1 in v.
 template <int P>
 struct FourSums {
     static constexpr int N = P == 1 ? 4 : P == 2 ? 2 : 1;
-    int first = 0;
-    __device__ __forceinline__ void operator()(float (&v)[4], int part) {
+    __device__ __forceinline__ static int first(int part) { return P == 1 ? 0 : P == 2 ? 2 * part : 2 * (part & 1) + (part >> 1 & 1); }
+    __device__ __forceinline__ static void sum(float (&v)[4], int part) {
         if constexpr (P >= 2) {
             const bool up = part & 1;
-            first = up ? 2 : 0;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const float send = up ? v[i] : v[i + 2], keep = up ? v[i + 2] : v[i];
@@ -247,7 +386,6 @@ struct FourSums {
         }
         if constexpr (P >= 4) {
             const bool up = part & 2;
-            first += up ? 1 : 0;
             const float send = up ? v[0] : v[1], keep = up ? v[1] : v[0];
             v[0] = keep + __shfl_xor_sync(0xffffffffu, send, 2);
         }
@@ -256,413 +394,486 @@ struct FourSums {
     }
 };
 
+template <class T>
+__device__ __forceinline__ T *token_at(const TokenView &v, long long n, long long t) {
+    return static_cast<T *>(const_cast<void *>(v.p)) + n * v.ldn + t * v.ldt;
+}
+
 enum ScanMode { kScanMain, kScanCarry, kScanCarryBack };
+
+// ---- forward ------------------------------------------------------------------------------
+template <class T, class S, int MODE>
+struct ScanTile {
+    static constexpr bool kMain = MODE == kScanMain, kB = MODE != kScanCarryBack, kC = MODE != kScanCarry;
+    using Fetch = ScanFetch<T, S, MODE == kScanCarry ? 2 : 3, kB, kC>;
+    typename Fetch::Raw raw;
+    float2 du[2][S::T][S::CB];                              // delta, delta x (backwards f)
+    float2 ep[kMain ? 2 : 1][kMain ? S::T : 1][S::CB];      // D x, gate
+    float bc[2][kMain ? 2 : 1][S::T][S::SP];
+};
 
 // kScanMain       y and the last state, the states for the gradient where wanted
 // kScanCarry      a segment's effect on the state: what it adds, sum of deltas
 // kScanCarryBack  a segment's effect on the gradient of the state behind it
-template <int SP, int R, int TT, int THREADS, int MODE>
-__global__ void __launch_bounds__(THREADS) scan_kernel(const __grid_constant__ ScanParams Q) {
-    using Place = ScanPlace<SP, R, THREADS>;
-    constexpr int P = Place::P, CB = Place::CB, GROUPS = CB / 4;
-    constexpr int NG = (TT * GROUPS + THREADS - 1) / THREADS;  // groups of four channels of a thread and tile
-    __shared__ float2 du[TT][CB];
-    __shared__ __align__(16) float bs[TT][SP], cs[MODE == kScanMain ? TT : 1][SP];
+// Two buffers and one barrier a tile: a tile's values are formed after the one
+// before has been worked on, from copies that were under way meanwhile.  Tiles are
+// filled up with steps of size 0.
+template <class E, class S, int MODE>
+__global__ void __launch_bounds__(S::THREADS) scan_kernel(const __grid_constant__ ScanParams Q) {
+    constexpr int P = S::P, R = S::R, NP = S::NP, T = S::T, N = FourSums<P>::N;
+    using Tile = ScanTile<E, S, MODE>;
+    extern __shared__ __align__(16) char space[];
+    Tile &sm = *reinterpret_cast<Tile *>(space);
     griddep_wait();
     griddep_launch_dependents();
-    const Place at(Q);
+    const ScanPlace<S> at(Q);
     // the effect of the last segment, backwards the first, reaches no other one
     if (MODE != kScanMain && at.seg == (MODE == kScanCarry ? Q.segs - 1 : 0)) return;
-    const long long begin = at.seg * Q.seg_len, stop = min(Q.l, begin + Q.seg_len), end = min(at.len, stop);
-    const int channel = at.channel();
-    const bool live = at.live();
-    float a2[R], h[R];
-    load_decay<R>(Q, channel, at.part, live, a2);
+    typename Tile::Fetch fetch(Q, at);
+    fetch.in[0] = Q.dt;
+    if constexpr (MODE == kScanCarryBack) fetch.in[1] = Q.dy;
+    else fetch.in[1] = Q.x;
+    if constexpr (MODE != kScanCarry) fetch.in[2] = Q.z;
+    const int gc = fetch.gc, valid = fetch.valid;
+    long long t0 = at.begin;
+    int left = static_cast<int>(max(0LL, at.end - t0));  // tokens from the tile on
+    fetch.start(sm.raw, t0, left);
+
+    f2 a2[NP], h[NP];
+    load_decay<S>(Q, at, 0, a2);
 #pragma unroll
-    for (int r = 0; r < R; ++r) h[r] = 0.0f;
+    for (int i = 0; i < NP; ++i) h[i] = pair(0.0f);
     if (MODE == kScanMain) {
-        if (Q.state != nullptr && live)
-            load_states<R>(Q.state + at.n * Q.s_ldn + channel * Q.s_ldc, at.part, Q.states, live, h);
+        if (Q.state != nullptr) load_states<S>(Q.state + at.n * Q.s_ldn + at.channel * Q.s_ldc, at.part, Q.states, at.live, 0, h);
         for (int j = 0; j < at.seg; ++j) {
-            const long long row = (at.n * Q.segs + j) * Q.channels + channel;
-            float e[R];
-            load_states<R>(Q.carry + row * Q.states, at.part, Q.states, live, e);
-            const float sum = live ? Q.sums[row] : 0.0f;
+            const long long row = (at.n * Q.segs + j) * Q.channels + at.channel;
+            f2 e[NP];
+            load_states<S>(Q.carry + row * Q.states, at.part, Q.states, at.live, 0, e);
+            const f2 sum = pair(at.live ? Q.sums[row] : 0.0f);
 #pragma unroll
-            for (int r = 0; r < R; ++r) h[r] = fmaf(exp2_fast(sum * a2[r]), h[r], e[r]);
+            for (int i = 0; i < NP; ++i) h[i] = fma2(exp2_fast(sum * a2[i]), h[i], e[i]);
         }
     }
-    // the thread's groups of four channels: the same channels in every tile
-    const int gc = (threadIdx.x % GROUPS) * 4, valid = at.count - gc;
-    float bias[4], skip[4];
+    f2 bias[2], skip[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        bias[i] = Q.bias != nullptr && i < valid ? load_param(Q.bias, Q.bias_type, at.first + gc + i) : 0.0f;
-        skip[i] = MODE == kScanMain && Q.d != nullptr && i < valid ? load_param(Q.d, Q.d_type, at.first + gc + i) : 0.0f;
+    for (int i = 0; i < 2; ++i) {
+        float b[2] = {}, d[2] = {};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (Q.bias != nullptr && 2 * i + k < valid) b[k] = load_param(Q.bias, Q.bias_type, at.first + gc + 2 * i + k);
+            if (MODE == kScanMain && Q.d != nullptr && 2 * i + k < valid) d[k] = load_param(Q.d, Q.d_type, at.first + gc + 2 * i + k);
+        }
+        bias[i] = pair(b[0], b[1]);
+        skip[i] = pair(d[0], d[1]);
     }
+    const bool gated = MODE != kScanCarry && Q.z.p != nullptr, softplus = Q.softplus;
+    // the values of a tile whose copies have arrived
+    const auto form = [&](long long t0, int tokens, int buf) {
+        cp_async_wait<0>();
+#pragma unroll
+        for (int g = 0; g < S::NG; ++g) {
+            const int t = fetch.row + g * Tile::Fetch::ROWS;
+            if (t >= T) continue;
+            f2 delta[2] = {pair(0.0f), pair(0.0f)}, u[2] = {pair(0.0f), pair(0.0f)};
+            f2 gate[2] = {pair(1.0f), pair(1.0f)}, dx[2] = {pair(0.0f), pair(0.0f)};
+            if (t < tokens) {
+                f2 raw[2], x[2], slope[2];
+                fetch.four(sm.raw, 0, g, t0, raw);
+                fetch.four(sm.raw, 1, g, t0, x);
+                scan_deltas<false>(softplus, raw, bias, delta, slope);
+                if constexpr (MODE != kScanCarry) {
+                    if (gated) {
+                        f2 z[2];
+                        fetch.four(sm.raw, 2, g, t0, z);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) gate2<false>(z[i], gate[i], slope[i]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    u[i] = x[i] * (MODE == kScanCarryBack ? gate[i] : delta[i]);
+                    dx[i] = x[i] * skip[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float4 w;
+                split(delta[i], w.x, w.z);
+                split(u[i], w.y, w.w);
+                *reinterpret_cast<float4 *>(&sm.du[buf][t][gc + 2 * i]) = w;
+                if constexpr (MODE == kScanMain) {
+                    split(dx[i], w.x, w.z);
+                    split(gate[i], w.y, w.w);
+                    *reinterpret_cast<float4 *>(&sm.ep[buf][t][gc + 2 * i]) = w;
+                }
+            }
+        }
+        fetch.quads(sm.raw, t0, tokens, [&](bool is_b, int t, int s, const float4 &v) {
+            float *p = &sm.bc[buf][MODE == kScanMain && !is_b ? 1 : 0][t][s];
+            if constexpr (R == 4) *reinterpret_cast<float4 *>(p) = v;
+            else *p = v.x;
+        });
+    };
+    form(t0, left, 0);
+    fetch.start(sm.raw, t0 + T, left - T);
     float sum = 0.0f;  // of the deltas
-    for (long long t0 = begin; t0 < stop; t0 += TT) {
-        const int tokens = static_cast<int>(max(0LL, min(static_cast<long long>(TT), end - t0)));
-        if (MODE != kScanMain && tokens == 0) break;
-        Four x[NG], z[NG];
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const int t = (threadIdx.x + g * THREADS) / GROUPS;
-            if (t >= tokens) continue;
-            const long long c = at.first + gc, tt = t0 + t;
-            const TokenView &in = MODE == kScanCarryBack ? Q.dy : Q.x;
-            x[g] = load_four(in.p, Q.type, Q.vec, at.n * in.ldn + tt * in.ldt + c, valid);
-            if (MODE != kScanCarry && Q.z.p != nullptr)
-                z[g] = load_four(Q.z.p, Q.type, Q.vec, at.n * Q.z.ldn + tt * Q.z.ldt + c, valid);
-            float d[4], v[4];
-            floats_of(load_four(Q.dt.p, Q.type, Q.vec, at.n * Q.dt.ldn + tt * Q.dt.ldt + c, valid), Q.type, d);
-            floats_of(x[g], Q.type, v);
-            if (MODE == kScanCarryBack && Q.z.p != nullptr) {
-                float zz[4], gate[4], slope[4];
-                floats_of(z[g], Q.type, zz);
-                gates(zz, gate, slope);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] *= gate[i];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float slope;
-                const float delta = scan_delta(Q, d[i] + bias[i], slope);
-                du[t][gc + i] = make_float2(delta, MODE == kScanCarryBack ? v[i] : delta * v[i]);
-            }
-        }
-        stage_states<SP>(Q, MODE == kScanCarryBack ? Q.c : Q.b, at.n, t0, at.group, tokens, tokens, &bs[0][0]);
-        if (MODE == kScanMain) stage_states<SP>(Q, Q.c, at.n, t0, at.group, tokens, tokens, &cs[0][0]);
+    const long long chunks = (Q.l + T - 1) / T;
+    float *kept = Q.kept + ((at.n * chunks + at.begin / T) * Q.channels + at.channel) * Q.states;
+    const bool writes = at.part < 4 && at.live;
+    for (int buf = 0; left > 0; left -= T, t0 += T, buf ^= 1) {
         __syncthreads();
-        for (int t = 0; t < tokens; t += 4) {
-            if (MODE == kScanMain && Q.kept != nullptr && (t0 + t) % kScanChunk == 0) {
-                const long long chunks = (Q.l + kScanChunk - 1) / kScanChunk, chunk = (t0 + t) / kScanChunk;
-                store_states<R>(Q.kept + ((at.n * chunks + chunk) * Q.channels + channel) * Q.states, at.part, Q.states, live, h);
-            }
+        E *y_at = token_at<E>(Q.y, at.n, t0 + FourSums<P>::first(at.part)) + at.channel;  // the lane's token of each four
+        if (MODE == kScanMain && Q.kept != nullptr) {
+            store_states<S>(kept, at.part, Q.states, at.live, 0, h);
+            kept += static_cast<long long>(Q.channels) * Q.states;
+        }
+        const float2 *du = &sm.du[buf][0][at.chan];
+        const float *b = &sm.bc[buf][0][0][at.part * R], *c = &sm.bc[buf][MODE == kScanMain ? 1 : 0][0][at.part * R];
+#pragma unroll
+        for (int t4 = 0; t4 < T; t4 += 4) {
             float y[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                y[q] = 0.0f;
-                if (t + q >= tokens) continue;
-                const float2 v = du[t + q][at.chan];
-                const float *b = &bs[t + q][at.part * R];
-                if (MODE == kScanCarryBack) {
+            for (int k = 0; k < 4; ++k) {
+                const int t = t4 + k;
+                const float2 v = du[t * S::CB];
+                f2 w[NP];
+                tile_states<S>(b + t * S::SP, w);
+                if constexpr (MODE == kScanCarryBack) {
                     sum += v.x;
 #pragma unroll
-                    for (int r = 0; r < R; ++r) h[r] = fmaf(exp2_fast(sum * a2[r]), v.y * b[r], h[r]);
+                    for (int i = 0; i < NP; ++i) h[i] = fma2(exp2_fast(pair(sum) * a2[i]), pair(v.y) * w[i], h[i]);
                 } else {
-                    if (MODE == kScanCarry) sum += v.x;
+                    if constexpr (MODE == kScanCarry) sum += v.x;
 #pragma unroll
-                    for (int r = 0; r < R; ++r) h[r] = fmaf(exp2_fast(v.x * a2[r]), h[r], v.y * b[r]);
-                    if (MODE == kScanMain) {
-                        const float *c = &cs[t + q][at.part * R];
+                    for (int i = 0; i < NP; ++i) h[i] = fma2(exp2_fast(pair(v.x) * a2[i]), h[i], pair(v.y) * w[i]);
+                }
+                if constexpr (MODE == kScanMain) {
+                    tile_states<S>(c + t * S::SP, w);
+                    f2 p = w[0] * h[0];
 #pragma unroll
-                        for (int r = 0; r < R; ++r) y[q] = fmaf(c[r], h[r], y[q]);
-                    }
+                    for (int i = 1; i < NP; ++i) p = fma2(w[i], h[i], p);
+                    y[k] = sum_of(p);
                 }
             }
-            if (MODE == kScanMain) {
-                FourSums<P> sums;
-                sums(y, at.part);
-                __syncwarp();  // every lane of the channel has read these tokens
-                if (at.part < 4) {
+            if constexpr (MODE == kScanMain) {
+                FourSums<P>::sum(y, at.part);
 #pragma unroll
-                    for (int i = 0; i < FourSums<P>::N; ++i)
-                        if (t + sums.first + i < tokens) du[t + sums.first + i][at.chan].x = y[i];
+                for (int i = 0; i < N; ++i) {
+                    const int t = t4 + FourSums<P>::first(at.part) + i;
+                    if (writes && t < left) {
+                        const float2 e = sm.ep[buf][t][at.chan];
+                        y_at[i * Q.y.ldt] = from_float<E>((y[i] + e.x) * e.y);
+                    }
                 }
+                y_at += 4 * Q.y.ldt;
             }
         }
-        __syncthreads();
-        if (MODE == kScanMain) {
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const int t = (threadIdx.x + g * THREADS) / GROUPS;
-                if (t >= TT || t0 + t >= stop) continue;
-                float out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (t < tokens) {
-                    float v[4];
-                    floats_of(x[g], Q.type, v);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) out[i] = fmaf(skip[i], v[i], du[t][gc + i].x);
-                    if (Q.z.p != nullptr) {
-                        float zz[4], gate[4], slope[4];
-                        floats_of(z[g], Q.type, zz);
-                        gates(zz, gate, slope);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) out[i] *= gate[i];
-                    }
-                }
-                store_four(Q.y.p, Q.type, Q.vec, at.n * Q.y.ldn + (t0 + t) * Q.y.ldt + at.first + gc, valid, out);
-            }
-            __syncthreads();
+        if (left > T) {
+            form(t0 + T, left - T, buf ^ 1);
+            fetch.start(sm.raw, t0 + 2 * T, left - 2 * T);
         }
     }
+    cp_async_wait<0>();
     if (MODE == kScanMain) {
-        if (Q.state_out != nullptr && at.seg == Q.segs - 1 && live)
-            store_states<R>(Q.state_out + at.n * Q.so_ldn + channel * Q.so_ldc, at.part, Q.states, live, h);
-    } else if (live) {
-        const long long row = (at.n * Q.segs + at.seg) * Q.channels + channel;
-        store_states<R>(Q.carry + row * Q.states, at.part, Q.states, live, h);
+        if (Q.state_out != nullptr && at.seg == Q.segs - 1)
+            store_states<S>(Q.state_out + at.n * Q.so_ldn + at.channel * Q.so_ldc, at.part, Q.states, at.live, 0, h);
+        for (long long i = max(at.end, at.begin) * S::GROUPS + threadIdx.x; i < at.stop * S::GROUPS; i += S::THREADS) {
+            const int c0 = static_cast<int>(i % S::GROUPS) * 4;
+            store_zeros<E>(token_at<E>(Q.y, at.n, i / S::GROUPS) + at.first + c0, Q.vec, at.count - c0);
+        }
+    } else if (at.live) {
+        const long long row = (at.n * Q.segs + at.seg) * Q.channels + at.channel;
+        store_states<S>(Q.carry + row * Q.states, at.part, Q.states, at.live, 0, h);
         if (at.part == 0) Q.sums[row] = sum;
     }
 }
 
-// Sums of 2 R values over the channels of a warp.  Lanes share the work: each
-// step halves what a lane holds, until one value is left.
-template <int N, int O, int P>
-__device__ __forceinline__ void channel_sums(float (&v)[N], int lane, int &first, bool &writes) {
-    if constexpr (O >= P) {
-        const bool up = (lane & O) != 0;
-        if constexpr (N > 1) {
-            float half[N / 2];
-            if (up) first += N / 2;
+// ---- gradient -------------------------------------------------------------------------------
+// Sums over the channels of a warp of what a lane has for B and for C, R values
+// each.  Each step halves what a lane holds.  Lanes keep their states in an order
+// of their own (place r holds state r ^ swap), so that in the first steps every
+// lane sends the same places and nothing is selected.
+template <class S>
+struct ChannelSums {
+    static constexpr int P = S::P, R = S::R;
+    static constexpr bool kTwo = R == 4 && P <= 16, kOne = R == 4 && P <= 8, kSides = P <= 4;
+    static constexpr int LEFT = !kTwo ? R : !kOne ? 2 : 1;  // of B and of C, before the sides are shared
+    __device__ __forceinline__ static int swap(int lane) { return (kTwo && (lane & 16) ? 2 : 0) | (kOne && (lane & 8) ? 1 : 0); }
+    // b, c: what the lane has; store(place in [2][SP], value)
+    template <class F>
+    __device__ __forceinline__ static void sum(float (&b)[4], float (&c)[4], int lane, int part, F store) {
+        if constexpr (kTwo) {
 #pragma unroll
-            for (int i = 0; i < N / 2; ++i) {
-                const float send = up ? v[i] : v[i + N / 2], keep = up ? v[i + N / 2] : v[i];
-                half[i] = keep + __shfl_xor_sync(0xffffffffu, send, O);
+            for (int r = 0; r < 2; ++r) {
+                b[r] += __shfl_xor_sync(0xffffffffu, b[r + 2], 16);
+                c[r] += __shfl_xor_sync(0xffffffffu, c[r + 2], 16);
             }
-            channel_sums<N / 2, O / 2, P>(half, lane, first, writes);
+        }
+        if constexpr (kOne) {
+            b[0] += __shfl_xor_sync(0xffffffffu, b[1], 8);
+            c[0] += __shfl_xor_sync(0xffffffffu, c[1], 8);
+        }
+        // place 0 of a lane now holds state 0 ^ swap
+        const int s = part * R;
+        if constexpr (kSides) {  // one lane takes B, its neighbour C
+            constexpr int O = R == 4 ? 4 : 16;
+            const bool up = (lane & O) != 0;
+            float v = (up ? c[0] : b[0]) + __shfl_xor_sync(0xffffffffu, up ? b[0] : c[0], O);
+            bool writes = true;
 #pragma unroll
-            for (int i = 0; i < N / 2; ++i) v[i] = half[i];
+            for (int o = R == 4 ? 2 : 8; o >= P; o /= 2) {
+                v += __shfl_xor_sync(0xffffffffu, v, o);
+                writes = writes && (lane & o) == 0;
+            }
+            if (writes) store((up ? S::SP : 0) + s + swap(lane), v);
         } else {
-            v[0] += __shfl_xor_sync(0xffffffffu, v[0], O);
-            if (up) writes = false;
-            channel_sums<1, O / 2, P>(v, lane, first, writes);
+#pragma unroll
+            for (int r = 0; r < LEFT; ++r) {
+                store(s + (r ^ swap(lane)), b[r]);
+                store(S::SP + s + (r ^ swap(lane)), c[r]);
+            }
         }
     }
-}
-// Values left to a lane: 2 R over 32 / P channels, one at least.
-template <int R, int P>
-constexpr int kSumsLeft = 2 * R * P > 32 ? 2 * R * P / 32 : 1;
+};
 
-// The gradient: tiles of kScanChunk tokens, from a segment's last to its first.
-// A tile's states and decays are formed once more from the state kept in front of
-// it and stay in registers for the way back.
-template <int SP, int R, int THREADS>
-__global__ void __launch_bounds__(THREADS) scan_grad_kernel(const __grid_constant__ ScanParams Q) {
-    using Place = ScanPlace<SP, R, THREADS>;
-    constexpr int P = Place::P, CB = Place::CB, GROUPS = CB / 4, T = kScanChunk, WARPS = THREADS / 32;
-    constexpr int NG = (T * GROUPS + THREADS - 1) / THREADS;
-    __shared__ float4 sm[T][CB];  // delta, delta x, f; then q . B, (q a h) . A, ., and C . h last
-    __shared__ __align__(16) float bs[T][SP], cs[T][SP];
-    __shared__ float red[WARPS][T][2 * SP];
+template <class T, class S>
+struct ScanGradTile {
+    static constexpr int PITCH = S::T * S::SP + 16;  // of a copy in another order: apart in the banks
+    using Fetch = ScanFetch<T, S, 4, true, true>;
+    typename Fetch::Raw raw;
+    float4 v[S::T][S::CB];             // delta, delta x, f, x
+    float2 e[S::T][S::CB];             // slope of delta, dy times the gate's slope
+    float bc[2][S::R][PITCH];          // B and C in the orders that lanes keep
+    float red[S::THREADS / 32][S::T][2 * S::SP];
+};
+
+// Tiles of 16 tokens, from a segment's last to its first.  A tile's states are
+// formed once more from the state kept in front of it and stay in registers for
+// the way back; the decays are formed twice (kept too they would take the
+// registers of half of the warps).
+template <class E, class S>
+__global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel(const __grid_constant__ ScanParams Q) {
+    constexpr int P = S::P, R = S::R, NP = S::NP, T = S::T, WARPS = S::THREADS / 32, N = FourSums<P>::N;
+    using Tile = ScanGradTile<E, S>;
+    using Sums = ChannelSums<S>;
+    extern __shared__ __align__(16) char space[];
+    Tile &sm = *reinterpret_cast<Tile *>(space);
     griddep_wait();
     griddep_launch_dependents();
-    const Place at(Q);
-    const long long begin = at.seg * Q.seg_len, stop = min(Q.l, begin + Q.seg_len), end = min(at.len, stop);
+    const ScanPlace<S> at(Q);
+    const bool gated = Q.z.p != nullptr, softplus = Q.softplus;
     const long long chunks = (Q.l + T - 1) / T;
-    const int channel = at.channel(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const bool live = at.live();
-    float a2[R], q[R], da[R];
-    load_decay<R>(Q, channel, at.part, live, a2);
+    // the last tile with tokens of the sequence, and how many tiles there are
+    int tiles = at.end > at.begin ? static_cast<int>((at.end - at.begin + T - 1) / T) : 0;
+    long long t0 = at.begin + (tiles - 1) * static_cast<long long>(T);
+    int tokens = static_cast<int>(at.end - t0);
+    typename Tile::Fetch fetch(Q, at);
+    fetch.in[0] = Q.dt;
+    fetch.in[1] = Q.x;
+    fetch.in[2] = Q.dy;
+    fetch.in[3] = Q.z;
+    const int gc = fetch.gc, valid = fetch.valid, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int swap = Sums::swap(lane);
+    if (tiles > 0) fetch.start(sm.raw, t0, tokens);
+
+    f2 a2[NP], q[NP], da[NP];
+    load_decay<S>(Q, at, swap, a2);
 #pragma unroll
-    for (int r = 0; r < R; ++r) q[r] = da[r] = 0.0f;
-    if (Q.dlast != nullptr && live)
-        load_states<R>(Q.dlast + at.n * Q.dl_ldn + channel * Q.dl_ldc, at.part, Q.states, live, q);
+    for (int i = 0; i < NP; ++i) q[i] = da[i] = pair(0.0f);
+    if (Q.dlast != nullptr) load_states<S>(Q.dlast + at.n * Q.dl_ldn + at.channel * Q.dl_ldc, at.part, Q.states, at.live, swap, q);
     for (int j = Q.segs - 1; j > at.seg; --j) {
-        const long long row = (at.n * Q.segs + j) * Q.channels + channel;
-        float e[R];
-        load_states<R>(Q.carry + row * Q.states, at.part, Q.states, live, e);
-        const float sum = live ? Q.sums[row] : 0.0f;
+        const long long row = (at.n * Q.segs + j) * Q.channels + at.channel;
+        f2 e[NP];
+        load_states<S>(Q.carry + row * Q.states, at.part, Q.states, at.live, swap, e);
+        const f2 sum = pair(at.live ? Q.sums[row] : 0.0f);
 #pragma unroll
-        for (int r = 0; r < R; ++r) q[r] = fmaf(exp2_fast(sum * a2[r]), q[r], e[r]);
+        for (int i = 0; i < NP; ++i) q[i] = fma2(exp2_fast(sum * a2[i]), q[i], e[i]);
     }
-    const int gc = (threadIdx.x % GROUPS) * 4, valid = at.count - gc;
-    float bias[4], skip[4], dskip[4], dbias[4];
+    f2 bias[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        bias[i] = Q.bias != nullptr && i < valid ? load_param(Q.bias, Q.bias_type, at.first + gc + i) : 0.0f;
-        skip[i] = Q.d != nullptr && i < valid ? load_param(Q.d, Q.d_type, at.first + gc + i) : 0.0f;
-        dskip[i] = dbias[i] = 0.0f;
+    for (int i = 0; i < 2; ++i) {
+        float b[2] = {};
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (Q.bias != nullptr && 2 * i + k < valid) b[k] = load_param(Q.bias, Q.bias_type, at.first + gc + 2 * i + k);
+        bias[i] = pair(b[0], b[1]);
     }
-    for (long long t0 = begin + (stop - 1 - begin) / T * T; t0 >= begin; t0 -= T) {
-        const int tokens = static_cast<int>(max(0LL, min(static_cast<long long>(T), end - t0)));
-        Four rx[NG], rd[NG], rz[NG], rg[NG];
+    const float skip = Q.d != nullptr && at.live ? load_param(Q.d, Q.d_type, at.channel) : 0.0f;
+    float dskip = 0.0f, dbias = 0.0f;  // the lane's tokens of its channel
+    const bool writes = at.part < 4 && at.live;
+    for (; tiles > 0; --tiles, t0 -= T, tokens = T) {
+        f2 before[NP], h[T][NP];
+        load_states<S>(Q.kept + ((at.n * chunks + t0 / T) * Q.channels + at.channel) * Q.states, at.part, Q.states, at.live, swap,
+                       before);
+        cp_async_wait<0>();
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const int t = (threadIdx.x + g * THREADS) / GROUPS;
-            if (t >= tokens) continue;
-            const long long c = at.first + gc, tt = t0 + t;
-            rx[g] = load_four(Q.x.p, Q.type, Q.vec, at.n * Q.x.ldn + tt * Q.x.ldt + c, valid);
-            rd[g] = load_four(Q.dt.p, Q.type, Q.vec, at.n * Q.dt.ldn + tt * Q.dt.ldt + c, valid);
-            rg[g] = load_four(Q.dy.p, Q.type, Q.vec, at.n * Q.dy.ldn + tt * Q.dy.ldt + c, valid);
-            float x[4], d[4], f[4];
-            floats_of(rx[g], Q.type, x);
-            floats_of(rd[g], Q.type, d);
-            floats_of(rg[g], Q.type, f);
-            if (Q.z.p != nullptr) {
-                rz[g] = load_four(Q.z.p, Q.type, Q.vec, at.n * Q.z.ldn + tt * Q.z.ldt + c, valid);
-                float z[4], gate[4], slope[4];
-                floats_of(rz[g], Q.type, z);
-                gates(z, gate, slope);
+        for (int g = 0; g < S::NG; ++g) {
+            const int t = fetch.row + g * Tile::Fetch::ROWS;
+            if (t >= T) continue;
+            f2 delta[2], slope[2], x[2], f[2], w[2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) f[i] *= gate[i];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float slope;
-                const float delta = scan_delta(Q, d[i] + bias[i], slope);
-                sm[t][gc + i] = make_float4(delta, delta * x[i], f[i], 0.0f);
-            }
-        }
-        stage_states<SP>(Q, Q.b, at.n, t0, at.group, tokens, T, &bs[0][0]);
-        stage_states<SP>(Q, Q.c, at.n, t0, at.group, tokens, T, &cs[0][0]);
-        __syncthreads();
-        if (tokens > 0) {
-            float before[R], h[T][R], a[T][R];
-            load_states<R>(Q.kept + ((at.n * chunks + t0 / T) * Q.channels + channel) * Q.states, at.part, Q.states, live, before);
-#pragma unroll
-            for (int t4 = 0; t4 < T; t4 += 4) {
-                float y[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int t = t4 + k;
-                    y[k] = 0.0f;
-                    if (t >= tokens) continue;
-                    const float4 v = sm[t][at.chan];
-#pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        a[t][r] = exp2_fast(v.x * a2[r]);
-                        h[t][r] = fmaf(a[t][r], t == 0 ? before[r] : h[t == 0 ? 0 : t - 1][r], v.y * bs[t][at.part * R + r]);
-                        y[k] = fmaf(cs[t][at.part * R + r], h[t][r], y[k]);
-                    }
-                }
-                if (Q.z.p != nullptr) {
-                    FourSums<P> sums;
-                    sums(y, at.part);
-                    if (at.part < 4) {
-#pragma unroll
-                        for (int i = 0; i < FourSums<P>::N; ++i)
-                            if (t4 + sums.first + i < tokens) sm[t4 + sums.first + i][at.chan].w = y[i];
-                    }
-                }
-            }
-            float da1[R];
-#pragma unroll
-            for (int r = 0; r < R; ++r) da1[r] = 0.0f;
-#pragma unroll
-            for (int t4 = T - 4; t4 >= 0; t4 -= 4) {
-                float db[4], dd[4];
-#pragma unroll
-                for (int k = 3; k >= 0; --k) {
-                    const int t = t4 + k;
-                    db[k] = dd[k] = 0.0f;
-                    if (t >= tokens) continue;
-                    const float4 v = sm[t][at.chan];
-                    float g[2 * R];
-#pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        q[r] = fmaf(v.z, cs[t][at.part * R + r], q[r]);
-                        g[r] = live ? q[r] * v.y : 0.0f;
-                        g[R + r] = live ? v.z * h[t][r] : 0.0f;
-                        db[k] = fmaf(q[r], bs[t][at.part * R + r], db[k]);
-                        q[r] *= a[t][r];
-                        const float m = q[r] * (t == 0 ? before[r] : h[t == 0 ? 0 : t - 1][r]);
-                        dd[k] = fmaf(m, a2[r], dd[k]);
-                        da1[r] = fmaf(m, v.x, da1[r]);
-                    }
-                    int first = 0;
-                    bool writes = true;
-                    channel_sums<2 * R, 16, P>(g, lane, first, writes);
-                    if (writes) {
-#pragma unroll
-                        for (int i = 0; i < (kSumsLeft<R, P>); ++i) {
-                            const int j = first + i;
-                            red[warp][t][j < R ? at.part * R + j : SP + at.part * R + j - R] = g[i];
-                        }
-                    }
-                }
-                FourSums<P> sums, other;
-                sums(db, at.part);
-                other(dd, at.part);
-                __syncwarp();  // every lane of the channel has read these tokens
-                if (at.part < 4) {
-#pragma unroll
-                    for (int i = 0; i < FourSums<P>::N; ++i)
-                        if (t4 + sums.first + i < tokens) {
-                            float4 &v = sm[t4 + sums.first + i][at.chan];
-                            v.x = db[i];
-                            v.y = dd[i] * (1.0f / kLog2E);  // A, not A log2(e)
-                        }
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < R; ++r) da[r] += da1[r];
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < tokens * 2 * SP; i += THREADS) {
-            const int t = i / (2 * SP), j = i - t * 2 * SP, s = j % SP;
-            if (s >= Q.states) continue;
-            float v = red[0][t][j];
-#pragma unroll
-            for (int w = 1; w < WARPS; ++w) v += red[w][t][j];
-            const long long row = ((at.tile * Q.n + at.n) * Q.l + t0 + t) * Q.groups + at.group;
-            Q.part_bc[(row * 2 + j / SP) * Q.states + s] = v;
-        }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const int t = (threadIdx.x + g * THREADS) / GROUPS;
-            if (t >= T || t0 + t >= stop) continue;
-            float dx[4] = {}, ddt[4] = {}, dz[4] = {};
+            for (int i = 0; i < 2; ++i) delta[i] = slope[i] = x[i] = f[i] = w[i] = pair(0.0f);
             if (t < tokens) {
-                float x[4], d[4], f[4], z[4], gate[4], gslope[4];
-                floats_of(rx[g], Q.type, x);
-                floats_of(rd[g], Q.type, d);
-                floats_of(rg[g], Q.type, f);
-                if (Q.z.p != nullptr) {
-                    floats_of(rz[g], Q.type, z);
-                    gates(z, gate, gslope);
-                }
+                f2 raw[2];
+                fetch.four(sm.raw, 0, g, t0, raw);
+                fetch.four(sm.raw, 1, g, t0, x);
+                fetch.four(sm.raw, 2, g, t0, f);
+                scan_deltas<true>(softplus, raw, bias, delta, slope);
+                if (gated) {
+                    f2 z[2], gate, gslope;
+                    fetch.four(sm.raw, 3, g, t0, z);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float4 v = sm[t][gc + i];
-                    float slope;
-                    const float delta = scan_delta(Q, d[i] + bias[i], slope);
-                    if (Q.z.p != nullptr) {
-                        dz[i] = f[i] * fmaf(skip[i], x[i], v.w) * gslope[i];
-                        f[i] *= gate[i];
-                    }
-                    dx[i] = fmaf(delta, v.x, skip[i] * f[i]);
-                    ddt[i] = fmaf(x[i], v.x, v.y) * slope;
-                    if (i < valid) {
-                        dskip[i] = fmaf(f[i], x[i], dskip[i]);
-                        dbias[i] += ddt[i];
+                    for (int i = 0; i < 2; ++i) {
+                        gate2<true>(z[i], gate, gslope);
+                        w[i] = f[i] * gslope;
+                        f[i] = f[i] * gate;
                     }
                 }
             }
-            const long long c = at.first + gc, tt = t0 + t;
-            store_four(Q.dx.p, Q.type, Q.vec, at.n * Q.dx.ldn + tt * Q.dx.ldt + c, valid, dx);
-            store_four(Q.ddt.p, Q.type, Q.vec, at.n * Q.ddt.ldn + tt * Q.ddt.ldt + c, valid, ddt);
-            if (Q.z.p != nullptr) store_four(Q.dz.p, Q.type, Q.vec, at.n * Q.dz.ldn + tt * Q.dz.ldt + c, valid, dz);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float4 v0, v1, e;
+                split(delta[i], v0.x, v1.x);
+                split(delta[i] * x[i], v0.y, v1.y);
+                split(f[i], v0.z, v1.z);
+                split(x[i], v0.w, v1.w);
+                split(slope[i], e.x, e.z);
+                split(w[i], e.y, e.w);
+                sm.v[t][gc + 2 * i] = v0;
+                sm.v[t][gc + 2 * i + 1] = v1;
+                *reinterpret_cast<float4 *>(&sm.e[t][gc + 2 * i]) = e;
+            }
         }
+        fetch.quads(sm.raw, t0, tokens, [&](bool is_b, int t, int s, const float4 &v) {
+            float *p = &sm.bc[is_b ? 0 : 1][0][t * S::SP + s];
+            if constexpr (R == 4) {
+                *reinterpret_cast<float4 *>(p) = v;
+                if constexpr (Sums::kOne) *reinterpret_cast<float4 *>(p + Tile::PITCH) = make_float4(v.y, v.x, v.w, v.z);
+                if constexpr (Sums::kTwo) *reinterpret_cast<float4 *>(p + 2 * Tile::PITCH) = make_float4(v.z, v.w, v.x, v.y);
+                if constexpr (Sums::kOne) *reinterpret_cast<float4 *>(p + 3 * Tile::PITCH) = make_float4(v.w, v.z, v.y, v.x);
+            } else {
+                *p = v.x;
+            }
+        });
         __syncthreads();
-    }
-    if (Q.state_out != nullptr && at.seg == 0 && live)
-        store_states<R>(Q.state_out + at.n * Q.so_ldn + channel * Q.so_ldc, at.part, Q.states, live, q);
-    const long long row = at.n * Q.segs + at.seg;
-    if (Q.part_a != nullptr && live)
-        store_states<R>(Q.part_a + (row * Q.channels + channel) * Q.states, at.part, Q.states, live, da);
-    if (Q.part_d == nullptr) return;
-    // D and dt_bias: over the threads that take the same four channels
-    float *join = reinterpret_cast<float *>(&sm[0][0]);
-    constexpr int ROWS = THREADS / GROUPS;
+        if (tiles > 1) {
+            fetch.start(sm.raw, t0 - T, T);
+        }
+        const float4 *v = &sm.v[0][at.chan];
+        const float *b = &sm.bc[0][R == 4 ? swap : 0][at.part * R], *c = &sm.bc[1][R == 4 ? swap : 0][at.part * R];
+        float y[T / 4][N];  // C . h of the lane's tokens
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        for (int base = 0; base < ROWS; base += T) {  // T rows at a time
-            __syncthreads();
-            const int r = static_cast<int>(threadIdx.x) / GROUPS - base;
-            if (r >= 0 && r < T) {
+        for (int t4 = 0; t4 < T; t4 += 4) {
+            float s[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) join[r * CB + gc + i] = half == 0 ? dskip[i] : dbias[i];
+            for (int k = 0; k < 4; ++k) {
+                const int t = t4 + k;
+                const float2 du = *reinterpret_cast<const float2 *>(&v[t * S::CB]);
+                f2 w[NP];
+                tile_states<S>(b + t * S::SP, w);
+#pragma unroll
+                for (int i = 0; i < NP; ++i)
+                    h[t][i] = fma2(exp2_fast(pair(du.x) * a2[i]), t == 0 ? before[i] : h[t == 0 ? 0 : t - 1][i], pair(du.y) * w[i]);
+                tile_states<S>(c + t * S::SP, w);
+                f2 p = w[0] * h[t][0];
+#pragma unroll
+                for (int i = 1; i < NP; ++i) p = fma2(w[i], h[t][i], p);
+                s[k] = sum_of(p);
             }
-            __syncthreads();
-            for (int c = threadIdx.x; c < at.count; c += THREADS) {
-                float *out = Q.part_d + (row * 2 + half) * Q.channels + at.first + c;
-                float s = base == 0 ? 0.0f : *out;
-                for (int k = 0; k < min(T, ROWS - base); ++k) s += join[k * CB + c];
-                *out = s;
+            FourSums<P>::sum(s, at.part);
+#pragma unroll
+            for (int i = 0; i < N; ++i) y[t4 / 4][i] = s[i];
+            asm volatile("" ::: "memory");  // loads of later tokens stay behind: their registers are the states'
+        }
+        f2 da1[NP];  // sums of this tile
+        float dskip1 = 0.0f, dbias1 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) da1[i] = pair(0.0f);
+#pragma unroll
+        for (int t4 = T - 4; t4 >= 0; t4 -= 4) {
+            float qb[4], qa[4];
+#pragma unroll
+            for (int k = 3; k >= 0; --k) {
+                const int t = t4 + k;
+                const float4 d = v[t * S::CB];
+                f2 wb[NP], wc[NP], sb, sa;
+                float gb[4], gcc[4];
+                tile_states<S>(c + t * S::SP, wc);
+                tile_states<S>(b + t * S::SP, wb);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    q[i] = fma2(pair(d.z), wc[i], q[i]);
+                    split(q[i] * pair(d.y), gb[2 * i], gb[2 * i + 1]);
+                    split(h[t][i] * pair(d.z), gcc[2 * i], gcc[2 * i + 1]);
+                    sb = i == 0 ? q[0] * wb[0] : fma2(q[i], wb[i], sb);
+                    q[i] = q[i] * exp2_fast(pair(d.x) * a2[i]);
+                    const f2 m = q[i] * (t == 0 ? before[i] : h[t == 0 ? 0 : t - 1][i]);
+                    sa = i == 0 ? m * a2[0] : fma2(m, a2[i], sa);
+                    da1[i] = fma2(m, pair(d.x), da1[i]);
+                }
+                qb[k] = sum_of(sb);
+                qa[k] = sum_of(sa);
+                Sums::sum(gb, gcc, lane, at.part, [&](int p, float s) { sm.red[warp][t][p] = s; });
+                asm volatile("" ::: "memory");
+            }
+            FourSums<P>::sum(qb, at.part);
+            FourSums<P>::sum(qa, at.part);
+            const long long row = t0 + t4 + FourSums<P>::first(at.part);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int t = t4 + FourSums<P>::first(at.part) + i;
+                if (writes && t < tokens) {
+                    const float4 d = v[t * S::CB];
+                    const float2 e = sm.e[t][at.chan];
+                    // qa holds A log2(e), not A
+                    const float ddt = fmaf(d.w, qb[i], qa[i] * (1.0f / kLog2E)) * e.x;
+                    dskip1 = fmaf(d.z, d.w, dskip1);
+                    dbias1 += ddt;
+                    token_at<E>(Q.dx, at.n, row + i)[at.channel] = from_float<E>(fmaf(d.x, qb[i], skip * d.z));
+                    token_at<E>(Q.ddt, at.n, row + i)[at.channel] = from_float<E>(ddt);
+                    if (gated) token_at<E>(Q.dz, at.n, row + i)[at.channel] = from_float<E>(e.y * fmaf(skip, d.w, y[t4 / 4][i]));
+                }
             }
         }
+#pragma unroll
+        for (int i = 0; i < NP; ++i) da[i] = da[i] + da1[i];
+        dskip += dskip1;
+        dbias += dbias1;
+        __syncthreads();
+        float *part = Q.part_bc + (((at.tile * Q.n + at.n) * Q.l + t0) * Q.groups + at.group) * 2 * Q.states;
+        for (int i = threadIdx.x; i < tokens * 2 * S::SP; i += S::THREADS) {
+            const int t = i / (2 * S::SP), j = i % (2 * S::SP), s = j % S::SP;
+            if (s >= Q.states) continue;
+            float sum = sm.red[0][t][j];
+#pragma unroll
+            for (int w = 1; w < WARPS; ++w) sum += sm.red[w][t][j];
+            part[(t * static_cast<long long>(Q.groups) * 2 + j / S::SP) * Q.states + s] = sum;
+        }
+    }
+    const auto zeros = [&](const TokenView &w) {
+        if (w.p == nullptr) return;
+        for (long long i = max(at.end, at.begin) * S::GROUPS + threadIdx.x; i < at.stop * S::GROUPS; i += S::THREADS) {
+            const int c0 = static_cast<int>(i % S::GROUPS) * 4;
+            store_zeros<E>(token_at<E>(w, at.n, i / S::GROUPS) + at.first + c0, Q.vec, at.count - c0);
+        }
+    };
+    zeros(Q.dx);
+    zeros(Q.ddt);
+    zeros(Q.dz);
+    if (Q.state_out != nullptr && at.seg == 0)
+        store_states<S>(Q.state_out + at.n * Q.so_ldn + at.channel * Q.so_ldc, at.part, Q.states, at.live, swap, q);
+    const long long row = at.n * Q.segs + at.seg;
+    if (Q.part_a != nullptr)
+        store_states<S>(Q.part_a + (row * Q.channels + at.channel) * Q.states, at.part, Q.states, at.live, swap, da);
+    if (Q.part_d == nullptr) return;
+#pragma unroll
+    for (int o = 1; o < P; o *= 2) {
+        dskip += __shfl_xor_sync(0xffffffffu, dskip, o);
+        dbias += __shfl_xor_sync(0xffffffffu, dbias, o);
+    }
+    if (at.part == 0 && at.live) {
+        Q.part_d[row * 2 * Q.channels + at.channel] = dskip;
+        Q.part_d[(row * 2 + 1) * Q.channels + at.channel] = dbias;
     }
 }
 
@@ -679,48 +890,96 @@ __global__ void __launch_bounds__(kJoinThreads) scan_join_kernel(const __grid_co
 
 // One token of every sequence: x, dt, z, y are [n][channels].  A thread has read
 // its part of the state before it writes it, so state_out may be the state itself.
-template <int SP, int R, int THREADS>
-__global__ void __launch_bounds__(THREADS) scan_step_kernel(const __grid_constant__ ScanParams Q) {
-    using Place = ScanPlace<SP, R, THREADS>;
-    constexpr int P = Place::P;
+template <class E, class S>
+__global__ void __launch_bounds__(S::THREADS) scan_step_kernel(const __grid_constant__ ScanParams Q) {
+    constexpr int P = S::P, R = S::R, NP = S::NP;
     griddep_wait();
     griddep_launch_dependents();
-    const Place at(Q);
-    const int channel = at.channel();
-    const bool live = at.live();
+    const ScanPlace<S> at(Q);
+    const auto element = [&](const TokenView &v, int c) { return to_float(static_cast<const E *>(v.p)[at.n * v.ldn + c]); };
     float y = 0.0f, x = 0.0f;
-    if (live) {
-        float a2[R], h[R];
-        load_states<R>(Q.state + at.n * Q.s_ldn + channel * Q.s_ldc, at.part, Q.states, live, h);
-        load_decay<R>(Q, channel, at.part, live, a2);
-        x = load_param(Q.x.p, Q.type, at.n * Q.x.ldn + channel);
-        float raw = load_param(Q.dt.p, Q.type, at.n * Q.dt.ldn + channel), slope;
-        if (Q.bias != nullptr) raw += load_param(Q.bias, Q.bias_type, channel);
-        const float delta = scan_delta(Q, raw, slope), u = delta * x;
+    if (at.live) {
+        f2 a2[NP], h[NP], delta[2], slope[2];
+        load_states<S>(Q.state + at.n * Q.s_ldn + at.channel * Q.s_ldc, at.part, Q.states, true, 0, h);
+        load_decay<S>(Q, at, 0, a2);
+        x = element(Q.x, at.channel);
+        const f2 raw[2] = {pair(element(Q.dt, at.channel)), pair(0.0f)};
+        const f2 bias[2] = {pair(Q.bias != nullptr ? load_param(Q.bias, Q.bias_type, at.channel) : 0.0f), pair(0.0f)};
+        scan_deltas<false>(Q.softplus, raw, bias, delta, slope);
+        float d, unused, b[4] = {}, c[4] = {};
+        split(delta[0], d, unused);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int s = at.part * R + r;
             if (s >= Q.states) continue;
-            const float b = load_param(Q.b.p, Q.type, at.n * Q.b.ldn + at.group * Q.b.ldg + s);
-            const float c = load_param(Q.c.p, Q.type, at.n * Q.c.ldn + at.group * Q.c.ldg + s);
-            h[r] = fmaf(exp2_fast(delta * a2[r]), h[r], u * b);
-            y = fmaf(c, h[r], y);
+            b[r] = element(Q.b, static_cast<int>(at.group * Q.b.ldg) + s);
+            c[r] = element(Q.c, static_cast<int>(at.group * Q.c.ldg) + s);
         }
-        store_states<R>(Q.state_out + at.n * Q.so_ldn + channel * Q.so_ldc, at.part, Q.states, live, h);
+        f2 s = pair(0.0f);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            h[i] = fma2(exp2_fast(pair(d) * a2[i]), h[i], pair(d * x) * pair(b[2 * i], b[2 * i + 1]));
+            s = fma2(pair(c[2 * i], c[2 * i + 1]), h[i], s);
+        }
+        y = sum_of(s);
+        store_states<S>(Q.state_out + at.n * Q.so_ldn + at.channel * Q.so_ldc, at.part, Q.states, true, 0, h);
     }
 #pragma unroll
     for (int o = 1; o < P; o *= 2) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (live && at.part == 0) {
-        if (Q.d != nullptr) y = fmaf(load_param(Q.d, Q.d_type, channel), x, y);
+    if (at.live && at.part == 0) {
+        if (Q.d != nullptr) y = fmaf(load_param(Q.d, Q.d_type, at.channel), x, y);
         if (Q.z.p != nullptr) {
-            const float z = load_param(Q.z.p, Q.type, at.n * Q.z.ldn + channel);
-            const float zz[4] = {z, 0.0f, 0.0f, 0.0f};
-            float gate[4], slope[4];
-            gates(zz, gate, slope);
-            y *= gate[0];
+            f2 gate, slope;
+            gate2<false>(pair(element(Q.z, at.channel)), gate, slope);
+            float g, unused;
+            split(gate, g, unused);
+            y *= g;
         }
-        store_param(const_cast<void *>(Q.y.p), Q.type, at.n * Q.y.ldn + channel, y);
+        static_cast<E *>(const_cast<void *>(Q.y.p))[at.n * Q.y.ldn + at.channel] = from_float<E>(y);
     }
 }
+
+// ---- instances, one translation unit for each element type -----------------------------------
+enum ScanKernel { kMain, kCarry, kCarryBack, kGrad, kStep };
+struct ScanLaunch {
+    const void *fn;
+    int threads;
+    size_t smem;
+};
+// Threads of a block of the gradient: what the tiles of few lanes take of shared
+// memory grows with the channels of a block.
+constexpr int kScanThreads = 128;
+constexpr int grad_threads(int sp) { return sp >= 16 ? 256 : kScanThreads; }
+
+template <class E, int SP>
+ScanLaunch scan_instance(ScanKernel k) {
+    using S = ScanShape<SP, kScanThreads>;
+    using G = ScanShape<SP, grad_threads(SP)>;
+    switch (k) {
+    case kMain:
+        return {reinterpret_cast<const void *>(&scan_kernel<E, S, kScanMain>), S::THREADS, sizeof(ScanTile<E, S, kScanMain>)};
+    case kCarry:
+        return {reinterpret_cast<const void *>(&scan_kernel<E, S, kScanCarry>), S::THREADS, sizeof(ScanTile<E, S, kScanCarry>)};
+    case kCarryBack:
+        return {reinterpret_cast<const void *>(&scan_kernel<E, S, kScanCarryBack>), S::THREADS,
+                sizeof(ScanTile<E, S, kScanCarryBack>)};
+    case kGrad: return {reinterpret_cast<const void *>(&scan_grad_kernel<E, G>), G::THREADS, sizeof(ScanGradTile<E, G>)};
+    default: return {reinterpret_cast<const void *>(&scan_step_kernel<E, S>), S::THREADS, 0};
+    }
+}
+template <class E>
+ScanLaunch scan_launch(ScanKernel k, int sp) {
+    switch (sp) {
+    case 1: return scan_instance<E, 1>(k);
+    case 4: return scan_instance<E, 4>(k);
+    case 8: return scan_instance<E, 8>(k);
+    case 16: return scan_instance<E, 16>(k);
+    case 32: return scan_instance<E, 32>(k);
+    default: return scan_instance<E, 64>(k);
+    }
+}
+extern template ScanLaunch scan_launch<float>(ScanKernel, int);
+extern template ScanLaunch scan_launch<__half>(ScanKernel, int);
+extern template ScanLaunch scan_launch<__nv_bfloat16>(ScanKernel, int);
 
 }  // namespace gcb

@@ -38,7 +38,7 @@ namespace {
 
 using namespace gcb;
 
-constexpr int kMostStates = 64, kScanThreads = 128;
+constexpr int kMostStates = 64;
 
 // A call's tensors: the descriptors with the same index as their views.
 struct ScanCall {
@@ -105,6 +105,7 @@ int view_scan(const gc_b200_scan_args *q, ScanCall &c) {
     for (const auto &v : views)
         if (v.first != nullptr && (st = strided_of(v.first, *v.second)) != GC_OK) return st;
     if (c.states > kMostStates) return gc_error(GC_UNSUPPORTED, "more than 64 states");
+    if (c.l > INT32_MAX / 2) return gc_error(GC_UNSUPPORTED, "more than 2^30 tokens");
     for (const gc_tensor *t : {q->a, q->d, q->dt_bias})
         if ((st = check_dense(t, "parameters must be dense")) != GC_OK) return st;
     return GC_OK;
@@ -116,10 +117,10 @@ Range lengths_range(const gc_b200_scan_args *q, const ScanCall &c) {
 // ---- plans ------------------------------------------------------------------------------------
 // Lanes of four states; a state count is rounded up to a power of two.
 struct ScanPlan {
-    int sp = 16, lanes = 4, per_lane = 4, channels = 32;  // channels of a block
-    int tiles = 1, segs = 1;
+    int type = 0, sp = 16, lanes = 4, per_lane = 4;
+    int tiles = 1, grad_tiles = 1, segs = 1;  // blocks that share a group's channels
     long long seg_len = 0, blocks = 0;
-    bool vec = false;
+    bool vec = false, bvec = false;
 };
 int padded_states(int64_t s) {
     int sp = 1;
@@ -129,15 +130,16 @@ int padded_states(int64_t s) {
 // Segments: as many as give each multiprocessor six blocks, of at least 64 tokens.
 ScanPlan plan_scan(const ScanCall &c, int sms) {
     ScanPlan p;
+    p.type = c.x.type;
     p.sp = padded_states(c.states);
     p.per_lane = std::min(p.sp, 4);
     p.lanes = p.sp / p.per_lane;
-    p.channels = kScanThreads / p.lanes;
     const int64_t cpg = c.c / c.groups;
-    p.tiles = static_cast<int>(ceil_div(cpg, p.channels));
+    p.tiles = static_cast<int>(ceil_div(cpg, kScanThreads / p.lanes));
+    p.grad_tiles = static_cast<int>(ceil_div(cpg, grad_threads(p.sp) / p.lanes));
     const long long blocks = c.n * c.groups * p.tiles;
     const long long wanted = std::max(1LL, std::min(ceil_div(6LL * sms, std::max(1LL, blocks)), static_cast<long long>(c.l / 64)));
-    p.seg_len = std::max(1LL, gcb::round_up(ceil_div(c.l, wanted), 32));
+    p.seg_len = std::max(1LL, gcb::round_up(ceil_div(c.l, wanted), kScanChunk));
     p.segs = static_cast<int>(std::max(1LL, ceil_div(c.l, p.seg_len)));
     p.blocks = blocks * p.segs;
     return p;
@@ -161,7 +163,7 @@ ScanSpace space_of(const ScanCall &c, const ScanPlan &p, bool backward) {
         s.sums = up16(rows * c.c * sizeof(float));
     }
     if (backward) {
-        s.bc = up16(static_cast<uint64_t>(p.tiles) * c.n * c.l * c.groups * 2 * c.states * sizeof(float));
+        s.bc = up16(static_cast<uint64_t>(p.grad_tiles) * c.n * c.l * c.groups * 2 * c.states * sizeof(float));
         s.a = up16(rows * c.c * c.states * sizeof(float));
         s.d = up16(rows * 2 * c.c * sizeof(float));
     }
@@ -200,8 +202,8 @@ void fill(ScanParams &P, const gc_b200_scan_args *q, const ScanCall &c, const Sc
     P.states = static_cast<int>(c.states);
     P.groups = static_cast<int>(c.groups);
     P.cpg = static_cast<int>(c.c / c.groups);
-    P.type = c.x.type;
     P.vec = plan.vec ? 1 : 0;
+    P.bvec = plan.bvec ? 1 : 0;
     P.softplus = q->softplus != 0;
     P.tiles = plan.tiles;
     P.seg_len = plan.seg_len;
@@ -214,32 +216,24 @@ void set_state_out(ScanParams &P, const Strided &v) {
     P.so_ldc = v.s[1];
 }
 
-// ---- kernels ------------------------------------------------------------------------------------
-enum ScanKernel { kMain, kCarry, kCarryBack, kGrad, kStep };
-template <int SP, int R>
-const void *scan_instance(ScanKernel k) {
-    constexpr int P = SP / R, TT = P >= 4 ? 32 : 8 * P, TH = kScanThreads;
-    switch (k) {
-    case kMain: return reinterpret_cast<const void *>(&scan_kernel<SP, R, TT, TH, kScanMain>);
-    case kCarry: return reinterpret_cast<const void *>(&scan_kernel<SP, R, TT, TH, kScanCarry>);
-    case kCarryBack: return reinterpret_cast<const void *>(&scan_kernel<SP, R, TT, TH, kScanCarryBack>);
-    case kGrad: return reinterpret_cast<const void *>(&scan_grad_kernel<SP, R, TH>);
-    default: return reinterpret_cast<const void *>(&scan_step_kernel<SP, R, TH>);
-    }
+// ---- launches -----------------------------------------------------------------------------------
+ScanLaunch launch_of(ScanKernel k, int type, int sp) {
+    return type == kElemF16    ? scan_launch<__half>(k, sp)
+           : type == kElemBF16 ? scan_launch<__nv_bfloat16>(k, sp)
+                               : scan_launch<float>(k, sp);
 }
-const void *scan_kernel_of(ScanKernel k, const ScanPlan &p) {
-    switch (p.sp) {
-    case 1: return scan_instance<1, 1>(k);
-    case 4: return scan_instance<4, 4>(k);
-    case 8: return scan_instance<8, 4>(k);
-    case 16: return scan_instance<16, 4>(k);
-    case 32: return scan_instance<32, 4>(k);
-    default: return scan_instance<64, 4>(k);
+int launch(ScanKernel k, const ScanPlan &p, ScanParams &P, int dev, const DeviceFacts &facts, cudaStream_t s, cudaError_t &e) {
+    const ScanLaunch l = launch_of(k, p.type, p.sp);
+    if (l.smem > 48 * 1024) {
+        const int st = opt_in_smem(dev, l.fn, facts.smem_optin);
+        if (st != GC_OK) return st;
     }
-}
-cudaError_t launch(ScanKernel k, const ScanPlan &p, ScanParams &P, cudaStream_t s) {
+    P.tiles = l.threads == kScanThreads ? p.tiles : p.grad_tiles;
+    const long long blocks = P.n * P.groups * P.tiles * P.segs;
+    if (blocks > INT32_MAX) return gc_error(GC_UNSUPPORTED, "more work than a grid has blocks");
     void *args[] = {&P};
-    return launch_pdl(scan_kernel_of(k, p), dim3(static_cast<unsigned>(p.blocks)), dim3(kScanThreads), args, 0, s);
+    e = launch_pdl(l.fn, dim3(static_cast<unsigned>(blocks)), dim3(l.threads), args, l.smem, s);
+    return GC_OK;
 }
 
 int current_facts(DeviceFacts &facts) {
@@ -304,8 +298,8 @@ int gc_b200_selective_scan(const gc_b200_scan_args *q, gc_tensor *y, gc_tensor *
         if ((st = check_workspace(kept, kept_bytes, kept_bytes_of(c))) != GC_OK) return st;
         if ((st = check_device_memory(kept, q->x->device_index, dev)) != GC_OK) return st;
     }
-    if (plan.blocks > INT32_MAX) return too_many_blocks();
     plan.vec = fours({&c.x, &c.dt, &c.z, &c.y}, c);
+    plan.bvec = group_aligned(c.b, 4) && group_aligned(c.bc, 4);
     ScanParams P{};
     fill(P, q, c, plan, false);
     P.y = tokens_of(c.y, false);
@@ -315,8 +309,8 @@ int gc_b200_selective_scan(const gc_b200_scan_args *q, gc_tensor *y, gc_tensor *
     P.kept = static_cast<float *>(kept);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
-    if (plan.segs > 1) e = launch(kCarry, plan, P, s);
-    if (e == cudaSuccess) e = launch(kMain, plan, P, s);
+    if (plan.segs > 1 && (st = launch(kCarry, plan, P, dev, facts, s, e)) != GC_OK) return st;
+    if (e == cudaSuccess && (st = launch(kMain, plan, P, dev, facts, s, e)) != GC_OK) return st;
     return launched(e, PlanRecord::kSequence, "selective_scan", plan.blocks, kScanThreads, plan.vec ? 1 : 0, plan.lanes,
                     plan.per_lane, plan.segs, plan.segs > 1 ? 2 : 1);
 } catch (...) {
@@ -375,8 +369,8 @@ int gc_b200_selective_scan_backward(const gc_b200_scan_args *q, const gc_tensor 
     if ((st = check_device_memory(workspace, q->x->device_index, dev)) != GC_OK) return st;
     if ((st = check_workspace(kept, kept_bytes, kept_bytes_of(c))) != GC_OK) return st;
     if (kept_bytes_of(c) != 0 && (st = check_device_memory(kept, q->x->device_index, dev)) != GC_OK) return st;
-    if (plan.blocks > INT32_MAX) return too_many_blocks();
     plan.vec = fours({&c.x, &c.dt, &c.z, &dyv, &dx, &ddt, &dz}, c);
+    plan.bvec = group_aligned(c.b, 4) && group_aligned(c.bc, 4);
     ScanParams P{};
     fill(P, q, c, plan, false);
     P.dy = tokens_of(dyv, false);
@@ -399,19 +393,19 @@ int gc_b200_selective_scan_backward(const gc_b200_scan_args *q, const gc_tensor 
     if (sums_d) P.part_d = reinterpret_cast<float *>(w + space.carry + space.sums + space.bc + space.a);
     int launches = 1;
     if (plan.segs > 1) {
-        e = launch(kCarryBack, plan, P, s);
+        if ((st = launch(kCarryBack, plan, P, dev, facts, s, e)) != GC_OK) return st;
         ++launches;
     }
-    if (e == cudaSuccess) e = launch(kGrad, plan, P, s);
+    if (e == cudaSuccess && (st = launch(kGrad, plan, P, dev, facts, s, e)) != GC_OK) return st;
     if (e == cudaSuccess && c.l > 0 && (g->b != nullptr || g->c != nullptr)) {
         ScanJoinParams J{};
         J.part = P.part_bc;
         J.rows = c.n * c.l * c.groups;
         J.l = c.l;
-        J.tiles = plan.tiles;
+        J.tiles = plan.grad_tiles;
         J.states = P.states;
         J.groups = P.groups;
-        J.type = P.type;
+        J.type = c.x.type;
         if (g->b != nullptr) J.db = pairs_of(db, false);
         if (g->c != nullptr) J.dc = pairs_of(dc, false);
         J.lengths = q->lengths;
@@ -470,12 +464,13 @@ int gc_b200_selective_scan_step(const gc_b200_scan_args *q, gc_tensor *y, gc_ten
     DeviceFacts facts;
     if ((st = device_facts(dev, facts)) != GC_OK) return st;
     const ScanPlan plan = plan_scan(c, facts.sms);
-    if (plan.blocks > INT32_MAX) return too_many_blocks();
     ScanParams P{};
     fill(P, q, c, plan, true);
     P.y = tokens_of(c.y, true);
     set_state_out(P, out);
-    const cudaError_t e = launch(kStep, plan, P, reinterpret_cast<cudaStream_t>(stream));
+    cudaError_t e = cudaSuccess;
+    P.segs = 1;
+    if ((st = launch(kStep, plan, P, dev, facts, reinterpret_cast<cudaStream_t>(stream), e)) != GC_OK) return st;
     return launched(e, PlanRecord::kSequence, "selective_scan_step", plan.blocks, kScanThreads, 0, plan.lanes, plan.per_lane,
                     plan.segs, 1);
 } catch (...) {
