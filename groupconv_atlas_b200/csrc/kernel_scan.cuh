@@ -13,7 +13,7 @@
 // What bounds these kernels is the exponential of every (token, channel, state):
 // the special-function unit does 16 a clock and multiprocessor.  A channel's
 // states are spread over P lanes of R = 4 each, held as pairs of floats; a block
-// takes THREADS / P channels and walks along the tokens in tiles of 16.  A tile's
+// takes 2 THREADS / P channels and walks along the tokens in tiles.  A tile's
 // inputs are copied to shared memory while the tile before is worked on; softplus,
 // gate and products of a token and channel are then formed once for its P lanes.
 // Where sequences and channels alone are too few to fill the GPU, each
@@ -28,9 +28,11 @@
 
 namespace gcb {
 
-// Tokens between the states that the forward pass keeps for the gradient, and
-// that the gradient's kernel takes at a time.
-constexpr int kScanChunk = 16;
+// Tokens between the states that the scan keeps for its gradient; the gradient
+// takes so many at a time.  (With 16 the states of two channels take the registers
+// of half of the warps: 570 us against 432 at N4 L2048 C2048 bf16, for half of the
+// memory.)
+constexpr int kScanChunk = 8;
 
 // A tensor of tokens: strides of a sequence, a token and (B, C) a group.
 struct TokenView {
@@ -186,22 +188,24 @@ __device__ __forceinline__ void gate2(f2 z, f2 &gate, f2 &slope) {
 }
 
 // ---- shapes and places ---------------------------------------------------------------------
-template <int SP_, int THREADS_>
+// A thread takes a part of the states of two neighbouring channels, so that what
+// it reads of B and C serves both.
+template <int SP_, int THREADS_, int T_>
 struct ScanShape {
-    static constexpr int SP = SP_, THREADS = THREADS_, T = kScanChunk;
-    static constexpr int R = SP >= 4 ? 4 : 1, NP = (R + 1) / 2;  // states of a lane, as pairs
-    static constexpr int P = SP / R, CB = THREADS / P;           // lanes of a channel, channels of a block
+    static constexpr int SP = SP_, THREADS = THREADS_, T = T_;   // T: tokens of a tile
+    static constexpr int R = SP >= 4 ? 4 : 1, NP = (R + 1) / 2;  // states of a lane and channel, as pairs
+    static constexpr int P = SP / R, CB = 2 * THREADS / P;       // lanes of a channel, channels of a block
     static constexpr int GROUPS = CB / 4, NG = T * GROUPS > THREADS ? T * GROUPS / THREADS : 1;
     static constexpr int QUADS = SP >= 4 ? SP / 4 : 1;           // of a token's B or C
 };
 
-// A warp's lanes: channel * P + part; a part has the states part * R ...
+// A warp's lanes: pair of channels * P + part; a part has the states part * R ...
 template <class S>
 struct ScanPlace {
     long long n, len, begin, stop, end;  // the segment's tokens; end: of those in the sequence
     int seg, group, tile, first, count;  // first channel of the block, its channels
-    int chan, part, channel;             // the thread's
-    bool live;
+    int chan, part, channel;             // the thread's first channel, in the block and in all
+    bool live[2];
     __device__ __forceinline__ explicit ScanPlace(const ScanParams &Q) {
         const int per = Q.groups * Q.tiles;
         long long b = blockIdx.x;
@@ -213,10 +217,11 @@ struct ScanPlace {
         tile = gt - group * Q.tiles;
         first = group * Q.cpg + tile * S::CB;
         count = min(S::CB, Q.cpg - tile * S::CB);
-        chan = threadIdx.x / S::P;
+        chan = threadIdx.x / S::P * 2;
         part = threadIdx.x % S::P;
         channel = first + chan;
-        live = chan < count;
+        live[0] = chan < count;
+        live[1] = chan + 1 < count;
         len = Q.l;
         if (Q.lengths != nullptr) {
             const int v = Q.lengths[n];
@@ -261,17 +266,31 @@ __device__ __forceinline__ void store_states(float *p, int part, int states, boo
 // numbers, whose exponentials are the same, so that a step size of 0 leaves a
 // state as it is; tiles are filled up with such steps.
 template <class S>
-__device__ __forceinline__ void load_decay(const ScanParams &Q, const ScanPlace<S> &at, int swap, f2 (&v)[S::NP]) {
+__device__ __forceinline__ void load_decay(const ScanParams &Q, const ScanPlace<S> &at, int k, int swap, f2 (&v)[S::NP]) {
     float f[4] = {};
 #pragma unroll
     for (int r = 0; r < S::R; ++r) {
         const int s = at.part * S::R + (r ^ swap);
-        if (at.live && s < Q.states) f[r] = load_param(Q.a, Q.a_type, static_cast<long long>(at.channel) * Q.states + s) * kLog2E;
+        if (at.live[k] && s < Q.states)
+            f[r] = load_param(Q.a, Q.a_type, static_cast<long long>(at.channel + k) * Q.states + s) * kLog2E;
         if (f[r] > 3e38f) f[r] = 3e38f;
         if (f[r] < -3e38f) f[r] = -3e38f;
     }
 #pragma unroll
     for (int i = 0; i < S::NP; ++i) v[i] = pair(f[2 * i], f[2 * i + 1]);
+}
+// Element (or, where `vec`, both at once) of the two channels from p.
+template <class T>
+__device__ __forceinline__ void store_two(T *p, bool vec, const bool (&live)[2], float a, float b) {
+    if (vec && live[1]) {  // pairs lie on pairs
+        struct alignas(2 * sizeof(T)) Two {
+            T a, b;
+        };
+        *reinterpret_cast<Two *>(p) = Two{from_float<T>(a), from_float<T>(b)};
+    } else {
+        if (live[0]) p[0] = from_float<T>(a);
+        if (live[1]) p[1] = from_float<T>(b);
+    }
 }
 // A lane's states of a token from shared memory.
 template <class S>
@@ -439,19 +458,22 @@ __global__ void __launch_bounds__(S::THREADS) scan_kernel(const __grid_constant_
     int left = static_cast<int>(max(0LL, at.end - t0));  // tokens from the tile on
     fetch.start(sm.raw, t0, left);
 
-    f2 a2[NP], h[NP];
-    load_decay<S>(Q, at, 0, a2);
+    f2 a2[2][NP], h[2][NP];
 #pragma unroll
-    for (int i = 0; i < NP; ++i) h[i] = pair(0.0f);
-    if (MODE == kScanMain) {
-        if (Q.state != nullptr) load_states<S>(Q.state + at.n * Q.s_ldn + at.channel * Q.s_ldc, at.part, Q.states, at.live, 0, h);
+    for (int k = 0; k < 2; ++k) {
+        load_decay<S>(Q, at, k, 0, a2[k]);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) h[k][i] = pair(0.0f);
+        if (MODE != kScanMain) continue;
+        if (Q.state != nullptr)
+            load_states<S>(Q.state + at.n * Q.s_ldn + (at.channel + k) * Q.s_ldc, at.part, Q.states, at.live[k], 0, h[k]);
         for (int j = 0; j < at.seg; ++j) {
-            const long long row = (at.n * Q.segs + j) * Q.channels + at.channel;
+            const long long row = (at.n * Q.segs + j) * Q.channels + at.channel + k;
             f2 e[NP];
-            load_states<S>(Q.carry + row * Q.states, at.part, Q.states, at.live, 0, e);
-            const f2 sum = pair(at.live ? Q.sums[row] : 0.0f);
+            load_states<S>(Q.carry + row * Q.states, at.part, Q.states, at.live[k], 0, e);
+            const f2 sum = pair(at.live[k] ? Q.sums[row] : 0.0f);
 #pragma unroll
-            for (int i = 0; i < NP; ++i) h[i] = fma2(exp2_fast(sum * a2[i]), h[i], e[i]);
+            for (int i = 0; i < NP; ++i) h[k][i] = fma2(exp2_fast(sum * a2[k][i]), h[k][i], e[i]);
         }
     }
     f2 bias[2], skip[2];
@@ -516,53 +538,58 @@ __global__ void __launch_bounds__(S::THREADS) scan_kernel(const __grid_constant_
     };
     form(t0, left, 0);
     fetch.start(sm.raw, t0 + T, left - T);
-    float sum = 0.0f;  // of the deltas
-    const long long chunks = (Q.l + T - 1) / T;
-    float *kept = Q.kept + ((at.n * chunks + at.begin / T) * Q.channels + at.channel) * Q.states;
-    const bool writes = at.part < 4 && at.live;
+    float sum[2] = {0.0f, 0.0f};  // of the deltas
+    const long long chunks = (Q.l + kScanChunk - 1) / kScanChunk;
+    float *kept = Q.kept + ((at.n * chunks + at.begin / kScanChunk) * Q.channels + at.channel) * Q.states;
+    const bool writes = at.part < 4, vec = Q.vec;
     for (int buf = 0; left > 0; left -= T, t0 += T, buf ^= 1) {
         __syncthreads();
         E *y_at = token_at<E>(Q.y, at.n, t0 + FourSums<P>::first(at.part)) + at.channel;  // the lane's token of each four
-        if (MODE == kScanMain && Q.kept != nullptr) {
-            store_states<S>(kept, at.part, Q.states, at.live, 0, h);
-            kept += static_cast<long long>(Q.channels) * Q.states;
-        }
         const float2 *du = &sm.du[buf][0][at.chan];
         const float *b = &sm.bc[buf][0][0][at.part * R], *c = &sm.bc[buf][MODE == kScanMain ? 1 : 0][0][at.part * R];
 #pragma unroll
         for (int t4 = 0; t4 < T; t4 += 4) {
-            float y[4];
+            if (MODE == kScanMain && t4 % kScanChunk == 0 && Q.kept != nullptr && t4 < left) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int t = t4 + k;
-                const float2 v = du[t * S::CB];
-                f2 w[NP];
-                tile_states<S>(b + t * S::SP, w);
-                if constexpr (MODE == kScanCarryBack) {
-                    sum += v.x;
+                for (int k = 0; k < 2; ++k) store_states<S>(kept + k * Q.states, at.part, Q.states, at.live[k], 0, h[k]);
+                kept += static_cast<long long>(Q.channels) * Q.states;
+            }
+            float y[2][4];
 #pragma unroll
-                    for (int i = 0; i < NP; ++i) h[i] = fma2(exp2_fast(pair(sum) * a2[i]), pair(v.y) * w[i], h[i]);
-                } else {
-                    if constexpr (MODE == kScanCarry) sum += v.x;
+            for (int j = 0; j < 4; ++j) {
+                const int t = t4 + j;
+                const float4 v = *reinterpret_cast<const float4 *>(&du[t * S::CB]);
+                const float delta[2] = {v.x, v.z}, u[2] = {v.y, v.w};
+                f2 wb[NP], wc[NP];
+                tile_states<S>(b + t * S::SP, wb);
+                if constexpr (MODE == kScanMain) tile_states<S>(c + t * S::SP, wc);
 #pragma unroll
-                    for (int i = 0; i < NP; ++i) h[i] = fma2(exp2_fast(pair(v.x) * a2[i]), h[i], pair(v.y) * w[i]);
-                }
-                if constexpr (MODE == kScanMain) {
-                    tile_states<S>(c + t * S::SP, w);
-                    f2 p = w[0] * h[0];
+                for (int k = 0; k < 2; ++k) {
+                    if constexpr (MODE != kScanMain) sum[k] += delta[k];
+                    if constexpr (MODE == kScanCarryBack) {
 #pragma unroll
-                    for (int i = 1; i < NP; ++i) p = fma2(w[i], h[i], p);
-                    y[k] = sum_of(p);
+                        for (int i = 0; i < NP; ++i) h[k][i] = fma2(exp2_fast(pair(sum[k]) * a2[k][i]), pair(u[k]) * wb[i], h[k][i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NP; ++i) h[k][i] = fma2(exp2_fast(pair(delta[k]) * a2[k][i]), h[k][i], pair(u[k]) * wb[i]);
+                    }
+                    if constexpr (MODE == kScanMain) {
+                        f2 p = wc[0] * h[k][0];
+#pragma unroll
+                        for (int i = 1; i < NP; ++i) p = fma2(wc[i], h[k][i], p);
+                        y[k][j] = sum_of(p);
+                    }
                 }
             }
             if constexpr (MODE == kScanMain) {
-                FourSums<P>::sum(y, at.part);
+                FourSums<P>::sum(y[0], at.part);
+                FourSums<P>::sum(y[1], at.part);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const int t = t4 + FourSums<P>::first(at.part) + i;
                     if (writes && t < left) {
-                        const float2 e = sm.ep[buf][t][at.chan];
-                        y_at[i * Q.y.ldt] = from_float<E>((y[i] + e.x) * e.y);
+                        const float4 e = *reinterpret_cast<const float4 *>(&sm.ep[buf][t][at.chan]);
+                        store_two<E>(y_at + i * Q.y.ldt, vec, at.live, (y[0][i] + e.x) * e.y, (y[1][i] + e.z) * e.w);
                     }
                 }
                 y_at += 4 * Q.y.ldt;
@@ -576,15 +603,20 @@ __global__ void __launch_bounds__(S::THREADS) scan_kernel(const __grid_constant_
     cp_async_wait<0>();
     if (MODE == kScanMain) {
         if (Q.state_out != nullptr && at.seg == Q.segs - 1)
-            store_states<S>(Q.state_out + at.n * Q.so_ldn + at.channel * Q.so_ldc, at.part, Q.states, at.live, 0, h);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                store_states<S>(Q.state_out + at.n * Q.so_ldn + (at.channel + k) * Q.so_ldc, at.part, Q.states, at.live[k], 0, h[k]);
         for (long long i = max(at.end, at.begin) * S::GROUPS + threadIdx.x; i < at.stop * S::GROUPS; i += S::THREADS) {
             const int c0 = static_cast<int>(i % S::GROUPS) * 4;
             store_zeros<E>(token_at<E>(Q.y, at.n, i / S::GROUPS) + at.first + c0, Q.vec, at.count - c0);
         }
-    } else if (at.live) {
-        const long long row = (at.n * Q.segs + at.seg) * Q.channels + at.channel;
-        store_states<S>(Q.carry + row * Q.states, at.part, Q.states, at.live, 0, h);
-        if (at.part == 0) Q.sums[row] = sum;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const long long row = (at.n * Q.segs + at.seg) * Q.channels + at.channel + k;
+            store_states<S>(Q.carry + row * Q.states, at.part, Q.states, at.live[k], 0, h[k]);
+            if (at.part == 0 && at.live[k]) Q.sums[row] = sum[k];
+        }
     }
 }
 
@@ -641,13 +673,14 @@ struct ScanGradTile {
     static constexpr int PITCH = S::T * S::SP + 16;  // of a copy in another order: apart in the banks
     using Fetch = ScanFetch<T, S, 4, true, true>;
     typename Fetch::Raw raw;
-    float4 v[S::T][S::CB];             // delta, delta x, f, x
+    float2 du[S::T][S::CB];            // delta, delta x
+    float f[S::T][S::CB], x[S::T][S::CB];
     float2 e[S::T][S::CB];             // slope of delta, dy times the gate's slope
     float bc[2][S::R][PITCH];          // B and C in the orders that lanes keep
     float red[S::THREADS / 32][S::T][2 * S::SP];
 };
 
-// Tiles of 16 tokens, from a segment's last to its first.  A tile's states are
+// Tiles of 8 tokens, from a segment's last to its first.  A tile's states are
 // formed once more from the state kept in front of it and stay in registers for
 // the way back; the decays are formed twice (kept too they would take the
 // registers of half of the warps).
@@ -676,18 +709,22 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
     const int swap = Sums::swap(lane);
     if (tiles > 0) fetch.start(sm.raw, t0, tokens);
 
-    f2 a2[NP], q[NP], da[NP];
-    load_decay<S>(Q, at, swap, a2);
+    f2 a2[2][NP], q[2][NP], da[2][NP];
 #pragma unroll
-    for (int i = 0; i < NP; ++i) q[i] = da[i] = pair(0.0f);
-    if (Q.dlast != nullptr) load_states<S>(Q.dlast + at.n * Q.dl_ldn + at.channel * Q.dl_ldc, at.part, Q.states, at.live, swap, q);
-    for (int j = Q.segs - 1; j > at.seg; --j) {
-        const long long row = (at.n * Q.segs + j) * Q.channels + at.channel;
-        f2 e[NP];
-        load_states<S>(Q.carry + row * Q.states, at.part, Q.states, at.live, swap, e);
-        const f2 sum = pair(at.live ? Q.sums[row] : 0.0f);
+    for (int k = 0; k < 2; ++k) {
+        load_decay<S>(Q, at, k, swap, a2[k]);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) q[i] = fma2(exp2_fast(sum * a2[i]), q[i], e[i]);
+        for (int i = 0; i < NP; ++i) q[k][i] = da[k][i] = pair(0.0f);
+        if (Q.dlast != nullptr)
+            load_states<S>(Q.dlast + at.n * Q.dl_ldn + (at.channel + k) * Q.dl_ldc, at.part, Q.states, at.live[k], swap, q[k]);
+        for (int j = Q.segs - 1; j > at.seg; --j) {
+            const long long row = (at.n * Q.segs + j) * Q.channels + at.channel + k;
+            f2 e[NP];
+            load_states<S>(Q.carry + row * Q.states, at.part, Q.states, at.live[k], swap, e);
+            const f2 sum = pair(at.live[k] ? Q.sums[row] : 0.0f);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) q[k][i] = fma2(exp2_fast(sum * a2[k][i]), q[k][i], e[i]);
+        }
     }
     f2 bias[2];
 #pragma unroll
@@ -698,13 +735,17 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
             if (Q.bias != nullptr && 2 * i + k < valid) b[k] = load_param(Q.bias, Q.bias_type, at.first + gc + 2 * i + k);
         bias[i] = pair(b[0], b[1]);
     }
-    const float skip = Q.d != nullptr && at.live ? load_param(Q.d, Q.d_type, at.channel) : 0.0f;
-    float dskip = 0.0f, dbias = 0.0f;  // the lane's tokens of its channel
-    const bool writes = at.part < 4 && at.live;
+    float skip[2], dskip[2] = {0.0f, 0.0f}, dbias[2] = {0.0f, 0.0f};  // sums: over the lane's tokens
+#pragma unroll
+    for (int k = 0; k < 2; ++k) skip[k] = Q.d != nullptr && at.live[k] ? load_param(Q.d, Q.d_type, at.channel + k) : 0.0f;
+    const bool writes = at.part < 4, vec = Q.vec;
+
     for (; tiles > 0; --tiles, t0 -= T, tokens = T) {
-        f2 before[NP], h[T][NP];
-        load_states<S>(Q.kept + ((at.n * chunks + t0 / T) * Q.channels + at.channel) * Q.states, at.part, Q.states, at.live, swap,
-                       before);
+        f2 before[2][NP], h[T][2][NP];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            load_states<S>(Q.kept + ((at.n * chunks + t0 / T) * Q.channels + at.channel + k) * Q.states, at.part, Q.states,
+                           at.live[k], swap, before[k]);
         cp_async_wait<0>();
 #pragma unroll
         for (int g = 0; g < S::NG; ++g) {
@@ -732,17 +773,21 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                float4 v0, v1, e;
-                split(delta[i], v0.x, v1.x);
-                split(delta[i] * x[i], v0.y, v1.y);
-                split(f[i], v0.z, v1.z);
-                split(x[i], v0.w, v1.w);
+                float4 d, e;
+                split(delta[i], d.x, d.z);
+                split(delta[i] * x[i], d.y, d.w);
                 split(slope[i], e.x, e.z);
                 split(w[i], e.y, e.w);
-                sm.v[t][gc + 2 * i] = v0;
-                sm.v[t][gc + 2 * i + 1] = v1;
+                *reinterpret_cast<float4 *>(&sm.du[t][gc + 2 * i]) = d;
                 *reinterpret_cast<float4 *>(&sm.e[t][gc + 2 * i]) = e;
             }
+            float4 f4, x4;
+            split(f[0], f4.x, f4.y);
+            split(f[1], f4.z, f4.w);
+            split(x[0], x4.x, x4.y);
+            split(x[1], x4.z, x4.w);
+            *reinterpret_cast<float4 *>(&sm.f[t][gc]) = f4;
+            *reinterpret_cast<float4 *>(&sm.x[t][gc]) = x4;
         }
         fetch.quads(sm.raw, t0, tokens, [&](bool is_b, int t, int s, const float4 &v) {
             float *p = &sm.bc[is_b ? 0 : 1][0][t * S::SP + s];
@@ -759,86 +804,102 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
         if (tiles > 1) {
             fetch.start(sm.raw, t0 - T, T);
         }
-        const float4 *v = &sm.v[0][at.chan];
         const float *b = &sm.bc[0][R == 4 ? swap : 0][at.part * R], *c = &sm.bc[1][R == 4 ? swap : 0][at.part * R];
-        float y[T / 4][N];  // C . h of the lane's tokens
 #pragma unroll
-        for (int t4 = 0; t4 < T; t4 += 4) {
-            float s[4];
+        for (int t = 0; t < T; ++t) {
+            const float4 v = *reinterpret_cast<const float4 *>(&sm.du[t][at.chan]);
+            const float delta[2] = {v.x, v.z}, u[2] = {v.y, v.w};
+            f2 w[NP];
+            tile_states<S>(b + t * S::SP, w);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int t = t4 + k;
-                const float2 du = *reinterpret_cast<const float2 *>(&v[t * S::CB]);
-                f2 w[NP];
-                tile_states<S>(b + t * S::SP, w);
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int i = 0; i < NP; ++i)
-                    h[t][i] = fma2(exp2_fast(pair(du.x) * a2[i]), t == 0 ? before[i] : h[t == 0 ? 0 : t - 1][i], pair(du.y) * w[i]);
-                tile_states<S>(c + t * S::SP, w);
-                f2 p = w[0] * h[t][0];
-#pragma unroll
-                for (int i = 1; i < NP; ++i) p = fma2(w[i], h[t][i], p);
-                s[k] = sum_of(p);
-            }
-            FourSums<P>::sum(s, at.part);
-#pragma unroll
-            for (int i = 0; i < N; ++i) y[t4 / 4][i] = s[i];
-            asm volatile("" ::: "memory");  // loads of later tokens stay behind: their registers are the states'
+                    h[t][k][i] = fma2(exp2_fast(pair(delta[k]) * a2[k][i]), t == 0 ? before[k][i] : h[t == 0 ? 0 : t - 1][k][i],
+                                      pair(u[k]) * w[i]);
+            // loads of later tokens stay behind: their registers are the states'
+            if (t % 4 == 3) asm volatile("" ::: "memory");
         }
-        f2 da1[NP];  // sums of this tile
-        float dskip1 = 0.0f, dbias1 = 0.0f;
+        f2 da1[2][NP];  // sums of this tile
+        float dskip1[2] = {0.0f, 0.0f}, dbias1[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < NP; ++i) da1[i] = pair(0.0f);
+        for (int i = 0; i < NP; ++i) da1[0][i] = da1[1][i] = pair(0.0f);
 #pragma unroll
         for (int t4 = T - 4; t4 >= 0; t4 -= 4) {
-            float qb[4], qa[4];
+            float qb[2][4], qa[2][4], y[2][4];  // q . B, (q a h) . A, C . h
 #pragma unroll
-            for (int k = 3; k >= 0; --k) {
-                const int t = t4 + k;
-                const float4 d = v[t * S::CB];
-                f2 wb[NP], wc[NP], sb, sa;
-                float gb[4], gcc[4];
+            for (int j = 3; j >= 0; --j) {
+                const int t = t4 + j;
+                const float4 v = *reinterpret_cast<const float4 *>(&sm.du[t][at.chan]);
+                const float2 f2v = *reinterpret_cast<const float2 *>(&sm.f[t][at.chan]);
+                const float delta[2] = {v.x, v.z}, u[2] = {v.y, v.w}, f[2] = {f2v.x, f2v.y};
+                f2 wb[NP], wc[NP], gb[NP], gc2[NP];
                 tile_states<S>(c + t * S::SP, wc);
                 tile_states<S>(b + t * S::SP, wb);
 #pragma unroll
-                for (int i = 0; i < NP; ++i) {
-                    q[i] = fma2(pair(d.z), wc[i], q[i]);
-                    split(q[i] * pair(d.y), gb[2 * i], gb[2 * i + 1]);
-                    split(h[t][i] * pair(d.z), gcc[2 * i], gcc[2 * i + 1]);
-                    sb = i == 0 ? q[0] * wb[0] : fma2(q[i], wb[i], sb);
-                    q[i] = q[i] * exp2_fast(pair(d.x) * a2[i]);
-                    const f2 m = q[i] * (t == 0 ? before[i] : h[t == 0 ? 0 : t - 1][i]);
-                    sa = i == 0 ? m * a2[0] : fma2(m, a2[i], sa);
-                    da1[i] = fma2(m, pair(d.x), da1[i]);
+                for (int k = 0; k < 2; ++k) {
+                    f2 sb, sa, sy;
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) {
+                        q[k][i] = fma2(pair(f[k]), wc[i], q[k][i]);
+                        gb[i] = k == 0 ? q[k][i] * pair(u[k]) : fma2(q[k][i], pair(u[k]), gb[i]);
+                        gc2[i] = k == 0 ? h[t][k][i] * pair(f[k]) : fma2(h[t][k][i], pair(f[k]), gc2[i]);
+                        sb = i == 0 ? q[k][0] * wb[0] : fma2(q[k][i], wb[i], sb);
+                        sy = i == 0 ? h[t][k][0] * wc[0] : fma2(h[t][k][i], wc[i], sy);
+                        q[k][i] = q[k][i] * exp2_fast(pair(delta[k]) * a2[k][i]);
+                        const f2 m = q[k][i] * (t == 0 ? before[k][i] : h[t == 0 ? 0 : t - 1][k][i]);
+                        sa = i == 0 ? m * a2[k][0] : fma2(m, a2[k][i], sa);
+                        da1[k][i] = fma2(m, pair(delta[k]), da1[k][i]);
+                    }
+                    qb[k][j] = sum_of(sb);
+                    qa[k][j] = sum_of(sa);
+                    y[k][j] = sum_of(sy);
                 }
-                qb[k] = sum_of(sb);
-                qa[k] = sum_of(sa);
-                Sums::sum(gb, gcc, lane, at.part, [&](int p, float s) { sm.red[warp][t][p] = s; });
+                float gbv[4], gcv[4];
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    split(gb[i], gbv[2 * i], gbv[2 * i + 1]);
+                    split(gc2[i], gcv[2 * i], gcv[2 * i + 1]);
+                }
+                Sums::sum(gbv, gcv, lane, at.part, [&](int p, float s) { sm.red[warp][t][p] = s; });
                 asm volatile("" ::: "memory");
             }
-            FourSums<P>::sum(qb, at.part);
-            FourSums<P>::sum(qa, at.part);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                FourSums<P>::sum(qb[k], at.part);
+                FourSums<P>::sum(qa[k], at.part);
+                if (gated) FourSums<P>::sum(y[k], at.part);
+            }
             const long long row = t0 + t4 + FourSums<P>::first(at.part);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int t = t4 + FourSums<P>::first(at.part) + i;
                 if (writes && t < tokens) {
-                    const float4 d = v[t * S::CB];
-                    const float2 e = sm.e[t][at.chan];
-                    // qa holds A log2(e), not A
-                    const float ddt = fmaf(d.w, qb[i], qa[i] * (1.0f / kLog2E)) * e.x;
-                    dskip1 = fmaf(d.z, d.w, dskip1);
-                    dbias1 += ddt;
-                    token_at<E>(Q.dx, at.n, row + i)[at.channel] = from_float<E>(fmaf(d.x, qb[i], skip * d.z));
-                    token_at<E>(Q.ddt, at.n, row + i)[at.channel] = from_float<E>(ddt);
-                    if (gated) token_at<E>(Q.dz, at.n, row + i)[at.channel] = from_float<E>(e.y * fmaf(skip, d.w, y[t4 / 4][i]));
+                    float dx[2], ddt[2], dz[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float f = sm.f[t][at.chan + k], x = sm.x[t][at.chan + k];
+                        const float2 e = sm.e[t][at.chan + k];
+                        dx[k] = fmaf(sm.du[t][at.chan + k].x, qb[k][i], skip[k] * f);
+                        // qa holds A log2(e), not A
+                        ddt[k] = fmaf(x, qb[k][i], qa[k][i] * (1.0f / kLog2E)) * e.x;
+                        dz[k] = e.y * fmaf(skip[k], x, y[k][i]);
+                        dskip1[k] = fmaf(f, x, dskip1[k]);
+                        dbias1[k] += ddt[k];
+                    }
+                    store_two<E>(token_at<E>(Q.dx, at.n, row + i) + at.channel, vec, at.live, dx[0], dx[1]);
+                    store_two<E>(token_at<E>(Q.ddt, at.n, row + i) + at.channel, vec, at.live, ddt[0], ddt[1]);
+                    if (gated) store_two<E>(token_at<E>(Q.dz, at.n, row + i) + at.channel, vec, at.live, dz[0], dz[1]);
                 }
             }
         }
 #pragma unroll
-        for (int i = 0; i < NP; ++i) da[i] = da[i] + da1[i];
-        dskip += dskip1;
-        dbias += dbias1;
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) da[k][i] = da[k][i] + da1[k][i];
+            dskip[k] += dskip1[k];
+            dbias[k] += dbias1[k];
+        }
         __syncthreads();
         float *part = Q.part_bc + (((at.tile * Q.n + at.n) * Q.l + t0) * Q.groups + at.group) * 2 * Q.states;
         for (int i = threadIdx.x; i < tokens * 2 * S::SP; i += S::THREADS) {
@@ -860,20 +921,23 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
     zeros(Q.dx);
     zeros(Q.ddt);
     zeros(Q.dz);
-    if (Q.state_out != nullptr && at.seg == 0)
-        store_states<S>(Q.state_out + at.n * Q.so_ldn + at.channel * Q.so_ldc, at.part, Q.states, at.live, swap, q);
     const long long row = at.n * Q.segs + at.seg;
-    if (Q.part_a != nullptr)
-        store_states<S>(Q.part_a + (row * Q.channels + at.channel) * Q.states, at.part, Q.states, at.live, swap, da);
-    if (Q.part_d == nullptr) return;
 #pragma unroll
-    for (int o = 1; o < P; o *= 2) {
-        dskip += __shfl_xor_sync(0xffffffffu, dskip, o);
-        dbias += __shfl_xor_sync(0xffffffffu, dbias, o);
-    }
-    if (at.part == 0 && at.live) {
-        Q.part_d[row * 2 * Q.channels + at.channel] = dskip;
-        Q.part_d[(row * 2 + 1) * Q.channels + at.channel] = dbias;
+    for (int k = 0; k < 2; ++k) {
+        if (Q.state_out != nullptr && at.seg == 0)
+            store_states<S>(Q.state_out + at.n * Q.so_ldn + (at.channel + k) * Q.so_ldc, at.part, Q.states, at.live[k], swap, q[k]);
+        if (Q.part_a != nullptr)
+            store_states<S>(Q.part_a + (row * Q.channels + at.channel + k) * Q.states, at.part, Q.states, at.live[k], swap, da[k]);
+        if (Q.part_d == nullptr) continue;
+#pragma unroll
+        for (int o = 1; o < P; o *= 2) {
+            dskip[k] += __shfl_xor_sync(0xffffffffu, dskip[k], o);
+            dbias[k] += __shfl_xor_sync(0xffffffffu, dbias[k], o);
+        }
+        if (at.part == 0 && at.live[k]) {
+            Q.part_d[row * 2 * Q.channels + at.channel + k] = dskip[k];
+            Q.part_d[(row * 2 + 1) * Q.channels + at.channel + k] = dbias[k];
+        }
     }
 }
 
@@ -896,47 +960,62 @@ __global__ void __launch_bounds__(S::THREADS) scan_step_kernel(const __grid_cons
     griddep_wait();
     griddep_launch_dependents();
     const ScanPlace<S> at(Q);
-    const auto element = [&](const TokenView &v, int c) { return to_float(static_cast<const E *>(v.p)[at.n * v.ldn + c]); };
-    float y = 0.0f, x = 0.0f;
-    if (at.live) {
-        f2 a2[NP], h[NP], delta[2], slope[2];
-        load_states<S>(Q.state + at.n * Q.s_ldn + at.channel * Q.s_ldc, at.part, Q.states, true, 0, h);
-        load_decay<S>(Q, at, 0, a2);
-        x = element(Q.x, at.channel);
-        const f2 raw[2] = {pair(element(Q.dt, at.channel)), pair(0.0f)};
-        const f2 bias[2] = {pair(Q.bias != nullptr ? load_param(Q.bias, Q.bias_type, at.channel) : 0.0f), pair(0.0f)};
-        scan_deltas<false>(Q.softplus, raw, bias, delta, slope);
-        float d, unused, b[4] = {}, c[4] = {};
-        split(delta[0], d, unused);
+    const auto element = [&](const TokenView &v, long long c) { return to_float(static_cast<const E *>(v.p)[at.n * v.ldn + c]); };
+    const auto two = [&](const TokenView &v, float (&e)[2]) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int s = at.part * R + r;
-            if (s >= Q.states) continue;
-            b[r] = element(Q.b, static_cast<int>(at.group * Q.b.ldg) + s);
-            c[r] = element(Q.c, static_cast<int>(at.group * Q.c.ldg) + s);
-        }
+        for (int k = 0; k < 2; ++k) e[k] = at.live[k] ? element(v, at.channel + k) : 0.0f;
+    };
+    f2 a2[2][NP], h[2][NP], delta[2], slope[2], raw[2], bias[2] = {pair(0.0f), pair(0.0f)};
+    float x[2], dt[2], z[2], d[2], b[4] = {}, c[4] = {}, y[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        load_states<S>(Q.state + at.n * Q.s_ldn + (at.channel + k) * Q.s_ldc, at.part, Q.states, at.live[k], 0, h[k]);
+    two(Q.x, x);
+    two(Q.dt, dt);
+    if (Q.z.p != nullptr) two(Q.z, z);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int s = at.part * R + r;
+        if (s >= Q.states) continue;
+        b[r] = element(Q.b, at.group * Q.b.ldg + s);
+        c[r] = element(Q.c, at.group * Q.c.ldg + s);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) load_decay<S>(Q, at, k, 0, a2[k]);
+    if (Q.bias != nullptr) {
+        float v[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) v[k] = at.live[k] ? load_param(Q.bias, Q.bias_type, at.channel + k) : 0.0f;
+        bias[0] = pair(v[0], v[1]);
+    }
+    raw[0] = pair(dt[0], dt[1]);
+    raw[1] = pair(0.0f);
+    scan_deltas<false>(Q.softplus, raw, bias, delta, slope);
+    split(delta[0], d[0], d[1]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
         f2 s = pair(0.0f);
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            h[i] = fma2(exp2_fast(pair(d) * a2[i]), h[i], pair(d * x) * pair(b[2 * i], b[2 * i + 1]));
-            s = fma2(pair(c[2 * i], c[2 * i + 1]), h[i], s);
+            h[k][i] = fma2(exp2_fast(pair(d[k]) * a2[k][i]), h[k][i], pair(d[k] * x[k]) * pair(b[2 * i], b[2 * i + 1]));
+            s = fma2(pair(c[2 * i], c[2 * i + 1]), h[k][i], s);
         }
-        y = sum_of(s);
-        store_states<S>(Q.state_out + at.n * Q.so_ldn + at.channel * Q.so_ldc, at.part, Q.states, true, 0, h);
+        y[k] = sum_of(s);
+        store_states<S>(Q.state_out + at.n * Q.so_ldn + (at.channel + k) * Q.so_ldc, at.part, Q.states, at.live[k], 0, h[k]);
+#pragma unroll
+        for (int o = 1; o < P; o *= 2) y[k] += __shfl_xor_sync(0xffffffffu, y[k], o);
+    }
+    if (at.part != 0) return;
+    float gate[2] = {1.0f, 1.0f};
+    if (Q.z.p != nullptr) {
+        f2 g, unused;
+        gate2<false>(pair(z[0], z[1]), g, unused);
+        split(g, gate[0], gate[1]);
     }
 #pragma unroll
-    for (int o = 1; o < P; o *= 2) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (at.live && at.part == 0) {
-        if (Q.d != nullptr) y = fmaf(load_param(Q.d, Q.d_type, at.channel), x, y);
-        if (Q.z.p != nullptr) {
-            f2 gate, slope;
-            gate2<false>(pair(element(Q.z, at.channel)), gate, slope);
-            float g, unused;
-            split(gate, g, unused);
-            y *= g;
-        }
-        static_cast<E *>(const_cast<void *>(Q.y.p))[at.n * Q.y.ldn + at.channel] = from_float<E>(y);
-    }
+    for (int k = 0; k < 2; ++k)
+        if (Q.d != nullptr && at.live[k]) y[k] = fmaf(load_param(Q.d, Q.d_type, at.channel + k), x[k], y[k]);
+    store_two<E>(token_at<E>(Q.y, at.n, 0) + at.channel, false, at.live, y[0] * gate[0], y[1] * gate[1]);
 }
 
 // ---- instances, one translation unit for each element type -----------------------------------
@@ -948,13 +1027,13 @@ struct ScanLaunch {
 };
 // Threads of a block of the gradient: what the tiles of few lanes take of shared
 // memory grows with the channels of a block.
-constexpr int kScanThreads = 128;
-constexpr int grad_threads(int sp) { return sp >= 16 ? 256 : kScanThreads; }
+constexpr int kScanThreads = 64;
+constexpr int grad_threads(int sp) { return sp >= 16 ? 128 : kScanThreads; }
 
 template <class E, int SP>
 ScanLaunch scan_instance(ScanKernel k) {
-    using S = ScanShape<SP, kScanThreads>;
-    using G = ScanShape<SP, grad_threads(SP)>;
+    using S = ScanShape<SP, kScanThreads, 16>;
+    using G = ScanShape<SP, grad_threads(SP), kScanChunk>;
     switch (k) {
     case kMain:
         return {reinterpret_cast<const void *>(&scan_kernel<E, S, kScanMain>), S::THREADS, sizeof(ScanTile<E, S, kScanMain>)};

@@ -127,19 +127,20 @@ int padded_states(int64_t s) {
     while (sp < s) sp *= 2;
     return sp == 2 ? 4 : sp;
 }
-// Segments: as many as give each multiprocessor six blocks, of at least 64 tokens.
-ScanPlan plan_scan(const ScanCall &c, int sms) {
+// Segments: as many as give each multiprocessor 16 blocks (24 in the gradient,
+// whose own kernel has half as many), of at least 64 tokens.
+ScanPlan plan_scan(const ScanCall &c, int sms, bool backward) {
     ScanPlan p;
     p.type = c.x.type;
     p.sp = padded_states(c.states);
     p.per_lane = std::min(p.sp, 4);
     p.lanes = p.sp / p.per_lane;
     const int64_t cpg = c.c / c.groups;
-    p.tiles = static_cast<int>(ceil_div(cpg, kScanThreads / p.lanes));
-    p.grad_tiles = static_cast<int>(ceil_div(cpg, grad_threads(p.sp) / p.lanes));
-    const long long blocks = c.n * c.groups * p.tiles;
-    const long long wanted = std::max(1LL, std::min(ceil_div(6LL * sms, std::max(1LL, blocks)), static_cast<long long>(c.l / 64)));
-    p.seg_len = std::max(1LL, gcb::round_up(ceil_div(c.l, wanted), kScanChunk));
+    p.tiles = static_cast<int>(ceil_div(cpg, 2 * kScanThreads / p.lanes));
+    p.grad_tiles = static_cast<int>(ceil_div(cpg, 2 * grad_threads(p.sp) / p.lanes));
+    const long long blocks = std::max(1LL, static_cast<long long>(c.n) * c.groups * p.tiles);
+    const long long wanted = std::min(ceil_div((backward ? 24LL : 16LL) * sms, blocks), static_cast<long long>(c.l / 64));
+    p.seg_len = std::max(1LL, gcb::round_up(ceil_div(c.l, std::max(1LL, wanted)), 16));
     p.segs = static_cast<int>(std::max(1LL, ceil_div(c.l, p.seg_len)));
     p.blocks = blocks * p.segs;
     return p;
@@ -259,10 +260,9 @@ int gc_b200_selective_scan_sizes(const gc_b200_scan_args *q, uint64_t *workspace
     if (c.n == 0) return gc_error(GC_OK, "");
     DeviceFacts facts;
     if ((st = current_facts(facts)) != GC_OK) return st;
-    const ScanPlan plan = plan_scan(c, facts.sms);
-    *workspace = space_of(c, plan, false).total();
+    *workspace = space_of(c, plan_scan(c, facts.sms, false), false).total();
     *kept = kept_bytes_of(c);
-    *backward_workspace = space_of(c, plan, true).total();
+    *backward_workspace = space_of(c, plan_scan(c, facts.sms, true), true).total();
     return gc_error(GC_OK, "");
 } catch (...) {
     return internal_error();
@@ -290,7 +290,7 @@ int gc_b200_selective_scan(const gc_b200_scan_args *q, gc_tensor *y, gc_tensor *
     if (c.l == 0 && state_out == nullptr) return gc_error(GC_OK, "");
     DeviceFacts facts;
     if ((st = device_facts(dev, facts)) != GC_OK) return st;
-    ScanPlan plan = plan_scan(c, facts.sms);
+    ScanPlan plan = plan_scan(c, facts.sms, false);
     const ScanSpace space = space_of(c, plan, false);
     if ((st = check_workspace(workspace, workspace_bytes, space.total())) != GC_OK) return st;
     if (space.total() != 0 && (st = check_device_memory(workspace, q->x->device_index, dev)) != GC_OK) return st;
@@ -363,7 +363,7 @@ int gc_b200_selective_scan_backward(const gc_b200_scan_args *q, const gc_tensor 
     }
     DeviceFacts facts;
     if ((st = device_facts(dev, facts)) != GC_OK) return st;
-    ScanPlan plan = plan_scan(c, facts.sms);
+    ScanPlan plan = plan_scan(c, facts.sms, true);
     const ScanSpace space = space_of(c, plan, true);
     if ((st = check_workspace(workspace, workspace_bytes, space.total())) != GC_OK) return st;
     if ((st = check_device_memory(workspace, q->x->device_index, dev)) != GC_OK) return st;
@@ -463,7 +463,7 @@ int gc_b200_selective_scan_step(const gc_b200_scan_args *q, gc_tensor *y, gc_ten
         return st;
     DeviceFacts facts;
     if ((st = device_facts(dev, facts)) != GC_OK) return st;
-    const ScanPlan plan = plan_scan(c, facts.sms);
+    const ScanPlan plan = plan_scan(c, facts.sms, false);
     ScanParams P{};
     fill(P, q, c, plan, true);
     P.y = tokens_of(c.y, true);

@@ -263,7 +263,7 @@ def test_infinities_stay_in_their_channel(native, torch_cuda):
 @pytest.mark.parametrize('segments', [False, True])
 def test_long_sequences(native, torch_cuda, segments):
     """Two thousand tokens with decays close to 1, whose errors add up."""
-    n, ch = (1, 8) if segments else (900, 8)
+    n, ch = (1, 8) if segments else (4000, 8)
     v = make(n, 2048, ch, 4, 1, torch.float32, 11)
     few = {k: v[k][:2] if v[k].shape[0] == n and k not in ('a', 'd', 'dt_bias') else v[k] for k in v}
     ref = ScanReference(*(few[k] for k in NAMES[:8]), True, few['state']).backward(few['dy'], few['dlast'])
