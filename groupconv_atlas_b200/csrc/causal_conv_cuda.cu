@@ -127,6 +127,12 @@ const void *conv_kernel(ConvKernel k, int type, bool vec, int taps, int act) {
     return vec ? conv_typed<float, 4>(k, taps, act) : conv_typed<float, 1>(k, taps, act);
 }
 
+// Dynamic shared memory of a kernel's ring.
+size_t ring_bytes(int type, bool vec) { return static_cast<size_t>(kConvRing) * kConvThreads * (vec ? 4 : 1) * elem_size(type); }
+int opt_in_ring(int dev, const void *fn, size_t bytes, const DeviceFacts &facts) {
+    return bytes > 40 * 1024 ? opt_in_smem(dev, fn, facts.smem_optin - 8192) : GC_OK;
+}
+
 // Tokens of a thread: as many as leave four warps for each quarter of a
 // multiprocessor, 8 to 64.
 int stretch_of(const ConvCall &call, int v, int sms) {
@@ -230,8 +236,10 @@ int gc_b200_causal_conv(const gc_tensor *x, const gc_tensor *weight, const gc_te
     const wide blocks = (static_cast<wide>(call.n) * P.segs * P.vcols + kConvThreads - 1) / kConvThreads;
     if (blocks > INT32_MAX) return gc_error(GC_UNSUPPORTED, "more work than a grid has blocks");
     void *args[] = {&P};
-    const cudaError_t e = launch_pdl(conv_kernel(kForward, call.x.type, vec, P.taps, activation),
-                                     dim3(static_cast<unsigned>(blocks)), dim3(kConvThreads), args, 0,
+    const void *fn = conv_kernel(kForward, call.x.type, vec, P.taps, activation);
+    const size_t smem = ring_bytes(call.x.type, vec);
+    if ((st = opt_in_ring(dev, fn, smem, facts)) != GC_OK) return st;
+    const cudaError_t e = launch_pdl(fn, dim3(static_cast<unsigned>(blocks)), dim3(kConvThreads), args, smem,
                                      reinterpret_cast<cudaStream_t>(stream));
     return launched(e, PlanRecord::kSequence, "causal_conv", static_cast<long long>(blocks), kConvThreads, vec ? 1 : 0,
                     P.vcols, P.stretch, P.segs, 1);
@@ -308,8 +316,10 @@ int gc_b200_causal_conv_backward(const gc_tensor *dy, const gc_tensor *x, const 
     P.part = sums ? static_cast<float *>(workspace) : nullptr;
     void *args[] = {&P};
     const long long grid = plan.tiles * plan.blocks_y;
-    e = launch_pdl(conv_kernel(kBackward, call.x.type, vec, P.taps, activation), dim3(static_cast<unsigned>(grid)),
-                   dim3(kConvThreads), args, 0, s);
+    const void *fn = conv_kernel(kBackward, call.x.type, vec, P.taps, activation);
+    const size_t smem = ring_bytes(call.x.type, vec);
+    if ((st = opt_in_ring(dev, fn, smem, facts)) != GC_OK) return st;
+    e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(kConvThreads), args, smem, s);
     if (e == cudaSuccess && sums) {
         SumParams S{};
         S.part = P.part;

@@ -139,9 +139,44 @@ __device__ __forceinline__ Lanes<V> conv_at(const ConvSeqParams &P, const Lanes<
     return v;
 }
 
+// A thread's groups at p, p + step, .. copied ahead through a ring in shared memory
+// that is its own: D copies under way, no barrier, no registers.  The ring holds
+// kConvRing groups of every thread.
+constexpr int kConvRing = 16;
+template <class T, int V>
+struct ConvRing {
+    static constexpr bool kCopies = Group<T, V>::kBytes >= 4;
+    Group<T, V> *mine;
+    __device__ __forceinline__ explicit ConvRing(char *space) : mine(reinterpret_cast<Group<T, V> *>(space) + threadIdx.x) {}
+    __device__ __forceinline__ void copy(int slot, const T *p) const {
+        const uint32_t dst = smem_addr(mine + slot * kConvThreads);
+        if constexpr (Group<T, V>::kBytes == 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(p) : "memory");
+        else if constexpr (Group<T, V>::kBytes == 8)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(p) : "memory");
+        else if constexpr (kCopies)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(p) : "memory");
+    }
+    // What cannot be copied asynchronously (two bytes): `count` groups at once, for
+    // slots first, first + every, ..
+    template <int MOST>
+    __device__ __forceinline__ void fill(int first, int every, const T *p, long long step, int count) const {
+        if constexpr (!kCopies) {
+            Group<T, V> g[MOST];
+#pragma unroll
+            for (int k = 0; k < MOST; ++k)
+                if (k < count) g[k] = load_group<T, V>(p + k * step);
+#pragma unroll
+            for (int k = 0; k < MOST; ++k)
+                if (k < count) mine[(first + k * every) * kConvThreads] = g[k];
+        }
+    }
+    __device__ __forceinline__ Lanes<V> at(int slot) const { return lanes_of_group<T, V>(mine[slot * kConvThreads]); }
+};
+
 template <class T, int V, int KT, int ACT>
 __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const __grid_constant__ ConvSeqParams P) {
-    constexpr int U = 8;
+    extern __shared__ __align__(16) char space[];
     griddep_wait();
     griddep_launch_dependents();
     const long long id = static_cast<long long>(blockIdx.x) * kConvThreads + threadIdx.x;
@@ -153,28 +188,34 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const __grid_
     Lanes<V> w[KT], window[KT - 1];
     T *y = static_cast<T *>(P.y) + n * P.y_ldn + c0;
     if (t0 < end) {
+        const ConvRing<T, V> ring(space);
+        const int count = static_cast<int>(end - t0);
+        const T *x = static_cast<const T *>(P.x) + n * P.x_ldn + t0 * P.x_ldt + c0;
+#pragma unroll
+        for (int k = 0; k < kConvRing; ++k, x += P.x_ldt) {
+            if (k < count) ring.copy(k, x);
+            cp_async_commit();
+        }
         load_taps<V, KT>(P, c0, w);
         const Lanes<V> bias = load_bias<V>(P, c0);
 #pragma unroll
         for (int k = 0; k < KT - 1; ++k) window[k] = k >= KT - P.taps ? input_at<T, V>(P, n, t0 - (KT - 1) + k, c0) : no_lanes<V>();
-        const T *x = static_cast<const T *>(P.x) + n * P.x_ldn + c0;
-        for (long long t = t0; t < end; t += U) {
-            Group<T, V> raw[U];
+        T *out = y + t0 * P.y_ldt;
+#pragma unroll 4
+        for (int k = 0; k < count; ++k, x += P.x_ldt, out += P.y_ldt) {
+            cp_async_wait<kConvRing - 1>();
+            const int slot = k % kConvRing;
+            if (slot == 0) ring.template fill<kConvRing>(0, 1, x - kConvRing * P.x_ldt, P.x_ldt, count - k);
+            const Lanes<V> cur = ring.at(slot);
+            if (k + kConvRing < count) ring.copy(slot, x);
+            cp_async_commit();
+            Lanes<V> v = conv_at<V, KT, ACT>(P, w, window, cur, bias);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (t + u < end) raw[u] = load_group<T, V>(x + (t + u) * P.x_ldt);
+            for (int i = 0; i < Lanes<V>::kPairs; ++i) v.p[i] = activate<ACT>(P.act, v.p[i]);
+            store_group<T, V>(out, v);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (t + u < end) {
-                    const Lanes<V> cur = lanes_of_group<T, V>(raw[u]);
-                    Lanes<V> v = conv_at<V, KT, ACT>(P, w, window, cur, bias);
-#pragma unroll
-                    for (int i = 0; i < Lanes<V>::kPairs; ++i) v.p[i] = activate<ACT>(P.act, v.p[i]);
-                    store_group<T, V>(y + (t + u) * P.y_ldt, v);
-#pragma unroll
-                    for (int k = 0; k + 1 < KT - 1; ++k) window[k] = window[k + 1];
-                    window[KT - 2] = cur;
-                }
+            for (int i = 0; i + 1 < KT - 1; ++i) window[i] = window[i + 1];
+            window[KT - 2] = cur;
         }
     }
     for (long long t = max(end, t0); t < t1; ++t) store_group<T, V>(y + t * P.y_ldt, no_lanes<V>());
@@ -219,8 +260,9 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(const __
 // more.  dw and dbias add up over a stretch, then over stretches, then over the
 // workers of the block in a fixed order.
 template <class T, int V, int KT, int ACT>
-__global__ void __launch_bounds__(kConvThreads) causal_conv_grad_kernel(const __grid_constant__ ConvSeqParams P) {
-    constexpr int U = 4, NP = Lanes<V>::kPairs;
+__global__ void __launch_bounds__(kConvThreads, KT <= 4 ? 2 : 1) causal_conv_grad_kernel(const __grid_constant__ ConvSeqParams P) {
+    constexpr int NP = Lanes<V>::kPairs, D = kConvRing / 2;  // D: tokens under way, of x and of dy
+    extern __shared__ __align__(16) char space[];
     __shared__ float sm[kConvThreads * V];
     griddep_wait();
     griddep_launch_dependents();
@@ -241,75 +283,94 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_grad_kernel(const __
             const long long len = length_of(P.lengths, n, P.l), t0 = seg * P.stretch, t1 = min(P.l, t0 + P.stretch);
             const T *x = static_cast<const T *>(P.x) + n * P.x_ldn + c0, *dy = static_cast<const T *>(P.dy) + n * P.dy_ldn + c0;
             T *dx = static_cast<T *>(P.y) + n * P.y_ldn + c0;
+            const ConvRing<T, V> ring(space);
+            const int count = static_cast<int>(t1 + KT - 1 - t0);                                 // tokens to walk over
+            const int inside = static_cast<int>(max(0LL, min(len, t1 + KT - 1) - t0));  // of those, in the sequence
+            const T *px = x + t0 * P.x_ldt, *pg = dy + t0 * P.dy_ldt;
+#pragma unroll
+            for (int k = 0; k < D; ++k, px += P.x_ldt, pg += P.dy_ldt) {
+                if (k < inside) {
+                    ring.copy(2 * k, px);
+                    ring.copy(2 * k + 1, pg);
+                }
+                cp_async_commit();
+            }
             Lanes<V> xw[KT - 1], gw[KT - 1], dw1[KT], db1 = no_lanes<V>();
 #pragma unroll
             for (int k = 0; k < KT; ++k) dw1[k] = no_lanes<V>();
 #pragma unroll
             for (int k = 0; k < KT - 1; ++k) {
-                xw[k] = k >= pad && t0 < len ? input_at<T, V>(P, n, t0 - (KT - 1) + k, c0) : no_lanes<V>();
+                xw[k] = k >= pad && inside > 0 ? input_at<T, V>(P, n, t0 - (KT - 1) + k, c0) : no_lanes<V>();
                 gw[k] = no_lanes<V>();
             }
-            for (long long t = t0; t < t1 + KT - 1; t += U) {
-                Group<T, V> rx[U], rg[U];
+            const int first = seg == 0 ? KT - P.taps : KT - 1;  // from here on a finished place is the stretch's, or the state's
+            T *out = dx + (t0 - (KT - 1)) * P.y_ldt;
+            for (int k = 0; k < count; ++k, px += P.x_ldt, pg += P.dy_ldt, out += P.y_ldt) {
+                cp_async_wait<D - 1>();
+                const int slot = k % D * 2;
+                if (slot == 0) {
+                    ring.template fill<D>(0, 2, px - D * P.x_ldt, P.x_ldt, inside - k);
+                    ring.template fill<D>(1, 2, pg - D * P.dy_ldt, P.dy_ldt, inside - k);
+                }
+                Lanes<V> cur = no_lanes<V>(), g = no_lanes<V>();
+                if (k < inside) {
+                    cur = ring.at(slot);
+                    g = ring.at(slot + 1);
+                }
+                if (k + D < inside) {
+                    ring.copy(slot, px);
+                    ring.copy(slot + 1, pg);
+                }
+                cp_async_commit();
+                if (k < inside) {
+                    if (ACT != kActNone) {
+                        const Lanes<V> v = conv_at<V, KT, ACT>(P, w, xw, cur, bias);
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (t + u < len && t + u < t1 + KT - 1) {
-                        rx[u] = load_group<T, V>(x + (t + u) * P.x_ldt);
-                        rg[u] = load_group<T, V>(dy + (t + u) * P.dy_ldt);
+                        for (int i = 0; i < NP; ++i) g.p[i] = activate_grad<ACT>(P.act, v.p[i], g.p[i]);
                     }
+                    if (k < t1 - t0) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const long long at = t + u, s = at - (KT - 1);
-                    if (at >= t1 + KT - 1) break;
-                    Lanes<V> cur = no_lanes<V>(), g = no_lanes<V>();
-                    if (at < len) {
-                        cur = lanes_of_group<T, V>(rx[u]);
-                        g = lanes_of_group<T, V>(rg[u]);
-                        if (ACT != kActNone) {
-                            const Lanes<V> v = conv_at<V, KT, ACT>(P, w, xw, cur, bias);
+                        for (int i = 0; i < NP; ++i) {
+                            db1.p[i] = db1.p[i] + g.p[i];
 #pragma unroll
-                            for (int i = 0; i < NP; ++i) g.p[i] = activate_grad<ACT>(P.act, v.p[i], g.p[i]);
-                        }
-                        if (at < t1) {
-#pragma unroll
-                            for (int i = 0; i < NP; ++i) {
-                                db1.p[i] = db1.p[i] + g.p[i];
-#pragma unroll
-                                for (int k = 0; k < KT; ++k)
-                                    if (k >= pad)
-                                        dw1[k].p[i] = fma2(g.p[i], k < KT - 1 ? xw[k < KT - 1 ? k : 0].p[i] : cur.p[i], dw1[k].p[i]);
-                            }
+                            for (int j = 0; j < KT; ++j)
+                                if (j >= pad)
+                                    dw1[j].p[i] = fma2(g.p[i], j < KT - 1 ? xw[j < KT - 1 ? j : 0].p[i] : cur.p[i], dw1[j].p[i]);
                         }
                     }
-                    if (s >= t0 || (seg == 0 && s >= 1 - P.taps)) {
-                        Lanes<V> d = no_lanes<V>();
+                }
+                if (k >= first) {
+                    const long long s = t0 + k - (KT - 1);
+                    Lanes<V> d = no_lanes<V>();
+                    if (s < len) {
 #pragma unroll
-                        for (int k = 0; k < KT; ++k)
-                            if (k >= pad && s < len) {
+                        for (int j = 0; j < KT; ++j)
+                            if (j >= pad) {
 #pragma unroll
                                 for (int i = 0; i < NP; ++i)
-                                    d.p[i] = fma2(w[k].p[i], k == 0 ? g.p[i] : gw[k == 0 ? 0 : KT - 1 - k].p[i], d.p[i]);
+                                    d.p[i] = fma2(w[j].p[i], j == 0 ? g.p[i] : gw[j == 0 ? 0 : KT - 1 - j].p[i], d.p[i]);
                             }
                         const long long j = s + P.taps - 1 - len;  // its place in the last state
-                        if (P.dstate != nullptr && j >= 0 && s < len) {
+                        if (P.dstate != nullptr && j >= 0) {
                             const Lanes<V> e = lanes_of_group<T, V>(load_group<T, V>(
                                 static_cast<const T *>(P.dstate) + n * P.ds_ldn + j * P.ds_ldt + c0));
 #pragma unroll
                             for (int i = 0; i < NP; ++i) d.p[i] = d.p[i] + e.p[i];
                         }
-                        if (s >= 0) store_group<T, V>(dx + s * P.y_ldt, d);
-                        else if (P.state_out != nullptr)
-                            store_group<T, V>(static_cast<T *>(P.state_out) + n * P.so_ldn + (s + P.taps - 1) * P.so_ldt + c0, d);
                     }
-#pragma unroll
-                    for (int k = 0; k + 1 < KT - 1; ++k) {
-                        xw[k] = xw[k + 1];
-                        gw[k] = gw[k + 1];
-                    }
-                    xw[KT - 2] = cur;
-                    gw[KT - 2] = g;
+                    if (s >= 0) store_group<T, V>(out, d);
+                    else if (P.state_out != nullptr)
+                        store_group<T, V>(static_cast<T *>(P.state_out) + n * P.so_ldn + (s + P.taps - 1) * P.so_ldt + c0, d);
                 }
+#pragma unroll
+                for (int i = 0; i + 1 < KT - 1; ++i) {
+                    xw[i] = xw[i + 1];
+                    gw[i] = gw[i + 1];
+                }
+                xw[KT - 2] = cur;
+                gw[KT - 2] = g;
             }
+            cp_async_wait<0>();
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 db.p[i] = db.p[i] + db1.p[i];

@@ -21,6 +21,7 @@ struct LayerNormParams {
     int team;            // threads that take a row
     const void *gamma, *beta;
     int gamma_type, beta_type;
+    int aligned;         // whether both can be read 16 bytes at a time
     float eps;
     float2 *stats;       // mean and rstd of each row; nullable in the forward pass
     float *part;         // gradient: dgamma and dbeta of each block, [block][2][c]; NULL where neither is wanted
@@ -54,9 +55,48 @@ __device__ __forceinline__ void team_sums(float (&v)[N], int team, float *buf, i
     }
 }
 
+// A parameter's values at a vector's columns; 16-byte accesses where they are aligned.
+template <int V>
+__device__ __forceinline__ Lanes<V> row_params(const void *p, int type, bool aligned, int i, float none) {
+    float v[V];
+    if constexpr (V == 8) {
+        if (p != nullptr && aligned) {
+            if (type == kElemF32) {
+                const float4 a = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i));
+                const float4 b = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i) + 1);
+                Lanes<V> r;
+                r.p[0] = pair(a.x, a.y);
+                r.p[1] = pair(a.z, a.w);
+                r.p[2] = pair(b.x, b.y);
+                r.p[3] = pair(b.z, b.w);
+                return r;
+            }
+            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i));
+            return type == kElemBF16 ? unpack_lanes<__nv_bfloat16, V>(u, static_cast<const __nv_bfloat16 *>(nullptr))
+                                     : unpack_lanes<__half, V>(u, static_cast<const __half *>(nullptr));
+        }
+    } else if constexpr (V == 4) {
+        if (p != nullptr && aligned)
+            return unpack_lanes<float, V>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const float *>(p) + i)),
+                                          static_cast<const float *>(nullptr));
+    }
+    load_params<V>(p, type, i, none, v);
+    return lanes_of<V>(v);
+}
+template <int V>
+__device__ __forceinline__ float lanes_sum(const Lanes<V> &l) {
+    f2 s = l.p[0];
+#pragma unroll
+    for (int i = 1; i < Lanes<V>::kPairs; ++i) s = s + l.p[i];
+    float a, b;
+    split(s, a, b);
+    return a + b;
+}
+
 // NV vectors a thread and row, ROWS rows at a time.
 template <class T, int V, int NV, int ROWS>
 __global__ void __launch_bounds__(kRowMost) layer_norm_kernel(const __grid_constant__ LayerNormParams P) {
+    constexpr int NP = Lanes<V>::kPairs;
     __shared__ float buf[2 * (kRowMost / 32) * ROWS];
     griddep_wait();
     griddep_launch_dependents();
@@ -71,7 +111,6 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_kernel(const __grid_const
         for (int r = 0; r < ROWS; ++r) {
             const long long row = first + team + r * all;
             const T *src = static_cast<const T *>(P.x) + row * P.x_ld;
-            s[r] = 0.0f;
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int v = lane + j * P.team;
@@ -80,30 +119,29 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_kernel(const __grid_const
         }
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            const long long row = first + team + r * all;
+            s[r] = 0.0f;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
-                if (row < P.rows && lane + j * P.team < P.vcols) {
-                    float e[V];
-                    values_of<V>(lanes_of_raw<T, V>(raw[r][j]), e);
-#pragma unroll
-                    for (int k = 0; k < V; ++k) s[r] += e[k];
-                }
+                if (first + team + r * all < P.rows && lane + j * P.team < P.vcols) s[r] += lanes_sum<V>(lanes_of_raw<T, V>(raw[r][j]));
         }
         team_sums<ROWS>(s, P.team, buf, turn);
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            const long long row = first + team + r * all;
             s[r] *= inv;
-            q[r] = 0.0f;
+            f2 sum = pair(0.0f);
 #pragma unroll
             for (int j = 0; j < NV; ++j)
-                if (row < P.rows && lane + j * P.team < P.vcols) {
-                    float e[V];
-                    values_of<V>(lanes_of_raw<T, V>(raw[r][j]), e);
+                if (first + team + r * all < P.rows && lane + j * P.team < P.vcols) {
+                    const Lanes<V> e = lanes_of_raw<T, V>(raw[r][j]);
 #pragma unroll
-                    for (int k = 0; k < V; ++k) q[r] = fmaf(e[k] - s[r], e[k] - s[r], q[r]);
+                    for (int i = 0; i < NP; ++i) {
+                        const f2 d = e.p[i] + (V == 1 ? pair(-s[r], 0.0f) : pair(-s[r]));
+                        sum = fma2(d, d, sum);
+                    }
                 }
+            float a, b;
+            split(sum, a, b);
+            q[r] = a + b;
         }
         team_sums<ROWS>(q, P.team, buf, turn);
 #pragma unroll
@@ -112,18 +150,17 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_kernel(const __grid_const
         for (int j = 0; j < NV; ++j) {
             const int v = lane + j * P.team;
             if (v >= P.vcols) continue;
-            float gamma[V], beta[V];
-            load_params<V>(P.gamma, P.gamma_type, static_cast<long long>(v) * V, 1.0f, gamma);
-            load_params<V>(P.beta, P.beta_type, static_cast<long long>(v) * V, 0.0f, beta);
+            const Lanes<V> gamma = row_params<V>(P.gamma, P.gamma_type, P.aligned, v * V, 1.0f);
+            const Lanes<V> beta = row_params<V>(P.beta, P.beta_type, P.aligned, v * V, 0.0f);
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 const long long row = first + team + r * all;
                 if (row >= P.rows) continue;
-                float e[V];
-                values_of<V>(lanes_of_raw<T, V>(raw[r][j]), e);
+                Lanes<V> e = lanes_of_raw<T, V>(raw[r][j]);
 #pragma unroll
-                for (int k = 0; k < V; ++k) e[k] = fmaf((e[k] - s[r]) * q[r], gamma[k], beta[k]);
-                store_elems<T, V>(static_cast<T *>(P.y) + row * P.y_ld + static_cast<long long>(v) * V, e);
+                for (int i = 0; i < NP; ++i)
+                    e.p[i] = fma2((e.p[i] + pair(-s[r])) * pair(q[r]), gamma.p[i], beta.p[i]);
+                store_lanes<T, V>(static_cast<T *>(P.y) + row * P.y_ld + static_cast<long long>(v) * V, e);
             }
         }
         if (P.stats != nullptr && lane == 0) {
@@ -140,70 +177,93 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_kernel(const __grid_const
 // their columns in registers, over at most 64 rows (the launch sees to that); at
 // the end the block joins its teams in a fixed order.  Dynamic shared memory:
 // [warps][2][c] values where a row takes at most a warp.
-template <class T, int V, int NV>
+template <class T, int V, int NV, int ROWS>
 __global__ void __launch_bounds__(kRowMost) layer_norm_grad_kernel(const __grid_constant__ LayerNormParams P) {
+    constexpr int NP = Lanes<V>::kPairs;
     extern __shared__ float joined[];
-    __shared__ float buf[2 * (kRowMost / 32) * 2];
+    __shared__ float buf[2 * (kRowMost / 32) * 2 * ROWS];
     griddep_wait();
     griddep_launch_dependents();
     const int teams = blockDim.x / P.team, team = threadIdx.x / P.team, lane = threadIdx.x - team * P.team;
     const long long all = static_cast<long long>(gridDim.x) * teams;
     const float inv = 1.0f / static_cast<float>(P.c);
-    float gamma[NV][V], dgamma[NV][V], dbeta[NV][V];
+    Lanes<V> gamma[NV], sum_g[NV], sum_b[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) gamma[j][k] = dgamma[j][k] = dbeta[j][k] = 0.0f;
         const int v = lane + j * P.team;
-        if (v < P.vcols) load_params<V>(P.gamma, P.gamma_type, static_cast<long long>(v) * V, 1.0f, gamma[j]);
+        if (v < P.vcols) gamma[j] = row_params<V>(P.gamma, P.gamma_type, P.aligned, v * V, 1.0f);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            sum_g[j].p[i] = sum_b[j].p[i] = pair(0.0f);
+            if (v >= P.vcols) gamma[j].p[i] = pair(0.0f);
+        }
     }
     int turn = 0;
-    for (long long first = static_cast<long long>(blockIdx.x) * teams; first < P.rows; first += all) {
-        const long long row = first + team;
-        const bool live = row < P.rows;
-        Raw<T, V> rx[NV], rg[NV];
+    for (long long first = static_cast<long long>(blockIdx.x) * teams; first < P.rows; first += all * ROWS) {
+        Raw<T, V> rx[ROWS][NV], rg[ROWS][NV];
+        float2 st[ROWS];
+        float sums[2 * ROWS];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int v = lane + j * P.team;
-            if (live && v < P.vcols) {
-                rx[j] = load_raw<T, V>(static_cast<const T *>(P.x) + row * P.x_ld + static_cast<long long>(v) * V);
-                rg[j] = load_raw<T, V>(static_cast<const T *>(P.dy) + row * P.dy_ld + static_cast<long long>(v) * V);
-            }
-        }
-        const float2 st = live ? P.stats[row] : make_float2(0.0f, 0.0f);
-        float sums[2] = {0.0f, 0.0f};
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = first + team + r * all;
+            st[r] = row < P.rows ? P.stats[row] : make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (live && lane + j * P.team < P.vcols) {
-                float e[V], d[V];
-                values_of<V>(lanes_of_raw<T, V>(rx[j]), e);
-                values_of<V>(lanes_of_raw<T, V>(rg[j]), d);
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const float xhat = (e[k] - st.x) * st.y, g = d[k] * gamma[j][k];
-                    sums[0] += g;
-                    sums[1] = fmaf(g, xhat, sums[1]);
-                    dgamma[j][k] = fmaf(d[k], xhat, dgamma[j][k]);
-                    dbeta[j][k] += d[k];
+            for (int j = 0; j < NV; ++j) {
+                const long long v = lane + j * P.team;
+                if (row < P.rows && v < P.vcols) {
+                    rx[r][j] = load_raw<T, V>(static_cast<const T *>(P.x) + row * P.x_ld + v * V);
+                    rg[r][j] = load_raw<T, V>(static_cast<const T *>(P.dy) + row * P.dy_ld + v * V);
                 }
             }
-        team_sums<2>(sums, P.team, buf, turn);
-        const float m1 = sums[0] * inv, m2 = sums[1] * inv;
+        }
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int v = lane + j * P.team;
-            if (live && v < P.vcols) {
-                float e[V], d[V];
-                values_of<V>(lanes_of_raw<T, V>(rx[j]), e);
-                values_of<V>(lanes_of_raw<T, V>(rg[j]), d);
+        for (int r = 0; r < ROWS; ++r) {
+            f2 s1 = pair(0.0f), s2 = pair(0.0f);
 #pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const float xhat = (e[k] - st.x) * st.y;
-                    e[k] = st.y * (fmaf(d[k], gamma[j][k], -m1) - xhat * m2);
+            for (int j = 0; j < NV; ++j)
+                if (first + team + r * all < P.rows && lane + j * P.team < P.vcols) {
+                    const Lanes<V> e = lanes_of_raw<T, V>(rx[r][j]), d = lanes_of_raw<T, V>(rg[r][j]);
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) {
+                        const f2 xhat = (e.p[i] + pair(-st[r].x)) * pair(st[r].y), g = d.p[i] * gamma[j].p[i];
+                        s1 = s1 + g;
+                        s2 = fma2(g, xhat, s2);
+                        sum_g[j].p[i] = fma2(d.p[i], xhat, sum_g[j].p[i]);
+                        sum_b[j].p[i] = sum_b[j].p[i] + d.p[i];
+                    }
                 }
-                store_elems<T, V>(static_cast<T *>(P.y) + row * P.y_ld + static_cast<long long>(v) * V, e);
+            float a, b;
+            split(s1, a, b);
+            sums[2 * r] = V == 1 ? a : a + b;
+            split(s2, a, b);
+            sums[2 * r + 1] = V == 1 ? a : a + b;
+        }
+        team_sums<2 * ROWS>(sums, P.team, buf, turn);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = first + team + r * all;
+            const f2 m1 = pair(-sums[2 * r] * inv), m2 = pair(-sums[2 * r + 1] * inv);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const long long v = lane + j * P.team;
+                if (row < P.rows && v < P.vcols) {
+                    const Lanes<V> e = lanes_of_raw<T, V>(rx[r][j]), d = lanes_of_raw<T, V>(rg[r][j]);
+                    Lanes<V> o;
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) {
+                        const f2 xhat = (e.p[i] + pair(-st[r].x)) * pair(st[r].y);
+                        o.p[i] = pair(st[r].y) * fma2(xhat, m2, fma2(d.p[i], gamma[j].p[i], m1));
+                    }
+                    store_lanes<T, V>(static_cast<T *>(P.y) + row * P.y_ld + v * V, o);
+                }
             }
         }
+    }
+    float dgamma[NV][V], dbeta[NV][V];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        values_of<V>(sum_g[j], dgamma[j]);
+        values_of<V>(sum_b[j], dbeta[j]);
     }
     if (P.part == nullptr) return;
     float *out = P.part + static_cast<long long>(blockIdx.x) * 2 * P.c;

@@ -77,23 +77,41 @@ struct RowPlan {
 
 const char *const kDenseParams = "parameters must be dense";
 
-// One vector of a row for each thread, two or four where a row would need more
-// than a block; rows of at most a warp share a block.  Single elements are taken
-// four or sixteen a thread.
+// Vectors of a row for each thread, by how many of the threads' places stay empty,
+// then by the longest run of a thread: sums between threads cost more than those
+// in one (96 columns FP32 in teams of 8 with three vectors, 32 with one: 24 us and
+// 15 at 100352 rows).  A team of up to 32 threads has no barriers; the gradient,
+// which holds its columns' sums in registers, goes over to whole blocks earlier.
+// Single elements are taken four or sixteen (backwards eight) a thread.
 void plan_rows(int c, int type, bool vec, bool backward, RowPlan &p) {
     p.type = type;
     p.vec = vec;
     p.v = !vec ? 1 : type == kElemF32 ? 4 : 8;
     const long long vcols = c / p.v;
-    const int low = vec ? 1 : 4, high = !vec ? 16 : backward && p.v == 8 ? 2 : 4;
-    p.nv = low;
-    if (vec && !backward) {  // short rows stay within a warp, which has no barriers
-        if (vcols > 32 && vcols <= 64) p.nv = 2;
-        else if (vcols > 64 && vcols <= 128) p.nv = 4;
-    } else if (vec && vcols > 32 && vcols <= 64) {
-        p.nv = 2;
+    p.threads = kRowThreads;
+    if (vec) {
+        const int most = backward ? (p.v == 8 ? 3 : 4) : 8;
+        long long best = 0;
+        for (const int nv : {8, 6, 4, 3, 2, 1}) {
+            if (nv > most) continue;
+            int team = 1;
+            while (static_cast<long long>(team) * nv < vcols) team *= 2;
+            if (team > 32) continue;
+            if (best == 0 || static_cast<long long>(team) * nv < best) {
+                best = static_cast<long long>(team) * nv;
+                p.nv = nv;
+                p.team = team;
+            }
+        }
+        if (best != 0) {
+            if (backward) p.smem = static_cast<size_t>(p.threads / 32) * 2 * c * sizeof(float);
+            return;
+        }
+        p.nv = backward ? 1 : 4;
+        while (p.nv < (backward ? (p.v == 8 ? 2 : 4) : 8) && ceil_div(vcols, p.nv) > kRowMost) p.nv *= 2;
+    } else {
+        p.nv = ceil_div(vcols, 4) <= kRowMost ? 4 : backward ? 8 : 16;
     }
-    while (p.nv < high && ceil_div(vcols, p.nv) > kRowMost) p.nv *= vec ? 2 : 4;
     const long long lanes = ceil_div(vcols, p.nv);
     p.whole = lanes > kRowMost;
     if (p.whole) {
@@ -101,34 +119,42 @@ void plan_rows(int c, int type, bool vec, bool backward, RowPlan &p) {
     } else if (lanes > 32) {
         p.team = p.threads = static_cast<int>(round_up(lanes, 32));
     } else {
-        p.threads = kRowThreads;
         for (p.team = 1; p.team < lanes;) p.team *= 2;
+        if (backward) p.smem = static_cast<size_t>(p.threads / 32) * 2 * c * sizeof(float);
     }
-    if (backward && !p.whole && p.team <= 32) p.smem = static_cast<size_t>(p.threads / 32) * 2 * c * sizeof(float);
 }
 
 template <class T, int V>
 const void *forward_typed(int nv) {
-    if constexpr (V == 1)
+    if constexpr (V == 1) {
         return nv == 4 ? reinterpret_cast<const void *>(&layer_norm_kernel<T, 1, 4, 2>)
                        : reinterpret_cast<const void *>(&layer_norm_kernel<T, 1, 16, 1>);
-    else
-        return nv == 1   ? reinterpret_cast<const void *>(&layer_norm_kernel<T, V, 1, 4>)
-               : nv == 2 ? reinterpret_cast<const void *>(&layer_norm_kernel<T, V, 2, 2>)
-                         : reinterpret_cast<const void *>(&layer_norm_kernel<T, V, 4, 1>);
+    } else {
+        switch (nv) {
+        case 1: return reinterpret_cast<const void *>(&layer_norm_kernel<T, V, 1, 4>);
+        case 2: return reinterpret_cast<const void *>(&layer_norm_kernel<T, V, 2, 2>);
+        case 3: return reinterpret_cast<const void *>(&layer_norm_kernel<T, V, 3, 2>);
+        case 4: return reinterpret_cast<const void *>(&layer_norm_kernel<T, V, 4, 1>);
+        case 6: return reinterpret_cast<const void *>(&layer_norm_kernel<T, V, 6, 1>);
+        default: return reinterpret_cast<const void *>(&layer_norm_kernel<T, V, 8, 1>);
+        }
+    }
 }
 template <class T, int V>
 const void *backward_typed(int nv) {
-    if constexpr (V == 1)
-        return nv == 4 ? reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, 1, 4>)
-                       : reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, 1, 16>);
-    else if constexpr (V == 8)
-        return nv == 1 ? reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, V, 1>)
-                       : reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, V, 2>);
-    else
-        return nv == 1   ? reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, V, 1>)
-               : nv == 2 ? reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, V, 2>)
-                         : reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, V, 4>);
+    if constexpr (V == 1) {
+        return nv == 4 ? reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, 1, 4, 2>)
+                       : reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, 1, 8, 1>);
+    } else {
+        switch (nv) {
+        case 1: return reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, V, 1, 2>);
+        case 2: return reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, V, 2, 1>);
+        case 3: return reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, V, 3, 1>);
+        default:
+            if constexpr (V == 4) return reinterpret_cast<const void *>(&layer_norm_grad_kernel<T, V, 4, 1>);
+            else return nullptr;  // not planned
+        }
+    }
 }
 template <class T>
 const void *row_kernel(const RowPlan &p, bool backward) {
@@ -150,6 +176,14 @@ long long grad_blocks(const RowPlan &p, long long rows, int sms) {
     const int teams = p.threads / p.team;
     return std::max(std::min(ceil_div(rows, teams), 2LL * sms * (kRowMost / p.threads)),
                     ceil_div(rows, static_cast<long long>(kSumRun) * teams));
+}
+
+// Whether the parameters can be read 16 bytes at a time (4 or 8 columns; their
+// type may be wider than the data's).
+bool aligned_params(std::initializer_list<const gc_tensor *> params, int v) {
+    for (const gc_tensor *t : params)
+        if (t != nullptr && (!aligned16(t->data) || (v == 4 && t->dtype != GC_F32))) return false;
+    return true;
 }
 
 bool vectors(std::initializer_list<const Rows *> views) {
@@ -213,6 +247,7 @@ int gc_b200_layer_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
     P.eps = static_cast<float>(eps);
     set_param(gamma, P.gamma, P.gamma_type);
     set_param(beta, P.beta, P.beta_type);
+    P.aligned = aligned_params({gamma, beta}, plan.v) ? 1 : 0;
     P.stats = stats != nullptr ? static_cast<float2 *>(stats->data) : nullptr;
     const void *fn = row_kernel(plan, false);
     // as many blocks as a multiprocessor has threads for; each takes rows in turn
@@ -295,10 +330,11 @@ int gc_b200_layer_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
     P.vcols = P.c / plan.v;
     P.team = plan.team;
     set_param(gamma, P.gamma, P.gamma_type);
+    P.aligned = aligned_params({gamma}, plan.v) ? 1 : 0;
     P.stats = static_cast<float2 *>(stats->data);
     P.part = sums ? static_cast<float *>(workspace) : nullptr;
     const void *fn = row_kernel(plan, true);
-    if (plan.smem > 48 * 1024 && (st = opt_in_smem(dev, fn, dynamic_limit(facts))) != GC_OK) return st;
+    if (plan.smem > 40 * 1024 && (st = opt_in_smem(dev, fn, dynamic_limit(facts))) != GC_OK) return st;
     void *args[] = {&P};
     e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(plan.threads), args, plan.smem, s);
     if (e == cudaSuccess && sums) {
