@@ -82,6 +82,7 @@ void fill(ConvSeqParams &P, const ConvCall &call, const gc_tensor *weight, const
     P.taps = static_cast<int>(call.taps);
     P.w = weight->data;
     P.w_type = elem_type(weight->dtype);
+    P.w_four = P.taps == 4 && aligned16(weight->data) ? 1 : 0;
     P.bias = bias != nullptr ? bias->data : nullptr;
     P.bias_type = bias != nullptr ? elem_type(bias->dtype) : kElemF32;
     P.act = act;
@@ -107,18 +108,19 @@ void fill(ConvSeqParams &P, const ConvCall &call, const gc_tensor *weight, const
 }
 
 enum ConvKernel { kForward, kBackward, kStep };
-template <class T, int V, int KT, int ACT>
+template <class T, int V, int KT, bool FULL, int ACT>
 const void *conv_instance(ConvKernel k) {
-    return k == kForward    ? reinterpret_cast<const void *>(&causal_conv_kernel<T, V, KT, ACT>)
-           : k == kBackward ? reinterpret_cast<const void *>(&causal_conv_grad_kernel<T, V, KT, ACT>)
-                            : reinterpret_cast<const void *>(&causal_conv_step_kernel<T, V, KT, ACT>);
+    return k == kForward    ? reinterpret_cast<const void *>(&causal_conv_kernel<T, V, KT, FULL, ACT>)
+           : k == kBackward ? reinterpret_cast<const void *>(&causal_conv_grad_kernel<T, V, KT, FULL, ACT>)
+                            : reinterpret_cast<const void *>(&causal_conv_step_kernel<T, V, KT, FULL, ACT>);
 }
 template <class T, int V>
 const void *conv_typed(ConvKernel k, int taps, int act) {
-    if (taps > 4) return conv_instance<T, V, 8, -1>(k);
-    if (act == GC_B200_ACT_SILU) return conv_instance<T, V, 4, kActSilu>(k);
-    if (act == GC_B200_ACT_NONE) return conv_instance<T, V, 4, kActNone>(k);
-    return conv_instance<T, V, 4, -1>(k);
+    if (taps > 4) return conv_instance<T, V, 8, false, -1>(k);
+    if (taps < 4) return conv_instance<T, V, 4, false, -1>(k);
+    if (act == GC_B200_ACT_SILU) return conv_instance<T, V, 4, true, kActSilu>(k);
+    if (act == GC_B200_ACT_NONE) return conv_instance<T, V, 4, true, kActNone>(k);
+    return conv_instance<T, V, 4, true, -1>(k);
 }
 const void *conv_kernel(ConvKernel k, int type, bool vec, int taps, int act) {
     if (type == kElemF16) return vec ? conv_typed<__half, 4>(k, taps, act) : conv_typed<__half, 1>(k, taps, act);
@@ -127,18 +129,22 @@ const void *conv_kernel(ConvKernel k, int type, bool vec, int taps, int act) {
     return vec ? conv_typed<float, 4>(k, taps, act) : conv_typed<float, 1>(k, taps, act);
 }
 
-// Dynamic shared memory of a kernel's ring.
-size_t ring_bytes(int type, bool vec) { return static_cast<size_t>(kConvRing) * kConvThreads * (vec ? 4 : 1) * elem_size(type); }
+// Dynamic shared memory of a kernel's ring; the gradient's sums take its place.
+size_t ring_bytes(int type, bool vec, int taps) {
+    const size_t v = vec ? 4 : 1, ring = kConvRing * kConvThreads * v * elem_size(type);
+    return std::max(ring, (taps + 1) * v * kConvThreads * sizeof(float));
+}
 int opt_in_ring(int dev, const void *fn, size_t bytes, const DeviceFacts &facts) {
     return bytes > 40 * 1024 ? opt_in_smem(dev, fn, facts.smem_optin - 8192) : GC_OK;
 }
 
-// Tokens of a thread: as many as leave four warps for each quarter of a
-// multiprocessor, 8 to 64.
-int stretch_of(const ConvCall &call, int v, int sms) {
-    const long long threads = call.n * ceil_div(call.c, v), wanted = static_cast<long long>(sms) * 512;
-    long long stretch = 64;
-    while (stretch > 8 && threads * ceil_div(call.l, stretch) < wanted) stretch /= 2;
+// Tokens of a thread: 16 to 64, as many as leave a wave of threads.  Each thread
+// loads its weights and the window in front of its stretch: shorter stretches were
+// no faster (N8 L2048 C2048 bf16 forward 37 us at 32 and at 64, gradient 103 and 98).
+int stretch_of(const ConvCall &call, int v, int sms, bool backward) {
+    const long long threads = call.n * ceil_div(call.c, v), wanted = (backward ? 384LL : 768LL) * sms;
+    long long stretch = backward ? 128 : 64;
+    while (stretch > 16 && threads * ceil_div(call.l, stretch) < wanted) stretch /= 2;
     return static_cast<int>(stretch);
 }
 
@@ -156,7 +162,7 @@ GradPlan plan_grad(const ConvCall &call, bool vec, int sms) {
     p.tiles = ceil_div(vcols, 32);
     p.cols = static_cast<int>(ceil_div(vcols, p.tiles));
     p.workers = kConvThreads / p.cols;
-    p.stretch = stretch_of(call, vec ? 4 : 1, sms);
+    p.stretch = stretch_of(call, vec ? 4 : 1, sms, true);
     p.segs = ceil_div(call.l, p.stretch);
     p.blocks_y = std::max(1LL, std::min(ceil_div(call.n * p.segs, p.workers), ceil_div(4LL * sms, p.tiles)));
     return p;
@@ -231,13 +237,13 @@ int gc_b200_causal_conv(const gc_tensor *x, const gc_tensor *weight, const gc_te
     ConvSeqParams P{};
     fill(P, call, weight, bias, activation, lengths, false);
     P.vcols = P.c / (vec ? 4 : 1);
-    P.stretch = stretch_of(call, vec ? 4 : 1, facts.sms);
+    P.stretch = stretch_of(call, vec ? 4 : 1, facts.sms, false);
     P.segs = std::max(1LL, ceil_div(call.l, P.stretch));
     const wide blocks = (static_cast<wide>(call.n) * P.segs * P.vcols + kConvThreads - 1) / kConvThreads;
     if (blocks > INT32_MAX) return gc_error(GC_UNSUPPORTED, "more work than a grid has blocks");
     void *args[] = {&P};
     const void *fn = conv_kernel(kForward, call.x.type, vec, P.taps, activation);
-    const size_t smem = ring_bytes(call.x.type, vec);
+    const size_t smem = ring_bytes(call.x.type, vec, 0);
     if ((st = opt_in_ring(dev, fn, smem, facts)) != GC_OK) return st;
     const cudaError_t e = launch_pdl(fn, dim3(static_cast<unsigned>(blocks)), dim3(kConvThreads), args, smem,
                                      reinterpret_cast<cudaStream_t>(stream));
@@ -317,7 +323,7 @@ int gc_b200_causal_conv_backward(const gc_tensor *dy, const gc_tensor *x, const 
     void *args[] = {&P};
     const long long grid = plan.tiles * plan.blocks_y;
     const void *fn = conv_kernel(kBackward, call.x.type, vec, P.taps, activation);
-    const size_t smem = ring_bytes(call.x.type, vec);
+    const size_t smem = ring_bytes(call.x.type, vec, P.taps);
     if ((st = opt_in_ring(dev, fn, smem, facts)) != GC_OK) return st;
     e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(kConvThreads), args, smem, s);
     if (e == cudaSuccess && sums) {

@@ -25,6 +25,7 @@ struct ConvSeqParams {
     int c, vcols, taps;
     const void *w, *bias;  // w: [c][taps]
     int w_type, bias_type;
+    int w_four;            // four taps, aligned
     int act;
     const int *lengths;    // nullable
     const void *state;     // nullable, [n][taps - 1][c]
@@ -89,9 +90,37 @@ __device__ __forceinline__ Lanes<V> no_lanes() {
     return r;
 }
 
-// The weights of V channels, tap by tap, right-aligned in KT.
+// The weights of V channels, tap by tap, right-aligned in KT.  Four taps of four
+// channels lie side by side: two or four 16-byte accesses.
 template <int V, int KT>
 __device__ __forceinline__ void load_taps(const ConvSeqParams &P, int c0, Lanes<V> (&w)[KT]) {
+    if constexpr (V == 4 && KT == 4) {
+        if (P.w_four) {
+            float f[4][4];  // [channel][tap]
+            if (P.w_type == kElemF32) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    unpack(__ldg(reinterpret_cast<const uint4 *>(static_cast<const float *>(P.w) + c0 * 4) + j), f[j],
+                           static_cast<const float *>(nullptr));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(P.w) + c0 * 4) + j);
+                    float v[8];
+                    if (P.w_type == kElemBF16) unpack(u, v, static_cast<const __nv_bfloat16 *>(nullptr));
+                    else unpack(u, v, static_cast<const __half *>(nullptr));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[2 * j + i / 4][i % 4] = v[i];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float v[4] = {f[0][k], f[1][k], f[2][k], f[3][k]};
+                w[k] = lanes_of<4>(v);
+            }
+            return;
+        }
+    }
     const int pad = KT - P.taps;
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
@@ -124,19 +153,30 @@ __device__ __forceinline__ long long length_of(const int *lengths, long long n, 
     return v < 0 ? 0 : min(static_cast<long long>(v), l);
 }
 
-template <int V, int KT, int ACT>
-__device__ __forceinline__ Lanes<V> conv_at(const ConvSeqParams &P, const Lanes<V> (&w)[KT], const Lanes<V> (&window)[KT - 1],
-                                            const Lanes<V> &cur, const Lanes<V> &bias) {
-    const int pad = KT - P.taps;
+// FULL: as many taps as the kernel holds.
+// The window of a thread is a ring of KT inputs, the newest at place `u`; loops over
+// tokens are unrolled by KT, so that places are known at compile time and nothing
+// is moved.
+template <int V, int KT, bool FULL>
+__device__ __forceinline__ Lanes<V> conv_at(const ConvSeqParams &P, const Lanes<V> (&w)[KT], const Lanes<V> (&window)[KT], int u,
+                                            const Lanes<V> &bias) {
+    const int pad = FULL ? 0 : KT - P.taps;
     Lanes<V> v = bias;
 #pragma unroll
     for (int k = 0; k < KT; ++k)
         if (k >= pad) {
 #pragma unroll
-            for (int i = 0; i < Lanes<V>::kPairs; ++i)
-                v.p[i] = fma2(w[k].p[i], k < KT - 1 ? window[k < KT - 1 ? k : 0].p[i] : cur.p[i], v.p[i]);
+            for (int i = 0; i < Lanes<V>::kPairs; ++i) v.p[i] = fma2(w[k].p[i], window[(u + 1 + k) % KT].p[i], v.p[i]);
         }
     return v;
+}
+// The window in front of token t.
+template <class T, int V, int KT>
+__device__ __forceinline__ void load_window(const ConvSeqParams &P, long long n, long long t, int c0, bool any, Lanes<V> (&window)[KT]) {
+    window[0] = no_lanes<V>();
+#pragma unroll
+    for (int k = 1; k < KT; ++k)
+        window[k] = any && k > KT - P.taps ? input_at<T, V>(P, n, t - KT + k, c0) : no_lanes<V>();
 }
 
 // A thread's groups at p, p + step, .. copied ahead through a ring in shared memory
@@ -174,7 +214,7 @@ struct ConvRing {
     __device__ __forceinline__ Lanes<V> at(int slot) const { return lanes_of_group<T, V>(mine[slot * kConvThreads]); }
 };
 
-template <class T, int V, int KT, int ACT>
+template <class T, int V, int KT, bool FULL, int ACT>
 __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const __grid_constant__ ConvSeqParams P) {
     extern __shared__ __align__(16) char space[];
     griddep_wait();
@@ -185,7 +225,7 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const __grid_
     if (n >= P.n) return;
     const long long len = length_of(P.lengths, n, P.l), t0 = seg * P.stretch, t1 = min(P.l, t0 + P.stretch);
     const long long end = min(len, t1);
-    Lanes<V> w[KT], window[KT - 1];
+    Lanes<V> w[KT], window[KT];
     T *y = static_cast<T *>(P.y) + n * P.y_ldn + c0;
     if (t0 < end) {
         const ConvRing<T, V> ring(space);
@@ -198,24 +238,22 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const __grid_
         }
         load_taps<V, KT>(P, c0, w);
         const Lanes<V> bias = load_bias<V>(P, c0);
-#pragma unroll
-        for (int k = 0; k < KT - 1; ++k) window[k] = k >= KT - P.taps ? input_at<T, V>(P, n, t0 - (KT - 1) + k, c0) : no_lanes<V>();
+        load_window<T, V, KT>(P, n, t0, c0, true, window);
         T *out = y + t0 * P.y_ldt;
-#pragma unroll 4
-        for (int k = 0; k < count; ++k, x += P.x_ldt, out += P.y_ldt) {
-            cp_async_wait<kConvRing - 1>();
-            const int slot = k % kConvRing;
-            if (slot == 0) ring.template fill<kConvRing>(0, 1, x - kConvRing * P.x_ldt, P.x_ldt, count - k);
-            const Lanes<V> cur = ring.at(slot);
-            if (k + kConvRing < count) ring.copy(slot, x);
-            cp_async_commit();
-            Lanes<V> v = conv_at<V, KT, ACT>(P, w, window, cur, bias);
+        for (int k0 = 0; k0 < count; k0 += KT) {
+            if (k0 % kConvRing == 0) ring.template fill<kConvRing>(0, 1, x - kConvRing * P.x_ldt, P.x_ldt, count - k0);
+            const int slot = k0 % kConvRing;
 #pragma unroll
-            for (int i = 0; i < Lanes<V>::kPairs; ++i) v.p[i] = activate<ACT>(P.act, v.p[i]);
-            store_group<T, V>(out, v);
+            for (int u = 0; u < KT; ++u, x += P.x_ldt, out += P.y_ldt) {
+                cp_async_wait<kConvRing - 1>();
+                window[u] = ring.at(slot + u);
+                if (k0 + u + kConvRing < count) ring.copy(slot + u, x);
+                cp_async_commit();
+                Lanes<V> v = conv_at<V, KT, FULL>(P, w, window, u, bias);
 #pragma unroll
-            for (int i = 0; i + 1 < KT - 1; ++i) window[i] = window[i + 1];
-            window[KT - 2] = cur;
+                for (int i = 0; i < Lanes<V>::kPairs; ++i) v.p[i] = activate<ACT>(P.act, v.p[i]);
+                if (k0 + u < count) store_group<T, V>(out, v);
+            }
         }
     }
     for (long long t = max(end, t0); t < t1; ++t) store_group<T, V>(y + t * P.y_ldt, no_lanes<V>());
@@ -228,7 +266,7 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const __grid_
 
 // One token: x and y are [n][c].  A thread has read all of its channels' state
 // before it writes, so state_out may be the state itself.
-template <class T, int V, int KT, int ACT>
+template <class T, int V, int KT, bool FULL, int ACT>
 __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(const __grid_constant__ ConvSeqParams P) {
     griddep_wait();
     griddep_launch_dependents();
@@ -236,12 +274,11 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(const __
     const int c0 = static_cast<int>(id % P.vcols) * V;
     const long long n = id / P.vcols;
     if (n >= P.n) return;
-    Lanes<V> w[KT], window[KT - 1];
-#pragma unroll
-    for (int k = 0; k < KT - 1; ++k) window[k] = k >= KT - P.taps ? input_at<T, V>(P, n, k - (KT - 1), c0) : no_lanes<V>();
-    const Lanes<V> cur = input_at<T, V>(P, n, 0, c0);
+    Lanes<V> w[KT], window[KT];
+    load_window<T, V, KT>(P, n, 0, c0, true, window);
+    window[0] = input_at<T, V>(P, n, 0, c0);
     load_taps<V, KT>(P, c0, w);
-    Lanes<V> v = conv_at<V, KT, ACT>(P, w, window, cur, load_bias<V>(P, c0));
+    Lanes<V> v = conv_at<V, KT, FULL>(P, w, window, 0, load_bias<V>(P, c0));
 #pragma unroll
     for (int i = 0; i < Lanes<V>::kPairs; ++i) v.p[i] = activate<ACT>(P.act, v.p[i]);
     store_group<T, V>(static_cast<T *>(P.y) + n * P.y_ldn + c0, v);
@@ -249,9 +286,9 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(const __
     T *out = static_cast<T *>(P.state_out) + n * P.so_ldn + c0;
     const int pad = KT - P.taps;
 #pragma unroll
-    for (int k = 1; k < KT - 1; ++k)
-        if (k > pad) store_group<T, V>(out + (k - 1 - pad) * P.so_ldt, window[k]);
-    store_group<T, V>(out + (P.taps - 2) * P.so_ldt, cur);
+    for (int k = 2; k < KT; ++k)
+        if (k > pad + 1) store_group<T, V>(out + (k - 2 - pad) * P.so_ldt, window[k]);
+    store_group<T, V>(out + (P.taps - 2) * P.so_ldt, window[0]);
 }
 
 // The gradient.  A block takes a tile of `cols` vector columns; its workers take
@@ -259,18 +296,17 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(const __
 // finishes dx[t - (KT - 1)]; the KT - 1 tokens behind its stretch are formed once
 // more.  dw and dbias add up over a stretch, then over stretches, then over the
 // workers of the block in a fixed order.
-template <class T, int V, int KT, int ACT>
+template <class T, int V, int KT, bool FULL, int ACT>
 __global__ void __launch_bounds__(kConvThreads, KT <= 4 ? 2 : 1) causal_conv_grad_kernel(const __grid_constant__ ConvSeqParams P) {
     constexpr int NP = Lanes<V>::kPairs, D = kConvRing / 2;  // D: tokens under way, of x and of dy
     extern __shared__ __align__(16) char space[];
-    __shared__ float sm[kConvThreads * V];
     griddep_wait();
     griddep_launch_dependents();
     const long long tile = blockIdx.x / P.blocks_y, by = blockIdx.x - tile * P.blocks_y;
     const int worker = threadIdx.x / P.cols, col = threadIdx.x - worker * P.cols;
     const long long vcol = tile * P.cols + col;
     const bool live = worker < P.workers && vcol < P.vcols;
-    const int c0 = static_cast<int>(vcol) * V, pad = KT - P.taps;
+    const int c0 = static_cast<int>(vcol) * V, pad = FULL ? 0 : KT - P.taps;
     Lanes<V> dw[KT], db = no_lanes<V>();
 #pragma unroll
     for (int k = 0; k < KT; ++k) dw[k] = no_lanes<V>();
@@ -295,80 +331,86 @@ __global__ void __launch_bounds__(kConvThreads, KT <= 4 ? 2 : 1) causal_conv_gra
                 }
                 cp_async_commit();
             }
-            Lanes<V> xw[KT - 1], gw[KT - 1], dw1[KT], db1 = no_lanes<V>();
+            Lanes<V> xw[KT], gw[KT], dw1[KT], db1 = no_lanes<V>();
 #pragma unroll
-            for (int k = 0; k < KT; ++k) dw1[k] = no_lanes<V>();
-#pragma unroll
-            for (int k = 0; k < KT - 1; ++k) {
-                xw[k] = k >= pad && inside > 0 ? input_at<T, V>(P, n, t0 - (KT - 1) + k, c0) : no_lanes<V>();
-                gw[k] = no_lanes<V>();
-            }
+            for (int k = 0; k < KT; ++k) dw1[k] = gw[k] = no_lanes<V>();
+            load_window<T, V, KT>(P, n, t0, c0, inside > 0, xw);
             const int first = seg == 0 ? KT - P.taps : KT - 1;  // from here on a finished place is the stretch's, or the state's
+            const int own = static_cast<int>(t1 - t0);
+            // tokens between which nothing has to be asked: all places finished are tokens of the
+            // sequence away from its last state, all tokens are the stretch's
+            const int plain_from = KT - 1, plain_to = P.dstate != nullptr ? 0 : min(inside, own);
             T *out = dx + (t0 - (KT - 1)) * P.y_ldt;
-            for (int k = 0; k < count; ++k, px += P.x_ldt, pg += P.dy_ldt, out += P.y_ldt) {
+            const auto token = [&](int k, int u, auto ask) {
+                constexpr bool ASK = decltype(ask)::value;
                 cp_async_wait<D - 1>();
                 const int slot = k % D * 2;
-                if (slot == 0) {
-                    ring.template fill<D>(0, 2, px - D * P.x_ldt, P.x_ldt, inside - k);
-                    ring.template fill<D>(1, 2, pg - D * P.dy_ldt, P.dy_ldt, inside - k);
-                }
-                Lanes<V> cur = no_lanes<V>(), g = no_lanes<V>();
-                if (k < inside) {
-                    cur = ring.at(slot);
-                    g = ring.at(slot + 1);
+                const bool live = !ASK || k < inside;
+                xw[u] = gw[u] = no_lanes<V>();
+                if (live) {
+                    xw[u] = ring.at(slot);
+                    gw[u] = ring.at(slot + 1);
                 }
                 if (k + D < inside) {
                     ring.copy(slot, px);
                     ring.copy(slot + 1, pg);
                 }
                 cp_async_commit();
-                if (k < inside) {
+                if (live) {
                     if (ACT != kActNone) {
-                        const Lanes<V> v = conv_at<V, KT, ACT>(P, w, xw, cur, bias);
+                        const Lanes<V> v = conv_at<V, KT, FULL>(P, w, xw, u, bias);
 #pragma unroll
-                        for (int i = 0; i < NP; ++i) g.p[i] = activate_grad<ACT>(P.act, v.p[i], g.p[i]);
+                        for (int i = 0; i < NP; ++i) gw[u].p[i] = activate_grad<ACT>(P.act, v.p[i], gw[u].p[i]);
                     }
-                    if (k < t1 - t0) {
+                    if (!ASK || k < own) {
 #pragma unroll
                         for (int i = 0; i < NP; ++i) {
-                            db1.p[i] = db1.p[i] + g.p[i];
+                            db1.p[i] = db1.p[i] + gw[u].p[i];
 #pragma unroll
                             for (int j = 0; j < KT; ++j)
-                                if (j >= pad)
-                                    dw1[j].p[i] = fma2(g.p[i], j < KT - 1 ? xw[j < KT - 1 ? j : 0].p[i] : cur.p[i], dw1[j].p[i]);
+                                if (j >= pad) dw1[j].p[i] = fma2(gw[u].p[i], xw[(u + 1 + j) % KT].p[i], dw1[j].p[i]);
                         }
                     }
                 }
-                if (k >= first) {
+                if (!ASK || k >= first) {
                     const long long s = t0 + k - (KT - 1);
                     Lanes<V> d = no_lanes<V>();
-                    if (s < len) {
+                    if (!ASK || s < len) {
 #pragma unroll
                         for (int j = 0; j < KT; ++j)
                             if (j >= pad) {
 #pragma unroll
-                                for (int i = 0; i < NP; ++i)
-                                    d.p[i] = fma2(w[j].p[i], j == 0 ? g.p[i] : gw[j == 0 ? 0 : KT - 1 - j].p[i], d.p[i]);
+                                for (int i = 0; i < NP; ++i) d.p[i] = fma2(w[j].p[i], gw[(u - j + KT) % KT].p[i], d.p[i]);
                             }
                         const long long j = s + P.taps - 1 - len;  // its place in the last state
-                        if (P.dstate != nullptr && j >= 0) {
+                        if (ASK && P.dstate != nullptr && j >= 0) {
                             const Lanes<V> e = lanes_of_group<T, V>(load_group<T, V>(
                                 static_cast<const T *>(P.dstate) + n * P.ds_ldn + j * P.ds_ldt + c0));
 #pragma unroll
                             for (int i = 0; i < NP; ++i) d.p[i] = d.p[i] + e.p[i];
                         }
                     }
-                    if (s >= 0) store_group<T, V>(out, d);
+                    if (!ASK || s >= 0) store_group<T, V>(out, d);
                     else if (P.state_out != nullptr)
                         store_group<T, V>(static_cast<T *>(P.state_out) + n * P.so_ldn + (s + P.taps - 1) * P.so_ldt + c0, d);
                 }
-#pragma unroll
-                for (int i = 0; i + 1 < KT - 1; ++i) {
-                    xw[i] = xw[i + 1];
-                    gw[i] = gw[i + 1];
+                px += P.x_ldt;
+                pg += P.dy_ldt;
+                out += P.y_ldt;
+            };
+            for (int k0 = 0; k0 < count; k0 += KT) {
+                if (k0 % D == 0) {
+                    ring.template fill<D>(0, 2, px - D * P.x_ldt, P.x_ldt, inside - k0);
+                    ring.template fill<D>(1, 2, pg - D * P.dy_ldt, P.dy_ldt, inside - k0);
                 }
-                xw[KT - 2] = cur;
-                gw[KT - 2] = g;
+                if (k0 >= plain_from && k0 + KT <= plain_to) {
+#pragma unroll
+                    for (int u = 0; u < KT; ++u) token(k0 + u, u, std::false_type());
+                } else {
+#pragma unroll
+                    for (int u = 0; u < KT; ++u)
+                        if (k0 + u < count) token(k0 + u, u, std::true_type());
+                }
             }
             cp_async_wait<0>();
 #pragma unroll
@@ -380,25 +422,26 @@ __global__ void __launch_bounds__(kConvThreads, KT <= 4 ? 2 : 1) causal_conv_gra
         }
     }
     if (P.part == nullptr) return;
+    // all sums side by side in the ring's place, each then joined by one thread
+    float *sm = reinterpret_cast<float *>(space);
+    const int pitch = P.workers * P.cols;
+    __syncthreads();
 #pragma unroll
     for (int q = 0; q <= KT; ++q) {
-        if (q < pad) continue;
         float v[V];
         values_of<V>(q < KT ? dw[q < KT ? q : 0] : db, v);
-        __syncthreads();
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            if (worker < P.workers) sm[(j * P.workers + worker) * P.cols + col] = v[j];
-        __syncthreads();
-        if (worker == 0 && vcol < P.vcols) {
-            float *out = P.part + (by * (P.taps + 1) + (q < KT ? q - pad : P.taps)) * P.c + c0;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float s = sm[j * P.workers * P.cols + col];
-                for (int i = 1; i < P.workers; ++i) s += sm[(j * P.workers + i) * P.cols + col];
-                out[j] = s;
-            }
-        }
+            if (worker < P.workers && q >= pad) sm[((q - pad) * V + j) * pitch + worker * P.cols + col] = v[j];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < (P.taps + 1) * V * P.cols; i += kConvThreads) {
+        const int k = i % P.cols, j = i / P.cols % V, q = i / P.cols / V;  // column, element, tap (the last: bias)
+        if (tile * P.cols + k >= P.vcols) continue;
+        const float *src = sm + (q * V + j) * pitch + k;
+        float s = src[0];
+        for (int w = 1; w < P.workers; ++w) s += src[w * P.cols];
+        P.part[(by * (P.taps + 1) + q) * P.c + (tile * P.cols + k) * V + j] = s;
     }
 }
 

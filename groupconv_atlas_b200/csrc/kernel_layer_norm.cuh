@@ -84,6 +84,20 @@ __device__ __forceinline__ Lanes<V> row_params(const void *p, int type, bool ali
     return lanes_of<V>(v);
 }
 template <int V>
+__device__ __forceinline__ Lanes<V> float_params(const float *p) {
+    float v[V];
+    if constexpr (V == 1) {
+        v[0] = *p;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4 *>(p + i));
+            v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+        }
+    }
+    return lanes_of<V>(v);
+}
+template <int V>
 __device__ __forceinline__ float lanes_sum(const Lanes<V> &l) {
     f2 s = l.p[0];
 #pragma unroll
@@ -103,6 +117,7 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_kernel(const __grid_const
     const int teams = blockDim.x / P.team, team = threadIdx.x / P.team, lane = threadIdx.x - team * P.team;
     const long long all = static_cast<long long>(gridDim.x) * teams;
     const float inv = 1.0f / static_cast<float>(P.c);
+    const bool plain = P.aligned && P.gamma != nullptr && P.beta != nullptr && P.gamma_type == kElemF32 && P.beta_type == kElemF32;
     int turn = 0;
     for (long long first = static_cast<long long>(blockIdx.x) * teams; first < P.rows; first += all * ROWS) {
         Raw<T, V> raw[ROWS][NV];
@@ -146,12 +161,7 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_kernel(const __grid_const
         team_sums<ROWS>(q, P.team, buf, turn);
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) q[r] = 1.0f / sqrtf(fmaf(q[r], inv, P.eps));
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int v = lane + j * P.team;
-            if (v >= P.vcols) continue;
-            const Lanes<V> gamma = row_params<V>(P.gamma, P.gamma_type, P.aligned, v * V, 1.0f);
-            const Lanes<V> beta = row_params<V>(P.beta, P.beta_type, P.aligned, v * V, 0.0f);
+        const auto finish = [&](int j, int v, const Lanes<V> &gamma, const Lanes<V> &beta) {
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 const long long row = first + team + r * all;
@@ -161,6 +171,23 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_kernel(const __grid_const
                 for (int i = 0; i < NP; ++i)
                     e.p[i] = fma2((e.p[i] + pair(-s[r])) * pair(q[r]), gamma.p[i], beta.p[i]);
                 store_lanes<T, V>(static_cast<T *>(P.y) + row * P.y_ld + static_cast<long long>(v) * V, e);
+            }
+        };
+        if (V > 1 && plain) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int v = lane + j * P.team;
+                if (v < P.vcols)
+                    finish(j, v, float_params<V>(static_cast<const float *>(P.gamma) + v * V),
+                           float_params<V>(static_cast<const float *>(P.beta) + v * V));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int v = lane + j * P.team;
+                if (v < P.vcols)
+                    finish(j, v, row_params<V>(P.gamma, P.gamma_type, P.aligned, v * V, 1.0f),
+                           row_params<V>(P.beta, P.beta_type, P.aligned, v * V, 0.0f));
             }
         }
         if (P.stats != nullptr && lane == 0) {

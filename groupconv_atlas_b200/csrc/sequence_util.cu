@@ -15,11 +15,11 @@ __global__ void __launch_bounds__(kSumWarps * 32) sum_rows_kernel(const __grid_c
     if (col < P.cols) {
         const float *src = P.part + (static_cast<long long>(warp) * P.planes + plane) * P.cols + col;
         const long long step = static_cast<long long>(kSumWarps) * P.planes * P.cols;
-        for (long long row = warp; row < P.rows;) {
+        for (long long left = (P.rows - warp + kSumWarps - 1) / kSumWarps; left > 0; left -= kSumRun) {
+            const int run = static_cast<int>(min(left, static_cast<long long>(kSumRun)));
             float s = 0.0f;
 #pragma unroll 8
-            for (int u = 0; u < kSumRun; ++u, row += kSumWarps, src += step)
-                if (row < P.rows) s += *src;
+            for (int u = 0; u < run; ++u, src += step) s += *src;
             sum += s;
         }
     }
