@@ -67,12 +67,13 @@ int check_layouts(const gc_tensor *weight, const gc_tensor *bias, int act, const
 
 bool empty_view(const Strided &v) { return v.data == nullptr || v.empty; }
 
-// Whether the data can be taken four elements at a time.
-bool groups_of_four(std::initializer_list<const Strided *> views) {
+// Whether the data can be taken so many elements at a time.
+bool groups_of(std::initializer_list<const Strided *> views, int e) {
     for (const Strided *v : views)
-        if (!empty_view(*v) && !group_aligned(*v, 4)) return false;
+        if (!empty_view(*v) && !group_aligned(*v, e)) return false;
     return true;
 }
+bool groups_of_four(std::initializer_list<const Strided *> views) { return groups_of(views, 4); }
 
 void fill(ConvSeqParams &P, const ConvCall &call, const gc_tensor *weight, const gc_tensor *bias, int act,
           const int32_t *lengths, bool step) {
@@ -122,6 +123,12 @@ const void *conv_typed(ConvKernel k, int taps, int act) {
     if (act == GC_B200_ACT_NONE) return conv_instance<T, V, 4, true, kActNone>(k);
     return conv_instance<T, V, 4, true, -1>(k);
 }
+template <class T>
+const void *conv_eight(int act) {
+    if (act == GC_B200_ACT_SILU) return reinterpret_cast<const void *>(&causal_conv_kernel<T, 8, 4, true, kActSilu>);
+    if (act == GC_B200_ACT_NONE) return reinterpret_cast<const void *>(&causal_conv_kernel<T, 8, 4, true, kActNone>);
+    return reinterpret_cast<const void *>(&causal_conv_kernel<T, 8, 4, true, -1>);
+}
 const void *conv_kernel(ConvKernel k, int type, bool vec, int taps, int act) {
     if (type == kElemF16) return vec ? conv_typed<__half, 4>(k, taps, act) : conv_typed<__half, 1>(k, taps, act);
     if (type == kElemBF16)
@@ -130,8 +137,8 @@ const void *conv_kernel(ConvKernel k, int type, bool vec, int taps, int act) {
 }
 
 // Dynamic shared memory of a kernel's ring; the gradient's sums take its place.
-size_t ring_bytes(int type, bool vec, int taps) {
-    const size_t v = vec ? 4 : 1, ring = kConvRing * kConvThreads * v * elem_size(type);
+size_t ring_bytes(int type, size_t v, int taps) {
+    const size_t ring = kConvRing * kConvThreads * v * elem_size(type);
     return std::max(ring, (taps + 1) * v * kConvThreads * sizeof(float));
 }
 int opt_in_ring(int dev, const void *fn, size_t bytes, const DeviceFacts &facts) {
@@ -236,14 +243,20 @@ int gc_b200_causal_conv(const gc_tensor *x, const gc_tensor *weight, const gc_te
     const bool vec = groups_of_four({&call.x, &call.y, &call.state, &call.state_out});
     ConvSeqParams P{};
     fill(P, call, weight, bias, activation, lengths, false);
-    P.vcols = P.c / (vec ? 4 : 1);
+    // Eight channels of 16 bits a thread where they lie on 16 bytes: 29 us against 36
+    // with four at N8 L2048 C2048 (the gradient has no registers for eight).
+    const bool eight = vec && call.x.type != kElemF32 && P.taps == 4 && groups_of({&call.x, &call.y, &call.state, &call.state_out}, 8);
+    const int v = eight ? 8 : vec ? 4 : 1;
+    P.vcols = P.c / v;
     P.stretch = stretch_of(call, vec ? 4 : 1, facts.sms, false);
     P.segs = std::max(1LL, ceil_div(call.l, P.stretch));
     const wide blocks = (static_cast<wide>(call.n) * P.segs * P.vcols + kConvThreads - 1) / kConvThreads;
     if (blocks > INT32_MAX) return gc_error(GC_UNSUPPORTED, "more work than a grid has blocks");
     void *args[] = {&P};
-    const void *fn = conv_kernel(kForward, call.x.type, vec, P.taps, activation);
-    const size_t smem = ring_bytes(call.x.type, vec, 0);
+    const void *fn = !eight                    ? conv_kernel(kForward, call.x.type, vec, P.taps, activation)
+                     : call.x.type == kElemF16 ? conv_eight<__half>(activation)
+                                               : conv_eight<__nv_bfloat16>(activation);
+    const size_t smem = ring_bytes(call.x.type, v, 0);
     if ((st = opt_in_ring(dev, fn, smem, facts)) != GC_OK) return st;
     const cudaError_t e = launch_pdl(fn, dim3(static_cast<unsigned>(blocks)), dim3(kConvThreads), args, smem,
                                      reinterpret_cast<cudaStream_t>(stream));
@@ -323,7 +336,7 @@ int gc_b200_causal_conv_backward(const gc_tensor *dy, const gc_tensor *x, const 
     void *args[] = {&P};
     const long long grid = plan.tiles * plan.blocks_y;
     const void *fn = conv_kernel(kBackward, call.x.type, vec, P.taps, activation);
-    const size_t smem = ring_bytes(call.x.type, vec, P.taps);
+    const size_t smem = ring_bytes(call.x.type, vec ? 4 : 1, P.taps);
     if ((st = opt_in_ring(dev, fn, smem, facts)) != GC_OK) return st;
     e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(kConvThreads), args, smem, s);
     if (e == cudaSuccess && sums) {

@@ -94,17 +94,17 @@ __device__ __forceinline__ Lanes<V> no_lanes() {
 // channels lie side by side: two or four 16-byte accesses.
 template <int V, int KT>
 __device__ __forceinline__ void load_taps(const ConvSeqParams &P, int c0, Lanes<V> (&w)[KT]) {
-    if constexpr (V == 4 && KT == 4) {
+    if constexpr (V > 1 && KT == 4) {
         if (P.w_four) {
-            float f[4][4];  // [channel][tap]
+            float f[V][4];  // [channel][tap]
             if (P.w_type == kElemF32) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < V; ++j)
                     unpack(__ldg(reinterpret_cast<const uint4 *>(static_cast<const float *>(P.w) + c0 * 4) + j), f[j],
                            static_cast<const float *>(nullptr));
             } else {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < V / 2; ++j) {
                     const uint4 u = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(P.w) + c0 * 4) + j);
                     float v[8];
                     if (P.w_type == kElemBF16) unpack(u, v, static_cast<const __nv_bfloat16 *>(nullptr));
@@ -115,8 +115,10 @@ __device__ __forceinline__ void load_taps(const ConvSeqParams &P, int c0, Lanes<
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float v[4] = {f[0][k], f[1][k], f[2][k], f[3][k]};
-                w[k] = lanes_of<4>(v);
+                float v[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] = f[j][k];
+                w[k] = lanes_of<V>(v);
             }
             return;
         }

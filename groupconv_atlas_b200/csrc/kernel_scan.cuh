@@ -235,31 +235,48 @@ struct ScanPlace {
 
 // A lane's states of a [..][states] tensor, as pairs; zeros where there are none.
 // `swap` reorders them: place r holds state r ^ swap.
+// Four floats in the order that `swap` asks for.
+__device__ __forceinline__ float4 reorder(float4 v, int swap) {
+    if (swap & 2) v = make_float4(v.z, v.w, v.x, v.y);
+    if (swap & 1) v = make_float4(v.y, v.x, v.w, v.z);
+    return v;
+}
+template <class S>
+__device__ __forceinline__ bool whole_states(const void *p, int states) {
+    return S::R == 4 && states % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
 template <class S>
 __device__ __forceinline__ void load_states(const float *p, int part, int states, bool live, int swap, f2 (&v)[S::NP]) {
-    float f[4] = {};
-#pragma unroll
-    for (int r = 0; r < S::R; ++r) {
-        const int s = part * S::R + (r ^ swap);
-        f[r] = live && s < states ? p[s] : 0.0f;
+    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (whole_states<S>(p, states)) {
+        if (live && part * 4 < states) f = *reinterpret_cast<const float4 *>(p + part * 4);
+    } else if (live) {
+        const float *q = p + part * S::R;
+        const int left = min(states - part * S::R, S::R);
+        if (left > 0) f.x = q[0];
+        if (left > 1) f.y = q[1];
+        if (left > 2) f.z = q[2];
+        if (left > 3) f.w = q[3];
     }
-#pragma unroll
-    for (int i = 0; i < S::NP; ++i) v[i] = pair(f[2 * i], f[2 * i + 1]);
+    f = reorder(f, swap);
+    v[0] = pair(f.x, f.y);
+    if constexpr (S::NP == 2) v[1] = pair(f.z, f.w);
 }
 template <class S>
 __device__ __forceinline__ void store_states(float *p, int part, int states, bool live, int swap, const f2 (&v)[S::NP]) {
-    float f[4];
-#pragma unroll
-    for (int i = 0; i < S::NP; ++i) split(v[i], f[2 * i], f[2 * i + 1]);
-    if (S::R == 4 && swap == 0 && states % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-        if (live && part * 4 < states)
-            *reinterpret_cast<float4 *>(p + part * 4) = make_float4(f[0], f[1], f[2], f[3]);
-        return;
-    }
-#pragma unroll
-    for (int r = 0; r < S::R; ++r) {
-        const int s = part * S::R + (r ^ swap);
-        if (live && s < states) p[s] = f[r];
+    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    split(v[0], f.x, f.y);
+    if constexpr (S::NP == 2) split(v[1], f.z, f.w);
+    f = reorder(f, swap);  // its own inverse
+    if (whole_states<S>(p, states)) {
+        if (live && part * 4 < states) *reinterpret_cast<float4 *>(p + part * 4) = f;
+    } else if (live) {
+        float *q = p + part * S::R;
+        const int left = min(states - part * S::R, S::R);
+        if (left > 0) q[0] = f.x;
+        if (left > 1) q[1] = f.y;
+        if (left > 2) q[2] = f.z;
+        if (left > 3) q[3] = f.w;
     }
 }
 // A log2(e): the exponentials are powers of 2.  Infinities become the largest
@@ -267,17 +284,29 @@ __device__ __forceinline__ void store_states(float *p, int part, int states, boo
 // state as it is; tiles are filled up with such steps.
 template <class S>
 __device__ __forceinline__ void load_decay(const ScanParams &Q, const ScanPlace<S> &at, int k, int swap, f2 (&v)[S::NP]) {
-    float f[4] = {};
-#pragma unroll
-    for (int r = 0; r < S::R; ++r) {
-        const int s = at.part * S::R + (r ^ swap);
-        if (at.live[k] && s < Q.states)
-            f[r] = load_param(Q.a, Q.a_type, static_cast<long long>(at.channel + k) * Q.states + s) * kLog2E;
-        if (f[r] > 3e38f) f[r] = 3e38f;
-        if (f[r] < -3e38f) f[r] = -3e38f;
+    if (Q.a_type == kElemF32) {
+        load_states<S>(static_cast<const float *>(Q.a) + static_cast<long long>(at.channel + k) * Q.states, at.part, Q.states,
+                       at.live[k], swap, v);
+    } else {
+        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const long long i = static_cast<long long>(at.channel + k) * Q.states + at.part * S::R;
+        const int left = at.live[k] ? min(Q.states - at.part * S::R, S::R) : 0;
+        if (left > 0) f.x = load_param(Q.a, Q.a_type, i);
+        if (left > 1) f.y = load_param(Q.a, Q.a_type, i + 1);
+        if (left > 2) f.z = load_param(Q.a, Q.a_type, i + 2);
+        if (left > 3) f.w = load_param(Q.a, Q.a_type, i + 3);
+        f = reorder(f, swap);
+        v[0] = pair(f.x, f.y);
+        if constexpr (S::NP == 2) v[1] = pair(f.z, f.w);
     }
 #pragma unroll
-    for (int i = 0; i < S::NP; ++i) v[i] = pair(f[2 * i], f[2 * i + 1]);
+    for (int i = 0; i < S::NP; ++i) {
+        float a, b;
+        split(v[i] * pair(kLog2E), a, b);
+        a = a > 3e38f ? 3e38f : a < -3e38f ? -3e38f : a;
+        b = b > 3e38f ? 3e38f : b < -3e38f ? -3e38f : b;
+        v[i] = pair(a, b);
+    }
 }
 // Element (or, where `vec`, both at once) of the two channels from p.
 template <class T>
@@ -677,7 +706,7 @@ struct ScanGradTile {
     float f[S::T][S::CB], x[S::T][S::CB];
     float2 e[S::T][S::CB];             // slope of delta, dy times the gate's slope
     float bc[2][S::R][PITCH];          // B and C in the orders that lanes keep
-    float red[S::THREADS / 32][S::T][2 * S::SP];
+    alignas(16) float red[S::THREADS / 32][S::T][2 * S::SP];
 };
 
 // Tiles of 8 tokens, from a segment's last to its first.  A tile's states are
@@ -875,16 +904,20 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
             for (int i = 0; i < N; ++i) {
                 const int t = t4 + FourSums<P>::first(at.part) + i;
                 if (writes && t < tokens) {
+                    const float4 e = *reinterpret_cast<const float4 *>(&sm.e[t][at.chan]);
+                    const float4 d = *reinterpret_cast<const float4 *>(&sm.du[t][at.chan]);
+                    const float2 ff = *reinterpret_cast<const float2 *>(&sm.f[t][at.chan]);
+                    const float2 xx = *reinterpret_cast<const float2 *>(&sm.x[t][at.chan]);
+                    const float delta[2] = {d.x, d.z}, f[2] = {ff.x, ff.y}, x[2] = {xx.x, xx.y};
+                    const float slope[2] = {e.x, e.z}, w[2] = {e.y, e.w};
                     float dx[2], ddt[2], dz[2];
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        const float f = sm.f[t][at.chan + k], x = sm.x[t][at.chan + k];
-                        const float2 e = sm.e[t][at.chan + k];
-                        dx[k] = fmaf(sm.du[t][at.chan + k].x, qb[k][i], skip[k] * f);
+                        dx[k] = fmaf(delta[k], qb[k][i], skip[k] * f[k]);
                         // qa holds A log2(e), not A
-                        ddt[k] = fmaf(x, qb[k][i], qa[k][i] * (1.0f / kLog2E)) * e.x;
-                        dz[k] = e.y * fmaf(skip[k], x, y[k][i]);
-                        dskip1[k] = fmaf(f, x, dskip1[k]);
+                        ddt[k] = fmaf(x[k], qb[k][i], qa[k][i] * (1.0f / kLog2E)) * slope[k];
+                        dz[k] = w[k] * fmaf(skip[k], x[k], y[k][i]);
+                        dskip1[k] = fmaf(f[k], x[k], dskip1[k]);
                         dbias1[k] += ddt[k];
                     }
                     store_two<E>(token_at<E>(Q.dx, at.n, row + i) + at.channel, vec, at.live, dx[0], dx[1]);
@@ -902,13 +935,28 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
         }
         __syncthreads();
         float *part = Q.part_bc + (((at.tile * Q.n + at.n) * Q.l + t0) * Q.groups + at.group) * 2 * Q.states;
-        for (int i = threadIdx.x; i < tokens * 2 * S::SP; i += S::THREADS) {
-            const int t = i / (2 * S::SP), j = i % (2 * S::SP), s = j % S::SP;
-            if (s >= Q.states) continue;
-            float sum = sm.red[0][t][j];
+        const long long next = static_cast<long long>(Q.groups) * 2 * Q.states;  // a token further
+        if (R == 4 && Q.states % 4 == 0) {
+            for (int i = threadIdx.x; i < tokens * 2 * S::QUADS; i += S::THREADS) {
+                const int t = i / (2 * S::QUADS), j = i % (2 * S::QUADS) * 4, s = j % S::SP;
+                if (s >= Q.states) continue;
+                float4 sum = *reinterpret_cast<const float4 *>(&sm.red[0][t][j]);
 #pragma unroll
-            for (int w = 1; w < WARPS; ++w) sum += sm.red[w][t][j];
-            part[(t * static_cast<long long>(Q.groups) * 2 + j / S::SP) * Q.states + s] = sum;
+                for (int w = 1; w < WARPS; ++w) {
+                    const float4 v = *reinterpret_cast<const float4 *>(&sm.red[w][t][j]);
+                    sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+                }
+                *reinterpret_cast<float4 *>(part + t * next + (j / S::SP) * Q.states + s) = sum;
+            }
+        } else {
+            for (int i = threadIdx.x; i < tokens * 2 * S::SP; i += S::THREADS) {
+                const int t = i / (2 * S::SP), j = i % (2 * S::SP), s = j % S::SP;
+                if (s >= Q.states) continue;
+                float sum = sm.red[0][t][j];
+#pragma unroll
+                for (int w = 1; w < WARPS; ++w) sum += sm.red[w][t][j];
+                part[t * next + (j / S::SP) * Q.states + s] = sum;
+            }
         }
     }
     const auto zeros = [&](const TokenView &w) {
