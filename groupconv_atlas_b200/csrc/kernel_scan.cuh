@@ -190,13 +190,19 @@ __device__ __forceinline__ void gate2(f2 z, f2 &gate, f2 &slope) {
 // ---- shapes and places ---------------------------------------------------------------------
 // A thread takes a part of the states of two neighbouring channels, so that what
 // it reads of B and C serves both.
-template <int SP_, int THREADS_, int T_>
+template <int SP_, int MOST, int THREADS_, int T_>
 struct ScanShape {
-    static constexpr int SP = SP_, THREADS = THREADS_, T = T_;   // T: tokens of a tile
-    static constexpr int R = SP >= 4 ? 4 : 1, NP = (R + 1) / 2;  // states of a lane and channel, as pairs
+    static constexpr int SP = SP_, THREADS = THREADS_, T = T_;           // T: tokens of a tile
+    static constexpr int R = SP < MOST ? SP : MOST, NP = (R + 1) / 2;    // states of a lane and channel, as pairs
     static constexpr int P = SP / R, CB = 2 * THREADS / P;       // lanes of a channel, channels of a block
     static constexpr int GROUPS = CB / 4, NG = T * GROUPS > THREADS ? T * GROUPS / THREADS : 1;
     static constexpr int QUADS = SP >= 4 ? SP / 4 : 1;           // of a token's B or C
+    // Values of pairs of channels, 16 bytes each: even pairs, then odd ones, a place
+    // apart in the banks, and tokens two.  Threads that store the pairs of their four
+    // channels, lanes that read one token's pairs and lanes that read pairs of four
+    // tokens all meet different banks.
+    static constexpr int ODD = GROUPS + 1, PAIRS = 2 * ODD;
+    __device__ __forceinline__ static int place(int chan) { return (chan >> 1 & 1) * ODD + (chan >> 2); }
 };
 
 // A warp's lanes: pair of channels * P + part; a part has the states part * R ...
@@ -241,42 +247,49 @@ __device__ __forceinline__ float4 reorder(float4 v, int swap) {
     if (swap & 1) v = make_float4(v.y, v.x, v.w, v.z);
     return v;
 }
-template <class S>
 __device__ __forceinline__ bool whole_states(const void *p, int states) {
-    return S::R == 4 && states % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+    return states % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 template <class S>
 __device__ __forceinline__ void load_states(const float *p, int part, int states, bool live, int swap, f2 (&v)[S::NP]) {
-    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (whole_states<S>(p, states)) {
-        if (live && part * 4 < states) f = *reinterpret_cast<const float4 *>(p + part * 4);
-    } else if (live) {
-        const float *q = p + part * S::R;
-        const int left = min(states - part * S::R, S::R);
-        if (left > 0) f.x = q[0];
-        if (left > 1) f.y = q[1];
-        if (left > 2) f.z = q[2];
-        if (left > 3) f.w = q[3];
+    const bool whole = whole_states(p, states);
+#pragma unroll
+    for (int r = 0; r < S::R; r += 4) {
+        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float *q = p + part * S::R + r;
+        const int left = live ? min(states - part * S::R - r, S::R - r) : 0;
+        if (S::R >= 4 && whole) {
+            if (left > 0) f = *reinterpret_cast<const float4 *>(q);
+        } else {
+            if (left > 0) f.x = q[0];
+            if (left > 1) f.y = q[1];
+            if (left > 2) f.z = q[2];
+            if (left > 3) f.w = q[3];
+        }
+        f = reorder(f, swap);
+        v[r / 2] = pair(f.x, f.y);
+        if constexpr (S::NP > 1) v[r / 2 + 1] = pair(f.z, f.w);
     }
-    f = reorder(f, swap);
-    v[0] = pair(f.x, f.y);
-    if constexpr (S::NP == 2) v[1] = pair(f.z, f.w);
 }
 template <class S>
 __device__ __forceinline__ void store_states(float *p, int part, int states, bool live, int swap, const f2 (&v)[S::NP]) {
-    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    split(v[0], f.x, f.y);
-    if constexpr (S::NP == 2) split(v[1], f.z, f.w);
-    f = reorder(f, swap);  // its own inverse
-    if (whole_states<S>(p, states)) {
-        if (live && part * 4 < states) *reinterpret_cast<float4 *>(p + part * 4) = f;
-    } else if (live) {
-        float *q = p + part * S::R;
-        const int left = min(states - part * S::R, S::R);
-        if (left > 0) q[0] = f.x;
-        if (left > 1) q[1] = f.y;
-        if (left > 2) q[2] = f.z;
-        if (left > 3) q[3] = f.w;
+    const bool whole = whole_states(p, states);
+#pragma unroll
+    for (int r = 0; r < S::R; r += 4) {
+        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        split(v[r / 2], f.x, f.y);
+        if constexpr (S::NP > 1) split(v[r / 2 + 1], f.z, f.w);
+        f = reorder(f, swap);  // its own inverse
+        float *q = p + part * S::R + r;
+        const int left = live ? min(states - part * S::R - r, S::R - r) : 0;
+        if (S::R >= 4 && whole) {
+            if (left > 0) *reinterpret_cast<float4 *>(q) = f;
+        } else {
+            if (left > 0) q[0] = f.x;
+            if (left > 1) q[1] = f.y;
+            if (left > 2) q[2] = f.z;
+            if (left > 3) q[3] = f.w;
+        }
     }
 }
 // A log2(e): the exponentials are powers of 2.  Infinities become the largest
@@ -288,16 +301,19 @@ __device__ __forceinline__ void load_decay(const ScanParams &Q, const ScanPlace<
         load_states<S>(static_cast<const float *>(Q.a) + static_cast<long long>(at.channel + k) * Q.states, at.part, Q.states,
                        at.live[k], swap, v);
     } else {
-        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const long long i = static_cast<long long>(at.channel + k) * Q.states + at.part * S::R;
-        const int left = at.live[k] ? min(Q.states - at.part * S::R, S::R) : 0;
-        if (left > 0) f.x = load_param(Q.a, Q.a_type, i);
-        if (left > 1) f.y = load_param(Q.a, Q.a_type, i + 1);
-        if (left > 2) f.z = load_param(Q.a, Q.a_type, i + 2);
-        if (left > 3) f.w = load_param(Q.a, Q.a_type, i + 3);
-        f = reorder(f, swap);
-        v[0] = pair(f.x, f.y);
-        if constexpr (S::NP == 2) v[1] = pair(f.z, f.w);
+#pragma unroll
+        for (int r = 0; r < S::R; r += 4) {
+            float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const int first = at.part * S::R + r, left = at.live[k] ? min(Q.states - first, S::R - r) : 0;
+            const long long i = static_cast<long long>(at.channel + k) * Q.states + first;
+            if (left > 0) f.x = load_param(Q.a, Q.a_type, i);
+            if (left > 1) f.y = load_param(Q.a, Q.a_type, i + 1);
+            if (left > 2) f.z = load_param(Q.a, Q.a_type, i + 2);
+            if (left > 3) f.w = load_param(Q.a, Q.a_type, i + 3);
+            f = reorder(f, swap);
+            v[r / 2] = pair(f.x, f.y);
+            if constexpr (S::NP > 1) v[r / 2 + 1] = pair(f.z, f.w);
+        }
     }
 #pragma unroll
     for (int i = 0; i < S::NP; ++i) {
@@ -307,6 +323,13 @@ __device__ __forceinline__ void load_decay(const ScanParams &Q, const ScanPlace<
         b = b > 3e38f ? 3e38f : b < -3e38f ? -3e38f : b;
         v[i] = pair(a, b);
     }
+}
+// The states of a thread's own place, in its order.
+template <class S>
+__device__ __forceinline__ void own_states(float4 f, int swap, f2 (&v)[S::NP]) {
+    f = reorder(f, swap);
+    v[0] = pair(f.x, f.y);
+    if constexpr (S::NP > 1) v[1] = pair(f.z, f.w);
 }
 // Element (or, where `vec`, both at once) of the two channels from p.
 template <class T>
@@ -324,10 +347,13 @@ __device__ __forceinline__ void store_two(T *p, bool vec, const bool (&live)[2],
 // A lane's states of a token from shared memory.
 template <class S>
 __device__ __forceinline__ void tile_states(const float *p, f2 (&v)[S::NP]) {
-    if constexpr (S::R == 4) {
-        const float4 f = *reinterpret_cast<const float4 *>(p);
-        v[0] = pair(f.x, f.y);
-        v[1] = pair(f.z, f.w);
+    if constexpr (S::R >= 4) {
+#pragma unroll
+        for (int i = 0; i < S::NP; i += 2) {
+            const float4 f = *reinterpret_cast<const float4 *>(p + 2 * i);
+            v[i] = pair(f.x, f.y);
+            v[i + 1] = pair(f.z, f.w);
+        }
     } else {
         v[0] = pair(*p, 0.0f);
     }
@@ -455,8 +481,8 @@ struct ScanTile {
     static constexpr bool kMain = MODE == kScanMain, kB = MODE != kScanCarryBack, kC = MODE != kScanCarry;
     using Fetch = ScanFetch<T, S, MODE == kScanCarry ? 2 : 3, kB, kC>;
     typename Fetch::Raw raw;
-    float2 du[2][S::T][S::CB];                              // delta, delta x (backwards f)
-    float2 ep[kMain ? 2 : 1][kMain ? S::T : 1][S::CB];      // D x, gate
+    float4 du[2][S::T][S::PAIRS];                           // delta, delta x (backwards f) of two channels
+    float4 ep[kMain ? 2 : 1][kMain ? S::T : 1][S::PAIRS];   // D x, gate
     float bc[2][kMain ? 2 : 1][S::T][S::SP];
 };
 
@@ -551,17 +577,17 @@ __global__ void __launch_bounds__(S::THREADS) scan_kernel(const __grid_constant_
                 float4 w;
                 split(delta[i], w.x, w.z);
                 split(u[i], w.y, w.w);
-                *reinterpret_cast<float4 *>(&sm.du[buf][t][gc + 2 * i]) = w;
+                sm.du[buf][t][i * S::ODD + gc / 4] = w;
                 if constexpr (MODE == kScanMain) {
                     split(dx[i], w.x, w.z);
                     split(gate[i], w.y, w.w);
-                    *reinterpret_cast<float4 *>(&sm.ep[buf][t][gc + 2 * i]) = w;
+                    sm.ep[buf][t][i * S::ODD + gc / 4] = w;
                 }
             }
         }
         fetch.quads(sm.raw, t0, tokens, [&](bool is_b, int t, int s, const float4 &v) {
             float *p = &sm.bc[buf][MODE == kScanMain && !is_b ? 1 : 0][t][s];
-            if constexpr (R == 4) *reinterpret_cast<float4 *>(p) = v;
+            if constexpr (R >= 4) *reinterpret_cast<float4 *>(p) = v;
             else *p = v.x;
         });
     };
@@ -571,10 +597,11 @@ __global__ void __launch_bounds__(S::THREADS) scan_kernel(const __grid_constant_
     const long long chunks = (Q.l + kScanChunk - 1) / kScanChunk;
     float *kept = Q.kept + ((at.n * chunks + at.begin / kScanChunk) * Q.channels + at.channel) * Q.states;
     const bool writes = at.part < 4, vec = Q.vec;
+    const int place = S::place(at.chan);
     for (int buf = 0; left > 0; left -= T, t0 += T, buf ^= 1) {
         __syncthreads();
         E *y_at = token_at<E>(Q.y, at.n, t0 + FourSums<P>::first(at.part)) + at.channel;  // the lane's token of each four
-        const float2 *du = &sm.du[buf][0][at.chan];
+        const float4 *du = &sm.du[buf][0][place];
         const float *b = &sm.bc[buf][0][0][at.part * R], *c = &sm.bc[buf][MODE == kScanMain ? 1 : 0][0][at.part * R];
 #pragma unroll
         for (int t4 = 0; t4 < T; t4 += 4) {
@@ -587,7 +614,7 @@ __global__ void __launch_bounds__(S::THREADS) scan_kernel(const __grid_constant_
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int t = t4 + j;
-                const float4 v = *reinterpret_cast<const float4 *>(&du[t * S::CB]);
+                const float4 v = du[t * S::PAIRS];
                 const float delta[2] = {v.x, v.z}, u[2] = {v.y, v.w};
                 f2 wb[NP], wc[NP];
                 tile_states<S>(b + t * S::SP, wb);
@@ -617,12 +644,15 @@ __global__ void __launch_bounds__(S::THREADS) scan_kernel(const __grid_constant_
                 for (int i = 0; i < N; ++i) {
                     const int t = t4 + FourSums<P>::first(at.part) + i;
                     if (writes && t < left) {
-                        const float4 e = *reinterpret_cast<const float4 *>(&sm.ep[buf][t][at.chan]);
+                        const float4 e = sm.ep[buf][t][place];
                         store_two<E>(y_at + i * Q.y.ldt, vec, at.live, (y[0][i] + e.x) * e.y, (y[1][i] + e.z) * e.w);
                     }
                 }
                 y_at += 4 * Q.y.ldt;
             }
+#ifdef CLOB
+            asm volatile("" ::: "memory");  // loads of later tokens stay behind
+#endif
         }
         if (left > T) {
             form(t0 + T, left - T, buf ^ 1);
@@ -702,11 +732,14 @@ struct ScanGradTile {
     static constexpr int PITCH = S::T * S::SP + 16;  // of a copy in another order: apart in the banks
     using Fetch = ScanFetch<T, S, 4, true, true>;
     typename Fetch::Raw raw;
-    float2 du[S::T][S::CB];            // delta, delta x
-    float f[S::T][S::CB], x[S::T][S::CB];
-    float2 e[S::T][S::CB];             // slope of delta, dy times the gate's slope
-    float bc[2][S::R][PITCH];          // B and C in the orders that lanes keep
+    float4 du[S::T][S::PAIRS];         // delta, delta x of two channels
+    float4 e[S::T][S::PAIRS];          // slope of delta, dy times the gate's slope
+    alignas(16) float f[S::T][S::CB + 8], x[S::T][S::CB + 8];
+    alignas(16) float bc[2][S::R][PITCH];  // B and C in the orders that lanes keep
     alignas(16) float red[S::THREADS / 32][S::T][2 * S::SP];
+    // a thread's own: the states in front of this tile and the next, bias of its four
+    // channels, sums for D and dt_bias of its two
+    float4 kept[2][2][S::THREADS], bias[S::THREADS], sums[S::THREADS];
 };
 
 // Tiles of 8 tokens, from a segment's last to its first.  A tile's states are
@@ -725,6 +758,21 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
     const ScanPlace<S> at(Q);
     const bool gated = Q.z.p != nullptr, softplus = Q.softplus;
     const long long chunks = (Q.l + T - 1) / T;
+    const int place = S::place(at.chan);
+    // the states in front of a tile to the thread's own place
+    const auto keep = [&](long long t0, int buf) {
+        const bool whole = whole_states(Q.kept, Q.states);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int left = at.live[k] ? min(Q.states - at.part * R, R) : 0;
+            const float *p = Q.kept + ((at.n * chunks + t0 / T) * Q.channels + at.channel + k) * Q.states + at.part * R;
+            float4 &own = sm.kept[buf][k][threadIdx.x];
+            if (R == 4 && whole && left > 0)
+                cp_async_16(&own, p);
+            else
+                own = make_float4(left > 0 ? p[0] : 0.0f, left > 1 ? p[1] : 0.0f, left > 2 ? p[2] : 0.0f, left > 3 ? p[3] : 0.0f);
+        }
+    };
     // the last tile with tokens of the sequence, and how many tiles there are
     int tiles = at.end > at.begin ? static_cast<int>((at.end - at.begin + T - 1) / T) : 0;
     long long t0 = at.begin + (tiles - 1) * static_cast<long long>(T);
@@ -736,7 +784,10 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
     fetch.in[3] = Q.z;
     const int gc = fetch.gc, valid = fetch.valid, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int swap = Sums::swap(lane);
-    if (tiles > 0) fetch.start(sm.raw, t0, tokens);
+    if (tiles > 0) {
+        keep(t0, 0);
+        fetch.start(sm.raw, t0, tokens);
+    }
 
     f2 a2[2][NP], q[2][NP], da[2][NP];
 #pragma unroll
@@ -755,26 +806,21 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
             for (int i = 0; i < NP; ++i) q[k][i] = fma2(exp2_fast(sum * a2[k][i]), q[k][i], e[i]);
         }
     }
-    f2 bias[2];
+    {
+        float b[4] = {};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        float b[2] = {};
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            if (Q.bias != nullptr && 2 * i + k < valid) b[k] = load_param(Q.bias, Q.bias_type, at.first + gc + 2 * i + k);
-        bias[i] = pair(b[0], b[1]);
+        for (int i = 0; i < 4; ++i)
+            if (Q.bias != nullptr && i < valid) b[i] = load_param(Q.bias, Q.bias_type, at.first + gc + i);
+        sm.bias[threadIdx.x] = make_float4(b[0], b[1], b[2], b[3]);
+        sm.sums[threadIdx.x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    float skip[2], dskip[2] = {0.0f, 0.0f}, dbias[2] = {0.0f, 0.0f};  // sums: over the lane's tokens
+    float skip[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) skip[k] = Q.d != nullptr && at.live[k] ? load_param(Q.d, Q.d_type, at.channel + k) : 0.0f;
     const bool writes = at.part < 4, vec = Q.vec;
 
-    for (; tiles > 0; --tiles, t0 -= T, tokens = T) {
-        f2 before[2][NP], h[T][2][NP];
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            load_states<S>(Q.kept + ((at.n * chunks + t0 / T) * Q.channels + at.channel + k) * Q.states, at.part, Q.states,
-                           at.live[k], swap, before[k]);
+    for (int buf = 0; tiles > 0; --tiles, t0 -= T, tokens = T, buf ^= 1) {
+        f2 h[T][2][NP];
         cp_async_wait<0>();
 #pragma unroll
         for (int g = 0; g < S::NG; ++g) {
@@ -784,6 +830,8 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
 #pragma unroll
             for (int i = 0; i < 2; ++i) delta[i] = slope[i] = x[i] = f[i] = w[i] = pair(0.0f);
             if (t < tokens) {
+                const float4 b4 = sm.bias[threadIdx.x];
+                const f2 bias[2] = {pair(b4.x, b4.y), pair(b4.z, b4.w)};
                 f2 raw[2];
                 fetch.four(sm.raw, 0, g, t0, raw);
                 fetch.four(sm.raw, 1, g, t0, x);
@@ -807,8 +855,8 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
                 split(delta[i] * x[i], d.y, d.w);
                 split(slope[i], e.x, e.z);
                 split(w[i], e.y, e.w);
-                *reinterpret_cast<float4 *>(&sm.du[t][gc + 2 * i]) = d;
-                *reinterpret_cast<float4 *>(&sm.e[t][gc + 2 * i]) = e;
+                sm.du[t][i * S::ODD + gc / 4] = d;
+                sm.e[t][i * S::ODD + gc / 4] = e;
             }
             float4 f4, x4;
             split(f[0], f4.x, f4.y);
@@ -831,21 +879,26 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
         });
         __syncthreads();
         if (tiles > 1) {
+            keep(t0 - T, buf ^ 1);
             fetch.start(sm.raw, t0 - T, T);
         }
+        const auto before = [&](int k, f2 (&v)[NP]) { own_states<S>(sm.kept[buf][k][threadIdx.x], swap, v); };
         const float *b = &sm.bc[0][R == 4 ? swap : 0][at.part * R], *c = &sm.bc[1][R == 4 ? swap : 0][at.part * R];
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            const float4 v = *reinterpret_cast<const float4 *>(&sm.du[t][at.chan]);
+            const float4 v = sm.du[t][place];
             const float delta[2] = {v.x, v.z}, u[2] = {v.y, v.w};
             f2 w[NP];
             tile_states<S>(b + t * S::SP, w);
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+            for (int k = 0; k < 2; ++k) {
+                f2 last[NP];
+                if (t == 0) before(k, last);
 #pragma unroll
                 for (int i = 0; i < NP; ++i)
-                    h[t][k][i] = fma2(exp2_fast(pair(delta[k]) * a2[k][i]), t == 0 ? before[k][i] : h[t == 0 ? 0 : t - 1][k][i],
+                    h[t][k][i] = fma2(exp2_fast(pair(delta[k]) * a2[k][i]), t == 0 ? last[i] : h[t == 0 ? 0 : t - 1][k][i],
                                       pair(u[k]) * w[i]);
+            }
             // loads of later tokens stay behind: their registers are the states'
             if (t % 4 == 3) asm volatile("" ::: "memory");
         }
@@ -859,7 +912,7 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
 #pragma unroll
             for (int j = 3; j >= 0; --j) {
                 const int t = t4 + j;
-                const float4 v = *reinterpret_cast<const float4 *>(&sm.du[t][at.chan]);
+                const float4 v = sm.du[t][place];
                 const float2 f2v = *reinterpret_cast<const float2 *>(&sm.f[t][at.chan]);
                 const float delta[2] = {v.x, v.z}, u[2] = {v.y, v.w}, f[2] = {f2v.x, f2v.y};
                 f2 wb[NP], wc[NP], gb[NP], gc2[NP];
@@ -867,7 +920,8 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
                 tile_states<S>(b + t * S::SP, wb);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    f2 sb, sa, sy;
+                    f2 sb, sa, sy, last[NP];
+                    if (t == 0) before(k, last);
 #pragma unroll
                     for (int i = 0; i < NP; ++i) {
                         q[k][i] = fma2(pair(f[k]), wc[i], q[k][i]);
@@ -876,7 +930,7 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
                         sb = i == 0 ? q[k][0] * wb[0] : fma2(q[k][i], wb[i], sb);
                         sy = i == 0 ? h[t][k][0] * wc[0] : fma2(h[t][k][i], wc[i], sy);
                         q[k][i] = q[k][i] * exp2_fast(pair(delta[k]) * a2[k][i]);
-                        const f2 m = q[k][i] * (t == 0 ? before[k][i] : h[t == 0 ? 0 : t - 1][k][i]);
+                        const f2 m = q[k][i] * (t == 0 ? last[i] : h[t == 0 ? 0 : t - 1][k][i]);
                         sa = i == 0 ? m * a2[k][0] : fma2(m, a2[k][i], sa);
                         da1[k][i] = fma2(m, pair(delta[k]), da1[k][i]);
                     }
@@ -904,8 +958,7 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
             for (int i = 0; i < N; ++i) {
                 const int t = t4 + FourSums<P>::first(at.part) + i;
                 if (writes && t < tokens) {
-                    const float4 e = *reinterpret_cast<const float4 *>(&sm.e[t][at.chan]);
-                    const float4 d = *reinterpret_cast<const float4 *>(&sm.du[t][at.chan]);
+                    const float4 e = sm.e[t][place], d = sm.du[t][place];
                     const float2 ff = *reinterpret_cast<const float2 *>(&sm.f[t][at.chan]);
                     const float2 xx = *reinterpret_cast<const float2 *>(&sm.x[t][at.chan]);
                     const float delta[2] = {d.x, d.z}, f[2] = {ff.x, ff.y}, x[2] = {xx.x, xx.y};
@@ -930,8 +983,10 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
         for (int k = 0; k < 2; ++k) {
 #pragma unroll
             for (int i = 0; i < NP; ++i) da[k][i] = da[k][i] + da1[k][i];
-            dskip[k] += dskip1[k];
-            dbias[k] += dbias1[k];
+        }
+        {
+            const float4 v = sm.sums[threadIdx.x];
+            sm.sums[threadIdx.x] = make_float4(v.x + dskip1[0], v.y + dskip1[1], v.z + dbias1[0], v.w + dbias1[1]);
         }
         __syncthreads();
         float *part = Q.part_bc + (((at.tile * Q.n + at.n) * Q.l + t0) * Q.groups + at.group) * 2 * Q.states;
@@ -977,6 +1032,8 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
         if (Q.part_a != nullptr)
             store_states<S>(Q.part_a + (row * Q.channels + at.channel + k) * Q.states, at.part, Q.states, at.live[k], swap, da[k]);
         if (Q.part_d == nullptr) continue;
+        const float4 own = sm.sums[threadIdx.x];
+        float dskip[2] = {own.x, own.y}, dbias[2] = {own.z, own.w};
 #pragma unroll
         for (int o = 1; o < P; o *= 2) {
             dskip[k] += __shfl_xor_sync(0xffffffffu, dskip[k], o);
@@ -1014,7 +1071,7 @@ __global__ void __launch_bounds__(S::THREADS) scan_step_kernel(const __grid_cons
         for (int k = 0; k < 2; ++k) e[k] = at.live[k] ? element(v, at.channel + k) : 0.0f;
     };
     f2 a2[2][NP], h[2][NP], delta[2], slope[2], raw[2], bias[2] = {pair(0.0f), pair(0.0f)};
-    float x[2], dt[2], z[2], d[2], b[4] = {}, c[4] = {}, y[2];
+    float x[2], dt[2], z[2], d[2], b[2 * NP] = {}, c[2 * NP] = {}, y[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k)
         load_states<S>(Q.state + at.n * Q.s_ldn + (at.channel + k) * Q.s_ldc, at.part, Q.states, at.live[k], 0, h[k]);
@@ -1075,13 +1132,17 @@ struct ScanLaunch {
 };
 // Threads of a block of the gradient: what the tiles of few lanes take of shared
 // memory grows with the channels of a block.
+#ifndef FR
+#define FR 4
+#define FT 16
+#endif
 constexpr int kScanThreads = 64;
 constexpr int grad_threads(int sp) { return sp >= 16 ? 128 : kScanThreads; }
 
 template <class E, int SP>
 ScanLaunch scan_instance(ScanKernel k) {
-    using S = ScanShape<SP, kScanThreads, 16>;
-    using G = ScanShape<SP, grad_threads(SP), kScanChunk>;
+    using S = ScanShape<SP, FR, kScanThreads, FT>;
+    using G = ScanShape<SP, 4, grad_threads(SP), kScanChunk>;
     switch (k) {
     case kMain:
         return {reinterpret_cast<const void *>(&scan_kernel<E, S, kScanMain>), S::THREADS, sizeof(ScanTile<E, S, kScanMain>)};

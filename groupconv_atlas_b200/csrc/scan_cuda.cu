@@ -38,6 +38,9 @@ namespace {
 
 using namespace gcb;
 
+#ifndef WANT
+#define WANT 16LL
+#endif
 constexpr int kMostStates = 64;
 
 // A call's tensors: the descriptors with the same index as their views.
@@ -133,13 +136,13 @@ ScanPlan plan_scan(const ScanCall &c, int sms, bool backward) {
     ScanPlan p;
     p.type = c.x.type;
     p.sp = padded_states(c.states);
-    p.per_lane = std::min(p.sp, 4);
+    p.per_lane = std::min(p.sp, FR);
     p.lanes = p.sp / p.per_lane;
     const int64_t cpg = c.c / c.groups;
     p.tiles = static_cast<int>(ceil_div(cpg, 2 * kScanThreads / p.lanes));
-    p.grad_tiles = static_cast<int>(ceil_div(cpg, 2 * grad_threads(p.sp) / p.lanes));
+    p.grad_tiles = static_cast<int>(ceil_div(cpg, 2 * grad_threads(p.sp) / (p.sp / std::min(p.sp, 4))));
     const long long blocks = std::max(1LL, static_cast<long long>(c.n) * c.groups * p.tiles);
-    const long long wanted = std::min(ceil_div((backward ? 24LL : 16LL) * sms, blocks), static_cast<long long>(c.l / 64));
+    const long long wanted = std::min(ceil_div((backward ? 24LL : WANT) * sms, blocks), static_cast<long long>(c.l / 64));
     p.seg_len = std::max(1LL, gcb::round_up(ceil_div(c.l, std::max(1LL, wanted)), 16));
     p.segs = static_cast<int>(std::max(1LL, ceil_div(c.l, p.seg_len)));
     p.blocks = blocks * p.segs;
@@ -229,7 +232,7 @@ int launch(ScanKernel k, const ScanPlan &p, ScanParams &P, int dev, const Device
         const int st = opt_in_smem(dev, l.fn, facts.smem_optin);
         if (st != GC_OK) return st;
     }
-    P.tiles = l.threads == kScanThreads ? p.tiles : p.grad_tiles;
+    P.tiles = k == kGrad ? p.grad_tiles : p.tiles;
     const long long blocks = P.n * P.groups * P.tiles * P.segs;
     if (blocks > INT32_MAX) return gc_error(GC_UNSUPPORTED, "more work than a grid has blocks");
     void *args[] = {&P};
