@@ -252,6 +252,7 @@ int gc_b200_causal_conv(const gc_tensor *x, const gc_tensor *weight, const gc_te
     P.segs = std::max(1LL, ceil_div(call.l, P.stretch));
     const wide blocks = (static_cast<wide>(call.n) * P.segs * P.vcols + kConvThreads - 1) / kConvThreads;
     if (blocks > INT32_MAX) return gc_error(GC_UNSUPPORTED, "more work than a grid has blocks");
+    P.small = blocks * kConvThreads <= UINT32_MAX ? 1 : 0;
     void *args[] = {&P};
     const void *fn = !eight                    ? conv_kernel(kForward, call.x.type, vec, P.taps, activation)
                      : call.x.type == kElemF16 ? conv_eight<__half>(activation)
@@ -389,6 +390,7 @@ int gc_b200_causal_conv_step(const gc_tensor *x, const gc_tensor *weight, const 
     P.vcols = P.c / (vec ? 4 : 1);
     const wide blocks = (static_cast<wide>(call.n) * P.vcols + kConvThreads - 1) / kConvThreads;
     if (blocks > INT32_MAX) return gc_error(GC_UNSUPPORTED, "more work than a grid has blocks");
+    P.small = blocks * kConvThreads <= UINT32_MAX ? 1 : 0;
     void *args[] = {&P};
     const cudaError_t e = launch_pdl(conv_kernel(kStep, call.x.type, vec, P.taps, activation),
                                      dim3(static_cast<unsigned>(blocks)), dim3(kConvThreads), args, 0,

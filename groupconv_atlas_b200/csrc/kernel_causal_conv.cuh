@@ -34,6 +34,7 @@ struct ConvSeqParams {
     long long s_ldn, s_ldt, so_ldn, so_ldt, ds_ldn, ds_ldt;
     int stretch;           // tokens of a thread
     long long segs;        // stretches of a sequence
+    int small;             // fewer than 2^32 threads
     // gradient
     int cols, workers;     // vector columns and workers of a block
     long long blocks_y;    // blocks that share a tile of columns
@@ -221,9 +222,20 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const __grid_
     extern __shared__ __align__(16) char space[];
     griddep_wait();
     griddep_launch_dependents();
-    const long long id = static_cast<long long>(blockIdx.x) * kConvThreads + threadIdx.x;
-    const int c0 = static_cast<int>(id % P.vcols) * V;
-    const long long rest = id / P.vcols, seg = rest % P.segs, n = rest / P.segs;
+    long long n, seg;
+    int c0;
+    if (P.small) {  // 32-bit divisions
+        const unsigned id = blockIdx.x * kConvThreads + threadIdx.x, vcols = P.vcols, segs = static_cast<unsigned>(P.segs);
+        const unsigned rest = id / vcols;
+        c0 = static_cast<int>(id - rest * vcols) * V;
+        n = rest / segs;
+        seg = rest % segs;
+    } else {
+        const long long id = static_cast<long long>(blockIdx.x) * kConvThreads + threadIdx.x, rest = id / P.vcols;
+        c0 = static_cast<int>(id % P.vcols) * V;
+        seg = rest % P.segs;
+        n = rest / P.segs;
+    }
     if (n >= P.n) return;
     const long long len = length_of(P.lengths, n, P.l), t0 = seg * P.stretch, t1 = min(P.l, t0 + P.stretch);
     const long long end = min(len, t1);
@@ -272,9 +284,17 @@ template <class T, int V, int KT, bool FULL, int ACT>
 __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(const __grid_constant__ ConvSeqParams P) {
     griddep_wait();
     griddep_launch_dependents();
-    const long long id = static_cast<long long>(blockIdx.x) * kConvThreads + threadIdx.x;
-    const int c0 = static_cast<int>(id % P.vcols) * V;
-    const long long n = id / P.vcols;
+    long long n;
+    int c0;
+    if (P.small) {
+        const unsigned id = blockIdx.x * kConvThreads + threadIdx.x, vcols = P.vcols;
+        n = id / vcols;
+        c0 = static_cast<int>(id % vcols) * V;
+    } else {
+        const long long id = static_cast<long long>(blockIdx.x) * kConvThreads + threadIdx.x;
+        n = id / P.vcols;
+        c0 = static_cast<int>(id % P.vcols) * V;
+    }
     if (n >= P.n) return;
     Lanes<V> w[KT], window[KT];
     load_window<T, V, KT>(P, n, 0, c0, true, window);

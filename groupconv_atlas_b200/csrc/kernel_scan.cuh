@@ -213,14 +213,12 @@ struct ScanPlace {
     int chan, part, channel;             // the thread's first channel, in the block and in all
     bool live[2];
     __device__ __forceinline__ explicit ScanPlace(const ScanParams &Q) {
-        const int per = Q.groups * Q.tiles;
-        long long b = blockIdx.x;
-        const int gt = static_cast<int>(b % per);
-        b /= per;
-        seg = static_cast<int>(b % Q.segs);
-        n = b / Q.segs;
-        group = gt / Q.tiles;
-        tile = gt - group * Q.tiles;
+        // 32-bit divisions: those of 64 bits would be most of a step's instructions
+        const unsigned tiles = Q.tiles, per = Q.groups * tiles, segs = Q.segs, b = blockIdx.x / per, gt = blockIdx.x - b * per;
+        n = b / segs;
+        seg = static_cast<int>(b % segs);
+        group = static_cast<int>(gt / tiles);
+        tile = static_cast<int>(gt % tiles);
         first = group * Q.cpg + tile * S::CB;
         count = min(S::CB, Q.cpg - tile * S::CB);
         chan = threadIdx.x / S::P * 2;
@@ -473,6 +471,31 @@ __device__ __forceinline__ T *token_at(const TokenView &v, long long n, long lon
     return static_cast<T *>(const_cast<void *>(v.p)) + n * v.ldn + t * v.ldt;
 }
 
+// The state (or, backwards, its gradient) after the segments first, first + step, ..
+// before `stop`: each adds what it adds to what its decay leaves.  Four segments'
+// effects are loaded at once.
+template <class S>
+__device__ __forceinline__ void pass_segments(const ScanParams &Q, const ScanPlace<S> &at, int k, int swap, int first, int count,
+                                              int step, const f2 (&a2)[S::NP], f2 (&h)[S::NP]) {
+    for (int j0 = 0; j0 < count; j0 += 4) {
+        f2 e[4][S::NP];
+        float sum[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool any = at.live[k] && j0 + j < count;
+            const long long row = (at.n * Q.segs + first + (j0 + j) * step) * Q.channels + at.channel + k;
+            load_states<S>(Q.carry + row * Q.states, at.part, Q.states, any, swap, e[j]);
+            sum[j] = any ? Q.sums[row] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j0 + j >= count) continue;
+#pragma unroll
+            for (int i = 0; i < S::NP; ++i) h[i] = fma2(exp2_fast(pair(sum[j]) * a2[i]), h[i], e[j][i]);
+        }
+    }
+}
+
 enum ScanMode { kScanMain, kScanCarry, kScanCarryBack };
 
 // ---- forward ------------------------------------------------------------------------------
@@ -492,8 +515,10 @@ struct ScanTile {
 // Two buffers and one barrier a tile: a tile's values are formed after the one
 // before has been worked on, from copies that were under way meanwhile.  Tiles are
 // filled up with steps of size 0.
+// (Ten blocks a multiprocessor: 97 registers a thread.  Left to itself the main kernel
+// takes 110 and is a quarter slower, at 80 it is no faster.)
 template <class E, class S, int MODE>
-__global__ void __launch_bounds__(S::THREADS) scan_kernel(const __grid_constant__ ScanParams Q) {
+__global__ void __launch_bounds__(S::THREADS, MODE == kScanMain && S::P >= 4 ? 10 : 1) scan_kernel(const __grid_constant__ ScanParams Q) {
     constexpr int P = S::P, R = S::R, NP = S::NP, T = S::T, N = FourSums<P>::N;
     using Tile = ScanTile<E, S, MODE>;
     extern __shared__ __align__(16) char space[];
@@ -522,14 +547,7 @@ __global__ void __launch_bounds__(S::THREADS) scan_kernel(const __grid_constant_
         if (MODE != kScanMain) continue;
         if (Q.state != nullptr)
             load_states<S>(Q.state + at.n * Q.s_ldn + (at.channel + k) * Q.s_ldc, at.part, Q.states, at.live[k], 0, h[k]);
-        for (int j = 0; j < at.seg; ++j) {
-            const long long row = (at.n * Q.segs + j) * Q.channels + at.channel + k;
-            f2 e[NP];
-            load_states<S>(Q.carry + row * Q.states, at.part, Q.states, at.live[k], 0, e);
-            const f2 sum = pair(at.live[k] ? Q.sums[row] : 0.0f);
-#pragma unroll
-            for (int i = 0; i < NP; ++i) h[k][i] = fma2(exp2_fast(sum * a2[k][i]), h[k][i], e[i]);
-        }
+        pass_segments<S>(Q, at, k, 0, 0, at.seg, 1, a2[k], h[k]);
     }
     f2 bias[2], skip[2];
 #pragma unroll
@@ -650,9 +668,7 @@ __global__ void __launch_bounds__(S::THREADS) scan_kernel(const __grid_constant_
                 }
                 y_at += 4 * Q.y.ldt;
             }
-#ifdef CLOB
-            asm volatile("" ::: "memory");  // loads of later tokens stay behind
-#endif
+            asm volatile("" ::: "memory");  // loads of later tokens stay behind: their registers are the states'
         }
         if (left > T) {
             form(t0 + T, left - T, buf ^ 1);
@@ -797,14 +813,7 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
         for (int i = 0; i < NP; ++i) q[k][i] = da[k][i] = pair(0.0f);
         if (Q.dlast != nullptr)
             load_states<S>(Q.dlast + at.n * Q.dl_ldn + (at.channel + k) * Q.dl_ldc, at.part, Q.states, at.live[k], swap, q[k]);
-        for (int j = Q.segs - 1; j > at.seg; --j) {
-            const long long row = (at.n * Q.segs + j) * Q.channels + at.channel + k;
-            f2 e[NP];
-            load_states<S>(Q.carry + row * Q.states, at.part, Q.states, at.live[k], swap, e);
-            const f2 sum = pair(at.live[k] ? Q.sums[row] : 0.0f);
-#pragma unroll
-            for (int i = 0; i < NP; ++i) q[k][i] = fma2(exp2_fast(sum * a2[k][i]), q[k][i], e[i]);
-        }
+        pass_segments<S>(Q, at, k, swap, Q.segs - 1, Q.segs - 1 - at.seg, -1, a2[k], q[k]);
     }
     {
         float b[4] = {};
@@ -1057,74 +1066,128 @@ struct ScanJoinParams {
 constexpr int kJoinThreads = 256;
 __global__ void __launch_bounds__(kJoinThreads) scan_join_kernel(const __grid_constant__ ScanJoinParams Q);
 
-// One token of every sequence: x, dt, z, y are [n][channels].  A thread has read
-// its part of the state before it writes it, so state_out may be the state itself.
-template <class E, class S>
+// One token of every sequence: x, dt, z, y are [n][channels].  A thread has read its
+// part of a state before it writes it, so state_out may be the state itself.
+//
+// WHOLE: every access of a thread is one access of 16, 8 or 4 bytes and nothing has
+// to be asked: as many states as lanes have, blocks full of channels, parameters in
+// 32 bits, a gate.  A step moves 76 bytes for each channel and part, and the
+// general kernel's questions are five times its arithmetic (N64 C4096 bf16: 16 us
+// there).
+template <class E, class S, bool WHOLE>
 __global__ void __launch_bounds__(S::THREADS) scan_step_kernel(const __grid_constant__ ScanParams Q) {
     constexpr int P = S::P, R = S::R, NP = S::NP;
     griddep_wait();
     griddep_launch_dependents();
-    const ScanPlace<S> at(Q);
-    const auto element = [&](const TokenView &v, long long c) { return to_float(static_cast<const E *>(v.p)[at.n * v.ldn + c]); };
-    const auto two = [&](const TokenView &v, float (&e)[2]) {
+    f2 a2[2][NP], h[2][NP], b[2], c[2];
+    float x[2], dt[2], z[2], bias[2] = {}, skip[2] = {};
+    long long n;
+    int channel, part;
+    bool live[2] = {true, true};
+    if constexpr (WHOLE) {
+        n = blockIdx.y;
+        const int group = Q.groups == 1 ? 0 : static_cast<int>(blockIdx.x / static_cast<unsigned>(Q.tiles));
+        channel = static_cast<int>(blockIdx.x * S::CB + threadIdx.x / P * 2);
+        part = threadIdx.x % P;
+        const int at = channel * S::SP + part * R;
+        const auto two = [&](const TokenView &v, float (&e)[2]) {
+            const E *p = static_cast<const E *>(v.p) + n * v.ldn + channel;
+            E r[2];
+            memcpy(r, __builtin_assume_aligned(p, 2 * sizeof(E)), 2 * sizeof(E));
+            e[0] = to_float(r[0]);
+            e[1] = to_float(r[1]);
+        };
+        const auto quad = [&](const float *p, f2 (&v)[NP]) {
+            const float4 f = *reinterpret_cast<const float4 *>(p);
+            v[0] = pair(f.x, f.y);
+            v[NP - 1] = pair(f.z, f.w);
+        };
+        const float *state = Q.state + n * Q.s_ldn + at, *decay = static_cast<const float *>(Q.a) + at;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) e[k] = at.live[k] ? element(v, at.channel + k) : 0.0f;
-    };
-    f2 a2[2][NP], h[2][NP], delta[2], slope[2], raw[2], bias[2] = {pair(0.0f), pair(0.0f)};
-    float x[2], dt[2], z[2], d[2], b[2 * NP] = {}, c[2 * NP] = {}, y[2];
+        for (int k = 0; k < 2; ++k) quad(state + k * S::SP, h[k]);
+        two(Q.x, x);
+        two(Q.dt, dt);
+        two(Q.z, z);
+        const E *pb = static_cast<const E *>(Q.b.p) + n * Q.b.ldn + group * Q.b.ldg + part * R;
+        const E *pc = static_cast<const E *>(Q.c.p) + n * Q.c.ldn + group * Q.c.ldg + part * R;
+        const Four<E> fb = load_four<E>(pb, true, 4), fc = load_four<E>(pc, true, 4);
+        const float2 vb = *reinterpret_cast<const float2 *>(static_cast<const float *>(Q.bias) + channel);
+        const float2 vd = *reinterpret_cast<const float2 *>(static_cast<const float *>(Q.d) + channel);
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-        load_states<S>(Q.state + at.n * Q.s_ldn + (at.channel + k) * Q.s_ldc, at.part, Q.states, at.live[k], 0, h[k]);
-    two(Q.x, x);
-    two(Q.dt, dt);
-    if (Q.z.p != nullptr) two(Q.z, z);
+        for (int k = 0; k < 2; ++k) {
+            quad(decay + k * S::SP, a2[k]);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int s = at.part * R + r;
-        if (s >= Q.states) continue;
-        b[r] = element(Q.b, at.group * Q.b.ldg + s);
-        c[r] = element(Q.c, at.group * Q.c.ldg + s);
+            for (int i = 0; i < NP; ++i) a2[k][i] = a2[k][i] * pair(kLog2E);
+        }
+        floats_of<E>(fb, b);
+        floats_of<E>(fc, c);
+        bias[0] = vb.x, bias[1] = vb.y;
+        skip[0] = vd.x, skip[1] = vd.y;
+    } else {
+        const ScanPlace<S> at(Q);
+        n = at.n;
+        channel = at.channel;
+        part = at.part;
+        const auto two = [&](const TokenView &v, float (&e)[2]) {
+            const E *p = static_cast<const E *>(v.p) + n * v.ldn + channel;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) e[k] = at.live[k] ? to_float(p[k]) : 0.0f;
+        };
+        const auto pairs = [&](const TokenView &v, f2 (&e)[2]) {
+            const int s = part * R;
+            floats_of<E>(load_four<E>(static_cast<const E *>(v.p) + n * v.ldn + at.group * v.ldg + s, false, min(Q.states - s, R)), e);
+        };
+        two(Q.x, x);
+        two(Q.dt, dt);
+        if (Q.z.p != nullptr) two(Q.z, z);
+        pairs(Q.b, b);
+        pairs(Q.c, c);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            live[k] = at.live[k];
+            load_states<S>(Q.state + n * Q.s_ldn + (channel + k) * Q.s_ldc, part, Q.states, live[k], 0, h[k]);
+            load_decay<S>(Q, at, k, 0, a2[k]);
+            if (Q.bias != nullptr && live[k]) bias[k] = load_param(Q.bias, Q.bias_type, channel + k);
+            if (Q.d != nullptr && live[k]) skip[k] = load_param(Q.d, Q.d_type, channel + k);
+        }
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) load_decay<S>(Q, at, k, 0, a2[k]);
-    if (Q.bias != nullptr) {
-        float v[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) v[k] = at.live[k] ? load_param(Q.bias, Q.bias_type, at.channel + k) : 0.0f;
-        bias[0] = pair(v[0], v[1]);
-    }
-    raw[0] = pair(dt[0], dt[1]);
-    raw[1] = pair(0.0f);
-    scan_deltas<false>(Q.softplus, raw, bias, delta, slope);
-    split(delta[0], d[0], d[1]);
+    f2 delta = pair(dt[0], dt[1]) + pair(bias[0], bias[1]), slope;
+    if (Q.softplus) softplus2<false>(delta, delta, slope);
+    float d[2], y[2], gate[2] = {1.0f, 1.0f};
+    split(delta, d[0], d[1]);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         f2 s = pair(0.0f);
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            h[k][i] = fma2(exp2_fast(pair(d[k]) * a2[k][i]), h[k][i], pair(d[k] * x[k]) * pair(b[2 * i], b[2 * i + 1]));
-            s = fma2(pair(c[2 * i], c[2 * i + 1]), h[k][i], s);
+            h[k][i] = fma2(exp2_fast(pair(d[k]) * a2[k][i]), h[k][i], pair(d[k] * x[k]) * b[i]);
+            s = fma2(c[i], h[k][i], s);
         }
         y[k] = sum_of(s);
-        store_states<S>(Q.state_out + at.n * Q.so_ldn + (at.channel + k) * Q.so_ldc, at.part, Q.states, at.live[k], 0, h[k]);
+        float *out = Q.state_out + n * Q.so_ldn;
+        if constexpr (WHOLE) {
+            float4 f;
+            split(h[k][0], f.x, f.y);
+            split(h[k][NP - 1], f.z, f.w);
+            *reinterpret_cast<float4 *>(out + channel * S::SP + part * R + k * S::SP) = f;
+        } else {
+            store_states<S>(out + (channel + k) * Q.so_ldc, part, Q.states, live[k], 0, h[k]);
+        }
 #pragma unroll
         for (int o = 1; o < P; o *= 2) y[k] += __shfl_xor_sync(0xffffffffu, y[k], o);
+        y[k] = fmaf(skip[k], x[k], y[k]);
     }
-    if (at.part != 0) return;
-    float gate[2] = {1.0f, 1.0f};
-    if (Q.z.p != nullptr) {
-        f2 g, unused;
-        gate2<false>(pair(z[0], z[1]), g, unused);
+    if (part != 0) return;
+    if (WHOLE || Q.z.p != nullptr) {
+        f2 g;
+        gate2<false>(pair(z[0], z[1]), g, slope);
         split(g, gate[0], gate[1]);
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-        if (Q.d != nullptr && at.live[k]) y[k] = fmaf(load_param(Q.d, Q.d_type, at.channel + k), x[k], y[k]);
-    store_two<E>(token_at<E>(Q.y, at.n, 0) + at.channel, false, at.live, y[0] * gate[0], y[1] * gate[1]);
+    store_two<E>(token_at<E>(Q.y, n, 0) + channel, WHOLE, live, y[0] * gate[0], y[1] * gate[1]);
 }
 
 // ---- instances, one translation unit for each element type -----------------------------------
-enum ScanKernel { kMain, kCarry, kCarryBack, kGrad, kStep };
+enum ScanKernel { kMain, kCarry, kCarryBack, kGrad, kStep, kStepWhole };
 struct ScanLaunch {
     const void *fn;
     int threads;
@@ -1132,17 +1195,13 @@ struct ScanLaunch {
 };
 // Threads of a block of the gradient: what the tiles of few lanes take of shared
 // memory grows with the channels of a block.
-#ifndef FR
-#define FR 4
-#define FT 16
-#endif
-constexpr int kScanThreads = 64;
+constexpr int kScanThreads = 64, kScanStates = 4;  // states of a lane: with 8 the scan was slower by a third
 constexpr int grad_threads(int sp) { return sp >= 16 ? 128 : kScanThreads; }
 
 template <class E, int SP>
 ScanLaunch scan_instance(ScanKernel k) {
-    using S = ScanShape<SP, FR, kScanThreads, FT>;
-    using G = ScanShape<SP, 4, grad_threads(SP), kScanChunk>;
+    using S = ScanShape<SP, kScanStates, kScanThreads, 16>;
+    using G = ScanShape<SP, kScanStates, grad_threads(SP), kScanChunk>;
     switch (k) {
     case kMain:
         return {reinterpret_cast<const void *>(&scan_kernel<E, S, kScanMain>), S::THREADS, sizeof(ScanTile<E, S, kScanMain>)};
@@ -1152,7 +1211,10 @@ ScanLaunch scan_instance(ScanKernel k) {
         return {reinterpret_cast<const void *>(&scan_kernel<E, S, kScanCarryBack>), S::THREADS,
                 sizeof(ScanTile<E, S, kScanCarryBack>)};
     case kGrad: return {reinterpret_cast<const void *>(&scan_grad_kernel<E, G>), G::THREADS, sizeof(ScanGradTile<E, G>)};
-    default: return {reinterpret_cast<const void *>(&scan_step_kernel<E, S>), S::THREADS, 0};
+    case kStepWhole:
+        if constexpr (SP >= 4) return {reinterpret_cast<const void *>(&scan_step_kernel<E, S, true>), S::THREADS, 0};
+        else return {nullptr, 0, 0};  // not planned
+    default: return {reinterpret_cast<const void *>(&scan_step_kernel<E, S, false>), S::THREADS, 0};
     }
 }
 template <class E>

@@ -38,9 +38,6 @@ namespace {
 
 using namespace gcb;
 
-#ifndef WANT
-#define WANT 16LL
-#endif
 constexpr int kMostStates = 64;
 
 // A call's tensors: the descriptors with the same index as their views.
@@ -131,18 +128,19 @@ int padded_states(int64_t s) {
     return sp == 2 ? 4 : sp;
 }
 // Segments: as many as give each multiprocessor 16 blocks (24 in the gradient,
-// whose own kernel has half as many), of at least 64 tokens.
+// whose own kernel has half as many), of at least 32 tokens.  N1 L8192 C2048 bf16: 260 us
+// so, 281 with ten blocks, 273 with 20; N5 L777 C330 FP32: 35 us, 42 with 64 tokens.
 ScanPlan plan_scan(const ScanCall &c, int sms, bool backward) {
     ScanPlan p;
     p.type = c.x.type;
     p.sp = padded_states(c.states);
-    p.per_lane = std::min(p.sp, FR);
+    p.per_lane = std::min(p.sp, kScanStates);
     p.lanes = p.sp / p.per_lane;
     const int64_t cpg = c.c / c.groups;
     p.tiles = static_cast<int>(ceil_div(cpg, 2 * kScanThreads / p.lanes));
-    p.grad_tiles = static_cast<int>(ceil_div(cpg, 2 * grad_threads(p.sp) / (p.sp / std::min(p.sp, 4))));
+    p.grad_tiles = static_cast<int>(ceil_div(cpg, 2 * grad_threads(p.sp) / p.lanes));
     const long long blocks = std::max(1LL, static_cast<long long>(c.n) * c.groups * p.tiles);
-    const long long wanted = std::min(ceil_div((backward ? 24LL : WANT) * sms, blocks), static_cast<long long>(c.l / 64));
+    const long long wanted = std::min(ceil_div((backward ? 24LL : 16LL) * sms, blocks), static_cast<long long>(c.l / 32));
     p.seg_len = std::max(1LL, gcb::round_up(ceil_div(c.l, std::max(1LL, wanted)), 16));
     p.segs = static_cast<int>(std::max(1LL, ceil_div(c.l, p.seg_len)));
     p.blocks = blocks * p.segs;
@@ -466,16 +464,29 @@ int gc_b200_selective_scan_step(const gc_b200_scan_args *q, gc_tensor *y, gc_ten
         return st;
     DeviceFacts facts;
     if ((st = device_facts(dev, facts)) != GC_OK) return st;
-    const ScanPlan plan = plan_scan(c, facts.sms, false);
+    ScanPlan plan = plan_scan(c, facts.sms, false);
+    plan.segs = 1;
     ScanParams P{};
     fill(P, q, c, plan, true);
     P.y = tokens_of(c.y, true);
     set_state_out(P, out);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
-    P.segs = 1;
-    if ((st = launch(kStep, plan, P, dev, facts, reinterpret_cast<cudaStream_t>(stream), e)) != GC_OK) return st;
-    return launched(e, PlanRecord::kSequence, "selective_scan_step", plan.blocks, kScanThreads, 0, plan.lanes, plan.per_lane,
-                    plan.segs, 1);
+    const int channels = 2 * kScanThreads / plan.lanes;  // of a block
+    bool whole = plan.sp >= 4 && c.states == plan.sp && P.cpg % channels == 0 && c.n <= 65535 && q->z != nullptr &&
+                 fours({&c.x, &c.dt, &c.z, &c.y}, c) && group_aligned(c.b, 4) && group_aligned(c.bc, 4);
+    for (const gc_tensor *t : {q->a, q->d, q->dt_bias}) whole = whole && t != nullptr && t->dtype == GC_F32 && aligned16(t->data);
+    for (const Strided *v : {static_cast<const Strided *>(&c.state), static_cast<const Strided *>(&out)})
+        whole = whole && group_aligned(*v, 4) && v->s[1] == c.states;
+    if (whole) {
+        const ScanLaunch l = launch_of(kStepWhole, plan.type, plan.sp);
+        void *args[] = {&P};
+        e = launch_pdl(l.fn, dim3(static_cast<unsigned>(P.groups * P.tiles), static_cast<unsigned>(c.n)), dim3(l.threads), args, 0, s);
+    } else if ((st = launch(kStep, plan, P, dev, facts, s, e)) != GC_OK) {
+        return st;
+    }
+    return launched(e, PlanRecord::kSequence, "selective_scan_step", P.n * P.groups * P.tiles, kScanThreads, whole ? 1 : 0,
+                    plan.lanes, plan.per_lane, 1, 1);
 } catch (...) {
     return internal_error();
 }

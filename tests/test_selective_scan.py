@@ -173,7 +173,9 @@ def test_nothing(native, torch_cuda, shape):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize('shape', [(1, 4, 16, 1), (5, 33, 16, 1), (3, 200, 7, 2), (2, 9, 64, 3), (300, 12, 1, 1), (2, 140, 32, 1)])
+@pytest.mark.parametrize('shape', [(1, 4, 16, 1), (5, 33, 16, 1), (3, 200, 7, 2), (2, 9, 64, 3), (300, 12, 1, 1), (2, 140, 32, 1),
+                                   # blocks full of channels, as many states as lanes have: every access whole
+                                   (7, 64, 16, 2), (2, 128, 4, 1), (3, 64, 8, 1), (2, 32, 32, 2), (2, 16, 64, 1)])
 @pytest.mark.parametrize('dtype', TYPES)
 def test_one_token(native, torch_cuda, shape, dtype):
     """Step by step against one call's reference, in place and to another tensor."""
