@@ -78,12 +78,14 @@ struct RowPlan {
 const char *const kDenseParams = "parameters must be dense";
 
 // Vectors of a row for each thread, by how many of the threads' places stay empty,
-// then by the longest run of a thread: sums between threads cost more than those
-// in one (96 columns FP32 in teams of 8 with three vectors, 32 with one: 24 us and
-// 15 at 100352 rows).  A team of up to 32 threads has no barriers; the gradient,
-// which holds its columns' sums in registers, goes over to whole blocks earlier.
-// Single elements are taken four or sixteen (backwards eight) a thread.
-void plan_rows(int c, int type, bool vec, bool backward, RowPlan &p) {
+// then by the longest run of a thread: sums between threads cost more than those in
+// one (100352 rows of 96 FP32: 18 us in teams of 4 with six vectors each, 24 in teams
+// of 8 with three), unless the rows are few, when each thread's own work is what
+// takes the time (196 rows of 384 bf16: 6.0 us with six, 4.0 with three).  A team of
+// up to 32 threads has no barriers; the gradient, which holds its columns' sums in
+// registers, goes over to whole blocks earlier.  Single elements are taken four or
+// sixteen (backwards eight) a thread.
+void plan_rows(int c, int type, bool vec, bool backward, bool few, RowPlan &p) {
     p.type = type;
     p.vec = vec;
     p.v = !vec ? 1 : type == kElemF32 ? 4 : 8;
@@ -92,7 +94,9 @@ void plan_rows(int c, int type, bool vec, bool backward, RowPlan &p) {
     if (vec) {
         const int most = backward ? (p.v == 8 ? 3 : 4) : 8;
         long long best = 0;
-        for (const int nv : {8, 6, 4, 3, 2, 1}) {
+        static const int longest[] = {8, 6, 4, 3, 2, 1}, shortest[] = {4, 3, 6, 8, 2, 1};
+        for (int i = 0; i < 6; ++i) {
+            const int nv = few ? shortest[i] : longest[i];
             if (nv > most) continue;
             int team = 1;
             while (static_cast<long long>(team) * nv < vcols) team *= 2;
@@ -234,7 +238,8 @@ int gc_b200_layer_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
     DeviceFacts facts;
     if ((st = device_facts(dev, facts)) != GC_OK) return st;
     RowPlan plan;
-    plan_rows(static_cast<int>(c), v[0].t.type, vectors({&v[0], &v[1]}), false, plan);
+    plan_rows(static_cast<int>(c), v[0].t.type, vectors({&v[0], &v[1]}), false,
+              v[0].rows <= 4096LL * facts.sms / std::max<int64_t>(c, 1), plan);
     LayerNormParams P{};
     P.x = v[0].t.data;
     P.x_ld = v[0].ld;
@@ -250,8 +255,10 @@ int gc_b200_layer_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
     P.aligned = aligned_params({gamma, beta}, plan.v) ? 1 : 0;
     P.stats = stats != nullptr ? static_cast<float2 *>(stats->data) : nullptr;
     const void *fn = row_kernel(plan, false);
-    // as many blocks as a multiprocessor has threads for; each takes rows in turn
-    const long long grid = std::min(ceil_div(P.rows, plan.threads / plan.team), 2048LL / plan.threads * facts.sms);
+    // Four times the blocks that a multiprocessor has threads for, each taking rows in
+    // turn: the multiprocessors are not served alike (16384 rows of 2048 bf16: 32 us,
+    // 35 with a quarter of the blocks).
+    const long long grid = std::min(ceil_div(P.rows, plan.threads / plan.team), 8192LL / plan.threads * facts.sms);
     void *args[] = {&P};
     const cudaError_t e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(plan.threads), args, 0,
                                      reinterpret_cast<cudaStream_t>(stream));
@@ -273,7 +280,7 @@ int gc_b200_layer_norm_backward_workspace(const gc_tensor *dy, const gc_tensor *
     if ((st = current_facts(facts)) != GC_OK) return st;
     RowPlan plan;
     const int c = static_cast<int>(x->dims[x->rank - 1]);
-    plan_rows(c, v[0].t.type, vectors({&v[0], &v[1], &v[2]}), true, plan);
+    plan_rows(c, v[0].t.type, vectors({&v[0], &v[1], &v[2]}), true, false, plan);
     *bytes = up16(static_cast<uint64_t>(grad_blocks(plan, v[0].rows, facts.sms)) * 2 * c * sizeof(float));
     return gc_error(GC_OK, "");
 } catch (...) {
@@ -310,7 +317,7 @@ int gc_b200_layer_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
     DeviceFacts facts;
     if ((st = device_facts(dev, facts)) != GC_OK) return st;
     RowPlan plan;
-    plan_rows(static_cast<int>(c), v[0].t.type, vectors({&v[0], &v[1], &v[2]}), true, plan);
+    plan_rows(static_cast<int>(c), v[0].t.type, vectors({&v[0], &v[1], &v[2]}), true, false, plan);
     const long long grid = grad_blocks(plan, v[0].rows, facts.sms);
     if (sums) {
         const uint64_t need = up16(static_cast<uint64_t>(grid) * 2 * c * sizeof(float));
