@@ -9,6 +9,8 @@
 // power of two of at most 32, several to a warp, or a whole block.  The variance
 // is the mean of squares about the mean, from the values in registers.
 #pragma once
+#include <cstring>
+
 #include "norm_util.cuh"
 
 namespace gcb {
@@ -333,6 +335,241 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_grad_kernel(const __grid_
     for (int i = threadIdx.x; i < 2 * P.c; i += blockDim.x) {
         float s = joined[i];
         for (int w = 1; w < warps; ++w) s += joined[2 * w * P.c + i];
+        out[i] = s;
+    }
+}
+
+// ---- rows that do not start on 16 bytes -----------------------------------------------
+// Rows of odd length lie one after the other, so each starts at a place of its own
+// within 16 bytes.  A thread takes the aligned vectors that cover a row; its first
+// and last ones hold columns of the neighbouring rows too, and are read and written
+// element by element.  (Eight times fewer accesses than single elements: 8191 rows of
+// 1001 bf16 37 us there, see the launch.)  x, dy and the result start alike.
+template <class T>
+struct EdgeVector {
+    static constexpr int V = kVec<T>;
+    int low, c;  // the vector's first column (negative in a row's first vector), columns of a row
+    __device__ __forceinline__ bool any() const { return low < c; }
+    __device__ __forceinline__ bool full() const { return low >= 0 && low + V <= c; }
+    __device__ __forceinline__ bool has(int k) const { return low + k >= 0 && low + k < c; }
+    __device__ __forceinline__ Raw<T, V> load(const T *row) const {
+        Raw<T, V> r;
+        if (full()) {
+            r = load_raw<T, V>(row + low);
+        } else {
+            T e[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) e[k] = has(k) ? row[low + k] : from_float<T>(0.0f);
+            memcpy(&r.u, e, sizeof(r.u));
+        }
+        return r;
+    }
+    __device__ __forceinline__ void store(T *row, const Lanes<V> &l) const {
+        if (full()) {
+            store_lanes<T, V>(row + low, l);
+        } else {
+            float v[V];
+            values_of<V>(l, v);
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (has(k)) row[low + k] = from_float<T>(v[k]);
+        }
+    }
+};
+// Values without those that are none of the row's.
+template <class T>
+__device__ __forceinline__ void mask_edges(const EdgeVector<T> &at, Lanes<kVec<T>> &l) {
+    if (at.full()) return;
+    float v[kVec<T>];
+    values_of<kVec<T>>(l, v);
+#pragma unroll
+    for (int k = 0; k < kVec<T>; ++k)
+        if (!at.has(k)) v[k] = 0.0f;
+    l = lanes_of<kVec<T>>(v);
+}
+// Columns in shared memory: a gap after every vector, so that threads, which read a
+// vector apart whatever the row's place is, meet different banks.
+template <int V>
+__device__ __forceinline__ int gapped(int c) { return c + c / V; }
+template <class T>
+__device__ __forceinline__ Lanes<kVec<T>> edge_params(const EdgeVector<T> &at, const float *p) {
+    float v[kVec<T>];
+#pragma unroll
+    for (int k = 0; k < kVec<T>; ++k) v[k] = at.has(k) ? p[gapped<kVec<T>>(at.low + k)] : 0.0f;
+    return lanes_of<kVec<T>>(v);
+}
+// A row's place within 16 bytes, in elements.
+template <class T>
+__device__ __forceinline__ int row_phase(const T *row) {
+    return static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
+}
+
+// Dynamic shared memory: gamma and beta, gapped.  vcols: vectors that may touch a row.
+template <class T, int NV>
+__global__ void __launch_bounds__(kRowMost) layer_norm_edges_kernel(const __grid_constant__ LayerNormParams P) {
+    constexpr int V = kVec<T>, NP = Lanes<V>::kPairs;
+    extern __shared__ float params[];
+    __shared__ float buf[2 * (kRowMost / 32)];
+    griddep_wait();
+    griddep_launch_dependents();
+    float *gamma = params, *beta = params + gapped<V>(P.c - 1) + 1;
+    for (int i = threadIdx.x; i < P.c; i += blockDim.x) {
+        gamma[gapped<V>(i)] = P.gamma != nullptr ? load_param(P.gamma, P.gamma_type, i) : 1.0f;
+        beta[gapped<V>(i)] = P.beta != nullptr ? load_param(P.beta, P.beta_type, i) : 0.0f;
+    }
+    __syncthreads();
+    const int teams = blockDim.x / P.team, team = threadIdx.x / P.team, lane = threadIdx.x - team * P.team;
+    const long long all = static_cast<long long>(gridDim.x) * teams;
+    const float inv = 1.0f / static_cast<float>(P.c);
+    int turn = 0;
+    for (long long first = static_cast<long long>(blockIdx.x) * teams; first < P.rows; first += all) {
+        const long long row = first + team;
+        const T *x = static_cast<const T *>(P.x) + row * P.x_ld;
+        const int phase = row_phase(x), count = row < P.rows ? P.c : -V;  // no columns in a row that is none
+        Lanes<V> e[NV];
+        float s[1] = {0.0f}, q[1] = {0.0f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const EdgeVector<T> at{(lane + j * P.team) * V - phase, count};
+            if (at.any()) e[j] = lanes_of_raw<T, V>(at.load(x));
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (EdgeVector<T>{(lane + j * P.team) * V - phase, count}.any()) s[0] += lanes_sum<V>(e[j]);
+        team_sums<1>(s, P.team, buf, turn);
+        const float mean = s[0] * inv;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const EdgeVector<T> at{(lane + j * P.team) * V - phase, count};
+            if (!at.any()) continue;
+            f2 sum = pair(0.0f);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) e[j].p[i] = e[j].p[i] + pair(-mean);
+            mask_edges<T>(at, e[j]);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) sum = fma2(e[j].p[i], e[j].p[i], sum);
+            float a, b;
+            split(sum, a, b);
+            q[0] += a + b;
+        }
+        team_sums<1>(q, P.team, buf, turn);
+        const float rstd = 1.0f / sqrtf(fmaf(q[0], inv, P.eps));
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const EdgeVector<T> at{(lane + j * P.team) * V - phase, count};
+            if (!at.any()) continue;
+            const Lanes<V> g = edge_params<T>(at, gamma), b = edge_params<T>(at, beta);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) e[j].p[i] = fma2(e[j].p[i] * pair(rstd), g.p[i], b.p[i]);
+            at.store(static_cast<T *>(P.y) + row * P.y_ld, e[j]);
+        }
+        if (P.stats != nullptr && lane == 0 && row < P.rows) P.stats[row] = make_float2(mean, rstd);
+    }
+}
+
+// A team's rows all start at the same place (the launch sees to the step), so that
+// its columns, their sums and gamma stay in its threads.  Dynamic shared memory:
+// [teams][2][c] values where a row takes a warp.
+template <class T, int NV>
+__global__ void __launch_bounds__(kRowMost) layer_norm_edges_grad_kernel(const __grid_constant__ LayerNormParams P) {
+    constexpr int V = kVec<T>, NP = Lanes<V>::kPairs;
+    extern __shared__ float joined[];
+    __shared__ float buf[2 * (kRowMost / 32) * 2];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int teams = blockDim.x / P.team, team = threadIdx.x / P.team, lane = threadIdx.x - team * P.team;
+    const long long all = static_cast<long long>(gridDim.x) * teams;
+    const float inv = 1.0f / static_cast<float>(P.c);
+    const long long mine = static_cast<long long>(blockIdx.x) * teams + team;
+    const int phase = row_phase(static_cast<const T *>(P.x) + mine * P.x_ld);
+    Lanes<V> gamma[NV], sum_g[NV], sum_b[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const EdgeVector<T> at{(lane + j * P.team) * V - phase, P.c};
+        float v[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            v[k] = 0.0f;
+            if (at.has(k)) v[k] = P.gamma != nullptr ? load_param(P.gamma, P.gamma_type, at.low + k) : 1.0f;
+        }
+        gamma[j] = lanes_of<V>(v);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) sum_g[j].p[i] = sum_b[j].p[i] = pair(0.0f);
+    }
+    int turn = 0;
+    for (long long first = static_cast<long long>(blockIdx.x) * teams; first < P.rows; first += all) {
+        const long long row = first + team;
+        const int count = row < P.rows ? P.c : -V;
+        const T *x = static_cast<const T *>(P.x) + row * P.x_ld, *dy = static_cast<const T *>(P.dy) + row * P.dy_ld;
+        Raw<T, V> rx[NV], rg[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const EdgeVector<T> at{(lane + j * P.team) * V - phase, count};
+            if (at.any()) {
+                rx[j] = at.load(x);
+                rg[j] = at.load(dy);
+            }
+        }
+        const float2 st = row < P.rows ? P.stats[row] : make_float2(0.0f, 0.0f);
+        float sums[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const EdgeVector<T> at{(lane + j * P.team) * V - phase, count};
+            if (!at.any()) continue;
+            // where a place is no column of the row dy and gamma are 0
+            const Lanes<V> e = lanes_of_raw<T, V>(rx[j]), d = lanes_of_raw<T, V>(rg[j]);
+            f2 s1 = pair(0.0f), s2 = pair(0.0f);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const f2 xhat = (e.p[i] + pair(-st.x)) * pair(st.y), g = d.p[i] * gamma[j].p[i];
+                s1 = s1 + g;
+                s2 = fma2(g, xhat, s2);
+                sum_g[j].p[i] = fma2(d.p[i], xhat, sum_g[j].p[i]);
+                sum_b[j].p[i] = sum_b[j].p[i] + d.p[i];
+            }
+            float a, b;
+            split(s1, a, b);
+            sums[0] += a + b;
+            split(s2, a, b);
+            sums[1] += a + b;
+        }
+        team_sums<2>(sums, P.team, buf, turn);
+        const f2 m1 = pair(-sums[0] * inv), m2 = pair(-sums[1] * inv);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const EdgeVector<T> at{(lane + j * P.team) * V - phase, count};
+            if (!at.any()) continue;
+            const Lanes<V> e = lanes_of_raw<T, V>(rx[j]), d = lanes_of_raw<T, V>(rg[j]);
+            Lanes<V> o;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const f2 xhat = (e.p[i] + pair(-st.x)) * pair(st.y);
+                o.p[i] = pair(st.y) * fma2(xhat, m2, fma2(d.p[i], gamma[j].p[i], m1));
+            }
+            at.store(static_cast<T *>(P.y) + row * P.y_ld, o);
+        }
+    }
+    if (P.part == nullptr) return;
+    float *out = P.part + static_cast<long long>(blockIdx.x) * 2 * P.c;
+    float *own = P.team > 32 ? out : joined + team * 2 * P.c;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const EdgeVector<T> at{(lane + j * P.team) * V - phase, P.c};
+        float g[V], b[V];
+        values_of<V>(sum_g[j], g);
+        values_of<V>(sum_b[j], b);
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (at.has(k)) {
+                own[at.low + k] = g[k];
+                own[P.c + at.low + k] = b[k];
+            }
+    }
+    if (P.team > 32) return;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * P.c; i += blockDim.x) {
+        float s = joined[i];
+        for (int w = 1; w < teams; ++w) s += joined[2 * w * P.c + i];
         out[i] = s;
     }
 }

@@ -70,6 +70,7 @@ int check_row_stats(const gc_tensor *t, const gc_tensor *x, long long rows) {
 
 struct RowPlan {
     bool vec = false, whole = false;  // whole: rows too long for registers
+    bool edges = false;               // rows that start anywhere within 16 bytes, in vectors all the same
     int type = 0, v = 1, nv = 1, team = 1, threads = kRowThreads;
     size_t smem = 0;
     long long blocks = 0;
@@ -160,8 +161,52 @@ const void *backward_typed(int nv) {
         }
     }
 }
+// Rows that start anywhere: aligned vectors cover a row, one more than it would need,
+// in teams of a warp at least.  False where that does not apply.
+bool plan_edges(int c, int type, bool backward, RowPlan &p) {
+    p = RowPlan{};
+    p.type = type;
+    p.v = type == kElemF32 ? 4 : 8;
+    const int vcols = (c + p.v - 2) / p.v + 1, most = backward ? (p.v == 8 ? 2 : 4) : 4;
+    if (vcols <= 32 || c > 4096) return false;
+    p.edges = true;
+    for (p.nv = 1; p.nv < most && vcols > 32 * p.nv;) p.nv *= 2;
+    if (vcols <= 32 * p.nv) {
+        p.team = 32;
+        p.threads = kRowThreads;
+        if (backward) p.smem = static_cast<size_t>(p.threads / 32) * 2 * c * sizeof(float);
+    } else {
+        for (p.nv = backward ? 1 : 2; p.nv < most && ceil_div(vcols, p.nv) > kRowMost;) p.nv *= 2;
+        if (ceil_div(vcols, p.nv) > kRowMost) return false;
+        p.team = p.threads = static_cast<int>(round_up(ceil_div(vcols, p.nv), 32));
+    }
+    if (!backward) p.smem = 2 * static_cast<size_t>((c - 1) + (c - 1) / p.v + 1) * sizeof(float);
+    return true;
+}
+// Whether x, dy and the result start at the same place within 16 bytes in every row.
+bool start_alike(std::initializer_list<const Rows *> views) {
+    const Rows *first = *views.begin();
+    const int size = elem_size(first->t.type);
+    for (const Rows *v : views)
+        if ((reinterpret_cast<uintptr_t>(v->t.data) - reinterpret_cast<uintptr_t>(first->t.data)) % 16 != 0 ||
+            (v->rows > 1 && (v->ld - first->ld) * size % 16 != 0))
+            return false;
+    return true;
+}
+template <class T>
+const void *edges_kernel(int nv, bool backward) {
+    if (backward)
+        return nv == 1   ? reinterpret_cast<const void *>(&layer_norm_edges_grad_kernel<T, 1>)
+               : nv == 2 ? reinterpret_cast<const void *>(&layer_norm_edges_grad_kernel<T, 2>)
+                         : reinterpret_cast<const void *>(&layer_norm_edges_grad_kernel<T, sizeof(T) == 4 ? 4 : 2>);
+    return nv == 1   ? reinterpret_cast<const void *>(&layer_norm_edges_kernel<T, 1>)
+           : nv == 2 ? reinterpret_cast<const void *>(&layer_norm_edges_kernel<T, 2>)
+                     : reinterpret_cast<const void *>(&layer_norm_edges_kernel<T, 4>);
+}
+
 template <class T>
 const void *row_kernel(const RowPlan &p, bool backward) {
+    if (p.edges) return edges_kernel<T>(p.nv, backward);
     if (p.whole)
         return backward ? reinterpret_cast<const void *>(&layer_norm_long_grad_kernel<T>)
                         : reinterpret_cast<const void *>(&layer_norm_long_kernel<T>);
@@ -178,8 +223,10 @@ const void *row_kernel(const RowPlan &p, bool backward) {
 // more than 64 rows.
 long long grad_blocks(const RowPlan &p, long long rows, int sms) {
     const int teams = p.threads / p.team;
-    return std::max(std::min(ceil_div(rows, teams), 2LL * sms * (kRowMost / p.threads)),
-                    ceil_div(rows, static_cast<long long>(kSumRun) * teams));
+    const long long blocks = std::max(std::min(ceil_div(rows, teams), 2LL * sms * (kRowMost / p.threads)),
+                                      ceil_div(rows, static_cast<long long>(kSumRun) * teams));
+    // every eighth row at most starts at the same place: a team's rows lie so far apart
+    return p.edges ? round_up(blocks, 8) : blocks;
 }
 
 // Whether the parameters can be read 16 bytes at a time (4 or 8 columns; their
@@ -188,6 +235,15 @@ bool aligned_params(std::initializer_list<const gc_tensor *> params, int v) {
     for (const gc_tensor *t : params)
         if (t != nullptr && (!aligned16(t->data) || (v == 4 && t->dtype != GC_F32))) return false;
     return true;
+}
+
+bool vectors(std::initializer_list<const Rows *> views);
+RowPlan plan_backward(int c, const Rows (&v)[3]) {
+    RowPlan plan;
+    const bool vec = vectors({&v[0], &v[1], &v[2]});
+    if (vec || !start_alike({&v[0], &v[1], &v[2]}) || !plan_edges(c, v[0].t.type, true, plan))
+        plan_rows(c, v[0].t.type, vec, true, false, plan);
+    return plan;
 }
 
 bool vectors(std::initializer_list<const Rows *> views) {
@@ -238,8 +294,9 @@ int gc_b200_layer_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
     DeviceFacts facts;
     if ((st = device_facts(dev, facts)) != GC_OK) return st;
     RowPlan plan;
-    plan_rows(static_cast<int>(c), v[0].t.type, vectors({&v[0], &v[1]}), false,
-              v[0].rows <= 4096LL * facts.sms / std::max<int64_t>(c, 1), plan);
+    const bool vec = vectors({&v[0], &v[1]});
+    if (vec || !start_alike({&v[0], &v[1]}) || !plan_edges(static_cast<int>(c), v[0].t.type, false, plan))
+        plan_rows(static_cast<int>(c), v[0].t.type, vec, false, v[0].rows <= 4096LL * facts.sms / std::max<int64_t>(c, 1), plan);
     LayerNormParams P{};
     P.x = v[0].t.data;
     P.x_ld = v[0].ld;
@@ -258,11 +315,11 @@ int gc_b200_layer_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
     // Four times the blocks that a multiprocessor has threads for, each taking rows in
     // turn: the multiprocessors are not served alike (16384 rows of 2048 bf16: 32 us,
     // 35 with a quarter of the blocks).
-    const long long grid = std::min(ceil_div(P.rows, plan.threads / plan.team), 8192LL / plan.threads * facts.sms);
+    const long long grid = std::min(ceil_div(P.rows, plan.threads / plan.team), (plan.edges ? 2048LL : 8192LL) / plan.threads * facts.sms);
     void *args[] = {&P};
-    const cudaError_t e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(plan.threads), args, 0,
+    const cudaError_t e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(plan.threads), args, plan.smem,
                                      reinterpret_cast<cudaStream_t>(stream));
-    return launched(e, PlanRecord::kSequence, plan.whole ? "layer_norm_long" : "layer_norm", grid, plan.threads,
+    return launched(e, PlanRecord::kSequence, plan.whole ? "layer_norm_long" : plan.edges ? "layer_norm_edges" : "layer_norm", grid, plan.threads,
                     plan.vec ? 1 : 0, plan.team, plan.nv, 1, 1);
 } catch (...) {
     return internal_error();
@@ -278,9 +335,8 @@ int gc_b200_layer_norm_backward_workspace(const gc_tensor *dy, const gc_tensor *
     if (v[0].t.empty) return gc_error(GC_OK, "");
     DeviceFacts facts;
     if ((st = current_facts(facts)) != GC_OK) return st;
-    RowPlan plan;
     const int c = static_cast<int>(x->dims[x->rank - 1]);
-    plan_rows(c, v[0].t.type, vectors({&v[0], &v[1], &v[2]}), true, false, plan);
+    const RowPlan plan = plan_backward(c, v);
     *bytes = up16(static_cast<uint64_t>(grad_blocks(plan, v[0].rows, facts.sms)) * 2 * c * sizeof(float));
     return gc_error(GC_OK, "");
 } catch (...) {
@@ -316,8 +372,7 @@ int gc_b200_layer_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
     }
     DeviceFacts facts;
     if ((st = device_facts(dev, facts)) != GC_OK) return st;
-    RowPlan plan;
-    plan_rows(static_cast<int>(c), v[0].t.type, vectors({&v[0], &v[1], &v[2]}), true, false, plan);
+    const RowPlan plan = plan_backward(static_cast<int>(c), v);
     const long long grid = grad_blocks(plan, v[0].rows, facts.sms);
     if (sums) {
         const uint64_t need = up16(static_cast<uint64_t>(grid) * 2 * c * sizeof(float));
@@ -360,7 +415,7 @@ int gc_b200_layer_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
         e = launch_pdl(reinterpret_cast<const void *>(&sum_rows_kernel), dim3(static_cast<unsigned>(2 * ceil_div(c, 32))),
                        dim3(kSumWarps * 32), sum_args, 0, s);
     }
-    return launched(e, PlanRecord::kSequence, plan.whole ? "layer_norm_long_backward" : "layer_norm_backward", grid,
+    return launched(e, PlanRecord::kSequence, plan.whole ? "layer_norm_long_backward" : plan.edges ? "layer_norm_edges_backward" : "layer_norm_backward", grid,
                     plan.threads, plan.vec ? 1 : 0, plan.team, plan.nv, 1, sums ? 2 : 1);
 } catch (...) {
     return internal_error();

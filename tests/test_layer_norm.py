@@ -15,7 +15,10 @@ TYPES = {'f32': torch.float32, 'f16': torch.float16, 'bf16': torch.bfloat16}
 # than one turn of the blocks
 SHAPES = [(1, 1), (3, 3), (5, 8), (70, 16), (33, 40), (257, 96), (50, 256), (19, 384), (21, 512), (40, 768), (9, 1024),
           (17, 1001), (6, 2048), (3, 2056), (4, 4096), (5, 4104), (3, 8192), (2, 8200), (3, 129), (4, 2047), (3, 6001),
-          (2, 9001), (2, 20000), (20000, 12), (9000, 33), (2500, 600)]
+          (2, 9001), (2, 20000), (20000, 12), (9000, 33), (2500, 600),
+          # odd lengths in aligned vectors: one, two and four a thread, a warp and blocks as teams, rows of every
+          # place within 16 bytes, more than one turn
+          (11, 259), (300, 515), (1700, 333), (70, 1023), (33, 4095), (9, 2053), (5000, 135), (40, 510), (23, 254)]
 
 
 def make(shape, dtype, seed=0, params=torch.float32):
