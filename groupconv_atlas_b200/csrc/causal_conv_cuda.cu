@@ -147,7 +147,7 @@ int opt_in_ring(int dev, const void *fn, size_t bytes, const DeviceFacts &facts)
 
 // Tokens of a thread: 16 to 64, as many as leave a wave of threads.  Each thread
 // loads its weights and the window in front of its stretch: shorter stretches were
-// no faster (N8 L2048 C2048 bf16 forward 37 us at 32 and at 64, gradient 103 and 98).
+// no faster (N8 L2048 C2048 bf16: forward the same at 32 and at 64, gradient 5 % more at 32).
 int stretch_of(const ConvCall &call, int v, int sms, bool backward) {
     const long long threads = call.n * ceil_div(call.c, v), wanted = (backward ? 384LL : 768LL) * sms;
     long long stretch = backward ? 128 : 64;

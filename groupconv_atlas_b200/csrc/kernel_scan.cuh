@@ -20,6 +20,11 @@
 // sequence is cut into segments: a first launch gives each segment's effect on
 // the state (what it adds, and the sum of its deltas, whose product with A is its
 // decay's logarithm), from which every block forms the state that it starts with.
+//
+// N4 L2048 C2048 S16 bf16, kernel after kernel: segments' effects 91 us, scan 176;
+// backwards 98 and 372, sums 30.  The exponentials alone would take 58 us in each;
+// shared memory (every lane reads each product, B and C of its states) is 60 to
+// 70 % busy, the special-function unit 46 %.
 #pragma once
 #include <cstring>
 #include <type_traits>
@@ -515,10 +520,13 @@ struct ScanTile {
 // Two buffers and one barrier a tile: a tile's values are formed after the one
 // before has been worked on, from copies that were under way meanwhile.  Tiles are
 // filled up with steps of size 0.
-// (Ten blocks a multiprocessor: 97 registers a thread.  Left to itself the main kernel
-// takes 110 and is a quarter slower, at 80 it is no faster.)
+// Blocks a multiprocessor, by what registers they leave: with 96 the main kernel is a
+// quarter faster than with the 110 that it would take, and no slower than with 80.  The
+// other modes would take 240 and get 160, with blocks of more than one at a time left on a
+// multiprocessor (N1 L8192 C2048 S16 bf16, whole call: 257 us left to itself, 245 with 160,
+// 261 with 128, 272 with 72; the training step of N4 L2048 C2048 771, 738, 745, 737).
 template <class E, class S, int MODE>
-__global__ void __launch_bounds__(S::THREADS, MODE == kScanMain && S::P >= 4 ? 10 : 1) scan_kernel(const __grid_constant__ ScanParams Q) {
+__global__ void __launch_bounds__(S::THREADS, S::P < 4 ? 8 : MODE == kScanMain ? 10 : 6) scan_kernel(const __grid_constant__ ScanParams Q) {
     constexpr int P = S::P, R = S::R, NP = S::NP, T = S::T, N = FourSums<P>::N;
     using Tile = ScanTile<E, S, MODE>;
     extern __shared__ __align__(16) char space[];
@@ -1200,7 +1208,8 @@ constexpr int grad_threads(int sp) { return sp >= 16 ? 128 : kScanThreads; }
 
 template <class E, int SP>
 ScanLaunch scan_instance(ScanKernel k) {
-    using S = ScanShape<SP, kScanStates, kScanThreads, 16>;
+    // few lanes mean many channels a block, whose tiles take the shared memory of blocks
+    using S = ScanShape<SP, kScanStates, kScanThreads, SP >= 16 ? 16 : 8>;
     using G = ScanShape<SP, kScanStates, grad_threads(SP), kScanChunk>;
     switch (k) {
     case kMain:
