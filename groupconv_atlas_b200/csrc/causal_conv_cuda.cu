@@ -355,9 +355,7 @@ int gc_b200_causal_conv_backward(const gc_tensor *dy, const gc_tensor *x, const 
         S.out[P.taps] = dbias != nullptr ? dbias->data : nullptr;
         S.type[P.taps] = dbias != nullptr ? elem_type(dbias->dtype) : kElemF32;
         S.mul[P.taps] = 1;
-        void *sum_args[] = {&S};
-        e = launch_pdl(reinterpret_cast<const void *>(&sum_rows_kernel),
-                       dim3(static_cast<unsigned>(S.planes * ceil_div(call.c, 32))), dim3(kSumWarps * 32), sum_args, 0, s);
+        e = launch_sum_rows(S, s);
     }
     return launched(e, PlanRecord::kSequence, "causal_conv_backward", grid, kConvThreads, vec ? 1 : 0, P.cols, P.stretch,
                     P.segs, sums ? 2 : 1);

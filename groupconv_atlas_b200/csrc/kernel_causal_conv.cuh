@@ -10,7 +10,7 @@
 // the window in front of each thread's stretch, which its neighbour's reads have
 // brought into the caches).  The kernels hold KT taps, K or more; what a missing
 // tap would multiply is left out, not multiplied by 0.  N8 L2048 C2048 bf16, K 4,
-// SiLU: forward 30 us (4.5 TB/s), gradient 67 (3 TB/s: its sums of weights and the
+// SiLU: forward 29 us (4.6 TB/s), gradient 59 (3.4 TB/s: its sums of weights and the
 // activation's slope take more issue slots than the loads).
 #pragma once
 #include <type_traits>

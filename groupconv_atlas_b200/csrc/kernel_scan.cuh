@@ -21,8 +21,8 @@
 // the state (what it adds, and the sum of its deltas, whose product with A is its
 // decay's logarithm), from which every block forms the state that it starts with.
 //
-// N4 L2048 C2048 S16 bf16, kernel after kernel: segments' effects 91 us, scan 176;
-// backwards 98 and 372, sums 30.  The exponentials alone would take 58 us in each;
+// N4 L2048 C2048 S16 bf16, kernel after kernel: segments' effects 88 us, scan 173;
+// backwards 102 and 370, sums 22.  The exponentials alone would take 58 us in each;
 // shared memory (every lane reads each product, B and C of its states) is 60 to
 // 70 % busy, the special-function unit 46 %.
 #pragma once

@@ -411,9 +411,7 @@ int gc_b200_layer_norm_backward(const gc_tensor *dy, const gc_tensor *x, const g
             S.type[i] = t != nullptr ? elem_type(t->dtype) : kElemF32;
             S.mul[i++] = 1;
         }
-        void *sum_args[] = {&S};
-        e = launch_pdl(reinterpret_cast<const void *>(&sum_rows_kernel), dim3(static_cast<unsigned>(2 * ceil_div(c, 32))),
-                       dim3(kSumWarps * 32), sum_args, 0, s);
+        e = launch_sum_rows(S, s);
     }
     return launched(e, PlanRecord::kSequence, plan.whole ? "layer_norm_long_backward" : plan.edges ? "layer_norm_edges_backward" : "layer_norm_backward", grid,
                     plan.threads, plan.vec ? 1 : 0, plan.team, plan.nv, 1, sums ? 2 : 1);

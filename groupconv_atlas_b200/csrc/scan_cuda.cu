@@ -430,9 +430,7 @@ int gc_b200_selective_scan_backward(const gc_b200_scan_args *q, const gc_tensor 
             S.type[i] = t != nullptr ? elem_type(t->dtype) : kElemF32;
             S.mul[i++] = 1;
         }
-        void *args[] = {&S};
-        e = launch_pdl(reinterpret_cast<const void *>(&sum_rows_kernel),
-                       dim3(static_cast<unsigned>(S.planes * ceil_div(S.cols, 32))), dim3(kSumWarps * 32), args, 0, s);
+        e = launch_sum_rows(S, s);
         ++launches;
     }
     return launched(e, PlanRecord::kSequence, "selective_scan_backward", plan.blocks, kScanThreads, plan.vec ? 1 : 0,

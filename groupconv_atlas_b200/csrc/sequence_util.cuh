@@ -85,10 +85,13 @@ inline int check_dense(const gc_tensor *t, const char *message) {
 // ---- sums over rows of partial results ------------------------------------------------
 // part holds `rows` rows of `planes` planes of `cols` 32-bit values; plane q's
 // sum over the rows goes to element col * mul[q] + add[q] of out[q] (skipped
-// where that is NULL).  A block takes 32 columns of a plane; its warps take the
-// rows in turn, in runs of 64 values in 32 bits joined in 64, and are joined in
-// a fixed order.
-constexpr int kSumPlanes = 9, kSumWarps = 16, kSumRun = 64;
+// where that is NULL).  A block takes 32 columns of a plane (a line of a row), or,
+// of more than 256 rows, 8 (a sector): how many loads follow one another is then what
+// counts.  With 32 columns 1184 rows of 2 x 1001 take 14 us, with 8 columns 9; 52 rows
+// of 32768 take 7 and 15, 37 rows of 5 x 2048 4 and 6.  Its workers take the rows in
+// turn, eight loads under way, in runs of 64 values in 32 bits joined in 64, and are
+// joined in a fixed order.
+constexpr int kSumPlanes = 9, kSumThreads = 512, kSumRun = 64;
 struct SumParams {
     const float *part;
     long long rows, cols;
@@ -97,6 +100,6 @@ struct SumParams {
     int type[kSumPlanes];
     long long mul[kSumPlanes], add[kSumPlanes];
 };
-__global__ void __launch_bounds__(kSumWarps * 32) sum_rows_kernel(const __grid_constant__ SumParams P);
+cudaError_t launch_sum_rows(SumParams &P, cudaStream_t stream);
 
 }  // namespace gcb
