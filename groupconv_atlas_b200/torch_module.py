@@ -552,7 +552,9 @@ class B200SelectiveBlock(torch.nn.Module):
 
     forward(x) on (N, L, width) serves training; prefill(x, lengths) runs prompts
     and returns (result, states); step(x, states) takes one token (N, width) of
-    every sequence and updates the states in place."""
+    every sequence and updates the states in place.  lengths: what lies behind a
+    sequence's end comes back as it was; in training it has to be finite, since
+    the projections' weight gradients read it."""
 
     def __init__(self, width: int, channels: int | None = None, states: int = 16, taps: int = 4, rank: int | None = None,
                  eps: float = 1e-5, device=None, dtype=None):
