@@ -577,7 +577,8 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_edges_grad_kernel(const _
 }
 
 // Rows too long for a block's registers: read three times (the second and third
-// time from the caches), one row to a block.
+// time from the caches), one row to a block.  Columns in 64 bits: a row may have up
+// to 2^31 - 1, a step beyond which 32 do not hold, nor do they twice as many.
 template <class T>
 __global__ void __launch_bounds__(kRowMost) layer_norm_long_kernel(const __grid_constant__ LayerNormParams P) {
     __shared__ float buf[2 * (kRowMost / 32)];
@@ -589,16 +590,16 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_long_kernel(const __grid_
         const T *src = static_cast<const T *>(P.x) + row * P.x_ld;
         T *dst = static_cast<T *>(P.y) + row * P.y_ld;
         float s[1] = {0.0f}, q[1] = {0.0f};
-        for (int i = threadIdx.x; i < P.c; i += kRowMost) s[0] += to_float(src[i]);
+        for (long long i = threadIdx.x; i < P.c; i += kRowMost) s[0] += to_float(src[i]);
         team_sums<1>(s, kRowMost, buf, turn);
         const float mean = s[0] * inv;
-        for (int i = threadIdx.x; i < P.c; i += kRowMost) {
+        for (long long i = threadIdx.x; i < P.c; i += kRowMost) {
             const float d = to_float(src[i]) - mean;
             q[0] = fmaf(d, d, q[0]);
         }
         team_sums<1>(q, kRowMost, buf, turn);
         const float rstd = 1.0f / sqrtf(fmaf(q[0], inv, P.eps));
-        for (int i = threadIdx.x; i < P.c; i += kRowMost) {
+        for (long long i = threadIdx.x; i < P.c; i += kRowMost) {
             const float gamma = P.gamma != nullptr ? load_param(P.gamma, P.gamma_type, i) : 1.0f;
             const float beta = P.beta != nullptr ? load_param(P.beta, P.beta_type, i) : 0.0f;
             dst[i] = from_float<T>(fmaf((to_float(src[i]) - mean) * rstd, gamma, beta));
@@ -622,7 +623,7 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_long_grad_kernel(const __
         T *dst = static_cast<T *>(P.y) + row * P.y_ld;
         const float2 st = P.stats[row];
         float sums[2] = {0.0f, 0.0f};
-        for (int i = threadIdx.x; i < P.c; i += kRowMost) {
+        for (long long i = threadIdx.x; i < P.c; i += kRowMost) {
             const float gamma = P.gamma != nullptr ? load_param(P.gamma, P.gamma_type, i) : 1.0f;
             const float d = to_float(dy[i]), xhat = (to_float(x[i]) - st.x) * st.y, g = d * gamma;
             sums[0] += g;
@@ -635,7 +636,7 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_long_grad_kernel(const __
         }
         team_sums<2>(sums, kRowMost, buf, turn);
         const float m1 = sums[0] * inv, m2 = sums[1] * inv;
-        for (int i = threadIdx.x; i < P.c; i += kRowMost) {
+        for (long long i = threadIdx.x; i < P.c; i += kRowMost) {
             const float gamma = P.gamma != nullptr ? load_param(P.gamma, P.gamma_type, i) : 1.0f;
             const float xhat = (to_float(x[i]) - st.x) * st.y;
             dst[i] = from_float<T>(st.y * (fmaf(to_float(dy[i]), gamma, -m1) - xhat * m2));
