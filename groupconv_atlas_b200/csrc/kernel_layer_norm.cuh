@@ -579,6 +579,23 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_edges_grad_kernel(const _
 // Rows too long for a block's registers: read three times (the second and third
 // time from the caches), one row to a block.  Columns in 64 bits: a row may have up
 // to 2^31 - 1, a step beyond which 32 do not hold, nor do they twice as many.
+//
+// A thread's share of such a row's sums, which has no bound: runs of 64 values in 32
+// bits joined in 64.  add(column, the run's sums).
+template <int N, class F>
+__device__ __forceinline__ void long_sums(long long c, float (&v)[N], F add) {
+    constexpr long long kRun = 64LL * kRowMost;
+    double all[N] = {};
+    for (long long start = threadIdx.x; start < c; start += kRun) {
+        const long long stop = min(c, start + kRun);
+        float run[N] = {};
+        for (long long i = start; i < stop; i += kRowMost) add(i, run);
+#pragma unroll
+        for (int k = 0; k < N; ++k) all[k] += run[k];
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = static_cast<float>(all[k]);
+}
 template <class T>
 __global__ void __launch_bounds__(kRowMost) layer_norm_long_kernel(const __grid_constant__ LayerNormParams P) {
     __shared__ float buf[2 * (kRowMost / 32)];
@@ -589,14 +606,14 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_long_kernel(const __grid_
     for (long long row = blockIdx.x; row < P.rows; row += gridDim.x) {
         const T *src = static_cast<const T *>(P.x) + row * P.x_ld;
         T *dst = static_cast<T *>(P.y) + row * P.y_ld;
-        float s[1] = {0.0f}, q[1] = {0.0f};
-        for (long long i = threadIdx.x; i < P.c; i += kRowMost) s[0] += to_float(src[i]);
+        float s[1], q[1];
+        long_sums<1>(P.c, s, [&](long long i, float (&run)[1]) { run[0] += to_float(src[i]); });
         team_sums<1>(s, kRowMost, buf, turn);
         const float mean = s[0] * inv;
-        for (long long i = threadIdx.x; i < P.c; i += kRowMost) {
+        long_sums<1>(P.c, q, [&](long long i, float (&run)[1]) {
             const float d = to_float(src[i]) - mean;
-            q[0] = fmaf(d, d, q[0]);
-        }
+            run[0] = fmaf(d, d, run[0]);
+        });
         team_sums<1>(q, kRowMost, buf, turn);
         const float rstd = 1.0f / sqrtf(fmaf(q[0], inv, P.eps));
         for (long long i = threadIdx.x; i < P.c; i += kRowMost) {
@@ -622,18 +639,18 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_long_grad_kernel(const __
         const T *x = static_cast<const T *>(P.x) + row * P.x_ld, *dy = static_cast<const T *>(P.dy) + row * P.dy_ld;
         T *dst = static_cast<T *>(P.y) + row * P.y_ld;
         const float2 st = P.stats[row];
-        float sums[2] = {0.0f, 0.0f};
-        for (long long i = threadIdx.x; i < P.c; i += kRowMost) {
+        float sums[2];
+        long_sums<2>(P.c, sums, [&](long long i, float (&run)[2]) {
             const float gamma = P.gamma != nullptr ? load_param(P.gamma, P.gamma_type, i) : 1.0f;
             const float d = to_float(dy[i]), xhat = (to_float(x[i]) - st.x) * st.y, g = d * gamma;
-            sums[0] += g;
-            sums[1] = fmaf(g, xhat, sums[1]);
+            run[0] += g;
+            run[1] = fmaf(g, xhat, run[1]);
             if (out != nullptr) {
                 const bool fresh = row == blockIdx.x;
                 out[i] = fmaf(d, xhat, fresh ? 0.0f : out[i]);
                 out[P.c + i] = d + (fresh ? 0.0f : out[P.c + i]);
             }
-        }
+        });
         team_sums<2>(sums, kRowMost, buf, turn);
         const float m1 = sums[0] * inv, m2 = sums[1] * inv;
         for (long long i = threadIdx.x; i < P.c; i += kRowMost) {

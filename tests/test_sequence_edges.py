@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from groupconv_atlas_b200 import api, torch_module
+from tests import test_layer_norm
 
 
 # ---- rows past 2^30 elements -------------------------------------------------------------------------
@@ -35,3 +36,15 @@ def test_gradient_of_a_row_past_2_30_elements(native, torch_cuda):
     y = torch_module.layer_norm(x, gamma, beta, 2.0 ** -8)
     dx, dgamma, dbeta = torch.autograd.grad(y, (x, gamma, beta), dy)
     assert torch.equal(dbeta, dy[0]) and not dgamma.any() and torch.equal(dx, 16 * dy)
+
+
+# ---- long sums --------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_rows_of_many_millions(native, torch_cuda):
+    """Values of one size: a thread that adds its share of the squares, or of dy, one
+    after the other in 32 bits is off by thousands of half steps (7700 and 5000 by
+    arithmetic, of 32768 additions)."""
+    v, c = float.fromhex('0x1.702dep0'), (1 << 24) + 3
+    x = torch.full((1, c), v)
+    x[0, ::2] = -v
+    test_layer_norm.check(x, None, None, torch.full((1, c), v))
