@@ -133,6 +133,12 @@ __device__ __forceinline__ float rcp_fast(float v) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
+// The larger, or NaN where one of them is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 __device__ __forceinline__ float sum_of(f2 v) {
     float a, b;
     split(v, a, b);
@@ -145,12 +151,15 @@ constexpr float kLog2E = 1.4426950408889634f;
 // hyperbolic tangent, whose argument is at most 1/3: the first term left out is
 // below 2e-8 of the sum.  Step sizes far below 1 come from small e, where a
 // logarithm of the rounded 1 + e would lose what matters.  Two denominators share
-// a reciprocal; they are between 1 and 3.
+// a reciprocal; they are between 1 and 3 whatever the arguments are, since a NaN, which
+// would reach the other value through it, takes no part: |v| is held below 128, where
+// e is 0 already (the smaller of a NaN and a number is the number), and a NaN comes
+// back with max(v, 0).
 template <bool SLOPE>
 __device__ __forceinline__ void softplus2(f2 v, f2 &value, f2 &slope) {
     float v0, v1, p0, p1;
     split(v, v0, v1);
-    const f2 e = exp2_fast(pair(fabsf(v0), fabsf(v1)) * pair(-kLog2E));
+    const f2 e = exp2_fast(pair(fminf(fabsf(v0), 128.0f), fminf(fabsf(v1), 128.0f)) * pair(-kLog2E));
     split(e + pair(2.0f), p0, p1);
     const f2 u = e * (pair(p1, p0) * pair(rcp_fast(p0 * p1))), w = u * u;
     f2 s = fma2(w, pair(1.0f / 13.0f), pair(1.0f / 11.0f));
@@ -159,7 +168,7 @@ __device__ __forceinline__ void softplus2(f2 v, f2 &value, f2 &slope) {
     s = fma2(w, s, pair(1.0f / 5.0f));
     s = fma2(w, s, pair(1.0f / 3.0f));
     s = fma2(w, s, pair(1.0f));
-    value = fma2(u + u, s, pair(fmaxf(v0, 0.0f), fmaxf(v1, 0.0f)));
+    value = fma2(u + u, s, pair(max_nan(v0, 0.0f), max_nan(v1, 0.0f)));
     if constexpr (SLOPE) {
         float e0, e1;
         split(e, e0, e1);

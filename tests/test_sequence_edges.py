@@ -5,7 +5,10 @@ import pytest
 import torch
 
 from groupconv_atlas_b200 import api, torch_module
-from tests import test_layer_norm
+from tests import test_layer_norm, test_selective_scan
+from tests.norm_helpers import HALF
+from tests.sequence_helpers import ScanReference, assert_close
+from tests.test_selective_scan import NAMES, TYPES, run
 
 
 # ---- rows past 2^30 elements -------------------------------------------------------------------------
@@ -48,3 +51,70 @@ def test_rows_of_many_millions(native, torch_cuda):
     x = torch.full((1, c), v)
     x[0, ::2] = -v
     test_layer_norm.check(x, None, None, torch.full((1, c), v))
+
+
+# ---- step sizes that are no numbers ----------------------------------------------------------------
+def scan_with_gradient(v):
+    leaves = {k: v[k].cuda().requires_grad_() for k in NAMES}
+    y, last = run(v, leaves, True, None, True)
+    grads = torch.autograd.grad([y, last], list(leaves.values()), [v['dy'].cuda(), v['dlast'].cuda()])
+    return {'y': y.detach(), 'last': last.detach(), **{'d' + k: g for k, g in zip(NAMES, grads)}}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('shape', [(2, 100, 36, 16, 1), (2, 40, 33, 7, 3)])
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('place', ['dt', 'dt_bias'])
+@pytest.mark.parametrize('value', [float('nan'), float('inf'), -float('inf')])
+@pytest.mark.parametrize('channel', [4, 5])
+def test_step_sizes_stay_in_their_channel(native, torch_cuda, shape, dtype, place, value, channel):
+    """Every other channel's results and gradients are those without the value (dB and
+    dC are sums over channels).  A step size of 0, from -inf, leaves the state as it is."""
+    v = test_selective_scan.make(*shape, TYPES[dtype], 31)
+    ref = ScanReference(*(v[k] for k in NAMES[:8]), True, v['state']).backward(v['dy'], v['dlast'])
+    clean = scan_with_gradient(v)
+    v[place] = v[place].clone()
+    if place == 'dt':
+        v['dt'][1, 20, channel] = value
+    else:
+        v['dt_bias'][channel] = value
+    got = scan_with_gradient(v)
+    others = torch.arange(shape[2]) != channel
+    for name in ('y', 'dx', 'ddt', 'dz'):
+        assert_close(got[name].cpu()[..., others], getattr(ref, name)[..., others], getattr(ref, 'tol_' + name)[..., others] + 2.0 ** -40, name)
+        if place == 'dt':
+            assert torch.equal(got[name][0], clean[name][0]), name  # the other sequence
+    for name in ('last', 'dstate'):
+        assert_close(got[name].cpu()[:, others], getattr(ref, name)[:, others], getattr(ref, 'tol_' + name)[:, others] + 2.0 ** -40, name)
+    for name in ('da', 'dd', 'ddt_bias'):
+        want = getattr(ref, name)[others]
+        tol = getattr(ref, 'tol_' + name)[others] + HALF[torch.float32] * want.abs() + 2.0 ** -25
+        assert_close(got[name].cpu()[others], want, tol, name)
+    own = got['y'][1, 20:, channel]
+    assert torch.isfinite(own).all() if value == -float('inf') else not torch.isfinite(own).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('shape', [(3, 64, 16, 2), (3, 33, 7, 3)])  # every access whole, or not
+@pytest.mark.parametrize('place', ['dt', 'dt_bias'])
+@pytest.mark.parametrize('value', [float('nan'), float('inf'), -float('inf')])
+@pytest.mark.parametrize('channel', [4, 5])
+def test_step_sizes_of_a_token_stay_in_their_channel(native, torch_cuda, shape, place, value, channel):
+    n, ch, s, groups = shape
+    v = test_selective_scan.make(n, 1, ch, s, groups, torch.float32, 32)
+    ref = ScanReference(*(v[k] for k in NAMES[:8]), True, v['state'])
+    if place == 'dt':
+        v['dt'][1, 0, channel] = value
+    else:
+        v['dt_bias'][channel] = value
+    q = {k: t.cuda() for k, t in v.items()}
+    state = q['state'].clone()
+    y = torch_module.selective_scan_step(q['x'][:, 0], q['dt'][:, 0], q['a'], q['b'][:, 0], q['c'][:, 0], state, q['d'],
+                                         q['z'][:, 0], q['dt_bias'])
+    others = torch.arange(ch) != channel
+    assert_close(y.cpu()[:, others], ref.y[:, 0, others], ref.tol_y[:, 0, others], 'y')
+    assert_close(state.cpu()[:, others], ref.last[:, others], ref.tol_last[:, others], 'state')
+    if value == -float('inf'):
+        assert torch.equal(state[1, channel], q['state'][1, channel]) and torch.isfinite(y).all()
+    else:
+        assert not torch.isfinite(y[1, channel])
