@@ -306,7 +306,14 @@ __device__ __forceinline__ void store_states(float *p, int part, int states, boo
 }
 // A log2(e): the exponentials are powers of 2.  Infinities become the largest
 // numbers, whose exponentials are the same, so that a step size of 0 leaves a
-// state as it is; tiles are filled up with such steps.
+// state as it is; tiles are filled up with such steps.  A NaN stays one.
+__device__ __forceinline__ f2 decay_exponent(f2 v) {
+    float a, b;
+    split(v * pair(kLog2E), a, b);
+    a = a > 3e38f ? 3e38f : a < -3e38f ? -3e38f : a;
+    b = b > 3e38f ? 3e38f : b < -3e38f ? -3e38f : b;
+    return pair(a, b);
+}
 template <class S>
 __device__ __forceinline__ void load_decay(const ScanParams &Q, const ScanPlace<S> &at, int k, int swap, f2 (&v)[S::NP]) {
     if (Q.a_type == kElemF32) {
@@ -328,13 +335,7 @@ __device__ __forceinline__ void load_decay(const ScanParams &Q, const ScanPlace<
         }
     }
 #pragma unroll
-    for (int i = 0; i < S::NP; ++i) {
-        float a, b;
-        split(v[i] * pair(kLog2E), a, b);
-        a = a > 3e38f ? 3e38f : a < -3e38f ? -3e38f : a;
-        b = b > 3e38f ? 3e38f : b < -3e38f ? -3e38f : b;
-        v[i] = pair(a, b);
-    }
+    for (int i = 0; i < S::NP; ++i) v[i] = decay_exponent(v[i]);
 }
 // The states of a thread's own place, in its order.
 template <class S>
@@ -1134,7 +1135,7 @@ __global__ void __launch_bounds__(S::THREADS) scan_step_kernel(const __grid_cons
         for (int k = 0; k < 2; ++k) {
             quad(decay + k * S::SP, a2[k]);
 #pragma unroll
-            for (int i = 0; i < NP; ++i) a2[k][i] = a2[k][i] * pair(kLog2E);
+            for (int i = 0; i < NP; ++i) a2[k][i] = decay_exponent(a2[k][i]);
         }
         floats_of<E>(fb, b);
         floats_of<E>(fc, c);

@@ -118,3 +118,21 @@ def test_step_sizes_of_a_token_stay_in_their_channel(native, torch_cuda, shape, 
         assert torch.equal(state[1, channel], q['state'][1, channel]) and torch.isfinite(y).all()
     else:
         assert not torch.isfinite(y[1, channel])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('shape', [(3, 64, 16, 2), (3, 33, 7, 3)])
+def test_infinite_decays_of_a_token(native, torch_cuda, shape):
+    """A = -inf forgets the state, and with a step size of 0 leaves it as it is, in
+    every kernel alike."""
+    n, ch, s, groups = shape
+    v = {k: t.cuda() for k, t in test_selective_scan.make(n, 1, ch, s, groups, torch.float32, 33).items()}
+    v['a'][3] = -float('inf')
+    v['dt'][0] = -300.0
+    y, last = run(v, v, True, None, True)
+    state = v['state'].clone()
+    one = torch_module.selective_scan_step(v['x'][:, 0], v['dt'][:, 0], v['a'], v['b'][:, 0], v['c'][:, 0], state, v['d'],
+                                           v['z'][:, 0], v['dt_bias'])
+    assert torch.isfinite(one).all() and torch.equal(state[0], v['state'][0]) and torch.equal(last[0], v['state'][0])
+    torch.testing.assert_close(one, y[:, 0], rtol=1e-5, atol=1e-6)
+    torch.testing.assert_close(state, last, rtol=1e-5, atol=1e-6)
