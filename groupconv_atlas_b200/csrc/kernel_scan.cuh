@@ -38,6 +38,9 @@ namespace gcb {
 // of half of the warps: 570 us against 432 at N4 L2048 C2048 bf16, for half of the
 // memory.)
 constexpr int kScanChunk = 8;
+// Tiles of the gradient whose sums for A, D and dt_bias are added up in 32 bits one
+// after the other; such runs are joined by sum_rows_kernel.
+constexpr int kScanRun = 64;
 
 // A tensor of tokens: strides of a sequence, a token and (B, C) a group.
 struct TokenView {
@@ -62,7 +65,8 @@ struct ScanParams {
     float *carry, *sums;               // [n][segs][channels][states], [n][segs][channels]
     float *kept;                       // [n][chunks][channels][states] or NULL
     float *part_bc;                    // gradient: [tile][n][l][groups][2][states]
-    float *part_a, *part_d;            // [n * segs][channels][states], [n * segs][2][channels] (D, dt_bias)
+    float *part_a, *part_d;            // [n * segs * runs][channels][states], [n * segs * runs][2][channels] (D, dt_bias)
+    int runs;                          // of kScanRun tiles, in a segment
 };
 
 // ---- four elements ---------------------------------------------------------------------------
@@ -845,6 +849,31 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
 #pragma unroll
     for (int k = 0; k < 2; ++k) skip[k] = Q.d != nullptr && at.live[k] ? load_param(Q.d, Q.d_type, at.channel + k) : 0.0f;
     const bool writes = at.part < 4, vec = Q.vec;
+    // A run's sums to its row of the partial results, and the next run's from 0.
+    const auto end_run = [&](int run) {
+        const long long row = (at.n * Q.segs + at.seg) * Q.runs + run;
+        const float4 own = sm.sums[threadIdx.x];
+        float dskip[2] = {own.x, own.y}, dbias[2] = {own.z, own.w};
+        sm.sums[threadIdx.x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (Q.part_a != nullptr)
+                store_states<S>(Q.part_a + (row * Q.channels + at.channel + k) * Q.states, at.part, Q.states, at.live[k], swap, da[k]);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) da[k][i] = pair(0.0f);
+            if (Q.part_d == nullptr) continue;
+#pragma unroll
+            for (int o = 1; o < P; o *= 2) {
+                dskip[k] += __shfl_xor_sync(0xffffffffu, dskip[k], o);
+                dbias[k] += __shfl_xor_sync(0xffffffffu, dbias[k], o);
+            }
+            if (at.part == 0 && at.live[k]) {
+                Q.part_d[row * 2 * Q.channels + at.channel + k] = dskip[k];
+                Q.part_d[(row * 2 + 1) * Q.channels + at.channel + k] = dbias[k];
+            }
+        }
+    };
+    for (int run = (tiles + kScanRun - 1) / kScanRun; run < Q.runs; ++run) end_run(run);  // behind the sequence's end
 
     for (int buf = 0; tiles > 0; --tiles, t0 -= T, tokens = T, buf ^= 1) {
         f2 h[T][2][NP];
@@ -1015,6 +1044,7 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
             const float4 v = sm.sums[threadIdx.x];
             sm.sums[threadIdx.x] = make_float4(v.x + dskip1[0], v.y + dskip1[1], v.z + dbias1[0], v.w + dbias1[1]);
         }
+        if ((tiles - 1) % kScanRun == 0) end_run((tiles - 1) / kScanRun);
         __syncthreads();
         float *part = Q.part_bc + (((at.tile * Q.n + at.n) * Q.l + t0) * Q.groups + at.group) * 2 * Q.states;
         const long long next = static_cast<long long>(Q.groups) * 2 * Q.states;  // a token further
@@ -1051,26 +1081,10 @@ __global__ void __launch_bounds__(S::THREADS, 512 / S::THREADS) scan_grad_kernel
     zeros(Q.dx);
     zeros(Q.ddt);
     zeros(Q.dz);
-    const long long row = at.n * Q.segs + at.seg;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < 2; ++k)
         if (Q.state_out != nullptr && at.seg == 0)
             store_states<S>(Q.state_out + at.n * Q.so_ldn + (at.channel + k) * Q.so_ldc, at.part, Q.states, at.live[k], swap, q[k]);
-        if (Q.part_a != nullptr)
-            store_states<S>(Q.part_a + (row * Q.channels + at.channel + k) * Q.states, at.part, Q.states, at.live[k], swap, da[k]);
-        if (Q.part_d == nullptr) continue;
-        const float4 own = sm.sums[threadIdx.x];
-        float dskip[2] = {own.x, own.y}, dbias[2] = {own.z, own.w};
-#pragma unroll
-        for (int o = 1; o < P; o *= 2) {
-            dskip[k] += __shfl_xor_sync(0xffffffffu, dskip[k], o);
-            dbias[k] += __shfl_xor_sync(0xffffffffu, dbias[k], o);
-        }
-        if (at.part == 0 && at.live[k]) {
-            Q.part_d[row * 2 * Q.channels + at.channel + k] = dskip[k];
-            Q.part_d[(row * 2 + 1) * Q.channels + at.channel + k] = dbias[k];
-        }
-    }
 }
 
 // dB and dC: the sums over the blocks that share a group's channels.

@@ -119,6 +119,7 @@ Range lengths_range(const gc_b200_scan_args *q, const ScanCall &c) {
 struct ScanPlan {
     int type = 0, sp = 16, lanes = 4, per_lane = 4;
     int tiles = 1, grad_tiles = 1, segs = 1;  // blocks that share a group's channels
+    int runs = 1;                             // of the gradient's sums, in a segment
     long long seg_len = 0, blocks = 0;
     bool vec = false, bvec = false;
 };
@@ -143,6 +144,7 @@ ScanPlan plan_scan(const ScanCall &c, int sms, bool backward) {
     const long long wanted = std::min(ceil_div((backward ? 24LL : 16LL) * sms, blocks), static_cast<long long>(c.l / 32));
     p.seg_len = std::max(1LL, gcb::round_up(ceil_div(c.l, std::max(1LL, wanted)), 16));
     p.segs = static_cast<int>(std::max(1LL, ceil_div(c.l, p.seg_len)));
+    p.runs = static_cast<int>(ceil_div(p.seg_len, kScanChunk * kScanRun));
     p.blocks = blocks * p.segs;
     return p;
 }
@@ -166,8 +168,8 @@ ScanSpace space_of(const ScanCall &c, const ScanPlan &p, bool backward) {
     }
     if (backward) {
         s.bc = up16(static_cast<uint64_t>(p.grad_tiles) * c.n * c.l * c.groups * 2 * c.states * sizeof(float));
-        s.a = up16(rows * c.c * c.states * sizeof(float));
-        s.d = up16(rows * 2 * c.c * sizeof(float));
+        s.a = up16(rows * p.runs * c.c * c.states * sizeof(float));
+        s.d = up16(rows * p.runs * 2 * c.c * sizeof(float));
     }
     return s;
 }
@@ -210,6 +212,7 @@ void fill(ScanParams &P, const gc_b200_scan_args *q, const ScanCall &c, const Sc
     P.tiles = plan.tiles;
     P.seg_len = plan.seg_len;
     P.segs = plan.segs;
+    P.runs = plan.runs;
 }
 void set_state_out(ScanParams &P, const Strided &v) {
     if (v.data == nullptr || v.empty) return;
@@ -421,7 +424,7 @@ int gc_b200_selective_scan_backward(const gc_b200_scan_args *q, const gc_tensor 
         if (which == 0 ? g->a == nullptr : !sums_d) continue;
         SumParams S{};
         S.part = which == 0 ? P.part_a : P.part_d;
-        S.rows = c.n * plan.segs;
+        S.rows = c.n * plan.segs * plan.runs;
         S.cols = which == 0 ? c.c * c.states : c.c;
         S.planes = which == 0 ? 1 : 2;
         int i = 0;

@@ -6,8 +6,8 @@ import torch
 
 from groupconv_atlas_b200 import api, torch_module
 from tests import test_layer_norm, test_selective_scan
-from tests.norm_helpers import HALF
-from tests.sequence_helpers import ScanReference, assert_close
+from tests.norm_helpers import HALF, U
+from tests.sequence_helpers import LONG, ScanReference, assert_close
 from tests.test_selective_scan import NAMES, TYPES, run
 
 
@@ -51,6 +51,58 @@ def test_rows_of_many_millions(native, torch_cuda):
     x = torch.full((1, c), v)
     x[0, ::2] = -v
     test_layer_norm.check(x, None, None, torch.full((1, c), v))
+
+
+@pytest.mark.gpu
+def test_parameters_of_a_long_scan(native, torch_cuda):
+    """Steady states give dA, dD and ddt_bias sums of one value each, over segments of
+    65536 tokens: added up in 32 bits tile after tile these would be off by more than
+    1100 half steps.  Beside the sums' LONG u: a[t] = exp(-1) is off by 7 u, so the
+    steady h and q = 1 / (1 - a) of what they add by at most (0.37 * 7 + 3) / 0.63 u < 9 u,
+    their product with a and the slope's two terms by 2 * 9 + 7 + 6 < 32 u of terms whose
+    difference is above a quarter of their sum: 128 u."""
+    n, l, value = 3600, 65536, float.fromhex('0x1.d45a1cp0')
+    one = lambda *shape: torch.ones(shape, device='cuda')
+    names = ('x', 'dt', 'a', 'b', 'c', 'd', 'dt_bias')
+    leaves = dict(zip(names, (one(n, l, 1), one(n, l, 1), -one(1, 1), one(n, l, 1, 1), one(n, l, 1, 1), one(1), 0 * one(1))))
+    for t in leaves.values():
+        t.requires_grad_()
+    y = torch_module.selective_scan(*(leaves[k] for k in names[:5]), D=leaves['d'], dt_bias=leaves['dt_bias'], softplus=False)
+    assert 'parts=1 ' in api.Native().last_plan()
+    wanted = [leaves[k] for k in ('a', 'd', 'dt_bias')]
+    da, dd, dbias = torch.autograd.grad(y, wanted, torch.full_like(y, value))
+    a, h, q = torch.exp(torch.tensor(-1.0, dtype=torch.double)).item(), [0.0], [0.0]
+    for _ in range(l):
+        h.append(a * h[-1] + 1.0)
+        q.append(a * q[-1] + value)
+    m = [q[l - t] * a * h[t] for t in range(l)]  # q[t] a h[t - 1]
+    want = {'da': sum(m), 'dd': l * value, 'dbias': sum(q[l - t] - m[t] for t in range(l))}
+    for name, got in (('da', da), ('dd', dd), ('dbias', dbias)):
+        w = n * want[name]
+        assert abs(got.item() - w) <= (LONG + 128) * U * w, (name, got.item() / w - 1)
+
+
+@pytest.mark.gpu
+def test_runs_of_sequences_that_end_early(native, torch_cuda):
+    """One segment of three runs of 512 tokens: sequences that end in each, and at
+    their borders; the runs behind an end count as 0, whatever memory held."""
+    n, l, ends = 4000, 1030, [1030, 1029, 1025, 1024, 1023, 513, 512, 511, 1, 0]
+    v = test_selective_scan.make(len(ends), l, 8, 4, 1, torch.float32, 34)
+    v['lengths'] = torch.tensor(ends, dtype=torch.int32)
+    ref = ScanReference(*(v[k] for k in NAMES[:8]), True, v['state'], v['lengths']).backward(v['dy'], v['dlast'])
+    params = ('a', 'd', 'dt_bias')
+    many = lambda t: torch.cat([t, t.new_zeros((n - len(ends),) + t.shape[1:])]).cuda()
+    q = {k: v[k].cuda() if k in params else many(v[k]) for k in NAMES}
+    for k in params:
+        q[k].requires_grad_()
+    y, last = run(v, q, True, many(v['lengths']), True)
+    assert 'parts=1 ' in api.Native().last_plan()
+    spoiled = torch.full((1 << 28,), float('nan'), device='cuda')
+    del spoiled
+    grads = torch.autograd.grad([y, last], [q[k] for k in params], [many(v['dy']), many(v['dlast'])])
+    for k, g in zip(params, grads):
+        want, tol = getattr(ref, {'a': 'da', 'd': 'dd', 'dt_bias': 'ddt_bias'}[k]), getattr(ref, f'tol_d{k}')
+        assert_close(g, want, tol + HALF[torch.float32] * want.abs() + 2.0 ** -25, k)
 
 
 # ---- step sizes that are no numbers ----------------------------------------------------------------
