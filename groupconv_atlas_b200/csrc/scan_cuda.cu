@@ -23,13 +23,19 @@ __global__ void __launch_bounds__(kJoinThreads) scan_join_kernel(const __grid_co
     const long long group = row % Q.groups, token = row / Q.groups, t = token % Q.l, n = token / Q.l;
     const TokenView &out = which == 0 ? Q.db : Q.dc;
     if (out.p == nullptr) return;
-    float v = 0.0f;
+    double all = 0.0;
     if (Q.lengths == nullptr || t < Q.lengths[n]) {
         const float *src = Q.part + id;
+        const long long step = Q.rows * width;
+        for (int k0 = 0; k0 < Q.tiles; k0 += kSumRun) {  // runs in 32 bits, joined in 64
+            const int stop = min(Q.tiles, k0 + kSumRun);
+            float v = 0.0f;
 #pragma unroll 4
-        for (int k = 0; k < Q.tiles; ++k) v += src[k * Q.rows * width];
+            for (int k = k0; k < stop; ++k) v += src[k * step];
+            all += v;
+        }
     }
-    store_param(const_cast<void *>(out.p), Q.type, n * out.ldn + t * out.ldt + group * out.ldg + s, v);
+    store_param(const_cast<void *>(out.p), Q.type, n * out.ldn + t * out.ldt + group * out.ldg + s, static_cast<float>(all));
 }
 
 }  // namespace gcb

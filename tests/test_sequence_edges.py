@@ -105,6 +105,21 @@ def test_runs_of_sequences_that_end_early(native, torch_cuda):
         assert_close(g, want, tol + HALF[torch.float32] * want.abs() + 2.0 ** -25, k)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('states', [16, 64])
+def test_pairs_of_many_channels(native, torch_cuda, states):
+    """dB and dC are sums over 2^18 channels; of one value each they would be off by
+    hundreds of half steps if blocks were added up one after the other in 32 bits.
+    Each term is a product of few factors: 8 u beside the sums."""
+    ch, value = 1 << 18, float.fromhex('0x1.141894p0')
+    one = lambda *shape: torch.ones(shape, device='cuda')
+    b, c = one(1, 1, 1, states).requires_grad_(), one(1, 1, 1, states).requires_grad_()
+    y = torch_module.selective_scan(one(1, 1, ch), one(1, 1, ch), -one(ch, states), b, c, softplus=False)
+    for g in torch.autograd.grad(y, [b, c], torch.full_like(y, value)):
+        g = g.double().cpu()
+        assert ((g - ch * value).abs() <= (LONG // 2 + 8) * U * ch * value).all(), g.reshape(-1)[0].item() / (ch * value) - 1
+
+
 # ---- step sizes that are no numbers ----------------------------------------------------------------
 def scan_with_gradient(v):
     leaves = {k: v[k].cuda().requires_grad_() for k in NAMES}
