@@ -156,7 +156,8 @@ int stretch_of(const ConvCall &call, int v, int sms, bool backward) {
 }
 
 // The gradient's blocks: tiles of up to 32 vector columns, and for each as many
-// blocks as fill the GPU.
+// blocks as fill the GPU, or as leave each worker 64 stretches, whose sums it adds up
+// one after the other.
 struct GradPlan {
     bool vec = false;
     int cols = 1, workers = 1, stretch = 8;
@@ -171,7 +172,9 @@ GradPlan plan_grad(const ConvCall &call, bool vec, int sms) {
     p.workers = kConvThreads / p.cols;
     p.stretch = stretch_of(call, vec ? 4 : 1, sms, true);
     p.segs = ceil_div(call.l, p.stretch);
-    p.blocks_y = std::max(1LL, std::min(ceil_div(call.n * p.segs, p.workers), ceil_div(4LL * sms, p.tiles)));
+    const long long items = call.n * p.segs;
+    p.blocks_y = std::max({1LL, std::min(ceil_div(items, p.workers), ceil_div(4LL * sms, p.tiles)),
+                           ceil_div(items, static_cast<long long>(kSumRun) * p.workers)});
     return p;
 }
 
@@ -336,6 +339,7 @@ int gc_b200_causal_conv_backward(const gc_tensor *dy, const gc_tensor *x, const 
     P.part = sums ? static_cast<float *>(workspace) : nullptr;
     void *args[] = {&P};
     const long long grid = plan.tiles * plan.blocks_y;
+    if (grid > INT32_MAX) return gc_error(GC_UNSUPPORTED, "more work than a grid has blocks");
     const void *fn = conv_kernel(kBackward, call.x.type, vec, P.taps, activation);
     const size_t smem = ring_bytes(call.x.type, vec ? 4 : 1, P.taps);
     if ((st = opt_in_ring(dev, fn, smem, facts)) != GC_OK) return st;

@@ -318,8 +318,9 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(const __
 // The gradient.  A block takes a tile of `cols` vector columns; its workers take
 // stretches of sequences in turn.  Walking forward, a worker forms g[t] and
 // finishes dx[t - (KT - 1)]; the KT - 1 tokens behind its stretch are formed once
-// more.  dw and dbias add up over a stretch, then over stretches, then over the
-// workers of the block in a fixed order.
+// more.  dw and dbias add up over a stretch (128 tokens at most), then over 64
+// stretches at most (the plan sees to that), then over the workers of the block, in a
+// fixed order.
 template <class T, int V, int KT, bool FULL, int ACT>
 __global__ void __launch_bounds__(kConvThreads, KT <= 4 ? 2 : 1) causal_conv_grad_kernel(const __grid_constant__ ConvSeqParams P) {
     constexpr int NP = Lanes<V>::kPairs, D = kConvRing / 2;  // D: tokens under way, of x and of dy
