@@ -411,15 +411,18 @@ struct ScanFetch {
         return is_b(id) ? static_cast<const T *>(b.p) + at.n * b.ldn + (t0 + t) * b.ldt + at.group * b.ldg + s
                         : static_cast<const T *>(c.p) + at.n * c.ldn + (t0 + t) * c.ldt + at.group * c.ldg + s;
     }
+    // tokens: from t0 on, of which a tile is copied at most
     __device__ __forceinline__ void start(Raw &raw, long long t0, int tokens) const {
         if (vec && valid > 0) {
 #pragma unroll
-            for (int g = 0; g < S::NG; ++g)
-                if (row + g * ROWS < tokens) {
+            for (int g = 0; g < S::NG; ++g) {
+                const int t = row + g * ROWS;
+                if (t < tokens && (S::NG * ROWS <= S::T || t < S::T)) {  // threads may be more than a tile's tokens need
 #pragma unroll
                     for (int k = 0; k < NT; ++k)
                         if (in[k].p != nullptr) copy_four<T>(&raw.four[k][g][threadIdx.x], four_at(k, g, t0));
                 }
+            }
         }
         if (bvec) {
 #pragma unroll
