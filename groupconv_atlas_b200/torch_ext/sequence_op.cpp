@@ -247,6 +247,7 @@ std::pair<at::Tensor, at::Tensor> causal_conv(const at::Tensor &x, const at::Ten
 // Steps write into a tensor of the caller's.
 void prepare_step(std::initializer_list<at::Tensor> inputs, const at::Tensor &out) {
     refuse_forward_mode(inputs);
+    no_forward_mode(out);
     if (any_wants_grad(inputs) || any_wants_grad({out}))
         throw std::runtime_error("a step has no gradient: call it under torch.no_grad()");
 }

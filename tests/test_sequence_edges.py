@@ -1,11 +1,13 @@
 """Layer norm, the causal convolution and the selective scan where calls can go
 wrong: rows past 2^30 elements, long sums, values that are no numbers, what autograd
 does around a call, first calls, calls of two threads."""
+import contextlib
+
 import pytest
 import torch
 
 from groupconv_atlas_b200 import api, torch_module
-from tests import test_layer_norm, test_selective_scan
+from tests import test_causal_conv, test_layer_norm, test_selective_scan
 from tests.norm_helpers import HALF, U
 from tests.sequence_helpers import LONG, ScanReference, assert_close
 from tests.test_selective_scan import NAMES, TYPES, run
@@ -203,3 +205,129 @@ def test_infinite_decays_of_a_token(native, torch_cuda, shape):
     assert torch.isfinite(one).all() and torch.equal(state[0], v['state'][0]) and torch.equal(last[0], v['state'][0])
     torch.testing.assert_close(one, y[:, 0], rtol=1e-5, atol=1e-6)
     torch.testing.assert_close(state, last, rtol=1e-5, atol=1e-6)
+
+
+# ---- what autograd does around a call --------------------------------------------------------------
+def norm_call(t):
+    return torch_module.layer_norm(t['x'], t['w'], t['b'])
+
+
+def conv_call(t):
+    return torch_module.causal_conv(t['x'], t['w'], t['b'], 'silu', t['state'], t['lengths'], True)
+
+
+def scan_call(t):
+    return run(t, {k: t[k] for k in NAMES}, True, t['lengths'], True)
+
+
+def operands(op):
+    """Tensors of a call on the host, all that it takes."""
+    if op == 'norm':
+        x, w, b, _ = test_layer_norm.make((3, 5, 24), torch.float32, 41)
+        return {'x': x, 'w': w, 'b': b}
+    v = test_causal_conv.make(2, 21, 12, 4, torch.float32, 42) if op == 'conv' else test_selective_scan.make(
+        2, 70, 12, 8, 2, torch.float32, 43)
+    return {k: t for k, t in v.items() if k not in ('dy', 'dlast')}
+
+
+CALLS = {'norm': norm_call, 'conv': conv_call, 'scan': scan_call}
+FLOATS = [(op, name) for op in CALLS for name, t in operands(op).items() if t.is_floating_point()]
+HOOKS = {'host': lambda: torch.autograd.graph.save_on_cpu(),
+         'pinned': lambda: torch.autograd.graph.save_on_cpu(pin_memory=True),
+         'strided': lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: torch.stack([t, t], -1)[..., 0])}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('op', CALLS)
+@pytest.mark.parametrize('hooks', HOOKS)
+def test_hooks_on_saved_tensors(native, torch_cuda, op, hooks):
+    t = {k: v.cuda() for k, v in operands(op).items()}
+    grads = []
+    for context in (contextlib.nullcontext, HOOKS[hooks]):
+        leaves = {k: v.clone().requires_grad_(v.is_floating_point()) for k, v in t.items()}
+        with context():
+            out = CALLS[op]({k: v * 1 for k, v in leaves.items()})
+        out = out if isinstance(out, tuple) else (out,)
+        seeds = [torch.cos(torch.arange(o.numel(), device='cuda').reshape(o.shape)).to(o.dtype) for o in out]
+        grads.append(torch.autograd.grad(out, [v for v in leaves.values() if v.requires_grad], seeds))
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('grad', [True, False])
+@pytest.mark.parametrize('op,name', FLOATS)
+def test_forward_mode_of_any_operand_is_refused(native, op, name, grad):
+    """Duals whose primal requires no gradient too: their tangent would be lost."""
+    import torch.autograd.forward_ad as fwd
+    t = operands(op)
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        t[name] = fwd.make_dual(t[name], torch.ones_like(t[name]))
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            CALLS[op](t)
+
+
+def token_calls(t, u, out=None):
+    """The steps on the first token of operands('conv') and operands('scan')."""
+    at = lambda v: v[:, 0]
+    return {'conv': lambda: torch_module.causal_conv_step(at(t['x']), t['w'], t['state'], t['b'], 'silu', state_out=out),
+            'scan': lambda: torch_module.selective_scan_step(at(u['x']), at(u['dt']), u['a'], at(u['b']), at(u['c']), u['state'],
+                                                             u['d'], at(u['z']), u['dt_bias'], state_out=out)}
+
+
+@pytest.mark.parametrize('op,name', [(op, n) for op, n in FLOATS if op != 'norm'] + [('conv', 'out'), ('scan', 'out')])
+def test_forward_mode_of_steps_is_refused(native, op, name):
+    """The tensor that a step writes its state to as well."""
+    import torch.autograd.forward_ad as fwd
+    t = {'conv': operands('conv'), 'scan': operands('scan')}
+    out = torch.zeros_like(t[op]['state'])
+    with fwd.dual_level(), torch.no_grad():
+        if name == 'out':
+            out = fwd.make_dual(out, torch.ones_like(out))
+        else:
+            t[op][name] = fwd.make_dual(t[op][name], torch.ones_like(t[op][name]))
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            token_calls(t['conv'], t['scan'], out)[op]()
+
+
+@pytest.mark.parametrize('op', CALLS)
+def test_tracing_is_refused(native, op):
+    """A traced graph would hold the outputs' allocations alone."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    t = operands(op)
+    call = lambda x: CALLS[op]({**t, 'x': x})
+    with pytest.raises(RuntimeError, match='cannot be traced'):
+        torch.jit.trace(call, (t['x'],))
+    with pytest.raises(RuntimeError, match='cannot be traced'):
+        make_fx(call)(t['x'])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('op,name', FLOATS)
+def test_function_transforms_are_refused(native, torch_cuda, op, name):
+    """vmap and torch.func.grad hand in tensors without memory of their own."""
+    t = {k: v.cuda() for k, v in operands(op).items()}
+
+    def call(v):
+        out = CALLS[op]({**t, name: v})
+        return (out[0] if isinstance(out, tuple) else out).sum()
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(call)(torch.stack([t[name]] * 2))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(call)(t[name])
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('op', ['conv', 'scan'])
+def test_steps_under_vmap_are_refused(native, torch_cuda, op):
+    """And leave the state as it was."""
+    t, u = ({k: v.cuda() for k, v in operands(o).items()} for o in ('conv', 'scan'))
+    q = t if op == 'conv' else u
+    before = q['state'].clone()
+    for name in [n for o, n in FLOATS if o == op and n != 'state']:
+        def call(v):
+            mine = {**q, name: v}
+            return token_calls(mine if op == 'conv' else t, mine if op == 'scan' else u)[op]()
+        with torch.no_grad(), pytest.raises(RuntimeError):
+            torch.func.vmap(call)(torch.stack([q[name]] * 2))
+        assert torch.equal(q['state'], before), name
