@@ -2,6 +2,9 @@
 wrong: rows past 2^30 elements, long sums, values that are no numbers, what autograd
 does around a call, first calls, calls of two threads."""
 import contextlib
+import subprocess
+import sys
+import threading
 
 import pytest
 import torch
@@ -331,3 +334,63 @@ def test_steps_under_vmap_are_refused(native, torch_cuda, op):
         with torch.no_grad(), pytest.raises(RuntimeError):
             torch.func.vmap(call)(torch.stack([q[name]] * 2))
         assert torch.equal(q['state'], before), name
+
+
+# ---- first calls, calls of two threads --------------------------------------------------------------
+FIRST_USE = """
+import torch
+from groupconv_atlas_b200 import torch_module as tm
+r = lambda *s: torch.randn(s, device='cuda')
+x, odd, w = r(64, 512), r(64, 501), r(16, 4)
+u, dt, A, B, C = r(2, 200, 16), r(2, 200, 16), -r(16, 16).exp(), r(2, 200, 16), r(2, 200, 16)
+long, half, cache, h = r(2, 9000), r(2, 64, 64).bfloat16(), r(2, 3, 16), r(2, 16, 16)
+small = r(64, 16).bfloat16()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    a = [t.requires_grad_() for t in (x, odd, long, u, half, small)]
+    y = [tm.layer_norm(x), tm.layer_norm(odd), tm.layer_norm(long), tm.causal_conv(u, w), tm.causal_conv(half, r(64, 4).bfloat16()),
+         tm.selective_scan(u, dt, A, B, C), tm.layer_norm(small)]
+    g = torch.autograd.grad(y, a, [torch.ones_like(t) for t in y])
+    with torch.no_grad():
+        y += [tm.causal_conv_step(u[:, 0], w, cache), tm.selective_scan_step(u[:, 0], dt[:, 0], A, B[:, 0], C[:, 0], h)]
+graph.replay()
+torch.cuda.synchronize()
+assert all(bool(torch.isfinite(t).all()) for t in (*y, *g)) and all(bool(t.any()) for t in y)
+"""
+
+
+@pytest.mark.gpu
+def test_first_use_inside_a_capture(native, torch_cuda):
+    """Nothing that a first call sets up disturbs a capture."""
+    done = subprocess.run([sys.executable, '-c', FIRST_USE], cwd=api.ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_two_threads_and_streams(native, torch_cuda):
+    """Training steps of two host threads on streams of their own do not meet."""
+    sets = [{k: t.cuda() for k, t in test_selective_scan.make(2, 130, 24, 16, 1, torch.bfloat16, s).items()} for s in (44, 45)]
+    weight = torch.randn(24, 4, device='cuda')
+
+    def step(v):
+        leaves = {k: v[k].detach().requires_grad_() for k in NAMES}
+        u = torch_module.causal_conv(torch_module.layer_norm(leaves['x']), weight, activation='silu')
+        y = run(v, {**leaves, 'x': u}, True, v['lengths'], False)
+        return [y.detach(), *torch.autograd.grad(y, list(leaves.values()), v['dy'])]
+    want = [step(v) for v in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                got = step(sets[i])
+                stream.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
