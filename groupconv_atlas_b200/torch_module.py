@@ -537,8 +537,10 @@ class B200CausalConv1d(torch.nn.Module):
     def step(self, x: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
         return causal_conv_step(x, self.weight, state, self.bias, self.activation)
 
-    def new_state(self, n: int) -> torch.Tensor:
-        return self.weight.new_zeros((n, self.weight.shape[-1] - 1, self.weight.shape[0]))
+    def new_state(self, n: int, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """A state of zeros of the type that the inputs will have, the weight's unless
+        given."""
+        return self.weight.new_zeros((n, self.weight.shape[-1] - 1, self.weight.shape[0]), dtype=dtype)
 
     def extra_repr(self) -> str:
         return f'{self.weight.shape[0]}, taps={self.weight.shape[-1]}, activation={self.activation}'
@@ -606,8 +608,11 @@ class B200SelectiveBlock(torch.nn.Module):
         return x + self.output(y)
 
     def new_states(self, n: int):
-        """States of n sequences that have not begun."""
-        return self.conv.new_state(n), self.D.new_zeros((n, self.D.shape[0], self.states), dtype=torch.float32)
+        """States of n sequences that have not begun, for steps under the autocast in
+        effect: the convolution's is of the type that the projections give."""
+        device = self.input.weight.device.type
+        dtype = torch.get_autocast_dtype(device) if torch.is_autocast_enabled(device) else self.input.weight.dtype
+        return self.conv.new_state(n, dtype), self.D.new_zeros((n, self.D.shape[0], self.states), dtype=torch.float32)
 
 
 def substitute(module: torch.nn.Module, predicate, native: api.Native | None = None) -> list[str]:

@@ -394,3 +394,40 @@ def test_two_threads_and_streams(native, torch_cuda):
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not bad
+
+
+# ---- the block -------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize('half', [torch.bfloat16, torch.float16])
+def test_block_under_autocast(native, torch_cuda, half):
+    """Parameters in 32 bits, branches in 16: new states fit the steps; prompts and
+    tokens agree with the whole sequence.  Each of the few products of 16-bit values
+    on the way is off by half a step of its factors: 2^-5 covers them at width 32."""
+    torch.manual_seed(2)
+    block = torch_module.B200SelectiveBlock(32, states=8, device='cuda')
+    x = torch.randn(3, 20, 32, device='cuda')
+    with torch.no_grad(), torch.autocast('cuda', half):
+        want = block(x)
+        states = block.new_states(3)
+        for t in range(4):
+            torch.testing.assert_close(block.step(x[:, t], states), want[:, t], rtol=2 ** -5, atol=2 ** -5)
+        y, states = block.prefill(x[:, 4:10], None, states)
+        torch.testing.assert_close(y, want[:, 4:10], rtol=2 ** -5, atol=2 ** -5)
+        torch.testing.assert_close(block.step(x[:, 10], states), want[:, 10], rtol=2 ** -5, atol=2 ** -5)
+    with torch.autocast('cuda', half):
+        loss = block(x).square().mean()
+    loss.backward()
+    assert all(p.grad.dtype == torch.float32 and torch.isfinite(p.grad).all() and p.grad.any() for p in block.parameters())
+
+
+@pytest.mark.gpu
+def test_new_states_are_of_the_branch_s_type(native, torch_cuda):
+    """The convolution's parameters may stay in 32 bits beside 16-bit projections."""
+    block = torch_module.B200SelectiveBlock(16, states=4, device='cuda')
+    for m in (block.norm, block.input, block.select, block.dt, block.output):
+        m.to(torch.bfloat16)
+    with torch.no_grad():
+        x = torch.randn(2, 5, 16, device='cuda', dtype=torch.bfloat16)
+        states = block.new_states(2)
+        first = block.step(x[:, 0], states)
+        torch.testing.assert_close(first, block(x)[:, 0], rtol=2 ** -5, atol=2 ** -5)
