@@ -572,10 +572,11 @@ class B200SelectiveBlock(torch.nn.Module):
         self.dt = nn.Linear(rank, channels, bias=False, **kw)
         self.output = nn.Linear(channels, width, bias=False, **kw)
         # the scan's own parameters stay in 32 bits: decays close to 1 do not survive 8 bits of mantissa
-        first = torch.exp(torch.rand(channels, device=device) * 4.6051702 - 6.9077553)  # step sizes of 1e-3 to 1e-1
+        kw = {'device': device, 'dtype': torch.float32}
+        first = torch.exp(torch.rand(channels, **kw) * 4.6051702 - 6.9077553)  # step sizes of 1e-3 to 1e-1
         self.dt_bias = nn.Parameter(first + torch.log(-torch.expm1(-first)))
-        self.A_log = nn.Parameter(torch.log(torch.arange(1, states + 1, device=device).float()).repeat(channels, 1))
-        self.D = nn.Parameter(torch.ones(channels, device=device))
+        self.A_log = nn.Parameter(torch.log(torch.arange(1, states + 1, **kw)).repeat(channels, 1))
+        self.D = nn.Parameter(torch.ones(channels, **kw))
 
     def _scan_inputs(self, u: torch.Tensor):
         dt, B, C = self.select(u).split((self.rank, self.states, self.states), -1)

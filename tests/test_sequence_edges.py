@@ -431,3 +431,15 @@ def test_new_states_are_of_the_branch_s_type(native, torch_cuda):
         states = block.new_states(2)
         first = block.step(x[:, 0], states)
         torch.testing.assert_close(first, block(x)[:, 0], rtol=2 ** -5, atol=2 ** -5)
+
+
+@pytest.mark.parametrize('default', [torch.float64, torch.bfloat16])
+def test_scan_parameters_are_in_32_bits_whatever_the_default(default):
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        block = torch_module.B200SelectiveBlock(16, states=4, dtype=torch.float32)
+        states = block.new_states(2)
+    finally:
+        torch.set_default_dtype(before)
+    assert {p.dtype for p in block.parameters()} == {torch.float32} and {s.dtype for s in states} == {torch.float32}
