@@ -199,10 +199,20 @@ def _pointers(struct, arrays):
     return struct
 
 
+def length_words(lengths, n):
+    """Address of the lengths of n sequences, or None.  The library takes an address
+    alone, so the tensor is looked at here."""
+    if lengths is None:
+        return None
+    if str(lengths.dtype) != 'torch.int32' or tuple(lengths.shape) != (n,) or not lengths.is_contiguous():
+        raise ValueError(f'lengths must be {n} dense int32 words')
+    return lengths.data_ptr()
+
+
 def scan_args(x, dt, a, b, c, d=None, z=None, dt_bias=None, state=None, lengths=None, softplus=True):
     """Arguments of the selective scan's calls, from borrowed device tensors."""
     args = _pointers(ScanArgs(), dict(x=x, dt=dt, a=a, b=b, c=c, d=d, z=z, dt_bias=dt_bias, state=state))
-    args.lengths = lengths.data_ptr() if lengths is not None else None
+    args.lengths = length_words(lengths, x.shape[0])
     args.softplus = 1 if softplus else 0
     return args
 
@@ -414,16 +424,12 @@ class Native:
         self.check(self.lib.gc_b200_layer_norm_backward(*ptrs, *self._space(workspace), self._stream(stream)))
         return dx
 
-    @staticmethod
-    def _words(lengths):
-        return None if lengths is None else lengths.data_ptr()
-
     def causal_conv(self, x, weight, y, bias=None, state=None, lengths=None, state_out=None, activation='none', stream=0):
         """gc_b200_causal_conv on borrowed device tensors: x, y (N, L, C), weight
         (C, K), states (N, K - 1, C), lengths N int32 words."""
         act = NORM_ACTIVATIONS.get(activation, activation) if isinstance(activation, str) else activation
         _, (xp, wp, bp, sp, yp, op) = self._views(x, weight, bias, state, y, state_out)
-        self.check(self.lib.gc_b200_causal_conv(xp, wp, bp, sp, self._words(lengths), yp, op, native_int(act),
+        self.check(self.lib.gc_b200_causal_conv(xp, wp, bp, sp, length_words(lengths, x.shape[0]), yp, op, native_int(act),
                                                 self._stream(stream)))
         return y
 
@@ -439,7 +445,7 @@ class Native:
         """gc_b200_causal_conv_backward: gradients from causal_conv's arguments."""
         act = NORM_ACTIVATIONS.get(activation, activation) if isinstance(activation, str) else activation
         _, p = self._views(dy, x, weight, bias, state, dstate_out, dx, dweight, dbias, dstate)
-        self.check(self.lib.gc_b200_causal_conv_backward(*p[:6], self._words(lengths), *p[6:], native_int(act),
+        self.check(self.lib.gc_b200_causal_conv_backward(*p[:6], length_words(lengths, x.shape[0]), *p[6:], native_int(act),
                                                          *self._space(workspace), self._stream(stream)))
         return dx
 

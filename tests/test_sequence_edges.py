@@ -443,3 +443,17 @@ def test_scan_parameters_are_in_32_bits_whatever_the_default(default):
     finally:
         torch.set_default_dtype(before)
     assert {p.dtype for p in block.parameters()} == {torch.float32} and {s.dtype for s in states} == {torch.float32}
+
+
+@pytest.mark.parametrize('bad', [torch.zeros(2, dtype=torch.int64), torch.zeros(3, dtype=torch.int32),
+                                 torch.zeros(4, dtype=torch.int32)[::2], torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2)])
+def test_lengths_of_the_ctypes_calls(native, bad):
+    """N dense words of 32 bits: the library cannot see what they are."""
+    v = test_causal_conv.make(2, 9, 8, 4, torch.float32)
+    u = test_selective_scan.make(2, 9, 8, 4, 2, torch.float32)
+    with pytest.raises(ValueError):
+        native.causal_conv(v['x'], v['w'], torch.empty_like(v['x']), lengths=bad)
+    with pytest.raises(ValueError):
+        native.causal_conv_backward(v['dy'], v['x'], v['w'], torch.empty_like(v['x']), lengths=bad)
+    with pytest.raises(ValueError):
+        api.scan_args(u['x'], u['dt'], u['a'], u['b'], u['c'], lengths=bad)
