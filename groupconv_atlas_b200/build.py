@@ -127,7 +127,8 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
     """Compile the PyTorch front end (torch_ext/*.cpp, thin C++ callers of the
     C ABI that allocate outputs with PyTorch) against the in-tree library, when
     it is older than its sources; each source to an object of its own, in
-    parallel."""
+    parallel.  Objects lie apart by interpreter, PyTorch and C++ ABI, whose
+    headers they hold."""
     import sysconfig
     import torch
     from torch.utils import cpp_extension
@@ -143,10 +144,11 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
              '-DTORCH_EXTENSION_NAME=_gcb_torch', '-DTORCH_API_INCLUDE_EXTENSION_H',
              *[f'-I{d}' for d in cpp_extension.include_paths()], f'-I{sysconfig.get_paths()["include"]}',
              f'-I{cuda_include}', f'-I{INCLUDE}']
-    OBJECTS.mkdir(exist_ok=True)
+    objects_dir = OBJECTS / f'front{sysconfig.get_config_var("EXT_SUFFIX")}-torch-{torch.__version__}-abi{abi}'
+    objects_dir.mkdir(parents=True, exist_ok=True)
 
     def compile_one(source):
-        out = OBJECTS / (source.name + '.o')
+        out = objects_dir / (source.name + '.o')
         if force or not out.exists() or any(d.stat().st_mtime > out.stat().st_mtime for d in [source, *shared]):
             part = out.with_suffix('.part')
             run_tool(['g++', *flags, '-c', str(source), '-o', str(part)], verbose)
