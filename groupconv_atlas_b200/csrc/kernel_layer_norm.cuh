@@ -354,6 +354,9 @@ struct EdgeVector {
     __device__ __forceinline__ bool any() const { return low < c; }
     __device__ __forceinline__ bool full() const { return low >= 0 && low + V <= c; }
     __device__ __forceinline__ bool has(int k) const { return low + k >= 0 && low + k < c; }
+    // NEAREST: where a place is no column of the row, the value of the nearest that is;
+    // else 0 there.
+    template <bool NEAREST = false>
     __device__ __forceinline__ Raw<T, V> load(const T *row) const {
         Raw<T, V> r;
         if (full()) {
@@ -361,7 +364,10 @@ struct EdgeVector {
         } else {
             T e[V];
 #pragma unroll
-            for (int k = 0; k < V; ++k) e[k] = has(k) ? row[low + k] : from_float<T>(0.0f);
+            for (int k = 0; k < V; ++k) {
+                if constexpr (NEAREST) e[k] = row[max(0, min(low + k, c - 1))];
+                else e[k] = has(k) ? row[low + k] : from_float<T>(0.0f);
+            }
             memcpy(&r.u, e, sizeof(r.u));
         }
         return r;
@@ -508,7 +514,7 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_edges_grad_kernel(const _
         for (int j = 0; j < NV; ++j) {
             const EdgeVector<T> at{(lane + j * P.team) * V - phase, count};
             if (at.any()) {
-                rx[j] = at.load(x);
+                rx[j] = at.template load<true>(x);
                 rg[j] = at.load(dy);
             }
         }
@@ -518,7 +524,8 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_edges_grad_kernel(const _
         for (int j = 0; j < NV; ++j) {
             const EdgeVector<T> at{(lane + j * P.team) * V - phase, count};
             if (!at.any()) continue;
-            // where a place is no column of the row dy and gamma are 0
+            // where a place is no column of the row dy and gamma are 0, and xhat is a
+            // column's (with x = 0 there, (0 - mean) rstd could be infinite)
             const Lanes<V> e = lanes_of_raw<T, V>(rx[j]), d = lanes_of_raw<T, V>(rg[j]);
             f2 s1 = pair(0.0f), s2 = pair(0.0f);
 #pragma unroll

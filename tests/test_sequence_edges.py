@@ -59,6 +59,24 @@ def test_rows_of_many_millions(native, torch_cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('c', [255, 257, 1001, 2047])
+def test_constant_rows_of_large_values(native, torch_cuda, c):
+    """Rows of one value, 2^100, and rstd = 2^30: the places of a row's first and last
+    vector that are none of its columns count for nothing, though (0 - mean) rstd is
+    infinite.  mean is exact, so xhat is 0: dx = rstd (dy - mean(dy)), its sum within
+    2 c u of c for dy of -1 and 1 in turn and one 0."""
+    x = torch.full((5, c), 2.0 ** 100, device='cuda').requires_grad_()
+    gamma = torch.ones(c, device='cuda', requires_grad=True)
+    dy = torch.ones(5, c, device='cuda')
+    dy[:, ::2] = -1
+    dy[:, 0] = 0
+    y = torch_module.layer_norm(x, gamma, None, 2.0 ** -60)
+    dx, dgamma = torch.autograd.grad(y, (x, gamma), dy)
+    assert not y.any() and not dgamma.any()
+    assert torch.equal(dx, 2.0 ** 30 * dy)
+
+
+@pytest.mark.gpu
 def test_parameters_of_a_long_scan(native, torch_cuda):
     """Steady states give dA, dD and ddt_bias sums of one value each, over segments of
     65536 tokens: added up in 32 bits tile after tile these would be off by more than
