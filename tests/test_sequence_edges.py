@@ -12,7 +12,7 @@ import torch
 from groupconv_atlas_b200 import api, torch_module
 from tests import test_causal_conv, test_layer_norm, test_selective_scan
 from tests.norm_helpers import HALF, U
-from tests.sequence_helpers import LONG, ScanReference, assert_close
+from tests.sequence_helpers import LONG, ConvReference, ScanReference, assert_close
 from tests.test_selective_scan import NAMES, TYPES, run
 
 
@@ -44,6 +44,32 @@ def test_gradient_of_a_row_past_2_30_elements(native, torch_cuda):
     y = torch_module.layer_norm(x, gamma, beta, 2.0 ** -8)
     dx, dgamma, dbeta = torch.autograd.grad(y, (x, gamma, beta), dy)
     assert torch.equal(dbeta, dy[0]) and not dgamma.any() and torch.equal(dx, 16 * dy)
+
+
+@pytest.mark.gpu
+def test_gradient_of_a_scan_of_more_than_2_32_elements(native, torch_cuda):
+    """Only the last 40 tokens of the last sequence are not zeros; in front of them x
+    and dy are, so that the state and every gradient are."""
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip('needs 100 GB of device memory')
+    n, l, ch = 2, 33000, 65540
+    v = test_selective_scan.make(1, 40, ch, 1, 1, torch.bfloat16, 37)
+    big = lambda t, fill: torch.full((n, l) + t.shape[2:], fill, dtype=t.dtype, device='cuda')
+    q = {'x': big(v['x'], 0.0), 'dt': big(v['dt'], -1.0), 'b': big(v['b'], 1.0), 'c': big(v['c'], 1.0), 'a': v['a'].cuda()}
+    for k in ('x', 'dt', 'b', 'c'):
+        q[k][-1, -40:] = v[k][0].cuda()
+    dy = big(v['dy'], 0.0)
+    dy[-1, -40:] = v['dy'][0].cuda()
+    leaves = {k: t.requires_grad_() for k, t in q.items()}
+    y = run(v, leaves, True, None, False)
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))
+    ref = ScanReference(*(v[k] for k in NAMES[:5])).backward(v['dy'])
+    for k in ('dt', 'c'):  # x and b in front receive what the tokens behind them pass back
+        assert not grads[k][0].any() and not grads[k][1, :-40].any(), k
+    assert not grads['x'][0].any() and not grads['b'][0].any()
+    for k in ('x', 'dt', 'b', 'c'):
+        assert_close(grads[k][-1:, -40:], getattr(ref, 'd' + k), getattr(ref, 'tol_d' + k) + 2.0 ** -40, k)
+    assert_close(grads['a'], ref.da, ref.tol_da + HALF[torch.float32] * ref.da.abs() + 2.0 ** -25, 'a')
 
 
 # ---- long sums --------------------------------------------------------------------------------------
@@ -208,6 +234,32 @@ def test_step_sizes_of_a_token_stay_in_their_channel(native, torch_cuda, shape, 
         assert torch.equal(state[1, channel], q['state'][1, channel]) and torch.isfinite(y).all()
     else:
         assert not torch.isfinite(y[1, channel])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('value', [float('nan'), float('inf'), -float('inf')])
+@pytest.mark.parametrize('channel', [4, 5])
+@pytest.mark.parametrize('op', ['gate', 'convolution'])
+def test_arguments_of_silu_stay_in_their_channel(native, torch_cuda, op, value, channel):
+    """silu's pairs share a reciprocal as well: the neighbour's values and gradients."""
+    if op == 'gate':
+        v = test_selective_scan.make(2, 40, 36, 16, 1, torch.float32, 35)
+        ref = ScanReference(*(v[k] for k in NAMES[:8]), True, v['state']).backward(v['dy'], v['dlast'])
+        v['z'][1, 20, channel] = value
+        got = scan_with_gradient(v)
+        names = ('y', 'dx', 'ddt', 'dz')
+    else:
+        v = test_causal_conv.make(2, 40, 36, 4, torch.float32, 36)
+        ref = ConvReference(v['x'], v['w'], v['b'], 'silu').backward(v['dy'])
+        v['x'][1, 20, channel] = value
+        leaves = [v[k].cuda().requires_grad_() for k in ('x', 'w', 'b')]
+        y = torch_module.causal_conv(*leaves, 'silu')
+        got = {'y': y.detach(), 'dx': torch.autograd.grad(y, leaves, v['dy'].cuda())[0]}
+        names = ('y', 'dx')
+    others = torch.arange(36) != channel
+    for name in names:
+        assert_close(got[name].cpu()[..., others], getattr(ref, name)[..., others], getattr(ref, 'tol_' + name)[..., others] + 2.0 ** -40, name)
+        assert_close(got[name][0], getattr(ref, name)[0], getattr(ref, 'tol_' + name)[0] + 2.0 ** -40, name)
 
 
 @pytest.mark.gpu
