@@ -145,9 +145,11 @@ int opt_in_ring(int dev, const void *fn, size_t bytes, const DeviceFacts &facts)
     return bytes > 40 * 1024 ? opt_in_smem(dev, fn, facts.smem_optin - 8192) : GC_OK;
 }
 
-// Tokens of a thread: 16 to 64, as many as leave a wave of threads.  Each thread
-// loads its weights and the window in front of its stretch: shorter stretches were
-// no faster (N8 L2048 C2048 bf16: forward the same at 32 and at 64, gradient 5 % more at 32).
+// Tokens of a thread: 16 to 64, backwards 128, as many as leave so many threads; v:
+// channels of a thread, four also where the forward kernel takes eight, which then has half
+// of the threads.  Each thread loads its weights and the window in front of its stretch:
+// shorter stretches were no faster (N8 L2048 C2048 bf16: forward the same at 32 and at 64,
+// gradient 5 % more at 32).
 int stretch_of(const ConvCall &call, int v, int sms, bool backward) {
     const long long threads = call.n * ceil_div(call.c, v), wanted = (backward ? 384LL : 768LL) * sms;
     long long stretch = backward ? 128 : 64;

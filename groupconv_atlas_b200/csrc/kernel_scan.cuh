@@ -22,9 +22,10 @@
 // decay's logarithm), from which every block forms the state that it starts with.
 //
 // N4 L2048 C2048 S16 bf16, kernel after kernel: segments' effects 88 us, scan 173;
-// backwards 102 and 370, sums 22.  The exponentials alone would take 58 us in each;
-// shared memory (every lane reads each product, B and C of its states) is 60 to
-// 70 % busy, the special-function unit 46 %.
+// backwards 102 and 370, sums 22.  The exponentials alone would take 58 us in each.
+// There are 10 to 15 warps a multiprocessor at a time, which keep the shared memory's
+// pipe (every lane reads each product, B and C of its states) 44 to 57 % busy and issue in
+// 48 to 62 % of the slots: dependent instructions wait for one another.
 #pragma once
 #include <cstring>
 #include <type_traits>
@@ -537,11 +538,12 @@ struct ScanTile {
 // Two buffers and one barrier a tile: a tile's values are formed after the one
 // before has been worked on, from copies that were under way meanwhile.  Tiles are
 // filled up with steps of size 0.
-// Blocks a multiprocessor, by what registers they leave: with 96 the main kernel is a
-// quarter faster than with the 110 that it would take, and no slower than with 80.  The
-// other modes would take 240 and get 160, with blocks of more than one at a time left on a
-// multiprocessor (N1 L8192 C2048 S16 bf16, whole call: 257 us left to itself, 245 with 160,
-// 261 with 128, 272 with 72; the training step of N4 L2048 C2048 771, 738, 745, 737).
+// The bounds hold registers down; what fits a multiprocessor is up to shared memory as
+// well.  At 16 states in 16 bits that is eight blocks of the main kernel, whose bound is
+// ten: N4 L2048 C2048 bf16, whole call, 244 us with 96 registers, 252 with 80 (twelve), 250
+// with 96 otherwise arranged (nine), 231 with 128 (eight).  The other modes would take 240
+// and get 168, six blocks (N1 L8192 C2048 S16 bf16, whole call: 257 us left to itself, 245
+// so, 261 with 128, 272 with 72; the training step of N4 L2048 C2048 771, 738, 745, 737).
 template <class E, class S, int MODE>
 __global__ void __launch_bounds__(S::THREADS, S::P < 4 ? 8 : MODE == kScanMain ? 10 : 6) scan_kernel(const __grid_constant__ ScanParams Q) {
     constexpr int P = S::P, R = S::R, NP = S::NP, T = S::T, N = FourSums<P>::N;

@@ -219,8 +219,9 @@ const void *row_kernel(const RowPlan &p, bool backward) {
                                  : row_kernel<float>(p, backward);
 }
 
-// Blocks of the gradient: two a multiprocessor, more where a team would add up
-// more than 64 rows.
+// Blocks of the gradient: 1024 threads a multiprocessor, more where a team would add up
+// more than 64 rows.  By their registers fewer fit at once: of 592 blocks at 16384 x 2048
+// bf16 444 (70 registers, 1.33 rounds), of 1184 at 8191 x 1001 bf16 740 (81, 1.6 rounds).
 long long grad_blocks(const RowPlan &p, long long rows, int sms) {
     const int teams = p.threads / p.team;
     const long long blocks = std::max(std::min(ceil_div(rows, teams), 2LL * sms * (kRowMost / p.threads)),
@@ -312,9 +313,9 @@ int gc_b200_layer_norm(const gc_tensor *x, const gc_tensor *gamma, const gc_tens
     P.aligned = aligned_params({gamma, beta}, plan.v) ? 1 : 0;
     P.stats = stats != nullptr ? static_cast<float2 *>(stats->data) : nullptr;
     const void *fn = row_kernel(plan, false);
-    // Four times the blocks that a multiprocessor has threads for, each taking rows in
-    // turn: the multiprocessors are not served alike (16384 rows of 2048 bf16: 32 us,
-    // 35 with a quarter of the blocks).
+    // Four times the blocks that a multiprocessor has threads for, which take rows in
+    // turn where there are more: the multiprocessors are not served alike (16384 rows of
+    // 2048 bf16, a row for each team then: 32 us, 35 with a quarter of the blocks).
     const long long grid = std::min(ceil_div(P.rows, plan.threads / plan.team), (plan.edges ? 2048LL : 8192LL) / plan.threads * facts.sms);
     void *args[] = {&P};
     const cudaError_t e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(plan.threads), args, plan.smem,

@@ -135,8 +135,11 @@ int padded_states(int64_t s) {
     return sp == 2 ? 4 : sp;
 }
 // Segments: as many as give each multiprocessor 16 blocks (24 in the gradient,
-// whose own kernel has half as many), of at least 32 tokens.  N1 L8192 C2048 bf16 takes
-// 8 % longer with ten blocks and 5 % with 20, N5 L777 C330 FP32 20 % with 64 tokens.
+// whose own kernel has half as many), of at least 32 tokens.  Eight blocks fit at once at
+// 16 states in 16 bits, so that 16 are two rounds there; FP32 has room for seven, 64 states
+// for six, up to four states for four or five, and rounding up gives N4 L2048 C2048 2.16
+// rounds.  N1 L8192 C2048 bf16 takes 8 % longer with ten blocks (1.3 rounds) and 5 % with 20
+// (2.6), N5 L777 C330 FP32 20 % with 64 tokens.
 ScanPlan plan_scan(const ScanCall &c, int sms, bool backward) {
     ScanPlan p;
     p.type = c.x.type;

@@ -267,7 +267,8 @@ int gc_b200_dropout(const gc_tensor *x, const gc_tensor *residual, gc_tensor *y,
  * Element types as above.  Data tensors of one call have one type; parameters
  * are dense, F32 or of the data's type.  The last axis of a data tensor is dense;
  * its other strides are free as long as no two elements share memory (for layer
- * norm the rows are evenly spaced), else GC_UNSUPPORTED.  Axes of 0 are valid.
+ * norm the rows are evenly spaced), else GC_UNSUPPORTED.  No rows, sequences or
+ * tokens are valid, no columns, channels or states are not.
  * Sums, statistics and states are held in 32 bits or more; a result is rounded
  * once.  Outputs and workspaces overlap neither inputs nor one another.
  * Workspaces are 16-byte aligned device memory whose contents need not be set and
