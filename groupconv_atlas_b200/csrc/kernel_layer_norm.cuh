@@ -104,6 +104,15 @@ __device__ __forceinline__ Lanes<V> float_params(const float *p) {
     }
     return lanes_of<V>(v);
 }
+// g = dy gamma, rounded by itself in its sum and in dx alike, so that what is g's mean
+// leaves 0 (rows of one column, rows whose g is one value).  Of pairs a product and a
+// sum behind it become one fma, .rn or not; of single values they do not.
+__device__ __forceinline__ f2 rounded_product(f2 a, f2 b) {
+    float a0, a1, b0, b1;
+    split(a, a0, a1);
+    split(b, b0, b1);
+    return pair(__fmul_rn(a0, b0), __fmul_rn(a1, b1));
+}
 template <int V>
 __device__ __forceinline__ float lanes_sum(const Lanes<V> &l) {
     f2 s = l.p[0];
@@ -259,7 +268,7 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_grad_kernel(const __grid_
                     const Lanes<V> e = lanes_of_raw<T, V>(rx[r][j]), d = lanes_of_raw<T, V>(rg[r][j]);
 #pragma unroll
                     for (int i = 0; i < NP; ++i) {
-                        const f2 xhat = (e.p[i] + pair(-st[r].x)) * pair(st[r].y), g = d.p[i] * gamma[j].p[i];
+                        const f2 xhat = (e.p[i] + pair(-st[r].x)) * pair(st[r].y), g = rounded_product(d.p[i], gamma[j].p[i]);
                         s1 = s1 + g;
                         s2 = fma2(g, xhat, s2);
                         sum_g[j].p[i] = fma2(d.p[i], xhat, sum_g[j].p[i]);
@@ -286,7 +295,7 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_grad_kernel(const __grid_
 #pragma unroll
                     for (int i = 0; i < NP; ++i) {
                         const f2 xhat = (e.p[i] + pair(-st[r].x)) * pair(st[r].y);
-                        o.p[i] = pair(st[r].y) * fma2(xhat, m2, fma2(d.p[i], gamma[j].p[i], m1));
+                        o.p[i] = pair(st[r].y) * fma2(xhat, m2, rounded_product(d.p[i], gamma[j].p[i]) + m1);
                     }
                     store_lanes<T, V>(static_cast<T *>(P.y) + row * P.y_ld + v * V, o);
                 }
@@ -533,7 +542,7 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_edges_grad_kernel(const _
             f2 s1 = pair(0.0f), s2 = pair(0.0f);
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-                const f2 xhat = (e.p[i] + pair(-st.x)) * pair(st.y), g = d.p[i] * gamma[j].p[i];
+                const f2 xhat = (e.p[i] + pair(-st.x)) * pair(st.y), g = rounded_product(d.p[i], gamma[j].p[i]);
                 s1 = s1 + g;
                 s2 = fma2(g, xhat, s2);
                 sum_g[j].p[i] = fma2(d.p[i], xhat, sum_g[j].p[i]);
@@ -556,7 +565,7 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_edges_grad_kernel(const _
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const f2 xhat = (e.p[i] + pair(-st.x)) * pair(st.y);
-                o.p[i] = pair(st.y) * fma2(xhat, m2, fma2(d.p[i], gamma[j].p[i], m1));
+                o.p[i] = pair(st.y) * fma2(xhat, m2, rounded_product(d.p[i], gamma[j].p[i]) + m1);
             }
             at.store(static_cast<T *>(P.y) + row * P.y_ld, o);
         }
@@ -653,7 +662,7 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_long_grad_kernel(const __
         float sums[2];
         long_sums<2>(P.c, sums, [&](long long i, float (&run)[2]) {
             const float gamma = P.gamma != nullptr ? load_param(P.gamma, P.gamma_type, i) : 1.0f;
-            const float d = to_float(dy[i]), xhat = (to_float(x[i]) - st.x) * st.y, g = d * gamma;
+            const float d = to_float(dy[i]), xhat = (to_float(x[i]) - st.x) * st.y, g = __fmul_rn(d, gamma);
             run[0] += g;
             run[1] = fmaf(g, xhat, run[1]);
             if (out != nullptr) {
@@ -667,7 +676,7 @@ __global__ void __launch_bounds__(kRowMost) layer_norm_long_grad_kernel(const __
         for (long long i = threadIdx.x; i < P.c; i += kRowMost) {
             const float gamma = P.gamma != nullptr ? load_param(P.gamma, P.gamma_type, i) : 1.0f;
             const float xhat = (to_float(x[i]) - st.x) * st.y;
-            dst[i] = from_float<T>(st.y * (fmaf(to_float(dy[i]), gamma, -m1) - xhat * m2));
+            dst[i] = from_float<T>(st.y * (__fmul_rn(to_float(dy[i]), gamma) - m1 - xhat * m2));
         }
     }
 }

@@ -221,7 +221,7 @@ const void *row_kernel(const RowPlan &p, bool backward) {
 
 // Blocks of the gradient: 1024 threads a multiprocessor, more where a team would add up
 // more than 64 rows.  By their registers fewer fit at once: of 592 blocks at 16384 x 2048
-// bf16 444 (70 registers, 1.33 rounds), of 1184 at 8191 x 1001 bf16 740 (81, 1.6 rounds).
+// bf16 444 (70 registers, 1.33 rounds), of 1184 at 8191 x 1001 bf16 740 (83, 1.6 rounds).
 long long grad_blocks(const RowPlan &p, long long rows, int sms) {
     const int teams = p.threads / p.team;
     const long long blocks = std::max(std::min(ceil_div(rows, teams), 2LL * sms * (kRowMost / p.threads)),

@@ -103,6 +103,18 @@ def test_constant_rows_of_large_values(native, torch_cuda, c):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows', [1, 300, 100000])
+def test_rows_of_one_column(native, torch_cuda, dtype, rows):
+    """y is beta whatever x is, and dx exactly 0: dy gamma and its mean are rounded alike."""
+    x, gamma, beta, dy = test_layer_norm.make((rows, 1), TYPES[dtype], 38)
+    leaves = [t.cuda().requires_grad_() for t in (x, gamma, beta)]
+    y = torch_module.layer_norm(*leaves)
+    dx, dgamma, _ = torch.autograd.grad(y, leaves, dy.cuda())
+    assert torch.equal(y, leaves[2].detach().to(y.dtype).expand_as(y)) and not dx.any() and not dgamma.any()
+
+
+@pytest.mark.gpu
 def test_parameters_of_a_long_scan(native, torch_cuda):
     """Steady states give dA, dD and ddt_bias sums of one value each, over segments of
     65536 tokens: added up in 32 bits tile after tile these would be off by more than
