@@ -167,6 +167,24 @@ def test_runs_of_sequences_that_end_early(native, torch_cuda):
 
 
 @pytest.mark.gpu
+def test_weights_of_many_stretches(native, torch_cuda):
+    """So many tokens that a block more than the GPU asks for takes part, each worker
+    having 64 stretches; x and dy of one value each, so that dbias and each tap of dweight
+    are their counts times a value (1.1015625, exact in bfloat16, and its square)."""
+    if torch.cuda.mem_get_info()[0] < 70 << 30:
+        pytest.skip('needs 70 GB of device memory')
+    n, l, c, k, value = 5, 140000, 8192, 4, 1.1015625
+    x = torch.full((n, l, c), value, device='cuda', dtype=torch.bfloat16).requires_grad_()
+    w, b = torch.zeros(c, k, device='cuda', requires_grad=True), torch.zeros(c, device='cuda', requires_grad=True)
+    y = torch_module.causal_conv(x, w, b)
+    dw, db = torch.autograd.grad(y, (w, b), torch.full_like(y, value))
+    count = torch.tensor([n * (l - (k - 1 - j)) for j in range(k)], dtype=torch.double)  # tap j reads zeros before token K - 1 - j
+    assert_close(db, torch.full((c,), n * l * value, dtype=torch.double), torch.full((c,), LONG * U * n * l * value, dtype=torch.double))
+    want = (count * value * value).expand(c, k)
+    assert_close(dw, want, (LONG + 2) * U * want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('states', [16, 64])
 def test_pairs_of_many_channels(native, torch_cuda, states):
     """dB and dC are sums over 2^18 channels; of one value each they would be off by

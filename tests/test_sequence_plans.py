@@ -8,7 +8,7 @@ def test_a_worker_of_the_convolution_takes_at_most_64_stretches(run):
     tokens of a stretch and 64 stretches, before partial results are joined."""
     run("""
 for n, l, c, k, dtype in [(8, 2048, 2048, 4, 17), (3, 1021, 333, 3, 0), (64, 1 << 20, 33, 4, 0), (1, 1 << 28, 4, 4, 17),
-                          (1000, 70000, 129, 8, 16), (1 << 22, 200, 7, 1, 0), (4, 1 << 20, 8192, 4, 17)]:
+                          (1000, 70000, 129, 8, 16), (1 << 22, 200, 7, 1, 0), (4, 1 << 20, 8192, 4, 17), (5, 140000, 8192, 4, 17)]:
     v = Conv(n, l, c, k, dtype)
     st, need = v.size()
     assert st == OK
