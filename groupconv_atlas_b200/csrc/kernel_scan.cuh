@@ -489,6 +489,14 @@ struct FourSums {
     }
 };
 
+// The exponent of what v has grown by over many tokens: 0 where v is, which an infinite
+// growth (A > 0) would make no number.
+__device__ __forceinline__ f2 growth(f2 exponent, f2 v) {
+    float a, b, x, y;
+    split(exponent, a, b);
+    split(v, x, y);
+    return pair(x == 0.0f ? 0.0f : a, y == 0.0f ? 0.0f : b);
+}
 template <class T>
 __device__ __forceinline__ T *token_at(const TokenView &v, long long n, long long t) {
     return static_cast<T *>(const_cast<void *>(v.p)) + n * v.ldn + t * v.ldt;
@@ -514,7 +522,7 @@ __device__ __forceinline__ void pass_segments(const ScanParams &Q, const ScanPla
         for (int j = 0; j < 4; ++j) {
             if (j0 + j >= count) continue;
 #pragma unroll
-            for (int i = 0; i < S::NP; ++i) h[i] = fma2(exp2_fast(pair(sum[j]) * a2[i]), h[i], e[j][i]);
+            for (int i = 0; i < S::NP; ++i) h[i] = fma2(exp2_fast(growth(pair(sum[j]) * a2[i], h[i])), h[i], e[j][i]);
         }
     }
 }
@@ -661,15 +669,17 @@ __global__ void __launch_bounds__(S::THREADS, S::P < 4 ? 8 : MODE == kScanMain ?
                 const int t = t4 + j;
                 const float4 v = du[t * S::PAIRS];
                 const float delta[2] = {v.x, v.z}, u[2] = {v.y, v.w};
+                float since[2];  // the segment's deltas so far, where f is not 0 (an infinite growth of nothing is nothing)
                 f2 wb[NP], wc[NP];
                 tile_states<S>(b + t * S::SP, wb);
                 if constexpr (MODE == kScanMain) tile_states<S>(c + t * S::SP, wc);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     if constexpr (MODE != kScanMain) sum[k] += delta[k];
+                    since[k] = MODE != kScanCarryBack || u[k] == 0.0f ? 0.0f : sum[k];
                     if constexpr (MODE == kScanCarryBack) {
 #pragma unroll
-                        for (int i = 0; i < NP; ++i) h[k][i] = fma2(exp2_fast(pair(sum[k]) * a2[k][i]), pair(u[k]) * wb[i], h[k][i]);
+                        for (int i = 0; i < NP; ++i) h[k][i] = fma2(exp2_fast(pair(since[k]) * a2[k][i]), pair(u[k]) * wb[i], h[k][i]);
                     } else {
 #pragma unroll
                         for (int i = 0; i < NP; ++i) h[k][i] = fma2(exp2_fast(pair(delta[k]) * a2[k][i]), h[k][i], pair(u[k]) * wb[i]);

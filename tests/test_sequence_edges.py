@@ -267,6 +267,31 @@ def test_step_sizes_of_a_token_stay_in_their_channel(native, torch_cuda, shape, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('states', [4, 16])
+def test_growing_states_that_nothing_has_entered(native, torch_cuda, states):
+    """A > 0: a segment's growth, exp(96) over 32 tokens, is infinite in 32 bits, and so
+    is its product with nothing (0 inf) no number.  x is 0 but for the last tokens, dy but
+    for the first."""
+    n, l, ch = 2, 640, 8
+    v = test_selective_scan.make(n, l, ch, states, 1, torch.float32, 39)
+    v['dt'] = torch.ones_like(v['dt'])
+    v['a'] = 3 * torch.rand(ch, states, generator=torch.Generator().manual_seed(40)).round()
+    v['x'][:, :-12] = 0
+    v['dy'][:, 12:] = 0
+    ref = ScanReference(*(v[k] for k in NAMES[:7]), softplus=False).backward(v['dy'])
+    leaves = {k: v[k].cuda().requires_grad_() for k in NAMES[:7]}
+    y = run(v, leaves, False, None, False)
+    assert 'parts=1 ' not in api.Native().last_plan()
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), v['dy'].cuda())))
+    assert_close(y, ref.y, ref.tol_y, 'y')
+    for k in ('x', 'dt', 'b', 'c', 'z'):
+        assert_close(grads[k], getattr(ref, 'd' + k), getattr(ref, 'tol_d' + k) + 2.0 ** -40, k)
+    for k in ('a', 'd'):
+        want = getattr(ref, 'd' + k)
+        assert_close(grads[k], want, getattr(ref, 'tol_d' + k) + HALF[torch.float32] * want.abs() + 2.0 ** -25, k)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('value', [float('nan'), float('inf'), -float('inf')])
 @pytest.mark.parametrize('channel', [4, 5])
 @pytest.mark.parametrize('op', ['gate', 'convolution'])
